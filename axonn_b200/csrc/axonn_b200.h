@@ -312,6 +312,34 @@ int axb_heap_attach(void* heap, int peer, int fd);
 unsigned long long axb_heap_info(void* heap, int what);
 int axb_heap_destroy(void* heap);
 
+/* ---- key/value cache in blocks of 16, 32, 64 or 128 tokens (kv_cache.cu, cached_attention.cu).  One layer: codes
+ * [N, G, block_tokens, D] of 8 bits (e4m3, or int8), scales [N, G] fp32; tables [R, W] int32 name the blocks of a request, -1 behind
+ * them.  Slots are block * block_tokens + place, -1 for a token without one.  D 64 or 128; dtype 0 or 1.
+ * plan: places for the first fresh[r] of S tokens behind the lengths[r] that request r has; tables is written, the rest are outputs. */
+int axb_plan_blocks(const int* lengths, const int* fresh, int* tables, const int* free_blocks, const int* taken, long long* slots,
+                    int* positions, int* lengths_out, int* taken_out, int R, int S, int W, int N, int block_tokens, void* stream);
+/* store: keys and values of qkv [R, S, G, P + 2, D] (strides in elements, heads of a group dense) at slots [R, S] as the plan gives them;
+ * with cs [angles, D / 2, 2] keys are rotated by their positions, and the queries into q [R, S, G * P, D] */
+int axb_store_blocks(const void* qkv, long long row_stride, long long token_stride, long long group_stride, const long long* slots,
+                     const int* positions, const float* cs, void* q, void* k, void* v, float* ks, float* vs, int R, int S, int G, int P,
+                     int D, int N, int block_tokens, int angles, int dtype, int int8, void* stream);
+/* reorder: row r of a group of K goes on from row parents[r] of it; layers stacked in front; *_out are outputs */
+int axb_reorder_blocks(void* k, void* v, float* ks, float* vs, const int* tables, const int* lengths, const int* spare, const int* parents,
+                       int* tables_out, int* lengths_out, int* spare_out, int layers, int R, int K, int W, int N, int G, int block_tokens,
+                       int row_bytes, void* stream);
+/* attention of q [R, S, G, P, D] (strides in elements), whose last fresh[r] (NULL: S) tokens are the last of lengths[r], into out
+ * [R, S, G * P, D]; work: axb_cached_attention_words() 32-bit words, 16-byte aligned, of this call alone */
+long long axb_cached_attention_words(int R, int S, int P, int D);
+int axb_cached_attention(const void* q, long long q_row, long long q_token, long long q_group, const void* k, const void* v,
+                         const float* ks, const float* vs, const int* tables, const int* lengths, const int* fresh, void* out, void* work,
+                         int R, int S, int G, int P, int D, int W, int N, int block_tokens, float scale, int dtype, int int8, void* stream);
+
+/* ---- selection of beam search (beam.cu): logits [B, K, V], scores [B, K] -> the K best continuations of every prompt; done [B, K] (or
+ * NULL) with its end token.  work: axb_beam_select_words() 32-bit words, 8-byte aligned, of this call alone */
+long long axb_beam_select_words(int B, int K, int V);
+int axb_beam_select(const void* logits, const float* scores, const void* done, int eos, float* out_scores, long long* out_tokens,
+                    int* out_parents, void* out_done, void* work, int B, int K, int V, int dtype, void* stream);
+
 /* ---- top-k gradient pruning (prune.cu): keep the k largest |g|, zero the rest, in place.
  * dtype: the codes above (0 bf16, 1 fp16, 2 fp32).  `work`: device scratch of axb_prune_workspace_words() 32-bit words, 8-byte aligned. */
 int axb_prune_workspace_words(void);

@@ -1,0 +1,558 @@
+// Attention of new tokens over a key/value cache in blocks of 8-bit codes (see kv_cache.cu for the layout).
+//
+//   s = scale * ks * (q . k)      o = sum_t p_t vs v_t / sum_t p_t,   p = softmax of s over the tokens that a query sees
+//
+// What bounds it is reading 2 D bytes per token and KV head once.  The unit of work is a tile of 16 tokens of one request, KV head and
+// group of up to 8 or 16 query columns (query heads of the KV head x new tokens); a warp takes a run of tiles, as long as every other
+// warp's, whatever the lengths of the requests: it ends inside one sequence and goes on in the next.  A sequence that one warp has seen
+// whole is written at once, the others leave partial sums that a second launch adds up in the order of the tokens.
+//
+// A warp keeps everything in registers.  Scores are S^T = K Q^T (m16n8k16, rows = tokens), so that the few query columns fill the narrow
+// side of the instruction; O^T = V^T P^T (rows = values of the head).  Which value of a head is which row or k index is free as long as
+// both operands agree, and is chosen such that every thread reads 16 consecutive bytes: of K 16 values of its token, of V 16 values of
+// each of its four tokens, whose bytes are then interleaved pairwise.  Codes become fp16, which holds them exactly; queries are scaled
+// by a power of two into fp16 (2^-11 of the largest at 16-bit inputs: exact but for values below 2^-21 of a row's largest), probabilities
+// are rounded to fp16 (2^-11 each).  Scores, sums and outputs are 32-bit.
+//
+// The scale of a block of values moves into the exponent: a tile weighs exp2(s + log2 vs - m'), with m' the running maximum of that sum,
+// beside exp2(s - m) for the denominator, so that neither overflows nor vanishes whatever the scales of the blocks are.  References are
+// raised only when a score exceeds them by 2^8.
+#include <cuda_fp8.h>
+
+#include "common.cuh"
+
+namespace axb {
+
+constexpr int CA_TILE = 16;
+constexpr int CA_WARPS = 4;
+constexpr int CA_MAX_ROWS = 4096;        // requests of one launch: their tiles are counted in shared memory
+constexpr int CA_LEAST_TILES = 2;        // of a warp's run: shorter ones are not worth their partial sums
+constexpr float CA_LOWEST = -3.0e38f;
+
+struct AttendArgs {
+  const void* q;
+  long long q_row, q_token, q_group;     // strides in elements; heads of a group are dense
+  void* out;                             // [R, S, G * P, D]
+  const uint8_t *k, *v;
+  const float *ks, *vs;
+  const int *tables, *lengths, *fresh;
+  int R, S, G, P, W, N, shift;
+  int groups;                            // of query columns
+  float scale_log2;
+  int workers;                           // warps of the grid
+  int* before;                           // [R + 1] tiles of the requests before each
+  float* part;                           // [2 * workers][columns][D + 4]: sums, then m, m', l
+};
+
+// The warp that has unit u, of `active` warps that share `units`; a warp starts at units * w / active.
+__device__ __forceinline__ int active_warps(long long units, int workers) {
+  const long long want = (units + CA_LEAST_TILES - 1) / CA_LEAST_TILES;
+  return static_cast<int>(want < workers ? (want < 1 ? 1 : want) : workers);
+}
+__device__ __forceinline__ long long first_unit(long long units, int w, int active) { return units * w / active; }
+__device__ __forceinline__ int owner(long long u, long long units, int active) {
+  return static_cast<int>(((u + 1) * active - 1) / units);
+}
+
+__device__ __forceinline__ float exp2_fast(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ void mma_f16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+               : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
+  uint32_t y;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+  return y;
+}
+__device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
+  const __half2 h = __floats2half2_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+// Four codes as fp16: bytes 0 and 1, bytes 2 and 3.
+template <bool INT8> __device__ __forceinline__ void widen(uint32_t w, uint32_t& lo, uint32_t& hi) {
+  if constexpr (INT8) {      // 1024 + (x + 128) is the half with x + 128 in its low byte
+    const __half2 off = __halves2half2(__ushort_as_half(0x6480), __ushort_as_half(0x6480));
+    w ^= 0x80808080u;
+    const uint32_t l = __byte_perm(w, 0x64646464u, 0x4140), h = __byte_perm(w, 0x64646464u, 0x4342);
+    const __half2 a = __hsub2(*reinterpret_cast<const __half2*>(&l), off), b = __hsub2(*reinterpret_cast<const __half2*>(&h), off);
+    lo = *reinterpret_cast<const uint32_t*>(&a);
+    hi = *reinterpret_cast<const uint32_t*>(&b);
+  } else {
+    asm("{\n\t.reg .b16 l, h;\n\tmov.b32 {l, h}, %2;\n\tcvt.rn.f16x2.e4m3x2 %0, l;\n\tcvt.rn.f16x2.e4m3x2 %1, h;\n\t}"
+        : "=r"(lo), "=r"(hi) : "r"(w));
+  }
+}
+template <int WORDS> __device__ __forceinline__ void load_words(const uint8_t* p, uint32_t* w) {
+  if constexpr (WORDS == 4) {
+    const uint4 u = __ldg(reinterpret_cast<const uint4*>(p));
+    w[0] = u.x; w[1] = u.y; w[2] = u.z; w[3] = u.w;
+  } else {
+    const uint2 u = __ldg(reinterpret_cast<const uint2*>(p));
+    w[0] = u.x; w[1] = u.y;
+  }
+}
+
+// Codes and scales of one tile, as a thread holds them: lane = 4 g + j has tokens g and g + 8 of K, tokens 2 j, 2 j + 1, 2 j + 8 and
+// 2 j + 9 of V.
+template <int D> struct Tile {
+  uint32_t k[2][D / 16];
+  uint32_t v[4][D / 32];
+  float ks, vs;
+  bool there;
+};
+
+template <typename T, int D, bool INT8, int NT>
+__global__ void __launch_bounds__(32 * CA_WARPS, NT == 1 ? 4 : 3) attend_kernel(const AttendArgs a) {
+  constexpr int KC = D / 64, MT = D / 16, VW = D / 32, COLS = 8 * NT;
+  extern __shared__ int before[];          // [R + 1]
+  __shared__ int sums[CA_WARPS];
+  pdl_launch_next();
+  pdl_wait();
+  const int tid = threadIdx.x, lane = tid & 31, g8 = lane >> 2, j4 = lane & 3, BT = 1 << a.shift;
+  const int most = min(static_cast<long long>(a.W) << a.shift, 0x7fffff00ll);
+
+  // tiles of the requests before each: one scan per block of the grid
+  {
+    const int per = (a.R + 32 * CA_WARPS - 1) / (32 * CA_WARPS), r0 = tid * per;
+    int mine = 0;
+    for (int r = r0; r < min(r0 + per, a.R); ++r) mine += (min(max(a.lengths[r], 0), most) + CA_TILE - 1) / CA_TILE;
+    int incl = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) { const int u = __shfl_up_sync(0xffffffffu, incl, o); if (lane >= o) incl += u; }
+    if (lane == 31) sums[tid >> 5] = incl;
+    __syncthreads();
+    int at = incl - mine;
+    for (int i = 0; i < tid >> 5; ++i) at += sums[i];
+    for (int r = r0; r < min(r0 + per, a.R); ++r) {
+      before[r] = at;
+      if (blockIdx.x == 0) a.before[r] = at;
+      at += (min(max(a.lengths[r], 0), most) + CA_TILE - 1) / CA_TILE;
+    }
+    if (r0 < a.R && r0 + per >= a.R) { before[a.R] = at; if (blockIdx.x == 0) a.before[a.R] = at; }
+    __syncthreads();
+  }
+  const int worker = blockIdx.x * CA_WARPS + (tid >> 5), per_tile = a.G * a.groups;
+  const long long units = static_cast<long long>(before[a.R]) * per_tile;
+  const int active = active_warps(units, a.workers);
+  if (worker >= active || units == 0) return;
+  const long long begin = first_unit(units, worker, active), end = first_unit(units, worker + 1, active);
+
+  int r = 0;
+  for (int hi = a.R; hi - r > 1;) { const int mid = (r + hi) / 2; if (before[mid] <= begin / per_tile) r = mid; else hi = mid; }
+  for (long long u = begin; u < end;) {
+    while (before[r + 1] <= u / per_tile) ++r;
+    const int tiles = before[r + 1] - before[r];
+    const long long within = u - static_cast<long long>(before[r]) * per_tile;
+    const int item = static_cast<int>(within / tiles), g = item / a.groups, group = item % a.groups;
+    const int t0 = static_cast<int>(within % tiles), t1 = static_cast<int>(min(static_cast<long long>(tiles), t0 + (end - u)));
+    const int length = min(max(a.lengths[r], 0), most), fresh = a.fresh ? min(max(a.fresh[r], 0), a.S) : a.S;
+    const int col0 = group * COLS, cols = min(a.S * a.P - col0, COLS);
+
+    // queries as the B operand of the scores, scaled into fp16; what their columns see
+    uint32_t qf[NT][D / 16][2];
+    float cscale[NT][2];
+    int seen[NT][2], all = 0x7fffffff;         // tokens that columns 2 j, 2 j + 1 see; those that every column sees
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+      const int c = col0 + n * 8 + g8;
+      float f[KC][16], largest = 0.f;
+      if (n * 8 + g8 < cols) {
+        const T* p = static_cast<const T*>(a.q) + r * a.q_row + (c / a.P) * a.q_token + g * a.q_group + (c % a.P) * D + j4 * 16;
+#pragma unroll
+        for (int h = 0; h < KC; ++h)
+#pragma unroll
+          for (int x = 0; x < 2; ++x) {
+            const uint4 w4 = __ldg(reinterpret_cast<const uint4*>(p + h * 64 + x * 8));
+            const uint32_t w[4] = {w4.x, w4.y, w4.z, w4.w};
+#pragma unroll
+            for (int y = 0; y < 4; ++y) {
+              float2 t;
+              if constexpr (__is_same(T, __half)) t = __half22float2(*reinterpret_cast<const __half2*>(&w[y]));
+              else t = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&w[y]));
+              f[h][x * 8 + 2 * y] = t.x; f[h][x * 8 + 2 * y + 1] = t.y;
+              largest = fmaxf(largest, fmaxf(fabsf(t.x), fabsf(t.y)));
+            }
+          }
+      } else {
+#pragma unroll
+        for (int h = 0; h < KC; ++h)
+#pragma unroll
+          for (int x = 0; x < 16; ++x) f[h][x] = 0.f;
+      }
+      largest = fmaxf(largest, __shfl_xor_sync(0xffffffffu, largest, 1));
+      largest = fmaxf(largest, __shfl_xor_sync(0xffffffffu, largest, 2));
+      // 2^(7 - e) for a largest of 2^e .. 2^(e + 1); zero and what is not finite stay as they are
+      int e = static_cast<int>(__float_as_uint(largest) >> 23) - 127;
+      e = e > 127 || e < -126 ? 7 : max(e, -110);
+      const float up = __uint_as_float(static_cast<uint32_t>(127 + 7 - e) << 23);
+      const float down = __uint_as_float(static_cast<uint32_t>(127 + e - 7) << 23) * a.scale_log2;
+#pragma unroll
+      for (int s = 0; s < D / 16; ++s) {
+        const float* x = &f[s / 4][(s % 4) * 4];
+        qf[n][s][0] = pack_f16(x[0] * up, x[1] * up);
+        qf[n][s][1] = pack_f16(x[2] * up, x[3] * up);
+      }
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        cscale[n][h] = __shfl_sync(0xffffffffu, down, (2 * j4 + h) * 4);
+        const int cc = n * 8 + 2 * j4 + h, i = (col0 + cc) / a.P;
+        seen[n][h] = cc < cols && i < fresh ? min(max(length - fresh + i + 1, 0), length) : 0;
+        if (seen[n][h] > 0) all = min(all, seen[n][h]);
+      }
+    }
+    all = __reduce_min_sync(0xffffffffu, all);
+
+    float acc[NT][MT][4], m1[NT][2], m2[NT][2], l[NT][2];
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+#pragma unroll
+      for (int i = 0; i < MT; ++i) acc[n][i][0] = acc[n][i][1] = acc[n][i][2] = acc[n][i][3] = 0.f;
+      m1[n][0] = m1[n][1] = m2[n][0] = m2[n][1] = CA_LOWEST;
+      l[n][0] = l[n][1] = 0.f;
+    }
+
+    // the ids of 32 blocks, one per lane, ahead of their use
+    const int* table = a.tables + static_cast<size_t>(r) * a.W;
+    const int down_shift = a.shift - 4;      // tiles to blocks
+    int id_base = t0 >> down_shift;
+    int ids = id_base + lane < a.W ? table[id_base + lane] : -1;
+    auto fetch = [&](int t, Tile<D>& x) {
+      const int b = t >> down_shift;
+      if (b - id_base == 32) { id_base = b; ids = b + lane < a.W ? table[b + lane] : -1; }
+      const int id = __shfl_sync(0xffffffffu, ids, b - id_base);
+      x.there = id >= 0 && id < a.N;
+      if (!x.there) return;
+      const size_t head = static_cast<size_t>(id) * a.G + g;
+      x.ks = __ldg(a.ks + head);
+      x.vs = __ldg(a.vs + head);
+      const size_t row = (head << a.shift) + ((t * CA_TILE) & (BT - 1));
+      const uint8_t* k = a.k + (row + g8) * D + j4 * 16;
+      const uint8_t* v = a.v + (row + 2 * j4) * D + g8 * (D / 8);
+#pragma unroll
+      for (int h = 0; h < KC; ++h) {
+        load_words<4>(k + h * 64, x.k[0] + 4 * h);
+        load_words<4>(k + 8 * D + h * 64, x.k[1] + 4 * h);
+      }
+      load_words<VW>(v, x.v[0]);
+      load_words<VW>(v + D, x.v[1]);
+      load_words<VW>(v + 8 * D, x.v[2]);
+      load_words<VW>(v + 9 * D, x.v[3]);
+    };
+
+    Tile<D> next;
+    fetch(t0, next);
+    for (int t = t0; t < t1; ++t) {
+      Tile<D> x = next;
+      if (t + 1 < t1) fetch(t + 1, next);
+      if (!x.there) continue;
+
+      float s[NT][4];
+#pragma unroll
+      for (int n = 0; n < NT; ++n) s[n][0] = s[n][1] = s[n][2] = s[n][3] = 0.f;
+#pragma unroll
+      for (int i = 0; i < D / 16; ++i) {
+        uint32_t a0, a1, a2, a3;
+        widen<INT8>(x.k[0][i], a0, a2);
+        widen<INT8>(x.k[1][i], a1, a3);
+#pragma unroll
+        for (int n = 0; n < NT; ++n) mma_f16(s[n], a0, a1, a2, a3, qf[n][i][0], qf[n][i][1]);
+      }
+      // vs = 2^ev fv, 1 <= fv < 2
+      const float ev = static_cast<float>(static_cast<int>(__float_as_uint(x.vs) >> 23) - 127);
+      const float fv = __uint_as_float((__float_as_uint(x.vs) & 0x7fffffu) | 0x3f800000u);
+      bool above = false;
+      const bool ragged = t * CA_TILE + CA_TILE > all;
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          s[n][i] *= cscale[n][i & 1] * x.ks;
+          if (ragged && t * CA_TILE + g8 + (i >> 1) * 8 >= seen[n][i & 1]) s[n][i] = -INFINITY;
+          above |= s[n][i] > m1[n][i & 1] + 8.f || s[n][i] + ev > m2[n][i & 1] + 8.f;
+        }
+      if (__any_sync(0xffffffffu, above)) {
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            float top = fmaxf(s[n][h], s[n][h + 2]);
+#pragma unroll
+            for (int o = 4; o < 32; o <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+            const float n1 = fmaxf(m1[n][h], top), n2 = fmaxf(m2[n][h], top + ev);
+            l[n][h] *= exp2_fast(m1[n][h] - n1);
+            const float f = exp2_fast(m2[n][h] - n2);
+            m1[n][h] = n1; m2[n][h] = n2;
+#pragma unroll
+            for (int i = 0; i < MT; ++i) { acc[n][i][h] *= f; acc[n][i][h + 2] *= f; }
+          }
+      }
+      uint32_t p[NT][2];
+#pragma unroll
+      for (int n = 0; n < NT; ++n) {
+        float w[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          l[n][i & 1] += exp2_fast(s[n][i] - m1[n][i & 1]);
+          w[i] = exp2_fast(s[n][i] + ev - m2[n][i & 1]) * fv;
+        }
+        p[n][0] = transpose8x8(pack_f16(w[0], w[1]));
+        p[n][1] = transpose8x8(pack_f16(w[2], w[3]));
+      }
+      if (ragged) {
+        // rows behind the sequence hold anything; a NaN that some columns see and others do not is kept from the others below
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          if (t * CA_TILE + 2 * j4 + (i & 1) + (i >> 1) * 8 >= length)
+#pragma unroll
+            for (int w = 0; w < VW; ++w) x.v[i][w] = 0u;
+        if constexpr (!INT8) {
+          bool bad = false;
+          uint32_t nan[4][VW];
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+#pragma unroll
+            for (int w = 0; w < VW; ++w) {
+              nan[i][w] = __vcmpeq4(x.v[i][w] & 0x7f7f7f7fu, 0x7f7f7f7fu);
+              bad |= nan[i][w] != 0u;
+            }
+          if (__any_sync(0xffffffffu, bad)) {
+            // 1 where a value is NaN, times 1 where a column sees its token: a count above zero makes the sum NaN
+            uint32_t see[NT][2];
+#pragma unroll
+            for (int n = 0; n < NT; ++n)
+#pragma unroll
+              for (int e = 0; e < 2; ++e) {
+                const int token = t * CA_TILE + g8 + 8 * e;
+                see[n][e] = transpose8x8(pack_f16(token < seen[n][0] ? 1.f : 0.f, token < seen[n][1] ? 1.f : 0.f));
+              }
+#pragma unroll
+            for (int w = 0; w < VW; ++w) {
+#pragma unroll
+              for (int i = 0; i < 4; ++i) x.v[i][w] &= ~nan[i][w];
+#pragma unroll
+              for (int h = 0; h < 2; ++h) {
+                const uint32_t one = 0x38383838u;      // 1 in e4m3
+                const uint32_t x0 = __byte_perm(nan[0][w] & one, nan[1][w] & one, h ? 0x7362 : 0x5140);
+                const uint32_t x1 = __byte_perm(nan[2][w] & one, nan[3][w] & one, h ? 0x7362 : 0x5140);
+                uint32_t a0, a1, a2, a3;
+                widen<false>(x0, a0, a1);
+                widen<false>(x1, a2, a3);
+#pragma unroll
+                for (int n = 0; n < NT; ++n) {
+                  float count[4] = {0.f, 0.f, 0.f, 0.f};
+                  mma_f16(count, a0, a1, a2, a3, see[n][0], see[n][1]);
+#pragma unroll
+                  for (int i = 0; i < 4; ++i) if (count[i] > 0.f) acc[n][2 * w + h][i] = __uint_as_float(0x7fffffffu);
+                }
+              }
+            }
+          }
+        }
+      }
+#pragma unroll
+      for (int w = 0; w < VW; ++w)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          uint32_t a0, a1, a2, a3;
+          widen<INT8>(__byte_perm(x.v[0][w], x.v[1][w], h ? 0x7362 : 0x5140), a0, a1);
+          widen<INT8>(__byte_perm(x.v[2][w], x.v[3][w], h ? 0x7362 : 0x5140), a2, a3);
+#pragma unroll
+          for (int n = 0; n < NT; ++n) mma_f16(acc[n][2 * w + h], a0, a1, a2, a3, p[n][0], p[n][1]);
+        }
+    }
+
+    // thread (g8, j4) has values g8 * D / 8 .. of columns 2 j4 and 2 j4 + 1
+    const bool whole = t0 == 0 && t1 == tiles;
+    const size_t slot = 2 * static_cast<size_t>(worker) + (u == begin ? 0 : 1);
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        float total = l[n][h];
+#pragma unroll
+        for (int o = 4; o < 32; o <<= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
+        const int cc = n * 8 + 2 * j4 + h;
+        if (cc >= cols) continue;
+        if (whole) {
+          const int c = col0 + cc;
+          const float f = total != 0.f ? exp2_fast(m2[n][h] - m1[n][h]) / total : 0.f;      // 0: no block is there
+          T* o = static_cast<T*>(a.out) + ((static_cast<size_t>(r) * a.S + c / a.P) * a.G * a.P + g * a.P + c % a.P) * D + g8 * (D / 8);
+#pragma unroll
+          for (int x = 0; x < D / 64; ++x) {
+            uint32_t w[4];
+#pragma unroll
+            for (int y = 0; y < 4; ++y) {
+              const float* s = acc[n][x * 4 + y];
+              const float lo = seen[n][h] > 0 ? s[h] * f : 0.f, hi = seen[n][h] > 0 ? s[h + 2] * f : 0.f;
+              if constexpr (__is_same(T, __half)) w[y] = pack_f16(lo, hi);
+              else { const __nv_bfloat162 b = __floats2bfloat162_rn(lo, hi); w[y] = *reinterpret_cast<const uint32_t*>(&b); }
+            }
+            *reinterpret_cast<uint4*>(o + x * 8) = make_uint4(w[0], w[1], w[2], w[3]);
+          }
+        } else {
+          float* o = a.part + (slot * COLS + cc) * (D + 4);
+#pragma unroll
+          for (int i = 0; i < MT; i += 2)
+            *reinterpret_cast<float4*>(o + g8 * (D / 8) + 2 * i) =
+                make_float4(acc[n][i][h], acc[n][i][h + 2], acc[n][i + 1][h], acc[n][i + 1][h + 2]);
+          if (g8 == 0) *reinterpret_cast<float4*>(o + D) = make_float4(m1[n][h], m2[n][h], seen[n][h] > 0 ? total : 0.f, 0.f);
+        }
+      }
+    u += t1 - t0;
+  }
+}
+
+constexpr int MERGE_WARPS = 16;
+
+// Adds up the partial sums of the sequences that several warps share, in the order of their tokens, and writes zeros for requests
+// without tokens.  One block per sequence (request, KV head, group of columns); its warps share columns and parts.
+template <typename T, int D>
+__global__ void __launch_bounds__(32 * MERGE_WARPS) attend_merge_kernel(const AttendArgs a, int columns) {
+  constexpr int PER = D / 32;
+  __shared__ float sums[MERGE_WARPS][D], stats[MERGE_WARPS][3];
+  pdl_launch_next();
+  pdl_wait();
+  const int lane = threadIdx.x & 31, w = threadIdx.x >> 5, per_tile = a.G * a.groups;
+  const long long units = static_cast<long long>(a.before[a.R]) * per_tile;
+  const int active = active_warps(units, a.workers);
+  const long long items = static_cast<long long>(a.R) * per_tile;
+  for (long long item = blockIdx.x; item < items; item += gridDim.x) {
+    const int r = static_cast<int>(item / per_tile), rest = static_cast<int>(item % per_tile), g = rest / a.groups;
+    const int tiles = a.before[r + 1] - a.before[r], col0 = rest % a.groups * columns, cols = min(a.S * a.P - col0, columns);
+    int w0 = 0, w1 = -1;
+    long long from = 0;
+    if (tiles) {
+      from = static_cast<long long>(a.before[r]) * per_tile + static_cast<long long>(rest) * tiles;
+      w0 = owner(from, units, active);
+      w1 = owner(from + tiles - 1, units, active);
+      if (w0 == w1) continue;
+    }
+    // `share` warps per column, each with a run of the parts
+    int share = 1;
+    while (2 * share * cols <= MERGE_WARPS) share *= 2;
+    const int parts = w1 - w0 + 1, per = (parts + share - 1) / share;
+    for (int c0 = 0; c0 < cols; c0 += MERGE_WARPS / share) {
+      const int cc = c0 + w / share, mine = w % share;
+      float top1 = CA_LOWEST, top2 = CA_LOWEST, l = 0.f, o[PER];
+#pragma unroll
+      for (int i = 0; i < PER; ++i) o[i] = 0.f;
+      if (cc < cols)
+        for (int x0 = mine * per; x0 < min(parts, mine * per + per); x0 += 4) {
+          float4 st[4];
+          float f[4][PER];
+          const int n = min(4, min(parts, mine * per + per) - x0);
+#pragma unroll
+          for (int y = 0; y < 4; ++y)
+            if (y < n) {
+              const int worker = w0 + x0 + y;
+              const size_t slot = 2 * static_cast<size_t>(worker) + (x0 + y == 0 && from != first_unit(units, worker, active) ? 1 : 0);
+              const float* p = a.part + (slot * columns + cc) * (D + 4);
+              st[y] = *reinterpret_cast<const float4*>(p + D);
+#pragma unroll
+              for (int i = 0; i < PER; ++i) f[y][i] = p[i * 32 + lane];
+            }
+#pragma unroll
+          for (int y = 0; y < 4; ++y)
+            if (y < n) {
+              const float n1 = fmaxf(top1, st[y].x), n2 = fmaxf(top2, st[y].y);
+              const float a2 = exp2_fast(top2 - n2), b2 = exp2_fast(st[y].y - n2);
+              l = l * exp2_fast(top1 - n1) + st[y].z * exp2_fast(st[y].x - n1);
+#pragma unroll
+              for (int i = 0; i < PER; ++i) o[i] = o[i] * a2 + f[y][i] * b2;
+              top1 = n1; top2 = n2;
+            }
+        }
+      if (share > 1) {
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < PER; ++i) sums[w][i * 32 + lane] = o[i];
+        if (lane == 0) { stats[w][0] = top1; stats[w][1] = top2; stats[w][2] = l; }
+        __syncthreads();
+        if (mine == 0)
+          for (int y = w + 1; y < w + share; ++y) {
+            const float n1 = fmaxf(top1, stats[y][0]), n2 = fmaxf(top2, stats[y][1]);
+            const float a2 = exp2_fast(top2 - n2), b2 = exp2_fast(stats[y][1] - n2);
+            l = l * exp2_fast(top1 - n1) + stats[y][2] * exp2_fast(stats[y][0] - n1);
+#pragma unroll
+            for (int i = 0; i < PER; ++i) o[i] = o[i] * a2 + sums[y][i * 32 + lane] * b2;
+            top1 = n1; top2 = n2;
+          }
+      }
+      if (mine == 0 && cc < cols) {
+        const int c = col0 + cc;
+        // a column that sees nothing: no tokens, or none of this request's queries
+        const int length = a.lengths[r], fresh = a.fresh ? min(max(a.fresh[r], 0), a.S) : a.S;
+        const bool sees = tiles && c / a.P < fresh && length - fresh + c / a.P + 1 > 0;
+        const float f = l != 0.f ? exp2_fast(top2 - top1) / l : 0.f;
+        T* out = static_cast<T*>(a.out) + ((static_cast<size_t>(r) * a.S + c / a.P) * a.G * a.P + g * a.P + c % a.P) * D;
+#pragma unroll
+        for (int i = 0; i < PER; ++i) {
+          const float x = sees ? o[i] * f : 0.f;
+          if constexpr (__is_same(T, __half)) out[i * 32 + lane] = __float2half_rn(x);
+          else out[i * 32 + lane] = __float2bfloat16_rn(x);
+        }
+      }
+    }
+  }
+}
+
+static int attend_columns(int queries) { return queries <= 8 ? 8 : 16; }
+static int attend_blocks(int columns) { return sm_count_current() * (columns == 8 ? 4 : 3); }
+
+}  // namespace axb
+
+using namespace axb;
+
+// 32-bit words of the workspace: the tile counts, then two partial results per warp
+extern "C" long long axb_cached_attention_words(int R, int S, int P, int D) {
+  const int columns = attend_columns(S * P);
+  return (R + 1 + 3) / 4 * 4 + 2ll * attend_blocks(columns) * CA_WARPS * columns * (D + 4);
+}
+
+extern "C" int axb_cached_attention(const void* q, long long q_row, long long q_token, long long q_group, const void* k, const void* v,
+                                    const float* ks, const float* vs, const int* tables, const int* lengths, const int* fresh, void* out,
+                                    void* work, int R, int S, int G, int P, int D, int W, int N, int block_tokens, float scale, int dtype,
+                                    int int8, void* stream) {
+  int shift = 4;
+  while (shift < 7 && block_tokens != 1 << shift) ++shift;
+  if (block_tokens != 1 << shift) { set_error("cached_attention: blocks hold 16, 32, 64 or 128 tokens, not %d", block_tokens); return -1; }
+  if (D != 64 && D != 128) { set_error("cached_attention: heads of 64 or 128 values, not %d", D); return -1; }
+  if (dtype != 0 && dtype != 1) { set_error("cached_attention: bf16 or fp16"); return -1; }
+  if (R <= 0 || S <= 0 || G <= 0 || P <= 0 || W <= 0 || N <= 0) { set_error("cached_attention: empty sizes"); return -1; }
+  if (((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(k) | reinterpret_cast<uintptr_t>(v) | reinterpret_cast<uintptr_t>(out) |
+        reinterpret_cast<uintptr_t>(work)) & 15) || (q_row | q_token | q_group) % 8) {
+    set_error("cached_attention: operands must be 16-byte aligned, strides multiples of 8 elements");
+    return -1;
+  }
+  const int columns = attend_columns(S * P), groups = (S * P + columns - 1) / columns, blocks = attend_blocks(columns);
+  AttendArgs a{q, q_row, q_token, q_group, out, (const uint8_t*)k, (const uint8_t*)v, ks, vs, tables, lengths, fresh, R, S, G, P, W, N, shift,
+               groups, scale * 1.4426950408889634f, blocks * CA_WARPS, (int*)work, nullptr};
+  void (*kern)(AttendArgs) = nullptr;
+#define AXB_PICK(T, D_, NT) (int8 ? attend_kernel<T, D_, true, NT> : attend_kernel<T, D_, false, NT>)
+#define AXB_PICK_D(T, NT) (D == 64 ? AXB_PICK(T, 64, NT) : AXB_PICK(T, 128, NT))
+  if (columns == 8) kern = dtype == 0 ? AXB_PICK_D(__nv_bfloat16, 1) : AXB_PICK_D(__half, 1);
+  else kern = dtype == 0 ? AXB_PICK_D(__nv_bfloat16, 2) : AXB_PICK_D(__half, 2);
+#undef AXB_PICK_D
+#undef AXB_PICK
+  void (*merge)(AttendArgs, int) = dtype == 0 ? (D == 64 ? attend_merge_kernel<__nv_bfloat16, 64> : attend_merge_kernel<__nv_bfloat16, 128>)
+                                              : (D == 64 ? attend_merge_kernel<__half, 64> : attend_merge_kernel<__half, 128>);
+  const int size = 2, rows_at_once = CA_MAX_ROWS;
+  for (int r0 = 0; r0 < R; r0 += rows_at_once) {
+    a.R = R - r0 < rows_at_once ? R - r0 : rows_at_once;
+    a.q = static_cast<const char*>(q) + r0 * q_row * size;
+    a.out = static_cast<char*>(out) + static_cast<size_t>(r0) * S * G * P * D * size;
+    a.tables = tables + static_cast<size_t>(r0) * W;
+    a.lengths = lengths + r0;
+    a.fresh = fresh ? fresh + r0 : nullptr;
+    a.part = reinterpret_cast<float*>(a.before + (a.R + 1 + 3) / 4 * 4);
+    AXB_CUDA(pdl_launch(kern, dim3(blocks), dim3(32 * CA_WARPS), (a.R + 1) * sizeof(int), (cudaStream_t)stream, a));
+    const long long items = static_cast<long long>(a.R) * G * groups;
+    const int most = 2 * sm_count_current();
+    AXB_CUDA(pdl_launch(merge, dim3((unsigned)(items < most ? items : most)), dim3(32 * MERGE_WARPS), 0, (cudaStream_t)stream, a, columns));
+  }
+  return 0;
+}

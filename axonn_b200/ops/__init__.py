@@ -7,6 +7,7 @@ PyTorch composition used on CPU (and as the numerical oracle in the tests).
 
 from .activation import gelu_backward_colsum, gelu, gelu_backward, swiglu  # noqa: F401
 from .attention import flash_attention, flash_attention_packed  # noqa: F401
+from .beam import BeamStep, beam_select  # noqa: F401
 from .gemm import (  # noqa: F401
     gemm_on_pairs,
     EPI_BIAS,
@@ -16,6 +17,14 @@ from .gemm import (  # noqa: F401
     matmul_nn,
     matmul_nt,
     matmul_tn,
+)
+from .kv_cache import (  # noqa: F401
+    BlockLayer,
+    BlockPlan,
+    cached_attention,
+    plan_blocks,
+    reorder_blocks,
+    store_blocks,
 )
 from .linear import linear, linear_batched, swiglu_experts  # noqa: F401
 from .loss import cross_entropy, projected_cross_entropy  # noqa: F401

@@ -81,6 +81,13 @@ _SIGNATURES = {
     "axb_moe_route": "piiiii" "ppppppppppp" "p",
     "axb_moe_route_bwd": "piii" "pppppp" "p",
     "axb_prune_topk": "p" "lil" "p" "i" "p",
+    "axb_plan_blocks": "ppppppppp" "iiiii" "p",
+    "axb_store_blocks": "p" "lll" "pppp" "pppp" "iiiiiiiiii" "p",
+    "axb_reorder_blocks": "pppp" "pppp" "ppp" "iiiiiiii" "p",
+    "axb_cached_attention_words": "iiii",
+    "axb_cached_attention": "p" "lll" "pppp" "ppp" "pp" "iiiiiiii" "f" "ii" "p",
+    "axb_beam_select_words": "iii",
+    "axb_beam_select": "ppp" "i" "ppppp" "iiii" "p",
 }
 # Switches of kernels that are gone.  The one kernel that is left covers what they selected; a program that still sets
 # one is told so instead of being ignored.
@@ -112,7 +119,9 @@ def lib():
             for name, sig in _SIGNATURES.items():
                 if hasattr(L, name):
                     getattr(L, name).argtypes = [_CTYPES[c] for c in sig]
-            L.axb_flash_attn_bwd_scratch.restype = ctypes.c_longlong
+            for name in ("axb_flash_attn_bwd_scratch", "axb_cached_attention_words", "axb_beam_select_words"):
+                if hasattr(L, name):
+                    getattr(L, name).restype = ctypes.c_longlong
             ms = os.environ.get("AXONN_COMM_TIMEOUT_MS")
             if ms:
                 L.axb_set_wait_timeout_ms(ctypes.c_uint(int(ms)))
