@@ -23,10 +23,11 @@
 
 namespace axb {
 
-constexpr int CA_TILE = 16;
+constexpr int CA_TILE = 32;              // tokens of a tile: two halves of 16, the rows of an instruction
 constexpr int CA_WARPS = 4;
-constexpr int CA_MAX_ROWS = 4096;        // requests of one launch: their tiles are counted in shared memory
-constexpr int CA_LEAST_TILES = 2;        // of a warp's run: shorter ones are not worth their partial sums
+constexpr int CA_STAGES = 2;             // tiles of a warp's ring
+constexpr int CA_MAX_ROWS = 1024;        // requests of one launch: their tiles are counted in shared memory
+constexpr int CA_LEAST_TILES = 4;        // of a block's run: shorter ones are not worth their partial sums
 constexpr float CA_LOWEST = -3.0e38f;
 
 struct AttendArgs {
@@ -39,13 +40,14 @@ struct AttendArgs {
   int R, S, G, P, W, N, shift;
   int groups;                            // of query columns
   float scale_log2;
-  int workers;                           // warps of the grid
+  int workers;                           // blocks of the grid
   int* before;                           // [R + 1] tiles of the requests before each
   float* part;                           // [2 * workers][columns][D + 4]: sums, then m, m', l
+  float* head;                           // the same of the first sequence of every warp: [workers * CA_WARPS][columns][D + 4]
 };
 
-// The warp that has unit u, of `active` warps that share `units`; a warp starts at units * w / active.
-__device__ __forceinline__ int active_warps(long long units, int workers) {
+// The block that has unit u, of `active` blocks that share `units`; block w starts at units * w / active.
+__device__ __forceinline__ int active_blocks(long long units, int workers) {
   const long long want = (units + CA_LEAST_TILES - 1) / CA_LEAST_TILES;
   return static_cast<int>(want < workers ? (want < 1 ? 1 : want) : workers);
 }
@@ -86,33 +88,74 @@ template <bool INT8> __device__ __forceinline__ void widen(uint32_t w, uint32_t&
         : "=r"(lo), "=r"(hi) : "r"(w));
   }
 }
-template <int WORDS> __device__ __forceinline__ void load_words(const uint8_t* p, uint32_t* w) {
-  if constexpr (WORDS == 4) {
-    const uint4 u = __ldg(reinterpret_cast<const uint4*>(p));
-    w[0] = u.x; w[1] = u.y; w[2] = u.z; w[3] = u.w;
-  } else {
-    const uint2 u = __ldg(reinterpret_cast<const uint2*>(p));
-    w[0] = u.x; w[1] = u.y;
+__device__ __forceinline__ void copy16(uint32_t to, const void* from) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to), "l"(from) : "memory");
+}
+__device__ __forceinline__ void copy4(uint32_t to, const void* from) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(to), "l"(from) : "memory");
+}
+template <int WORDS> __device__ __forceinline__ void shared_words(uint32_t p, uint32_t* w) {
+  if constexpr (WORDS == 4) asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]) : "r"(p) : "memory");
+  else asm volatile("ld.shared.v2.b32 {%0, %1}, [%2];" : "=r"(w[0]), "=r"(w[1]) : "r"(p) : "memory");
+}
+
+// A tile in shared memory: 32 rows of keys, 32 of values, then for each half ks, vs and whether the block exists.  The 16-byte words of
+// a 128-byte line are exchanged such that neither the reads of K (two rows, four words each at a time) nor those of V (four rows, two
+// words) meet.
+template <int D> struct Stage {
+  static constexpr int BYTES = CA_TILE * D, SIZE = 2 * BYTES + 32;
+  static __device__ __forceinline__ int key_word(int row, int c) {
+    return D == 128 ? row * 8 + (c ^ ((row & 1) << 2)) : row * 4 + c;
+  }
+  static __device__ __forceinline__ int value_word(int row, int c) {
+    return D == 128 ? row * 8 + (c ^ (row & 6)) : (row >> 1) * 8 + ((((row & 1) << 2) + c) ^ (row & 6));
+  }
+};
+
+// Shared memory of a warp: its ring, which the partial sums of its last sequence take the place of.  (Those of its first one go to
+// global memory: the ring is in use then.)
+template <int D, int NT> __host__ __device__ constexpr int warp_bytes() {
+  const int ring = CA_STAGES * Stage<D>::SIZE, parts = 8 * NT * (D + 4) * 4;
+  return ring > parts ? ring : parts;
+}
+
+// What two partial results of a column add up to: references, denominator, sums.
+template <int N> struct Partial {
+  float m1 = CA_LOWEST, m2 = CA_LOWEST, l = 0.f, o[N] = {};
+  __device__ __forceinline__ void add(float other1, float other2, float other_l, const float (&f)[N]) {
+    const float n1 = fmaxf(m1, other1), n2 = fmaxf(m2, other2), a = exp2_fast(m2 - n2), b = exp2_fast(other2 - n2);
+    l = l * exp2_fast(m1 - n1) + other_l * exp2_fast(other1 - n1);
+#pragma unroll
+    for (int i = 0; i < N; ++i) o[i] = o[i] * a + f[i] * b;
+    m1 = n1; m2 = n2;
+  }
+};
+template <typename T> __device__ __forceinline__ T* output_row(const AttendArgs& a, int r, int g, int c, int D) {
+  return static_cast<T*>(a.out) + ((static_cast<size_t>(r) * a.S + c / a.P) * a.G * a.P + g * a.P + c % a.P) * D;
+}
+// Lane i has values i, i + 32 ...; a denominator of 0: nothing of what the column sees is there.
+template <typename T, int N> __device__ __forceinline__ void write_row(T* out, const Partial<N>& p, int lane) {
+  const float f = p.l != 0.f ? exp2_fast(p.m2 - p.m1) / p.l : 0.f;
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    const float x = p.l != 0.f ? p.o[i] * f : 0.f;
+    if constexpr (__is_same(T, __half)) out[i * 32 + lane] = __float2half_rn(x);
+    else out[i * 32 + lane] = __float2bfloat16_rn(x);
   }
 }
 
-// Codes and scales of one tile, as a thread holds them: lane = 4 g + j has tokens g and g + 8 of K, tokens 2 j, 2 j + 1, 2 j + 8 and
-// 2 j + 9 of V.
-template <int D> struct Tile {
-  uint32_t k[2][D / 16];
-  uint32_t v[4][D / 32];
-  float ks, vs;
-  bool there;
-};
+struct Open { int r, item, from_first, to_last; };      // item < 0: none
 
 template <typename T, int D, bool INT8, int NT>
-__global__ void __launch_bounds__(32 * CA_WARPS, NT == 1 ? 4 : 3) attend_kernel(const AttendArgs a) {
+__global__ void __launch_bounds__(32 * CA_WARPS, NT == 1 ? 3 : 2) attend_kernel(const AttendArgs a) {
   constexpr int KC = D / 64, MT = D / 16, VW = D / 32, COLS = 8 * NT;
-  extern __shared__ int before[];          // [R + 1]
+  extern __shared__ __align__(16) uint8_t ring[];      // of every warp; then the tiles of the requests before each, [R + 1]
+  int* before = reinterpret_cast<int*>(ring + CA_WARPS * warp_bytes<D, NT>());
   __shared__ int sums[CA_WARPS];
+  __shared__ Open open[CA_WARPS][2];         // the sequences that a warp has not seen whole: its first and its last
   pdl_launch_next();
   pdl_wait();
-  const int tid = threadIdx.x, lane = tid & 31, g8 = lane >> 2, j4 = lane & 3, BT = 1 << a.shift;
+  const int tid = threadIdx.x, lane = tid & 31, wid = tid >> 5, g8 = lane >> 2, j4 = lane & 3, BT = 1 << a.shift;
   const int most = min(static_cast<long long>(a.W) << a.shift, 0x7fffff00ll);
 
   // tiles of the requests before each: one scan per block of the grid
@@ -135,11 +178,14 @@ __global__ void __launch_bounds__(32 * CA_WARPS, NT == 1 ? 4 : 3) attend_kernel(
     if (r0 < a.R && r0 + per >= a.R) { before[a.R] = at; if (blockIdx.x == 0) a.before[a.R] = at; }
     __syncthreads();
   }
-  const int worker = blockIdx.x * CA_WARPS + (tid >> 5), per_tile = a.G * a.groups;
+  const int per_tile = a.G * a.groups;
   const long long units = static_cast<long long>(before[a.R]) * per_tile;
-  const int active = active_warps(units, a.workers);
-  if (worker >= active || units == 0) return;
-  const long long begin = first_unit(units, worker, active), end = first_unit(units, worker + 1, active);
+  const int active = active_blocks(units, a.workers);
+  if (blockIdx.x >= active || units == 0) return;
+  const long long block_begin = first_unit(units, blockIdx.x, active), block_units = first_unit(units, blockIdx.x + 1, active) - block_begin;
+  const long long begin = block_begin + block_units * wid / CA_WARPS, end = block_begin + block_units * (wid + 1) / CA_WARPS;
+  if (lane < 2) open[wid][lane].item = -1;
+  __syncwarp();
 
   int r = 0;
   for (int hi = a.R; hi - r > 1;) { const int mid = (r + hi) / 2; if (before[mid] <= begin / per_tile) r = mid; else hi = mid; }
@@ -217,157 +263,206 @@ __global__ void __launch_bounds__(32 * CA_WARPS, NT == 1 ? 4 : 3) attend_kernel(
 
     // the ids of 32 blocks, one per lane, ahead of their use
     const int* table = a.tables + static_cast<size_t>(r) * a.W;
-    const int down_shift = a.shift - 4;      // tiles to blocks
-    int id_base = t0 >> down_shift;
+    const int halves = (length + 15) / 16, down_shift = a.shift - 4;      // halves of tiles to blocks
+    int id_base = 2 * t0 >> down_shift;
     int ids = id_base + lane < a.W ? table[id_base + lane] : -1;
-    auto fetch = [&](int t, Tile<D>& x) {
-      const int b = t >> down_shift;
-      if (b - id_base == 32) { id_base = b; ids = b + lane < a.W ? table[b + lane] : -1; }
-      const int id = __shfl_sync(0xffffffffu, ids, b - id_base);
-      x.there = id >= 0 && id < a.N;
-      if (!x.there) return;
-      const size_t head = static_cast<size_t>(id) * a.G + g;
-      x.ks = __ldg(a.ks + head);
-      x.vs = __ldg(a.vs + head);
-      const size_t row = (head << a.shift) + ((t * CA_TILE) & (BT - 1));
-      const uint8_t* k = a.k + (row + g8) * D + j4 * 16;
-      const uint8_t* v = a.v + (row + 2 * j4) * D + g8 * (D / 8);
+    const uint32_t mine = smem_u32(ring) + wid * warp_bytes<D, NT>();
+    auto fetch = [&](int t, int stage) {
+      if (t < t1) {
+        const uint32_t to = mine + stage * Stage<D>::SIZE;
 #pragma unroll
-      for (int h = 0; h < KC; ++h) {
-        load_words<4>(k + h * 64, x.k[0] + 4 * h);
-        load_words<4>(k + 8 * D + h * 64, x.k[1] + 4 * h);
+        for (int h = 0; h < 2; ++h) {
+          const int half = 2 * t + h, b = half >> down_shift;
+          if (b - id_base == 32) { id_base = b; ids = b + lane < a.W ? table[b + lane] : -1; }
+          const int id = __shfl_sync(0xffffffffu, ids, b - id_base);
+          const bool there = half < halves && id >= 0 && id < a.N;
+          if (lane == 0) asm volatile("st.shared.b32 [%0], %1;" ::"r"(to + 2 * Stage<D>::BYTES + 16 * h + 8), "r"(static_cast<int>(there)) : "memory");
+          if (!there) continue;
+          const size_t head = static_cast<size_t>(id) * a.G + g;
+          if (lane < 2) copy4(to + 2 * Stage<D>::BYTES + 16 * h + 4 * lane, (lane ? a.vs : a.ks) + head);
+          const size_t from = ((head << a.shift) + ((half * 16) & (BT - 1))) * D;
+#pragma unroll
+          for (int x = 0; x < D / 32; ++x) {
+            const int i = x * 32 + lane, row = 16 * h + i / (D / 16), c = i % (D / 16);
+            copy16(to + Stage<D>::key_word(row, c) * 16, a.k + from + i * 16);
+            copy16(to + Stage<D>::BYTES + Stage<D>::value_word(row, c) * 16, a.v + from + i * 16);
+          }
+        }
       }
-      load_words<VW>(v, x.v[0]);
-      load_words<VW>(v + D, x.v[1]);
-      load_words<VW>(v + 8 * D, x.v[2]);
-      load_words<VW>(v + 9 * D, x.v[3]);
+      asm volatile("cp.async.commit_group;" ::: "memory");
     };
 
-    Tile<D> next;
-    fetch(t0, next);
+    __syncwarp();                            // the ring's last tile of the sequence before has been read
+    for (int i = 0; i < CA_STAGES - 1; ++i) fetch(t0 + i, i);
+    int stage = 0;
     for (int t = t0; t < t1; ++t) {
-      Tile<D> x = next;
-      if (t + 1 < t1) fetch(t + 1, next);
-      if (!x.there) continue;
+      __syncwarp();                          // the tile before has been read
+      fetch(t + CA_STAGES - 1, stage == 0 ? CA_STAGES - 1 : stage - 1);
+      asm volatile("cp.async.wait_group %0;" ::"n"(CA_STAGES - 1) : "memory");
+      __syncwarp();                          // everyone's part of this tile is there
+      const uint32_t at = mine + stage * Stage<D>::SIZE;
+      stage = stage == CA_STAGES - 1 ? 0 : stage + 1;
+      float ks[2], vs[2];
+      bool there[2];
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        uint32_t w[4];
+        shared_words<4>(at + 2 * Stage<D>::BYTES + 16 * h, w);
+        there[h] = w[2] != 0u;
+        ks[h] = there[h] ? __uint_as_float(w[0]) : 1.f;
+        vs[h] = there[h] ? __uint_as_float(w[1]) : 1.f;
+      }
+      if (!there[0] && !there[1]) continue;
 
-      float s[NT][4];
+      float s[2][NT][4];
 #pragma unroll
-      for (int n = 0; n < NT; ++n) s[n][0] = s[n][1] = s[n][2] = s[n][3] = 0.f;
+      for (int h = 0; h < 2; ++h) {
+        uint32_t k[2][D / 16];
 #pragma unroll
-      for (int i = 0; i < D / 16; ++i) {
-        uint32_t a0, a1, a2, a3;
-        widen<INT8>(x.k[0][i], a0, a2);
-        widen<INT8>(x.k[1][i], a1, a3);
+        for (int x = 0; x < KC; ++x) {
+          shared_words<4>(at + Stage<D>::key_word(16 * h + g8, 4 * x + j4) * 16, k[0] + 4 * x);
+          shared_words<4>(at + Stage<D>::key_word(16 * h + g8 + 8, 4 * x + j4) * 16, k[1] + 4 * x);
+        }
 #pragma unroll
-        for (int n = 0; n < NT; ++n) mma_f16(s[n], a0, a1, a2, a3, qf[n][i][0], qf[n][i][1]);
+        for (int n = 0; n < NT; ++n) s[h][n][0] = s[h][n][1] = s[h][n][2] = s[h][n][3] = 0.f;
+#pragma unroll
+        for (int i = 0; i < D / 16; ++i) {
+          uint32_t a0, a1, a2, a3;
+          widen<INT8>(k[0][i], a0, a2);
+          widen<INT8>(k[1][i], a1, a3);
+#pragma unroll
+          for (int n = 0; n < NT; ++n) mma_f16(s[h][n], a0, a1, a2, a3, qf[n][i][0], qf[n][i][1]);
+        }
       }
       // vs = 2^ev fv, 1 <= fv < 2
-      const float ev = static_cast<float>(static_cast<int>(__float_as_uint(x.vs) >> 23) - 127);
-      const float fv = __uint_as_float((__float_as_uint(x.vs) & 0x7fffffu) | 0x3f800000u);
+      float ev[2], fv[2];
       bool above = false;
-      const bool ragged = t * CA_TILE + CA_TILE > all;
+      const bool ragged = t * CA_TILE + CA_TILE > all || !there[0] || !there[1];
 #pragma unroll
-      for (int n = 0; n < NT; ++n)
+      for (int h = 0; h < 2; ++h) {
+        ev[h] = static_cast<float>(static_cast<int>(__float_as_uint(vs[h]) >> 23) - 127);
+        fv[h] = __uint_as_float((__float_as_uint(vs[h]) & 0x7fffffu) | 0x3f800000u);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          s[n][i] *= cscale[n][i & 1] * x.ks;
-          if (ragged && t * CA_TILE + g8 + (i >> 1) * 8 >= seen[n][i & 1]) s[n][i] = -INFINITY;
-          above |= s[n][i] > m1[n][i & 1] + 8.f || s[n][i] + ev > m2[n][i & 1] + 8.f;
-        }
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            float& x = s[h][n][i];
+            x *= cscale[n][i & 1] * ks[h];
+            if (ragged && (!there[h] || t * CA_TILE + 16 * h + g8 + (i >> 1) * 8 >= seen[n][i & 1])) x = -INFINITY;
+            above |= x > m1[n][i & 1] + 8.f || x + ev[h] > m2[n][i & 1] + 8.f;
+          }
+      }
       if (__any_sync(0xffffffffu, above)) {
 #pragma unroll
         for (int n = 0; n < NT; ++n)
 #pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            float top = fmaxf(s[n][h], s[n][h + 2]);
+          for (int i = 0; i < 2; ++i) {
+            float n1 = fmaxf(fmaxf(s[0][n][i], s[0][n][i + 2]), fmaxf(s[1][n][i], s[1][n][i + 2]));
+            float n2 = fmaxf(fmaxf(s[0][n][i], s[0][n][i + 2]) + ev[0], fmaxf(s[1][n][i], s[1][n][i + 2]) + ev[1]);
 #pragma unroll
-            for (int o = 4; o < 32; o <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-            const float n1 = fmaxf(m1[n][h], top), n2 = fmaxf(m2[n][h], top + ev);
-            l[n][h] *= exp2_fast(m1[n][h] - n1);
-            const float f = exp2_fast(m2[n][h] - n2);
-            m1[n][h] = n1; m2[n][h] = n2;
+            for (int o = 4; o < 32; o <<= 1) {
+              n1 = fmaxf(n1, __shfl_xor_sync(0xffffffffu, n1, o));
+              n2 = fmaxf(n2, __shfl_xor_sync(0xffffffffu, n2, o));
+            }
+            n1 = fmaxf(m1[n][i], n1); n2 = fmaxf(m2[n][i], n2);
+            l[n][i] *= exp2_fast(m1[n][i] - n1);
+            const float f = exp2_fast(m2[n][i] - n2);
+            m1[n][i] = n1; m2[n][i] = n2;
 #pragma unroll
-            for (int i = 0; i < MT; ++i) { acc[n][i][h] *= f; acc[n][i][h + 2] *= f; }
+            for (int y = 0; y < MT; ++y) { acc[n][y][i] *= f; acc[n][y][i + 2] *= f; }
           }
       }
-      uint32_t p[NT][2];
 #pragma unroll
-      for (int n = 0; n < NT; ++n) {
-        float w[4];
+      for (int h = 0; h < 2; ++h) {
+        uint32_t p[NT][2], v[4][VW];
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          l[n][i & 1] += exp2_fast(s[n][i] - m1[n][i & 1]);
-          w[i] = exp2_fast(s[n][i] + ev - m2[n][i & 1]) * fv;
+          const int row = 16 * h + 2 * j4 + (i & 1) + (i >> 1) * 8;
+          // D / 8 bytes of the row: a word of 16, or half of one
+          shared_words<VW>(at + Stage<D>::BYTES + (D == 128 ? Stage<D>::value_word(row, g8) * 16 : Stage<D>::value_word(row, g8 >> 1) * 16 + (g8 & 1) * 8), v[i]);
         }
-        p[n][0] = transpose8x8(pack_f16(w[0], w[1]));
-        p[n][1] = transpose8x8(pack_f16(w[2], w[3]));
-      }
-      if (ragged) {
-        // rows behind the sequence hold anything; a NaN that some columns see and others do not is kept from the others below
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
-          if (t * CA_TILE + 2 * j4 + (i & 1) + (i >> 1) * 8 >= length)
+        for (int n = 0; n < NT; ++n) {
+          float w[4];
 #pragma unroll
-            for (int w = 0; w < VW; ++w) x.v[i][w] = 0u;
-        if constexpr (!INT8) {
-          bool bad = false;
-          uint32_t nan[4][VW];
+          for (int i = 0; i < 4; ++i) {
+            l[n][i & 1] += exp2_fast(s[h][n][i] - m1[n][i & 1]);
+            w[i] = exp2_fast(s[h][n][i] + ev[h] - m2[n][i & 1]) * fv[h];
+          }
+          p[n][0] = transpose8x8(pack_f16(w[0], w[1]));
+          p[n][1] = transpose8x8(pack_f16(w[2], w[3]));
+        }
+        if (ragged) {
+          // rows behind the sequence hold anything; a NaN that some columns see and others do not is kept from the others below
 #pragma unroll
           for (int i = 0; i < 4; ++i)
+            if (!there[h] || t * CA_TILE + 16 * h + 2 * j4 + (i & 1) + (i >> 1) * 8 >= length)
 #pragma unroll
-            for (int w = 0; w < VW; ++w) {
-              nan[i][w] = __vcmpeq4(x.v[i][w] & 0x7f7f7f7fu, 0x7f7f7f7fu);
-              bad |= nan[i][w] != 0u;
-            }
-          if (__any_sync(0xffffffffu, bad)) {
-            // 1 where a value is NaN, times 1 where a column sees its token: a count above zero makes the sum NaN
-            uint32_t see[NT][2];
+              for (int w = 0; w < VW; ++w) v[i][w] = 0u;
+          if constexpr (!INT8) {
+            bool bad = false;
 #pragma unroll
-            for (int n = 0; n < NT; ++n)
+            for (int i = 0; i < 4; ++i)
 #pragma unroll
-              for (int e = 0; e < 2; ++e) {
-                const int token = t * CA_TILE + g8 + 8 * e;
-                see[n][e] = transpose8x8(pack_f16(token < seen[n][0] ? 1.f : 0.f, token < seen[n][1] ? 1.f : 0.f));
-              }
+              for (int w = 0; w < VW; ++w) bad |= __vcmpeq4(v[i][w] & 0x7f7f7f7fu, 0x7f7f7f7fu) != 0u;
+            if (__any_sync(0xffffffffu, bad)) {
+              // 1 where a value is NaN, times 1 where a column sees its token: a count above zero makes the sum NaN
+              uint32_t see[NT][2];
 #pragma unroll
-            for (int w = 0; w < VW; ++w) {
+              for (int n = 0; n < NT; ++n)
 #pragma unroll
-              for (int i = 0; i < 4; ++i) x.v[i][w] &= ~nan[i][w];
+                for (int e = 0; e < 2; ++e) {
+                  const int token = t * CA_TILE + 16 * h + g8 + 8 * e;
+                  see[n][e] = transpose8x8(pack_f16(token < seen[n][0] ? 1.f : 0.f, token < seen[n][1] ? 1.f : 0.f));
+                }
 #pragma unroll
-              for (int h = 0; h < 2; ++h) {
-                const uint32_t one = 0x38383838u;      // 1 in e4m3
-                const uint32_t x0 = __byte_perm(nan[0][w] & one, nan[1][w] & one, h ? 0x7362 : 0x5140);
-                const uint32_t x1 = __byte_perm(nan[2][w] & one, nan[3][w] & one, h ? 0x7362 : 0x5140);
-                uint32_t a0, a1, a2, a3;
-                widen<false>(x0, a0, a1);
-                widen<false>(x1, a2, a3);
+              for (int w = 0; w < VW; ++w) {
+                uint32_t one[4];                 // 1 in e4m3
 #pragma unroll
-                for (int n = 0; n < NT; ++n) {
-                  float count[4] = {0.f, 0.f, 0.f, 0.f};
-                  mma_f16(count, a0, a1, a2, a3, see[n][0], see[n][1]);
+                for (int i = 0; i < 4; ++i) {
+                  const uint32_t nan = __vcmpeq4(v[i][w] & 0x7f7f7f7fu, 0x7f7f7f7fu);
+                  v[i][w] &= ~nan;
+                  one[i] = nan & 0x38383838u;
+                }
 #pragma unroll
-                  for (int i = 0; i < 4; ++i) if (count[i] > 0.f) acc[n][2 * w + h][i] = __uint_as_float(0x7fffffffu);
+                for (int x = 0; x < 2; ++x) {
+                  uint32_t a0, a1, a2, a3;
+                  widen<false>(__byte_perm(one[0], one[1], x ? 0x7362 : 0x5140), a0, a1);
+                  widen<false>(__byte_perm(one[2], one[3], x ? 0x7362 : 0x5140), a2, a3);
+#pragma unroll
+                  for (int n = 0; n < NT; ++n) {
+                    float count[4] = {0.f, 0.f, 0.f, 0.f};
+                    mma_f16(count, a0, a1, a2, a3, see[n][0], see[n][1]);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) if (count[i] > 0.f) acc[n][2 * w + x][i] = __uint_as_float(0x7fffffffu);
+                  }
                 }
               }
             }
           }
         }
+#pragma unroll
+        for (int w = 0; w < VW; ++w)
+#pragma unroll
+          for (int x = 0; x < 2; ++x) {
+            uint32_t a0, a1, a2, a3;
+            widen<INT8>(__byte_perm(v[0][w], v[1][w], x ? 0x7362 : 0x5140), a0, a1);
+            widen<INT8>(__byte_perm(v[2][w], v[3][w], x ? 0x7362 : 0x5140), a2, a3);
+#pragma unroll
+            for (int n = 0; n < NT; ++n) mma_f16(acc[n][2 * w + x], a0, a1, a2, a3, p[n][0], p[n][1]);
+          }
       }
-#pragma unroll
-      for (int w = 0; w < VW; ++w)
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          uint32_t a0, a1, a2, a3;
-          widen<INT8>(__byte_perm(x.v[0][w], x.v[1][w], h ? 0x7362 : 0x5140), a0, a1);
-          widen<INT8>(__byte_perm(x.v[2][w], x.v[3][w], h ? 0x7362 : 0x5140), a2, a3);
-#pragma unroll
-          for (int n = 0; n < NT; ++n) mma_f16(acc[n][2 * w + h], a0, a1, a2, a3, p[n][0], p[n][1]);
-        }
     }
 
     // thread (g8, j4) has values g8 * D / 8 .. of columns 2 j4 and 2 j4 + 1
     const bool whole = t0 == 0 && t1 == tiles;
-    const size_t slot = 2 * static_cast<size_t>(worker) + (u == begin ? 0 : 1);
+    const int slot = u == begin ? 0 : 1;
+    if (!whole) {
+      __syncwarp();                          // the ring has been read: the sums take its place
+      if (lane == 0) open[wid][slot] = Open{r, item, t0 == 0, t1 == tiles};
+    }
+    float* parts = slot == 0 ? a.head + (static_cast<size_t>(blockIdx.x) * CA_WARPS + wid) * COLS * (D + 4)
+                             : reinterpret_cast<float*>(ring + wid * warp_bytes<D, NT>());
 #pragma unroll
     for (int n = 0; n < NT; ++n)
 #pragma unroll
@@ -375,40 +470,77 @@ __global__ void __launch_bounds__(32 * CA_WARPS, NT == 1 ? 4 : 3) attend_kernel(
         float total = l[n][h];
 #pragma unroll
         for (int o = 4; o < 32; o <<= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
+        if (seen[n][h] <= 0) total = 0.f;
         const int cc = n * 8 + 2 * j4 + h;
         if (cc >= cols) continue;
         if (whole) {
-          const int c = col0 + cc;
-          const float f = total != 0.f ? exp2_fast(m2[n][h] - m1[n][h]) / total : 0.f;      // 0: no block is there
-          T* o = static_cast<T*>(a.out) + ((static_cast<size_t>(r) * a.S + c / a.P) * a.G * a.P + g * a.P + c % a.P) * D + g8 * (D / 8);
+          const float f = total != 0.f ? exp2_fast(m2[n][h] - m1[n][h]) / total : 0.f;      // 0: nothing of what the column sees is there
+          T* o = output_row<T>(a, r, g, col0 + cc, D) + g8 * (D / 8);
 #pragma unroll
           for (int x = 0; x < D / 64; ++x) {
             uint32_t w[4];
 #pragma unroll
             for (int y = 0; y < 4; ++y) {
-              const float* s = acc[n][x * 4 + y];
-              const float lo = seen[n][h] > 0 ? s[h] * f : 0.f, hi = seen[n][h] > 0 ? s[h + 2] * f : 0.f;
+              const float* z = acc[n][x * 4 + y];
+              const float lo = total != 0.f ? z[h] * f : 0.f, hi = total != 0.f ? z[h + 2] * f : 0.f;
               if constexpr (__is_same(T, __half)) w[y] = pack_f16(lo, hi);
               else { const __nv_bfloat162 b = __floats2bfloat162_rn(lo, hi); w[y] = *reinterpret_cast<const uint32_t*>(&b); }
             }
             *reinterpret_cast<uint4*>(o + x * 8) = make_uint4(w[0], w[1], w[2], w[3]);
           }
         } else {
-          float* o = a.part + (slot * COLS + cc) * (D + 4);
+          float* o = parts + cc * (D + 4);
 #pragma unroll
           for (int i = 0; i < MT; i += 2)
             *reinterpret_cast<float4*>(o + g8 * (D / 8) + 2 * i) =
                 make_float4(acc[n][i][h], acc[n][i][h + 2], acc[n][i + 1][h], acc[n][i + 1][h + 2]);
-          if (g8 == 0) *reinterpret_cast<float4*>(o + D) = make_float4(m1[n][h], m2[n][h], seen[n][h] > 0 ? total : 0.f, 0.f);
+          if (g8 == 0) *reinterpret_cast<float4*>(o + D) = make_float4(m1[n][h], m2[n][h], total, 0.f);
         }
       }
     u += t1 - t0;
   }
+
+  // Sequences that several warps of the block share: put together here, finished where the block has seen them whole.
+  __syncthreads();
+  const Open* all_open = &open[0][0];
+  for (int i = 0; i < 2 * CA_WARPS;) {
+    const Open first = all_open[i];
+    if (first.item < 0) { ++i; continue; }
+    int last = i, next = i + 1;
+    for (; next < 2 * CA_WARPS && (all_open[next].item < 0 || (all_open[next].item == first.item && all_open[next].r == first.r)); ++next)
+      if (all_open[next].item >= 0) last = next;
+    const bool whole = first.from_first && all_open[last].to_last;
+    const int g = first.item / a.groups, col0 = first.item % a.groups * COLS, cols = min(a.S * a.P - col0, COLS);
+    // the partial result of a sequence that began in another block, or at this block's first unit, is the block's first
+    const long long from = static_cast<long long>(before[first.r]) * per_tile +
+                           static_cast<long long>(first.item) * (before[first.r + 1] - before[first.r]);
+    const size_t slot = 2 * static_cast<size_t>(blockIdx.x) + (from <= block_begin ? 0 : 1);
+    for (int cc = wid; cc < cols; cc += CA_WARPS) {
+      Partial<D / 32> p;
+      for (int x = i; x <= last; ++x) {
+        if (all_open[x].item < 0) continue;
+        const float* z = (x & 1 ? reinterpret_cast<const float*>(ring + x / 2 * warp_bytes<D, NT>())
+                                : a.head + (static_cast<size_t>(blockIdx.x) * CA_WARPS + x / 2) * COLS * (D + 4)) + cc * (D + 4);
+        float f[D / 32];
+#pragma unroll
+        for (int y = 0; y < D / 32; ++y) f[y] = z[y * 32 + lane];
+        p.add(z[D], z[D + 1], z[D + 2], f);
+      }
+      if (whole) write_row(output_row<T>(a, first.r, g, col0 + cc, D), p, lane);
+      else {
+        float* o = a.part + (slot * COLS + cc) * (D + 4);
+#pragma unroll
+        for (int y = 0; y < D / 32; ++y) o[y * 32 + lane] = p.o[y];
+        if (lane == 0) *reinterpret_cast<float4*>(o + D) = make_float4(p.m1, p.m2, p.l, 0.f);
+      }
+    }
+    i = next;
+  }
 }
 
-constexpr int MERGE_WARPS = 16;
+constexpr int MERGE_WARPS = 8, MERGE_AT_ONCE = 4;
 
-// Adds up the partial sums of the sequences that several warps share, in the order of their tokens, and writes zeros for requests
+// Adds up the partial sums of the sequences that several blocks share, in the order of their tokens, and writes zeros for requests
 // without tokens.  One block per sequence (request, KV head, group of columns); its warps share columns and parts.
 template <typename T, int D>
 __global__ void __launch_bounds__(32 * MERGE_WARPS) attend_merge_kernel(const AttendArgs a, int columns) {
@@ -417,100 +549,73 @@ __global__ void __launch_bounds__(32 * MERGE_WARPS) attend_merge_kernel(const At
   pdl_launch_next();
   pdl_wait();
   const int lane = threadIdx.x & 31, w = threadIdx.x >> 5, per_tile = a.G * a.groups;
+  const int r = blockIdx.x / per_tile, item = blockIdx.x % per_tile, g = item / a.groups;
+  const int tiles = a.before[r + 1] - a.before[r], col0 = item % a.groups * columns, cols = min(a.S * a.P - col0, columns);
   const long long units = static_cast<long long>(a.before[a.R]) * per_tile;
-  const int active = active_warps(units, a.workers);
-  const long long items = static_cast<long long>(a.R) * per_tile;
-  for (long long item = blockIdx.x; item < items; item += gridDim.x) {
-    const int r = static_cast<int>(item / per_tile), rest = static_cast<int>(item % per_tile), g = rest / a.groups;
-    const int tiles = a.before[r + 1] - a.before[r], col0 = rest % a.groups * columns, cols = min(a.S * a.P - col0, columns);
-    int w0 = 0, w1 = -1;
-    long long from = 0;
-    if (tiles) {
-      from = static_cast<long long>(a.before[r]) * per_tile + static_cast<long long>(rest) * tiles;
-      w0 = owner(from, units, active);
-      w1 = owner(from + tiles - 1, units, active);
-      if (w0 == w1) continue;
-    }
-    // `share` warps per column, each with a run of the parts
-    int share = 1;
-    while (2 * share * cols <= MERGE_WARPS) share *= 2;
-    const int parts = w1 - w0 + 1, per = (parts + share - 1) / share;
-    for (int c0 = 0; c0 < cols; c0 += MERGE_WARPS / share) {
-      const int cc = c0 + w / share, mine = w % share;
-      float top1 = CA_LOWEST, top2 = CA_LOWEST, l = 0.f, o[PER];
+  const int active = active_blocks(units, a.workers);
+  const long long from = static_cast<long long>(a.before[r]) * per_tile + static_cast<long long>(item) * tiles;
+  int w0 = 0, parts = 0;
+  if (tiles) {
+    w0 = owner(from, units, active);
+    parts = owner(from + tiles - 1, units, active) - w0 + 1;
+    if (parts == 1) return;
+  }
+  // `share` warps per column, each with a run of the parts
+  int share = 1;
+  while (2 * share * cols <= MERGE_WARPS && share * MERGE_AT_ONCE < parts) share *= 2;
+  const int per = (parts + share - 1) / share, first_slot = tiles && from != first_unit(units, w0, active);
+  for (int c0 = 0; c0 < cols; c0 += MERGE_WARPS / share) {
+    const int cc = c0 + w / share, mine = w % share, end = min(parts, mine * per + per);
+    Partial<PER> p;
+    if (cc < cols)
+      for (int x0 = mine * per; x0 < end; x0 += MERGE_AT_ONCE) {
+        float4 st[MERGE_AT_ONCE];
+        float f[MERGE_AT_ONCE][PER];
 #pragma unroll
-      for (int i = 0; i < PER; ++i) o[i] = 0.f;
-      if (cc < cols)
-        for (int x0 = mine * per; x0 < min(parts, mine * per + per); x0 += 4) {
-          float4 st[4];
-          float f[4][PER];
-          const int n = min(4, min(parts, mine * per + per) - x0);
+        for (int y = 0; y < MERGE_AT_ONCE; ++y)
+          if (x0 + y < end) {
+            const size_t slot = 2 * static_cast<size_t>(w0 + x0 + y) + (x0 + y == 0 ? first_slot : 0);
+            const float* z = a.part + (slot * columns + cc) * (D + 4);
+            st[y] = *reinterpret_cast<const float4*>(z + D);
 #pragma unroll
-          for (int y = 0; y < 4; ++y)
-            if (y < n) {
-              const int worker = w0 + x0 + y;
-              const size_t slot = 2 * static_cast<size_t>(worker) + (x0 + y == 0 && from != first_unit(units, worker, active) ? 1 : 0);
-              const float* p = a.part + (slot * columns + cc) * (D + 4);
-              st[y] = *reinterpret_cast<const float4*>(p + D);
-#pragma unroll
-              for (int i = 0; i < PER; ++i) f[y][i] = p[i * 32 + lane];
-            }
-#pragma unroll
-          for (int y = 0; y < 4; ++y)
-            if (y < n) {
-              const float n1 = fmaxf(top1, st[y].x), n2 = fmaxf(top2, st[y].y);
-              const float a2 = exp2_fast(top2 - n2), b2 = exp2_fast(st[y].y - n2);
-              l = l * exp2_fast(top1 - n1) + st[y].z * exp2_fast(st[y].x - n1);
-#pragma unroll
-              for (int i = 0; i < PER; ++i) o[i] = o[i] * a2 + f[y][i] * b2;
-              top1 = n1; top2 = n2;
-            }
-        }
-      if (share > 1) {
-        __syncthreads();
-#pragma unroll
-        for (int i = 0; i < PER; ++i) sums[w][i * 32 + lane] = o[i];
-        if (lane == 0) { stats[w][0] = top1; stats[w][1] = top2; stats[w][2] = l; }
-        __syncthreads();
-        if (mine == 0)
-          for (int y = w + 1; y < w + share; ++y) {
-            const float n1 = fmaxf(top1, stats[y][0]), n2 = fmaxf(top2, stats[y][1]);
-            const float a2 = exp2_fast(top2 - n2), b2 = exp2_fast(stats[y][1] - n2);
-            l = l * exp2_fast(top1 - n1) + stats[y][2] * exp2_fast(stats[y][0] - n1);
-#pragma unroll
-            for (int i = 0; i < PER; ++i) o[i] = o[i] * a2 + sums[y][i * 32 + lane] * b2;
-            top1 = n1; top2 = n2;
+            for (int i = 0; i < PER; ++i) f[y][i] = z[i * 32 + lane];
           }
-      }
-      if (mine == 0 && cc < cols) {
-        const int c = col0 + cc;
-        // a column that sees nothing: no tokens, or none of this request's queries
-        const int length = a.lengths[r], fresh = a.fresh ? min(max(a.fresh[r], 0), a.S) : a.S;
-        const bool sees = tiles && c / a.P < fresh && length - fresh + c / a.P + 1 > 0;
-        const float f = l != 0.f ? exp2_fast(top2 - top1) / l : 0.f;
-        T* out = static_cast<T*>(a.out) + ((static_cast<size_t>(r) * a.S + c / a.P) * a.G * a.P + g * a.P + c % a.P) * D;
 #pragma unroll
-        for (int i = 0; i < PER; ++i) {
-          const float x = sees ? o[i] * f : 0.f;
-          if constexpr (__is_same(T, __half)) out[i * 32 + lane] = __float2half_rn(x);
-          else out[i * 32 + lane] = __float2bfloat16_rn(x);
-        }
+        for (int y = 0; y < MERGE_AT_ONCE; ++y)
+          if (x0 + y < end) p.add(st[y].x, st[y].y, st[y].z, f[y]);
       }
+    if (share > 1) {
+      __syncthreads();
+#pragma unroll
+      for (int i = 0; i < PER; ++i) sums[w][i * 32 + lane] = p.o[i];
+      if (lane == 0) { stats[w][0] = p.m1; stats[w][1] = p.m2; stats[w][2] = p.l; }
+      __syncthreads();
+      if (mine == 0)
+        for (int y = w + 1; y < w + share; ++y) {
+          float f[PER];
+#pragma unroll
+          for (int i = 0; i < PER; ++i) f[i] = sums[y][i * 32 + lane];
+          p.add(stats[y][0], stats[y][1], stats[y][2], f);
+        }
     }
+    if (mine == 0 && cc < cols) write_row(output_row<T>(a, r, g, col0 + cc, D), p, lane);
   }
 }
 
 static int attend_columns(int queries) { return queries <= 8 ? 8 : 16; }
-static int attend_blocks(int columns) { return sm_count_current() * (columns == 8 ? 4 : 3); }
+#ifndef CA_WAVES
+#define CA_WAVES 1
+#endif
+static int attend_blocks(int columns) { return sm_count_current() * (columns == 8 ? 3 : 2) * CA_WAVES; }
 
 }  // namespace axb
 
 using namespace axb;
 
-// 32-bit words of the workspace: the tile counts, then two partial results per warp
+// 32-bit words of the workspace: the tile counts, then two partial results per block
 extern "C" long long axb_cached_attention_words(int R, int S, int P, int D) {
   const int columns = attend_columns(S * P);
-  return (R + 1 + 3) / 4 * 4 + 2ll * attend_blocks(columns) * CA_WARPS * columns * (D + 4);
+  return (R + 1 + 3) / 4 * 4 + (2ll + CA_WARPS) * attend_blocks(columns) * columns * (D + 4);
 }
 
 extern "C" int axb_cached_attention(const void* q, long long q_row, long long q_token, long long q_group, const void* k, const void* v,
@@ -530,7 +635,7 @@ extern "C" int axb_cached_attention(const void* q, long long q_row, long long q_
   }
   const int columns = attend_columns(S * P), groups = (S * P + columns - 1) / columns, blocks = attend_blocks(columns);
   AttendArgs a{q, q_row, q_token, q_group, out, (const uint8_t*)k, (const uint8_t*)v, ks, vs, tables, lengths, fresh, R, S, G, P, W, N, shift,
-               groups, scale * 1.4426950408889634f, blocks * CA_WARPS, (int*)work, nullptr};
+               groups, scale * 1.4426950408889634f, blocks, (int*)work, nullptr, nullptr};
   void (*kern)(AttendArgs) = nullptr;
 #define AXB_PICK(T, D_, NT) (int8 ? attend_kernel<T, D_, true, NT> : attend_kernel<T, D_, false, NT>)
 #define AXB_PICK_D(T, NT) (D == 64 ? AXB_PICK(T, 64, NT) : AXB_PICK(T, 128, NT))
@@ -549,10 +654,12 @@ extern "C" int axb_cached_attention(const void* q, long long q_row, long long q_
     a.lengths = lengths + r0;
     a.fresh = fresh ? fresh + r0 : nullptr;
     a.part = reinterpret_cast<float*>(a.before + (a.R + 1 + 3) / 4 * 4);
-    AXB_CUDA(pdl_launch(kern, dim3(blocks), dim3(32 * CA_WARPS), (a.R + 1) * sizeof(int), (cudaStream_t)stream, a));
-    const long long items = static_cast<long long>(a.R) * G * groups;
-    const int most = 2 * sm_count_current();
-    AXB_CUDA(pdl_launch(merge, dim3((unsigned)(items < most ? items : most)), dim3(32 * MERGE_WARPS), 0, (cudaStream_t)stream, a, columns));
+    a.head = a.part + 2ll * blocks * columns * (D + 4);
+    const int per_warp = columns == 8 ? (D == 64 ? warp_bytes<64, 1>() : warp_bytes<128, 1>()) : (D == 64 ? warp_bytes<64, 2>() : warp_bytes<128, 2>());
+    const size_t shared = CA_WARPS * per_warp + (a.R + 1) * sizeof(int);
+    AXB_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(shared)));
+    AXB_CUDA(pdl_launch(kern, dim3(blocks), dim3(32 * CA_WARPS), shared, (cudaStream_t)stream, a));
+    AXB_CUDA(pdl_launch(merge, dim3(a.R * G * groups), dim3(32 * MERGE_WARPS), 0, (cudaStream_t)stream, a, columns));
   }
   return 0;
 }
