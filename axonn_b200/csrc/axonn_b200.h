@@ -336,7 +336,7 @@ int axb_cached_attention(const void* q, long long q_row, long long q_token, long
 
 /* ---- selection of beam search (beam.cu): logits [B, K, V], scores [B, K] -> the K best continuations of every prompt; done [B, K] (or
  * NULL) with its end token.  work: axb_beam_select_words() 32-bit words, 8-byte aligned, of this call alone */
-long long axb_beam_select_words(int B, int K, int V);
+long long axb_beam_select_words(int B, int K, int V, int dtype);
 int axb_beam_select(const void* logits, const float* scores, const void* done, int eos, float* out_scores, long long* out_tokens,
                     int* out_parents, void* out_done, void* work, int B, int K, int V, int dtype, void* stream);
 

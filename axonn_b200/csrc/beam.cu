@@ -1,21 +1,30 @@
 // Selection of beam search: of all continuations of the beams of a prompt, value = score + logit - log sum exp(logits of the beam), the
 // `beams` best, equal values in the order of (beam, token).
 //
-// Bound by reading the logits once.  A first launch cuts every beam's row into parts: each warp keeps a running maximum and sum of
-// exponentials per lane and the best logits of what it has seen, sorted, one per lane; a value that does not beat the worst of them costs
-// a comparison per eight.  The order within a beam is that of its logits, so that nothing has to be known of the sum.  A second launch
-// puts the parts of a beam together and merges the beams' lists.  Sums and values there are 64-bit: the order of two beams' tokens
+// Bound by reading the logits once.  A first launch cuts every beam's row into parts of 8 KB, each of which a warp copies into shared
+// memory and goes over twice: no block ever waits for its warps, and the loops are short (the same code for 8 KB in registers is five
+// times as long, and was waited for longer than the data).  The K-th largest of the lanes' maxima is reached by at least K values of the part and by few others,
+// which go into a list in shared memory, of which the K best are kept.  (Where too many values reach the bound - rows of equal values -
+// the K best are found one by one.)  The order within a beam is that of its logits, so that nothing has to be known of the sum.  A second
+// launch puts the parts of a beam together and merges the beams.  Sums and values there are 64-bit: the order of two beams' tokens
 // depends on differences of their sums' logarithms that 32-bit values of twenty or so round away.
 //
-// A value that is not a number counts as -inf, and so do a score of +inf and every value of a beam whose sum is none.  Of a beam that has ended only the
-// end token goes on, with the beam's score.
+// A value that is not a number counts as -inf, and so do a score of +inf and every value of a beam whose sum is none.  Of a beam that has
+// ended only the end token goes on, with the beam's score.
+#include <type_traits>
+
 #include "common.cuh"
 
 namespace axb {
 
-constexpr int BEAM_MOST = 32;            // beams: a warp's list has one entry per lane
-constexpr int BEAM_WARPS = 8;
-constexpr int BEAM_PARTS = 32;           // of a row, at most: one per lane
+constexpr int BEAM_MOST = 32;            // beams
+constexpr int BEAM_WARPS = 4;            // of a block of the first launch
+constexpr int BEAM_LOADS = 16;           // 16-byte words of a lane
+constexpr int BEAM_PART = 32 * BEAM_LOADS * 16;      // bytes of a part
+constexpr int BEAM_LIST = 64;            // values that reach the bound, at most
+constexpr int SELECT_THREADS = 256;
+constexpr float BEAM_LOWEST = -3.4028234663852886e38f;
+constexpr float BEAM_HUGE = 1e38f;       // a maximum whose product with L is finite
 constexpr float LOG2E = 1.4426950408889634f;
 
 struct BeamArgs {
@@ -26,11 +35,11 @@ struct BeamArgs {
   long long* out_tokens;
   int* out_parents;
   unsigned char* out_done;
-  // of every row and part: K keys and K tokens, best first, and (maximum, sum)
-  uint32_t* keys;
-  int* tokens;
+  // of every row and part: (maximum, sum), then K keys and tokens, best first
   float2* sums;
-  int B, K, V, eos, parts, part_steps;   // part_steps: steps of 256 values of a warp in a part
+  uint2* lists;
+  int K, V, eos, parts;
+  long long items;                       // parts of all rows
 };
 
 // 32-bit key with the order of the numbers; 0 is below all of them.  -0 counts as 0.
@@ -40,224 +49,321 @@ __device__ __forceinline__ uint32_t order_key(float x) {
 }
 __device__ __forceinline__ float key_value(uint32_t k) { return __uint_as_float(k & 0x80000000u ? k & 0x7fffffffu : ~k); }
 
-// A warp's list: lane i has the i-th best (larger key, then lower token); key 0: none.
-struct BestList {
-  uint32_t key = 0u;
-  int token = -1;
-  __device__ __forceinline__ void insert(uint32_t k, int t, int lane) {
-    const uint32_t better = __ballot_sync(0xffffffffu, key > k || (key == k && key != 0u && token < t));
-    const int at = __popc(better);
-    const uint32_t up_key = __shfl_up_sync(0xffffffffu, key, 1);
-    const int up_token = __shfl_up_sync(0xffffffffu, token, 1);
-    if (lane > at) { key = up_key; token = up_token; }
-    else if (lane == at) { key = k; token = t; }
+// The best of what the lanes hold (the larger key, then the lower token); key 0: none is left.  It is taken out.
+template <int N> __device__ __forceinline__ uint2 take_best(uint32_t (&key)[N], int (&token)[N]) {
+  uint32_t k = 0u;
+#pragma unroll
+  for (int i = 0; i < N; ++i) k = max(k, key[i]);
+  k = __reduce_max_sync(0xffffffffu, k);
+  int t = 0x7fffffff;
+#pragma unroll
+  for (int i = 0; i < N; ++i) if (key[i] == k) t = min(t, token[i]);
+  t = __reduce_min_sync(0xffffffffu, t);
+#pragma unroll
+  for (int i = 0; i < N; ++i) if (token[i] == t) key[i] = 0u;
+  return make_uint2(k, static_cast<uint32_t>(t));
+}
+
+// The `K` best of a list's `count` entries, at most 32 N, in their order.
+template <int N> __device__ __forceinline__ void keep_best(const uint2* list, int count, uint2* out, int K) {
+  const int lane = threadIdx.x & 31;
+  uint32_t key[N];
+  int token[N];
+  uint2 mine = make_uint2(0u, 0u);
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    const int e = i * 32 + lane;
+    key[i] = 0u; token[i] = 0x7fffffff;
+    if (e < count) { key[i] = list[e].x; token[i] = static_cast<int>(list[e].y); }
+  }
+  for (int e = 0; e < K; ++e) {
+    const uint2 best = take_best(key, token);
+    if (lane == e) mine = best;
+  }
+  if (lane < K) out[lane] = mine;
+}
+
+// 16 bytes of logits: words of two 16-bit values or one of 32 bits.
+template <typename T> struct Values {
+  static constexpr int COUNT = 16 / sizeof(T), PER_WORD = 4 / sizeof(T);
+  uint32_t word[4];
+  __device__ __forceinline__ float operator[](int i) const {
+    if constexpr (__is_same(T, float)) return __uint_as_float(word[i]);
+    else {
+      const uint32_t w = word[i / 2];
+      if constexpr (__is_same(T, __nv_bfloat16)) return __uint_as_float(i & 1 ? w & 0xffff0000u : w << 16);
+      else return __half2float(__ushort_as_half(static_cast<unsigned short>(i & 1 ? w >> 16 : w & 0xffffu)));
+    }
+  }
+  __device__ __forceinline__ uint32_t largest() const { return larger(larger(word[0], word[1]), larger(word[2], word[3])); }
+  // the larger ones of two words' values; whether any of a word's values reaches `w`'s; a word of one value, the larger value of a word
+  static __device__ __forceinline__ uint32_t larger(uint32_t a, uint32_t b) {
+    if constexpr (__is_same(T, float)) return __float_as_uint(fmaxf(__uint_as_float(a), __uint_as_float(b)));
+    else if constexpr (__is_same(T, __nv_bfloat16)) {
+      const __nv_bfloat162 m = __hmax2(*reinterpret_cast<const __nv_bfloat162*>(&a), *reinterpret_cast<const __nv_bfloat162*>(&b));
+      return *reinterpret_cast<const uint32_t*>(&m);
+    } else {
+      const __half2 m = __hmax2(*reinterpret_cast<const __half2*>(&a), *reinterpret_cast<const __half2*>(&b));
+      return *reinterpret_cast<const uint32_t*>(&m);
+    }
+  }
+  static __device__ __forceinline__ uint32_t reaching(uint32_t a, uint32_t w) {
+    if constexpr (__is_same(T, float)) return __uint_as_float(a) >= __uint_as_float(w) ? 0xffffffffu : 0u;
+    else if constexpr (__is_same(T, __nv_bfloat16)) return __hge2_mask(*reinterpret_cast<const __nv_bfloat162*>(&a), *reinterpret_cast<const __nv_bfloat162*>(&w));
+    else return __hge2_mask(*reinterpret_cast<const __half2*>(&a), *reinterpret_cast<const __half2*>(&w));
+  }
+  static __device__ __forceinline__ uint32_t word_of(float x) {      // x is one of the type's numbers
+    if constexpr (__is_same(T, float)) return __float_as_uint(x);
+    else if constexpr (__is_same(T, __nv_bfloat16)) return (__float_as_uint(x) >> 16) * 0x10001u;
+    else return __half_as_ushort(__float2half_rn(x)) * 0x10001u;
+  }
+  static __device__ __forceinline__ float largest_of(uint32_t w) {
+    const Values v = {{w, w, w, w}};
+    if constexpr (__is_same(T, float)) return v[0];
+    else return fmaxf(v[0], v[1]);
   }
 };
 
-template <typename T> __device__ __forceinline__ float logit_value(T x);
-template <> __device__ __forceinline__ float logit_value(float x) { return x; }
-template <> __device__ __forceinline__ float logit_value(__nv_bfloat16 x) { return __bfloat162float(x); }
-template <> __device__ __forceinline__ float logit_value(__half x) { return __half2float(x); }
-
-// One step of a warp is 256 values.  VEC: every row starts on 16 bytes, lane has values 8 lane ..; otherwise lane has values lane, lane +
-// 32 ... - for all rows of a call alike, so that equal rows have equal sums.
-template <typename T, bool VEC> __device__ __forceinline__ int value_index(int lane, int j) { return VEC ? lane * 8 + j : j * 32 + lane; }
-template <typename T, bool VEC> __device__ __forceinline__ void load_step(const T* row, int base, int V, int lane, float (&x)[8]) {
-  if (VEC && base + 256 <= V) {
-    T t[8];
-#pragma unroll
-    for (int i = 0; i < static_cast<int>(sizeof(T)) / 2; ++i)
-      reinterpret_cast<uint4*>(t)[i] = __ldg(reinterpret_cast<const uint4*>(row + base + lane * 8) + i);
-#pragma unroll
-    for (int j = 0; j < 8; ++j) x[j] = logit_value(t[j]);
-  } else {
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const int i = base + value_index<T, VEC>(lane, j);
-      x[j] = i < V ? logit_value(row[i]) : __int_as_float(0xff800000);
-    }
-  }
+// Two 32-bit numbers in a register pair.
+__device__ __forceinline__ unsigned long long pair_of(float a, float b) {
+  unsigned long long p;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(p) : "f"(a), "f"(b));
+  return p;
+}
+__device__ __forceinline__ void unpair(unsigned long long p, float& a, float& b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(p)); }
+__device__ __forceinline__ unsigned long long fma_pair(unsigned long long a, unsigned long long b, unsigned long long c) {
+  unsigned long long d;
+  asm("fma.rn.ftz.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+  return d;
+}
+__device__ __forceinline__ unsigned long long add_pair(unsigned long long a, unsigned long long b) {
+  unsigned long long d;
+  asm("add.rn.ftz.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
 }
 
+// VEC: every row starts on 16 bytes.
 template <typename T, bool VEC>
 __global__ void __launch_bounds__(32 * BEAM_WARPS) beam_rows_kernel(const BeamArgs a) {
-  __shared__ uint32_t s_key[BEAM_WARPS][BEAM_MOST];
-  __shared__ int s_token[BEAM_WARPS][BEAM_MOST];
-  __shared__ float2 s_sum[BEAM_WARPS];
+  using X = Values<T>;
+  constexpr int PART = BEAM_PART / sizeof(T);
+  __shared__ uint4 s_part[BEAM_WARPS][BEAM_LOADS * 32];
+  __shared__ uint2 s_list[BEAM_WARPS][BEAM_LIST];
+  __shared__ unsigned s_count[BEAM_WARPS];
   pdl_launch_next();
   pdl_wait();
-  const int lane = threadIdx.x & 31, w = threadIdx.x >> 5, K = a.K, V = a.V;
-  const long long row_at = blockIdx.x;
-  if (a.done && a.done[row_at]) return;
-  const T* row = static_cast<const T*>(a.logits) + row_at * V;
-  const int first = blockIdx.y * a.part_steps * BEAM_WARPS * 256, last = min(static_cast<long long>(V), first + a.part_steps * BEAM_WARPS * 256ll);
-  float m = -3.4028234663852886e38f, sum = 0.f;
-  BestList best;
-  uint32_t worst = 0u;                   // key of the list's last entry: 0 while it is not full
-  bool begun = false;
-  int base = first + w * 256;
-  float next[8];
-  if (base < last) load_step<T, VEC>(row, base, V, lane, next);
-  for (; base < last; base += BEAM_WARPS * 256) {
-    float x[8];
-#pragma unroll
-    for (int j = 0; j < 8; ++j) x[j] = next[j];
-    if (base + BEAM_WARPS * 256 < last) load_step<T, VEC>(row, base + BEAM_WARPS * 256, V, lane, next);
-    float top = x[0];
-#pragma unroll
-    for (int j = 1; j < 8; ++j) top = fmaxf(top, x[j]);
-    if (top > m) { sum *= exp2f((m - top) * LOG2E); m = top; }
-#pragma unroll
-    for (int j = 0; j < 8; ++j) sum += exp2f((x[j] - m) * LOG2E);
-    uint32_t above = worst;              // keys above this are looked at
-    if (!begun) {
-      // the K-th largest of the lanes' maxima: at least K values reach it, and few others do
-      begun = true;
-      uint32_t k = order_key(top);
-#pragma unroll
-      for (int size = 2; size <= 32; size <<= 1)
-#pragma unroll
-        for (int o = size >> 1; o > 0; o >>= 1) {
-          const uint32_t other = __shfl_xor_sync(0xffffffffu, k, o);
-          const bool larger_here = ((lane & size) == 0) == ((lane & o) == 0);
-          k = larger_here ? max(k, other) : min(k, other);
-        }
-      above = __shfl_sync(0xffffffffu, k, K - 1);
-      above -= above != 0u;
-    }
-    if (__any_sync(0xffffffffu, order_key(top) > above)) {
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const int t = base + value_index<T, VEC>(lane, j);
-        const uint32_t k = t < V ? order_key(x[j]) : 0u;
-        uint32_t hits = __ballot_sync(0xffffffffu, k > above);
-        while (hits) {
-          const int from = __ffs(hits) - 1;
-          hits &= hits - 1;
-          best.insert(__shfl_sync(0xffffffffu, k, from), __shfl_sync(0xffffffffu, t, from), lane);
-        }
-      }
-      // what came in at an equal key keeps the order of the tokens: insert compares both
-      worst = __shfl_sync(0xffffffffu, best.key, K - 1);
-    }
+  const int lane = threadIdx.x & 31, w = threadIdx.x >> 5, K = a.K;
+  const long long part = static_cast<long long>(blockIdx.x) * BEAM_WARPS + w;
+  if (part >= a.items) return;
+  const int row = static_cast<int>(part / a.parts), base = static_cast<int>(part - static_cast<long long>(row) * a.parts) * PART, V = a.V - base;
+  if (a.done && a.done[row]) return;
+  const T* from = static_cast<const T*>(a.logits) + static_cast<long long>(row) * a.V + base;
+  uint4* words = s_part[w];
+  // 16 bytes of the warp's part; whole words are copied, the last ones of a row and rows off 16 bytes value by value, and what is not
+  // there is -inf
+  const int loads = (min(V, PART) * static_cast<int>(sizeof(T)) + 511) / 512;
+  const int whole = VEC ? min(V, PART) / X::COUNT : 0;
+  for (int i = 0; i < loads; ++i)
+    if (i * 32 + lane < whole)
+      asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(words + i * 32 + lane)), "l"(from + (i * 32 + lane) * X::COUNT) : "memory");
+  {
+    using Bits = std::conditional_t<sizeof(T) == 4, uint32_t, uint16_t>;
+    constexpr Bits lowest = static_cast<Bits>(__is_same(T, float) ? 0xff800000u : __is_same(T, __half) ? 0xfc00u : 0xff80u);
+    Bits* to = reinterpret_cast<Bits*>(words);
+#pragma unroll 8
+    for (int t = whole * X::COUNT + lane; t < loads * 32 * X::COUNT; t += 32) to[t] = t < V ? reinterpret_cast<const Bits*>(from)[t] : lowest;
   }
-  // the warps' lists, one by one: a list ends where its entries no longer come in
-  if (lane < K) { s_key[w][lane] = best.key; s_token[w][lane] = best.token; }
-  float top = m;
+  if (lane == 0) s_count[w] = 0u;
+  asm volatile("cp.async.wait_all;" ::: "memory");
+  __syncwarp();
+  auto at = [&](int i) {
+    const uint4 u = words[i * 32 + lane];
+    return X{{u.x, u.y, u.z, u.w}};
+  };
+  uint32_t most = X::word_of(-INFINITY);
+#pragma unroll 4
+  for (int i = 0; i < loads; ++i) most = X::larger(most, at(i).largest());
+  // the K-th largest of the lanes' maxima (equal ones count once: a lower bound does as well)
+  uint32_t mine = order_key(X::largest_of(most));
+  const uint32_t largest = __reduce_max_sync(0xffffffffu, mine);
+  uint32_t bound = largest;
+  for (int e = 1; e < K; ++e) {
+    if (mine == bound) mine = 0u;
+    bound = __reduce_max_sync(0xffffffffu, mine);
+  }
+  const uint32_t reach = X::word_of(bound ? key_value(bound) : -INFINITY);      // as numbers
+  const float m = fmaxf(key_value(largest), BEAM_LOWEST);
+  const bool ordinary = fabsf(m) < BEAM_HUGE;
+  const unsigned long long scale = pair_of(LOG2E, LOG2E), shift = pair_of(-m * LOG2E, -m * LOG2E);
+  unsigned long long sums = 0ull;
+  float sum = 0.f;
+#pragma unroll 2
+  for (int i = 0; i < loads; ++i) {
+    const X x = at(i);
+    if (ordinary) {
+      // exp(x - m) as exp2(x L - m L), two at a time: the rounding of m L is put right where the sums are used
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-  sum *= exp2f((m - top) * LOG2E);
+      for (int j = 0; j < X::COUNT; j += 2) {
+        float u, v;
+        unpair(fma_pair(pair_of(x[j], x[j + 1]), scale, shift), u, v);
+        sums = add_pair(sums, pair_of(exp2f(u), exp2f(v)));
+      }
+    } else {
+#pragma unroll
+      for (int j = 0; j < X::COUNT; ++j) sum += exp2f((x[j] - m) * LOG2E);
+    }
+    if (X::reaching(x.largest(), reach))
+#pragma unroll
+      for (int j = 0; j < X::COUNT; ++j)
+        if (X::reaching(x.word[j / X::PER_WORD], reach) >> (16 * (j % X::PER_WORD)) & 1u) {
+          const int t = (i * 32 + lane) * X::COUNT + j;
+          const unsigned n = t < V ? atomicAdd(&s_count[w], 1u) : BEAM_LIST;
+          if (n < BEAM_LIST) s_list[w][n] = make_uint2(order_key(x[j]), base + t);
+        }
+  }
+  float even, odd;
+  unpair(sums, even, odd);
+  sum += even + odd;
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-  if (lane == 0) s_sum[w] = make_float2(top, sum);
-  __syncthreads();
-  if (w) return;
-  for (int i = 1; i < BEAM_WARPS; ++i)
+  if (lane == 0) a.sums[part] = make_float2(m, sum);
+  __syncwarp();
+  const int count = static_cast<int>(s_count[w]);
+  uint2* out = a.lists + part * K;
+  if (count <= 32) keep_best<1>(s_list[w], count, out, K);
+  else if (count <= BEAM_LIST) keep_best<BEAM_LIST / 32>(s_list[w], count, out, K);
+  else {
+    // K times the best behind the one before
+    uint2 last = make_uint2(0xffffffffu, 0u);
     for (int e = 0; e < K; ++e) {
-      const uint32_t k = s_key[i][e], k_worst = __shfl_sync(0xffffffffu, best.key, K - 1);
-      const int t = s_token[i][e], t_worst = __shfl_sync(0xffffffffu, best.token, K - 1);
-      if (k == 0u || k < k_worst || (k == k_worst && t > t_worst)) break;
-      best.insert(k, t, lane);
+      uint32_t key[1] = {0u};
+      int token[1] = {0x7fffffff};
+      for (int i = 0; i < loads; ++i) {
+        const X x = at(i);
+#pragma unroll
+        for (int j = 0; j < X::COUNT; ++j) {
+          const uint32_t k = order_key(x[j]);
+          const int t = (i * 32 + lane) * X::COUNT + j;
+          const bool behind = e == 0 || k < last.x || (k == last.x && base + t > static_cast<int>(last.y));
+          if (t < V && behind && k > key[0]) { key[0] = k; token[0] = base + t; }      // t grows: the lowest of equal ones stays
+        }
+      }
+      last = take_best(key, token);
+      if (lane == 0) out[e] = last;
     }
-  const size_t o = (row_at * a.parts + blockIdx.y) * K;
-  if (lane < K) { a.keys[o + lane] = best.key; a.tokens[o + lane] = best.token; }
-  float2 s = lane < BEAM_WARPS ? s_sum[lane] : make_float2(-3.4028234663852886e38f, 0.f);
-  top = s.x;
-#pragma unroll
-  for (int d = 4; d > 0; d >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
-  sum = s.y * exp2f((s.x - top) * LOG2E);
-#pragma unroll
-  for (int d = 4; d > 0; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
-  if (lane == 0) a.sums[row_at * a.parts + blockIdx.y] = make_float2(top, sum);
+  }
 }
 
-// One block per prompt.  A warp per beam: the beam's sum, its parts' lists merged; then the beams' lists, K rounds, a lane per beam.
-__global__ void __launch_bounds__(32 * BEAM_WARPS) beam_select_kernel(const BeamArgs a) {
-  __shared__ double s_value[BEAM_MOST][BEAM_MOST];
+// 64-bit key with the order of the numbers, 0 below all of them.
+__device__ __forceinline__ unsigned long long order_key(double x) {
+  const unsigned long long b = static_cast<unsigned long long>(__double_as_longlong(x));
+  return b >> 63 ? ~b : b | 0x8000000000000000ull;
+}
+__device__ __forceinline__ double key_value(unsigned long long k) {
+  return __longlong_as_double(static_cast<long long>(k >> 63 ? k & 0x7fffffffffffffffull : ~k));
+}
+
+// A part's sum for the reference `top` of its row: the sum that was made is off by 2^(m L - rn(m L)), L the rounded log2(e).
+__device__ __forceinline__ double part_sum(float2 s, float top) {
+  const double off = fabsf(s.x) < BEAM_HUGE ? static_cast<double>(s.x) * static_cast<double>(LOG2E) - static_cast<double>(s.x * LOG2E) : 0.;
+  return static_cast<double>(s.y) * (1. - off * 0.6931471805599453) * static_cast<double>(exp2f((s.x - top) * LOG2E));
+}
+
+// One block per prompt.  A warp per beam: the beam's sum, its parts' lists; then the beams' lists, K rounds, a lane per beam.
+__global__ void __launch_bounds__(SELECT_THREADS) beam_select_kernel(const BeamArgs a) {
+  constexpr int AT_ONCE = 8;               // entries of a lane, beside one of the best so far
+  __shared__ unsigned long long s_value[BEAM_MOST][BEAM_MOST];      // order keys, 0: none
   __shared__ int s_token[BEAM_MOST][BEAM_MOST];
   pdl_launch_next();
   pdl_wait();
   const int lane = threadIdx.x & 31, w = threadIdx.x >> 5, K = a.K, V = a.V, b = blockIdx.x;
   const double none = -__longlong_as_double(0x7ff0000000000000ll);
-  for (int row = w; row < K; row += BEAM_WARPS) {
+  const long long entries = static_cast<long long>(a.parts) * K;
+  for (int row = w; row < K; row += SELECT_THREADS / 32) {
     const size_t at = static_cast<size_t>(b) * K + row;
-    const double score = a.scores[at] < -none ? a.scores[at] : none;      // no sum of logarithms of probabilities is +inf
+    const bool done = a.done && a.done[at];
+    const float given = a.scores[at];
+    uint2 first[AT_ONCE];
+    float2 s = make_float2(BEAM_LOWEST, 0.f);
+    if (!done) {                         // what most calls need, on its way together
+      if (lane < a.parts) s = a.sums[at * a.parts + lane];
+#pragma unroll
+      for (int i = 0; i < AT_ONCE; ++i)
+        first[i] = i * 32 + lane < entries ? a.lists[at * entries + i * 32 + lane] : make_uint2(0u, 0x7fffffffu);
+    }
+    const double score = given < -none ? given : none;      // no sum of logarithms of probabilities is +inf
     double value = none;
     int token = -1;                      // this lane's entry of the beam's list
-    if (a.done && a.done[at]) {
+    if (done) {
       if (score > none) {                // the end token, then the others in their order
         value = lane == 0 ? score : none;
         token = lane == 0 ? a.eos : lane - (lane <= a.eos);
       }
     } else {
-      float2 s = lane < a.parts ? a.sums[at * a.parts + lane] : make_float2(-3.4028234663852886e38f, 0.f);
       float top = s.x;
+      for (int i = 32 + lane; i < a.parts; i += 32) top = fmaxf(top, a.sums[at * a.parts + i].x);
 #pragma unroll
       for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-      double sum = static_cast<double>(s.y) * static_cast<double>(exp2f((s.x - top) * LOG2E));
+      double sum = part_sum(s, top);
+      for (int i = 32 + lane; i < a.parts; i += 32) {
+        s = a.sums[at * a.parts + i];
+        sum += part_sum(s, top);
+      }
 #pragma unroll
       for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
       const double log_sum = log(sum) + static_cast<double>(top);
-      BestList best;
-      if (lane < K) { best.key = a.keys[at * a.parts * K + lane]; best.token = a.tokens[at * a.parts * K + lane]; }
-      for (int p = 1; p < a.parts; ++p) {
-        // the part's list, an entry per lane; those that come in are its first ones
-        const uint32_t k = lane < K ? a.keys[(at * a.parts + p) * K + lane] : 0u;
-        const int t = lane < K ? a.tokens[(at * a.parts + p) * K + lane] : -1;
+      uint2 best = make_uint2(0u, 0x7fffffffu);
+      for (long long e0 = 0; e0 < entries; e0 += 32 * AT_ONCE) {
+        uint32_t key[AT_ONCE + 1] = {best.x};
+        int tokens[AT_ONCE + 1] = {static_cast<int>(best.y)};
+#pragma unroll
+        for (int i = 0; i < AT_ONCE; ++i) {
+          const long long e = e0 + i * 32 + lane;
+          if (e0) first[i] = e < entries ? a.lists[at * entries + e] : make_uint2(0u, 0x7fffffffu);
+          key[i + 1] = first[i].x; tokens[i + 1] = static_cast<int>(first[i].y);
+        }
         for (int e = 0; e < K; ++e) {
-          const uint32_t ke = __shfl_sync(0xffffffffu, k, e), k_worst = __shfl_sync(0xffffffffu, best.key, K - 1);
-          const int te = __shfl_sync(0xffffffffu, t, e), t_worst = __shfl_sync(0xffffffffu, best.token, K - 1);
-          if (ke == 0u || ke < k_worst || (ke == k_worst && te > t_worst)) break;
-          best.insert(ke, te, lane);
+          const uint2 x = take_best(key, tokens);
+          if (lane == e) best = x;
         }
       }
-      if (best.key) { value = score + (static_cast<double>(key_value(best.key)) - log_sum); token = best.token; }
+      if (best.x) { value = score + (static_cast<double>(key_value(best.x)) - log_sum); token = static_cast<int>(best.y); }
       if (!(value == value)) value = none;
     }
     if (__shfl_sync(0xffffffffu, value, 0) == none) token = lane;      // nothing of this beam counts: its first tokens
-    if (token >= V) token = -1;
-    if (lane < K) { s_value[row][lane] = value; s_token[row][lane] = token; }
+    if (lane < K) { s_value[row][lane] = token >= 0 && token < V ? order_key(value) : 0ull; s_token[row][lane] = token; }
   }
   __syncthreads();
   if (w) return;
   int at = 0;                            // of this lane's beam
+  unsigned long long mine = lane < K ? s_value[lane][0] : 0ull;
   for (int i = 0; i < K; ++i) {
-    const bool left = lane < K && at < K && s_token[lane][at] >= 0;
-    double value = left ? s_value[lane][at] : none;
     // the best value, then the lowest beam: within a beam the list has the order of the tokens
-    unsigned candidates = __ballot_sync(0xffffffffu, left);
-    double top = value;
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) { const double v = __shfl_xor_sync(0xffffffffu, top, o); top = v > top ? v : top; }
-    candidates &= __ballot_sync(0xffffffffu, left && value == top);
-    const int row = __ffs(candidates) - 1;
+    const uint32_t hi = static_cast<uint32_t>(mine >> 32), lo = static_cast<uint32_t>(mine);
+    const uint32_t top_hi = __reduce_max_sync(0xffffffffu, hi), top_lo = __reduce_max_sync(0xffffffffu, hi == top_hi ? lo : 0u);
+    const int row = __ffs(__ballot_sync(0xffffffffu, hi == top_hi && lo == top_lo)) - 1;
     if (lane == row) {
       const size_t o = static_cast<size_t>(b) * K + i;
       const int token = s_token[lane][at];
-      a.out_scores[o] = static_cast<float>(value);
+      a.out_scores[o] = static_cast<float>(key_value(mine));
       a.out_tokens[o] = token;
       a.out_parents[o] = lane;
       if (a.done) a.out_done[o] = a.done[static_cast<size_t>(b) * K + lane] || token == a.eos;
       ++at;
+      mine = at < K ? s_value[lane][at] : 0ull;
     }
   }
 }
 
-static int beam_parts(int rows, int V) {
-  // enough blocks for every SM to have a few, of at least a step per warp
-  const int most = (V + BEAM_WARPS * 256 - 1) / (BEAM_WARPS * 256);
-  int parts = (4 * sm_count_current() + rows - 1) / rows;
-  if (parts > BEAM_PARTS) parts = BEAM_PARTS;
-  return parts < most ? parts : most;
-}
+static int beam_parts(int V, int size) { return static_cast<int>((static_cast<long long>(V) * size + BEAM_PART - 1) / BEAM_PART); }
 
 }  // namespace axb
 
 using namespace axb;
 
 // 32-bit words of the workspace: two per row and part, then two per entry of their lists
-extern "C" long long axb_beam_select_words(int B, int K, int V) {
-  return 2ll * B * K * beam_parts(B * K, V) * (1 + K);
+extern "C" long long axb_beam_select_words(int B, int K, int V, int dtype) {
+  return 2ll * B * K * beam_parts(V, dtype == 2 ? 4 : 2) * (1 + K);
 }
 
 extern "C" int axb_beam_select(const void* logits, const float* scores, const void* done, int eos, float* out_scores, long long* out_tokens,
@@ -269,20 +375,17 @@ extern "C" int axb_beam_select(const void* logits, const float* scores, const vo
   if (V > 1 << 30) { set_error("beam_select: a vocabulary of at most %d", 1 << 30); return -1; }
   if (dtype < 0 || dtype > 2) { set_error("beam_select: bf16, fp16 or fp32 logits"); return -1; }
   if (reinterpret_cast<uintptr_t>(work) & 7) { set_error("beam_select: the workspace must be 8-byte aligned"); return -1; }
-  const int rows = B * K, parts = beam_parts(rows, V), size = dtype == 2 ? 4 : 2;
-  const long long steps = (V + 256ll * BEAM_WARPS - 1) / (256ll * BEAM_WARPS);
-  BeamArgs a{logits, scores, (const unsigned char*)done, out_scores, out_tokens, out_parents, (unsigned char*)out_done};
-  const size_t lists = static_cast<size_t>(rows) * parts;
-  a.sums = (float2*)work;
-  a.keys = (uint32_t*)work + 2 * lists;
-  a.tokens = (int*)a.keys + lists * K;
-  a.B = B; a.K = K; a.V = V; a.eos = eos; a.parts = parts;
-  a.part_steps = static_cast<int>((steps + parts - 1) / parts);
+  const int size = dtype == 2 ? 4 : 2, parts = beam_parts(V, size);
+  const long long items = static_cast<long long>(B) * K * parts;
+  const BeamArgs a{logits, scores, (const unsigned char*)done, out_scores, out_tokens, out_parents, (unsigned char*)out_done,
+                   (float2*)work, (uint2*)work + items, K, V, eos, parts, items};
   const bool vec = (reinterpret_cast<uintptr_t>(logits) & 15) == 0 && static_cast<long long>(V) * size % 16 == 0;
   void (*kern)(BeamArgs) = dtype == 0 ? (vec ? beam_rows_kernel<__nv_bfloat16, true> : beam_rows_kernel<__nv_bfloat16, false>)
                            : dtype == 1 ? (vec ? beam_rows_kernel<__half, true> : beam_rows_kernel<__half, false>)
                                         : (vec ? beam_rows_kernel<float, true> : beam_rows_kernel<float, false>);
-  AXB_CUDA(pdl_launch(kern, dim3(rows, parts), dim3(32 * BEAM_WARPS), 0, (cudaStream_t)stream, a));
-  AXB_CUDA(pdl_launch(beam_select_kernel, dim3(B), dim3(32 * BEAM_WARPS), 0, (cudaStream_t)stream, a));
+  const long long blocks = (items + BEAM_WARPS - 1) / BEAM_WARPS;
+  if (blocks > 0x7fffffffll) { set_error("beam_select: too many logits in one call"); return -1; }
+  AXB_CUDA(pdl_launch(kern, dim3((unsigned)blocks), dim3(32 * BEAM_WARPS), 0, (cudaStream_t)stream, a));
+  AXB_CUDA(pdl_launch(beam_select_kernel, dim3(B), dim3(SELECT_THREADS), 0, (cudaStream_t)stream, a));
   return 0;
 }

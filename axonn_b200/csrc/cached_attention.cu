@@ -24,7 +24,7 @@
 namespace axb {
 
 constexpr int CA_TILE = 32;              // tokens of a tile: two halves of 16, the rows of an instruction
-constexpr int CA_WARPS = 4;
+constexpr int CA_WARPS = 8;
 constexpr int CA_STAGES = 2;             // tiles of a warp's ring
 constexpr int CA_MAX_ROWS = 1024;        // requests of one launch: their tiles are counted in shared memory
 constexpr int CA_LEAST_TILES = 4;        // of a block's run: shorter ones are not worth their partial sums
@@ -43,7 +43,7 @@ struct AttendArgs {
   int workers;                           // blocks of the grid
   int* before;                           // [R + 1] tiles of the requests before each
   float* part;                           // [2 * workers][columns][D + 4]: sums, then m, m', l
-  float* head;                           // the same of the first sequence of every warp: [workers * CA_WARPS][columns][D + 4]
+  float* head;                           // the same of the first sequence of every warp: [workers * warps][columns][D + 4]
 };
 
 // The block that has unit u, of `active` blocks that share `units`; block w starts at units * w / active.
@@ -62,12 +62,12 @@ __device__ __forceinline__ float exp2_fast(float x) {
   return y;
 }
 __device__ __forceinline__ void mma_f16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
-  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
                : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 __device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
   uint32_t y;
-  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
   return y;
 }
 __device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
@@ -94,9 +94,14 @@ __device__ __forceinline__ void copy16(uint32_t to, const void* from) {
 __device__ __forceinline__ void copy4(uint32_t to, const void* from) {
   asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(to), "l"(from) : "memory");
 }
-template <int WORDS> __device__ __forceinline__ void shared_words(uint32_t p, uint32_t* w) {
-  if constexpr (WORDS == 4) asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]) : "r"(p) : "memory");
-  else asm volatile("ld.shared.v2.b32 {%0, %1}, [%2];" : "=r"(w[0]), "=r"(w[1]) : "r"(p) : "memory");
+template <int WORDS> __device__ __forceinline__ void shared_words(const uint8_t* p, uint32_t* w) {
+  if constexpr (WORDS == 4) {
+    const uint4 u = *reinterpret_cast<const uint4*>(p);
+    w[0] = u.x; w[1] = u.y; w[2] = u.z; w[3] = u.w;
+  } else {
+    const uint2 u = *reinterpret_cast<const uint2*>(p);
+    w[0] = u.x; w[1] = u.y;
+  }
 }
 
 // A tile in shared memory: 32 rows of keys, 32 of values, then for each half ks, vs and whether the block exists.  The 16-byte words of
@@ -113,7 +118,7 @@ template <int D> struct Stage {
 };
 
 // Shared memory of a warp: its ring, which the partial sums of its last sequence take the place of.  (Those of its first one go to
-// global memory: the ring is in use then.)
+// global memory where others follow: the ring is in use then.)
 template <int D, int NT> __host__ __device__ constexpr int warp_bytes() {
   const int ring = CA_STAGES * Stage<D>::SIZE, parts = 8 * NT * (D + 4) * 4;
   return ring > parts ? ring : parts;
@@ -147,10 +152,11 @@ template <typename T, int N> __device__ __forceinline__ void write_row(T* out, c
 struct Open { int r, item, from_first, to_last; };      // item < 0: none
 
 template <typename T, int D, bool INT8, int NT>
-__global__ void __launch_bounds__(32 * CA_WARPS, NT == 1 ? 3 : 2) attend_kernel(const AttendArgs a) {
+__global__ void __launch_bounds__(32 * CA_WARPS, 1) attend_kernel(const AttendArgs a) {
   constexpr int KC = D / 64, MT = D / 16, VW = D / 32, COLS = 8 * NT;
-  extern __shared__ __align__(16) uint8_t ring[];      // of every warp; then the tiles of the requests before each, [R + 1]
+  extern __shared__ __align__(16) uint8_t ring[];      // of every warp; then the tiles of the requests before each, [R + 1], and lengths
   int* before = reinterpret_cast<int*>(ring + CA_WARPS * warp_bytes<D, NT>());
+  int* lengths = before + a.R + 1;
   __shared__ int sums[CA_WARPS];
   __shared__ Open open[CA_WARPS][2];         // the sequences that a warp has not seen whole: its first and its last
   pdl_launch_next();
@@ -162,7 +168,10 @@ __global__ void __launch_bounds__(32 * CA_WARPS, NT == 1 ? 3 : 2) attend_kernel(
   {
     const int per = (a.R + 32 * CA_WARPS - 1) / (32 * CA_WARPS), r0 = tid * per;
     int mine = 0;
-    for (int r = r0; r < min(r0 + per, a.R); ++r) mine += (min(max(a.lengths[r], 0), most) + CA_TILE - 1) / CA_TILE;
+    for (int r = r0; r < min(r0 + per, a.R); ++r) {
+      lengths[r] = min(max(a.lengths[r], 0), most);
+      mine += (lengths[r] + CA_TILE - 1) / CA_TILE;
+    }
     int incl = mine;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) { const int u = __shfl_up_sync(0xffffffffu, incl, o); if (lane >= o) incl += u; }
@@ -173,7 +182,7 @@ __global__ void __launch_bounds__(32 * CA_WARPS, NT == 1 ? 3 : 2) attend_kernel(
     for (int r = r0; r < min(r0 + per, a.R); ++r) {
       before[r] = at;
       if (blockIdx.x == 0) a.before[r] = at;
-      at += (min(max(a.lengths[r], 0), most) + CA_TILE - 1) / CA_TILE;
+      at += (lengths[r] + CA_TILE - 1) / CA_TILE;
     }
     if (r0 < a.R && r0 + per >= a.R) { before[a.R] = at; if (blockIdx.x == 0) a.before[a.R] = at; }
     __syncthreads();
@@ -195,9 +204,42 @@ __global__ void __launch_bounds__(32 * CA_WARPS, NT == 1 ? 3 : 2) attend_kernel(
     const long long within = u - static_cast<long long>(before[r]) * per_tile;
     const int item = static_cast<int>(within / tiles), g = item / a.groups, group = item % a.groups;
     const int t0 = static_cast<int>(within % tiles), t1 = static_cast<int>(min(static_cast<long long>(tiles), t0 + (end - u)));
-    const int length = min(max(a.lengths[r], 0), most), fresh = a.fresh ? min(max(a.fresh[r], 0), a.S) : a.S;
+    const int length = lengths[r], fresh = a.fresh ? min(max(a.fresh[r], 0), a.S) : a.S;
     const int col0 = group * COLS, cols = min(a.S * a.P - col0, COLS);
 
+    // the ids of 32 blocks, one per lane, ahead of their use
+    const int* table = a.tables + static_cast<size_t>(r) * a.W;
+    const int halves = (length + 15) / 16, down_shift = a.shift - 4;      // halves of tiles to blocks
+    int id_base = 2 * t0 >> down_shift;
+    int ids = id_base + lane < a.W ? table[id_base + lane] : -1;
+    uint8_t* mine = ring + wid * warp_bytes<D, NT>();
+    auto fetch = [&](int t, int stage) {
+      if (t < t1) {
+        const uint32_t to = smem_u32(mine) + stage * Stage<D>::SIZE;
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const int half = 2 * t + h, b = half >> down_shift;
+          if (b - id_base == 32) { id_base = b; ids = b + lane < a.W ? table[b + lane] : -1; }
+          const int id = __shfl_sync(0xffffffffu, ids, b - id_base);
+          const bool there = half < halves && id >= 0 && id < a.N;
+          if (lane == 0) asm volatile("st.shared.b32 [%0], %1;" ::"r"(to + 2 * Stage<D>::BYTES + 16 * h + 8), "r"(static_cast<int>(there)) : "memory");
+          if (!there) continue;
+          const size_t head = static_cast<size_t>(id) * a.G + g;
+          if (lane < 2) copy4(to + 2 * Stage<D>::BYTES + 16 * h + 4 * lane, (lane ? a.vs : a.ks) + head);
+          const size_t from = ((head << a.shift) + ((half * 16) & (BT - 1))) * D;
+#pragma unroll
+          for (int x = 0; x < D / 32; ++x) {
+            const int i = x * 32 + lane, row = 16 * h + i / (D / 16), c = i % (D / 16);
+            copy16(to + Stage<D>::key_word(row, c) * 16, a.k + from + i * 16);
+            copy16(to + Stage<D>::BYTES + Stage<D>::value_word(row, c) * 16, a.v + from + i * 16);
+          }
+        }
+      }
+      asm volatile("cp.async.commit_group;" ::: "memory");
+    };
+
+    __syncwarp();                            // the ring's last tile of the sequence before has been read
+    for (int i = 0; i < CA_STAGES - 1; ++i) fetch(t0 + i, i);
     // queries as the B operand of the scores, scaled into fp16; what their columns see
     uint32_t qf[NT][D / 16][2];
     float cscale[NT][2];
@@ -261,46 +303,12 @@ __global__ void __launch_bounds__(32 * CA_WARPS, NT == 1 ? 3 : 2) attend_kernel(
       l[n][0] = l[n][1] = 0.f;
     }
 
-    // the ids of 32 blocks, one per lane, ahead of their use
-    const int* table = a.tables + static_cast<size_t>(r) * a.W;
-    const int halves = (length + 15) / 16, down_shift = a.shift - 4;      // halves of tiles to blocks
-    int id_base = 2 * t0 >> down_shift;
-    int ids = id_base + lane < a.W ? table[id_base + lane] : -1;
-    const uint32_t mine = smem_u32(ring) + wid * warp_bytes<D, NT>();
-    auto fetch = [&](int t, int stage) {
-      if (t < t1) {
-        const uint32_t to = mine + stage * Stage<D>::SIZE;
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          const int half = 2 * t + h, b = half >> down_shift;
-          if (b - id_base == 32) { id_base = b; ids = b + lane < a.W ? table[b + lane] : -1; }
-          const int id = __shfl_sync(0xffffffffu, ids, b - id_base);
-          const bool there = half < halves && id >= 0 && id < a.N;
-          if (lane == 0) asm volatile("st.shared.b32 [%0], %1;" ::"r"(to + 2 * Stage<D>::BYTES + 16 * h + 8), "r"(static_cast<int>(there)) : "memory");
-          if (!there) continue;
-          const size_t head = static_cast<size_t>(id) * a.G + g;
-          if (lane < 2) copy4(to + 2 * Stage<D>::BYTES + 16 * h + 4 * lane, (lane ? a.vs : a.ks) + head);
-          const size_t from = ((head << a.shift) + ((half * 16) & (BT - 1))) * D;
-#pragma unroll
-          for (int x = 0; x < D / 32; ++x) {
-            const int i = x * 32 + lane, row = 16 * h + i / (D / 16), c = i % (D / 16);
-            copy16(to + Stage<D>::key_word(row, c) * 16, a.k + from + i * 16);
-            copy16(to + Stage<D>::BYTES + Stage<D>::value_word(row, c) * 16, a.v + from + i * 16);
-          }
-        }
-      }
-      asm volatile("cp.async.commit_group;" ::: "memory");
-    };
-
-    __syncwarp();                            // the ring's last tile of the sequence before has been read
-    for (int i = 0; i < CA_STAGES - 1; ++i) fetch(t0 + i, i);
     int stage = 0;
     for (int t = t0; t < t1; ++t) {
-      __syncwarp();                          // the tile before has been read
+      asm volatile("cp.async.wait_group %0;" ::"n"(CA_STAGES - 2) : "memory");
+      __syncwarp();                          // everyone's part of this tile is there, and the tile before has been read
       fetch(t + CA_STAGES - 1, stage == 0 ? CA_STAGES - 1 : stage - 1);
-      asm volatile("cp.async.wait_group %0;" ::"n"(CA_STAGES - 1) : "memory");
-      __syncwarp();                          // everyone's part of this tile is there
-      const uint32_t at = mine + stage * Stage<D>::SIZE;
+      const uint8_t* at = mine + stage * Stage<D>::SIZE;
       stage = stage == CA_STAGES - 1 ? 0 : stage + 1;
       float ks[2], vs[2];
       bool there[2];
@@ -325,14 +333,19 @@ __global__ void __launch_bounds__(32 * CA_WARPS, NT == 1 ? 3 : 2) attend_kernel(
         }
 #pragma unroll
         for (int n = 0; n < NT; ++n) s[h][n][0] = s[h][n][1] = s[h][n][2] = s[h][n][3] = 0.f;
+        float odd[NT][4] = {};             // two chains of dependent products
 #pragma unroll
         for (int i = 0; i < D / 16; ++i) {
           uint32_t a0, a1, a2, a3;
           widen<INT8>(k[0][i], a0, a2);
           widen<INT8>(k[1][i], a1, a3);
 #pragma unroll
-          for (int n = 0; n < NT; ++n) mma_f16(s[h][n], a0, a1, a2, a3, qf[n][i][0], qf[n][i][1]);
+          for (int n = 0; n < NT; ++n) mma_f16(i & 1 ? odd[n] : s[h][n], a0, a1, a2, a3, qf[n][i][0], qf[n][i][1]);
         }
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) s[h][n][i] += odd[n][i];
       }
       // vs = 2^ev fv, 1 <= fv < 2
       float ev[2], fv[2];
@@ -456,7 +469,7 @@ __global__ void __launch_bounds__(32 * CA_WARPS, NT == 1 ? 3 : 2) attend_kernel(
 
     // thread (g8, j4) has values g8 * D / 8 .. of columns 2 j4 and 2 j4 + 1
     const bool whole = t0 == 0 && t1 == tiles;
-    const int slot = u == begin ? 0 : 1;
+    const int slot = u + (t1 - t0) < end ? 0 : 1;      // the last of this warp's, or its first of several
     if (!whole) {
       __syncwarp();                          // the ring has been read: the sums take its place
       if (lane == 0) open[wid][slot] = Open{r, item, t0 == 0, t1 == tiles};
@@ -603,10 +616,29 @@ __global__ void __launch_bounds__(32 * MERGE_WARPS) attend_merge_kernel(const At
 }
 
 static int attend_columns(int queries) { return queries <= 8 ? 8 : 16; }
-#ifndef CA_WAVES
-#define CA_WAVES 1
-#endif
-static int attend_blocks(int columns) { return sm_count_current() * (columns == 8 ? 3 : 2) * CA_WAVES; }
+
+template <typename T, int D, bool INT8, int NT>
+static int launch_attend(const AttendArgs& a, cudaStream_t stream) {
+  constexpr size_t ring = CA_WARPS * warp_bytes<D, NT>(), most = ring + (2 * CA_MAX_ROWS + 1) * sizeof(int);
+  static bool configured[64] = {false};
+  auto kern = attend_kernel<T, D, INT8, NT>;
+  int device = 0;
+  AXB_CUDA(cudaGetDevice(&device));
+  if (!configured[device & 63]) {
+    AXB_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(most)));
+    configured[device & 63] = true;
+  }
+  AXB_CUDA(pdl_launch(kern, dim3(a.workers), dim3(32 * CA_WARPS), ring + (2 * a.R + 1) * sizeof(int), stream, a));
+  AXB_CUDA(pdl_launch(attend_merge_kernel<T, D>, dim3(a.R * a.G * a.groups), dim3(32 * MERGE_WARPS), 0, stream, a, 8 * NT));
+  return 0;
+}
+template <typename T> static int launch_attend(const AttendArgs& a, int D, bool int8, int columns, cudaStream_t stream) {
+  if (columns == 8)
+    return D == 64 ? (int8 ? launch_attend<T, 64, true, 1>(a, stream) : launch_attend<T, 64, false, 1>(a, stream))
+                   : (int8 ? launch_attend<T, 128, true, 1>(a, stream) : launch_attend<T, 128, false, 1>(a, stream));
+  return D == 64 ? (int8 ? launch_attend<T, 64, true, 2>(a, stream) : launch_attend<T, 64, false, 2>(a, stream))
+                 : (int8 ? launch_attend<T, 128, true, 2>(a, stream) : launch_attend<T, 128, false, 2>(a, stream));
+}
 
 }  // namespace axb
 
@@ -615,7 +647,7 @@ using namespace axb;
 // 32-bit words of the workspace: the tile counts, then two partial results per block
 extern "C" long long axb_cached_attention_words(int R, int S, int P, int D) {
   const int columns = attend_columns(S * P);
-  return (R + 1 + 3) / 4 * 4 + (2ll + CA_WARPS) * attend_blocks(columns) * columns * (D + 4);
+  return (R + 1 + 3) / 4 * 4 + (2ll + CA_WARPS) * sm_count_current() * columns * (D + 4);
 }
 
 extern "C" int axb_cached_attention(const void* q, long long q_row, long long q_token, long long q_group, const void* k, const void* v,
@@ -633,33 +665,21 @@ extern "C" int axb_cached_attention(const void* q, long long q_row, long long q_
     set_error("cached_attention: operands must be 16-byte aligned, strides multiples of 8 elements");
     return -1;
   }
-  const int columns = attend_columns(S * P), groups = (S * P + columns - 1) / columns, blocks = attend_blocks(columns);
+  const int columns = attend_columns(S * P), groups = (S * P + columns - 1) / columns, blocks = sm_count_current();
   AttendArgs a{q, q_row, q_token, q_group, out, (const uint8_t*)k, (const uint8_t*)v, ks, vs, tables, lengths, fresh, R, S, G, P, W, N, shift,
                groups, scale * 1.4426950408889634f, blocks, (int*)work, nullptr, nullptr};
-  void (*kern)(AttendArgs) = nullptr;
-#define AXB_PICK(T, D_, NT) (int8 ? attend_kernel<T, D_, true, NT> : attend_kernel<T, D_, false, NT>)
-#define AXB_PICK_D(T, NT) (D == 64 ? AXB_PICK(T, 64, NT) : AXB_PICK(T, 128, NT))
-  if (columns == 8) kern = dtype == 0 ? AXB_PICK_D(__nv_bfloat16, 1) : AXB_PICK_D(__half, 1);
-  else kern = dtype == 0 ? AXB_PICK_D(__nv_bfloat16, 2) : AXB_PICK_D(__half, 2);
-#undef AXB_PICK_D
-#undef AXB_PICK
-  void (*merge)(AttendArgs, int) = dtype == 0 ? (D == 64 ? attend_merge_kernel<__nv_bfloat16, 64> : attend_merge_kernel<__nv_bfloat16, 128>)
-                                              : (D == 64 ? attend_merge_kernel<__half, 64> : attend_merge_kernel<__half, 128>);
-  const int size = 2, rows_at_once = CA_MAX_ROWS;
-  for (int r0 = 0; r0 < R; r0 += rows_at_once) {
-    a.R = R - r0 < rows_at_once ? R - r0 : rows_at_once;
-    a.q = static_cast<const char*>(q) + r0 * q_row * size;
-    a.out = static_cast<char*>(out) + static_cast<size_t>(r0) * S * G * P * D * size;
+  for (int r0 = 0; r0 < R; r0 += CA_MAX_ROWS) {
+    a.R = R - r0 < CA_MAX_ROWS ? R - r0 : CA_MAX_ROWS;
+    a.q = static_cast<const char*>(q) + r0 * q_row * 2;
+    a.out = static_cast<char*>(out) + static_cast<size_t>(r0) * S * G * P * D * 2;
     a.tables = tables + static_cast<size_t>(r0) * W;
     a.lengths = lengths + r0;
     a.fresh = fresh ? fresh + r0 : nullptr;
     a.part = reinterpret_cast<float*>(a.before + (a.R + 1 + 3) / 4 * 4);
     a.head = a.part + 2ll * blocks * columns * (D + 4);
-    const int per_warp = columns == 8 ? (D == 64 ? warp_bytes<64, 1>() : warp_bytes<128, 1>()) : (D == 64 ? warp_bytes<64, 2>() : warp_bytes<128, 2>());
-    const size_t shared = CA_WARPS * per_warp + (a.R + 1) * sizeof(int);
-    AXB_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(shared)));
-    AXB_CUDA(pdl_launch(kern, dim3(blocks), dim3(32 * CA_WARPS), shared, (cudaStream_t)stream, a));
-    AXB_CUDA(pdl_launch(merge, dim3(a.R * G * groups), dim3(32 * MERGE_WARPS), 0, (cudaStream_t)stream, a, columns));
+    const int st = dtype == 0 ? launch_attend<__nv_bfloat16>(a, D, int8 != 0, columns, (cudaStream_t)stream)
+                              : launch_attend<__half>(a, D, int8 != 0, columns, (cudaStream_t)stream);
+    if (st) return st;
   }
   return 0;
 }

@@ -86,7 +86,7 @@ _SIGNATURES = {
     "axb_reorder_blocks": "pppp" "pppp" "ppp" "iiiiiiii" "p",
     "axb_cached_attention_words": "iiii",
     "axb_cached_attention": "p" "lll" "pppp" "ppp" "pp" "iiiiiiii" "f" "ii" "p",
-    "axb_beam_select_words": "iii",
+    "axb_beam_select_words": "iiii",
     "axb_beam_select": "ppp" "i" "ppppp" "iiii" "p",
 }
 # Switches of kernels that are gone.  The one kernel that is left covers what they selected; a program that still sets

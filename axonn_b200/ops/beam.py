@@ -57,7 +57,7 @@ def beam_select(logits, scores, done=None, eos_id=None):
     out = BeamStep(torch.empty_like(scores), torch.empty(B, K, dtype=torch.int64, device=dev), torch.empty(B, K, dtype=torch.int32, device=dev),
                    None if done is None else torch.empty_like(done))
     L = _lib.lib()
-    work = torch.empty(L.axb_beam_select_words(B, K, V), dtype=torch.int32, device=dev)
+    work = torch.empty(L.axb_beam_select_words(B, K, V, _DT[logits.dtype]), dtype=torch.int32, device=dev)
     st = L.axb_beam_select(logits.data_ptr(), scores.data_ptr(), _lib.addr(done), -1 if done is None else eos_id, out.scores.data_ptr(),
                            out.tokens.data_ptr(), out.parents.data_ptr(), _lib.addr(out.done), work.data_ptr(), B, K, V, _DT[logits.dtype],
                            _lib.stream())

@@ -111,3 +111,15 @@ def test_select_in_graphs_on_two_streams():
                 graph.replay()
     torch.cuda.synchronize()
     assert all(torch.equal(a, b) for o, w in zip(outs, want) for a, b in zip(o[:3], w[:3]))
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+def test_rows_masked_by_the_lowest_value(dtype):
+    """Banned tokens as the type's lowest value or -inf, all of a row or of a part of it, in the first parts and the last."""
+    low = torch.finfo(dtype).min
+    logits = (torch.randn(2, 4, 20000, generator=torch.Generator().manual_seed(0)) * 2).to(dtype)
+    logits[0, 0], logits[0, 1, :9000], logits[0, 2, 9000:], logits[0, 3, 1:] = low, low, low, low
+    logits[1, 0], logits[1, 1, :9000], logits[1, 2, 9000:], logits[1, 3, 1:] = float("-inf"), float("-inf"), float("-inf"), float("-inf")
+    _same(logits, torch.tensor([[0.0, -1.0, -2.0, -3.0]] * 2))
+    _same(logits[:, :1].contiguous(), torch.zeros(2, 1))
+    _same(logits[:1, :1].repeat(1, 32, 1).contiguous(), -torch.rand(1, 32, generator=torch.Generator().manual_seed(1)))
