@@ -1,13 +1,14 @@
 // Selection of beam search: of all continuations of the beams of a prompt, value = score + logit - log sum exp(logits of the beam), the
 // `beams` best, equal values in the order of (beam, token).
 //
-// Bound by reading the logits once.  A first launch cuts every beam's row into parts of 8 KB, each of which a warp copies into shared
-// memory and goes over twice: no block ever waits for its warps, and the loops are short (the same code for 8 KB in registers is five
-// times as long, and was waited for longer than the data).  The K-th largest of the lanes' maxima is reached by at least K values of the part and by few others,
-// which go into a list in shared memory, of which the K best are kept.  (Where too many values reach the bound - rows of equal values -
-// the K best are found one by one.)  The order within a beam is that of its logits, so that nothing has to be known of the sum.  A second
-// launch puts the parts of a beam together and merges the beams.  Sums and values there are 64-bit: the order of two beams' tokens
-// depends on differences of their sums' logarithms that 32-bit values of twenty or so round away.
+// Bound by reading the logits once.  A first launch cuts every beam's row into runs of chunks of 4 KB.  A warp copies the chunks of its run
+// into shared memory, one ahead, and goes over each twice: no block ever waits for its warps, and the loops are short (the same code for
+// values in registers is five times as long, and was waited for longer than the data).  The K-th largest of the lanes' maxima is reached
+// by at least K values of the chunk and by few others; what reaches the largest such bound so far goes into a list, of which the K best
+// are kept in the end.  (Where too many values reach the bounds - rows of equal values - the K best are found one by one.)  The order
+// within a beam is that of its logits, so that nothing has to be known of the sum.  A second launch puts the runs of a beam together and
+// merges the beams.  Sums and values there are 64-bit: the order of two beams' tokens depends on differences of their sums' logarithms
+// that 32-bit values of twenty or so round away.
 //
 // A value that is not a number counts as -inf, and so do a score of +inf and every value of a beam whose sum is none.  Of a beam that has
 // ended only the end token goes on, with the beam's score.
@@ -19,9 +20,10 @@ namespace axb {
 
 constexpr int BEAM_MOST = 32;            // beams
 constexpr int BEAM_WARPS = 4;            // of a block of the first launch
-constexpr int BEAM_LOADS = 16;           // 16-byte words of a lane
-constexpr int BEAM_PART = 32 * BEAM_LOADS * 16;      // bytes of a part
-constexpr int BEAM_LIST = 64;            // values that reach the bound, at most
+constexpr int BEAM_LOADS = 8;            // 16-byte words of a lane, of a chunk
+constexpr int BEAM_CHUNK = 32 * BEAM_LOADS * 16;     // bytes
+constexpr int BEAM_LIST = 128;           // values of a run that reach the bounds, at most
+constexpr int BEAM_AT_ONCE = 32;         // runs per SM: 24 warps fit, beams that have ended leave room
 constexpr int SELECT_THREADS = 256;
 constexpr float BEAM_LOWEST = -3.4028234663852886e38f;
 constexpr float BEAM_HUGE = 1e38f;       // a maximum whose product with L is finite
@@ -35,11 +37,11 @@ struct BeamArgs {
   long long* out_tokens;
   int* out_parents;
   unsigned char* out_done;
-  // of every row and part: (maximum, sum), then K keys and tokens, best first
+  // of every row and run: (reference, sum), then K keys and tokens, best first
   float2* sums;
   uint2* lists;
-  int K, V, eos, parts;
-  long long items;                       // parts of all rows
+  int K, V, eos, parts, chunks;          // runs of a row, chunks of a run
+  long long items;                       // runs of all rows
 };
 
 // 32-bit key with the order of the numbers; 0 is below all of them.  -0 counts as 0.
@@ -112,6 +114,16 @@ template <typename T> struct Values {
     else if constexpr (__is_same(T, __nv_bfloat16)) return __hge2_mask(*reinterpret_cast<const __nv_bfloat162*>(&a), *reinterpret_cast<const __nv_bfloat162*>(&w));
     else return __hge2_mask(*reinterpret_cast<const __half2*>(&a), *reinterpret_cast<const __half2*>(&w));
   }
+  // bit j: value j reaches `w`'s
+  __device__ __forceinline__ uint32_t hits(uint32_t w) const {
+    if constexpr (PER_WORD == 1) {
+      return (reaching(word[0], w) & 1u) | (reaching(word[1], w) & 2u) | (reaching(word[2], w) & 4u) | (reaching(word[3], w) & 8u);
+    } else {
+      const uint32_t b = (reaching(word[0], w) & 0x00020001u) | (reaching(word[1], w) & 0x00080004u) | (reaching(word[2], w) & 0x00200010u) |
+                         (reaching(word[3], w) & 0x00800040u);
+      return (b | b >> 16) & 0xffu;
+    }
+  }
   static __device__ __forceinline__ uint32_t word_of(float x) {      // x is one of the type's numbers
     if constexpr (__is_same(T, float)) return __float_as_uint(x);
     else if constexpr (__is_same(T, __nv_bfloat16)) return (__float_as_uint(x) >> 16) * 0x10001u;
@@ -142,114 +154,144 @@ __device__ __forceinline__ unsigned long long add_pair(unsigned long long a, uns
   return d;
 }
 
-// VEC: every row starts on 16 bytes.
+// One chunk into shared memory, of which the row has V values from `from` on; VEC: every row starts on 16 bytes.  Whole words are
+// copied, the last ones of a row and rows off 16 bytes value by value; what is not there is -inf.
+template <typename T, bool VEC> __device__ __forceinline__ void copy_chunk(uint4* to, const T* from, int V) {
+  constexpr int COUNT = 16 / sizeof(T), CHUNK = BEAM_CHUNK / sizeof(T);
+  const int lane = threadIdx.x & 31, whole = VEC ? min(V, CHUNK) / COUNT : 0;
+#pragma unroll
+  for (int i = 0; i < BEAM_LOADS; ++i)
+    if (i * 32 + lane < whole)
+      asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(to + i * 32 + lane)), "l"(from + (i * 32 + lane) * COUNT) : "memory");
+  using Bits = std::conditional_t<sizeof(T) == 4, uint32_t, uint16_t>;
+  constexpr Bits lowest = static_cast<Bits>(__is_same(T, float) ? 0xff800000u : __is_same(T, __half) ? 0xfc00u : 0xff80u);
+#pragma unroll 8
+  for (int t = whole * COUNT + lane; t < CHUNK; t += 32) reinterpret_cast<Bits*>(to)[t] = t < V ? reinterpret_cast<const Bits*>(from)[t] : lowest;
+}
+
 template <typename T, bool VEC>
 __global__ void __launch_bounds__(32 * BEAM_WARPS) beam_rows_kernel(const BeamArgs a) {
   using X = Values<T>;
-  constexpr int PART = BEAM_PART / sizeof(T);
-  __shared__ uint4 s_part[BEAM_WARPS][BEAM_LOADS * 32];
+  constexpr int CHUNK = BEAM_CHUNK / sizeof(T);
+  __shared__ uint4 s_chunk[BEAM_WARPS][2][BEAM_LOADS * 32];
   __shared__ uint2 s_list[BEAM_WARPS][BEAM_LIST];
   __shared__ unsigned s_count[BEAM_WARPS];
   pdl_launch_next();
   pdl_wait();
   const int lane = threadIdx.x & 31, w = threadIdx.x >> 5, K = a.K;
-  const long long part = static_cast<long long>(blockIdx.x) * BEAM_WARPS + w;
-  if (part >= a.items) return;
-  const int row = static_cast<int>(part / a.parts), base = static_cast<int>(part - static_cast<long long>(row) * a.parts) * PART, V = a.V - base;
+  const long long run = static_cast<long long>(blockIdx.x) * BEAM_WARPS + w;
+  if (run >= a.items) return;
+  const int row = static_cast<int>(run / a.parts), first = static_cast<int>(run - static_cast<long long>(row) * a.parts) * a.chunks;
   if (a.done && a.done[row]) return;
-  const T* from = static_cast<const T*>(a.logits) + static_cast<long long>(row) * a.V + base;
-  uint4* words = s_part[w];
-  // 16 bytes of the warp's part; whole words are copied, the last ones of a row and rows off 16 bytes value by value, and what is not
-  // there is -inf
-  const int loads = (min(V, PART) * static_cast<int>(sizeof(T)) + 511) / 512;
-  const int whole = VEC ? min(V, PART) / X::COUNT : 0;
-  for (int i = 0; i < loads; ++i)
-    if (i * 32 + lane < whole)
-      asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(words + i * 32 + lane)), "l"(from + (i * 32 + lane) * X::COUNT) : "memory");
-  {
-    using Bits = std::conditional_t<sizeof(T) == 4, uint32_t, uint16_t>;
-    constexpr Bits lowest = static_cast<Bits>(__is_same(T, float) ? 0xff800000u : __is_same(T, __half) ? 0xfc00u : 0xff80u);
-    Bits* to = reinterpret_cast<Bits*>(words);
-#pragma unroll 8
-    for (int t = whole * X::COUNT + lane; t < loads * 32 * X::COUNT; t += 32) to[t] = t < V ? reinterpret_cast<const Bits*>(from)[t] : lowest;
-  }
-  if (lane == 0) s_count[w] = 0u;
-  asm volatile("cp.async.wait_all;" ::: "memory");
-  __syncwarp();
-  auto at = [&](int i) {
-    const uint4 u = words[i * 32 + lane];
-    return X{{u.x, u.y, u.z, u.w}};
+  const int last = min(first + a.chunks, (a.V + CHUNK - 1) / CHUNK);
+  const T* values = static_cast<const T*>(a.logits) + static_cast<long long>(row) * a.V;
+  auto copy = [&](int chunk, int buffer) {
+    if (chunk < last) copy_chunk<T, VEC>(s_chunk[w][buffer], values + static_cast<long long>(chunk) * CHUNK, a.V - chunk * CHUNK);
+    asm volatile("cp.async.commit_group;" ::: "memory");
   };
-  uint32_t most = X::word_of(-INFINITY);
-#pragma unroll 4
-  for (int i = 0; i < loads; ++i) most = X::larger(most, at(i).largest());
-  // the K-th largest of the lanes' maxima (equal ones count once: a lower bound does as well)
-  uint32_t mine = order_key(X::largest_of(most));
-  const uint32_t largest = __reduce_max_sync(0xffffffffu, mine);
-  uint32_t bound = largest;
-  for (int e = 1; e < K; ++e) {
-    if (mine == bound) mine = 0u;
-    bound = __reduce_max_sync(0xffffffffu, mine);
-  }
-  const uint32_t reach = X::word_of(bound ? key_value(bound) : -INFINITY);      // as numbers
-  const float m = fmaxf(key_value(largest), BEAM_LOWEST);
-  const bool ordinary = fabsf(m) < BEAM_HUGE;
-  const unsigned long long scale = pair_of(LOG2E, LOG2E), shift = pair_of(-m * LOG2E, -m * LOG2E);
-  unsigned long long sums = 0ull;
-  float sum = 0.f;
-#pragma unroll 2
-  for (int i = 0; i < loads; ++i) {
-    const X x = at(i);
+  if (lane == 0) s_count[w] = 0u;
+  copy(first, 0);
+  float m = BEAM_LOWEST, sum = 0.f;          // the reference, raised only where a value exceeds it by far: few roundings of the sum
+  uint32_t bound = 0u;
+  for (int chunk = first, buffer = 0; chunk < last; ++chunk, buffer ^= 1) {
+    __syncwarp();                            // the other buffer has been read
+    copy(chunk + 1, buffer ^ 1);
+    asm volatile("cp.async.wait_group 1;" ::: "memory");
+    __syncwarp();
+    const uint4* words = s_chunk[w][buffer] + lane;
+    auto at = [&](int i) {
+      const uint4 u = words[i * 32];
+      return X{{u.x, u.y, u.z, u.w}};
+    };
+    uint32_t most = at(0).largest();
+#pragma unroll
+    for (int i = 1; i < BEAM_LOADS; ++i) most = X::larger(most, at(i).largest());
+    // the K-th largest of the lanes' maxima (equal ones count once: a lower bound does as well)
+    uint32_t mine = order_key(X::largest_of(most));
+    const uint32_t largest = __reduce_max_sync(0xffffffffu, mine);
+    uint32_t kth = largest;
+    for (int e = 1; e < K; ++e) {
+      if (mine == kth) mine = 0u;
+      kth = __reduce_max_sync(0xffffffffu, mine);
+    }
+    bound = max(bound, kth);
+    const float top = fmaxf(key_value(largest), BEAM_LOWEST);
+    if (top > m + 8.f || chunk == first) {
+      sum *= fabsf(m) < BEAM_HUGE && fabsf(top) < BEAM_HUGE ? exp2f(m * LOG2E - top * LOG2E) : exp2f((m - top) * LOG2E);
+      m = top;
+    }
+    const bool ordinary = fabsf(m) < BEAM_HUGE;
+    const unsigned long long scale = pair_of(LOG2E, LOG2E), shift = pair_of(-m * LOG2E, -m * LOG2E);
+    const uint32_t reach = X::word_of(bound ? key_value(bound) : -INFINITY);      // as numbers
+    const int base = chunk * CHUNK;
+    uint64_t hits = 0ull;                    // a bit for every value of the lane's that reaches the bound
     if (ordinary) {
       // exp(x - m) as exp2(x L - m L), two at a time: the rounding of m L is put right where the sums are used
+      unsigned long long sums[2] = {0ull, 0ull};
+#pragma unroll 4
+      for (int i = 0; i < BEAM_LOADS; ++i) {
+        const X x = at(i);
+        hits |= static_cast<uint64_t>(x.hits(reach)) << (i * X::COUNT);
 #pragma unroll
-      for (int j = 0; j < X::COUNT; j += 2) {
-        float u, v;
-        unpair(fma_pair(pair_of(x[j], x[j + 1]), scale, shift), u, v);
-        sums = add_pair(sums, pair_of(exp2f(u), exp2f(v)));
-      }
-    } else {
-#pragma unroll
-      for (int j = 0; j < X::COUNT; ++j) sum += exp2f((x[j] - m) * LOG2E);
-    }
-    if (X::reaching(x.largest(), reach))
-#pragma unroll
-      for (int j = 0; j < X::COUNT; ++j)
-        if (X::reaching(x.word[j / X::PER_WORD], reach) >> (16 * (j % X::PER_WORD)) & 1u) {
-          const int t = (i * 32 + lane) * X::COUNT + j;
-          const unsigned n = t < V ? atomicAdd(&s_count[w], 1u) : BEAM_LIST;
-          if (n < BEAM_LIST) s_list[w][n] = make_uint2(order_key(x[j]), base + t);
+        for (int j = 0; j < X::COUNT; j += 2) {
+          float u, v;
+          unpair(fma_pair(pair_of(x[j], x[j + 1]), scale, shift), u, v);
+          sums[j / 2 & 1] = add_pair(sums[j / 2 & 1], pair_of(exp2f(u), exp2f(v)));
         }
+      }
+      float even, odd;
+      unpair(add_pair(sums[0], sums[1]), even, odd);
+      sum += even + odd;
+    } else {
+      for (int i = 0; i < BEAM_LOADS; ++i) {
+        const X x = at(i);
+        hits |= static_cast<uint64_t>(x.hits(reach)) << (i * X::COUNT);
+#pragma unroll
+        for (int j = 0; j < X::COUNT; ++j) sum += exp2f((x[j] - m) * LOG2E);
+      }
+    }
+    while (hits) {
+      const int i = __ffsll(static_cast<long long>(hits)) - 1, t = base + (i / X::COUNT * 32 + lane) * X::COUNT + i % X::COUNT;
+      hits &= hits - 1;
+      const unsigned n = t < a.V ? atomicAdd(&s_count[w], 1u) : BEAM_LIST;
+      if (n < BEAM_LIST) s_list[w][n] = make_uint2(order_key(static_cast<float>(reinterpret_cast<const T*>(words + i / X::COUNT * 32)[i % X::COUNT])), t);
+    }
   }
-  float even, odd;
-  unpair(sums, even, odd);
-  sum += even + odd;
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-  if (lane == 0) a.sums[part] = make_float2(m, sum);
+  if (lane == 0) a.sums[run] = make_float2(m, sum);
   __syncwarp();
   const int count = static_cast<int>(s_count[w]);
-  uint2* out = a.lists + part * K;
+  uint2* out = a.lists + run * K;
   if (count <= 32) keep_best<1>(s_list[w], count, out, K);
   else if (count <= BEAM_LIST) keep_best<BEAM_LIST / 32>(s_list[w], count, out, K);
   else {
     // K times the best behind the one before
-    uint2 last = make_uint2(0xffffffffu, 0u);
+    uint2 before = make_uint2(0xffffffffu, 0u);
     for (int e = 0; e < K; ++e) {
       uint32_t key[1] = {0u};
       int token[1] = {0x7fffffff};
-      for (int i = 0; i < loads; ++i) {
-        const X x = at(i);
+      for (int chunk = first; chunk < last; ++chunk) {
+        if (last - first > 1) {
+          __syncwarp();
+          copy(chunk, 0);
+          asm volatile("cp.async.wait_group 0;" ::: "memory");
+          __syncwarp();
+        }
+        for (int i = 0; i < BEAM_LOADS; ++i) {
+          const uint4 u = s_chunk[w][0][i * 32 + lane];
+          const X x = {{u.x, u.y, u.z, u.w}};
 #pragma unroll
-        for (int j = 0; j < X::COUNT; ++j) {
-          const uint32_t k = order_key(x[j]);
-          const int t = (i * 32 + lane) * X::COUNT + j;
-          const bool behind = e == 0 || k < last.x || (k == last.x && base + t > static_cast<int>(last.y));
-          if (t < V && behind && k > key[0]) { key[0] = k; token[0] = base + t; }      // t grows: the lowest of equal ones stays
+          for (int j = 0; j < X::COUNT; ++j) {
+            const uint32_t k = order_key(x[j]);
+            const int t = chunk * CHUNK + (i * 32 + lane) * X::COUNT + j;
+            const bool behind = e == 0 || k < before.x || (k == before.x && t > static_cast<int>(before.y));
+            if (t < a.V && behind && k > key[0]) { key[0] = k; token[0] = t; }      // t grows: the lowest of equal ones stays
+          }
         }
       }
-      last = take_best(key, token);
-      if (lane == 0) out[e] = last;
+      before = take_best(key, token);
+      if (lane == 0) out[e] = before;
     }
   }
 }
@@ -263,15 +305,15 @@ __device__ __forceinline__ double key_value(unsigned long long k) {
   return __longlong_as_double(static_cast<long long>(k >> 63 ? k & 0x7fffffffffffffffull : ~k));
 }
 
-// A part's sum for the reference `top` of its row: the sum that was made is off by 2^(m L - rn(m L)), L the rounded log2(e).
-__device__ __forceinline__ double part_sum(float2 s, float top) {
+// A run's sum for the reference `top` of its row: the sum that was made is off by 2^(m L - rn(m L)), L the rounded log2(e).
+__device__ __forceinline__ double run_sum(float2 s, float top) {
   const double off = fabsf(s.x) < BEAM_HUGE ? static_cast<double>(s.x) * static_cast<double>(LOG2E) - static_cast<double>(s.x * LOG2E) : 0.;
   return static_cast<double>(s.y) * (1. - off * 0.6931471805599453) * static_cast<double>(exp2f((s.x - top) * LOG2E));
 }
 
 // One block per prompt.  A warp per beam: the beam's sum, its parts' lists; then the beams' lists, K rounds, a lane per beam.
 __global__ void __launch_bounds__(SELECT_THREADS) beam_select_kernel(const BeamArgs a) {
-  constexpr int AT_ONCE = 8;               // entries of a lane, beside one of the best so far
+  constexpr int AT_ONCE = 4;               // entries of a lane, beside one of the best so far
   __shared__ unsigned long long s_value[BEAM_MOST][BEAM_MOST];      // order keys, 0: none
   __shared__ int s_token[BEAM_MOST][BEAM_MOST];
   pdl_launch_next();
@@ -304,10 +346,10 @@ __global__ void __launch_bounds__(SELECT_THREADS) beam_select_kernel(const BeamA
       for (int i = 32 + lane; i < a.parts; i += 32) top = fmaxf(top, a.sums[at * a.parts + i].x);
 #pragma unroll
       for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-      double sum = part_sum(s, top);
+      double sum = run_sum(s, top);
       for (int i = 32 + lane; i < a.parts; i += 32) {
         s = a.sums[at * a.parts + i];
-        sum += part_sum(s, top);
+        sum += run_sum(s, top);
       }
 #pragma unroll
       for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
@@ -355,15 +397,24 @@ __global__ void __launch_bounds__(SELECT_THREADS) beam_select_kernel(const BeamA
   }
 }
 
-static int beam_parts(int V, int size) { return static_cast<int>((static_cast<long long>(V) * size + BEAM_PART - 1) / BEAM_PART); }
+// Chunks of a run: as many warps as there are at once share them all.  Runs of a row.
+static int beam_chunks(int B, int K, int V, int size) {
+  const long long chunks = (static_cast<long long>(V) * size + BEAM_CHUNK - 1) / BEAM_CHUNK, warps = static_cast<long long>(BEAM_AT_ONCE) * sm_count_current();
+  const long long each = (chunks * B * K + warps - 1) / warps;
+  return static_cast<int>(each < chunks ? each : chunks);
+}
+static int beam_runs(int V, int size, int chunks) {
+  return static_cast<int>(((static_cast<long long>(V) * size + BEAM_CHUNK - 1) / BEAM_CHUNK + chunks - 1) / chunks);
+}
 
 }  // namespace axb
 
 using namespace axb;
 
-// 32-bit words of the workspace: two per row and part, then two per entry of their lists
+// 32-bit words of the workspace: two per row and run, then two per entry of their lists
 extern "C" long long axb_beam_select_words(int B, int K, int V, int dtype) {
-  return 2ll * B * K * beam_parts(V, dtype == 2 ? 4 : 2) * (1 + K);
+  const int size = dtype == 2 ? 4 : 2;
+  return 2ll * B * K * beam_runs(V, size, beam_chunks(B, K, V, size)) * (1 + K);
 }
 
 extern "C" int axb_beam_select(const void* logits, const float* scores, const void* done, int eos, float* out_scores, long long* out_tokens,
@@ -375,10 +426,10 @@ extern "C" int axb_beam_select(const void* logits, const float* scores, const vo
   if (V > 1 << 30) { set_error("beam_select: a vocabulary of at most %d", 1 << 30); return -1; }
   if (dtype < 0 || dtype > 2) { set_error("beam_select: bf16, fp16 or fp32 logits"); return -1; }
   if (reinterpret_cast<uintptr_t>(work) & 7) { set_error("beam_select: the workspace must be 8-byte aligned"); return -1; }
-  const int size = dtype == 2 ? 4 : 2, parts = beam_parts(V, size);
+  const int size = dtype == 2 ? 4 : 2, chunks = beam_chunks(B, K, V, size), parts = beam_runs(V, size, chunks);
   const long long items = static_cast<long long>(B) * K * parts;
   const BeamArgs a{logits, scores, (const unsigned char*)done, out_scores, out_tokens, out_parents, (unsigned char*)out_done,
-                   (float2*)work, (uint2*)work + items, K, V, eos, parts, items};
+                   (float2*)work, (uint2*)work + items, K, V, eos, parts, chunks, items};
   const bool vec = (reinterpret_cast<uintptr_t>(logits) & 15) == 0 && static_cast<long long>(V) * size % 16 == 0;
   void (*kern)(BeamArgs) = dtype == 0 ? (vec ? beam_rows_kernel<__nv_bfloat16, true> : beam_rows_kernel<__nv_bfloat16, false>)
                            : dtype == 1 ? (vec ? beam_rows_kernel<__half, true> : beam_rows_kernel<__half, false>)

@@ -115,17 +115,17 @@ struct StoreArgs {
   long long jobs, job_blocks;
 };
 
-template <typename T> __device__ __forceinline__ void load8(const T* p, float* f) {
-  const uint4 u = *reinterpret_cast<const uint4*>(p);
+template <typename T> __device__ __forceinline__ void widen8(const uint4& u, float* f) {
   const uint32_t w[4] = {u.x, u.y, u.z, u.w};
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     float2 t;
-    if constexpr (sizeof(T) == 2 && __is_same(T, __half)) t = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
+    if constexpr (__is_same(T, __half)) t = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
     else t = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&w[i]));
     f[2 * i] = t.x; f[2 * i + 1] = t.y;
   }
 }
+template <typename T> __device__ __forceinline__ void load8(const T* p, float* f) { widen8<T>(*reinterpret_cast<const uint4*>(p), f); }
 template <typename T> __device__ __forceinline__ void store8(T* p, const float* f) {
   uint32_t w[4];
 #pragma unroll
@@ -181,16 +181,18 @@ template <bool INT8> __device__ __forceinline__ float code_value(uint32_t byte) 
 }
 
 // Bound by reading the projection once and writing a byte per value: a thread keeps its values in registers between the search for the
-// largest and the codes.  A job is one head of one block, keys or values: a warp where few tokens arrive (a decoding step), a block of
-// threads with up to 64 values each where whole blocks are filled.  The queries' rotation is further blocks of the same launch.
-template <typename T, int D, bool INT8>
-__global__ void __launch_bounds__(256) store_kernel(const StoreArgs a) {
+// largest and the codes (as they came in where nothing is rotated: more blocks fit an SM, and more loads are on their way).  A job is one
+// head of one block, keys or values: a warp where few tokens arrive (a decoding step), a block of threads with up to 64 values each where
+// whole blocks are filled.  Nothing is waited for before the loads but the row's first slot; a token's own slot and position are looked at
+// when its values are there.  The queries' rotation is further blocks of the same launch.
+template <typename T, int D, bool INT8, bool ROPE>
+__global__ void __launch_bounds__(256, ROPE ? 2 : 4) store_kernel(const StoreArgs a) {
   constexpr int UNITS = D / 16;            // units of a token: eight pairs (i, i + D / 2) each
   __shared__ float part[8];
   pdl_launch_next();
   pdl_wait();
   const T* qkv = static_cast<const T*>(a.qkv);
-  if (blockIdx.x >= a.job_blocks) {        // queries
+  if (ROPE && blockIdx.x >= a.job_blocks) {        // queries
     const long long unit = (blockIdx.x - a.job_blocks) * static_cast<long long>(blockDim.x) + threadIdx.x;
     const int c = static_cast<int>(unit % UNITS) * 8, H = a.G * a.P;
     const long long row = unit / UNITS, token = row / H;
@@ -226,35 +228,44 @@ __global__ void __launch_bounds__(256) store_kernel(const StoreArgs a) {
   const int within = static_cast<int>(slot0 & (BT - 1));
   const int i0 = run == 0 ? 0 : run * BT - within, held = run == 0 ? within : 0;
   if (i0 >= a.S) return;
-  const long long first = run == 0 ? slot0 : slots[i0];
-  if (first < 0 || (first >> a.shift) >= a.N || (first & (BT - 1)) != held) return;
   const int n = min(BT - held, a.S - i0);
+  const long long first = slots[i0];
+  const T* x = qkv + r * a.row_stride + static_cast<long long>(i0) * a.token_stride + g * a.group_stride + (a.P + (values ? 1 : 0)) * D;
+  uint4 raw[STORE_UNITS][2];
+  long long slot[STORE_UNITS];
+  int position[STORE_UNITS];
+#pragma unroll
+  for (int u = 0; u < STORE_UNITS; ++u) {
+    const int unit = tid + u * threads, i = unit / UNITS, c = (unit % UNITS) * 8;
+    slot[u] = -1;
+    if (i >= n) continue;
+    const T* p = x + static_cast<long long>(i) * a.token_stride + c;
+    raw[u][0] = *reinterpret_cast<const uint4*>(p);
+    raw[u][1] = *reinterpret_cast<const uint4*>(p + D / 2);
+    slot[u] = slots[i0 + i];
+    if (ROPE) position[u] = a.positions[static_cast<size_t>(r) * a.S + i0 + i];
+  }
+  if (first < 0 || (first >> a.shift) >= a.N || (first & (BT - 1)) != held) return;
   const size_t head = static_cast<size_t>(first >> a.shift) * a.G + g;
   uint8_t* codes = (values ? a.v : a.k) + head * BT * D;
   float* scale_at = (values ? a.vs : a.ks) + head;
-  const T* x = qkv + r * a.row_stride + static_cast<long long>(i0) * a.token_stride + g * a.group_stride + (a.P + (values ? 1 : 0)) * D;
-  const bool turn = a.cs != nullptr && !values, placed = a.cs != nullptr;
-
   const float old = held ? *scale_at : 0.f;
-  float f[STORE_UNITS][16], largest = 0.f;
+  float f[ROPE ? STORE_UNITS : 1][16], largest = 0.f;
   uint32_t mine = 0;
 #pragma unroll
   for (int u = 0; u < STORE_UNITS; ++u) {
     const int unit = tid + u * threads, i = unit / UNITS, c = (unit % UNITS) * 8;
-    if (i >= n || slots[i0 + i] != first + i) continue;
-    int at = 0;
-    if (placed) { at = a.positions[static_cast<size_t>(r) * a.S + i0 + i]; if (at < 0 || at >= a.angles) continue; }
+    if (i >= n || slot[u] != first + i || (ROPE && (position[u] < 0 || position[u] >= a.angles))) continue;
     mine |= 1u << u;
-    const T* p = x + static_cast<long long>(i) * a.token_stride + c;
-    load8(p, f[u]);
-    load8(p + D / 2, f[u] + 8);
-    if (turn) rotate8(f[u], a.cs + (static_cast<size_t>(at) * (D / 2) + c) * 2);
+    float* y = f[ROPE ? u : 0];
+    widen8<T>(raw[u][0], y);
+    widen8<T>(raw[u][1], y + 8);
+    if (ROPE && !values) rotate8(y, a.cs + (static_cast<size_t>(position[u]) * (D / 2) + c) * 2);
 #pragma unroll
-    for (int j = 0; j < 16; ++j) { const float m = fabsf(f[u][j]); if (m <= 3.4028234663852886e38f) largest = fmaxf(largest, m); }
+    for (int j = 0; j < 16; ++j) { const float m = fabsf(y[j]); if (m <= 3.4028234663852886e38f) largest = fmaxf(largest, m); }
   }
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) largest = fmaxf(largest, __shfl_xor_sync(0xffffffffu, largest, o));
   bool some = __any_sync(0xffffffffu, mine != 0);
+  largest = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(largest)));      // not negative: the order of the bits
   if (threads > 32) {
     if ((tid & 31) == 0) part[tid >> 5] = some ? largest : -1.f;
     __syncthreads();
@@ -286,7 +297,8 @@ __global__ void __launch_bounds__(256) store_kernel(const StoreArgs a) {
     uint8_t* p = codes + static_cast<size_t>(held + i) * D + c;
 #pragma unroll
     for (int half = 0; half < 2; ++half) {
-      const float* s = f[u] + 8 * half;
+      float* s = f[ROPE ? u : 0] + 8 * half;
+      if (!ROPE) widen8<T>(raw[u][half], s);
       *reinterpret_cast<uint2*>(p + half * (D / 2)) =
           make_uint2(codes4<INT8>(s[0] * inverse, s[1] * inverse, s[2] * inverse, s[3] * inverse),
                      codes4<INT8>(s[4] * inverse, s[5] * inverse, s[6] * inverse, s[7] * inverse));
@@ -350,6 +362,14 @@ __global__ void __launch_bounds__(REORDER_THREADS) reorder_kernel(const ReorderA
   }
 }
 
+template <typename T, int D> static void (*store_variant(bool int8, bool rope))(StoreArgs) {
+  return int8 ? (rope ? store_kernel<T, D, true, true> : store_kernel<T, D, true, false>)
+              : (rope ? store_kernel<T, D, false, true> : store_kernel<T, D, false, false>);
+}
+template <typename T> static void (*store_variant(int D, bool int8, bool rope))(StoreArgs) {
+  return D == 64 ? store_variant<T, 64>(int8, rope) : store_variant<T, 128>(int8, rope);
+}
+
 // log2 of the tokens of a block, or -1
 static int block_shift(int block_tokens) {
   for (int s = 4; s <= 7; ++s) if (block_tokens == 1 << s) return s;
@@ -401,11 +421,7 @@ extern "C" int axb_store_blocks(const void* qkv, long long row_stride, long long
   const long long q_units = cs ? static_cast<long long>(R) * S * G * P * (D / 16) : 0;
   const long long grid = a.job_blocks + (q_units + threads - 1) / threads;
   if (grid > 0x7fffffffll) { set_error("store_blocks: too many tokens in one call"); return -1; }
-  void (*kern)(StoreArgs) = nullptr;
-  if (dtype == 0) kern = D == 64 ? (int8 ? store_kernel<__nv_bfloat16, 64, true> : store_kernel<__nv_bfloat16, 64, false>)
-                                 : (int8 ? store_kernel<__nv_bfloat16, 128, true> : store_kernel<__nv_bfloat16, 128, false>);
-  else kern = D == 64 ? (int8 ? store_kernel<__half, 64, true> : store_kernel<__half, 64, false>)
-                      : (int8 ? store_kernel<__half, 128, true> : store_kernel<__half, 128, false>);
+  void (*kern)(StoreArgs) = dtype == 0 ? store_variant<__nv_bfloat16>(D, int8 != 0, cs != nullptr) : store_variant<__half>(D, int8 != 0, cs != nullptr);
   AXB_CUDA(pdl_launch(kern, dim3((unsigned)grid), dim3(threads), 0, (cudaStream_t)stream, a));
   return 0;
 }
