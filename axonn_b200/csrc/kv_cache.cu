@@ -158,8 +158,16 @@ template <bool INT8> __device__ __forceinline__ int scale_exponent(float largest
   const int e = static_cast<int>(b >> 23) - 127 - (INT8 ? 6 : 8) + ((b & 0x7fffffu) > (INT8 ? 0x7e0000u : 0x600000u));
   return max(e, LOWEST_EXPONENT);
 }
-// Four values as codes.  Values past the largest code (infinities) become it; NaN stays NaN in e4m3 and is 0 in int8.
-template <bool INT8> __device__ __forceinline__ uint32_t codes4(float a, float b, float c, float d) {
+// Four values times `scale` as codes.  Values past the largest code (infinities) become it; NaN stays NaN in e4m3 and is 0 in int8.
+// FINITE: there are none of those; adding 1.5 x 2^23 leaves the rounded number in the low bits, with one rounding of the product.
+template <bool INT8, bool FINITE> __device__ __forceinline__ uint32_t codes4(float a, float b, float c, float d, float scale) {
+  if constexpr (INT8 && FINITE) {
+    constexpr float magic = 12582912.f;
+    const uint32_t lo = __byte_perm(__float_as_uint(__fmaf_rn(a, scale, magic)), __float_as_uint(__fmaf_rn(b, scale, magic)), 0x0040);
+    const uint32_t hi = __byte_perm(__float_as_uint(__fmaf_rn(c, scale, magic)), __float_as_uint(__fmaf_rn(d, scale, magic)), 0x0040);
+    return __byte_perm(lo, hi, 0x5410);
+  }
+  a *= scale; b *= scale; c *= scale; d *= scale;
   if constexpr (INT8) {
     const float f[4] = {a, b, c, d};
     uint32_t o = 0;
@@ -174,6 +182,17 @@ template <bool INT8> __device__ __forceinline__ uint32_t codes4(float a, float b
     const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(c, d), __NV_SATFINITE, __NV_E4M3);
     return lo | (hi << 16);
   }
+}
+// |a| and |b|, the larger one; NaN if one is
+__device__ __forceinline__ float largest_nan(float a, float b) {
+  float m;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(m) : "f"(a), "f"(fabsf(b)));
+  return m;
+}
+template <typename T> __device__ __forceinline__ uint32_t largest_nan_16(uint32_t a, uint32_t b) {
+  b &= 0x7fff7fffu;
+  if constexpr (__is_same(T, __half)) { const __half2 m = __hmax2_nan(*reinterpret_cast<const __half2*>(&a), *reinterpret_cast<const __half2*>(&b)); return *reinterpret_cast<const uint32_t*>(&m); }
+  else { const __nv_bfloat162 m = __hmax2_nan(*reinterpret_cast<const __nv_bfloat162*>(&a), *reinterpret_cast<const __nv_bfloat162*>(&b)); return *reinterpret_cast<const uint32_t*>(&m); }
 }
 template <bool INT8> __device__ __forceinline__ float code_value(uint32_t byte) {
   if constexpr (INT8) return static_cast<float>(static_cast<int8_t>(byte));
@@ -251,18 +270,44 @@ __global__ void __launch_bounds__(256, ROPE ? 2 : 4) store_kernel(const StoreArg
   float* scale_at = (values ? a.vs : a.ks) + head;
   const float old = held ? *scale_at : 0.f;
   float f[ROPE ? STORE_UNITS : 1][16], largest = 0.f;
-  uint32_t mine = 0;
+  uint32_t mine = 0, pairs = 0u;
 #pragma unroll
   for (int u = 0; u < STORE_UNITS; ++u) {
     const int unit = tid + u * threads, i = unit / UNITS, c = (unit % UNITS) * 8;
     if (i >= n || slot[u] != first + i || (ROPE && (position[u] < 0 || position[u] >= a.angles))) continue;
     mine |= 1u << u;
-    float* y = f[ROPE ? u : 0];
+    if (!ROPE) {
+#pragma unroll
+      for (int half = 0; half < 2; ++half)
+        pairs = largest_nan_16<T>(largest_nan_16<T>(largest_nan_16<T>(largest_nan_16<T>(pairs, raw[u][half].x), raw[u][half].y), raw[u][half].z), raw[u][half].w);
+      continue;
+    }
+    float* y = f[u];
     widen8<T>(raw[u][0], y);
     widen8<T>(raw[u][1], y + 8);
-    if (ROPE && !values) rotate8(y, a.cs + (static_cast<size_t>(position[u]) * (D / 2) + c) * 2);
+    if (!values) rotate8(y, a.cs + (static_cast<size_t>(position[u]) * (D / 2) + c) * 2);
 #pragma unroll
-    for (int j = 0; j < 16; ++j) { const float m = fabsf(y[j]); if (m <= 3.4028234663852886e38f) largest = fmaxf(largest, m); }
+    for (int j = 0; j < 16; ++j) largest = largest_nan(largest, y[j]);
+  }
+  if (!ROPE) {
+    float y[8];
+    widen8<T>(make_uint4(pairs, 0u, 0u, 0u), y);
+    largest = largest_nan(y[0], y[1]);
+  }
+  const bool finite = largest <= 3.4028234663852886e38f;
+  if (!finite) {                           // the largest of what is finite
+    largest = 0.f;
+#pragma unroll
+    for (int u = 0; u < STORE_UNITS; ++u) {
+      if (!(mine >> u & 1)) continue;
+#pragma unroll
+      for (int half = 0; half < 2; ++half) {
+        float* y = f[ROPE ? u : 0] + 8 * half;
+        if (!ROPE) widen8<T>(raw[u][half], y);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) { const float m = fabsf(y[j]); if (m <= 3.4028234663852886e38f) largest = fmaxf(largest, m); }
+      }
+    }
   }
   bool some = __any_sync(0xffffffffu, mine != 0);
   largest = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(largest)));      // not negative: the order of the bits
@@ -284,8 +329,8 @@ __global__ void __launch_bounds__(256, ROPE ? 2 : 4) store_kernel(const StoreArg
       uint32_t w[4] = {u.x, u.y, u.z, u.w};
 #pragma unroll
       for (int j = 0; j < 4; ++j)
-        w[j] = codes4<INT8>(code_value<INT8>(w[j] & 0xff) * shrink, code_value<INT8>((w[j] >> 8) & 0xff) * shrink,
-                            code_value<INT8>((w[j] >> 16) & 0xff) * shrink, code_value<INT8>(w[j] >> 24) * shrink);
+        w[j] = codes4<INT8, false>(code_value<INT8>(w[j] & 0xff), code_value<INT8>((w[j] >> 8) & 0xff), code_value<INT8>((w[j] >> 16) & 0xff),
+                                   code_value<INT8>(w[j] >> 24), shrink);
       *at = make_uint4(w[0], w[1], w[2], w[3]);
     }
   }
@@ -300,8 +345,8 @@ __global__ void __launch_bounds__(256, ROPE ? 2 : 4) store_kernel(const StoreArg
       float* s = f[ROPE ? u : 0] + 8 * half;
       if (!ROPE) widen8<T>(raw[u][half], s);
       *reinterpret_cast<uint2*>(p + half * (D / 2)) =
-          make_uint2(codes4<INT8>(s[0] * inverse, s[1] * inverse, s[2] * inverse, s[3] * inverse),
-                     codes4<INT8>(s[4] * inverse, s[5] * inverse, s[6] * inverse, s[7] * inverse));
+          finite ? make_uint2(codes4<INT8, true>(s[0], s[1], s[2], s[3], inverse), codes4<INT8, true>(s[4], s[5], s[6], s[7], inverse))
+                 : make_uint2(codes4<INT8, false>(s[0], s[1], s[2], s[3], inverse), codes4<INT8, false>(s[4], s[5], s[6], s[7], inverse));
     }
   }
   if (threads > 32) __syncthreads(); else __syncwarp();      // everyone has read the old scale
