@@ -1,5 +1,5 @@
 // Host paths of the operators that short calls are bound by: the same launches as the Python code beside them (ops/norm.py,
-// ops/attention_cuda.py, intra_layer/fully_connected.py), with the questions asked and the tensors allocated in C++, and the
+// ops/attention_cuda.py, ops/kv_cache.py, ops/beam.py, intra_layer/fully_connected.py), with the questions asked and the tensors allocated in C++, and the
 // normalisation's autograd node in C++, so that neither its backward nor the launches of a layer wait for the interpreter.
 //
 // A function returns None where the call is not one of those it takes; the caller then goes its general way, which accepts or
@@ -20,6 +20,8 @@
 
 #include <algorithm>
 #include <atomic>
+#include <cmath>
+#include <initializer_list>
 #include <string>
 
 #include "axonn_b200.h"
@@ -33,7 +35,10 @@ using std::optional;
 // the build, and a library of another one is not bound.
 #define AXB_LAUNCHERS(X) \
   X(axb_norm_fwd, norm_fwd) X(axb_norm_bwd, norm_bwd) X(axb_add_norm_fwd, add_norm_fwd) X(axb_add_norm_bwd, add_norm_bwd) \
-  X(axb_norm_grid, norm_grid) X(axb_gemm, gemm) X(axb_flash_attn_fwd, flash_fwd) X(axb_last_error, last_error)
+  X(axb_norm_grid, norm_grid) X(axb_gemm, gemm) X(axb_flash_attn_fwd, flash_fwd) X(axb_last_error, last_error) \
+  X(axb_plan_blocks, plan_blocks) X(axb_store_blocks, store_blocks) X(axb_reorder_blocks, reorder_blocks) \
+  X(axb_cached_attention_words, attention_words) X(axb_cached_attention, cached_attention) \
+  X(axb_beam_select_words, beam_words) X(axb_beam_select, beam_select)
 #define AXB_DECLARE(symbol, name) decltype(&::symbol) name = nullptr;
 AXB_LAUNCHERS(AXB_DECLARE)
 PyObject *kernel_error = nullptr, *parameter_type = nullptr;
@@ -255,6 +260,227 @@ PyObject* py_attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
   END_HANDLE_TH_ERRORS
 }
 
+// ---------------------------------------------------------------------------------------------------------------- block cache
+// Dense, of the type and the shape.
+bool is(const Tensor& t, at::ScalarType type, std::initializer_list<int64_t> shape) {
+  return t.scalar_type() == type && t.sizes() == at::IntArrayRef(shape) && t.is_contiguous();
+}
+bool block_size(int64_t n) { return n == 16 || n == 32 || n == 64 || n == 128; }
+
+// The tensors of the arguments named, all on the current device, none with a gradient to be had; where the second of a pair says so,
+// None may stand there and gives an undefined tensor.
+bool take_tensors(PyObject* const* a, std::initializer_list<std::pair<int, bool>> which, Tensor* out) {
+  const int device = c10::cuda::current_device();
+  for (const auto& [i, missing] : which) {
+    if (missing && a[i] == Py_None) { *out++ = Tensor(); continue; }
+    if (!plain(a[i])) return false;
+    *out = THPVariable_Unpack(a[i]);
+    if (out->get_device() != device || wants_grad(*out)) return false;
+    ++out;
+  }
+  return true;
+}
+
+// Codes and scales of a layer (dims 4) or of stacked layers (5), as the kernels take them.
+bool layer_ok(const Tensor& k, const Tensor& v, const Tensor& ks, const Tensor& vs, int dims) {
+  const auto type = k.scalar_type();
+  if ((type != at::kFloat8_e4m3fn && type != at::kChar) || v.scalar_type() != type || k.dim() != dims || v.sizes() != k.sizes() || k.numel() == 0 ||
+      !block_size(k.size(dims - 2)) || ks.scalar_type() != at::kFloat || vs.scalar_type() != at::kFloat || ks.dim() != dims - 2 ||
+      vs.dim() != dims - 2 || !k.is_contiguous() || !v.is_contiguous() || !ks.is_contiguous() || !vs.is_contiguous() || !on_16_bytes(k) || !on_16_bytes(v))
+    return false;
+  for (int i = 0; i < dims - 2; ++i)
+    if (ks.size(i) != k.size(i) || vs.size(i) != k.size(i)) return false;
+  for (int i = 0; i < dims; ++i)
+    if (k.size(i) > INT32_MAX) return false;
+  return true;
+}
+
+PyObject* tuple_of(std::initializer_list<Tensor> tensors) {
+  PyObject* tuple = PyTuple_New(static_cast<Py_ssize_t>(tensors.size()));
+  if (!tuple) return nullptr;
+  Py_ssize_t i = 0;
+  for (const Tensor& t : tensors) {
+    PyObject* o = t.defined() ? THPVariable_Wrap(t) : Py_NewRef(Py_None);
+    if (!o) { Py_DECREF(tuple); return nullptr; }
+    PyTuple_SET_ITEM(tuple, i++, o);
+  }
+  return tuple;
+}
+
+// plan_blocks(lengths, new, tables, free, taken, tokens, block_tokens) -> (slots, positions, lengths, taken) or None
+PyObject* py_plan_blocks(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  Tensor t[5];
+  if (n != 7 || observed() || !take_tensors(a, {{0, false}, {1, false}, {2, false}, {3, false}, {4, false}}, t)) Py_RETURN_NONE;
+  const auto& [lengths, fresh, tables, free_blocks, taken] = t;
+  const long tokens = PyLong_AsLong(a[5]), block = PyLong_AsLong(a[6]);
+  if (PyErr_Occurred()) return nullptr;
+  if (lengths.dim() != 1 || tables.dim() != 2 || free_blocks.dim() != 1) Py_RETURN_NONE;
+  const int64_t R = lengths.size(0), W = tables.size(1), N = free_blocks.size(0);
+  if (R == 0 || W == 0 || N == 0 || tokens <= 0 || std::max({R, W, N, static_cast<int64_t>(tokens)}) > INT32_MAX || !block_size(block) ||
+      !is(lengths, at::kInt, {R}) || !is(fresh, at::kInt, {R}) || !is(tables, at::kInt, {R, W}) || !is(free_blocks, at::kInt, {N}) ||
+      !is(taken, at::kInt, {1}))
+    Py_RETURN_NONE;
+  Tensor slots, positions, after, used;
+  {
+    NoGil no_gil;
+    slots = at::empty({R, tokens}, lengths.options().dtype(at::kLong));
+    positions = at::empty({R, tokens}, lengths.options());
+    after = at::empty({R}, lengths.options());
+    used = at::empty({1}, lengths.options());
+    check(plan_blocks(lengths.data_ptr<int>(), fresh.data_ptr<int>(), tables.data_ptr<int>(), free_blocks.data_ptr<int>(), taken.data_ptr<int>(),
+                      reinterpret_cast<long long*>(slots.data_ptr<int64_t>()), positions.data_ptr<int>(), after.data_ptr<int>(), used.data_ptr<int>(),
+                      static_cast<int>(R), static_cast<int>(tokens), static_cast<int>(W), static_cast<int>(N), static_cast<int>(block), stream()),
+          "axb_plan_blocks");
+  }
+  return tuple_of({slots, positions, after, used});
+  END_HANDLE_TH_ERRORS
+}
+
+// Strides of rows, tokens and groups of [R, S, G, heads, D] with dense heads, as the kernels can read them.
+bool head_strides(const Tensor& x, int64_t (&strides)[3]) {
+  if (x.stride(4) != 1 || (x.stride(3) != x.size(4) && x.size(3) != 1) || !on_16_bytes(x)) return false;
+  for (int i = 0; i < 3; ++i) {
+    strides[i] = x.size(i) == 1 ? 0 : x.stride(i);
+    if (strides[i] % 8) return false;
+  }
+  return true;
+}
+
+// store_blocks(qkv, k, v, k_scale, v_scale, slots, positions | None, rope table | None) -> (queries | None,) or None
+PyObject* py_store_blocks(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  Tensor t[8];
+  if (n != 8 || observed() ||
+      !take_tensors(a, {{0, false}, {1, false}, {2, false}, {3, false}, {4, false}, {5, false}, {6, true}, {7, true}}, t)) Py_RETURN_NONE;
+  const auto& [qkv, k, v, ks, vs, slots, positions, table] = t;
+  if (!layer_ok(k, v, ks, vs, 4) || qkv.dim() != 5 || (qkv.scalar_type() != at::kBFloat16 && qkv.scalar_type() != at::kHalf)) Py_RETURN_NONE;
+  const int64_t N = k.size(0), G = k.size(1), BT = k.size(2), D = k.size(3), R = qkv.size(0), S = qkv.size(1), P = qkv.size(3) - 2;
+  int64_t strides[3];
+  if (R == 0 || S == 0 || qkv.size(2) != G || P < 0 || qkv.size(4) != D || (D != 64 && D != 128) || std::max({R, S, P}) > INT32_MAX ||
+      !is(slots, at::kLong, {R, S}) || qkv.size(3) == 1 || !head_strides(qkv, strides))
+    Py_RETURN_NONE;
+  const bool rope = table.defined();
+  if (rope && (!positions.defined() || !is(positions, at::kInt, {R, S}) || table.dim() != 3 || !is(table, at::kFloat, {table.size(0), D / 2, 2}) ||
+               table.size(0) > INT32_MAX || !on_16_bytes(table)))
+    Py_RETURN_NONE;
+  Tensor q;
+  {
+    NoGil no_gil;
+    if (rope) q = at::empty({R, S, G * P, D}, qkv.options());
+    check(store_blocks(qkv.data_ptr(), strides[0], strides[1], strides[2], reinterpret_cast<const long long*>(slots.data_ptr<int64_t>()),
+                       rope ? positions.data_ptr<int>() : nullptr, rope ? table.data_ptr<float>() : nullptr, rope ? q.data_ptr() : nullptr,
+                       k.data_ptr(), v.data_ptr(), ks.data_ptr<float>(), vs.data_ptr<float>(), static_cast<int>(R), static_cast<int>(S),
+                       static_cast<int>(G), static_cast<int>(P), static_cast<int>(D), static_cast<int>(N), static_cast<int>(BT),
+                       rope ? static_cast<int>(table.size(0)) : 0, dtype_code(qkv), k.scalar_type() == at::kChar, stream()), "axb_store_blocks");
+  }
+  return tuple_of({q});
+  END_HANDLE_TH_ERRORS
+}
+
+// cached_attention(q, k, v, k_scale, v_scale, tables, lengths, new | None, scale | None) -> output or None
+PyObject* py_cached_attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  Tensor t[8];
+  if (n != 9 || observed() ||
+      !take_tensors(a, {{0, false}, {1, false}, {2, false}, {3, false}, {4, false}, {5, false}, {6, false}, {7, true}}, t)) Py_RETURN_NONE;
+  const auto& [given, k, v, ks, vs, tables, lengths, fresh] = t;
+  if (!layer_ok(k, v, ks, vs, 4) || (given.scalar_type() != at::kBFloat16 && given.scalar_type() != at::kHalf)) Py_RETURN_NONE;
+  const int64_t N = k.size(0), G = k.size(1), BT = k.size(2), D = k.size(3);
+  Tensor q = given;
+  if (q.dim() == 4) {
+    if (q.size(2) % G || q.size(2) == 0 || (q.stride(2) != q.size(3) && q.size(2) != 1)) Py_RETURN_NONE;
+    q = q.unflatten(2, {G, q.size(2) / G});
+  }
+  if (q.dim() != 5 || q.size(2) != G || q.size(4) != D || q.numel() == 0 || (D != 64 && D != 128) || tables.dim() != 2) Py_RETURN_NONE;
+  const int64_t R = q.size(0), S = q.size(1), P = q.size(3), W = tables.size(1);
+  int64_t strides[3];
+  if (std::max({R, S * P, W}) > INT32_MAX || W == 0 || !head_strides(q, strides) || !is(tables, at::kInt, {R, W}) || !is(lengths, at::kInt, {R}) ||
+      (fresh.defined() && !is(fresh, at::kInt, {R})))
+    Py_RETURN_NONE;
+  double scale = 1.0 / std::sqrt(static_cast<double>(D));
+  if (a[8] != Py_None) {
+    scale = PyFloat_AsDouble(a[8]);
+    if (scale == -1.0 && PyErr_Occurred()) return nullptr;
+    if (!std::isfinite(scale)) Py_RETURN_NONE;
+  }
+  Tensor out;
+  {
+    NoGil no_gil;
+    out = at::empty({R, S, G * P, D}, q.options());
+    const Tensor work = at::empty({attention_words(static_cast<int>(R), static_cast<int>(S), static_cast<int>(P), static_cast<int>(D))},
+                                  q.options().dtype(at::kFloat));
+    check(cached_attention(q.data_ptr(), strides[0], strides[1], strides[2], k.data_ptr(), v.data_ptr(), ks.data_ptr<float>(), vs.data_ptr<float>(),
+                           tables.data_ptr<int>(), lengths.data_ptr<int>(), fresh.defined() ? fresh.data_ptr<int>() : nullptr, out.data_ptr(),
+                           work.data_ptr(), static_cast<int>(R), static_cast<int>(S), static_cast<int>(G), static_cast<int>(P), static_cast<int>(D),
+                           static_cast<int>(W), static_cast<int>(N), static_cast<int>(BT), static_cast<float>(scale), dtype_code(q),
+                           k.scalar_type() == at::kChar, stream()), "axb_cached_attention", 2);
+  }
+  return THPVariable_Wrap(out);
+  END_HANDLE_TH_ERRORS
+}
+
+// reorder_blocks(k, v, k_scale, v_scale, tables, lengths, spare, parents) -> (tables, lengths, spare) or None
+PyObject* py_reorder_blocks(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  Tensor t[8];
+  if (n != 8 || observed() ||
+      !take_tensors(a, {{0, false}, {1, false}, {2, false}, {3, false}, {4, false}, {5, false}, {6, false}, {7, false}}, t)) Py_RETURN_NONE;
+  const auto& [k, v, ks, vs, tables, lengths, spare, parents] = t;
+  if (!layer_ok(k, v, ks, vs, 5) || tables.dim() != 2 || parents.dim() != 2) Py_RETURN_NONE;
+  const int64_t R = tables.size(0), W = tables.size(1), K = parents.size(1);
+  if (R == 0 || W == 0 || parents.numel() != R || std::max(R, W) > INT32_MAX || k.size(4) % 16 || !is(tables, at::kInt, {R, W}) ||
+      !is(lengths, at::kInt, {R}) || !is(spare, at::kInt, {R}) || !is(parents, at::kInt, {R / K, K}))
+    Py_RETURN_NONE;
+  Tensor out[3];
+  {
+    NoGil no_gil;
+    out[0] = at::empty({R, W}, tables.options());
+    out[1] = at::empty({R}, tables.options());
+    out[2] = at::empty({R}, tables.options());
+    check(reorder_blocks(k.data_ptr(), v.data_ptr(), ks.data_ptr<float>(), vs.data_ptr<float>(), tables.data_ptr<int>(), lengths.data_ptr<int>(),
+                         spare.data_ptr<int>(), parents.data_ptr<int>(), out[0].data_ptr<int>(), out[1].data_ptr<int>(), out[2].data_ptr<int>(),
+                         static_cast<int>(k.size(0)), static_cast<int>(R), static_cast<int>(K), static_cast<int>(W), static_cast<int>(k.size(1)),
+                         static_cast<int>(k.size(2)), static_cast<int>(k.size(3)), static_cast<int>(k.size(4)), stream()), "axb_reorder_blocks");
+  }
+  return tuple_of({out[0], out[1], out[2]});
+  END_HANDLE_TH_ERRORS
+}
+
+// ---------------------------------------------------------------------------------------------------------------- beam search
+// beam_select(logits, scores, done | None, eos | None) -> (scores, tokens, parents, done | None) or None
+PyObject* py_beam_select(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  Tensor t[3];
+  if (n != 4 || observed() || !take_tensors(a, {{0, false}, {1, false}, {2, true}}, t)) Py_RETURN_NONE;
+  const auto& [logits, scores, done] = t;
+  if (logits.dim() != 3 || dtype_code(logits) < 0 || !logits.is_contiguous() || logits.numel() == 0 || done.defined() == (a[3] == Py_None)) Py_RETURN_NONE;
+  const int64_t B = logits.size(0), K = logits.size(1), V = logits.size(2);
+  long eos = -1;
+  if (done.defined()) {
+    eos = PyLong_AsLong(a[3]);
+    if (eos == -1 && PyErr_Occurred()) return nullptr;
+    if (eos < 0 || eos >= V || !is(done, at::kBool, {B, K})) Py_RETURN_NONE;
+  }
+  if (K > 32 || V > (1 << 30) || B > INT32_MAX / K || !is(scores, at::kFloat, {B, K})) Py_RETURN_NONE;
+  Tensor out_scores, tokens, parents, out_done;
+  {
+    NoGil no_gil;
+    out_scores = at::empty({B, K}, scores.options());
+    tokens = at::empty({B, K}, scores.options().dtype(at::kLong));
+    parents = at::empty({B, K}, scores.options().dtype(at::kInt));
+    if (done.defined()) out_done = at::empty({B, K}, done.options());
+    const Tensor work = at::empty({beam_words(static_cast<int>(B), static_cast<int>(K), static_cast<int>(V), dtype_code(logits))},
+                                  scores.options().dtype(at::kInt));
+    check(beam_select(logits.data_ptr(), scores.data_ptr<float>(), done.defined() ? done.data_ptr() : nullptr, static_cast<int>(eos),
+                      out_scores.data_ptr<float>(), reinterpret_cast<long long*>(tokens.data_ptr<int64_t>()), parents.data_ptr<int>(),
+                      done.defined() ? out_done.data_ptr() : nullptr, work.data_ptr(), static_cast<int>(B), static_cast<int>(K),
+                      static_cast<int>(V), dtype_code(logits), stream()), "axb_beam_select", 2);
+  }
+  return tuple_of({out_scores, tokens, parents, out_done});
+  END_HANDLE_TH_ERRORS
+}
+
 // bind({launcher name: address}, KernelError, Parameter, axb_interface() of the library they are from) -> False if it is another one
 PyObject* py_bind(PyObject*, PyObject* const* a, Py_ssize_t n) {
   HANDLE_TH_ERRORS
@@ -283,6 +509,11 @@ PyMethodDef methods[] = {
     {"norm", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(py_norm)), METH_FASTCALL, nullptr},
     {"linear", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(py_linear)), METH_FASTCALL, nullptr},
     {"attention", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(py_attention)), METH_FASTCALL, nullptr},
+    {"plan_blocks", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(py_plan_blocks)), METH_FASTCALL, nullptr},
+    {"store_blocks", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(py_store_blocks)), METH_FASTCALL, nullptr},
+    {"cached_attention", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(py_cached_attention)), METH_FASTCALL, nullptr},
+    {"reorder_blocks", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(py_reorder_blocks)), METH_FASTCALL, nullptr},
+    {"beam_select", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(py_beam_select)), METH_FASTCALL, nullptr},
     {"launches", py_launches, METH_NOARGS, nullptr},
     {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "axonn_host", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};

@@ -31,7 +31,8 @@ LIB_PATH = os.environ.get("AXONN_LIB_PATH") or (
 _launches = 0
 _HOST = _UNSET = object()
 _HOST_LAUNCHERS = ("axb_norm_fwd", "axb_norm_bwd", "axb_add_norm_fwd", "axb_add_norm_bwd", "axb_norm_grid", "axb_gemm",
-                   "axb_flash_attn_fwd", "axb_last_error")
+                   "axb_flash_attn_fwd", "axb_last_error", "axb_plan_blocks", "axb_store_blocks", "axb_reorder_blocks",
+                   "axb_cached_attention_words", "axb_cached_attention", "axb_beam_select_words", "axb_beam_select")
 
 
 def __getattr__(name):

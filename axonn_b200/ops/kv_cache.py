@@ -18,6 +18,7 @@ from typing import NamedTuple, Optional
 import torch
 
 from . import _lib
+from .direct import host_paths
 
 BLOCK_TOKENS = (16, 32, 64, 128)
 CODE_TYPES = (torch.float8_e4m3fn, torch.int8)
@@ -87,6 +88,10 @@ def plan_blocks(lengths, new, tables, free, taken, tokens, block_tokens):
     the requests; their ids are written into ``tables`` (in place: entries behind what a request holds).  A request whose row of
     the table is full, or that comes when the list is used up, gets places for as many tokens as there is room for: its
     ``lengths`` entry of the plan tells.  ``lengths`` and ``taken`` themselves are left as they are."""
+    if lengths.is_cuda and (host := host_paths()) is not None:
+        out = host.plan_blocks(lengths, new, tables, free, taken, tokens, block_tokens)
+        if out is not None:
+            return BlockPlan(*out)
     dev, R = lengths.device, lengths.shape[0] if lengths.ndim == 1 else -1
     if _elsewhere(dev):
         with torch.cuda.device(dev):
@@ -156,6 +161,10 @@ def store_blocks(qkv, layer, slots, positions=None, rope_table=None) -> Optional
     With ``rope_table`` (``ops.rope_table``) and ``positions`` keys are stored rotated and the rotated queries are returned,
     ``[R, S, kv_heads * q_per_kv, D]`` (zeros for tokens without a slot); ``qkv`` is left as it is.  A token whose position the table
     lacks counts as one without a slot.  Without a table the result is ``None``."""
+    if qkv.is_cuda and (host := host_paths()) is not None:
+        out = host.store_blocks(qkv, *layer, slots, positions, rope_table)
+        if out is not None:
+            return out[0]
     dev = qkv.device
     if _elsewhere(dev):
         with torch.cuda.device(dev):
@@ -265,6 +274,10 @@ def cached_attention(q, layer, tables, lengths, new=None, scale=None):
     Blocks that a table lacks (-1 within the length) count as absent.  What lies behind a sequence in its last block is never
     looked at.  On a GPU: bf16 or fp16, D 64 or 128; the work is bound by reading the cache, once for up to 16 query columns
     (``S * q_per_kv``) - long prompts are better evaluated with ``flash_attention`` before they are stored."""
+    if q.is_cuda and (host := host_paths()) is not None:
+        out = host.cached_attention(q, *layer, tables, lengths, new, scale)
+        if out is not None:
+            return out
     dev = q.device
     if _elsewhere(dev):
         with torch.cuda.device(dev):
@@ -352,6 +365,10 @@ def reorder_blocks(blocks, tables, lengths, spare, parents):
     ``spare[r]``, and keeps the block that it leaves as the new spare one; ``spare [R]`` and the unfinished blocks of the rows are all
     different.  Returns the rows' new ``(tables, lengths, spare)``; the arguments are left as they are, but for the contents of the
     spare blocks.  A parent outside the group counts as the row itself."""
+    if tables.is_cuda and (host := host_paths()) is not None:
+        out = host.reorder_blocks(*blocks, tables, lengths, spare, parents)
+        if out is not None:
+            return out
     dev = tables.device
     if _elsewhere(dev):
         with torch.cuda.device(dev):

@@ -118,6 +118,8 @@ def put(codes, at, value):
 
 
 def same_bits(a, b):
+    if a.numel() == 0:
+        return a.dtype == b.dtype and a.shape == b.shape
     return a.dtype == b.dtype and a.shape == b.shape and torch.equal(a.contiguous().view(torch.uint8), b.contiguous().view(torch.uint8))
 
 

@@ -470,3 +470,44 @@ def test_refusals_on_the_gpu():
     off = torch.empty(layer.k.numel() + 1, dtype=torch.uint8, device=DEV)[1:].view(layer.k.shape).view(E4M3)
     with pytest.raises(ValueError, match="16 bytes"):
         ops.store_blocks(torch.zeros(1, 1, 2, 3, 64, device=DEV).half(), layer._replace(k=off), slots)
+
+
+def test_native_host_paths_launch_the_same(monkeypatch):
+    """The calls through the native host paths and through Python: the same bits, the same refusals; what the paths do not take (queries
+    off 16 bytes, gaps between heads) goes the general way."""
+    from axonn_b200.ops import _lib
+
+    assert _lib.host() is not None
+    lengths, new = [40, 33], [3, 2]
+    i32 = lambda *v: torch.tensor(v, dtype=torch.int32, device=DEV)  # noqa: E731
+    cache, tables = make_cache(6, 2, 16, 64, E4M3), make_tables(lengths, 3, 16, 6).to(DEV)
+    torch.manual_seed(0)
+    qkv = torch.randn(2, 3, 2, 5, 64).bfloat16().to(DEV)
+    table = rope_table(48, 64).to(DEV)
+    logits = torch.randn(2, 3, 1000, device=DEV)
+    scores, done = -torch.rand(2, 3, device=DEV), torch.tensor([[True, False, False], [False, False, True]], device=DEV)
+
+    def run():
+        out = list(ops.plan_blocks(i32(37, 31), i32(*new), tables, i32(5, 4, 3, 2, 1, 0), i32(1), 3, 16))
+        layer = ops.BlockLayer(*_gpu(*cache))
+        out += [ops.store_blocks(qkv, layer, out[0], out[1], table), *layer]
+        assert ops.store_blocks(qkv, layer, out[0]) is None
+        for q in (qkv[:, :, :, :3], qkv[:, :, :, :3].reshape(2, 3, 6, 64), torch.cat([qkv, qkv], 3)[:, :, :, 0:6:2]):
+            out += [ops.cached_attention(q, layer, tables, i32(*lengths), i32(*new)), ops.cached_attention(q, layer, tables, i32(*lengths), None, 0.1)]
+        stacked = ops.BlockLayer(*(t[None] for t in layer))
+        out += [*ops.reorder_blocks(stacked, i32(0, 1, 0, 2).view(2, 2), i32(20, 20), i32(4, 5), i32(1, 0).view(1, 2)), *layer]
+        out += [*ops.beam_select(logits, scores)[:3], *ops.beam_select(logits, scores, done, 7)]
+        for error, call in ((ValueError, lambda: ops.cached_attention(qkv, layer, tables, i32(1))),
+                            (ValueError, lambda: ops.beam_select(logits, scores, done, 1000)),
+                            (ValueError, lambda: ops.beam_select(logits, scores, done)),
+                            (ValueError, lambda: ops.plan_blocks(i32(1), i32(1), tables, i32(0), i32(0), 1, 16)),
+                            (RuntimeError, lambda: ops.beam_select(logits.clone().requires_grad_(), scores)),
+                            (ValueError, lambda: ops.store_blocks(qkv, layer, out[0], None, table)),
+                            (ValueError, lambda: ops.reorder_blocks(layer, tables, i32(1, 2), i32(1, 2), i32(0, 0).view(1, 2)))):
+            with pytest.raises(error):
+                call()
+        return out
+    native = run()
+    monkeypatch.setattr(_lib, "_HOST", None)
+    plain = run()
+    assert len(native) == len(plain) and all(same_bits(a, b) for a, b in zip(native, plain))
