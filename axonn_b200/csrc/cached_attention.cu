@@ -27,7 +27,7 @@ constexpr int CA_TILE = 32;              // tokens of a tile: two halves of 16, 
 constexpr int CA_WARPS = 8;
 constexpr int CA_STAGES = 2;             // tiles of a warp's ring
 constexpr int CA_MAX_ROWS = 1024;        // requests of one launch: their tiles are counted in shared memory
-constexpr int CA_LEAST_TILES = 4;        // of a block's run: shorter ones are not worth their partial sums
+constexpr int CA_LEAST_TILES = 8;        // of a block's run: shorter ones are not worth their partial sums
 constexpr float CA_LOWEST = -3.0e38f;
 
 struct AttendArgs {
@@ -43,7 +43,6 @@ struct AttendArgs {
   int workers;                           // blocks of the grid
   int* before;                           // [R + 1] tiles of the requests before each
   float* part;                           // [2 * workers][columns][D + 4]: sums, then m, m', l
-  float* head;                           // the same of the first sequence of every warp: [workers * warps][columns][D + 4]
 };
 
 // The block that has unit u, of `active` blocks that share `units`; block w starts at units * w / active.
@@ -88,8 +87,13 @@ template <bool INT8> __device__ __forceinline__ void widen(uint32_t w, uint32_t&
         : "=r"(lo), "=r"(hi) : "r"(w));
   }
 }
-__device__ __forceinline__ void copy16(uint32_t to, const void* from) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to), "l"(from) : "memory");
+__device__ __forceinline__ void copy16(uint32_t to, const void* from, uint64_t policy) {
+  asm volatile("cp.async.cg.shared.global.L2::cache_hint [%0], [%1], 16, %2;" ::"r"(to), "l"(from), "l"(policy) : "memory");
+}
+__device__ __forceinline__ uint64_t evict_first() {
+  uint64_t p;
+  asm("createpolicy.fractional.L2::evict_first.b64 %0, 1.0;" : "=l"(p));
+  return p;
 }
 __device__ __forceinline__ void copy4(uint32_t to, const void* from) {
   asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(to), "l"(from) : "memory");
@@ -117,39 +121,72 @@ template <int D> struct Stage {
   }
 };
 
-// Shared memory of a warp: its ring, which the partial sums of its last sequence take the place of.  (Those of its first one go to
-// global memory where others follow: the ring is in use then.)
-template <int D, int NT> __host__ __device__ constexpr int warp_bytes() {
-  const int ring = CA_STAGES * Stage<D>::SIZE, parts = 8 * NT * (D + 4) * 4;
-  return ring > parts ? ring : parts;
+// Shared memory of a warp: its ring, which the partial sums of its last sequence take the place of, and those of its first one where
+// others follow.
+template <int D, int NT> __host__ __device__ constexpr int part_bytes() { return 8 * NT * (D + 4) * 4; }
+template <int D, int NT> __host__ __device__ constexpr int ring_bytes() {
+  const int ring = CA_STAGES * Stage<D>::SIZE;
+  return ring > part_bytes<D, NT>() ? ring : part_bytes<D, NT>();
 }
+template <int D, int NT> __host__ __device__ constexpr int warp_bytes() { return ring_bytes<D, NT>() + part_bytes<D, NT>(); }
 
-// What two partial results of a column add up to: references, denominator, sums.
+// The sum of partial results of a column: references, denominator, sums; lane i has values N i .. of the D = 32 N.
 template <int N> struct Partial {
   float m1 = CA_LOWEST, m2 = CA_LOWEST, l = 0.f, o[N] = {};
-  __device__ __forceinline__ void add(float other1, float other2, float other_l, const float (&f)[N]) {
-    const float n1 = fmaxf(m1, other1), n2 = fmaxf(m2, other2), a = exp2_fast(m2 - n2), b = exp2_fast(other2 - n2);
-    l = l * exp2_fast(m1 - n1) + other_l * exp2_fast(other1 - n1);
+  // Up to 32 more: lane x has what stands behind the sums of the x-th (`there`: it exists), row(x) are its sums, x < n.
+  template <typename Row> __device__ __forceinline__ void add(bool there, float x1, float x2, float xl, int n, const Row& row) {
+    const int lane = threadIdx.x & 31;
+    if (!there) { x1 = x2 = CA_LOWEST; xl = 0.f; }
+    float n1 = fmaxf(m1, x1), n2 = fmaxf(m2, x2);
 #pragma unroll
-    for (int i = 0; i < N; ++i) o[i] = o[i] * a + f[i] * b;
+    for (int i = 16; i > 0; i >>= 1) { n1 = fmaxf(n1, __shfl_xor_sync(0xffffffffu, n1, i)); n2 = fmaxf(n2, __shfl_xor_sync(0xffffffffu, n2, i)); }
+    const float weight = there ? exp2_fast(x2 - n2) : 0.f, old = exp2_fast(m2 - n2);
+    float sum = xl * exp2_fast(x1 - n1);
+#pragma unroll
+    for (int i = 16; i > 0; i >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, i);
+    l = l * exp2_fast(m1 - n1) + sum;
+#pragma unroll
+    for (int i = 0; i < N; ++i) o[i] *= old;
+#pragma unroll 4
+    for (int x = 0; x < n; ++x) {
+      const float w = __shfl_sync(0xffffffffu, weight, x);
+      if (!__shfl_sync(0xffffffffu, there, x)) continue;
+      const float* z = row(x) + lane * N;
+      float f[N];
+      if constexpr (N == 4) { const float4 u = *reinterpret_cast<const float4*>(z); f[0] = u.x; f[1] = u.y; f[2] = u.z; f[3] = u.w; }
+      else { const float2 u = *reinterpret_cast<const float2*>(z); f[0] = u.x; f[1] = u.y; }
+#pragma unroll
+      for (int i = 0; i < N; ++i) o[i] += w * f[i];
+    }
     m1 = n1; m2 = n2;
   }
+  __device__ __forceinline__ void store(float* z) const {
+    const int lane = threadIdx.x & 31;
+    if constexpr (N == 4) *reinterpret_cast<float4*>(z + lane * N) = make_float4(o[0], o[1], o[2], o[3]);
+    else *reinterpret_cast<float2*>(z + lane * N) = make_float2(o[0], o[1]);
+    if (lane == 0) *reinterpret_cast<float4*>(z + 32 * N) = make_float4(m1, m2, l, 0.f);
+  }
 };
+template <typename T> __device__ __forceinline__ uint32_t pack_row(float lo, float hi) {
+  if constexpr (__is_same(T, __half)) return pack_f16(lo, hi);
+  else { const __nv_bfloat162 b = __floats2bfloat162_rn(lo, hi); return *reinterpret_cast<const uint32_t*>(&b); }
+}
 template <typename T> __device__ __forceinline__ T* output_row(const AttendArgs& a, int r, int g, int c, int D) {
   return static_cast<T*>(a.out) + ((static_cast<size_t>(r) * a.S + c / a.P) * a.G * a.P + g * a.P + c % a.P) * D;
 }
-// Lane i has values i, i + 32 ...; a denominator of 0: nothing of what the column sees is there.
-template <typename T, int N> __device__ __forceinline__ void write_row(T* out, const Partial<N>& p, int lane) {
+// A denominator of 0: nothing of what the column sees is there.
+template <typename T, int N> __device__ __forceinline__ void write_row(T* out, const Partial<N>& p) {
   const float f = p.l != 0.f ? exp2_fast(p.m2 - p.m1) / p.l : 0.f;
+  float x[N];
 #pragma unroll
-  for (int i = 0; i < N; ++i) {
-    const float x = p.l != 0.f ? p.o[i] * f : 0.f;
-    if constexpr (__is_same(T, __half)) out[i * 32 + lane] = __float2half_rn(x);
-    else out[i * 32 + lane] = __float2bfloat16_rn(x);
-  }
+  for (int i = 0; i < N; ++i) x[i] = p.l != 0.f ? p.o[i] * f : 0.f;
+  uint32_t* to = reinterpret_cast<uint32_t*>(out) + (threadIdx.x & 31) * (N / 2);
+  if constexpr (N == 4) *reinterpret_cast<uint2*>(to) = make_uint2(pack_row<T>(x[0], x[1]), pack_row<T>(x[2], x[3]));
+  else *to = pack_row<T>(x[0], x[1]);
 }
 
-struct Open { int r, item, from_first, to_last; };      // item < 0: none
+// A sequence that a warp has not seen whole: its request, KV head and group of columns, and what of it was seen; ends < 0: none.
+struct Open { int r, g, group, ends; };      // ends: 1 the first tile, 2 the last one
 
 template <typename T, int D, bool INT8, int NT>
 __global__ void __launch_bounds__(32 * CA_WARPS, 1) attend_kernel(const AttendArgs a) {
@@ -187,13 +224,14 @@ __global__ void __launch_bounds__(32 * CA_WARPS, 1) attend_kernel(const AttendAr
     if (r0 < a.R && r0 + per >= a.R) { before[a.R] = at; if (blockIdx.x == 0) a.before[a.R] = at; }
     __syncthreads();
   }
+  const uint64_t policy = evict_first();     // read once: what else is in the L2, the code of the ends among it, stays there
   const int per_tile = a.G * a.groups;
   const long long units = static_cast<long long>(before[a.R]) * per_tile;
   const int active = active_blocks(units, a.workers);
   if (blockIdx.x >= active || units == 0) return;
   const long long block_begin = first_unit(units, blockIdx.x, active), block_units = first_unit(units, blockIdx.x + 1, active) - block_begin;
   const long long begin = block_begin + block_units * wid / CA_WARPS, end = block_begin + block_units * (wid + 1) / CA_WARPS;
-  if (lane < 2) open[wid][lane].item = -1;
+  if (lane < 2) open[wid][lane].ends = -1;
   __syncwarp();
 
   int r = 0;
@@ -202,7 +240,7 @@ __global__ void __launch_bounds__(32 * CA_WARPS, 1) attend_kernel(const AttendAr
     while (before[r + 1] <= u / per_tile) ++r;
     const int tiles = before[r + 1] - before[r];
     const long long within = u - static_cast<long long>(before[r]) * per_tile;
-    const int item = static_cast<int>(within / tiles), g = item / a.groups, group = item % a.groups;
+    const int item = static_cast<int>(within / tiles), g = a.groups == 1 ? item : item / a.groups, group = item - g * a.groups;
     const int t0 = static_cast<int>(within % tiles), t1 = static_cast<int>(min(static_cast<long long>(tiles), t0 + (end - u)));
     const int length = lengths[r], fresh = a.fresh ? min(max(a.fresh[r], 0), a.S) : a.S;
     const int col0 = group * COLS, cols = min(a.S * a.P - col0, COLS);
@@ -230,8 +268,8 @@ __global__ void __launch_bounds__(32 * CA_WARPS, 1) attend_kernel(const AttendAr
 #pragma unroll
           for (int x = 0; x < D / 32; ++x) {
             const int i = x * 32 + lane, row = 16 * h + i / (D / 16), c = i % (D / 16);
-            copy16(to + Stage<D>::key_word(row, c) * 16, a.k + from + i * 16);
-            copy16(to + Stage<D>::BYTES + Stage<D>::value_word(row, c) * 16, a.v + from + i * 16);
+            copy16(to + Stage<D>::key_word(row, c) * 16, a.k + from + i * 16, policy);
+            copy16(to + Stage<D>::BYTES + Stage<D>::value_word(row, c) * 16, a.v + from + i * 16, policy);
           }
         }
       }
@@ -472,10 +510,9 @@ __global__ void __launch_bounds__(32 * CA_WARPS, 1) attend_kernel(const AttendAr
     const int slot = u + (t1 - t0) < end ? 0 : 1;      // the last of this warp's, or its first of several
     if (!whole) {
       __syncwarp();                          // the ring has been read: the sums take its place
-      if (lane == 0) open[wid][slot] = Open{r, item, t0 == 0, t1 == tiles};
+      if (lane == 0) open[wid][slot] = Open{r, g, group, (t0 == 0) + 2 * (t1 == tiles)};
     }
-    float* parts = slot == 0 ? a.head + (static_cast<size_t>(blockIdx.x) * CA_WARPS + wid) * COLS * (D + 4)
-                             : reinterpret_cast<float*>(ring + wid * warp_bytes<D, NT>());
+    float* parts = reinterpret_cast<float*>(mine + (slot == 0 ? ring_bytes<D, NT>() : 0));
 #pragma unroll
     for (int n = 0; n < NT; ++n)
 #pragma unroll
@@ -496,8 +533,7 @@ __global__ void __launch_bounds__(32 * CA_WARPS, 1) attend_kernel(const AttendAr
             for (int y = 0; y < 4; ++y) {
               const float* z = acc[n][x * 4 + y];
               const float lo = total != 0.f ? z[h] * f : 0.f, hi = total != 0.f ? z[h + 2] * f : 0.f;
-              if constexpr (__is_same(T, __half)) w[y] = pack_f16(lo, hi);
-              else { const __nv_bfloat162 b = __floats2bfloat162_rn(lo, hi); w[y] = *reinterpret_cast<const uint32_t*>(&b); }
+              w[y] = pack_row<T>(lo, hi);
             }
             *reinterpret_cast<uint4*>(o + x * 8) = make_uint4(w[0], w[1], w[2], w[3]);
           }
@@ -515,50 +551,53 @@ __global__ void __launch_bounds__(32 * CA_WARPS, 1) attend_kernel(const AttendAr
 
   // Sequences that several warps of the block share: put together here, finished where the block has seen them whole.
   __syncthreads();
-  const Open* all_open = &open[0][0];
-  for (int i = 0; i < 2 * CA_WARPS;) {
-    const Open first = all_open[i];
-    if (first.item < 0) { ++i; continue; }
-    int last = i, next = i + 1;
-    for (; next < 2 * CA_WARPS && (all_open[next].item < 0 || (all_open[next].item == first.item && all_open[next].r == first.r)); ++next)
-      if (all_open[next].item >= 0) last = next;
-    const bool whole = first.from_first && all_open[last].to_last;
-    const int g = first.item / a.groups, col0 = first.item % a.groups * COLS, cols = min(a.S * a.P - col0, COLS);
-    // the partial result of a sequence that began in another block, or at this block's first unit, is the block's first
-    const long long from = static_cast<long long>(before[first.r]) * per_tile +
-                           static_cast<long long>(first.item) * (before[first.r + 1] - before[first.r]);
-    const size_t slot = 2 * static_cast<size_t>(blockIdx.x) + (from <= block_begin ? 0 : 1);
-    for (int cc = wid; cc < cols; cc += CA_WARPS) {
+  // lane x looks at the x-th; a sequence starts where it is not that of the one before
+  Open mine_open = {0, 0, 0, -1};
+  if (lane < 2 * CA_WARPS) mine_open = (&open[0][0])[lane];
+  const unsigned some = __ballot_sync(0xffffffffu, mine_open.ends >= 0), earlier = some & ((1u << lane) - 1u);
+  const int prior = earlier ? 31 - __clz(earlier) : 0;
+  const int prior_r = __shfl_sync(0xffffffffu, mine_open.r, prior), prior_g = __shfl_sync(0xffffffffu, mine_open.g, prior);
+  const int prior_group = __shfl_sync(0xffffffffu, mine_open.group, prior);
+  const bool same = earlier && prior_r == mine_open.r && prior_g == mine_open.g && prior_group == mine_open.group;
+  unsigned starts = __ballot_sync(0xffffffffu, mine_open.ends >= 0 && !same);
+  int turn = 0;                              // columns of all those sequences, a warp for each in turn
+  while (starts) {
+    const int i = __ffs(starts) - 1;
+    starts &= starts - 1;
+    const unsigned here = some & (starts ? (1u << (__ffs(starts) - 1)) - 1u : 0xffffffffu) & ~((1u << i) - 1u);
+    const int last = 31 - __clz(here), first_r = __shfl_sync(0xffffffffu, mine_open.r, i), g = __shfl_sync(0xffffffffu, mine_open.g, i);
+    const int group = __shfl_sync(0xffffffffu, mine_open.group, i);
+    const int first_ends = __shfl_sync(0xffffffffu, mine_open.ends, i), last_ends = __shfl_sync(0xffffffffu, mine_open.ends, last);
+    const bool whole = (first_ends & 1) && (last_ends & 2);
+    const int col0 = group * COLS, cols = min(a.S * a.P - col0, COLS);
+    const int skip = (wid - turn % CA_WARPS + CA_WARPS) % CA_WARPS;
+    turn += cols;
+    for (int cc = skip; cc < cols; cc += CA_WARPS) {
       Partial<D / 32> p;
-      for (int x = i; x <= last; ++x) {
-        if (all_open[x].item < 0) continue;
-        const float* z = (x & 1 ? reinterpret_cast<const float*>(ring + x / 2 * warp_bytes<D, NT>())
-                                : a.head + (static_cast<size_t>(blockIdx.x) * CA_WARPS + x / 2) * COLS * (D + 4)) + cc * (D + 4);
-        float f[D / 32];
-#pragma unroll
-        for (int y = 0; y < D / 32; ++y) f[y] = z[y * 32 + lane];
-        p.add(z[D], z[D + 1], z[D + 2], f);
-      }
-      if (whole) write_row(output_row<T>(a, first.r, g, col0 + cc, D), p, lane);
-      else {
-        float* o = a.part + (slot * COLS + cc) * (D + 4);
-#pragma unroll
-        for (int y = 0; y < D / 32; ++y) o[y * 32 + lane] = p.o[y];
-        if (lane == 0) *reinterpret_cast<float4*>(o + D) = make_float4(p.m1, p.m2, p.l, 0.f);
-      }
+      auto row = [&](int x) {
+        x += i;
+        return reinterpret_cast<const float*>(ring + x / 2 * warp_bytes<D, NT>() + (x & 1 ? 0 : ring_bytes<D, NT>())) + cc * (D + 4);
+      };
+      const int n = last - i + 1;
+      const bool there = lane < n && (here >> (i + lane) & 1u);
+      const float4 stat = there ? *reinterpret_cast<const float4*>(row(lane) + D) : make_float4(0.f, 0.f, 0.f, 0.f);
+      p.add(there, stat.x, stat.y, stat.z, n, row);
+      if (whole) { write_row(output_row<T>(a, first_r, g, col0 + cc, D), p); continue; }
+      // the partial result of a sequence that began in another block, or at this block's first unit, is the block's first
+      const long long from = static_cast<long long>(before[first_r]) * per_tile +
+                             static_cast<long long>(g * a.groups + group) * (before[first_r + 1] - before[first_r]);
+      p.store(a.part + ((2 * static_cast<size_t>(blockIdx.x) + (from <= block_begin ? 0 : 1)) * COLS + cc) * (D + 4));
     }
-    i = next;
   }
 }
 
-constexpr int MERGE_WARPS = 8, MERGE_AT_ONCE = 4;
+constexpr int MERGE_WARPS = 8;
 
 // Adds up the partial sums of the sequences that several blocks share, in the order of their tokens, and writes zeros for requests
 // without tokens.  One block per sequence (request, KV head, group of columns); its warps share columns and parts.
 template <typename T, int D>
 __global__ void __launch_bounds__(32 * MERGE_WARPS) attend_merge_kernel(const AttendArgs a, int columns) {
-  constexpr int PER = D / 32;
-  __shared__ float sums[MERGE_WARPS][D], stats[MERGE_WARPS][3];
+  __shared__ __align__(16) float sums[MERGE_WARPS][D + 4];
   pdl_launch_next();
   pdl_wait();
   const int lane = threadIdx.x & 31, w = threadIdx.x >> 5, per_tile = a.G * a.groups;
@@ -575,43 +614,33 @@ __global__ void __launch_bounds__(32 * MERGE_WARPS) attend_merge_kernel(const At
   }
   // `share` warps per column, each with a run of the parts
   int share = 1;
-  while (2 * share * cols <= MERGE_WARPS && share * MERGE_AT_ONCE < parts) share *= 2;
+  while (2 * share * cols <= MERGE_WARPS && 4 * share < parts) share *= 2;
   const int per = (parts + share - 1) / share, first_slot = tiles && from != first_unit(units, w0, active);
   for (int c0 = 0; c0 < cols; c0 += MERGE_WARPS / share) {
     const int cc = c0 + w / share, mine = w % share, end = min(parts, mine * per + per);
-    Partial<PER> p;
+    Partial<D / 32> p;
     if (cc < cols)
-      for (int x0 = mine * per; x0 < end; x0 += MERGE_AT_ONCE) {
-        float4 st[MERGE_AT_ONCE];
-        float f[MERGE_AT_ONCE][PER];
-#pragma unroll
-        for (int y = 0; y < MERGE_AT_ONCE; ++y)
-          if (x0 + y < end) {
-            const size_t slot = 2 * static_cast<size_t>(w0 + x0 + y) + (x0 + y == 0 ? first_slot : 0);
-            const float* z = a.part + (slot * columns + cc) * (D + 4);
-            st[y] = *reinterpret_cast<const float4*>(z + D);
-#pragma unroll
-            for (int i = 0; i < PER; ++i) f[y][i] = z[i * 32 + lane];
-          }
-#pragma unroll
-        for (int y = 0; y < MERGE_AT_ONCE; ++y)
-          if (x0 + y < end) p.add(st[y].x, st[y].y, st[y].z, f[y]);
+      for (int x0 = mine * per; x0 < end; x0 += 32) {
+        auto row = [&](int x) {
+          x += x0;
+          return a.part + ((2 * static_cast<size_t>(w0 + x) + (x == 0 ? first_slot : 0)) * columns + cc) * (D + 4);
+        };
+        const int n = min(32, end - x0);
+        const float4 stat = lane < n ? *reinterpret_cast<const float4*>(row(lane) + D) : make_float4(0.f, 0.f, 0.f, 0.f);
+        p.add(lane < n, stat.x, stat.y, stat.z, n, row);
       }
     if (share > 1) {
       __syncthreads();
-#pragma unroll
-      for (int i = 0; i < PER; ++i) sums[w][i * 32 + lane] = p.o[i];
-      if (lane == 0) { stats[w][0] = p.m1; stats[w][1] = p.m2; stats[w][2] = p.l; }
+      p.store(sums[w]);
       __syncthreads();
-      if (mine == 0)
-        for (int y = w + 1; y < w + share; ++y) {
-          float f[PER];
-#pragma unroll
-          for (int i = 0; i < PER; ++i) f[i] = sums[y][i * 32 + lane];
-          p.add(stats[y][0], stats[y][1], stats[y][2], f);
-        }
+      if (mine == 0 && cc < cols) {
+        auto row = [&](int x) { return sums[w + x]; };
+        p = Partial<D / 32>();
+        const float4 stat = lane < share ? *reinterpret_cast<const float4*>(row(lane) + D) : make_float4(0.f, 0.f, 0.f, 0.f);
+        p.add(lane < share, stat.x, stat.y, stat.z, share, row);
+      }
     }
-    if (mine == 0 && cc < cols) write_row(output_row<T>(a, r, g, col0 + cc, D), p, lane);
+    if (mine == 0 && cc < cols) write_row(output_row<T>(a, r, g, col0 + cc, D), p);
   }
 }
 
@@ -647,7 +676,7 @@ using namespace axb;
 // 32-bit words of the workspace: the tile counts, then two partial results per block
 extern "C" long long axb_cached_attention_words(int R, int S, int P, int D) {
   const int columns = attend_columns(S * P);
-  return (R + 1 + 3) / 4 * 4 + (2ll + CA_WARPS) * sm_count_current() * columns * (D + 4);
+  return (R + 1 + 3) / 4 * 4 + 2ll * sm_count_current() * columns * (D + 4);
 }
 
 extern "C" int axb_cached_attention(const void* q, long long q_row, long long q_token, long long q_group, const void* k, const void* v,
@@ -667,7 +696,7 @@ extern "C" int axb_cached_attention(const void* q, long long q_row, long long q_
   }
   const int columns = attend_columns(S * P), groups = (S * P + columns - 1) / columns, blocks = sm_count_current();
   AttendArgs a{q, q_row, q_token, q_group, out, (const uint8_t*)k, (const uint8_t*)v, ks, vs, tables, lengths, fresh, R, S, G, P, W, N, shift,
-               groups, scale * 1.4426950408889634f, blocks, (int*)work, nullptr, nullptr};
+               groups, scale * 1.4426950408889634f, blocks, (int*)work, nullptr};
   for (int r0 = 0; r0 < R; r0 += CA_MAX_ROWS) {
     a.R = R - r0 < CA_MAX_ROWS ? R - r0 : CA_MAX_ROWS;
     a.q = static_cast<const char*>(q) + r0 * q_row * 2;
@@ -676,7 +705,6 @@ extern "C" int axb_cached_attention(const void* q, long long q_row, long long q_
     a.lengths = lengths + r0;
     a.fresh = fresh ? fresh + r0 : nullptr;
     a.part = reinterpret_cast<float*>(a.before + (a.R + 1 + 3) / 4 * 4);
-    a.head = a.part + 2ll * blocks * columns * (D + 4);
     const int st = dtype == 0 ? launch_attend<__nv_bfloat16>(a, D, int8 != 0, columns, (cudaStream_t)stream)
                               : launch_attend<__half>(a, D, int8 != 0, columns, (cudaStream_t)stream);
     if (st) return st;
