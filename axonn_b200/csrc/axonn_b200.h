@@ -329,7 +329,7 @@ int axb_reorder_blocks(void* k, void* v, float* ks, float* vs, const int* tables
                        int row_bytes, void* stream);
 /* attention of q [R, S, G, P, D] (strides in elements), whose last fresh[r] (NULL: S) tokens are the last of lengths[r], into out
  * [R, S, G * P, D]; work: axb_cached_attention_words() 32-bit words, 16-byte aligned, of this call alone */
-long long axb_cached_attention_words(int R, int S, int P, int D);
+long long axb_cached_attention_words(int R, int S, int G, int P, int D);
 int axb_cached_attention(const void* q, long long q_row, long long q_token, long long q_group, const void* k, const void* v,
                          const float* ks, const float* vs, const int* tables, const int* lengths, const int* fresh, void* out, void* work,
                          int R, int S, int G, int P, int D, int W, int N, int block_tokens, float scale, int dtype, int int8, void* stream);

@@ -28,6 +28,7 @@ constexpr int CA_WARPS = 8;
 constexpr int CA_STAGES = 2;             // tiles of a warp's ring
 constexpr int CA_MAX_ROWS = 1024;        // requests of one launch: their tiles are counted in shared memory
 constexpr int CA_LEAST_TILES = 8;        // of a block's run: shorter ones are not worth their partial sums
+constexpr int CA_START = 2;              // what the start of a sequence costs a warp, in tiles
 constexpr float CA_LOWEST = -3.0e38f;
 
 struct AttendArgs {
@@ -41,20 +42,19 @@ struct AttendArgs {
   int groups;                            // of query columns
   float scale_log2;
   int workers;                           // blocks of the grid
-  int* before;                           // [R + 1] tiles of the requests before each
+  int* before;                           // [R + 1] units of the requests before each, per KV head and group
+  int2* ends;                            // of every sequence: the slot of its first partial result (-1: finished), the block of its last
   float* part;                           // [2 * workers][columns][D + 4]: sums, then m, m', l
 };
 
-// The block that has unit u, of `active` blocks that share `units`; block w starts at units * w / active.
+// The units of a sequence are its tiles, after CA_START that stand for its start.  `active` blocks share all units; block w starts at
+// units * w / active.
+__device__ __forceinline__ int sequence_units(int length) { return length ? (length + CA_TILE - 1) / CA_TILE + CA_START : 0; }
 __device__ __forceinline__ int active_blocks(long long units, int workers) {
   const long long want = (units + CA_LEAST_TILES - 1) / CA_LEAST_TILES;
   return static_cast<int>(want < workers ? (want < 1 ? 1 : want) : workers);
 }
 __device__ __forceinline__ long long first_unit(long long units, int w, int active) { return units * w / active; }
-__device__ __forceinline__ int owner(long long u, long long units, int active) {
-  return static_cast<int>(((u + 1) * active - 1) / units);
-}
-
 __device__ __forceinline__ float exp2_fast(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
@@ -191,7 +191,7 @@ struct Open { int r, g, group, ends; };      // ends: 1 the first tile, 2 the la
 template <typename T, int D, bool INT8, int NT>
 __global__ void __launch_bounds__(32 * CA_WARPS, 1) attend_kernel(const AttendArgs a) {
   constexpr int KC = D / 64, MT = D / 16, VW = D / 32, COLS = 8 * NT;
-  extern __shared__ __align__(16) uint8_t ring[];      // of every warp; then the tiles of the requests before each, [R + 1], and lengths
+  extern __shared__ __align__(16) uint8_t ring[];      // of every warp; then the units of the requests before each, [R + 1], and lengths
   int* before = reinterpret_cast<int*>(ring + CA_WARPS * warp_bytes<D, NT>());
   int* lengths = before + a.R + 1;
   __shared__ int sums[CA_WARPS];
@@ -201,13 +201,13 @@ __global__ void __launch_bounds__(32 * CA_WARPS, 1) attend_kernel(const AttendAr
   const int tid = threadIdx.x, lane = tid & 31, wid = tid >> 5, g8 = lane >> 2, j4 = lane & 3, BT = 1 << a.shift;
   const int most = min(static_cast<long long>(a.W) << a.shift, 0x7fffff00ll);
 
-  // tiles of the requests before each: one scan per block of the grid
+  // units of the requests before each: one scan per block of the grid
   {
     const int per = (a.R + 32 * CA_WARPS - 1) / (32 * CA_WARPS), r0 = tid * per;
     int mine = 0;
     for (int r = r0; r < min(r0 + per, a.R); ++r) {
       lengths[r] = min(max(a.lengths[r], 0), most);
-      mine += (lengths[r] + CA_TILE - 1) / CA_TILE;
+      mine += sequence_units(lengths[r]);
     }
     int incl = mine;
 #pragma unroll
@@ -219,7 +219,7 @@ __global__ void __launch_bounds__(32 * CA_WARPS, 1) attend_kernel(const AttendAr
     for (int r = r0; r < min(r0 + per, a.R); ++r) {
       before[r] = at;
       if (blockIdx.x == 0) a.before[r] = at;
-      at += (lengths[r] + CA_TILE - 1) / CA_TILE;
+      at += sequence_units(lengths[r]);
     }
     if (r0 < a.R && r0 + per >= a.R) { before[a.R] = at; if (blockIdx.x == 0) a.before[a.R] = at; }
     __syncthreads();
@@ -229,8 +229,8 @@ __global__ void __launch_bounds__(32 * CA_WARPS, 1) attend_kernel(const AttendAr
   const long long units = static_cast<long long>(before[a.R]) * per_tile;
   const int active = active_blocks(units, a.workers);
   if (blockIdx.x >= active || units == 0) return;
-  const long long block_begin = first_unit(units, blockIdx.x, active), block_units = first_unit(units, blockIdx.x + 1, active) - block_begin;
-  const long long begin = block_begin + block_units * wid / CA_WARPS, end = block_begin + block_units * (wid + 1) / CA_WARPS;
+  const long long first = first_unit(units, blockIdx.x, active), many = first_unit(units, blockIdx.x + 1, active) - first;
+  const long long begin = first + many * wid / CA_WARPS, end = first + many * (wid + 1) / CA_WARPS;
   if (lane < 2) open[wid][lane].ends = -1;
   __syncwarp();
 
@@ -238,10 +238,14 @@ __global__ void __launch_bounds__(32 * CA_WARPS, 1) attend_kernel(const AttendAr
   for (int hi = a.R; hi - r > 1;) { const int mid = (r + hi) / 2; if (before[mid] <= begin / per_tile) r = mid; else hi = mid; }
   for (long long u = begin; u < end;) {
     while (before[r + 1] <= u / per_tile) ++r;
-    const int tiles = before[r + 1] - before[r];
+    const int per_sequence = before[r + 1] - before[r], tiles = per_sequence - CA_START;
     const long long within = u - static_cast<long long>(before[r]) * per_tile;
-    const int item = static_cast<int>(within / tiles), g = a.groups == 1 ? item : item / a.groups, group = item - g * a.groups;
-    const int t0 = static_cast<int>(within % tiles), t1 = static_cast<int>(min(static_cast<long long>(tiles), t0 + (end - u)));
+    const int item = static_cast<int>(within / per_sequence), g = a.groups == 1 ? item : item / a.groups, group = item - g * a.groups;
+    const int x0 = static_cast<int>(within - static_cast<long long>(item) * per_sequence);
+    const int x1 = static_cast<int>(min(static_cast<long long>(per_sequence), x0 + (end - u)));
+    u += x1 - x0;
+    const int t0 = max(x0 - CA_START, 0), t1 = x1 - CA_START;
+    if (t1 <= t0) continue;
     const int length = lengths[r], fresh = a.fresh ? min(max(a.fresh[r], 0), a.S) : a.S;
     const int col0 = group * COLS, cols = min(a.S * a.P - col0, COLS);
 
@@ -507,7 +511,8 @@ __global__ void __launch_bounds__(32 * CA_WARPS, 1) attend_kernel(const AttendAr
 
     // thread (g8, j4) has values g8 * D / 8 .. of columns 2 j4 and 2 j4 + 1
     const bool whole = t0 == 0 && t1 == tiles;
-    const int slot = u + (t1 - t0) < end ? 0 : 1;      // the last of this warp's, or its first of several
+    const int slot = u < end ? 0 : 1;        // the last of this warp's, or its first of several
+    if (whole && lane == 0) a.ends[static_cast<size_t>(r) * per_tile + item] = make_int2(-1, 0);
     if (!whole) {
       __syncwarp();                          // the ring has been read: the sums take its place
       if (lane == 0) open[wid][slot] = Open{r, g, group, (t0 == 0) + 2 * (t1 == tiles)};
@@ -546,7 +551,6 @@ __global__ void __launch_bounds__(32 * CA_WARPS, 1) attend_kernel(const AttendAr
           if (g8 == 0) *reinterpret_cast<float4*>(o + D) = make_float4(m1[n][h], m2[n][h], total, 0.f);
         }
       }
-    u += t1 - t0;
   }
 
   // Sequences that several warps of the block share: put together here, finished where the block has seen them whole.
@@ -571,6 +575,13 @@ __global__ void __launch_bounds__(32 * CA_WARPS, 1) attend_kernel(const AttendAr
     const bool whole = (first_ends & 1) && (last_ends & 2);
     const int col0 = group * COLS, cols = min(a.S * a.P - col0, COLS);
     const int skip = (wid - turn % CA_WARPS + CA_WARPS) % CA_WARPS;
+    // a sequence that began in another block is this block's first
+    const size_t slot = 2 * static_cast<size_t>(blockIdx.x) + (first_ends & 1);
+    if (threadIdx.x == 0) {
+      int2* ends = a.ends + static_cast<size_t>(first_r) * per_tile + g * a.groups + group;
+      if (first_ends & 1) ends->x = whole ? -1 : static_cast<int>(slot);
+      if (last_ends & 2) ends->y = blockIdx.x;
+    }
     turn += cols;
     for (int cc = skip; cc < cols; cc += CA_WARPS) {
       Partial<D / 32> p;
@@ -583,10 +594,7 @@ __global__ void __launch_bounds__(32 * CA_WARPS, 1) attend_kernel(const AttendAr
       const float4 stat = there ? *reinterpret_cast<const float4*>(row(lane) + D) : make_float4(0.f, 0.f, 0.f, 0.f);
       p.add(there, stat.x, stat.y, stat.z, n, row);
       if (whole) { write_row(output_row<T>(a, first_r, g, col0 + cc, D), p); continue; }
-      // the partial result of a sequence that began in another block, or at this block's first unit, is the block's first
-      const long long from = static_cast<long long>(before[first_r]) * per_tile +
-                             static_cast<long long>(g * a.groups + group) * (before[first_r + 1] - before[first_r]);
-      p.store(a.part + ((2 * static_cast<size_t>(blockIdx.x) + (from <= block_begin ? 0 : 1)) * COLS + cc) * (D + 4));
+      p.store(a.part + (slot * COLS + cc) * (D + 4));
     }
   }
 }
@@ -601,21 +609,16 @@ __global__ void __launch_bounds__(32 * MERGE_WARPS) attend_merge_kernel(const At
   pdl_launch_next();
   pdl_wait();
   const int lane = threadIdx.x & 31, w = threadIdx.x >> 5, per_tile = a.G * a.groups;
-  const int r = blockIdx.x / per_tile, item = blockIdx.x % per_tile, g = item / a.groups;
-  const int tiles = a.before[r + 1] - a.before[r], col0 = item % a.groups * columns, cols = min(a.S * a.P - col0, columns);
-  const long long units = static_cast<long long>(a.before[a.R]) * per_tile;
-  const int active = active_blocks(units, a.workers);
-  const long long from = static_cast<long long>(a.before[r]) * per_tile + static_cast<long long>(item) * tiles;
-  int w0 = 0, parts = 0;
-  if (tiles) {
-    w0 = owner(from, units, active);
-    parts = owner(from + tiles - 1, units, active) - w0 + 1;
-    if (parts == 1) return;
-  }
+  const int r = blockIdx.x / per_tile, item = blockIdx.x - r * per_tile, g = a.groups == 1 ? item : item / a.groups;
+  const int2 ends = a.ends[blockIdx.x];
+  const bool any = a.before[r + 1] != a.before[r];
+  if (any && ends.x < 0) return;
+  const int col0 = (item - g * a.groups) * columns, cols = min(a.S * a.P - col0, columns);
+  const int parts = any ? ends.y - ends.x / 2 + 1 : 0;
   // `share` warps per column, each with a run of the parts
   int share = 1;
   while (2 * share * cols <= MERGE_WARPS && 4 * share < parts) share *= 2;
-  const int per = (parts + share - 1) / share, first_slot = tiles && from != first_unit(units, w0, active);
+  const int per = (parts + share - 1) / share;
   for (int c0 = 0; c0 < cols; c0 += MERGE_WARPS / share) {
     const int cc = c0 + w / share, mine = w % share, end = min(parts, mine * per + per);
     Partial<D / 32> p;
@@ -623,7 +626,7 @@ __global__ void __launch_bounds__(32 * MERGE_WARPS) attend_merge_kernel(const At
       for (int x0 = mine * per; x0 < end; x0 += 32) {
         auto row = [&](int x) {
           x += x0;
-          return a.part + ((2 * static_cast<size_t>(w0 + x) + (x == 0 ? first_slot : 0)) * columns + cc) * (D + 4);
+          return a.part + (static_cast<size_t>(x == 0 ? ends.x : (ends.x & ~1) + 2 * x) * columns + cc) * (D + 4);
         };
         const int n = min(32, end - x0);
         const float4 stat = lane < n ? *reinterpret_cast<const float4*>(row(lane) + D) : make_float4(0.f, 0.f, 0.f, 0.f);
@@ -645,6 +648,10 @@ __global__ void __launch_bounds__(32 * MERGE_WARPS) attend_merge_kernel(const At
 }
 
 static int attend_columns(int queries) { return queries <= 8 ? 8 : 16; }
+static long long before_words(int rows) { return (rows + 1 + 3) / 4 * 4; }
+static long long ends_words(int rows, int G, int queries) {
+  return (2ll * rows * G * ((queries + attend_columns(queries) - 1) / attend_columns(queries)) + 3) / 4 * 4;
+}
 
 template <typename T, int D, bool INT8, int NT>
 static int launch_attend(const AttendArgs& a, cudaStream_t stream) {
@@ -673,10 +680,10 @@ template <typename T> static int launch_attend(const AttendArgs& a, int D, bool 
 
 using namespace axb;
 
-// 32-bit words of the workspace: the tile counts, then two partial results per block
-extern "C" long long axb_cached_attention_words(int R, int S, int P, int D) {
-  const int columns = attend_columns(S * P);
-  return (R + 1 + 3) / 4 * 4 + 2ll * sm_count_current() * columns * (D + 4);
+// 32-bit words of the workspace: the counts of units, the sequences' ends, two partial results per block
+extern "C" long long axb_cached_attention_words(int R, int S, int G, int P, int D) {
+  const int columns = attend_columns(S * P), rows = R < CA_MAX_ROWS ? R : CA_MAX_ROWS;
+  return before_words(rows) + ends_words(rows, G, S * P) + 2ll * sm_count_current() * columns * (D + 4);
 }
 
 extern "C" int axb_cached_attention(const void* q, long long q_row, long long q_token, long long q_group, const void* k, const void* v,
@@ -696,7 +703,7 @@ extern "C" int axb_cached_attention(const void* q, long long q_row, long long q_
   }
   const int columns = attend_columns(S * P), groups = (S * P + columns - 1) / columns, blocks = sm_count_current();
   AttendArgs a{q, q_row, q_token, q_group, out, (const uint8_t*)k, (const uint8_t*)v, ks, vs, tables, lengths, fresh, R, S, G, P, W, N, shift,
-               groups, scale * 1.4426950408889634f, blocks, (int*)work, nullptr};
+               groups, scale * 1.4426950408889634f, blocks, (int*)work, nullptr, nullptr};
   for (int r0 = 0; r0 < R; r0 += CA_MAX_ROWS) {
     a.R = R - r0 < CA_MAX_ROWS ? R - r0 : CA_MAX_ROWS;
     a.q = static_cast<const char*>(q) + r0 * q_row * 2;
@@ -704,7 +711,8 @@ extern "C" int axb_cached_attention(const void* q, long long q_row, long long q_
     a.tables = tables + static_cast<size_t>(r0) * W;
     a.lengths = lengths + r0;
     a.fresh = fresh ? fresh + r0 : nullptr;
-    a.part = reinterpret_cast<float*>(a.before + (a.R + 1 + 3) / 4 * 4);
+    a.ends = reinterpret_cast<int2*>(a.before + before_words(a.R));
+    a.part = reinterpret_cast<float*>(a.before + before_words(a.R) + ends_words(a.R, G, S * P));
     const int st = dtype == 0 ? launch_attend<__nv_bfloat16>(a, D, int8 != 0, columns, (cudaStream_t)stream)
                               : launch_attend<__half>(a, D, int8 != 0, columns, (cudaStream_t)stream);
     if (st) return st;

@@ -408,7 +408,7 @@ PyObject* py_cached_attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
   {
     NoGil no_gil;
     out = at::empty({R, S, G * P, D}, q.options());
-    const Tensor work = at::empty({attention_words(static_cast<int>(R), static_cast<int>(S), static_cast<int>(P), static_cast<int>(D))},
+    const Tensor work = at::empty({attention_words(static_cast<int>(R), static_cast<int>(S), static_cast<int>(G), static_cast<int>(P), static_cast<int>(D))},
                                   q.options().dtype(at::kFloat));
     check(cached_attention(q.data_ptr(), strides[0], strides[1], strides[2], k.data_ptr(), v.data_ptr(), ks.data_ptr<float>(), vs.data_ptr<float>(),
                            tables.data_ptr<int>(), lengths.data_ptr<int>(), fresh.defined() ? fresh.data_ptr<int>() : nullptr, out.data_ptr(),

@@ -85,7 +85,7 @@ _SIGNATURES = {
     "axb_plan_blocks": "ppppppppp" "iiiii" "p",
     "axb_store_blocks": "p" "lll" "pppp" "pppp" "iiiiiiiiii" "p",
     "axb_reorder_blocks": "pppp" "pppp" "ppp" "iiiiiiii" "p",
-    "axb_cached_attention_words": "iiii",
+    "axb_cached_attention_words": "iiiii",
     "axb_cached_attention": "p" "lll" "pppp" "ppp" "pp" "iiiiiiii" "f" "ii" "p",
     "axb_beam_select_words": "iiii",
     "axb_beam_select": "ppp" "i" "ppppp" "iiii" "p",

@@ -320,7 +320,7 @@ def cached_attention(q, layer, tables, lengths, new=None, scale=None):
         strides = (S * H * D, H * D, P * D)
     out = torch.empty(R, S, H, D, dtype=q.dtype, device=dev)
     L = _lib.lib()
-    work = torch.empty(L.axb_cached_attention_words(R, S, P, D), dtype=torch.float32, device=dev)
+    work = torch.empty(L.axb_cached_attention_words(R, S, G, P, D), dtype=torch.float32, device=dev)
     st = L.axb_cached_attention(q.data_ptr(), *strides, k.data_ptr(), v.data_ptr(), ks.data_ptr(), vs.data_ptr(), tables.data_ptr(),
                                 lengths.data_ptr(), _lib.addr(new), out.data_ptr(), work.data_ptr(), R, S, G, P, D, tables.shape[1], N,
                                 BT, scale, _HALF[q.dtype], int(k.dtype == torch.int8), _lib.stream())
