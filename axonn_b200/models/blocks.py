@@ -127,11 +127,15 @@ class ParallelAttention(nn.Module):
         self.proj = Linear(n_heads * self.head_dim, hidden, bias=bias, expert_mode=True, transpose=True,
                            init_method=lambda w: nn.init.normal_(w, std=out_init_std or init_std), dtype=dtype)
 
-    def forward(self, x):
+    def forward(self, x, cache=None):
+        """``cache``: this layer's part of a ``BlockCache`` (``cache.layer(i)``), in which the keys and values of ``x`` are stored and to
+        whose tokens its queries attend."""
         B, S, _ = x.shape
         D, G, qpk = self.head_dim, self.groups_l, self.q_per_kv
         qkv = self.qkv(x).view(B, S, G, qpk + 2, D)
-        if self.sequence_group is not None:
+        if cache is not None:
+            o = self._cached(qkv, cache)
+        elif self.sequence_group is not None:
             # x holds a slice of every sequence: trade it for whole sequences of a share of the heads, attend,
             # trade back (rotary embedding in between, on whole sequences)
             from ..parallel.sequence import ulysses_attention_packed
@@ -142,6 +146,21 @@ class ParallelAttention(nn.Module):
                 qkv = self._rope(qkv)
             o = ops.flash_attention_packed(qkv, causal=True)  # [B, S, G * qpk, D]
         return self.proj(o.reshape(B, S, G * qpk * D))
+
+    def _cached(self, qkv, cache):
+        """Attention through the cache: a prompt that starts the sequences attends to itself as it is, later tokens to what is stored."""
+        if self.sequence_group is not None:
+            raise ValueError("a cache holds whole sequences: it does not go with sequence parallelism")
+        if cache.starting:
+            if self.rope_theta is not None:
+                qkv = self._rope(qkv)
+            cache.store(qkv)
+            return ops.flash_attention_packed(qkv, causal=True)
+        if self.rope_theta is None:
+            cache.store(qkv)
+            return cache.attend(qkv[:, :, :, :-2])
+        table = ops.rope_table(max(cache.max_tokens, self.max_seq), self.head_dim, self.rope_theta, qkv.device)
+        return cache.attend(cache.store(qkv, table))
 
     def _rope(self, qkv):
         """Rotary embedding of the query heads and the key head of every group of ``[B, S, groups, q_per_kv + 2, D]``
@@ -209,7 +228,7 @@ class TransformerBlock(nn.Module):
     def _make_mlp(self, hidden, ffn, activation, bias, dtype, out_std):
         return ParallelMLP(hidden, ffn, activation, bias, dtype, out_init_std=out_std)
 
-    def forward_deferred(self, x, delta=None):
+    def forward_deferred(self, x, delta=None, cache=None):
         """The block with its residual adds fused into the normalisation kernels.  ``delta`` is the output of
         the previous block's MLP that has not been added to the residual stream ``x`` yet; returns
         ``(residual stream, this block's MLP output)`` - the caller (the next block, or the model's final norm)
@@ -218,7 +237,7 @@ class TransformerBlock(nn.Module):
             y = self.norm1(x)
         else:
             x, y = self.norm1.add_norm(x, delta)
-        a = self.attn(y)
+        a = self.attn(y) if cache is None else self.attn(y, cache)
         x, y = self.norm2.add_norm(x, a)
         return x, self.mlp(y)
 

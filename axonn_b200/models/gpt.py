@@ -57,7 +57,8 @@ class GPTConfig:
 class GPT(nn.Module):
     """Decoder-only transformer with learned positions, LayerNorm and GELU feed-forward layers on the
     tensor-parallel building blocks; ``forward(tokens, targets)`` returns the loss, ``forward(tokens)`` the
-    (vocabulary-sharded) logits."""
+    (vocabulary-sharded) logits, with a
+    ``BlockCache`` whose ``plan`` has placed the tokens those of every row's last new token."""
 
     def __init__(self, cfg: GPTConfig, dtype=torch.bfloat16):
         super().__init__()
@@ -75,20 +76,27 @@ class GPT(nn.Module):
         self.head = ParallelLMHead(cfg.hidden, cfg.vocab, dtype=dtype)
         self.sequence_group = None     # set by parallel.sequence.enable_sequence_parallel
 
-    def forward(self, tokens, targets=None):
+    def forward(self, tokens, targets=None, cache=None):
         B, S = tokens.shape
         first = 0 if self.sequence_group is None else dist.get_rank(self.sequence_group) * S
-        pos = _positions(self.pos_emb, first, S, tokens.device)     # this rank's slice of the positions
-        x = self.tok_emb(tokens) + pos[None]
+        if cache is None:
+            pos = _positions(self.pos_emb, first, S, tokens.device)[None]     # this rank's slice of the positions
+        else:
+            pos = self.pos_emb(cache.positions)
+        x = self.tok_emb(tokens) + pos
         delta = None   # MLP output of the previous block, added to x inside the next norm kernel
-        for blk in self.blocks:
-            if self.cfg.activation_checkpointing and self.training:
+        for i, blk in enumerate(self.blocks):
+            if cache is not None:
+                x, delta = blk.forward_deferred(x, delta, cache.layer(i))
+            elif self.cfg.activation_checkpointing and self.training:
                 if delta is not None:
                     x, delta = x + delta, None
                 x = checkpoint(blk, x, use_reentrant=False)
             else:
                 x, delta = blk.forward_deferred(x, delta)
         y = self.norm_f(x) if delta is None else self.norm_f.add_norm(x, delta)[1]
+        if cache is not None:
+            return self.head(cache.last(y))
         return self.head(y, targets)
 
     def num_parameters(self):

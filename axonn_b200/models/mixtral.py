@@ -73,7 +73,8 @@ class MoEBlock(TransformerBlock):
 class Mixtral(nn.Module):
     """Decoder-only transformer with RMSNorm, rotary grouped-query attention and an ``ExpertParallelMoE``
     feed-forward in every block; ``forward(tokens, targets)`` returns the loss including the routers' auxiliary
-    loss, ``forward(tokens)`` the (vocabulary-sharded) logits."""
+    loss, ``forward(tokens)`` the (vocabulary-sharded) logits, with a
+    ``BlockCache`` whose ``plan`` has placed the tokens those of every row's last new token."""
 
     def __init__(self, cfg: MixtralConfig, dtype=torch.bfloat16):
         super().__init__()
@@ -84,17 +85,21 @@ class Mixtral(nn.Module):
         self.norm_f = TPNorm(cfg.hidden, cfg.eps, rms=True, dtype=dtype)
         self.head = ParallelLMHead(cfg.hidden, cfg.vocab, dtype=dtype)
 
-    def forward(self, tokens, targets=None):
+    def forward(self, tokens, targets=None, cache=None):
         x = self.tok_emb(tokens)
         delta = None   # expert-layer output of the previous block, added to x inside the next norm kernel
-        for blk in self.blocks:
-            if self.cfg.activation_checkpointing and self.training:
+        for i, blk in enumerate(self.blocks):
+            if cache is not None:
+                x, delta = blk.forward_deferred(x, delta, cache.layer(i))
+            elif self.cfg.activation_checkpointing and self.training:
                 if delta is not None:
                     x, delta = x + delta, None
                 x = checkpoint(blk, x, use_reentrant=False)
             else:
                 x, delta = blk.forward_deferred(x, delta)
         y = self.norm_f(x) if delta is None else self.norm_f.add_norm(x, delta)[1]
+        if cache is not None:
+            return self.head(cache.last(y))
         out = self.head(y, targets)
         if targets is None:
             return out

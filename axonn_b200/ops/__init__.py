@@ -7,7 +7,7 @@ PyTorch composition used on CPU (and as the numerical oracle in the tests).
 
 from .activation import gelu_backward_colsum, gelu, gelu_backward, swiglu  # noqa: F401
 from .attention import flash_attention, flash_attention_packed  # noqa: F401
-from .beam import BeamStep, beam_select  # noqa: F401
+from .beam import MOST_BEAMS, BeamStep, beam_select  # noqa: F401
 from .gemm import (  # noqa: F401
     gemm_on_pairs,
     EPI_BIAS,
