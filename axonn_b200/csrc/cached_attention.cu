@@ -133,32 +133,39 @@ template <int D, int NT> __host__ __device__ constexpr int warp_bytes() { return
 // The sum of partial results of a column: references, denominator, sums; lane i has values N i .. of the D = 32 N.
 template <int N> struct Partial {
   float m1 = CA_LOWEST, m2 = CA_LOWEST, l = 0.f, o[N] = {};
-  // Up to 32 more: lane x has what stands behind the sums of the x-th (`there`: it exists), row(x) are its sums, x < n.
-  template <typename Row> __device__ __forceinline__ void add(bool there, float x1, float x2, float xl, int n, const Row& row) {
+  // n more, in their order: row(x) are the sums of the x-th with what belongs to them behind, there(x) whether it exists.  Four at a
+  // time, so that their loads wait for nothing.
+  template <typename There, typename Row> __device__ __forceinline__ void add(int n, const There& there, const Row& row) {
     const int lane = threadIdx.x & 31;
-    if (!there) { x1 = x2 = CA_LOWEST; xl = 0.f; }
-    float n1 = fmaxf(m1, x1), n2 = fmaxf(m2, x2);
+    for (int x0 = 0; x0 < n; x0 += 4) {
+      float f[4][N];
+      float4 stat[4];
 #pragma unroll
-    for (int i = 16; i > 0; i >>= 1) { n1 = fmaxf(n1, __shfl_xor_sync(0xffffffffu, n1, i)); n2 = fmaxf(n2, __shfl_xor_sync(0xffffffffu, n2, i)); }
-    const float weight = there ? exp2_fast(x2 - n2) : 0.f, old = exp2_fast(m2 - n2);
-    float sum = xl * exp2_fast(x1 - n1);
+      for (int y = 0; y < 4; ++y) {
+        stat[y] = make_float4(CA_LOWEST, CA_LOWEST, 0.f, 0.f);
 #pragma unroll
-    for (int i = 16; i > 0; i >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, i);
-    l = l * exp2_fast(m1 - n1) + sum;
+        for (int i = 0; i < N; ++i) f[y][i] = 0.f;
+        if (x0 + y >= n || !there(x0 + y)) continue;
+        const float* z = row(x0 + y);
+        stat[y] = *reinterpret_cast<const float4*>(z + 32 * N);
+        if constexpr (N == 4) { const float4 u = *reinterpret_cast<const float4*>(z + lane * N); f[y][0] = u.x; f[y][1] = u.y; f[y][2] = u.z; f[y][3] = u.w; }
+        else { const float2 u = *reinterpret_cast<const float2*>(z + lane * N); f[y][0] = u.x; f[y][1] = u.y; }
+      }
+      const float n1 = fmaxf(fmaxf(m1, fmaxf(stat[0].x, stat[1].x)), fmaxf(stat[2].x, stat[3].x));
+      const float n2 = fmaxf(fmaxf(m2, fmaxf(stat[0].y, stat[1].y)), fmaxf(stat[2].y, stat[3].y));
+      const float old = exp2_fast(m2 - n2);
+      l *= exp2_fast(m1 - n1);
 #pragma unroll
-    for (int i = 0; i < N; ++i) o[i] *= old;
-#pragma unroll 4
-    for (int x = 0; x < n; ++x) {
-      const float w = __shfl_sync(0xffffffffu, weight, x);
-      if (!__shfl_sync(0xffffffffu, there, x)) continue;
-      const float* z = row(x) + lane * N;
-      float f[N];
-      if constexpr (N == 4) { const float4 u = *reinterpret_cast<const float4*>(z); f[0] = u.x; f[1] = u.y; f[2] = u.z; f[3] = u.w; }
-      else { const float2 u = *reinterpret_cast<const float2*>(z); f[0] = u.x; f[1] = u.y; }
+      for (int i = 0; i < N; ++i) o[i] *= old;
 #pragma unroll
-      for (int i = 0; i < N; ++i) o[i] += w * f[i];
+      for (int y = 0; y < 4; ++y) {
+        const float w = exp2_fast(stat[y].y - n2);
+        l += stat[y].z * exp2_fast(stat[y].x - n1);
+#pragma unroll
+        for (int i = 0; i < N; ++i) o[i] += w * f[y][i];
+      }
+      m1 = n1; m2 = n2;
     }
-    m1 = n1; m2 = n2;
   }
   __device__ __forceinline__ void store(float* z) const {
     const int lane = threadIdx.x & 31;
@@ -589,10 +596,7 @@ __global__ void __launch_bounds__(32 * CA_WARPS, 1) attend_kernel(const AttendAr
         x += i;
         return reinterpret_cast<const float*>(ring + x / 2 * warp_bytes<D, NT>() + (x & 1 ? 0 : ring_bytes<D, NT>())) + cc * (D + 4);
       };
-      const int n = last - i + 1;
-      const bool there = lane < n && (here >> (i + lane) & 1u);
-      const float4 stat = there ? *reinterpret_cast<const float4*>(row(lane) + D) : make_float4(0.f, 0.f, 0.f, 0.f);
-      p.add(there, stat.x, stat.y, stat.z, n, row);
+      p.add(last - i + 1, [&](int x) { return (here >> (i + x) & 1u) != 0u; }, row);
       if (whole) { write_row(output_row<T>(a, first_r, g, col0 + cc, D), p); continue; }
       p.store(a.part + (slot * COLS + cc) * (D + 4));
     }
@@ -622,25 +626,18 @@ __global__ void __launch_bounds__(32 * MERGE_WARPS) attend_merge_kernel(const At
   for (int c0 = 0; c0 < cols; c0 += MERGE_WARPS / share) {
     const int cc = c0 + w / share, mine = w % share, end = min(parts, mine * per + per);
     Partial<D / 32> p;
+    const int x0 = mine * per;
     if (cc < cols)
-      for (int x0 = mine * per; x0 < end; x0 += 32) {
-        auto row = [&](int x) {
-          x += x0;
-          return a.part + (static_cast<size_t>(x == 0 ? ends.x : (ends.x & ~1) + 2 * x) * columns + cc) * (D + 4);
-        };
-        const int n = min(32, end - x0);
-        const float4 stat = lane < n ? *reinterpret_cast<const float4*>(row(lane) + D) : make_float4(0.f, 0.f, 0.f, 0.f);
-        p.add(lane < n, stat.x, stat.y, stat.z, n, row);
-      }
+      p.add(end - x0, [](int) { return true; }, [&](int x) {
+        return a.part + (static_cast<size_t>(x0 + x == 0 ? ends.x : (ends.x & ~1) + 2 * (x0 + x)) * columns + cc) * (D + 4);
+      });
     if (share > 1) {
       __syncthreads();
       p.store(sums[w]);
       __syncthreads();
       if (mine == 0 && cc < cols) {
-        auto row = [&](int x) { return sums[w + x]; };
         p = Partial<D / 32>();
-        const float4 stat = lane < share ? *reinterpret_cast<const float4*>(row(lane) + D) : make_float4(0.f, 0.f, 0.f, 0.f);
-        p.add(lane < share, stat.x, stat.y, stat.z, share, row);
+        p.add(share, [](int) { return true; }, [&](int x) { return sums[w + x]; });
       }
     }
     if (mine == 0 && cc < cols) write_row(output_row<T>(a, r, g, col0 + cc, D), p);
