@@ -701,8 +701,11 @@ extern "C" int axb_cached_attention(const void* q, long long q_row, long long q_
   const int columns = attend_columns(S * P), groups = (S * P + columns - 1) / columns, blocks = sm_count_current();
   AttendArgs a{q, q_row, q_token, q_group, out, (const uint8_t*)k, (const uint8_t*)v, ks, vs, tables, lengths, fresh, R, S, G, P, W, N, shift,
                groups, scale * 1.4426950408889634f, blocks, (int*)work, nullptr, nullptr};
-  for (int r0 = 0; r0 < R; r0 += CA_MAX_ROWS) {
-    a.R = R - r0 < CA_MAX_ROWS ? R - r0 : CA_MAX_ROWS;
+  // of the rows of a launch: their units, of very long tables, are counted in 31 bits
+  const long long most = (static_cast<long long>(W) << shift < 0x7fffffffll ? static_cast<long long>(W) << shift : 0x7fffffffll) / CA_TILE + 1 + CA_START;
+  const int rows = static_cast<int>(0x7fffffffll / most < CA_MAX_ROWS ? 0x7fffffffll / most : CA_MAX_ROWS);
+  for (int r0 = 0; r0 < R; r0 += rows) {
+    a.R = R - r0 < rows ? R - r0 : rows;
     a.q = static_cast<const char*>(q) + r0 * q_row * 2;
     a.out = static_cast<char*>(out) + static_cast<size_t>(r0) * S * G * P * D * 2;
     a.tables = tables + static_cast<size_t>(r0) * W;

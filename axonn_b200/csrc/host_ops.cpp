@@ -317,7 +317,7 @@ PyObject* py_plan_blocks(PyObject*, PyObject* const* a, Py_ssize_t n) {
   if (PyErr_Occurred()) return nullptr;
   if (lengths.dim() != 1 || tables.dim() != 2 || free_blocks.dim() != 1) Py_RETURN_NONE;
   const int64_t R = lengths.size(0), W = tables.size(1), N = free_blocks.size(0);
-  if (R == 0 || W == 0 || N == 0 || tokens <= 0 || std::max({R, W, N, static_cast<int64_t>(tokens)}) > INT32_MAX || !block_size(block) ||
+  if (R == 0 || W == 0 || N == 0 || tokens <= 0 || std::max({R, W * block, N, static_cast<int64_t>(tokens)}) > INT32_MAX || !block_size(block) ||
       !is(lengths, at::kInt, {R}) || !is(fresh, at::kInt, {R}) || !is(tables, at::kInt, {R, W}) || !is(free_blocks, at::kInt, {N}) ||
       !is(taken, at::kInt, {1}))
     Py_RETURN_NONE;

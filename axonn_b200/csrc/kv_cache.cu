@@ -60,16 +60,17 @@ __global__ void __launch_bounds__(PLAN_THREADS) plan_kernel(const PlanArgs a) {
   const int incl = warp_inclusive(p.need);
   if (lane == 31) { warp_sum[w] = incl; before[w] = earlier_in_warp; }
   __syncthreads();
-  int base = a.taken[0] + incl - p.need;
+  const int used = min(max(a.taken[0], 0), a.N);      // whatever stands there, nothing outside the list is read
+  long long base = static_cast<long long>(used) + incl - p.need;
   for (int i = 0; i < PLAN_THREADS / 32; ++i) base += before[i] + (i < w ? warp_sum[i] : 0);
   if (tid < n) {
-    const int got = min(max(a.N - base, 0), p.need);
+    const int got = static_cast<int>(min(max(a.N - base, 0ll), static_cast<long long>(p.need)));
     const long long room = (static_cast<long long>(p.held + got) << a.shift) - p.length;
     const int add = static_cast<int>(max(0ll, min(p.add, room)));
-    s_base[tid] = base; s_held[tid] = p.held; s_got[tid] = got; s_length[tid] = static_cast<int>(p.length); s_add[tid] = add;
+    s_base[tid] = static_cast<int>(min(base, static_cast<long long>(a.N))); s_held[tid] = p.held; s_got[tid] = got; s_length[tid] = static_cast<int>(p.length); s_add[tid] = add;
     if (blockIdx.y == 0) {
       a.lengths_out[r0 + tid] = static_cast<int>(p.length) + add;
-      if (r0 + tid == a.R - 1) a.taken_out[0] = max(a.taken[0], min(base + p.need, max(a.N, a.taken[0])));
+      if (r0 + tid == a.R - 1) a.taken_out[0] = static_cast<int>(min(base + p.need, static_cast<long long>(a.N)));
     }
   }
   __syncthreads();
@@ -435,6 +436,7 @@ extern "C" int axb_plan_blocks(const int* lengths, const int* fresh, int* tables
   const int shift = block_shift(block_tokens);
   if (shift < 0) return -1;
   if (R <= 0 || S <= 0 || W <= 0 || N <= 0) { set_error("plan_blocks: empty sizes"); return -1; }
+  if (static_cast<long long>(W) << shift > 0x7fffffffll) { set_error("plan_blocks: tables of more than 2^31 - 1 tokens"); return -1; }
   const int tokens = S < PLAN_TOKENS ? S : PLAN_TOKENS;
   int rows = PLAN_TOKENS / tokens;
   if (rows > PLAN_THREADS) rows = PLAN_THREADS;

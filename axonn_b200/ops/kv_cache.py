@@ -87,7 +87,8 @@ def plan_blocks(lengths, new, tables, free, taken, tokens, block_tokens):
     The blocks that are missing are the next ones of the list ``free``, of which ``taken[0]`` have been used, in the order of
     the requests; their ids are written into ``tables`` (in place: entries behind what a request holds).  A request whose row of
     the table is full, or that comes when the list is used up, gets places for as many tokens as there is room for: its
-    ``lengths`` entry of the plan tells.  ``lengths`` and ``taken`` themselves are left as they are."""
+    ``lengths`` entry of the plan tells.  ``lengths`` and ``taken`` themselves are left as they are (numbers below 0 and beyond the
+    list count as 0 and its end)."""
     if lengths.is_cuda and (host := host_paths()) is not None:
         out = host.plan_blocks(lengths, new, tables, free, taken, tokens, block_tokens)
         if out is not None:
@@ -105,6 +106,8 @@ def plan_blocks(lengths, new, tables, free, taken, tokens, block_tokens):
     _int32("tables", tables, R, tables.shape[1])
     _int32("free", free, free.shape[0])
     _int32("taken", taken, 1)
+    if tables.shape[1] * block_tokens >= 1 << 31:
+        raise ValueError(f"a row of {tables.shape[1]} blocks holds more than 2^31 - 1 tokens")
     _together(dev, new, tables, free, taken)
     if R == 0 or tokens == 0:
         return BlockPlan(torch.empty(R, tokens, dtype=torch.int64, device=dev), torch.empty(R, tokens, dtype=torch.int32, device=dev),
@@ -126,6 +129,7 @@ def _plan_torch(lengths, new, tables, free, taken, S, BT):
     length, add = lengths.long().clamp(min=0), new.long().clamp(0, S)
     held = ((length + BT - 1) // BT).clamp(max=W)
     need = ((length + add + BT - 1) // BT).clamp(max=W) - held
+    taken = taken.clamp(0, N)
     base = taken.long() + need.cumsum(0) - need
     got = torch.minimum((N - base).clamp(min=0), need)
     add = torch.minimum(add, ((held + got) * BT - length).clamp(min=0))
@@ -151,7 +155,8 @@ def _qkv_strides(qkv):
 
 def store_blocks(qkv, layer, slots, positions=None, rope_table=None) -> Optional[torch.Tensor]:
     """Store the keys and values of the packed projection output ``qkv [R, S, kv_heads, q_per_kv + 2, D]`` (per KV head: its query
-    heads, then its key, then its value) at ``slots [R, S]`` of ``layer``, as ``plan_blocks`` gives them.
+    heads, then its key, then its value) at ``slots [R, S]`` of ``layer``, as ``plan_blocks`` gives them: the tokens of a row follow one
+    another, those without a slot stand behind them, and no block takes tokens of two rows.
 
     The scale of a block and head is the smallest power of two by which the largest finite value of its new tokens does not exceed the
     largest code (448 in e4m3, 127 in int8); a block that holds tokens already keeps the larger of its scale and that one, and where
@@ -360,7 +365,7 @@ def reorder_blocks(blocks, tables, lengths, spare, parents):
     """Rows go on from other rows, as the beams of a prompt do: row ``j`` of group ``b`` from row ``parents[b, j]`` of that group.
 
     ``blocks``: a ``BlockLayer`` of all layers, stacked in front (``[layers, blocks, kv_heads, block_tokens, D]``); ``tables [R, W]``,
-    ``lengths [R]`` with ``R = groups * beams`` rows, ``parents [groups, beams]`` (int32).  Full blocks are shared by naming them.  The
+    ``lengths [R]`` with ``R = groups * beams`` rows, those of a group equally long, ``parents [groups, beams]`` (int32).  Full blocks are shared by naming them.  The
     block that a row still writes into is its own: a row with another parent has its parent's unfinished block copied into the block
     ``spare[r]``, and keeps the block that it leaves as the new spare one; ``spare [R]`` and the unfinished blocks of the rows are all
     different.  Returns the rows' new ``(tables, lengths, spare)``; the arguments are left as they are, but for the contents of the

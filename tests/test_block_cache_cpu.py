@@ -219,3 +219,24 @@ def test_refusals_of_the_c_entries():
     assert select(V=(1 << 30) + 1) == -1 and "vocabulary" in error()
     assert select(dtype=3) == -1 and "logits" in error()
     assert select(work=p + 4) == -1 and "aligned" in error()
+
+
+@pytest.mark.parametrize("taken,got", [(-3, 2), (0, 2), (3, 1), (4, 0), (9, 0), (2**31 - 1, 0)])
+def test_plan_from_any_number_of_taken_blocks(taken, got):
+    """Nothing outside the list is named."""
+    tables = torch.full((1, 4), -1, dtype=torch.int32)
+    one = lambda x: torch.tensor([x], dtype=torch.int32)  # noqa: E731
+    free = torch.tensor([10, 11, 12, 13], dtype=torch.int32)
+    plan = ops.plan_blocks(one(0), one(20), tables, free, one(taken), 20, 16)
+    first = min(max(taken, 0), 4)
+    assert tables[0].tolist() == [10 + first + i if i < got else -1 for i in range(4)]
+    assert int(plan.lengths) == min(20, 16 * got) and int(plan.taken) == first + got
+
+
+def test_plan_refuses_tables_of_more_tokens_than_lengths_count():
+    none = torch.empty(0, dtype=torch.int32)
+    with pytest.raises(ValueError, match="2.31"):
+        ops.plan_blocks(none, none, torch.empty(0, 1 << 27, dtype=torch.int32), torch.zeros(1, dtype=torch.int32),
+                        torch.zeros(1, dtype=torch.int32), 1, 16)
+    L, p = _lib.lib(), 4096
+    assert L.axb_plan_blocks(*[p] * 9, 1, 1, 1 << 27, 1, 16, None) == -1 and "2^31" in L.axb_last_error().decode()

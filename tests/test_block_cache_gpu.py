@@ -511,3 +511,14 @@ def test_native_host_paths_launch_the_same(monkeypatch):
     monkeypatch.setattr(_lib, "_HOST", None)
     plain = run()
     assert len(native) == len(plain) and all(same_bits(a, b) for a, b in zip(native, plain))
+
+
+@pytest.mark.parametrize("taken", [-7, 3, 5, 6, 2**31 - 1])
+def test_plan_from_any_number_of_taken_blocks(taken):
+    """As on the CPU, whatever number stands there."""
+    def plan(device):
+        tables = torch.full((3, 4), -1, dtype=torch.int32, device=device)
+        numbers = [torch.tensor(x, dtype=torch.int32, device=device) for x in ([0, 0, 0], [20, 5, 70], [10, 11, 12, 13, 14], [taken])]
+        return tables, *ops.plan_blocks(numbers[0], numbers[1], tables, numbers[2], numbers[3], 70, 16)
+    for got, want in zip(plan("cuda"), plan("cpu")):
+        assert torch.equal(got.cpu(), want)
