@@ -38,15 +38,17 @@ class BlockCache:
     """Cache for ``rows`` sequences of up to ``max_tokens`` tokens of ``model`` (``GPT``, ``Llama``, ``Mixtral``).
 
     ``plan(tokens, new)`` places the next tokens of every row, ``model(tokens, cache=cache)`` evaluates them and returns the logits
-    of each row's last one.  ``expand(beams)`` lets every row go on as ``beams`` rows, which ``reorder(parents)`` lets go on from one
-    another; ``prompt_tokens`` are stored before that (full blocks of theirs are shared), and ``beams`` here sets blocks aside for
-    it.  ``dtype``: ``torch.float8_e4m3fn`` or ``torch.int8``."""
+    of each row's last one; tokens past ``max_tokens`` get no place, and ``lengths`` tells how many have one.  ``expand(beams)`` lets
+    every row go on as ``beams`` rows, which ``reorder(parents)`` lets go on from one another; ``prompt_tokens`` (``None``: up to
+    ``max_tokens``) are stored before that, whose full blocks are shared, and ``beams`` here sets blocks aside for it.  ``dtype``: ``torch.float8_e4m3fn`` or ``torch.int8``."""
 
     def __init__(self, model, rows, max_tokens, block_tokens=64, dtype=torch.float8_e4m3fn, beams=None, prompt_tokens=None):
         attn = [blk.attn for blk in model.blocks]
         device = next(model.parameters()).device
         per = lambda n: -(-n // block_tokens)  # noqa: E731
-        self.block_tokens, self.max_tokens = block_tokens, max_tokens
+        if hasattr(model, "pos_emb") and max_tokens > model.cfg.seq_len:
+            raise ValueError(f"{max_tokens} tokens for a model that has learned {model.cfg.seq_len} positions")
+        self.block_tokens, self.max_tokens, self.beams = block_tokens, max_tokens, beams
         width = per(max_tokens)
         blocks = rows * width
         if beams is not None:
@@ -72,9 +74,13 @@ class BlockCache:
         """Place the next ``tokens`` tokens of every row, the first ``new[r]`` (int32; ``None``: all) of which are there."""
         if new is None:
             new = torch.full_like(self.lengths, tokens)
+        if self.max_tokens % self.block_tokens:                         # the last block has more places
+            new = torch.minimum(new, (self.max_tokens - self.lengths).clamp(min=0))
+        before = self.lengths
         self.starting = self.step is None
         self.step = ops.plan_blocks(self.lengths, new, self.tables, self.free, self.taken, tokens, self.block_tokens)
-        self.new, self.lengths, self.taken = new, self.step.lengths, self.step.taken
+        self.lengths, self.taken = self.step.lengths, self.step.taken
+        self.new = self.lengths - before
 
     @property
     def positions(self):
@@ -90,10 +96,14 @@ class BlockCache:
 
     def expand(self, beams):
         """Every row goes on as ``beams`` rows: full blocks are shared, the unfinished one is copied for each."""
+        if self.beams is None or not 1 <= beams <= self.beams or self.spare is not None:
+            raise ValueError(f"rows go on once, as up to {self.beams or 'beams='} rows that the cache was made for, not {beams}")
         rows = self.tables.shape[0]
         n = rows * beams
-        own, spare = self.free[self.taken.long() + torch.arange(2 * n, device=self.free.device)].view(2, n)
-        self.taken = self.taken + 2 * n
+        at = self.taken.long() + torch.arange(2 * n, device=self.free.device)
+        last = self.free.numel() - 1
+        own, spare = torch.where(at <= last, self.free[at.clamp(max=last)], -1).view(2, n)      # a prompt longer than was said: none is left
+        self.taken = (self.taken + 2 * n).clamp(max=last + 1)
         tables, lengths = self.tables.repeat_interleave(beams, 0), self.lengths.repeat_interleave(beams, 0)
         # the first of a row's beams keeps the row's blocks; each other one gets a block of its own, filled as that of a row that moves
         current = lengths[:, None] // self.block_tokens == torch.arange(tables.shape[1], device=tables.device)

@@ -57,8 +57,8 @@ class GPTConfig:
 class GPT(nn.Module):
     """Decoder-only transformer with learned positions, LayerNorm and GELU feed-forward layers on the
     tensor-parallel building blocks; ``forward(tokens, targets)`` returns the loss, ``forward(tokens)`` the
-    (vocabulary-sharded) logits, with a
-    ``BlockCache`` whose ``plan`` has placed the tokens those of every row's last new token."""
+    (vocabulary-sharded) logits, with a ``BlockCache``
+    whose ``plan`` has placed the tokens those of every row's last new token."""
 
     def __init__(self, cfg: GPTConfig, dtype=torch.bfloat16):
         super().__init__()
@@ -77,6 +77,8 @@ class GPT(nn.Module):
         self.sequence_group = None     # set by parallel.sequence.enable_sequence_parallel
 
     def forward(self, tokens, targets=None, cache=None):
+        if cache is not None and targets is not None:
+            raise ValueError("a cache is for generation: it does not go with targets")
         B, S = tokens.shape
         first = 0 if self.sequence_group is None else dist.get_rank(self.sequence_group) * S
         if cache is None:

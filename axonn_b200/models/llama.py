@@ -50,8 +50,8 @@ class LlamaConfig:
 class Llama(nn.Module):
     """Decoder-only transformer with RMSNorm, rotary grouped-query attention and SwiGLU feed-forward layers on the
     tensor-parallel building blocks; ``forward(tokens, targets)`` returns the loss, ``forward(tokens)`` the
-    (vocabulary-sharded) logits, with a
-    ``BlockCache`` whose ``plan`` has placed the tokens those of every row's last new token."""
+    (vocabulary-sharded) logits, with a ``BlockCache``
+    whose ``plan`` has placed the tokens those of every row's last new token."""
 
     def __init__(self, cfg: LlamaConfig, dtype=torch.bfloat16):
         super().__init__()
@@ -67,6 +67,8 @@ class Llama(nn.Module):
         self.head = ParallelLMHead(cfg.hidden, cfg.vocab, dtype=dtype)
 
     def forward(self, tokens, targets=None, cache=None):
+        if cache is not None and targets is not None:
+            raise ValueError("a cache is for generation: it does not go with targets")
         x = self.tok_emb(tokens)
         delta = None   # MLP output of the previous block, added to x inside the next norm kernel
         for i, blk in enumerate(self.blocks):

@@ -73,8 +73,8 @@ class MoEBlock(TransformerBlock):
 class Mixtral(nn.Module):
     """Decoder-only transformer with RMSNorm, rotary grouped-query attention and an ``ExpertParallelMoE``
     feed-forward in every block; ``forward(tokens, targets)`` returns the loss including the routers' auxiliary
-    loss, ``forward(tokens)`` the (vocabulary-sharded) logits, with a
-    ``BlockCache`` whose ``plan`` has placed the tokens those of every row's last new token."""
+    loss, ``forward(tokens)`` the (vocabulary-sharded) logits, with a ``BlockCache``
+    whose ``plan`` has placed the tokens those of every row's last new token."""
 
     def __init__(self, cfg: MixtralConfig, dtype=torch.bfloat16):
         super().__init__()
@@ -86,6 +86,8 @@ class Mixtral(nn.Module):
         self.head = ParallelLMHead(cfg.hidden, cfg.vocab, dtype=dtype)
 
     def forward(self, tokens, targets=None, cache=None):
+        if cache is not None and targets is not None:
+            raise ValueError("a cache is for generation: it does not go with targets")
         x = self.tok_emb(tokens)
         delta = None   # expert-layer output of the previous block, added to x inside the next norm kernel
         for i, blk in enumerate(self.blocks):

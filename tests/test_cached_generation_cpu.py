@@ -234,3 +234,45 @@ def _shared_blocks(rank, world):
 
 def test_beams_share_what_is_full():
     run_distributed(_shared_blocks, 1)
+
+
+def _ends_of_a_cache(rank, world):
+    """Tokens past the cache's end get no place; beams that no blocks were set aside for are refused, prompts longer than was said end."""
+    from axonn_b200.models import BlockCache
+
+    model = _model("gpt", (1, 1, 1), 1).eval()
+    with torch.no_grad():
+        cache = BlockCache(model, 2, 20, 16, torch.int8)
+        cache.plan(18, torch.tensor(LENGTHS, dtype=torch.int32))
+        model(torch.tensor(PROMPTS), cache=cache)
+        cache.plan(5)                                   # the last block has places for 32
+        assert cache.lengths.tolist() == [20, 11] and cache.new.tolist() == [2, 5]
+        assert cache.step.slots[0, 2:].tolist() == [-1] * 3 and int(cache.positions.max()) == 19
+        assert bool(model(torch.tensor(PROMPTS)[:, :5], cache=cache).isfinite().all())
+        cache.plan(1)
+        assert cache.lengths.tolist() == [20, 12] and cache.new.tolist() == [0, 1]
+        assert bool(model(torch.zeros(2, 1, dtype=torch.long), cache=cache).isfinite().all())
+        with pytest.raises(ValueError, match="targets"):
+            model(torch.zeros(2, 1, dtype=torch.long), torch.zeros(2, 1, dtype=torch.long), cache)
+        with pytest.raises(ValueError, match="go on once"):
+            cache.expand(2)
+        with pytest.raises(ValueError, match="40 positions"):
+            BlockCache(model, 1, 41)
+        beams = BlockCache(model, 1, 40, 16, torch.int8, beams=2, prompt_tokens=2)
+        with pytest.raises(ValueError, match="go on once"):
+            beams.expand(3)
+        for n in (18, 18):
+            beams.plan(n)
+            model(torch.tensor(PROMPTS)[:1], cache=beams)
+        beams.expand(2)
+        with pytest.raises(ValueError, match="go on once"):
+            beams.expand(2)
+        for _ in range(10):
+            beams.plan(1)
+            assert bool(model(torch.zeros(2, 1, dtype=torch.long), cache=beams).isfinite().all())
+            beams.reorder(torch.tensor([[1, 0]], dtype=torch.int32))
+        assert int(beams.taken) <= beams.free.numel() and int(beams.tables.max()) < beams.free.numel()
+
+
+def test_ends_of_a_cache():
+    run_distributed(_ends_of_a_cache, 1)
