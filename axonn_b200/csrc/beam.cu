@@ -186,7 +186,8 @@ __global__ void __launch_bounds__(32 * BEAM_WARPS) beam_rows_kernel(const BeamAr
   const int lane = threadIdx.x & 31, w = threadIdx.x >> 5, K = a.K;
   const long long run = static_cast<long long>(blockIdx.x) * BEAM_WARPS + w;
   if (run >= a.items) return;
-  const int row = static_cast<int>(run / a.parts), first = static_cast<int>(run - static_cast<long long>(row) * a.parts) * a.chunks;
+  // rows of several runs are 4 KB and more: their runs are counted in 32 bits
+  const int row = static_cast<int>(a.parts == 1 ? run : static_cast<unsigned>(run) / a.parts), first = static_cast<int>(run - static_cast<long long>(row) * a.parts) * a.chunks;
   if (a.done && a.done[row]) return;
   const int last = min(first + a.chunks, (a.V + CHUNK - 1) / CHUNK);
   const T* values = static_cast<const T*>(a.logits) + static_cast<long long>(row) * a.V;

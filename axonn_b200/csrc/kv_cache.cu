@@ -113,7 +113,7 @@ struct StoreArgs {
   int R, S, G, P, N, shift, angles;
   int runs;                          // blocks that a row's new tokens touch, at most
   int job_threads;                   // threads that share a job (one head of one block): a warp or the whole block
-  long long jobs, job_blocks;
+  unsigned jobs, job_blocks;
 };
 
 template <typename T> __device__ __forceinline__ void widen8(const uint4& u, float* f) {
@@ -215,13 +215,14 @@ __global__ void __launch_bounds__(256, ROPE ? 2 : 4) store_kernel(const StoreArg
   if (ROPE && blockIdx.x >= a.job_blocks) {        // queries
     const long long unit = (blockIdx.x - a.job_blocks) * static_cast<long long>(blockDim.x) + threadIdx.x;
     const int c = static_cast<int>(unit % UNITS) * 8, H = a.G * a.P;
-    const long long row = unit / UNITS, token = row / H;
-    if (token >= static_cast<long long>(a.R) * a.S) return;
-    const int h = static_cast<int>(row % H);
+    if (unit / UNITS >= static_cast<long long>(a.R) * a.S * H) return;
+    const unsigned row = static_cast<unsigned>(unit / UNITS), token = row / H;      // 31 bits: the host sees to that
+    const int h = static_cast<int>(row - token * H);
     float f[16];
     const int at = a.positions[token];
     if (a.slots[token] >= 0 && at >= 0 && at < a.angles) {
-      const T* p = qkv + (token / a.S) * a.row_stride + (token % a.S) * a.token_stride + (h / a.P) * a.group_stride + (h % a.P) * D + c;
+      const unsigned r = token / a.S, g = h / a.P;
+      const T* p = qkv + r * a.row_stride + (token - r * a.S) * a.token_stride + g * a.group_stride + (h - g * a.P) * D + c;
       load8(p, f);
       load8(p + D / 2, f + 8);
       rotate8(f, a.cs + (static_cast<size_t>(at) * (D / 2) + c) * 2);
@@ -229,18 +230,18 @@ __global__ void __launch_bounds__(256, ROPE ? 2 : 4) store_kernel(const StoreArg
 #pragma unroll
       for (int i = 0; i < 16; ++i) f[i] = 0.f;
     }
-    T* o = static_cast<T*>(a.q) + row * D + c;
+    T* o = static_cast<T*>(a.q) + static_cast<size_t>(row) * D + c;
     store8(o, f);
     store8(o + D / 2, f + 8);
     return;
   }
   const int threads = a.job_threads, tid = threads == 32 ? threadIdx.x & 31 : threadIdx.x;
-  const long long job = threads == 32 ? blockIdx.x * static_cast<long long>(blockDim.x / 32) + (threadIdx.x >> 5) : blockIdx.x;
+  const unsigned job = threads == 32 ? blockIdx.x * (blockDim.x / 32) + (threadIdx.x >> 5) : blockIdx.x;
   if (job >= a.jobs) return;               // whole warps: jobs of more than a warp are whole blocks
   // values next to keys, then heads, so that the rows that neighbouring blocks read lie together
   const bool values = job & 1;
-  const long long rest = job >> 1;
-  const int g = static_cast<int>(rest % a.G), run = static_cast<int>(rest / a.G % a.runs), r = static_cast<int>(rest / a.G / a.runs);
+  const unsigned rest = job >> 1, block = rest / a.G;
+  const int g = static_cast<int>(rest - block * a.G), r = static_cast<int>(block / a.runs), run = static_cast<int>(block - r * a.runs);
   const int BT = 1 << a.shift;
   const long long* slots = a.slots + static_cast<size_t>(r) * a.S;
   const long long slot0 = slots[0];
@@ -398,17 +399,23 @@ __global__ void __launch_bounds__(REORDER_THREADS) reorder_kernel(const ReorderA
   else if (tid >= 32 && tid < 32 + heads) a.vs[target + tid - 32] = a.vs[source + tid - 32];
   const int per_head = part * a.row_bytes / 16, total = 2 * heads * per_head;
   const size_t head_bytes = static_cast<size_t>(a.row_bytes) << a.shift;
-  auto at = [&](int i, size_t head) {
-    const int h = i / per_head;
-    uint8_t* p = h < heads ? a.k + (head + h) * head_bytes : a.v + (head + h - heads) * head_bytes;
-    return reinterpret_cast<uint4*>(p) + i % per_head;
-  };
+  // word `at` of head h, keys then values; REORDER_THREADS words further: heads and words to go, without a division
+  const int step_heads = REORDER_THREADS / per_head, step = REORDER_THREADS - step_heads * per_head;
+  int h = tid / per_head, at = tid - h * per_head;
   for (int i0 = tid; i0 < total; i0 += 4 * REORDER_THREADS) {
     uint4 u[4];
+    size_t to[4];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) if (i0 + j * REORDER_THREADS < total) u[j] = *at(i0 + j * REORDER_THREADS, source);
+    for (int j = 0; j < 4; ++j) {
+      const size_t word = (h < heads ? h : h - heads) * head_bytes + at * static_cast<size_t>(16);
+      to[j] = word;
+      if (i0 + j * REORDER_THREADS < total) u[j] = *reinterpret_cast<const uint4*>((h < heads ? a.k : a.v) + source * head_bytes + word);
+      h += step_heads; at += step;
+      if (at >= per_head) { at -= per_head; ++h; }
+    }
 #pragma unroll
-    for (int j = 0; j < 4; ++j) if (i0 + j * REORDER_THREADS < total) *at(i0 + j * REORDER_THREADS, target) = u[j];
+    for (int j = 0; j < 4; ++j)
+      if (i0 + j * REORDER_THREADS < total) *reinterpret_cast<uint4*>((i0 + j * REORDER_THREADS < total / 2 ? a.k : a.v) + target * head_bytes + to[j]) = u[j];
   }
 }
 
@@ -467,11 +474,11 @@ extern "C" int axb_store_blocks(const void* qkv, long long row_stride, long long
   const int units = (S < block_tokens ? S : block_tokens) * (D / 16);
   a.job_threads = units <= 32 * STORE_UNITS ? 32 : block_tokens * (D / 16) / STORE_UNITS;
   const int threads = a.job_threads == 32 ? 128 : a.job_threads, per_block = threads / a.job_threads;
-  a.jobs = 2ll * R * a.runs * G;
-  a.job_blocks = (a.jobs + per_block - 1) / per_block;
-  const long long q_units = cs ? static_cast<long long>(R) * S * G * P * (D / 16) : 0;
-  const long long grid = a.job_blocks + (q_units + threads - 1) / threads;
-  if (grid > 0x7fffffffll) { set_error("store_blocks: too many tokens in one call"); return -1; }
+  const long long jobs = 2ll * R * a.runs * G, job_blocks = (jobs + per_block - 1) / per_block;
+  const long long q_rows = cs ? static_cast<long long>(R) * S * G * P : 0, grid = job_blocks + (q_rows * (D / 16) + threads - 1) / threads;
+  a.jobs = static_cast<unsigned>(jobs);
+  a.job_blocks = static_cast<unsigned>(job_blocks);
+  if (grid > 0x7fffffffll || jobs > 0x7fffffffll || q_rows > 0x7fffffffll) { set_error("store_blocks: too many tokens in one call"); return -1; }
   void (*kern)(StoreArgs) = dtype == 0 ? store_variant<__nv_bfloat16>(D, int8 != 0, cs != nullptr) : store_variant<__half>(D, int8 != 0, cs != nullptr);
   AXB_CUDA(pdl_launch(kern, dim3((unsigned)grid), dim3(threads), 0, (cudaStream_t)stream, a));
   return 0;
