@@ -42,7 +42,9 @@ def greedy_generate(model, tokens, max_new_tokens: int, eos_id=None, cache_dtype
 
     With ``cache_dtype`` (``torch.float8_e4m3fn`` or ``torch.int8``) keys and values are kept in a ``BlockCache`` with blocks of
     ``block_tokens`` and every token is evaluated once; scores differ by the rounding of what is stored.  Prompts may then differ in
-    length: row ``r`` is ``tokens[r, :prompt_lengths[r]]``, and its new tokens follow there; what is left of a row is ``eos_id`` (or 0)."""
+    length: row ``r`` is ``tokens[r, :prompt_lengths[r]]``, and its new tokens follow there; what is left of a row is ``eos_id`` (or 0).
+    A ``Mixtral``'s expert capacity is that of a step's tokens, one per row, padding of the prompts among them: what is dropped differs
+    from an evaluation of whole prefixes unless ``capacity_factor`` leaves room for all."""
     if cache_dtype is None and prompt_lengths is not None:
         raise ValueError("prompts of different lengths need a cache (cache_dtype)")
     was_training = model.training
