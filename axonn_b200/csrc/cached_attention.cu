@@ -3,7 +3,7 @@
 //   s = scale * ks * (q . k)      o = sum_t p_t vs v_t / sum_t p_t,   p = softmax of s over the tokens that a query sees
 //
 // What bounds it is reading 2 D bytes per token and KV head once.  A sequence here is the tokens of one request, KV head and group of up
-// to 8 or 16 query columns (query heads of the KV head x new tokens); its unit of work is a tile of 32 tokens, after a start that counts
+// to 8 or 16 query columns (query heads of the KV head x new tokens; 128 where there are more than 64, see below); its unit of work is a tile of 32 tokens, after a start that counts
 // as two.  One block per SM takes a run of units as long as every other block's, whatever the lengths of the requests, and its eight
 // warps equal parts of that: a run ends inside one sequence and goes on in the next.  A sequence that one warp has seen whole is written
 // at once; those that warps of a block share are put together in shared memory, those that blocks share by a second launch, always in
@@ -54,16 +54,45 @@ struct AttendArgs {
   int* before;                           // [R + 1] units of the requests before each, per KV head and group
   int2* ends;                            // of every sequence: the slot of its first partial result (-1: finished), the block of its last
   float* part;                           // [2 * workers][columns][D + 4]: sums, then m, m', l
+  unsigned int* status;                  // for the waits of the wide kernel
+  unsigned long long timeout_ns;
 };
 
-// The units of a sequence are its tiles, after CA_START that stand for its start.  `active` blocks share all units; block w starts at
+// The units of a sequence are its tiles, after START that stand for its start.  `active` blocks share all units; block w starts at
 // units * w / active.
-__device__ __forceinline__ int sequence_units(int length) { return length ? (length + CA_TILE - 1) / CA_TILE + CA_START : 0; }
-__device__ __forceinline__ int active_blocks(long long units, int workers) {
-  const long long want = (units + CA_LEAST_TILES - 1) / CA_LEAST_TILES;
+template <int TILE, int START> __device__ __forceinline__ int sequence_units(int length) { return length ? (length - 1) / TILE + 1 + START : 0; }
+__device__ __forceinline__ int active_blocks(long long units, int workers, int least) {
+  const long long want = (units + least - 1) / least;
   return static_cast<int>(want < workers ? (want < 1 ? 1 : want) : workers);
 }
 __device__ __forceinline__ long long first_unit(long long units, int w, int active) { return units * w / active; }
+
+// Units of the requests before each, [R + 1], and lengths, in shared memory: one scan per block of the grid.
+template <int TILE, int START, int WARPS>
+__device__ __forceinline__ void scan_units(const AttendArgs& a, int* before, int* lengths) {
+  __shared__ int sums[WARPS];
+  const int tid = threadIdx.x, lane = tid & 31, most = min(static_cast<long long>(a.W) << a.shift, 0x7fffff00ll);
+  const int per = (a.R + 32 * WARPS - 1) / (32 * WARPS), r0 = tid * per;
+  int mine = 0;
+  for (int r = r0; r < min(r0 + per, a.R); ++r) {
+    lengths[r] = min(max(a.lengths[r], 0), most);
+    mine += sequence_units<TILE, START>(lengths[r]);
+  }
+  int incl = mine;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) { const int u = __shfl_up_sync(0xffffffffu, incl, o); if (lane >= o) incl += u; }
+  if (lane == 31) sums[tid >> 5] = incl;
+  __syncthreads();
+  int at = incl - mine;
+  for (int i = 0; i < tid >> 5; ++i) at += sums[i];
+  for (int r = r0; r < min(r0 + per, a.R); ++r) {
+    before[r] = at;
+    if (blockIdx.x == 0) a.before[r] = at;
+    at += sequence_units<TILE, START>(lengths[r]);
+  }
+  if (r0 < a.R && r0 + per >= a.R) { before[a.R] = at; if (blockIdx.x == 0) a.before[a.R] = at; }
+  __syncthreads();
+}
 __device__ __forceinline__ float exp2_fast(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
@@ -210,40 +239,15 @@ __global__ void __launch_bounds__(32 * CA_WARPS, 1) attend_kernel(const AttendAr
   extern __shared__ __align__(16) uint8_t ring[];      // of every warp; then the units of the requests before each, [R + 1], and lengths
   int* before = reinterpret_cast<int*>(ring + CA_WARPS * warp_bytes<D, NT>());
   int* lengths = before + a.R + 1;
-  __shared__ int sums[CA_WARPS];
   __shared__ Open open[CA_WARPS][2];         // the sequences that a warp has not seen whole: its first and its last
   pdl_launch_next();
   pdl_wait();
   const int tid = threadIdx.x, lane = tid & 31, wid = tid >> 5, g8 = lane >> 2, j4 = lane & 3, BT = 1 << a.shift;
-  const int most = min(static_cast<long long>(a.W) << a.shift, 0x7fffff00ll);
-
-  // units of the requests before each: one scan per block of the grid
-  {
-    const int per = (a.R + 32 * CA_WARPS - 1) / (32 * CA_WARPS), r0 = tid * per;
-    int mine = 0;
-    for (int r = r0; r < min(r0 + per, a.R); ++r) {
-      lengths[r] = min(max(a.lengths[r], 0), most);
-      mine += sequence_units(lengths[r]);
-    }
-    int incl = mine;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) { const int u = __shfl_up_sync(0xffffffffu, incl, o); if (lane >= o) incl += u; }
-    if (lane == 31) sums[tid >> 5] = incl;
-    __syncthreads();
-    int at = incl - mine;
-    for (int i = 0; i < tid >> 5; ++i) at += sums[i];
-    for (int r = r0; r < min(r0 + per, a.R); ++r) {
-      before[r] = at;
-      if (blockIdx.x == 0) a.before[r] = at;
-      at += sequence_units(lengths[r]);
-    }
-    if (r0 < a.R && r0 + per >= a.R) { before[a.R] = at; if (blockIdx.x == 0) a.before[a.R] = at; }
-    __syncthreads();
-  }
+  scan_units<CA_TILE, CA_START, CA_WARPS>(a, before, lengths);
   const uint64_t policy = evict_first();     // read once: what else is in the L2, the code of the ends among it, stays there
   const int per_tile = a.G * a.groups;
   const long long units = static_cast<long long>(before[a.R]) * per_tile;
-  const int active = active_blocks(units, a.workers);
+  const int active = active_blocks(units, a.workers, CA_LEAST_TILES);
   if (blockIdx.x >= active || units == 0) return;
   const long long first = first_unit(units, blockIdx.x, active), many = first_unit(units, blockIdx.x + 1, active) - first;
   const long long begin = first + many * wid / CA_WARPS, end = first + many * (wid + 1) / CA_WARPS;
@@ -612,6 +616,511 @@ __global__ void __launch_bounds__(32 * CA_WARPS, 1) attend_kernel(const AttendAr
   }
 }
 
+// ----------------------------------------------------------------------------- more than 64 query columns
+
+// The same sums on tcgen05, for groups of up to 128 columns (rows of the products: S = Q K^T, O = P V with M = 128): the codes of a tile of
+// 128 tokens are widened once for all of them.  24 requests of 4,096 tokens, 8 KV heads, 128 columns: 175 us (int8 155), 26 GFLOP of
+// products; 4,500 to 5,000 cycles a tile, of which the exponentials of a column's two threads are 1,700 (exp2 unit) and the rest is steps
+// that wait for one another: loads from tensor memory, the largest scores, the exchange between the two threads.  One block per SM, with
+// roles:
+//
+//   warps 0-7   softmax, two threads per column (lane of tensor memory), which share a tile's tokens and a sequence's values: the queries
+//               into shared memory, then per tile the weights as fp16 back into tensor memory, and the sums at the end of a sequence
+//   warps 8-15  codes, of keys (8-11) and values: 16 bytes of a lane, a tile ahead in registers, widened to fp16 into shared memory
+//               (128-byte rows, swizzled)
+//   warp 16     the products: S(t + 1) is issued before O += P(t) V(t), two buffers of scores, keys and values each
+//
+// Every wait is bounded.  What a column sees of a tile where it ends differs from column to column, and values that are NaN there must
+// not reach those that do not see them: they become zeros, and the sums of the columns that see them NaN, afterwards.
+constexpr int CW_TILE = 128;
+constexpr int CW_START = 1;              // what the start of a sequence costs a block, in tiles
+constexpr int CW_LEAST_TILES = 2;
+constexpr int CW_COLUMNS = 128;
+constexpr int CW_WARPS = 17, CW_CODE_WARPS = 4;      // all; that widen keys, and values
+
+template <int D> struct Wide {
+  static constexpr int CHUNK = 128 * 128;              // 128 rows of 64 fp16 values
+  static constexpr int MATRIX = D / 64 * CHUNK;
+  static constexpr int K = MATRIX, V = 3 * MATRIX, BARS = 5 * MATRIX, FIXED = BARS + 256 + 1024;
+  static constexpr int ROWS = 512 / D, PASSES = D / 16;      // token rows of a warp at a time, 16 bytes per lane; times per tile
+  static __device__ __forceinline__ int at(int row, int unit) { return (unit >> 3) * CHUNK + row * 128 + (((unit ^ row) & 7) << 4); }      // 16-byte unit of a row
+};
+
+__device__ __forceinline__ uint4 load_once(const void* p) {
+  uint4 u;
+  asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(u.x), "=r"(u.y), "=r"(u.z), "=r"(u.w) : "l"(p));
+  return u;
+}
+// 16 columns of tensor memory of a warp's 32 lanes.
+__device__ __forceinline__ void tmem_st_32x16(uint32_t at, const uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};"
+      : : "r"(at), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]),
+        "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]) : "memory");
+}
+
+// The pieces of sequences of a block's run, in their order; every role walks through them by itself.
+struct WideWalk {
+  long long u, end;
+  int r, g, group, item, t0, t1, tiles;
+  __device__ __forceinline__ WideWalk(const AttendArgs& a, const int* before) {
+    const int per_tile = a.G * a.groups;
+    const long long units = static_cast<long long>(before[a.R]) * per_tile;
+    const int active = active_blocks(units, a.workers, CW_LEAST_TILES);
+    u = end = 0;
+    r = 0;
+    if (blockIdx.x >= active || units == 0) return;
+    u = first_unit(units, blockIdx.x, active);
+    end = first_unit(units, blockIdx.x + 1, active);
+    for (int hi = a.R; hi - r > 1;) { const int mid = (r + hi) / 2; if (before[mid] <= u / per_tile) r = mid; else hi = mid; }
+  }
+  __device__ __forceinline__ bool next(const AttendArgs& a, const int* before) {
+    const int per_tile = a.G * a.groups;
+    while (u < end) {
+      while (before[r + 1] <= u / per_tile) ++r;
+      const int per_sequence = before[r + 1] - before[r];
+      const long long within = u - static_cast<long long>(before[r]) * per_tile;
+      item = static_cast<int>(within / per_sequence);
+      g = item / a.groups;
+      group = item - g * a.groups;
+      const int x0 = static_cast<int>(within - static_cast<long long>(item) * per_sequence);
+      const int x1 = static_cast<int>(min(static_cast<long long>(per_sequence), x0 + (end - u)));
+      u += x1 - x0;
+      tiles = per_sequence - CW_START;
+      t0 = max(x0 - CW_START, 0);
+      t1 = x1 - CW_START;
+      if (t1 > t0) return true;
+    }
+    return false;
+  }
+};
+
+// What the columns of a group see: all that see anything the tokens below lo, none those from hi on.
+struct WideSeen { int lo, hi; };
+__device__ __forceinline__ WideSeen wide_seen(const AttendArgs& a, int r, int length, int group) {
+  const int fresh = a.fresh ? min(max(a.fresh[r], 0), a.S) : a.S, col0 = group * CW_COLUMNS;
+  const int first = col0 / a.P, last = min((min(col0 + CW_COLUMNS, a.S * a.P) - 1) / a.P, fresh - 1);
+  return {min(max(length - fresh + min(first, fresh) + 1, 1), length), last < first ? 0 : min(max(length - fresh + last + 1, 0), length)};
+}
+
+template <typename T, int D, bool INT8>
+__global__ void __launch_bounds__(32 * CW_WARPS, 1) attend_wide_kernel(const AttendArgs a) {
+  using W = Wide<D>;
+  constexpr int CODE_PASSES = W::PASSES, PASS_ROWS = W::ROWS * CW_CODE_WARPS;
+  extern __shared__ uint8_t raw_smem[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(raw_smem) + 1023) & ~uintptr_t(1023));
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + W::BARS);
+  uint64_t *k_full = bars, *k_empty = bars + 2, *v_full = bars + 4, *v_empty = bars + 6, *s_full = bars + 8, *p_full = bars + 10;
+  uint64_t *meta_full = bars + 12, *q_full = bars + 16, *pv_done = bars + 17, *pair = bars + 18;
+  uint32_t* tmem_at = reinterpret_cast<uint32_t*>(bars + 22);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_at + 1);
+  int* before = reinterpret_cast<int*>(smem + W::BARS + 256);
+  int* lengths = before + a.R + 1;
+  // of the last four tiles: scales, whether a block exists, tokens whose values were NaN (32 of each warp that widens them)
+  __shared__ __align__(16) float4 s_scale[4][8];      // of keys; exponent and fraction of that of values
+  __shared__ uint32_t s_there[4];
+  __shared__ __align__(16) uint32_t s_nan[4][CW_CODE_WARPS];
+  __shared__ float2 s_top[2][2][CW_COLUMNS];           // what the two threads of a column tell each other
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, BT = 1 << a.shift;
+  if (tid == 0) {
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&k_full[i], CW_CODE_WARPS); mbar_init(&v_full[i], CW_CODE_WARPS); mbar_init(&k_empty[i], 1); mbar_init(&v_empty[i], 1);
+      mbar_init(&s_full[i], 1); mbar_init(&p_full[i], 8);
+    }
+    for (int i = 0; i < 4; ++i) { mbar_init(&meta_full[i], 1); mbar_init(&pair[i], 2); }
+    mbar_init(q_full, 8);
+    mbar_init(pv_done, 1);
+    *abort_flag = 0;
+    fence_mbar_init();
+  }
+  if (warp == 16) { tmem_alloc(tmem_at, 512); tmem_relinquish(); }
+  pdl_launch_next();
+  pdl_wait();
+  scan_units<CW_TILE, CW_START, CW_WARPS>(a, before, lengths);
+  tcgen05_fence_before();
+  __syncthreads();
+  tcgen05_fence_after();
+  const uint32_t tmem = *tmem_at, o_tmem = tmem + 256;      // scores: columns 0 .. 127 and 128 .. 255; weights: 384 .. 447 and 448 .. 511
+  const uint64_t timeout = a.timeout_ns;
+  bool ok = true;
+  WideWalk walk(a, before);
+  uint32_t cnt = 0;                        // tiles so far: buffers and phases
+
+  if (warp < 8) {                          // ------------------------------------------------ softmax
+    const int quarter = warp & 3, half = warp >> 2, row = quarter * 32 + lane;
+    const uint32_t lanes = static_cast<uint32_t>(quarter * 32) << 16;
+    uint32_t meets = 0;
+    auto meet = [&] {                      // the two warps of 32 columns
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&pair[quarter]);
+      const bool met = mbar_wait(&pair[quarter], meets++ & 1, abort_flag, timeout);
+      __syncwarp();
+      return met;
+    };
+    while (ok && walk.next(a, before)) {
+      const int length = lengths[walk.r], col0 = walk.group * CW_COLUMNS, cols = min(a.S * a.P - col0, CW_COLUMNS), c = col0 + row;
+      const int fresh = a.fresh ? min(max(a.fresh[walk.r], 0), a.S) : a.S;
+      const WideSeen see = wide_seen(a, walk.r, length, walk.group);
+      const int seen = row < cols && c / a.P < fresh ? min(max(length - fresh + c / a.P + 1, 0), length) : 0;
+      const bool mine = quarter * 32 < cols;      // of the warp
+      // queries: the products that read the ones before are done, their scores have been seen
+      float cscale = 0.f;
+      {
+        const T* q = static_cast<const T*>(a.q) + walk.r * a.q_row + (c / a.P) * a.q_token + walk.g * a.q_group + (c % a.P) * D;
+        float largest = 0.f;
+        auto value = [&](uint32_t w) {
+          if constexpr (__is_same(T, __half)) return __half22float2(*reinterpret_cast<const __half2*>(&w));
+          else return __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&w));
+        };
+        if (row < cols)
+#pragma unroll 4
+          for (int i = 0; i < D / 8; ++i) {
+            const uint4 u = __ldg(reinterpret_cast<const uint4*>(q) + i);
+            const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+            for (int j = 0; j < 4; ++j) { const float2 f = value(w[j]); largest = fmaxf(largest, fmaxf(fabsf(f.x), fabsf(f.y))); }
+          }
+        int e = static_cast<int>(__float_as_uint(largest) >> 23) - 127;      // as above: 2^(7 - e), scaled exactly
+        e = e > 127 || e < -126 ? 7 : max(e, -110);
+        const float up = copysignf(__uint_as_float(static_cast<uint32_t>(127 + 7 - e) << 23), a.scale_log2);      // so that the largest score is that of
+        cscale = __uint_as_float(static_cast<uint32_t>(127 + e - 7) << 23) * fabsf(a.scale_log2);               // the largest product
+#pragma unroll 4
+        for (int i = half * (D / 16); i < half * (D / 16) + D / 16; ++i) {
+          uint4 u = make_uint4(0u, 0u, 0u, 0u);
+          if (row < cols) {
+            u = __ldg(reinterpret_cast<const uint4*>(q) + i);
+            uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+            for (int j = 0; j < 4; ++j) { const float2 f = value(w[j]); w[j] = pack_f16(f.x * up, f.y * up); }
+            u = make_uint4(w[0], w[1], w[2], w[3]);
+          }
+          *reinterpret_cast<uint4*>(smem + W::at(row, i)) = u;
+        }
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(q_full);
+      }
+      float m1 = CA_LOWEST, m2 = CA_LOWEST, l = 0.f;
+      // the sums of columns that see a token whose values were NaN in tile t, the x-th so far
+      auto mend = [&](int t, uint32_t x) {
+        const uint4 some = *reinterpret_cast<const uint4*>(s_nan[x & 3]);
+        if ((some.x | some.y | some.z | some.w) == 0u) return;
+        for (int w = 0; w < CW_CODE_WARPS; ++w) {
+          uint32_t bad = s_nan[x & 3][w];
+          while (bad) {
+            const int bit = __ffs(bad) - 1, within = bit / W::ROWS * PASS_ROWS + w * W::ROWS + bit % W::ROWS, token = t * CW_TILE + within;
+            bad &= bad - 1;
+            const int id = a.tables[static_cast<size_t>(walk.r) * a.W + (token >> a.shift)];
+            const uint8_t* v = a.v + (((static_cast<size_t>(id) * a.G + walk.g) << a.shift) + (token & (BT - 1))) * D;
+            for (int b = half * (D / 64); b < half * (D / 64) + D / 64; ++b) {
+              uint32_t o[32];
+              tmem_ld_32x32(o_tmem + lanes + b * 32, o);
+              tmem_ld_wait(o);
+#pragma unroll
+              for (int i = 0; i < 32; ++i) if (token < seen && (v[b * 32 + i] & 0x7f) == 0x7f) o[i] = 0x7fffffffu;
+              tmem_st_32x32(o_tmem + lanes + b * 32, o);
+            }
+            tmem_st_wait();
+          }
+        }
+      };
+      for (int t = walk.t0; t < walk.t1; ++t, ++cnt) {
+        const uint32_t s_at = tmem + lanes + (cnt & 1) * 128, p_at = tmem + lanes + 384 + (cnt & 1) * 64;
+        if (!mbar_wait(&meta_full[cnt & 3], (cnt >> 2) & 1, abort_flag, timeout) ||
+            !mbar_wait(&s_full[cnt & 1], (cnt >> 1) & 1, abort_flag, timeout)) { ok = false; break; }
+        __syncwarp();
+        tcgen05_fence_after();
+        const uint32_t there = s_there[cnt & 3];
+        const bool ragged = t * CW_TILE + CW_TILE > see.lo || there != 0xffu;
+        // block b's scores of tokens that the column does not see
+        auto mask = [&](uint32_t* x, int b) {
+          const int end = there >> b & 1u ? seen - (t * CW_TILE + 16 * b) : 0;
+#pragma unroll
+          for (int i = 0; i < 16; ++i) if (i >= end) x[i] = 0xff800000u;
+        };
+        float g1 = -INFINITY, g2 = -INFINITY, e1 = 0.f;      // largest of the tile; sum of its weights
+        // weights for the references as they are, and the largest scores beside: where those are too far above, once more.  32 scores at a
+        // time, one copy of the code: seventeen warps' loops share the instruction cache.
+        auto weights = [&](bool write) {
+          float2 sum0 = make_float2(0.f, 0.f), sum1 = sum0;
+          g1 = g2 = -INFINITY;
+#pragma unroll 1
+          for (int b0 = 4 * half; b0 < 4 * half + 4; b0 += 2) {
+            uint32_t x[32], p[16];
+            tmem_ld_32x32(s_at + b0 * 16, x);
+            float4 scale[2];
+            float shift[2];
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              scale[h] = s_scale[cnt & 3][b0 + h];
+              const float f = cscale * scale[h].x;
+              scale[h].x = f < 1.17549435e-38f ? 1.17549435e-38f : f;      // above 0: -inf stays what it is
+              shift[h] = scale[h].y + m1 - m2;
+            }
+            tmem_ld_wait(x);
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              if (ragged) mask(x + h * 16, b0 + h);
+              float top[4];
+#pragma unroll
+              for (int i = 0; i < 4; ++i) {
+                const uint32_t* z = x + h * 16 + 4 * i;
+                top[i] = fmaxf(fmaxf(__uint_as_float(z[0]), __uint_as_float(z[1])), fmaxf(__uint_as_float(z[2]), __uint_as_float(z[3])));
+              }
+              const float y = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * scale[h].x;
+              g1 = fmaxf(g1, y);
+              g2 = fmaxf(g2, y + scale[h].y);
+            }
+            if (!write) continue;
+            // exp2(s + ev - m2) is exp2(s - m1) exp2(ev + m1 - m2), but where the latter would bring back what the former has lost
+            const bool apart = __any_sync(0xffffffffu, shift[0] > 60.f || shift[1] > 60.f);
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              const float2 f2 = make_float2(scale[h].x, scale[h].x), low = make_float2(-m1, -m1);
+              const float weight = exp2_fast(shift[h]) * scale[h].z;
+#pragma unroll
+              for (int i = 0; i < 8; ++i) {
+                const float2 z = make_float2(__uint_as_float(x[h * 16 + 2 * i]), __uint_as_float(x[h * 16 + 2 * i + 1]));
+                float2 e = __ffma2_rn(z, f2, low);
+                e.x = exp2_fast(e.x); e.y = exp2_fast(e.y);
+                if (i & 1) sum1 = __fadd2_rn(sum1, e); else sum0 = __fadd2_rn(sum0, e);
+                e = __fmul2_rn(e, make_float2(weight, weight));
+                p[h * 8 + i] = pack_f16(e.x, e.y);
+              }
+            }
+            if (apart)
+#pragma unroll
+              for (int h = 0; h < 2; ++h)
+#pragma unroll
+                for (int i = 0; i < 8; ++i)
+                  p[h * 8 + i] = pack_f16(exp2_fast(__uint_as_float(x[h * 16 + 2 * i]) * scale[h].x + scale[h].y - m2) * scale[h].z,
+                                          exp2_fast(__uint_as_float(x[h * 16 + 2 * i + 1]) * scale[h].x + scale[h].y - m2) * scale[h].z);
+            tmem_st_32x16(p_at + b0 * 8, p);
+          }
+          e1 = (sum0.x + sum0.y) + (sum1.x + sum1.y);
+        };
+        if (mine) {
+          weights(t > walk.t0);
+          s_top[cnt & 1][half][row] = make_float2(g1, g2);
+          if (!meet()) { ok = false; break; }
+          const float2 other = s_top[cnt & 1][half ^ 1][row];
+          g1 = fmaxf(g1, other.x); g2 = fmaxf(g2, other.y);
+        }
+        if (t > walk.t0) {
+          if (!mbar_wait(pv_done, (cnt - 1) & 1, abort_flag, timeout)) { ok = false; break; }
+          __syncwarp();
+          tcgen05_fence_after();
+          if (!INT8 && mine) mend(t - 1, cnt - 1);
+        }
+        if (mine) {
+          if (__any_sync(0xffffffffu, g1 > m1 + 8.f || g2 > m2 + 8.f) || t == walk.t0) {
+            const float n1 = fmaxf(m1, g1), n2 = fmaxf(m2, g2), f = exp2_fast(m2 - n2);
+            l *= exp2_fast(m1 - n1);
+            m1 = n1; m2 = n2;
+            if (t > walk.t0)
+#pragma unroll 1
+              for (int b = half * (D / 64); b < half * (D / 64) + D / 64; ++b) {
+                uint32_t o[32];
+                tmem_ld_32x32(o_tmem + lanes + b * 32, o);
+                tmem_ld_wait(o);
+#pragma unroll
+                for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * f);
+                tmem_st_32x32(o_tmem + lanes + b * 32, o);
+              }
+            weights(true);
+          }
+          l += e1;
+          tmem_st_wait();
+        }
+        tcgen05_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&p_full[cnt & 1]);
+      }
+      if (!ok || !mbar_wait(pv_done, (cnt - 1) & 1, abort_flag, timeout)) { ok = false; break; }
+      __syncwarp();
+      tcgen05_fence_after();
+      if (!INT8 && mine) mend(walk.t1 - 1, cnt - 1);
+      const bool starts = walk.t0 == 0, ends = walk.t1 == walk.tiles, whole = starts && ends;
+      const size_t slot = 2 * static_cast<size_t>(blockIdx.x) + starts;
+      if (tid == 0) {
+        int2* at = a.ends + static_cast<size_t>(walk.r) * a.G * a.groups + walk.item;
+        if (starts) at->x = whole ? -1 : static_cast<int>(slot);
+        if (ends) at->y = blockIdx.x;
+      }
+      if (mine) {
+        s_top[cnt & 1][half][row].x = l;
+        if (!meet()) { ok = false; break; }
+        l += s_top[cnt & 1][half ^ 1][row].x;
+        const float total = seen > 0 ? l : 0.f, f = total != 0.f ? exp2_fast(m2 - m1) / total : 0.f;
+        float* part = a.part + (slot * CW_COLUMNS + row) * (D + 4);
+        T* out = output_row<T>(a, walk.r, walk.g, c, D);
+#pragma unroll 1
+        for (int b = half * (D / 64); b < half * (D / 64) + D / 64; ++b) {
+          uint32_t o[32];
+          tmem_ld_32x32(o_tmem + lanes + b * 32, o);
+          tmem_ld_wait(o);
+          if (row >= cols) continue;
+#pragma unroll
+          for (int i = 0; i < 32; i += 8) {
+            if (whole) {
+              uint32_t w[4];
+#pragma unroll
+              for (int j = 0; j < 4; ++j)
+                w[j] = pack_row<T>(total != 0.f ? __uint_as_float(o[i + 2 * j]) * f : 0.f, total != 0.f ? __uint_as_float(o[i + 2 * j + 1]) * f : 0.f);
+              *reinterpret_cast<uint4*>(out + b * 32 + i) = make_uint4(w[0], w[1], w[2], w[3]);
+            } else {
+              *reinterpret_cast<uint4*>(part + b * 32 + i) = make_uint4(o[i], o[i + 1], o[i + 2], o[i + 3]);
+              *reinterpret_cast<uint4*>(part + b * 32 + i + 4) = make_uint4(o[i + 4], o[i + 5], o[i + 6], o[i + 7]);
+            }
+          }
+        }
+        if (!whole && row < cols && half == 0) *reinterpret_cast<float4*>(part + D) = make_float4(m1, m2, total, 0.f);
+      }
+      tcgen05_fence_before();              // the next sequence's first product follows this warp's next arrival
+    }
+    if (!ok && lane == 0) report_status(a.status, 0x443u);
+  } else if (warp < 16) {                  // ------------------------------------------------ codes: warps 8-11 keys, 12-15 values
+    const int w4 = warp & 3;
+    const bool keys = warp < 12;
+    uint64_t *full = keys ? k_full : v_full, *empty = keys ? k_empty : v_empty;
+    uint8_t* matrix = smem + (keys ? W::K : W::V);
+    const uint8_t* codes = keys ? a.k : a.v;
+    const int within = D == 128 ? ((lane >> 2) & 1) + 2 * (lane >> 4) : lane >> 2;      // row of the warp's; 16 bytes of it: pairs of rows
+    const int c16 = D == 128 ? (lane & 3) + 4 * ((lane >> 3) & 1) : lane & 3;           // share a store's banks
+    const int row0 = w4 * W::ROWS + within;
+    // what is on its way of a tile
+    struct Coming { uint4 x[CODE_PASSES]; float ks, vs; int lo; bool valid, there; };      // scales: of warp 8's lanes 0 .. 7
+    WideSeen see = {0, 0};
+    int length = 0, limit = 0, t = 0, ids = -1;      // lane i: block of tokens 16 i ..
+    const int* table = nullptr;
+    auto start = [&](bool fresh_piece) {
+      if (fresh_piece) {
+        length = lengths[walk.r];
+        see = wide_seen(a, walk.r, length, walk.group);
+        limit = keys ? length : see.hi;
+        table = a.tables + static_cast<size_t>(walk.r) * a.W;
+        t = walk.t0;
+      }
+      const int token = t * CW_TILE + 16 * lane;
+      ids = lane < 8 && token < length ? table[token >> a.shift] : -1;
+    };
+    bool have = walk.next(a, before);
+    if (have) start(true);
+    auto fetch = [&](Coming& s) {
+      s.valid = have;
+      if (!have) return;
+      const int id = ids >= 0 && ids < a.N ? ids : -1;
+      s.lo = see.lo - t * CW_TILE;
+#pragma unroll
+      for (int p = 0; p < CODE_PASSES; ++p) {
+        const int token = t * CW_TILE + p * PASS_ROWS + row0, block = __shfl_sync(0xffffffffu, id, (p * PASS_ROWS + w4 * W::ROWS) / 16);
+        s.x[p] = make_uint4(0u, 0u, 0u, 0u);
+        if (block >= 0 && token < limit)
+          s.x[p] = load_once(codes + ((((static_cast<size_t>(block) * a.G + walk.g) << a.shift) + (token & (BT - 1))) * D) + c16 * 16);
+      }
+      if (warp == 8) {
+        s.there = id >= 0;
+        const size_t head = static_cast<size_t>(max(id, 0)) * a.G + walk.g;
+        s.ks = id >= 0 ? a.ks[head] : 1.f;
+        s.vs = id >= 0 ? a.vs[head] : 1.f;
+      }
+      const bool fresh_piece = t + 1 == walk.t1;
+      if (fresh_piece) have = walk.next(a, before); else ++t;
+      if (have) start(fresh_piece);
+    };
+    auto widen_tile = [&](Coming& s) {
+      if (!mbar_wait(&empty[cnt & 1], ((cnt >> 1) & 1) ^ 1, abort_flag, timeout)) return false;
+      __syncwarp();
+      if (warp == 8) {
+        const uint32_t there = __ballot_sync(0xffffffffu, s.there);
+        const uint32_t vs = __float_as_uint(s.vs);       // 2^y z, 1 <= z < 2
+        if (lane < 8)
+          s_scale[cnt & 3][lane] = make_float4(s.ks, static_cast<float>(static_cast<int>(vs >> 23) - 127), __uint_as_float((vs & 0x7fffffu) | 0x3f800000u), 0.f);
+        if (lane == 0) s_there[cnt & 3] = there;
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&meta_full[cnt & 3]);
+      }
+      if (!INT8 && !keys) {
+        uint32_t bad_rows = 0u;
+        if (s.lo < CW_TILE) {
+#pragma unroll
+          for (int p = 0; p < CODE_PASSES; ++p) {
+            uint32_t w[4] = {s.x[p].x, s.x[p].y, s.x[p].z, s.x[p].w}, nan[4], any = 0u;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) { nan[j] = __vcmpeq4(w[j] & 0x7f7f7f7fu, 0x7f7f7f7fu); any |= nan[j]; }
+            const bool some = any != 0u && p * PASS_ROWS + row0 >= s.lo;
+            if (some) s.x[p] = make_uint4(w[0] & ~nan[0], w[1] & ~nan[1], w[2] & ~nan[2], w[3] & ~nan[3]);
+            const uint32_t lanes = __ballot_sync(0xffffffffu, some);
+#pragma unroll
+            for (int y = 0; y < W::ROWS; ++y) {
+              const uint32_t of_row = D == 128 ? (y & 1 ? 0xf0f0u : 0x0f0fu) << (y >> 1) * 16 : 0xfu << 4 * y;
+              if (lanes & of_row) bad_rows |= 1u << (p * W::ROWS + y);
+            }
+          }
+        }
+        if (lane == 0) s_nan[cnt & 3][w4] = bad_rows;
+      }
+#pragma unroll
+      for (int p = 0; p < CODE_PASSES; ++p) {
+        const uint32_t w[4] = {s.x[p].x, s.x[p].y, s.x[p].z, s.x[p].w};
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          uint4 f;
+          widen<INT8>(w[2 * h], f.x, f.y);
+          widen<INT8>(w[2 * h + 1], f.z, f.w);
+          *reinterpret_cast<uint4*>(matrix + (cnt & 1) * W::MATRIX + W::at(p * PASS_ROWS + row0, 2 * c16 + h)) = f;
+        }
+      }
+      fence_proxy_async_smem();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&full[cnt & 1]);
+      ++cnt;
+      return true;
+    };
+    Coming next;
+    for (fetch(next); next.valid; fetch(next))
+      if (!widen_tile(next)) { ok = false; break; }
+    if (!ok && lane == 0) report_status(a.status, 0x441u);
+  } else if (elect_one()) {                // ------------------------------------------------ products
+    const uint32_t idesc_s = umma_idesc(0, 0, 0, 128, 128), idesc_o = umma_idesc(0, 0, 1, 128, D);
+    const uint64_t q = umma_smem_desc(smem_u32(smem), 16, 1024);
+    auto scores = [&](uint32_t x) {        // of the x-th tile
+      if (!mbar_wait(&k_full[x & 1], (x >> 1) & 1, abort_flag, timeout)) return false;
+      tcgen05_fence_after();
+      const uint64_t kd = umma_smem_desc(smem_u32(smem + W::K + (x & 1) * W::MATRIX), 16, 1024);
+#pragma unroll
+      for (int i = 0; i < D / 16; ++i) {
+        const uint64_t off = ((i >> 2) * W::CHUNK + (i & 3) * 32) >> 4;
+        umma_f16(tmem + (x & 1) * 128, q + off, kd + off, idesc_s, i != 0 ? 1u : 0u);
+      }
+      umma_commit(&s_full[x & 1]);
+      umma_commit(&k_empty[x & 1]);
+      return true;
+    };
+    for (uint32_t piece = 0; ok && walk.next(a, before); ++piece) {
+      if (!mbar_wait(q_full, piece & 1, abort_flag, timeout) || !scores(cnt)) { ok = false; break; }
+      for (int t = walk.t0; t < walk.t1; ++t, ++cnt) {
+        if (t + 1 < walk.t1 && !scores(cnt + 1)) { ok = false; break; }
+        if (!mbar_wait(&p_full[cnt & 1], (cnt >> 1) & 1, abort_flag, timeout) ||
+            !mbar_wait(&v_full[cnt & 1], (cnt >> 1) & 1, abort_flag, timeout)) { ok = false; break; }
+        tcgen05_fence_after();
+        const uint64_t vd = umma_smem_desc(smem_u32(smem + W::V + (cnt & 1) * W::MATRIX), W::CHUNK, 1024);
+#pragma unroll
+        for (int i = 0; i < 8; ++i)        // 16 tokens each
+          umma_f16_ts(o_tmem, tmem + 384 + (cnt & 1) * 64 + i * 8, vd + ((i * 2048) >> 4), idesc_o, t > walk.t0 || i > 0 ? 1u : 0u);
+        umma_commit(&v_empty[cnt & 1]);
+        umma_commit(pv_done);
+      }
+    }
+    if (!ok) report_status(a.status, 0x442u);
+  }
+  tcgen05_fence_before();
+  __syncthreads();
+  if (warp == 16) { __syncwarp(); tcgen05_fence_after(); tmem_dealloc(tmem, 512); }
+}
+
+// ----------------------------------------------------------------------------- sequences that several blocks share
+
 constexpr int MERGE_WARPS = 8;
 
 // Adds up the partial sums of the sequences that several blocks share, in the order of their tokens, and writes zeros for requests
@@ -622,7 +1131,7 @@ __global__ void __launch_bounds__(32 * MERGE_WARPS) attend_merge_kernel(const At
   __shared__ __align__(16) float sums[MERGE_WARPS][D + 4];
   pdl_launch_next();
   pdl_wait();
-  const int lane = threadIdx.x & 31, w = threadIdx.x >> 5, per_tile = a.G * a.groups;
+  const int w = threadIdx.x >> 5, per_tile = a.G * a.groups;
   const int r = blockIdx.x / per_tile, item = blockIdx.x - r * per_tile, g = a.groups == 1 ? item : item / a.groups;
   const int2 ends = a.ends[blockIdx.x];
   const bool any = a.before[r + 1] != a.before[r];
@@ -654,8 +1163,9 @@ __global__ void __launch_bounds__(32 * MERGE_WARPS) attend_merge_kernel(const At
   }
 }
 
-// Of a tile's products, 8 or 16 columns: up to 8 queries fill the instruction's narrow side; more would read the cache twice with 8.
-static int attend_columns(int queries) { return queries <= 8 ? 8 : 16; }
+// Columns of a group.  24 requests of 4,096 tokens, 8 KV heads of 128 values, us with groups of 8, 16, 128 columns: 8 queries 40, 48, -;
+// 9 to 16 64, 51, -; 24 90, 84, 137; 64 240, 156, 155; 128 -, 295, 175; 512 -, 1178, 547.
+static int attend_columns(int queries) { return queries <= 8 ? 8 : queries <= 64 ? 16 : CW_COLUMNS; }
 static long long before_words(int rows) { return (rows + 1 + 3) / 4 * 4; }
 static long long ends_words(int rows, int G, int queries) {
   return (2ll * rows * G * ((queries + attend_columns(queries) - 1) / attend_columns(queries)) + 3) / 4 * 4;
@@ -676,7 +1186,25 @@ static int launch_attend(const AttendArgs& a, cudaStream_t stream) {
   AXB_CUDA(pdl_launch(attend_merge_kernel<T, D>, dim3(a.R * a.G * a.groups), dim3(32 * MERGE_WARPS), 0, stream, a, 8 * NT));
   return 0;
 }
+template <typename T, int D, bool INT8>
+static int launch_wide(const AttendArgs& a, cudaStream_t stream) {
+  constexpr size_t most = Wide<D>::FIXED + (2 * CA_MAX_ROWS + 1) * sizeof(int);
+  static bool configured[64] = {false};
+  auto kern = attend_wide_kernel<T, D, INT8>;
+  int device = 0;
+  AXB_CUDA(cudaGetDevice(&device));
+  if (!configured[device & 63]) {
+    AXB_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(most)));
+    configured[device & 63] = true;
+  }
+  AXB_CUDA(pdl_launch(kern, dim3(a.workers), dim3(32 * CW_WARPS), Wide<D>::FIXED + (2 * a.R + 1) * sizeof(int), stream, a));
+  AXB_CUDA(pdl_launch(attend_merge_kernel<T, D>, dim3(a.R * a.G * a.groups), dim3(32 * MERGE_WARPS), 0, stream, a, CW_COLUMNS));
+  return 0;
+}
 template <typename T> static int launch_attend(const AttendArgs& a, int D, bool int8, int columns, cudaStream_t stream) {
+  if (columns == CW_COLUMNS)
+    return D == 64 ? (int8 ? launch_wide<T, 64, true>(a, stream) : launch_wide<T, 64, false>(a, stream))
+                   : (int8 ? launch_wide<T, 128, true>(a, stream) : launch_wide<T, 128, false>(a, stream));
   if (columns == 8)
     return D == 64 ? (int8 ? launch_attend<T, 64, true, 1>(a, stream) : launch_attend<T, 64, false, 1>(a, stream))
                    : (int8 ? launch_attend<T, 128, true, 1>(a, stream) : launch_attend<T, 128, false, 1>(a, stream));
@@ -711,7 +1239,12 @@ extern "C" int axb_cached_attention(const void* q, long long q_row, long long q_
   }
   const int columns = attend_columns(S * P), groups = (S * P + columns - 1) / columns, blocks = sm_count_current();
   AttendArgs a{q, q_row, q_token, q_group, out, (const uint8_t*)k, (const uint8_t*)v, ks, vs, tables, lengths, fresh, R, S, G, P, W, N, shift,
-               groups, scale * 1.4426950408889634f, blocks, (int*)work, nullptr, nullptr};
+               groups, scale * 1.4426950408889634f, blocks, (int*)work, nullptr, nullptr, nullptr, wait_timeout_ns()};
+  if (columns == CW_COLUMNS) {
+    int device = 0;
+    AXB_CUDA(cudaGetDevice(&device));
+    if (!device_status_word(device, &a.status)) { set_error("cached_attention: no status word"); return -1; }
+  }
   // of the rows of a launch: their units, of very long tables, are counted in 31 bits
   const long long most = (static_cast<long long>(W) << shift < 0x7fffffffll ? static_cast<long long>(W) << shift : 0x7fffffffll) / CA_TILE + 1 + CA_START;
   const int rows = static_cast<int>(0x7fffffffll / most < CA_MAX_ROWS ? 0x7fffffffll / most : CA_MAX_ROWS);

@@ -251,6 +251,9 @@ _STATUS_NAMES = {
     0x431: "flash attention backward, dK / dV kernel: producer timed out",
     0x432: "flash attention backward, dK / dV kernel: MMA issuer timed out",
     0x433: "flash attention backward, dK / dV kernel: softmax warps timed out",
+    0x441: "attention over the block cache: warps that widen codes timed out",
+    0x442: "attention over the block cache: MMA issuer timed out",
+    0x443: "attention over the block cache: softmax warps timed out",
     0x151: "split-K GEMM producer timed out",
     0x152: "split-K GEMM MMA issuer timed out",
     0x154: "split-K GEMM epilogue timed out",

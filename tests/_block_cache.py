@@ -41,20 +41,19 @@ def attend64(q, layer, tables, lengths, new=None, scale=None):
     scale = D ** -0.5 if scale is None else scale
     out, size = torch.zeros(R, S, H, D, dtype=torch.float64), torch.zeros(R, S, H, D, dtype=torch.float64)
     for r, n in enumerate(lengths):
-        m = S if new is None else new[r]
-        for i in range(m):
-            seen = min(n - m + i + 1, tables.shape[1] * BT)
-            for g in range(G):
-                tokens = [(int(tables[r, t // BT]), t % BT) for t in range(max(seen, 0))]
-                tokens = [(b, t) for b, t in tokens if 0 <= b < k.shape[0]]
-                if not tokens:
-                    continue
-                b, t = (torch.tensor(x) for x in zip(*tokens))
-                K = k.float()[b, g, t].double() * ks[b, g].double()[:, None]
-                V = v.float()[b, g, t].double() * vs[b, g].double()[:, None]
-                h = slice(g * H // G, (g + 1) * H // G)
-                p = (q[r, i, h].double() @ K.T * scale).softmax(-1)
-                out[r, i, h], size[r, i, h] = p @ V, p @ V.abs()
+        m = S if new is None else min(new[r], S)
+        token = torch.arange(min(n, tables.shape[1] * BT))
+        block = tables[r].long()[token // BT]
+        token, block = (x[(block >= 0) & (block < k.shape[0])] for x in (token, block))
+        for g in range(G):
+            h = slice(g * H // G, (g + 1) * H // G)
+            K = k.float()[block, g, token % BT].double() * ks[block, g].double()[:, None]
+            V = v.float()[block, g, token % BT].double() * vs[block, g].double()[:, None]
+            for i in range(m):
+                seen = int((token < n - m + i + 1).sum())
+                if seen:
+                    p = (q[r, i, h].double() @ K[:seen].T * scale).softmax(-1)
+                    out[r, i, h], size[r, i, h] = p @ V[:seen], p @ V[:seen].abs()
     return out, size
 
 

@@ -522,3 +522,70 @@ def test_plan_from_any_number_of_taken_blocks(taken):
         return tables, *ops.plan_blocks(numbers[0], numbers[1], tables, numbers[2], numbers[3], 70, 16)
     for got, want in zip(plan("cuda"), plan("cpu")):
         assert torch.equal(got.cpu(), want)
+
+
+# ----------------------------------------------------------------------------- more than 64 query columns
+
+@pytest.mark.parametrize("S,G,P,D,codes,dtype", [(24, 2, 3, 128, E4M3, torch.bfloat16), (9, 1, 8, 64, INT8, torch.float16), (33, 2, 4, 128, INT8, torch.bfloat16),
+                                                 (9, 3, 8, 64, E4M3, torch.float16), (17, 1, 5, 128, E4M3, torch.float16), (130, 1, 1, 64, E4M3, torch.bfloat16),
+                                                 (1, 1, 72, 128, INT8, torch.bfloat16), (64, 1, 2, 128, INT8, torch.float16)])
+@pytest.mark.parametrize("BT", [16, 128])
+def test_attend_many_columns(S, G, P, D, codes, dtype, BT):
+    """Groups of 128 columns and what is left of them, tiles of 128 tokens and their borders, sequences that several blocks share."""
+    lengths = [700, 129, 128, S, 0, 1000, 1, 300, 127, 2600]
+    new = [S, S, max(S - 3, 1), S, 0, 1, 1, S + 5, 0, S]
+    W = -(-2600 // BT)
+    blocks = sum(-(-n // BT) for n in lengths) + 1
+    torch.manual_seed(S)
+    q = torch.randn(len(lengths), S, G * P, D).to(dtype)
+    cache, tables = make_cache(blocks, G, BT, D, codes), make_tables(lengths, W, BT, blocks)
+    out = _attend(q, cache, tables, lengths, new)
+    for r, m in enumerate(new):
+        assert not bool(out[r, max(m, 0):].any())
+    assert torch.equal(out, _attend(q, cache, tables, lengths, new))
+    tables[0, 1], tables[9, 3:2000 // BT] = -1, blocks + 7       # blocks that a table lacks, within a tile and several tiles long
+    _attend(q, cache, tables, lengths, new)
+
+
+@pytest.mark.parametrize("poison", [0x7f, 0xff])
+@pytest.mark.parametrize("D,BT", [(64, 16), (128, 64)])
+def test_what_many_columns_do_not_see_may_be_nan(poison, D, BT):
+    """NaN codes behind a sequence and in blocks of nobody; a stored NaN among the new tokens reaches the queries that see it alone."""
+    S, lengths = 20, [130, 20, 260, 31, 900]
+    W, blocks = -(-900 // BT), sum(-(-n // BT) for n in lengths) + 2
+    cache, tables = make_cache(blocks, 2, BT, D, E4M3), make_tables(lengths, W, BT, blocks)
+    used = torch.zeros(blocks, BT, dtype=torch.bool)
+    for r, n in enumerate(lengths):
+        for t in range(n):
+            used[int(tables[r, t // BT]), t % BT] = True
+    torch.manual_seed(1)
+    q = torch.randn(len(lengths), S, 8, D).bfloat16()
+    want = _attend(q, cache, tables, lengths)
+    bad = [t.clone() for t in cache]
+    for c in bad[:2]:
+        c.view(torch.uint8).transpose(1, 2)[~used] = poison
+    for s in bad[2:]:
+        s[~used.any(1)] = float("nan")
+    args = (q.to(DEV), ops.BlockLayer(*_gpu(*bad)), tables.to(DEV), torch.tensor(lengths, dtype=torch.int32, device=DEV))
+    assert torch.equal(ops.cached_attention(*args).cpu(), want)
+    for r, token in ((0, 127), (0, 128), (2, 245), (4, 899), (4, 880), (1, 7)):
+        for which in (0, 1):
+            worse = [x.clone() for x in bad]
+            worse[which].view(torch.uint8)[int(tables[r, token // BT]), 1, token % BT, 37] = poison
+            out = ops.cached_attention(args[0], ops.BlockLayer(*_gpu(*worse)), *args[2:]).cpu()
+            hit = torch.zeros_like(out, dtype=torch.bool)
+            hit[r, token - (lengths[r] - S):, 4:, :] = True if which == 0 else (torch.arange(D) == 37)
+            assert torch.equal(out[~hit], want[~hit]) and bool(out[hit].isnan().all())
+
+
+def test_attend_many_columns_and_blocks_of_very_different_scales():
+    """Scales of values from 2^-46 to 2^80: weights whose logarithms lie apart from their values'."""
+    BT, lengths = 16, [160, 64]
+    k, v, ks, vs = make_cache(14, 1, BT, 64, E4M3)
+    torch.manual_seed(2)
+    q = torch.randn(2, 9, 8, 64).bfloat16()
+    for top in (34.0, 80.0):
+        vs = torch.exp2(torch.tensor([-46.0, top, -6, -100, 0, 20, -20, 3, -30, 10, -6, -6, 7, -11]))[:, None]
+        _attend(q, (k, v, ks, vs), make_tables(lengths, 10, BT, 14), lengths)
+    for scale in (0.0, -0.07, 0.5):
+        _attend(q, (k, v, ks, torch.ones_like(vs)), make_tables(lengths, 10, BT, 14), lengths, scale=scale)
