@@ -3,8 +3,8 @@
 //   s = scale * ks * (q . k)      o = sum_t p_t vs v_t / sum_t p_t,   p = softmax of s over the tokens that a query sees
 //
 // What bounds it is reading 2 D bytes per token and KV head once.  A sequence here is the tokens of one request, KV head and group of up
-// to 8 or 16 query columns (query heads of the KV head x new tokens; 128 where there are more than 64, see below); its unit of work is a tile of 32 tokens, after a start that counts
-// as two.  One block per SM takes a run of units as long as every other block's, whatever the lengths of the requests, and its eight
+// to 8 or 16 query columns (query heads of the KV head x new tokens; 128 where there are more than 64, see below); its unit of work is a
+// tile of 32 tokens, after a start that counts as two.  One block per SM takes a run of units as long as every other block's, whatever the lengths of the requests, and its eight
 // warps equal parts of that: a run ends inside one sequence and goes on in the next.  A sequence that one warp has seen whole is written
 // at once; those that warps of a block share are put together in shared memory, those that blocks share by a second launch, always in
 // the order of the tokens: the same call gives the same bits.
@@ -619,16 +619,17 @@ __global__ void __launch_bounds__(32 * CA_WARPS, 1) attend_kernel(const AttendAr
 // ----------------------------------------------------------------------------- more than 64 query columns
 
 // The same sums on tcgen05, for groups of up to 128 columns (rows of the products: S = Q K^T, O = P V with M = 128): the codes of a tile of
-// 128 tokens are widened once for all of them.  24 requests of 4,096 tokens, 8 KV heads, 128 columns: 175 us (int8 155), 26 GFLOP of
-// products; 4,500 to 5,000 cycles a tile, of which the exponentials of a column's two threads are 1,700 (exp2 unit) and the rest is steps
-// that wait for one another: loads from tensor memory, the largest scores, the exchange between the two threads.  One block per SM, with
-// roles:
+// 128 tokens are widened once for all of them.  24 requests of 4,096 tokens, 8 KV heads, 128 columns: 158 us (int8 153), 52 GFLOP of
+// products; about 4,300 cycles a tile, of which the exp2 unit needs 1,000.  A warp's steps wait for one another (a load of 32 scores 300
+// cycles, their maximum 350, their weights 500), and two warps per scheduler do not hide that; registers allow no more.  With both threads
+// of a column on one tile, which have to meet in each, 175 us.  One block per SM, with roles:
 //
-//   warps 0-7   softmax, two threads per column (lane of tensor memory), which share a tile's tokens and a sequence's values: the queries
-//               into shared memory, then per tile the weights as fp16 back into tensor memory, and the sums at the end of a sequence
+//   warps 0-7   softmax, two threads per column (lane of tensor memory), for every other tile each, with sums of their own: the queries
+//               into shared memory, then per tile the largest score and the weights as fp16 in the place of the scores; at the end of a
+//               sequence both put its sums together
 //   warps 8-15  codes, of keys (8-11) and values: 16 bytes of a lane, a tile ahead in registers, widened to fp16 into shared memory
 //               (128-byte rows, swizzled)
-//   warp 16     the products: S(t + 1) is issued before O += P(t) V(t), two buffers of scores, keys and values each
+//   warp 16     the products: O += P(t) V(t), then S(t + 2) into the same buffer; two buffers of scores, sums, keys and values each
 //
 // Every wait is bounded.  What a column sees of a tile where it ends differs from column to column, and values that are NaN there must
 // not reach those that do not see them: they become zeros, and the sums of the columns that see them NaN, afterwards.
@@ -711,8 +712,8 @@ __global__ void __launch_bounds__(32 * CW_WARPS, 1) attend_wide_kernel(const Att
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(raw_smem) + 1023) & ~uintptr_t(1023));
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + W::BARS);
   uint64_t *k_full = bars, *k_empty = bars + 2, *v_full = bars + 4, *v_empty = bars + 6, *s_full = bars + 8, *p_full = bars + 10;
-  uint64_t *meta_full = bars + 12, *q_full = bars + 16, *pv_done = bars + 17, *pair = bars + 18;
-  uint32_t* tmem_at = reinterpret_cast<uint32_t*>(bars + 22);
+  uint64_t *meta_full = bars + 12, *q_full = bars + 16, *pv_done = bars + 17, *pair = bars + 19;
+  uint32_t* tmem_at = reinterpret_cast<uint32_t*>(bars + 23);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_at + 1);
   int* before = reinterpret_cast<int*>(smem + W::BARS + 256);
   int* lengths = before + a.R + 1;
@@ -720,16 +721,15 @@ __global__ void __launch_bounds__(32 * CW_WARPS, 1) attend_wide_kernel(const Att
   __shared__ __align__(16) float4 s_scale[4][8];      // of keys; exponent and fraction of that of values
   __shared__ uint32_t s_there[4];
   __shared__ __align__(16) uint32_t s_nan[4][CW_CODE_WARPS];
-  __shared__ float2 s_top[2][2][CW_COLUMNS];           // what the two threads of a column tell each other
+  __shared__ __align__(16) float4 s_state[2][CW_COLUMNS];      // of a column's two threads at the end of a sequence
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, BT = 1 << a.shift;
   if (tid == 0) {
     for (int i = 0; i < 2; ++i) {
       mbar_init(&k_full[i], CW_CODE_WARPS); mbar_init(&v_full[i], CW_CODE_WARPS); mbar_init(&k_empty[i], 1); mbar_init(&v_empty[i], 1);
-      mbar_init(&s_full[i], 1); mbar_init(&p_full[i], 8);
+      mbar_init(&s_full[i], 1); mbar_init(&p_full[i], 4); mbar_init(&pv_done[i], 1);
     }
     for (int i = 0; i < 4; ++i) { mbar_init(&meta_full[i], 1); mbar_init(&pair[i], 2); }
     mbar_init(q_full, 8);
-    mbar_init(pv_done, 1);
     *abort_flag = 0;
     fence_mbar_init();
   }
@@ -740,7 +740,7 @@ __global__ void __launch_bounds__(32 * CW_WARPS, 1) attend_wide_kernel(const Att
   tcgen05_fence_before();
   __syncthreads();
   tcgen05_fence_after();
-  const uint32_t tmem = *tmem_at, o_tmem = tmem + 256;      // scores: columns 0 .. 127 and 128 .. 255; weights: 384 .. 447 and 448 .. 511
+  const uint32_t tmem = *tmem_at;          // scores, then weights: columns 0 .. 127 and 128 .. 255; sums: 256 .. 383 and 384 .. 511
   const uint64_t timeout = a.timeout_ns;
   bool ok = true;
   WideWalk walk(a, before);
@@ -801,6 +801,7 @@ __global__ void __launch_bounds__(32 * CW_WARPS, 1) attend_wide_kernel(const Att
         if (lane == 0) mbar_arrive(q_full);
       }
       float m1 = CA_LOWEST, m2 = CA_LOWEST, l = 0.f;
+      const uint32_t s_at = tmem + lanes + half * 128, o_at = tmem + lanes + 256 + half * 128;
       // the sums of columns that see a token whose values were NaN in tile t, the x-th so far
       auto mend = [&](int t, uint32_t x) {
         const uint4 some = *reinterpret_cast<const uint4*>(s_nan[x & 3]);
@@ -812,55 +813,54 @@ __global__ void __launch_bounds__(32 * CW_WARPS, 1) attend_wide_kernel(const Att
             bad &= bad - 1;
             const int id = a.tables[static_cast<size_t>(walk.r) * a.W + (token >> a.shift)];
             const uint8_t* v = a.v + (((static_cast<size_t>(id) * a.G + walk.g) << a.shift) + (token & (BT - 1))) * D;
-            for (int b = half * (D / 64); b < half * (D / 64) + D / 64; ++b) {
+            for (int b = 0; b < D / 32; ++b) {
               uint32_t o[32];
-              tmem_ld_32x32(o_tmem + lanes + b * 32, o);
+              tmem_ld_32x32(o_at + b * 32, o);
               tmem_ld_wait(o);
 #pragma unroll
               for (int i = 0; i < 32; ++i) if (token < seen && (v[b * 32 + i] & 0x7f) == 0x7f) o[i] = 0x7fffffffu;
-              tmem_st_32x32(o_tmem + lanes + b * 32, o);
+              tmem_st_32x32(o_at + b * 32, o);
             }
             tmem_st_wait();
           }
         }
       };
+      int done = -1;                       // this warp's last tile
       for (int t = walk.t0; t < walk.t1; ++t, ++cnt) {
-        const uint32_t s_at = tmem + lanes + (cnt & 1) * 128, p_at = tmem + lanes + 384 + (cnt & 1) * 64;
+        if ((cnt & 1) != half) continue;
         if (!mbar_wait(&meta_full[cnt & 3], (cnt >> 2) & 1, abort_flag, timeout) ||
-            !mbar_wait(&s_full[cnt & 1], (cnt >> 1) & 1, abort_flag, timeout)) { ok = false; break; }
+            !mbar_wait(&s_full[half], (cnt >> 1) & 1, abort_flag, timeout)) { ok = false; break; }
         __syncwarp();
         tcgen05_fence_after();
         const uint32_t there = s_there[cnt & 3];
         const bool ragged = t * CW_TILE + CW_TILE > see.lo || there != 0xffu;
-        // block b's scores of tokens that the column does not see
-        auto mask = [&](uint32_t* x, int b) {
-          const int end = there >> b & 1u ? seen - (t * CW_TILE + 16 * b) : 0;
+        // 32 scores, masked where the column does not see their tokens, and the scales of their two blocks
+        auto scores = [&](int b0, uint32_t (&x)[32], float4 (&scale)[2]) {
+          tmem_ld_32x32(s_at + b0 * 16, x);
 #pragma unroll
-          for (int i = 0; i < 16; ++i) if (i >= end) x[i] = 0xff800000u;
-        };
-        float g1 = -INFINITY, g2 = -INFINITY, e1 = 0.f;      // largest of the tile; sum of its weights
-        // weights for the references as they are, and the largest scores beside: where those are too far above, once more.  32 scores at a
-        // time, one copy of the code: seventeen warps' loops share the instruction cache.
-        auto weights = [&](bool write) {
-          float2 sum0 = make_float2(0.f, 0.f), sum1 = sum0;
-          g1 = g2 = -INFINITY;
-#pragma unroll 1
-          for (int b0 = 4 * half; b0 < 4 * half + 4; b0 += 2) {
-            uint32_t x[32], p[16];
-            tmem_ld_32x32(s_at + b0 * 16, x);
-            float4 scale[2];
-            float shift[2];
+          for (int h = 0; h < 2; ++h) {
+            scale[h] = s_scale[cnt & 3][b0 + h];
+            const float f = cscale * scale[h].x;
+            scale[h].x = f < 1.17549435e-38f ? 1.17549435e-38f : f;      // above 0: -inf stays what it is
+          }
+          tmem_ld_wait(x);
+          if (ragged)
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
-              scale[h] = s_scale[cnt & 3][b0 + h];
-              const float f = cscale * scale[h].x;
-              scale[h].x = f < 1.17549435e-38f ? 1.17549435e-38f : f;      // above 0: -inf stays what it is
-              shift[h] = scale[h].y + m1 - m2;
+              const int end = there >> (b0 + h) & 1u ? seen - (t * CW_TILE + 16 * (b0 + h)) : 0;
+#pragma unroll
+              for (int i = 0; i < 16; ++i) if (i >= end) x[h * 16 + i] = 0xff800000u;
             }
-            tmem_ld_wait(x);
+        };
+        float g1 = -INFINITY, g2 = -INFINITY;
+        if (mine)
+#pragma unroll 1
+          for (int b0 = 0; b0 < 8; b0 += 2) {
+            uint32_t x[32];
+            float4 scale[2];
+            scores(b0, x, scale);
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
-              if (ragged) mask(x + h * 16, b0 + h);
               float top[4];
 #pragma unroll
               for (int i = 0; i < 4; ++i) {
@@ -871,8 +871,37 @@ __global__ void __launch_bounds__(32 * CW_WARPS, 1) attend_wide_kernel(const Att
               g1 = fmaxf(g1, y);
               g2 = fmaxf(g2, y + scale[h].y);
             }
-            if (!write) continue;
+          }
+        if (done >= 0) {                   // the sums so far: every phase of the barrier is seen, in order
+          if (!mbar_wait(&pv_done[half], ((cnt >> 1) & 1) ^ 1, abort_flag, timeout)) { ok = false; break; }
+          __syncwarp();
+          tcgen05_fence_after();
+          if (!INT8 && mine) mend(done, cnt - 2);
+        }
+        if (mine) {
+          if (__any_sync(0xffffffffu, g1 > m1 + 8.f || g2 > m2 + 8.f)) {
+            const float n1 = fmaxf(m1, g1), n2 = fmaxf(m2, g2), f = exp2_fast(m2 - n2);
+            l *= exp2_fast(m1 - n1);
+            m1 = n1; m2 = n2;
+            if (done >= 0)
+#pragma unroll 1
+              for (int b = 0; b < D / 32; ++b) {
+                uint32_t o[32];
+                tmem_ld_32x32(o_at + b * 32, o);
+                tmem_ld_wait(o);
+#pragma unroll
+                for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * f);
+                tmem_st_32x32(o_at + b * 32, o);
+              }
+          }
+          float2 sum0 = make_float2(0.f, 0.f), sum1 = sum0;
+#pragma unroll 1
+          for (int b0 = 0; b0 < 8; b0 += 2) {      // the weights of 32 scores take the place of the first 16 of them, or of earlier ones
+            uint32_t x[32], p[16];
+            float4 scale[2];
+            scores(b0, x, scale);
             // exp2(s + ev - m2) is exp2(s - m1) exp2(ev + m1 - m2), but where the latter would bring back what the former has lost
+            const float shift[2] = {scale[0].y + m1 - m2, scale[1].y + m1 - m2};
             const bool apart = __any_sync(0xffffffffu, shift[0] > 60.f || shift[1] > 60.f);
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
@@ -880,8 +909,7 @@ __global__ void __launch_bounds__(32 * CW_WARPS, 1) attend_wide_kernel(const Att
               const float weight = exp2_fast(shift[h]) * scale[h].z;
 #pragma unroll
               for (int i = 0; i < 8; ++i) {
-                const float2 z = make_float2(__uint_as_float(x[h * 16 + 2 * i]), __uint_as_float(x[h * 16 + 2 * i + 1]));
-                float2 e = __ffma2_rn(z, f2, low);
+                float2 e = __ffma2_rn(make_float2(__uint_as_float(x[h * 16 + 2 * i]), __uint_as_float(x[h * 16 + 2 * i + 1])), f2, low);
                 e.x = exp2_fast(e.x); e.y = exp2_fast(e.y);
                 if (i & 1) sum1 = __fadd2_rn(sum1, e); else sum0 = __fadd2_rn(sum0, e);
                 e = __fmul2_rn(e, make_float2(weight, weight));
@@ -895,51 +923,30 @@ __global__ void __launch_bounds__(32 * CW_WARPS, 1) attend_wide_kernel(const Att
                 for (int i = 0; i < 8; ++i)
                   p[h * 8 + i] = pack_f16(exp2_fast(__uint_as_float(x[h * 16 + 2 * i]) * scale[h].x + scale[h].y - m2) * scale[h].z,
                                           exp2_fast(__uint_as_float(x[h * 16 + 2 * i + 1]) * scale[h].x + scale[h].y - m2) * scale[h].z);
-            tmem_st_32x16(p_at + b0 * 8, p);
+            tmem_st_32x16(s_at + b0 * 8, p);
           }
-          e1 = (sum0.x + sum0.y) + (sum1.x + sum1.y);
-        };
-        if (mine) {
-          weights(t > walk.t0);
-          s_top[cnt & 1][half][row] = make_float2(g1, g2);
-          if (!meet()) { ok = false; break; }
-          const float2 other = s_top[cnt & 1][half ^ 1][row];
-          g1 = fmaxf(g1, other.x); g2 = fmaxf(g2, other.y);
-        }
-        if (t > walk.t0) {
-          if (!mbar_wait(pv_done, (cnt - 1) & 1, abort_flag, timeout)) { ok = false; break; }
-          __syncwarp();
-          tcgen05_fence_after();
-          if (!INT8 && mine) mend(t - 1, cnt - 1);
-        }
-        if (mine) {
-          if (__any_sync(0xffffffffu, g1 > m1 + 8.f || g2 > m2 + 8.f) || t == walk.t0) {
-            const float n1 = fmaxf(m1, g1), n2 = fmaxf(m2, g2), f = exp2_fast(m2 - n2);
-            l *= exp2_fast(m1 - n1);
-            m1 = n1; m2 = n2;
-            if (t > walk.t0)
-#pragma unroll 1
-              for (int b = half * (D / 64); b < half * (D / 64) + D / 64; ++b) {
-                uint32_t o[32];
-                tmem_ld_32x32(o_tmem + lanes + b * 32, o);
-                tmem_ld_wait(o);
-#pragma unroll
-                for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * f);
-                tmem_st_32x32(o_tmem + lanes + b * 32, o);
-              }
-            weights(true);
-          }
-          l += e1;
+          l += (sum0.x + sum0.y) + (sum1.x + sum1.y);
           tmem_st_wait();
         }
         tcgen05_fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive(&p_full[cnt & 1]);
+        if (lane == 0) mbar_arrive(&p_full[half]);
+        done = t;
       }
-      if (!ok || !mbar_wait(pv_done, (cnt - 1) & 1, abort_flag, timeout)) { ok = false; break; }
-      __syncwarp();
+      if (!ok) break;
+      if (done >= 0) {                     // the warp's last tile was the piece's last or the one before
+        const uint32_t x = cnt - (walk.t1 - done);
+        if (!mbar_wait(&pv_done[half], (x >> 1) & 1, abort_flag, timeout)) { ok = false; break; }
+        __syncwarp();
+        tcgen05_fence_after();
+        if (!INT8 && mine) mend(done, x);
+      }
+      // both halves of the tiles: each thread puts half of the values together
+      s_state[half][row] = make_float4(m1, m2, l, done >= 0 ? 1.f : 0.f);
+      tcgen05_fence_before();
+      if (!meet()) { ok = false; break; }
       tcgen05_fence_after();
-      if (!INT8 && mine) mend(walk.t1 - 1, cnt - 1);
+      const float4 other = s_state[half ^ 1][row];
       const bool starts = walk.t0 == 0, ends = walk.t1 == walk.tiles, whole = starts && ends;
       const size_t slot = 2 * static_cast<size_t>(blockIdx.x) + starts;
       if (tid == 0) {
@@ -948,35 +955,47 @@ __global__ void __launch_bounds__(32 * CW_WARPS, 1) attend_wide_kernel(const Att
         if (ends) at->y = blockIdx.x;
       }
       if (mine) {
-        s_top[cnt & 1][half][row].x = l;
-        if (!meet()) { ok = false; break; }
-        l += s_top[cnt & 1][half ^ 1][row].x;
-        const float total = seen > 0 ? l : 0.f, f = total != 0.f ? exp2_fast(m2 - m1) / total : 0.f;
+        const float n1 = fmaxf(m1, other.x), n2 = fmaxf(m2, other.y);
+        const float w0 = exp2_fast((half ? other.y : m2) - n2), w1 = exp2_fast((half ? m2 : other.y) - n2);
+        const bool first = half ? other.w != 0.f : done >= 0, second = half ? done >= 0 : other.w != 0.f;
+        // the first half's sum first, whichever thread adds
+        const float l0 = (half ? other.z : l) * exp2_fast((half ? other.x : m1) - n1), l1 = (half ? l : other.z) * exp2_fast((half ? m1 : other.x) - n1);
+        const float total = seen > 0 ? l0 + l1 : 0.f, f = total != 0.f ? exp2_fast(n2 - n1) / total : 0.f;
         float* part = a.part + (slot * CW_COLUMNS + row) * (D + 4);
         T* out = output_row<T>(a, walk.r, walk.g, c, D);
 #pragma unroll 1
         for (int b = half * (D / 64); b < half * (D / 64) + D / 64; ++b) {
-          uint32_t o[32];
-          tmem_ld_32x32(o_tmem + lanes + b * 32, o);
-          tmem_ld_wait(o);
+          float o[32];
+#pragma unroll
+          for (int i = 0; i < 32; ++i) o[i] = 0.f;
+#pragma unroll 1
+          for (int k = 0; k < 2; ++k) {
+            if (!(k ? second : first)) continue;
+            uint32_t x[32];
+            tmem_ld_32x32(tmem + lanes + 256 + k * 128 + b * 32, x);
+            tmem_ld_wait(x);
+            const float w = k ? w1 : w0;
+#pragma unroll
+            for (int i = 0; i < 32; ++i) o[i] += w * __uint_as_float(x[i]);
+          }
           if (row >= cols) continue;
 #pragma unroll
           for (int i = 0; i < 32; i += 8) {
             if (whole) {
               uint32_t w[4];
 #pragma unroll
-              for (int j = 0; j < 4; ++j)
-                w[j] = pack_row<T>(total != 0.f ? __uint_as_float(o[i + 2 * j]) * f : 0.f, total != 0.f ? __uint_as_float(o[i + 2 * j + 1]) * f : 0.f);
+              for (int j = 0; j < 4; ++j) w[j] = pack_row<T>(total != 0.f ? o[i + 2 * j] * f : 0.f, total != 0.f ? o[i + 2 * j + 1] * f : 0.f);
               *reinterpret_cast<uint4*>(out + b * 32 + i) = make_uint4(w[0], w[1], w[2], w[3]);
             } else {
-              *reinterpret_cast<uint4*>(part + b * 32 + i) = make_uint4(o[i], o[i + 1], o[i + 2], o[i + 3]);
-              *reinterpret_cast<uint4*>(part + b * 32 + i + 4) = make_uint4(o[i + 4], o[i + 5], o[i + 6], o[i + 7]);
+              *reinterpret_cast<float4*>(part + b * 32 + i) = make_float4(o[i], o[i + 1], o[i + 2], o[i + 3]);
+              *reinterpret_cast<float4*>(part + b * 32 + i + 4) = make_float4(o[i + 4], o[i + 5], o[i + 6], o[i + 7]);
             }
           }
         }
-        if (!whole && row < cols && half == 0) *reinterpret_cast<float4*>(part + D) = make_float4(m1, m2, total, 0.f);
+        if (!whole && row < cols && half == 0) *reinterpret_cast<float4*>(part + D) = make_float4(n1, n2, total, 0.f);
       }
-      tcgen05_fence_before();              // the next sequence's first product follows this warp's next arrival
+      tcgen05_fence_before();              // the next sequence's first products follow both warps' reads
+      if (!meet()) { ok = false; break; }
     }
     if (!ok && lane == 0) report_status(a.status, 0x443u);
   } else if (warp < 16) {                  // ------------------------------------------------ codes: warps 8-11 keys, 12-15 values
@@ -1098,18 +1117,18 @@ __global__ void __launch_bounds__(32 * CW_WARPS, 1) attend_wide_kernel(const Att
       return true;
     };
     for (uint32_t piece = 0; ok && walk.next(a, before); ++piece) {
-      if (!mbar_wait(q_full, piece & 1, abort_flag, timeout) || !scores(cnt)) { ok = false; break; }
+      if (!mbar_wait(q_full, piece & 1, abort_flag, timeout) || !scores(cnt) || (walk.t0 + 1 < walk.t1 && !scores(cnt + 1))) { ok = false; break; }
       for (int t = walk.t0; t < walk.t1; ++t, ++cnt) {
-        if (t + 1 < walk.t1 && !scores(cnt + 1)) { ok = false; break; }
         if (!mbar_wait(&p_full[cnt & 1], (cnt >> 1) & 1, abort_flag, timeout) ||
             !mbar_wait(&v_full[cnt & 1], (cnt >> 1) & 1, abort_flag, timeout)) { ok = false; break; }
         tcgen05_fence_after();
         const uint64_t vd = umma_smem_desc(smem_u32(smem + W::V + (cnt & 1) * W::MATRIX), W::CHUNK, 1024);
 #pragma unroll
         for (int i = 0; i < 8; ++i)        // 16 tokens each
-          umma_f16_ts(o_tmem, tmem + 384 + (cnt & 1) * 64 + i * 8, vd + ((i * 2048) >> 4), idesc_o, t > walk.t0 || i > 0 ? 1u : 0u);
+          umma_f16_ts(tmem + 256 + (cnt & 1) * 128, tmem + (cnt & 1) * 128 + i * 8, vd + ((i * 2048) >> 4), idesc_o, t > walk.t0 + 1 || i > 0 ? 1u : 0u);
         umma_commit(&v_empty[cnt & 1]);
-        umma_commit(pv_done);
+        umma_commit(&pv_done[cnt & 1]);
+        if (t + 2 < walk.t1 && !scores(cnt + 2)) { ok = false; break; }
       }
     }
     if (!ok) report_status(a.status, 0x442u);
@@ -1164,7 +1183,7 @@ __global__ void __launch_bounds__(32 * MERGE_WARPS) attend_merge_kernel(const At
 }
 
 // Columns of a group.  24 requests of 4,096 tokens, 8 KV heads of 128 values, us with groups of 8, 16, 128 columns: 8 queries 40, 48, -;
-// 9 to 16 64, 51, -; 24 90, 84, 137; 64 240, 156, 155; 128 -, 295, 175; 512 -, 1178, 547.
+// 9 to 16 64, 51, -; 24 90, 84, 137; 64 240, 156, 155; 128 -, 295, 158; 512 -, 1178, 482.
 static int attend_columns(int queries) { return queries <= 8 ? 8 : queries <= 64 ? 16 : CW_COLUMNS; }
 static long long before_words(int rows) { return (rows + 1 + 3) / 4 * 4; }
 static long long ends_words(int rows, int G, int queries) {
