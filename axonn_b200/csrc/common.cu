@@ -32,9 +32,12 @@ volatile unsigned int* device_status_word(int device, unsigned int** dev_ptr) {
   if (device < 0 || device >= 64) return nullptr;
   if (!g_status_host[device]) {
     unsigned int* h = nullptr;
-    if (cudaHostAlloc(reinterpret_cast<void**>(&h), 64, cudaHostAllocMapped | cudaHostAllocPortable) !=
-        cudaSuccess)
-      return nullptr;
+    // the first call may be one that is being captured: the allocation is not part of the graph
+    cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
+    cudaThreadExchangeStreamCaptureMode(&mode);
+    const cudaError_t e = cudaHostAlloc(reinterpret_cast<void**>(&h), 64, cudaHostAllocMapped | cudaHostAllocPortable);
+    cudaThreadExchangeStreamCaptureMode(&mode);
+    if (e != cudaSuccess) return nullptr;
     for (int i = 0; i < 16; ++i) h[i] = 0;
     unsigned int* d = nullptr;
     if (cudaHostGetDevicePointer(reinterpret_cast<void**>(&d), h, 0) != cudaSuccess) return nullptr;

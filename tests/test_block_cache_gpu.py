@@ -1,5 +1,9 @@
 """The block cache's kernels against 64-bit oracles (``_block_cache.py``) and, where results are exact, to the bit."""
 
+import os
+import subprocess
+import sys
+
 import pytest
 import torch
 
@@ -589,3 +593,58 @@ def test_attend_many_columns_and_blocks_of_very_different_scales():
         _attend(q, (k, v, ks, vs), make_tables(lengths, 10, BT, 14), lengths)
     for scale in (0.0, -0.07, 0.5):
         _attend(q, (k, v, ks, torch.ones_like(vs)), make_tables(lengths, 10, BT, 14), lengths, scale=scale)
+
+
+_CAPTURED_FIRST = """
+import torch
+from axonn_b200 import ops
+torch.manual_seed(0)
+layer = ops.BlockLayer(*(torch.randint(0, 100, (40, 1, 64, 64), dtype=torch.int8, device="cuda") for _ in range(2)),
+                       *(torch.full((40, 1), 2.0 ** -6, device="cuda") for _ in range(2)))
+tables = torch.arange(40, dtype=torch.int32, device="cuda").view(2, 20)
+lengths = torch.tensor([1200, 77], dtype=torch.int32, device="cuda")
+q = torch.zeros(2, 9, 8, 64, dtype=torch.bfloat16, device="cuda")
+graphs, outs = [], []
+for _ in range(2):
+    graphs.append(torch.cuda.CUDAGraph())
+    with torch.cuda.graph(graphs[-1]):
+        outs.append(ops.cached_attention(q, layer, tables, lengths))
+streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+for _ in range(3):
+    q.normal_()
+    torch.cuda.synchronize()
+    for g, s in zip(graphs, streams):
+        with torch.cuda.stream(s):
+            g.replay()
+    torch.cuda.synchronize()
+    want = ops.cached_attention(q, layer, tables, lengths)
+    assert all(torch.equal(o, want) for o in outs) and bool(want.any())
+print("same")
+"""
+
+
+def test_attend_many_columns_captured_first():
+    """The process's first call is captured, twice; both graphs replay on two streams at once."""
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    out = subprocess.run([sys.executable, "-c", _CAPTURED_FIRST], cwd=root, capture_output=True, text=True, timeout=300)
+    assert out.returncode == 0 and "same" in out.stdout, out.stderr[-2000:]
+
+
+def test_attend_many_columns_of_strided_queries_on_another_stream():
+    """Queries as the view of a packed projection, more requests than one launch counts; the same bits every time."""
+    torch.manual_seed(1)
+    R, S = 1030, 9
+    lengths = [(7 * r) % 150 for r in range(R)]
+    blocks = sum(-(-n // 16) for n in lengths)
+    qkv = torch.randn(R, S, 1, 10, 64).bfloat16()
+    cache, tables = make_cache(blocks, 1, 16, 64, INT8), make_tables(lengths, 10, 16, blocks)
+    args = (ops.BlockLayer(*_gpu(*cache)), tables.to(DEV), torch.tensor(lengths, dtype=torch.int32, device=DEV))
+    there = qkv.to(DEV)
+    torch.cuda.synchronize()
+    with torch.cuda.stream(torch.cuda.Stream()):
+        got = [ops.cached_attention(there[:, :, :, :-2], *args) for _ in range(3)]
+        torch.cuda.current_stream().synchronize()
+    assert all(torch.equal(g, got[0]) for g in got)
+    some = [0, 1, 22, 149, 700, 1023, 1024, 1025, 1029]
+    want, size = attend64(qkv[some, :, 0, :-2], cache, tables[some], [lengths[r] for r in some])
+    assert bool(((got[0][some].cpu().double() - want).abs() <= attend_bound(want, size, torch.bfloat16) + 2.0 ** -24).all())
