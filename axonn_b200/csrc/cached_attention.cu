@@ -3,7 +3,7 @@
 //   s = scale * ks * (q . k)      o = sum_t p_t vs v_t / sum_t p_t,   p = softmax of s over the tokens that a query sees
 //
 // What bounds it is reading 2 D bytes per token and KV head once.  A sequence here is the tokens of one request, KV head and group of up
-// to 8 or 16 query columns (query heads of the KV head x new tokens; 128 where there are more than 64, see below); its unit of work is a
+// to 8 or 16 query columns (query heads of the KV head x new tokens; 128 where there are more than 48, see below); its unit of work is a
 // tile of 32 tokens, after a start that counts as two.  One block per SM takes a run of units as long as every other block's, whatever the lengths of the requests, and its eight
 // warps equal parts of that: a run ends inside one sequence and goes on in the next.  A sequence that one warp has seen whole is written
 // at once; those that warps of a block share are put together in shared memory, those that blocks share by a second launch, always in
@@ -616,13 +616,13 @@ __global__ void __launch_bounds__(32 * CA_WARPS, 1) attend_kernel(const AttendAr
   }
 }
 
-// ----------------------------------------------------------------------------- more than 64 query columns
+// ----------------------------------------------------------------------------- more than 48 query columns
 
 // The same sums on tcgen05, for groups of up to 128 columns (rows of the products: S = Q K^T, O = P V with M = 128): the codes of a tile of
-// 128 tokens are widened once for all of them.  24 requests of 4,096 tokens, 8 KV heads, 128 columns: 158 us (int8 153), 52 GFLOP of
-// products; about 4,300 cycles a tile, of which the exp2 unit needs 1,000.  A warp's steps wait for one another (a load of 32 scores 300
+// 128 tokens are widened once for all of them.  24 requests of 4,096 tokens, 8 KV heads, 128 columns: 140 us (int8 136), 52 GFLOP of
+// products; about 4,000 cycles a tile, of which the exp2 unit needs 1,000.  A warp's steps wait for one another (a load of 32 scores 300
 // cycles, their maximum 350, their weights 500), and two warps per scheduler do not hide that; registers allow no more.  With both threads
-// of a column on one tile, which have to meet in each, 175 us.  One block per SM, with roles:
+// of a column on one tile, which have to meet in each, 17 us more.  One block per SM, with roles:
 //
 //   warps 0-7   softmax, two threads per column (lane of tensor memory), for every other tile each, with sums of their own: the queries
 //               into shared memory, then per tile the largest score and the weights as fp16 in the place of the scores; at the end of a
@@ -1143,7 +1143,7 @@ __global__ void __launch_bounds__(32 * CW_WARPS, 1) attend_wide_kernel(const Att
 constexpr int MERGE_WARPS = 8;
 
 // Adds up the partial sums of the sequences that several blocks share, in the order of their tokens, and writes zeros for requests
-// without tokens.  One block per sequence (request, KV head, group of columns); its warps share columns and parts.  Latency: 3 to 4 us
+// without tokens.  A block per eight columns of a sequence (request, KV head, group of columns); its warps share columns and parts.  Latency: 3 to 4 us
 // behind the first launch, at 4 MB of partial sums at most.
 template <typename T, int D>
 __global__ void __launch_bounds__(32 * MERGE_WARPS) attend_merge_kernel(const AttendArgs a, int columns) {
@@ -1161,7 +1161,7 @@ __global__ void __launch_bounds__(32 * MERGE_WARPS) attend_merge_kernel(const At
   int share = 1;
   while (2 * share * cols <= MERGE_WARPS && 4 * share < parts) share *= 2;
   const int per = (parts + share - 1) / share;
-  for (int c0 = 0; c0 < cols; c0 += MERGE_WARPS / share) {
+  for (int c0 = blockIdx.y * (MERGE_WARPS / share); c0 < cols; c0 += gridDim.y * (MERGE_WARPS / share)) {
     const int cc = c0 + w / share, mine = w % share, end = min(parts, mine * per + per);
     Partial<D / 32> p;
     const int x0 = mine * per;
@@ -1183,8 +1183,9 @@ __global__ void __launch_bounds__(32 * MERGE_WARPS) attend_merge_kernel(const At
 }
 
 // Columns of a group.  24 requests of 4,096 tokens, 8 KV heads of 128 values, us with groups of 8, 16, 128 columns: 8 queries 40, 48, -;
-// 9 to 16 64, 51, -; 24 90, 84, 137; 64 240, 156, 155; 128 -, 295, 158; 512 -, 1178, 482.
-static int attend_columns(int queries) { return queries <= 8 ? 8 : queries <= 64 ? 16 : CW_COLUMNS; }
+// 9 to 16 64, 50, -; 24 90, 84, 124; 48 -, 121, 127; 56 -, 155, 128; 64 240, 156, 129; 128 -, 295, 140; 512 -, 1178, 476.  1,000 tokens, 64
+// values, int8: 48 queries -, 36, 39.5; 56 -, 43, 40.
+static int attend_columns(int queries) { return queries <= 8 ? 8 : queries <= 48 ? 16 : CW_COLUMNS; }
 static long long before_words(int rows) { return (rows + 1 + 3) / 4 * 4; }
 static long long ends_words(int rows, int G, int queries) {
   return (2ll * rows * G * ((queries + attend_columns(queries) - 1) / attend_columns(queries)) + 3) / 4 * 4;
@@ -1202,7 +1203,7 @@ static int launch_attend(const AttendArgs& a, cudaStream_t stream) {
     configured[device & 63] = true;
   }
   AXB_CUDA(pdl_launch(kern, dim3(a.workers), dim3(32 * CA_WARPS), ring + (2 * a.R + 1) * sizeof(int), stream, a));
-  AXB_CUDA(pdl_launch(attend_merge_kernel<T, D>, dim3(a.R * a.G * a.groups), dim3(32 * MERGE_WARPS), 0, stream, a, 8 * NT));
+  AXB_CUDA(pdl_launch(attend_merge_kernel<T, D>, dim3(a.R * a.G * a.groups, NT), dim3(32 * MERGE_WARPS), 0, stream, a, 8 * NT));
   return 0;
 }
 template <typename T, int D, bool INT8>
@@ -1217,7 +1218,7 @@ static int launch_wide(const AttendArgs& a, cudaStream_t stream) {
     configured[device & 63] = true;
   }
   AXB_CUDA(pdl_launch(kern, dim3(a.workers), dim3(32 * CW_WARPS), Wide<D>::FIXED + (2 * a.R + 1) * sizeof(int), stream, a));
-  AXB_CUDA(pdl_launch(attend_merge_kernel<T, D>, dim3(a.R * a.G * a.groups), dim3(32 * MERGE_WARPS), 0, stream, a, CW_COLUMNS));
+  AXB_CUDA(pdl_launch(attend_merge_kernel<T, D>, dim3(a.R * a.G * a.groups, CW_COLUMNS / 8), dim3(32 * MERGE_WARPS), 0, stream, a, CW_COLUMNS));
   return 0;
 }
 template <typename T> static int launch_attend(const AttendArgs& a, int D, bool int8, int columns, cudaStream_t stream) {

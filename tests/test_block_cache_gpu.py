@@ -528,7 +528,7 @@ def test_plan_from_any_number_of_taken_blocks(taken):
         assert torch.equal(got.cpu(), want)
 
 
-# ----------------------------------------------------------------------------- more than 64 query columns
+# ----------------------------------------------------------------------------- more than 48 query columns
 
 @pytest.mark.parametrize("S,G,P,D,codes,dtype", [(24, 2, 3, 128, E4M3, torch.bfloat16), (9, 1, 8, 64, INT8, torch.float16), (33, 2, 4, 128, INT8, torch.bfloat16),
                                                  (9, 3, 8, 64, E4M3, torch.float16), (17, 1, 5, 128, E4M3, torch.float16), (130, 1, 1, 64, E4M3, torch.bfloat16),
