@@ -734,12 +734,12 @@ __global__ void __launch_bounds__(32 * CW_WARPS, 1) attend_wide_kernel(const Att
     fence_mbar_init();
   }
   if (warp == 16) { tmem_alloc(tmem_at, 512); tmem_relinquish(); }
-  pdl_launch_next();
-  pdl_wait();
-  scan_units<CW_TILE, CW_START, CW_WARPS>(a, before, lengths);
   tcgen05_fence_before();
   __syncthreads();
   tcgen05_fence_after();
+  pdl_launch_next();                       // the tensor memory is this block's
+  pdl_wait();
+  scan_units<CW_TILE, CW_START, CW_WARPS>(a, before, lengths);      // ends in a barrier
   const uint32_t tmem = *tmem_at;          // scores, then weights: columns 0 .. 127 and 128 .. 255; sums: 256 .. 383 and 384 .. 511
   const uint64_t timeout = a.timeout_ns;
   bool ok = true;
