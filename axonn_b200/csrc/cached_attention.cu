@@ -20,12 +20,14 @@
 // side of the instruction; O^T = V^T P^T (rows = values of the head).  Which value of a head is which row or k index is free as long as
 // both operands agree, and is chosen such that every thread reads 16 consecutive bytes: of K 16 values of its token, of V 16 values of
 // each of its four tokens, whose bytes are then interleaved pairwise.  Codes become fp16, which holds them exactly; queries are scaled
-// by a power of two into fp16 (2^-11 of the largest at 16-bit inputs: exact but for values below 2^-21 of a row's largest), probabilities
-// are rounded to fp16 (2^-11 each).  Scores, sums and outputs are 32-bit.
+// by a power of two into fp16 (exact but for values below 2^-21 of a row's largest at 16-bit inputs).  Scores, sums, denominators and
+// outputs are 32-bit.
 //
-// The scale of a block of values moves into the exponent: a tile weighs exp2(s + log2 vs - m'), with m' the running maximum of that sum,
-// beside exp2(s - m) for the denominator, so that neither overflows nor vanishes whatever the scales of the blocks are.  References are
-// raised only when a score exceeds them by 2^8.
+// The scale of a block of values moves into the exponent: a tile weighs exp2(s + log2 vs - m'), with m' following the maximum of that sum,
+// beside exp2(s - m) for the denominator, so that neither overflows nor vanishes whatever the scales of the blocks are.  These weights are
+// rounded to fp16, the type that holds the codes exactly: 2^-11 of each weight from 2^-26 (e^-18) of the largest one seen so far up, at most
+// 2^-37 of that largest below, where the rest of many tokens may still count beside one whose values are next to nothing (the denominator
+// has them whole).  That range is what m' is placed for (CA_RISE, CA_ROOM).
 #include <cuda_fp8.h>
 
 #include "common.cuh"
@@ -39,6 +41,11 @@ constexpr int CA_MAX_ROWS = 1024;        // requests of one launch: their tiles 
 constexpr int CA_LEAST_TILES = 8;        // of a block's run: shorter ones are not worth their partial sums
 constexpr int CA_START = 2;              // what the start of a sequence costs a warp, in tiles
 constexpr float CA_LOWEST = -3.0e38f;
+// References are raised when a score exceeds the one that they were raised for by CA_RISE octaves; that of the weights stands CA_ROOM below
+// it.  Weights stay below 2^(CA_ROOM + CA_RISE + 1) = 2^15, and fp16 has normal numbers down to 2^-14: 2^-(14 + CA_ROOM) = 2^-26 of a
+// weight at the reference.  References raised by 8, 4, 2, 1 octaves (room for 6, 10, 12, 13): ragged batch 90.1, 90.1, 90.0, 90.0 us; 16
+// columns 50.0, 50.5, 50.8, 51.0; 128 columns 139.6, 140.0, 140.1, 140.2.
+constexpr float CA_RISE = 2.f, CA_ROOM = 12.f;
 
 struct AttendArgs {
   const void* q;
@@ -424,7 +431,7 @@ __global__ void __launch_bounds__(32 * CA_WARPS, 1) attend_kernel(const AttendAr
             float& x = s[h][n][i];
             x *= cscale[n][i & 1] * ks[h];
             if (ragged && (!there[h] || t * CA_TILE + 16 * h + g8 + (i >> 1) * 8 >= seen[n][i & 1])) x = -INFINITY;
-            above |= x > m1[n][i & 1] + 8.f || x + ev[h] > m2[n][i & 1] + 8.f;
+            above |= x > m1[n][i & 1] + CA_RISE || x + ev[h] > m2[n][i & 1] + (CA_ROOM + CA_RISE);
           }
       }
       if (__any_sync(0xffffffffu, above)) {
@@ -439,7 +446,7 @@ __global__ void __launch_bounds__(32 * CA_WARPS, 1) attend_kernel(const AttendAr
               n1 = fmaxf(n1, __shfl_xor_sync(0xffffffffu, n1, o));
               n2 = fmaxf(n2, __shfl_xor_sync(0xffffffffu, n2, o));
             }
-            n1 = fmaxf(m1[n][i], n1); n2 = fmaxf(m2[n][i], n2);
+            n1 = fmaxf(m1[n][i], n1); n2 = fmaxf(m2[n][i], n2 - CA_ROOM);
             l[n][i] *= exp2_fast(m1[n][i] - n1);
             const float f = exp2_fast(m2[n][i] - n2);
             m1[n][i] = n1; m2[n][i] = n2;
@@ -879,8 +886,8 @@ __global__ void __launch_bounds__(32 * CW_WARPS, 1) attend_wide_kernel(const Att
           if (!INT8 && mine) mend(done, cnt - 2);
         }
         if (mine) {
-          if (__any_sync(0xffffffffu, g1 > m1 + 8.f || g2 > m2 + 8.f)) {
-            const float n1 = fmaxf(m1, g1), n2 = fmaxf(m2, g2), f = exp2_fast(m2 - n2);
+          if (__any_sync(0xffffffffu, g1 > m1 + CA_RISE || g2 > m2 + (CA_ROOM + CA_RISE))) {
+            const float n1 = fmaxf(m1, g1), n2 = fmaxf(m2, g2 - CA_ROOM), f = exp2_fast(m2 - n2);
             l *= exp2_fast(m1 - n1);
             m1 = n1; m2 = n2;
             if (done >= 0)
