@@ -31,7 +31,7 @@ constexpr int BEAM_LIST = 128;           // values of a run that reach the bound
 constexpr int BEAM_AT_ONCE = 32;         // runs per SM: 24 warps fit, beams that have ended leave room; 24, 48, 64: 22.9, 22.5, 21.8 us for 21.2
 constexpr int SELECT_THREADS = 256;
 constexpr float BEAM_LOWEST = -3.4028234663852886e38f;
-constexpr float BEAM_HUGE = 1e38f;       // a maximum whose product with L is finite
+constexpr float BEAM_ORDINARY = 4096.f;  // references whose product with L is rounded by at most 2^-12
 constexpr float LOG2E = 1.4426950408889634f;
 
 struct BeamArgs {
@@ -159,6 +159,13 @@ __device__ __forceinline__ unsigned long long add_pair(unsigned long long a, uns
   return d;
 }
 
+// What a sum of exponentials with the reference m has been divided by, as a power of two (L the rounded log2(e)).  An ordinary reference
+// is taken off as rn(m L), which one instruction does with x L; where the rounding of m L is no longer small (chunks of masked values,
+// logits of any size) exponents are (x - m) L.  The sums of both kinds go together through this number.
+__device__ __forceinline__ double reference_log2(float m) {
+  return fabsf(m) < BEAM_ORDINARY ? static_cast<double>(m * LOG2E) : static_cast<double>(m) * static_cast<double>(LOG2E);
+}
+
 // One chunk into shared memory, of which the row has V values from `from` on; VEC: every row starts on 16 bytes.  Whole words are
 // copied, the last ones of a row and rows off 16 bytes value by value; what is not there is -inf.
 template <typename T, bool VEC> __device__ __forceinline__ void copy_chunk(uint4* to, const T* from, int V) {
@@ -226,14 +233,14 @@ __global__ void __launch_bounds__(32 * BEAM_WARPS) beam_rows_kernel(const BeamAr
     bound = max(bound, kth);
     const float top = fmaxf(key_value(largest), BEAM_LOWEST);
     if (top > m + 8.f || chunk == first) {
-      sum *= fabsf(m) < BEAM_HUGE && fabsf(top) < BEAM_HUGE ? exp2f(m * LOG2E - top * LOG2E) : exp2f((m - top) * LOG2E);
+      sum *= exp2f(static_cast<float>(reference_log2(m) - reference_log2(top)));
       m = top;
     }
-    const bool ordinary = fabsf(m) < BEAM_HUGE;
+    const bool ordinary = fabsf(m) < BEAM_ORDINARY;
     const unsigned long long scale = pair_of(LOG2E, LOG2E), shift = pair_of(-m * LOG2E, -m * LOG2E);
     const uint32_t reach = X::word_of(bound ? key_value(bound) : -INFINITY);      // as numbers
     if (ordinary) {
-      // exp(x - m) as exp2(x L - m L), two at a time: the rounding of m L is put right where the sums are used
+      // exp(x - m) as exp2(x L - rn(m L)), two at a time
       unsigned long long sums[2] = {0ull, 0ull};
 #pragma unroll 4
       for (int i = 0; i < BEAM_LOADS; ++i) {
@@ -317,10 +324,9 @@ __device__ __forceinline__ double key_value(unsigned long long k) {
   return __longlong_as_double(static_cast<long long>(k >> 63 ? k & 0x7fffffffffffffffull : ~k));
 }
 
-// A run's sum for the reference `top` of its row: the sum that was made is off by 2^(m L - rn(m L)), L the rounded log2(e).
+// A run's sum for the reference `top` of its row.
 __device__ __forceinline__ double run_sum(float2 s, float top) {
-  const double off = fabsf(s.x) < BEAM_HUGE ? static_cast<double>(s.x) * static_cast<double>(LOG2E) - static_cast<double>(s.x * LOG2E) : 0.;
-  return static_cast<double>(s.y) * (1. - off * 0.6931471805599453) * static_cast<double>(exp2f((s.x - top) * LOG2E));
+  return static_cast<double>(s.y) * exp2(reference_log2(s.x) - static_cast<double>(top) * static_cast<double>(LOG2E));
 }
 
 // One block per prompt.  A warp per beam: the beam's sum, its parts' lists; then the beams' lists, K rounds, a lane per beam.
