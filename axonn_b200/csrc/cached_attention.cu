@@ -20,7 +20,7 @@
 // side of the instruction; O^T = V^T P^T (rows = values of the head).  Which value of a head is which row or k index is free as long as
 // both operands agree, and is chosen such that every thread reads 16 consecutive bytes: of K 16 values of its token, of V 16 values of
 // each of its four tokens, whose bytes are then interleaved pairwise.  Codes become fp16, which holds them exactly; queries are scaled
-// by a power of two into fp16 (exact but for values below 2^-21 of a row's largest at 16-bit inputs).  Scores, sums, denominators and
+// by a power of two into fp16 (exact but for values below 2^-28 of a row's largest at 16-bit inputs).  Scores, sums, denominators and
 // outputs are 32-bit.
 //
 // The scale of a block of values moves into the exponent: a tile weighs exp2(s + log2 vs - m'), with m' following the maximum of that sum,
@@ -142,6 +142,14 @@ __device__ __forceinline__ uint64_t evict_first() {
 }
 __device__ __forceinline__ void copy4(uint32_t to, const void* from) {
   asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(to), "l"(from) : "memory");
+}
+__device__ __forceinline__ float power_of_two(int e) { return __uint_as_float(static_cast<uint32_t>(127 + e) << 23); }
+// Queries times 2^-e are below 2^15 as fp16: as far up as sums of 128 products with codes allow in 32 bits, so that their smallest values
+// keep what they can.  Zero and what is not finite stay as they are; of queries below 2^-103 the range is not used up, so that the powers
+// of two, and their products with the softmax scale, stay normal numbers.
+__device__ __forceinline__ int query_exponent(float largest) {
+  const int e = static_cast<int>(__float_as_uint(largest) >> 23) - 127;
+  return e > 127 || e < -126 ? 0 : max(e, -103) - 14;
 }
 template <int WORDS> __device__ __forceinline__ void shared_words(const uint8_t* p, uint32_t* w) {
   if constexpr (WORDS == 4) {
@@ -342,11 +350,8 @@ __global__ void __launch_bounds__(32 * CA_WARPS, 1) attend_kernel(const AttendAr
       }
       largest = fmaxf(largest, __shfl_xor_sync(0xffffffffu, largest, 1));
       largest = fmaxf(largest, __shfl_xor_sync(0xffffffffu, largest, 2));
-      // 2^(7 - e) for a largest of 2^e .. 2^(e + 1); zero and what is not finite stay as they are
-      int e = static_cast<int>(__float_as_uint(largest) >> 23) - 127;
-      e = e > 127 || e < -126 ? 7 : max(e, -110);
-      const float up = __uint_as_float(static_cast<uint32_t>(127 + 7 - e) << 23);
-      const float down = __uint_as_float(static_cast<uint32_t>(127 + e - 7) << 23) * a.scale_log2;
+      const int e = query_exponent(largest);
+      const float up = power_of_two(-e), down = power_of_two(e) * a.scale_log2;
 #pragma unroll
       for (int s = 0; s < D / 16; ++s) {
         const float* x = &f[s / 4][(s % 4) * 4];
@@ -787,10 +792,9 @@ __global__ void __launch_bounds__(32 * CW_WARPS, 1) attend_wide_kernel(const Att
 #pragma unroll
             for (int j = 0; j < 4; ++j) { const float2 f = value(w[j]); largest = fmaxf(largest, fmaxf(fabsf(f.x), fabsf(f.y))); }
           }
-        int e = static_cast<int>(__float_as_uint(largest) >> 23) - 127;      // as above: 2^(7 - e), scaled exactly
-        e = e > 127 || e < -126 ? 7 : max(e, -110);
-        const float up = copysignf(__uint_as_float(static_cast<uint32_t>(127 + 7 - e) << 23), a.scale_log2);      // so that the largest score is that of
-        cscale = __uint_as_float(static_cast<uint32_t>(127 + e - 7) << 23) * fabsf(a.scale_log2);               // the largest product
+        const int e = query_exponent(largest);
+        const float up = copysignf(power_of_two(-e), a.scale_log2);      // so that the largest score is that of the largest product
+        cscale = power_of_two(e) * fabsf(a.scale_log2);
 #pragma unroll 4
         for (int i = half * (D / 16); i < half * (D / 16) + D / 16; ++i) {
           uint4 u = make_uint4(0u, 0u, 0u, 0u);
