@@ -251,8 +251,18 @@ __global__ void __launch_bounds__(256, ROPE ? 2 : 4) store_kernel(const StoreArg
   const int BT = 1 << a.shift;
   const long long* slots = a.slots + static_cast<size_t>(r) * a.S;
   const long long slot0 = slots[0];
-  if (slot0 < 0) return;
-  const int within = static_cast<int>(slot0 & (BT - 1));
+  int within = static_cast<int>(slot0 & (BT - 1));
+  if (slot0 < 0) {                         // none of the row's, or none in the block that its table lacks: later ones start a block
+    unsigned some = 0u;
+    int at = 1;
+    for (; at < BT && at < a.S; at += 32) {
+      some = __ballot_sync(0xffffffffu, at + (tid & 31) < a.S && slots[at + (tid & 31)] >= 0);
+      if (some) break;
+    }
+    if (!some || run == 0) return;
+    within = BT - (at + __ffs(some) - 1);
+    if (within <= 0) return;
+  }
   const int i0 = run == 0 ? 0 : run * BT - within, held = run == 0 ? within : 0;
   if (i0 >= a.S) return;
   const int n = min(BT - held, a.S - i0);

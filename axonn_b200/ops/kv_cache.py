@@ -87,7 +87,8 @@ def plan_blocks(lengths, new, tables, free, taken, tokens, block_tokens):
     The blocks that are missing are the next ones of the list ``free``, of which ``taken[0]`` have been used, in the order of
     the requests; their ids are written into ``tables`` (in place: entries behind what a request holds).  A request whose row of
     the table is full, or that comes when the list is used up, gets places for as many tokens as there is room for: its
-    ``lengths`` entry of the plan tells.  ``lengths`` and ``taken`` themselves are left as they are (numbers below 0 and beyond the
+    ``lengths`` entry of the plan tells.  Tokens of an unfinished block that the table lacks (-1 within the length) are counted, but have no
+    slot.  ``lengths`` and ``taken`` themselves are left as they are (numbers below 0 and beyond the
     list count as 0 and its end)."""
     if lengths.is_cuda and (host := host_paths()) is not None:
         out = host.plan_blocks(lengths, new, tables, free, taken, tokens, block_tokens)
@@ -156,7 +157,7 @@ def _qkv_strides(qkv):
 def store_blocks(qkv, layer, slots, positions=None, rope_table=None) -> Optional[torch.Tensor]:
     """Store the keys and values of the packed projection output ``qkv [R, S, kv_heads, q_per_kv + 2, D]`` (per KV head: its query
     heads, then its key, then its value) at ``slots [R, S]`` of ``layer``, as ``plan_blocks`` gives them: the tokens of a row follow one
-    another, those without a slot stand behind them, and no block takes tokens of two rows.
+    another, those without a slot stand behind them (or in front, where the table lacks their block), and no block takes tokens of two rows.
 
     The scale of a block and head is the smallest power of two by which the largest finite value of its new tokens does not exceed the
     largest code (448 in e4m3, 127 in int8); a block that holds tokens already keeps the larger of its scale and that one, and where
