@@ -226,7 +226,8 @@ __global__ void __launch_bounds__(256, ROPE ? 2 : 4) store_kernel(const StoreArg
     const int h = static_cast<int>(row - token * H);
     float f[16];
     const int at = a.positions[token];
-    if (a.slots[token] >= 0 && at >= 0 && at < a.angles) {
+    const long long slot = a.slots[token];
+    if (slot >= 0 && (slot >> a.shift) < a.N && at >= 0 && at < a.angles) {
       const unsigned r = token / a.S, g = h / a.P;
       const T* p = qkv + r * a.row_stride + (token - r * a.S) * a.token_stride + g * a.group_stride + (h - g * a.P) * D + c;
       load8(p, f);

@@ -43,3 +43,14 @@ def test_a_table_that_lacks_the_unfinished_block(BT, S, rope, codes, dtype, D):
     out = ops.cached_attention(q, layer, here, plan.lengths, torch.tensor(n, dtype=torch.int32, device=DEV)).cpu()
     o64, size = attend64(q.cpu(), want, want_tables, after, n)
     assert bool(((out.double() - o64).abs() <= attend_bound(o64, size, dtype) + 2.0 ** -24).all()) and bool(out.isfinite().all())
+
+
+@pytest.mark.parametrize("S", [1, 20, 70])
+def test_blocks_outside_the_cache(S):
+    """Ids that the cache does not have: their tokens are neither stored nor rotated."""
+    tables = torch.full((3, 8), -1, dtype=torch.int32)
+    args = ([0, 0, 0], [S, S, S], tables, [5, 900, 2, 64, 3, 1 << 30, 7, 8, 9, 10, 11, 12, 13, 14, 15], S, 2, 1, 64, 16, E4M3, torch.bfloat16, True, 64)
+    here, plan, _, layer, q = _plan_and_store(DEV, *args)
+    want_tables, want_plan, _, want, want_q = _plan_and_store("cpu", *args)
+    assert torch.equal(here.cpu(), want_tables) and all(torch.equal(a.cpu(), b) for a, b in zip(plan, want_plan))
+    assert all(same_bits(a.cpu(), b) for a, b in zip(layer, want)) and torch.equal(q.cpu(), want_q)
