@@ -247,7 +247,7 @@ def _store_torch(qkv, layer, slots, positions, table):
     slot, x = slot[there], qkv.detach().reshape(R * S, G, n, D)[there].float()
     q = None
     if table is not None:
-        turned = _rotate_torch(x[:, :, :-1].reshape(len(x), -1, D), table, at[there]).view(len(x), G, n - 1, D)
+        turned = _rotate_torch(x[:, :, :-1].reshape(len(x), G * (n - 1), D), table, at[there]).view(len(x), G, n - 1, D)
         q = torch.zeros(R * S, G, n - 2, D, dtype=qkv.dtype, device=qkv.device)
         q[there] = turned[:, :, :-1].to(qkv.dtype)
         q = q.view(R, S, G * (n - 2), D)
