@@ -4,15 +4,24 @@
 // Bound by reading the logits once.  A first launch cuts every beam's row into runs of chunks of 4 KB.  A warp copies the chunks of its run
 // into shared memory, one ahead, and goes over each twice: no block ever waits for its warps, and the loops are short (the same code for
 // values in registers is five times as long, and was waited for longer than the data).  The K-th largest of the lanes' maxima is reached
-// by at least K values of the chunk and by few others; what reaches the largest such bound so far goes into a list, of which the K best
-// are kept in the end.  (Where too many values reach the bounds - rows of equal values - the K best are found one by one.)  The order
-// within a beam is that of its logits, so that nothing has to be known of the sum.  A second launch puts the runs of a beam together and
-// merges the beams.  Sums and values there are 64-bit: the order of two beams' tokens depends on differences of their sums' logarithms
-// that 32-bit values of twenty or so round away.
+// by at least K values of the chunk and, with few beams, by few others; what reaches the largest such bound so far goes into a list, of
+// which the K best are kept in the end.  The order within a beam is that of its logits, so that nothing has to be known of the sum.  A
+// second launch puts the runs of a beam together and merges the beams.
+//
+// Where the list overflows, the K best are found one by one, and the run's chunks are read again for each: rows of mostly equal (masked)
+// values, and ordinary ones with many beams or many chunks in a run, as a bound is that of one chunk's 32 lanes and nothing is taken out
+// of the list.  Normal logits fill it with 32 values of four chunks for 8 beams, 89 for 16, 132 for 20, with 149 of 28 chunks for 8, and of
+// a single chunk for 28 beams and more.  The second launch is a block per prompt, whose warps merge a beam's lists in K rounds for every
+// 128 entries.  Both suit the beams of most searches, not 32: one prompt over 128,256 values takes 10.6, 34 and 370 us with 8, 16 and
+// 32 beams, 64 prompts over 32,000 values with 16 beams 153, 256 with 8 beams 42.
+//
+// A run's sum is 32-bit: terms of exp2, which a lane adds one after another, within 2^-18 of the sum.  Runs are joined and values formed in
+// 64 bits, as the order of two beams' tokens depends on differences of their sums' logarithms that 32-bit values of twenty or so round
+// away; candidates of two beams that are closer than their sums are exact may still change places.
 //
 // 32 prompts, 8 beams (a fifth have ended), 128,256 bf16 values: 21.2 us, 3.1 TB/s of what is read.  Then the schedulers issue in half of
-// the cycles and the unit of exp2 is busy for 0.4 of them: five warps per scheduler do not hide the dependent steps of a chunk.  One
-// prompt, 4 beams, 32,000 values: 5.7 us for two launches.  Tried beside it, same case: chunks of 2 KB 24.6 us, neighbouring warps on
+// the cycles and the unit of exp2 is busy for 0.45 of them: five warps per scheduler do not hide the dependent steps of a chunk.  One
+// prompt, 4 beams, 32,000 values: 5.8 us for two launches.  Tried beside it, same case: chunks of 2 KB 24.6 us, neighbouring warps on
 // different rows 23.3, blocks of one or two such warps 22.0, 22.6.
 //
 // A value that is not a number counts as -inf, and so do a score of +inf and every value of a beam whose sum is none.  Of a beam that has
@@ -28,7 +37,7 @@ constexpr int BEAM_WARPS = 4;            // of a block of the first launch
 constexpr int BEAM_LOADS = 8;            // 16-byte words of a lane, of a chunk
 constexpr int BEAM_CHUNK = 32 * BEAM_LOADS * 16;     // bytes
 constexpr int BEAM_LIST = 128;           // values of a run that reach the bounds, at most
-constexpr int BEAM_AT_ONCE = 32;         // runs per SM: 24 warps fit, beams that have ended leave room; 24, 48, 64: 22.9, 22.5, 21.8 us for 21.2
+constexpr int BEAM_AT_ONCE = 32;         // runs per SM: 24 warps fit, beams that have ended leave room; 24, 48, 64: 22.9, 22.5, 21.8 us for 21.2 (the 8 beams above)
 constexpr int SELECT_THREADS = 256;
 constexpr float BEAM_LOWEST = -3.4028234663852886e38f;
 constexpr float BEAM_ORDINARY = 4096.f;  // references whose product with L is rounded by at most 2^-12

@@ -10,8 +10,9 @@
 // the order of the tokens: the same call gives the same bits.
 //
 // Measured on one B200, D 128, device time: 64 requests of 17 to 8,192 tokens, 8 KV heads of 4 query heads: 90.0 us, 6.0 TB/s; 3 of 60,001
-// to 131,072: 96.9 us, 6.06 TB/s; 24 of 700 to 2,048, 16 KV heads, 8 new tokens, int8: 33.2 us, 4.1 TB/s, of which the ends of the runs
-// and the second launch are about 10; one request of 900 tokens 10.0 us, two launches' latency.  The loop alone issues in half of the
+// to 131,072: 96.6 us, 6.08 TB/s; 24 of 700 to 2,048, 16 KV heads, 8 new tokens, int8: 33.3 us, 4.1 TB/s, of which the ends of the runs
+// and the second launch are about 10; one request of 900 tokens 10.0 us, two launches' latency (blocks of a
+// cluster that join few sequences in their shared memory, in one launch, have not been tried).  The loop alone issues in half of the
 // cycles.  Tried for the long case when it took 100 us: 6, 7, 9, 12 warps per SM 113, 102, 126, 122; three tiles of a warp's ring instead
 // of two 109; more than 128 KB of an SM's copies on their way at once makes all of them slower.  Starts that count as 0, 2, 4 tiles:
 // ragged batch 102, 91, 91 us.
@@ -633,8 +634,9 @@ __global__ void __launch_bounds__(32 * CA_WARPS, 1) attend_kernel(const AttendAr
 // The same sums on tcgen05, for groups of up to 128 columns (rows of the products: S = Q K^T, O = P V with M = 128): the codes of a tile of
 // 128 tokens are widened once for all of them.  24 requests of 4,096 tokens, 8 KV heads, 128 columns: 140 us (int8 136), 52 GFLOP of
 // products; about 4,000 cycles a tile, of which the exp2 unit needs 1,000.  A warp's steps wait for one another (a load of 32 scores 300
-// cycles, their maximum 350, their weights 500), and two warps per scheduler do not hide that; registers allow no more.  With both threads
-// of a column on one tile, which have to meet in each, 17 us more.  One block per SM, with roles:
+// cycles, their maximum 350, their weights 500; scores are loaded twice, once for each), and two warps per scheduler do not hide that.  All
+// 17 warps have 96 registers; sharing those out by role has not been tried.  With both threads of a column on one tile, which have to
+// meet in each, 17 us more.  One block per SM, with roles:
 //
 //   warps 0-7   softmax, two threads per column (lane of tensor memory), for every other tile each, with sums of their own: the queries
 //               into shared memory, then per tile the largest score and the weights as fp16 in the place of the scores; at the end of a
@@ -1194,7 +1196,7 @@ __global__ void __launch_bounds__(32 * MERGE_WARPS) attend_merge_kernel(const At
 }
 
 // Columns of a group.  24 requests of 4,096 tokens, 8 KV heads of 128 values, us with groups of 8, 16, 128 columns: 8 queries 40, 48, -;
-// 9 to 16 64, 50, -; 24 90, 84, 124; 48 -, 121, 127; 56 -, 155, 128; 64 240, 156, 129; 128 -, 295, 140; 512 -, 1178, 476.  1,000 tokens, 64
+// 9 to 16 64, 51, -; 24 90, 84, 124; 48 -, 122, 127; 56 -, 155, 128; 64 240, 156, 129; 128 -, 295, 140; 512 -, 1178, 481.  1,000 tokens, 64
 // values, int8: 48 queries -, 36, 39.5; 56 -, 43, 40.
 static int attend_columns(int queries) { return queries <= 8 ? 8 : queries <= 48 ? 16 : CW_COLUMNS; }
 static long long before_words(int rows) { return (rows + 1 + 3) / 4 * 4; }

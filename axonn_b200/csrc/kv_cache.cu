@@ -210,7 +210,9 @@ template <bool INT8> __device__ __forceinline__ float code_value(uint32_t byte) 
 // 16 prompts of up to 2,048 tokens, 16 KV heads of 128 values, bf16 to int8 (309 MB): 59.1 us, 5.2 TB/s, 0.8 of a copy's rate; it issues in
 // two thirds of the cycles with half of the warps that fit an SM, four blocks of 256 by their 64 registers.  Two units per thread 69.6 us
 // (more of it is bookkeeping), three blocks 65.0, five or 56 registers 77, 63 (spills); slots by one lane per token 60.4.  A token each for
-// 128 requests, 8 KV heads of 4 query heads, rotated: 3.9 us, latency.
+// 128 requests, 8 KV heads of 4 query heads, rotated: 3.9 us, latency.  16 prompts of up to 2,048 tokens of those, rotated, e4m3 (629 MB):
+// 232 us, 2.7 TB/s, 0.41 of a copy's rate: values are held as 32-bit numbers, 114 registers leave two blocks of 256 per SM (0.22 of the
+// warps), and it issues in 0.31 of the cycles, waiting for its loads.
 template <typename T, int D, bool INT8, bool ROPE>
 __global__ void __launch_bounds__(256, ROPE ? 2 : 4) store_kernel(const StoreArgs a) {
   constexpr int UNITS = D / 16;            // units of a token: eight pairs (i, i + D / 2) each
@@ -388,7 +390,7 @@ struct ReorderArgs {
 // Bound by reading and writing the unfinished blocks of the rows that change, of all layers.  Sources are blocks that rows write into,
 // targets are spare ones, so that nothing is read after it was written and the order of the copies does not matter.  Unfinished blocks
 // hold 1 to block_tokens - 1 tokens: small blocks of the grid, many to an SM, even that out.  64 rows, 32 layers, 8 heads of 128 values,
-// blocks of 64 tokens (201 MB): 32.8 us, 6.1 TB/s (35.5 with a division for every 16 bytes, and then 46.2, 37.6, 37.0 at 8, 16 or 64
+// blocks of 64 tokens (201 MB): 32.6 us, 6.2 TB/s (35.5 with a division for every 16 bytes, and then 46.2, 37.6, 37.0 at 8, 16 or 64
 // blocks per SM, 39.1 and 38.1 with 256 threads and 8 or 32 blocks, 36.7 with eight loads ahead instead of four).  4 rows, 24 layers, 16
 // heads: 3.6 us, a launch's latency.
 __global__ void __launch_bounds__(REORDER_THREADS) reorder_kernel(const ReorderArgs a) {

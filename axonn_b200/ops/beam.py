@@ -29,7 +29,9 @@ def beam_select(logits, scores, done=None, eos_id=None):
     A continuation's value is the beam's score plus the log-probability of the token; equal values count in the order of (beam, token),
     and a beam's tokens in the order of their logits.  Of a beam that is ``done`` (bool) only ``eos_id`` goes on, at the beam's score;
     the two are given together.  A value that is not a number counts as ``-inf``, and so do a score of ``+inf`` and all of a beam
-    whose logits sum up to none (a NaN or ``+inf`` among them, or all ``-inf``).  Up to 32 beams."""
+    whose logits sum up to none (a NaN or ``+inf`` among them, or all ``-inf``).  Up to 32 beams.
+
+    On a GPU a beam's sum is exact to 2^-18: candidates of two beams whose values are closer may change places."""
     if logits.is_cuda and (host := host_paths()) is not None:
         out = host.beam_select(logits, scores, done, eos_id)
         if out is not None:

@@ -278,7 +278,8 @@ def cached_attention(q, layer, tables, lengths, new=None, scale=None):
     ``[R, S, heads, D]`` in the type of ``q``.
 
     Blocks that a table lacks (-1 within the length) count as absent.  What lies behind a sequence in its last block is never
-    looked at.  On a GPU: bf16 or fp16, D 64 or 128; the work is bound by reading the cache, once for up to 16 query columns
+    looked at.  On a GPU: bf16 or fp16, D 64 or 128; scores, sums and denominators are 32-bit, and softmax weights are rounded to fp16 (half
+    a step, 2^-11, of each down to e^-18 of a query's largest one, smaller ones by less than 2^-37 of that); the work is bound by reading the cache, once for up to 16 query columns
     (``S * q_per_kv``); more than 48 share the reading in groups of 128 on the tensor cores' own memory.  A prompt that starts a
     sequence is better evaluated with ``flash_attention`` before it is stored."""
     if q.is_cuda and (host := host_paths()) is not None:
