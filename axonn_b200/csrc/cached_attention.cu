@@ -145,9 +145,9 @@ __device__ __forceinline__ void copy4(uint32_t to, const void* from) {
   asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(to), "l"(from) : "memory");
 }
 __device__ __forceinline__ float power_of_two(int e) { return __uint_as_float(static_cast<uint32_t>(127 + e) << 23); }
-// Queries times 2^-e are below 2^15 as fp16: as far up as sums of 128 products with codes allow in 32 bits, so that their smallest values
-// keep what they can.  Zero and what is not finite stay as they are; of queries below 2^-103 the range is not used up, so that the powers
-// of two, and their products with the softmax scale, stay normal numbers.
+// Queries times 2^-e lie below 2^15, an octave under fp16's largest number, so that small values of a row keep what they can; sums of 128
+// products with codes stay far inside 32 bits.  Zero and what is not finite stay as they are; for queries below 2^-103 the range is not
+// used up, so that the powers of two, and their products with the softmax scale, stay normal numbers.
 __device__ __forceinline__ int query_exponent(float largest) {
   const int e = static_cast<int>(__float_as_uint(largest) >> 23) - 127;
   return e > 127 || e < -126 ? 0 : max(e, -103) - 14;
