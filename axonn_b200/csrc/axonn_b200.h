@@ -340,6 +340,30 @@ long long axb_beam_select_words(int B, int K, int V, int dtype);
 int axb_beam_select(const void* logits, const float* scores, const void* done, int eos, float* out_scores, long long* out_tokens,
                     int* out_parents, void* out_done, void* work, int B, int K, int V, int dtype, void* stream);
 
+/* ---- log-probabilities of given tokens (token_probs.cu): rows of V logits at batch * batch_stride + row * row_stride (strides in values),
+ * a slice of a vocabulary of `total` that begins at `start`; tokens [batches, per_batch] int64 (strides in words) or NULL, rows of the token
+ * `ignored` are left out; scale: 1 / temperature.  stats [rows, 4] fp32, 16-byte aligned, is written in any case.  whole: the slice is all of
+ * the vocabulary, and log_probs and entropy [rows] (or NULL) and the top log-probabilities [rows, top] are finished and stats (m, s, H, z_t);
+ * otherwise stats are (m, s, w, z_t) of the slice and the top logits are as they are.
+ * bwd: stats (m, s, H) of the whole vocabulary, gradients of log_probs, entropy and the top ones (or NULL), out [rows, V] dense. */
+int axb_token_log_probs(const void* logits, long long batch_stride, long long row_stride, const long long* tokens,
+                        long long token_batch_stride, long long token_stride, float* log_probs, float* entropy, float* top_log_probs,
+                        long long* top_tokens, float* stats, int batches, int per_batch, int V, long long start, long long total, int top,
+                        float scale, long long ignored, int whole, int dtype, void* stream);
+int axb_token_log_probs_bwd(const void* logits, long long batch_stride, long long row_stride, const long long* tokens,
+                            long long token_batch_stride, long long token_stride, const float* stats, const float* d_log_probs,
+                            const float* d_entropy, const float* d_top, const long long* top_tokens, void* out, int batches, int per_batch,
+                            int V, long long start, long long total, int top, float scale, long long ignored, int dtype, void* stream);
+
+/* ---- table lookup (embedding.cu): out [n, H] = scale * rows of table [V, H] (pitch in values) by tokens [n] of 4 or 8 bytes; the gradient
+ * dtable [V, H] of rows dy [n, H] (pitch in values), none for the token `padding` (-1: no such).  work: axb_embedding_grad_words()
+ * 32-bit words, 16-byte aligned, of this call alone */
+int axb_embedding(const void* tokens, int token_bytes, long long n, const void* table, long long pitch, int V, int H, float scale, void* out,
+                  int dtype, void* stream);
+long long axb_embedding_grad_words(long long n, int V, int H);
+int axb_embedding_grad(const void* tokens, int token_bytes, long long n, const void* dy, long long pitch, int V, int H, float scale,
+                       long long padding, void* dtable, void* work, int dtype, void* stream);
+
 /* ---- top-k gradient pruning (prune.cu): keep the k largest |g|, zero the rest, in place.
  * dtype: the codes above (0 bf16, 1 fp16, 2 fp32).  `work`: device scratch of axb_prune_workspace_words() 32-bit words, 8-byte aligned. */
 int axb_prune_workspace_words(void);

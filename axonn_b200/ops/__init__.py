@@ -8,6 +8,7 @@ PyTorch composition used on CPU (and as the numerical oracle in the tests).
 from .activation import gelu_backward_colsum, gelu, gelu_backward, swiglu  # noqa: F401
 from .attention import flash_attention, flash_attention_packed  # noqa: F401
 from .beam import MOST_BEAMS, BeamStep, beam_select  # noqa: F401
+from .embedding import embedding  # noqa: F401
 from .gemm import (  # noqa: F401
     gemm_on_pairs,
     EPI_BIAS,
@@ -38,3 +39,4 @@ from .multi_tensor import (  # noqa: F401
 from .norm import add_layer_norm, add_rms_norm, column_sum, layer_norm, rms_norm  # noqa: F401
 from .optim_step import AdamTable, adamw_reference_, multi_tensor_adamw, prune_topk_  # noqa: F401
 from .rope import apply_rope, rope_table  # noqa: F401
+from .token_probs import MOST_ALTERNATIVES, TokenLogProbs, token_log_probs  # noqa: F401

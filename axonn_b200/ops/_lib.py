@@ -89,6 +89,11 @@ _SIGNATURES = {
     "axb_cached_attention": "p" "lll" "pppp" "ppp" "pp" "iiiiiiii" "f" "ii" "p",
     "axb_beam_select_words": "iiii",
     "axb_beam_select": "ppp" "i" "ppppp" "iiii" "p",
+    "axb_token_log_probs": "p" "ll" "p" "ll" "ppppp" "iii" "ll" "i" "f" "l" "ii" "p",
+    "axb_token_log_probs_bwd": "p" "ll" "p" "ll" "pppppp" "iii" "ll" "i" "f" "l" "i" "p",
+    "axb_embedding": "p" "i" "l" "p" "l" "ii" "f" "p" "i" "p",
+    "axb_embedding_grad_words": "l" "ii",
+    "axb_embedding_grad": "p" "i" "l" "p" "l" "ii" "f" "l" "pp" "i" "p",
 }
 # Switches of kernels that are gone.  The one kernel that is left covers what they selected; a program that still sets
 # one is told so instead of being ignored.
@@ -120,7 +125,7 @@ def lib():
             for name, sig in _SIGNATURES.items():
                 if hasattr(L, name):
                     getattr(L, name).argtypes = [_CTYPES[c] for c in sig]
-            for name in ("axb_flash_attn_bwd_scratch", "axb_cached_attention_words", "axb_beam_select_words"):
+            for name in ("axb_flash_attn_bwd_scratch", "axb_cached_attention_words", "axb_beam_select_words", "axb_embedding_grad_words"):
                 if hasattr(L, name):
                     getattr(L, name).restype = ctypes.c_longlong
             ms = os.environ.get("AXONN_COMM_TIMEOUT_MS")

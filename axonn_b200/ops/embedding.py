@@ -1,0 +1,108 @@
+"""Rows of a table by token, scaled, with the gradient by sorted tokens (``csrc/embedding.cu``)."""
+
+import math
+
+import torch
+import torch.nn.functional as F
+
+from . import _lib
+from .direct import no_graph, plain_tensors
+from .kv_cache import _elsewhere
+
+_DT = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
+_INDEX = {torch.int32: 4, torch.int64: 8}
+
+
+def embedding(tokens, weight, scale=1.0, padding_idx=None):
+    """``weight[tokens] * scale``: ``tokens [...]`` (int32 or int64), ``weight [V, H]`` (bf16, fp16 or fp32), returns ``[..., H]`` in the type
+    of ``weight``, each value rounded once.
+
+    The gradient of ``weight`` has the sums of the rows of equal tokens, 32-bit in the order of the tokens (the same bits on every run),
+    scaled and rounded once; ``padding_idx`` gets none.  Gradients of gradients are lookups again.  A token outside the table
+    gives a row of NaN and no gradient on a GPU, and is an error on the CPU.  The call never synchronises and can be captured into a CUDA graph."""
+    if weight.ndim != 2 or weight.dtype not in _DT:
+        raise ValueError(f"weight must be [V, H] in bf16, fp16 or fp32, not {weight.dtype} {list(weight.shape)}")
+    if tokens.dtype not in _INDEX:
+        raise ValueError(f"tokens must be int32 or int64, not {tokens.dtype}")
+    if tokens.device != weight.device:
+        raise ValueError(f"tensors on {weight.device} and {tokens.device}")
+    if not math.isfinite(scale):
+        raise ValueError(f"the scale is a finite number, not {scale}")
+    V = weight.shape[0]
+    if padding_idx is not None:
+        if not -V <= padding_idx < V:
+            raise ValueError(f"padding_idx {padding_idx} is outside the table of {V} rows")
+        padding_idx %= V
+    if not plain_tensors(tokens, weight) or weight.numel() == 0 or V > 1 << 30 or weight.shape[1] > 1 << 25 or tokens.numel() >= 1 << 31:
+        return _torch(tokens, weight, scale, padding_idx)
+    if _elsewhere(weight.device):
+        with torch.cuda.device(weight.device):
+            return embedding(tokens, weight, scale, padding_idx)
+    if no_graph(weight):
+        return _rows(tokens, weight, scale)
+    return _EmbeddingFn.apply(tokens, weight, scale, -1 if padding_idx is None else padding_idx)
+
+
+def _torch(tokens, weight, scale, padding_idx):
+    out = F.embedding(tokens, weight, padding_idx)
+    return out if scale == 1.0 else (out.float() * scale).to(weight.dtype)
+
+
+def _rows(tokens, weight, scale):
+    weight = weight.detach()
+    if weight.shape[1] > 1 and weight.stride(1) != 1:
+        weight = weight.contiguous()
+    tokens = tokens.contiguous()
+    out = torch.empty(*tokens.shape, weight.shape[1], dtype=weight.dtype, device=weight.device)
+    if out.numel():
+        st = _lib.lib().axb_embedding(tokens.data_ptr(), _INDEX[tokens.dtype], tokens.numel(), weight.data_ptr(), weight.stride(0), *weight.shape, scale,
+                                      out.data_ptr(), _DT[weight.dtype], _lib.stream())
+        _lib.check(st, "axb_embedding")
+    return out
+
+
+def _table_gradient(tokens, dy, V, scale, padding):
+    """``dy [..., H]`` summed by token; the rows may have any stride."""
+    H = dy.shape[-1]
+    dy = dy.reshape(-1, H)
+    if H > 1 and dy.stride(1) != 1:
+        dy = dy.contiguous()
+    tokens = tokens.reshape(-1).contiguous()
+    n, L = tokens.numel(), _lib.lib()
+    out = torch.empty(V, H, dtype=dy.dtype, device=dy.device)
+    work = torch.empty(L.axb_embedding_grad_words(n, V, H), dtype=torch.int32, device=dy.device)
+    st = L.axb_embedding_grad(tokens.data_ptr(), _INDEX[tokens.dtype], n, dy.data_ptr(), dy.stride(0), V, H, scale, padding, out.data_ptr(),
+                              work.data_ptr(), _DT[dy.dtype], _lib.stream())
+    _lib.check(st, "axb_embedding_grad")
+    return out
+
+
+class _EmbeddingFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, tokens, weight, scale, padding):
+        ctx.save_for_backward(tokens)
+        ctx.scale, ctx.padding, ctx.V = scale, padding, weight.shape[0]
+        return _rows(tokens, weight, scale)
+
+    @staticmethod
+    def backward(ctx, dy):
+        (tokens,) = ctx.saved_tensors
+        return None, _EmbeddingGradFn.apply(tokens, dy, ctx.V, ctx.scale, ctx.padding), None, None
+
+
+class _EmbeddingGradFn(torch.autograd.Function):
+    """The gradient of the table as a function of that of the rows, and its own: rows of the table that it is asked with."""
+
+    @staticmethod
+    def forward(ctx, tokens, dy, V, scale, padding):
+        ctx.save_for_backward(tokens)
+        ctx.scale, ctx.padding = scale, padding
+        return _table_gradient(tokens, dy, V, scale, padding)
+
+    @staticmethod
+    def backward(ctx, d_table):
+        (tokens,) = ctx.saved_tensors
+        V = d_table.shape[0]
+        none = (tokens < 0) | (tokens >= V) | (tokens == ctx.padding)
+        rows = embedding(tokens.masked_fill(none, 0), d_table, ctx.scale)
+        return None, rows.masked_fill(none[..., None], 0), None, None, None
