@@ -1,82 +1,440 @@
 // Rows of a table by token, scaled, and the gradient of the table: the sums of the rows of equal tokens.
 //
 //   out_i = scale table[t_i];   dtable_v = scale sum_{i: t_i = v} dy_i   (nothing of the padding token)
-// A token outside the table gives a row of NaN and has no gradient.  Sums are 32-bit, in the order of the tokens, and rounded once.
+// A token outside the table gives a row of NaN and has no gradient.  Sums are 32-bit, in an order that the tokens alone decide, and
+// rounded once.
 //
-// A block per looked-up row; a block per 1024 columns of a row of the gradient, which goes over all tokens.
+// Both are bound by the rows' bytes.  The gradient sorts (token, place) pairs and sums along the sorted list, so that every row of the
+// gradient is written once, by one block, and no addition depends on when a block runs:
+//   1. One cluster sorts by a stable radix sort; its CTAs exchange the digits' counts through distributed shared memory.  It also notes
+//      which tokens there are.
+//   2. Blocks sum chunks of 32 pairs, columns split over blocks; other blocks of the same launch zero the rows of the tokens that
+//      there are not.  A chunk is summed with what the last token of it has in the next one, unless that token fills the whole next
+//      chunk: then its sum so far goes to the workspace.  A segment of any length so takes many blocks, and one of up to 32 pairs
+//      no extra traffic.
+//   3. The partial sums of long segments are joined in their order.
 #include "common.cuh"
 
 namespace axb {
 
-constexpr int EMB_THREADS = 128, EMB_COLS = 8;
+constexpr int SORT_THREADS = 1024, SORT_WARPS = SORT_THREADS / 32, SORT_DIGIT = 9, SORT_BINS = 1 << SORT_DIGIT;
+constexpr int SORT_SMEM = SORT_WARPS * SORT_BINS * 4;
+constexpr int CHUNK = 32;                     // pairs of a block of sums: a warp's lanes look one chunk ahead
+constexpr int SUM_THREADS = 128, SUM_AHEAD = 8;
+constexpr int ZERO_BYTES = 1 << 17;           // of the table, of a block that zeroes
+constexpr int JOIN_THREADS = 256, JOIN_COLS = 128, JOIN_BLOCKS = 32;
+constexpr int ROW_THREADS = 256, ROW_AHEAD = 4;
 
-template <typename T> __device__ __forceinline__ float emb_value(T x) {
+template <typename T> __device__ __forceinline__ float to_float(T x) {
   if constexpr (__is_same(T, float)) return x;
   else if constexpr (__is_same(T, __half)) return __half2float(x);
   else return __bfloat162float(x);
 }
-template <typename T> __device__ __forceinline__ T emb_store(float x) {
+template <typename T> __device__ __forceinline__ T from_float(float x) {
   if constexpr (__is_same(T, float)) return x;
   else if constexpr (__is_same(T, __half)) return __float2half_rn(x);
   else return __float2bfloat16_rn(x);
 }
 
-template <typename T, typename I>
-__global__ void __launch_bounds__(EMB_THREADS)
-embedding_kernel(const I* __restrict__ tokens, const T* __restrict__ table, long long pitch, int V, int H, float scale, T* __restrict__ out) {
-  const long long t = tokens[blockIdx.x];
-  T* to = out + static_cast<long long>(blockIdx.x) * H;
-  const bool there = t >= 0 && t < V;
-  const T* from = table + (there ? t : 0) * pitch;
-  for (int c = threadIdx.x; c < H; c += EMB_THREADS) to[c] = there ? emb_store<T>(emb_value(from[c]) * scale) : emb_store<T>(__int_as_float(0x7fffffff));
-}
+// N values that are moved at once
+template <typename T, int N> struct alignas(sizeof(T) * N) Piece { T v[N]; };
 
-template <typename T, typename I>
-__global__ void __launch_bounds__(EMB_THREADS)
-embedding_grad_kernel(const I* __restrict__ tokens, int n, const T* __restrict__ dy, long long pitch, int H, float scale, long long padding,
-                      T* __restrict__ dtable) {
-  __shared__ int s_at[EMB_THREADS];
-  __shared__ int s_count[EMB_THREADS / 32];
-  const long long v = blockIdx.x;
-  const int first = blockIdx.y * EMB_THREADS * EMB_COLS + threadIdx.x, lane = threadIdx.x & 31, w = threadIdx.x >> 5;
-  float sum[EMB_COLS] = {};
-  for (int i = 0; i < n && v != padding; i += EMB_THREADS) {
-    const int at = i + threadIdx.x;
-    const bool mine = at < n && tokens[at] == v;
-    const unsigned met = __ballot_sync(0xffffffffu, mine);
-    __syncthreads();
-    if (lane == 0) s_count[w] = __popc(met);
-    __syncthreads();
-    int base = 0, count = 0;
-    for (int k = 0; k < EMB_THREADS / 32; ++k) { if (k < w) base += s_count[k]; count += s_count[k]; }
-    if (count == 0) continue;
-    if (mine) s_at[base + __popc(met & ((1u << lane) - 1u))] = at;
-    __syncthreads();
-    for (int k = 0; k < count; ++k) {
-      const T* from = dy + s_at[k] * pitch;
+// ------------------------------------------------------------------------------------------------------------------------ lookup
+// `group` threads (a power of two) a row, ROWS rows for each of them at a time
+template <typename T, typename I, int N, int ROWS>
+__global__ void __launch_bounds__(ROW_THREADS)
+embedding_kernel(const I* __restrict__ tokens, long long n, const T* __restrict__ table, long long pitch, int V, int H, float scale,
+                 T* __restrict__ out, int group) {
+  using P = Piece<T, N>;
+  pdl_launch_next();
+  pdl_wait();
+  const int groups = ROW_THREADS / group, at = threadIdx.x & (group - 1);
+  const long long first = (static_cast<long long>(blockIdx.x) * groups + threadIdx.x / group) * ROWS;
+  long long t[ROWS];
 #pragma unroll
-      for (int c = 0; c < EMB_COLS; ++c) if (first + c * EMB_THREADS < H) sum[c] += emb_value(from[first + c * EMB_THREADS]);
+  for (int r = 0; r < ROWS; ++r) {
+    t[r] = first + r < n ? static_cast<long long>(tokens[first + r]) : -1;
+    if (t[r] >= V) t[r] = -1;
+  }
+  for (int c = at * N; c < H; c += group * N) {
+    P p[ROWS];
+#pragma unroll
+    for (int r = 0; r < ROWS; ++r)
+      if (t[r] >= 0) p[r] = *reinterpret_cast<const P*>(table + t[r] * pitch + c);
+#pragma unroll
+    for (int r = 0; r < ROWS; ++r) {
+      if (first + r >= n) break;
+#pragma unroll
+      for (int i = 0; i < N; ++i) p[r].v[i] = from_float<T>(t[r] >= 0 ? to_float(p[r].v[i]) * scale : __int_as_float(0x7fffffff));
+      *reinterpret_cast<P*>(out + (first + r) * H + c) = p[r];
     }
   }
-#pragma unroll
-  for (int c = 0; c < EMB_COLS; ++c) if (first + c * EMB_THREADS < H) dtable[v * H + first + c * EMB_THREADS] = emb_store<T>(sum[c] * scale);
 }
 
-template <typename T, typename I>
-static int embedding(const void* tokens, long long n, const void* table, long long pitch, int V, int H, float scale, void* out, cudaStream_t s) {
-  embedding_kernel<T, I><<<static_cast<unsigned>(n), EMB_THREADS, 0, s>>>(static_cast<const I*>(tokens), static_cast<const T*>(table), pitch, V, H,
-                                                                        scale, static_cast<T*>(out));
-  AXB_CUDA(cudaGetLastError());
+// ------------------------------------------------------------------------------------------------------------------------ gradient
+struct Digits { int passes, bits[4]; };
+
+__device__ __forceinline__ uint32_t cluster_ctas() {
+  uint32_t r;
+  asm volatile("mov.u32 %0, %%cluster_nctarank;" : "=r"(r));
+  return r;
+}
+__device__ __forceinline__ uint32_t read_of_cta(const uint32_t* p, uint32_t cta) {
+  uint32_t addr, v;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(addr) : "r"(smem_u32(p)), "r"(cta));
+  asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(addr) : "memory");
+  return v;
+}
+
+// One cluster.  `a` and `b` take turns; the result is in `b` after an odd number of passes, in `a` after an even one.  Tokens without a
+// gradient have the key V.  A warp has a contiguous run of pairs and counts of its own, so that equal digits keep their order.
+template <typename I>
+__global__ void __launch_bounds__(SORT_THREADS)
+sort_tokens_kernel(const I* __restrict__ tokens, int n, int V, long long padding, Digits digits, uint2* a, uint2* b, uint32_t* met) {
+  extern __shared__ uint32_t s_count[];         // [SORT_WARPS][SORT_BINS]
+  __shared__ uint32_t s_total[SORT_BINS], s_base[SORT_BINS], s_warp[SORT_BINS / 32];
+  pdl_launch_next();
+  pdl_wait();
+  const int tid = threadIdx.x, lane = tid & 31, w = tid >> 5;
+  const uint32_t cta = cluster_cta_rank(), ctas = cluster_ctas();
+  for (uint32_t i = cta * SORT_THREADS + tid; i < (V + 31u) / 32u; i += ctas * SORT_THREADS) met[i] = 0u;
+  const long long warps = static_cast<long long>(ctas) * SORT_WARPS, run = ((n + warps - 1) / warps + 31) / 32 * 32;
+  const long long from = (static_cast<long long>(cta) * SORT_WARPS + w) * run, to = min(from + run, static_cast<long long>(n));
+  uint32_t* mine = s_count + w * SORT_BINS;
+  const uint2* in = nullptr;
+  uint2* out = b;
+  int shift = 0;
+  auto pair_at = [&](long long i) {
+    if (in) return __ldcg(in + i);
+    const long long t = tokens[i];
+    return make_uint2(t >= 0 && t < V && t != padding ? static_cast<uint32_t>(t) : static_cast<uint32_t>(V), static_cast<uint32_t>(i));
+  };
+  for (int pass = 0; pass < digits.passes; ++pass) {
+    const int bits = digits.bits[pass], bins = 1 << bits;
+    const uint32_t mask = bins - 1u;
+    for (int i = lane; i < bins; i += 32) mine[i] = 0u;
+    __syncwarp();
+    for (long long i = from; i < to; i += 32) {
+      const bool there = i + lane < to;
+      const uint32_t d = there ? pair_at(i + lane).x >> shift & mask : 0xffffffffu;
+      const uint32_t same = __match_any_sync(0xffffffffu, d);
+      if (there && (same & ((1u << lane) - 1u)) == 0u) mine[d] += __popc(same);
+      __syncwarp();
+    }
+    __syncthreads();
+    // counts of the warps before, then those of the CTAs before and of the smaller digits
+    if (tid < bins) {
+      uint32_t sum = 0u;
+#pragma unroll 8
+      for (int k = 0; k < SORT_WARPS; ++k) {
+        const uint32_t c = s_count[k * SORT_BINS + tid];
+        s_count[k * SORT_BINS + tid] = sum;
+        sum += c;
+      }
+      s_total[tid] = sum;
+    }
+    __syncwarp();
+    cluster_sync_all();                          // also: `met` is zero
+    uint32_t before = 0u, all = 0u, upto = 0u;
+    if (tid < SORT_BINS) {
+      if (tid < bins)
+        for (uint32_t k = 0; k < ctas; ++k) {
+          const uint32_t c = read_of_cta(s_total + tid, k);
+          if (k < cta) before += c;
+          all += c;
+        }
+      upto = all;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const uint32_t v = __shfl_up_sync(0xffffffffu, upto, o);
+        if (lane >= o) upto += v;
+      }
+      if (lane == 31) s_warp[w] = upto;
+    }
+    __syncthreads();
+    if (tid < bins) {
+      for (int k = 0; k < w; ++k) upto += s_warp[k];
+      s_base[tid] = upto - all + before;
+    }
+    __syncthreads();
+    for (long long i = from; i < to; i += 32) {
+      const bool there = i + lane < to;
+      const uint2 p = there ? pair_at(i + lane) : make_uint2(0u, 0u);
+      const uint32_t d = there ? p.x >> shift & mask : 0xffffffffu;
+      const uint32_t same = __match_any_sync(0xffffffffu, d), lower = same & ((1u << lane) - 1u);
+      uint32_t at = 0u;
+      if (there) at = s_base[d] + mine[d] + __popc(lower);
+      __syncwarp();
+      if (there) {
+        if (lower == 0u) mine[d] += __popc(same);
+        if (pass == 0 && p.x < static_cast<uint32_t>(V)) atomicOr(met + (p.x >> 5), 1u << (p.x & 31u));
+        out[at] = p;
+      }
+      __syncwarp();
+    }
+    cluster_sync_all();                          // the pairs are there, and the totals have been read
+    in = out;
+    out = out == b ? a : b;
+    shift += bits;
+  }
+}
+
+// Where a chunk's work lies in the sorted list: pairs [from, to); `partial`: the last segment goes on in the next chunk's work, or began in
+// an earlier one.
+template <typename T, int N>
+__global__ void __launch_bounds__(SUM_THREADS)
+sum_rows_kernel(const uint2* __restrict__ pairs, int n, const T* __restrict__ dy, long long pitch, int V, int H, int Hp, float scale,
+                const uint32_t* __restrict__ met, T* __restrict__ dtable, float* __restrict__ partial, int slices, long long sum_blocks,
+                int zero_rows) {
+  using P = Piece<T, N>;
+  __shared__ uint2 s_pair[2 * CHUNK + 1];
+  pdl_launch_next();
+  pdl_wait();
+  const int tid = threadIdx.x, lane = tid & 31;
+  if (blockIdx.x >= sum_blocks) {
+    const int words = H / N, v0 = static_cast<int>(blockIdx.x - sum_blocks) * zero_rows, rows = min(zero_rows, V - v0);
+    const int row_step = SUM_THREADS / words, col_step = SUM_THREADS - row_step * words;
+    int row = tid / words, col = tid - row * words;
+    P zero;
+#pragma unroll
+    for (int i = 0; i < N; ++i) zero.v[i] = from_float<T>(0.f);
+    while (row < rows) {
+      const int v = v0 + row;
+      if (!(__ldg(met + (v >> 5)) >> (v & 31) & 1u)) *reinterpret_cast<P*>(dtable + static_cast<long long>(v) * H + col * N) = zero;
+      row += row_step; col += col_step;
+      if (col >= words) { col -= words; ++row; }
+    }
+    return;
+  }
+  const int chunk = static_cast<int>(blockIdx.x / slices), slice = static_cast<int>(blockIdx.x - static_cast<long long>(chunk) * slices);
+  const long long base = static_cast<long long>(chunk) * CHUNK;
+  if (tid <= 2 * CHUNK) {
+    const long long i = base - 1 + tid;
+    s_pair[tid] = i >= 0 && i < n ? pairs[i] : make_uint2(0xffffffffu, 0u);
+  }
+  __syncthreads();
+  const auto key = [&](int i) { return s_pair[1 + i].x; };          // of the pair `i` behind the chunk's first
+  const int here = static_cast<int>(min(static_cast<long long>(CHUNK), n - base));
+  const uint32_t first = key(0), last = key(here - 1);
+  const bool goes_on = key(-1) == first, all_one = here == CHUNK && first == last;
+  int from = 0, to = here;
+  bool open = false;                             // the last segment has pieces in other blocks
+  const unsigned ahead = __ballot_sync(0xffffffffu, key(CHUNK + lane) == last);      // of the next chunk, those of the last token
+  if (here == CHUNK) {
+    if (ahead == 0xffffffffu) open = true;
+    else to += __ffs(~ahead) - 1;
+  }
+  if (goes_on) {
+    if (all_one) open = true;
+    else from = __ffs(~__ballot_sync(0xffffffffu, lane < here && key(lane) == first)) - 1;
+  }
+  if (from >= here) return;
+  const int col = (slice * SUM_THREADS + tid) * N;
+  if (col >= H) return;
+  float sum[N] = {};
+  uint32_t now = key(from);
+  const auto store = [&] {
+    if (now >= static_cast<uint32_t>(V)) return;
+    P p;
+#pragma unroll
+    for (int i = 0; i < N; ++i) { p.v[i] = from_float<T>(sum[i] * scale); sum[i] = 0.f; }
+    *reinterpret_cast<P*>(dtable + static_cast<long long>(now) * H + col) = p;
+  };
+  for (int i = from; i < to; i += SUM_AHEAD) {
+    P p[SUM_AHEAD];
+#pragma unroll
+    for (int k = 0; k < SUM_AHEAD; ++k)
+      if (i + k < to && key(i + k) < static_cast<uint32_t>(V)) p[k] = *reinterpret_cast<const P*>(dy + s_pair[1 + i + k].y * pitch + col);
+#pragma unroll
+    for (int k = 0; k < SUM_AHEAD; ++k) {
+      if (i + k >= to || key(i + k) >= static_cast<uint32_t>(V)) break;
+      if (key(i + k) != now) { store(); now = key(i + k); }
+#pragma unroll
+      for (int c = 0; c < N; ++c) sum[c] += to_float(p[k].v[c]);
+    }
+  }
+  if (!open || now != last) { store(); return; }
+  if (now >= static_cast<uint32_t>(V)) return;
+  float* to_part = partial + static_cast<long long>(chunk) * Hp + col;
+#pragma unroll
+  for (int c = 0; c < N; ++c) to_part[c] = sum[c];
+}
+
+// Segments that fill the chunk behind the one that they begin in: their pieces are that chunk and all that they fill.
+template <typename T>
+__global__ void __launch_bounds__(JOIN_THREADS)
+join_rows_kernel(const uint2* __restrict__ pairs, int n, int V, int H, int Hp, float scale, const float* __restrict__ partial,
+                 T* __restrict__ dtable) {
+  __shared__ int s_first[JOIN_THREADS];
+  __shared__ int s_warp[JOIN_THREADS / 32];
+  __shared__ float4 s_sum[JOIN_THREADS / 32][32];
+  pdl_launch_next();
+  pdl_wait();
+  const int tid = threadIdx.x, lane = tid & 31, w = tid >> 5;
+  const int full = n / CHUNK;                    // chunks that a segment can fill
+  const auto last_of = [&](long long chunk) { return pairs[chunk * CHUNK + CHUNK - 1].x; };
+  const int col = blockIdx.y * JOIN_COLS + lane * 4;
+  int seen = 0;
+  for (int c0 = 0; c0 + 1 < full; c0 += JOIN_THREADS) {
+    const int c = c0 + tid;
+    bool begins = false;
+    if (c + 1 < full) {
+      const uint32_t k = last_of(c);
+      begins = k < static_cast<uint32_t>(V) && last_of(c + 1) == k && (c == 0 || last_of(c - 1) != k);
+    }
+    const unsigned flags = __ballot_sync(0xffffffffu, begins);
+    if (lane == 0) s_warp[w] = __popc(flags);
+    __syncthreads();
+    int before = 0, count = 0;
+    for (int i = 0; i < JOIN_THREADS / 32; ++i) { if (i < w) before += s_warp[i]; count += s_warp[i]; }
+    if (begins) s_first[before + __popc(flags & ((1u << lane) - 1u))] = c;
+    __syncthreads();
+    for (int i = 0; i < count; ++i) {
+      if ((seen + i) % JOIN_BLOCKS != static_cast<int>(blockIdx.x)) continue;
+      const int begin = s_first[i];
+      const uint32_t k = last_of(begin);
+      int pieces = 1;
+      for (int more = JOIN_THREADS; more == JOIN_THREADS; pieces += more) {
+        const int at = begin + pieces + tid;
+        more = __syncthreads_count(at < full && last_of(at) == k);
+      }
+      float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
+      if (col < Hp) {
+#pragma unroll 4
+        for (int r = w; r < pieces; r += JOIN_THREADS / 32) {
+          const float4 p = *reinterpret_cast<const float4*>(partial + static_cast<long long>(begin + r) * Hp + col);
+          sum.x += p.x; sum.y += p.y; sum.z += p.z; sum.w += p.w;
+        }
+      }
+      s_sum[w][lane] = sum;
+      __syncthreads();
+      if (w == 0) {
+#pragma unroll
+        for (int g = 1; g < JOIN_THREADS / 32; ++g) {
+          const float4 p = s_sum[g][lane];
+          sum.x += p.x; sum.y += p.y; sum.z += p.z; sum.w += p.w;
+        }
+        const float v[4] = {sum.x, sum.y, sum.z, sum.w};
+#pragma unroll
+        for (int g = 0; g < 4; ++g) if (col + g < H) dtable[static_cast<long long>(k) * H + col + g] = from_float<T>(v[g] * scale);
+      }
+      __syncthreads();
+    }
+    seen += count;
+    __syncthreads();
+  }
+}
+
+// ------------------------------------------------------------------------------------------------------------------------ launches
+// Bytes that are moved at once: what divides every address and pitch, 16 at most.
+static int piece_bytes(int value, std::initializer_list<unsigned long long> of) {
+  unsigned long long all = 16;
+  for (unsigned long long x : of) all |= x;
+  const int bytes = static_cast<int>(all & (~all + 1));
+  return bytes < value ? value : bytes;
+}
+static unsigned long long address(const void* p) { return reinterpret_cast<unsigned long long>(p); }
+
+template <typename T, typename I, int N>
+static int look_up(const void* tokens, long long n, const void* table, long long pitch, int V, int H, float scale, void* out, cudaStream_t s) {
+  const int words = H / N;
+  int group = 32;
+  while (group < ROW_THREADS && group < words) group *= 2;
+  const int groups = ROW_THREADS / group;
+  // several rows at a time where there are blocks enough for all SMs without
+  const bool ahead = n / groups >= 8ll * ROW_AHEAD * sm_count_current();
+  const long long per = static_cast<long long>(groups) * (ahead ? ROW_AHEAD : 1);
+  AXB_CUDA(pdl_launch(ahead ? embedding_kernel<T, I, N, ROW_AHEAD> : embedding_kernel<T, I, N, 1>, dim3(static_cast<unsigned>((n + per - 1) / per)),
+                      dim3(ROW_THREADS), 0, s, static_cast<const I*>(tokens), n, static_cast<const T*>(table), pitch, V, H, scale,
+                      static_cast<T*>(out), group));
   return 0;
 }
-template <typename T, typename I>
-static int embedding_grad(const void* tokens, long long n, const void* dy, long long pitch, int V, int H, float scale, long long padding,
-                          void* dtable, cudaStream_t s) {
-  const dim3 grid(V, (H + EMB_THREADS * EMB_COLS - 1) / (EMB_THREADS * EMB_COLS));
-  embedding_grad_kernel<T, I><<<grid, EMB_THREADS, 0, s>>>(static_cast<const I*>(tokens), static_cast<int>(n), static_cast<const T*>(dy), pitch, H,
-                                                         scale, padding, static_cast<T*>(dtable));
-  AXB_CUDA(cudaGetLastError());
+
+struct GradWork {
+  long long chunks, Hp, met, pairs, words;       // words before `met`: none; pairs of 2 words begin behind it
+  GradWork(long long n, int V, int H) {
+    chunks = (n + CHUNK - 1) / CHUNK;
+    Hp = (H + 3) / 4 * 4;
+    met = ((V + 31ll) / 32 + 3) / 4 * 4;
+    pairs = (2 * n + 3) / 4 * 4;
+    words = met + 2 * pairs + (chunks > 1 ? chunks * Hp : 0);
+  }
+};
+
+template <typename I>
+static int sort_tokens(const void* tokens, int n, int V, long long padding, uint2* a, uint2* b, uint32_t* met, Digits& digits, cudaStream_t s) {
+  int bits = 0;
+  while (V >> bits) ++bits;                      // V itself is the key of tokens without a gradient
+  digits.passes = (bits + SORT_DIGIT - 1) / SORT_DIGIT;
+  for (int i = 0, left = bits; i < digits.passes; ++i) {
+    digits.bits[i] = (left + digits.passes - i - 1) / (digits.passes - i);
+    left -= digits.bits[i];
+  }
+  auto kernel = sort_tokens_kernel<I>;
+  AXB_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, SORT_SMEM));
+  cudaLaunchConfig_t cfg = {};
+  const unsigned ctas = n <= 2 * SORT_THREADS ? 1 : 8;
+  cfg.gridDim = dim3(ctas); cfg.blockDim = dim3(SORT_THREADS); cfg.dynamicSmemBytes = SORT_SMEM; cfg.stream = s;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = ctas; attr[0].val.clusterDim.y = 1; attr[0].val.clusterDim.z = 1;
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[1].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr; cfg.numAttrs = max_ctas() == 0 ? 2 : 1;
+  AXB_CUDA(cudaLaunchKernelEx(&cfg, kernel, static_cast<const I*>(tokens), n, V, padding, digits, a, b, met));
   return 0;
+}
+
+template <typename T, int N>
+static int sum_rows(const uint2* pairs, int n, const void* dy, long long pitch, int V, int H, const GradWork& work, float scale,
+                    const uint32_t* met, void* dtable, float* partial, cudaStream_t s) {
+  const int slices = (H / N + SUM_THREADS - 1) / SUM_THREADS;
+  const int row_bytes = H * static_cast<int>(sizeof(T));
+  const int zero_rows = row_bytes >= ZERO_BYTES ? 1 : ZERO_BYTES / row_bytes;
+  const long long sum_blocks = work.chunks * slices, blocks = sum_blocks + (V + static_cast<long long>(zero_rows) - 1) / zero_rows;
+  if (blocks > 0x7fffffffll) { set_error("gradient of an embedding: %d tokens with rows of %d values are too many blocks", n, H); return -1; }
+  AXB_CUDA(pdl_launch(sum_rows_kernel<T, N>, dim3(static_cast<unsigned>(blocks)), dim3(SUM_THREADS), 0, s, pairs, n, static_cast<const T*>(dy),
+                      pitch, V, H, static_cast<int>(work.Hp), scale, met, static_cast<T*>(dtable), partial, slices, sum_blocks, zero_rows));
+  return 0;
+}
+
+template <typename T>
+static int gradient(const void* tokens, int token_bytes, int n, const void* dy, long long pitch, int V, int H, float scale, long long padding,
+                    void* dtable, uint32_t* words, cudaStream_t s) {
+  if (n == 0) {
+    AXB_CUDA(cudaMemsetAsync(dtable, 0, static_cast<size_t>(V) * H * sizeof(T), s));
+    return 0;
+  }
+  const GradWork work(n, V, H);
+  uint2 *a = reinterpret_cast<uint2*>(words + work.met), *b = reinterpret_cast<uint2*>(words + work.met + work.pairs);
+  float* partial = reinterpret_cast<float*>(words + work.met + 2 * work.pairs);
+  Digits digits;
+  if (token_bytes == 8 ? sort_tokens<long long>(tokens, n, V, padding, a, b, words, digits, s)
+                       : sort_tokens<int>(tokens, n, V, padding, a, b, words, digits, s)) return -1;
+  const uint2* pairs = digits.passes % 2 ? b : a;
+  const int size = sizeof(T), bytes = piece_bytes(size, {address(dy), address(dtable), static_cast<unsigned long long>(H) * size,
+                                                         static_cast<unsigned long long>(pitch) * size});
+  const auto sums = bytes == 16 ? sum_rows<T, 16 / sizeof(T)> : bytes == 8 ? sum_rows<T, 8 / sizeof(T)> : bytes == 4 ? sum_rows<T, 4 / sizeof(T)>
+                                                                                                                     : sum_rows<T, 1>;
+  if (sums(pairs, n, dy, pitch, V, H, work, scale, words, dtable, partial, s)) return -1;
+  if (n < 2 * CHUNK) return 0;
+  AXB_CUDA(pdl_launch(join_rows_kernel<T>, dim3(JOIN_BLOCKS, static_cast<unsigned>((work.Hp + JOIN_COLS - 1) / JOIN_COLS)), dim3(JOIN_THREADS), 0, s,
+                      pairs, n, V, H, static_cast<int>(work.Hp), scale, static_cast<const float*>(partial), static_cast<T*>(dtable)));
+  return 0;
+}
+
+template <typename T>
+static int look_up_by(const void* tokens, int token_bytes, long long n, const void* table, long long pitch, int V, int H, float scale, void* out,
+                      cudaStream_t s) {
+  const int size = sizeof(T), bytes = piece_bytes(size, {address(table), address(out), static_cast<unsigned long long>(H) * size,
+                                                         static_cast<unsigned long long>(pitch) * size});
+  const auto go = [&](auto index) {
+    using I = decltype(index);
+    const auto kernel = bytes == 16 ? look_up<T, I, 16 / sizeof(T)> : bytes == 8 ? look_up<T, I, 8 / sizeof(T)>
+                      : bytes == 4 ? look_up<T, I, 4 / sizeof(T)> : look_up<T, I, 1>;
+    return kernel(tokens, n, table, pitch, V, H, scale, out, s);
+  };
+  return token_bytes == 8 ? go(0ll) : go(0);
 }
 
 }  // namespace axb
@@ -93,19 +451,17 @@ extern "C" int axb_embedding(const void* tokens, int token_bytes, long long n, c
                              void* out, int dtype, void* stream) {
   if (refused("embedding", n, V, H, dtype, token_bytes)) return -1;
   if (n == 0) return 0;
-  const cudaStream_t s = static_cast<cudaStream_t>(stream);
-  const auto go = token_bytes == 8 ? (dtype == 0 ? embedding<__nv_bfloat16, long long> : dtype == 1 ? embedding<__half, long long> : embedding<float, long long>)
-                                   : (dtype == 0 ? embedding<__nv_bfloat16, int> : dtype == 1 ? embedding<__half, int> : embedding<float, int>);
-  return go(tokens, n, table, pitch, V, H, scale, out, s);
+  const auto go = dtype == 0 ? look_up_by<__nv_bfloat16> : dtype == 1 ? look_up_by<__half> : look_up_by<float>;
+  return go(tokens, token_bytes, n, table, pitch, V, H, scale, out, static_cast<cudaStream_t>(stream));
 }
 
-extern "C" long long axb_embedding_grad_words(long long n, int V, int H) { return 1; }
+extern "C" long long axb_embedding_grad_words(long long n, int V, int H) { return GradWork(n, V, H).words; }
 
 extern "C" int axb_embedding_grad(const void* tokens, int token_bytes, long long n, const void* dy, long long pitch, int V, int H, float scale,
                                   long long padding, void* dtable, void* work, int dtype, void* stream) {
   if (refused("gradient of an embedding", n, V, H, dtype, token_bytes)) return -1;
-  const cudaStream_t s = static_cast<cudaStream_t>(stream);
-  const auto go = token_bytes == 8 ? (dtype == 0 ? embedding_grad<__nv_bfloat16, long long> : dtype == 1 ? embedding_grad<__half, long long> : embedding_grad<float, long long>)
-                                   : (dtype == 0 ? embedding_grad<__nv_bfloat16, int> : dtype == 1 ? embedding_grad<__half, int> : embedding_grad<float, int>);
-  return go(tokens, n, dy, pitch, V, H, scale, padding, dtable, s);
+  if (address(work) % 16) { set_error("gradient of an embedding: the workspace must be 16-byte aligned"); return -1; }
+  const auto go = dtype == 0 ? gradient<__nv_bfloat16> : dtype == 1 ? gradient<__half> : gradient<float>;
+  return go(tokens, token_bytes, static_cast<int>(n), dy, pitch, V, H, scale, padding, dtable, static_cast<uint32_t*>(work),
+            static_cast<cudaStream_t>(stream));
 }

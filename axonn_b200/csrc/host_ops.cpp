@@ -1,6 +1,7 @@
 // Host paths of the operators that short calls are bound by: the same launches as the Python code beside them (ops/norm.py,
-// ops/attention_cuda.py, ops/kv_cache.py, ops/beam.py, intra_layer/fully_connected.py), with the questions asked and the tensors allocated in C++, and the
-// normalisation's autograd node in C++, so that neither its backward nor the launches of a layer wait for the interpreter.
+// ops/attention_cuda.py, ops/kv_cache.py, ops/beam.py, ops/token_probs.py, ops/embedding.py, intra_layer/fully_connected.py), with the questions
+// asked and the tensors allocated in C++, and the autograd nodes of the normalisation, the token log-probabilities and the table lookup in
+// C++, so that neither their backward nor the launches of a layer wait for the interpreter.
 //
 // A function returns None where the call is not one of those it takes; the caller then goes its general way, which accepts or
 // refuses it.  Nothing is kept from one call to the next.  The kernels are those of the library that ops/_lib.py has loaded: bind()
@@ -38,7 +39,9 @@ using std::optional;
   X(axb_norm_grid, norm_grid) X(axb_gemm, gemm) X(axb_flash_attn_fwd, flash_fwd) X(axb_last_error, last_error) \
   X(axb_plan_blocks, plan_blocks) X(axb_store_blocks, store_blocks) X(axb_reorder_blocks, reorder_blocks) \
   X(axb_cached_attention_words, attention_words) X(axb_cached_attention, cached_attention) \
-  X(axb_beam_select_words, beam_words) X(axb_beam_select, beam_select)
+  X(axb_beam_select_words, beam_words) X(axb_beam_select, beam_select) \
+  X(axb_token_log_probs, token_log_probs) X(axb_token_log_probs_bwd, token_log_probs_bwd) \
+  X(axb_embedding, embedding) X(axb_embedding_grad_words, embedding_grad_words) X(axb_embedding_grad, embedding_grad)
 #define AXB_DECLARE(symbol, name) decltype(&::symbol) name = nullptr;
 AXB_LAUNCHERS(AXB_DECLARE)
 PyObject *kernel_error = nullptr, *parameter_type = nullptr;
@@ -106,6 +109,23 @@ void run_norm(const Tensor& x, const optional<Tensor>& delta, const Tensor& gamm
   }
 }
 
+// Node::gradients() of kernels that leave no graph: differentiating them again is an error (first_derivative_only in ops/direct.py).
+template <typename Node>
+torch::autograd::variable_list first_derivative(torch::autograd::AutogradContext* ctx, const torch::autograd::variable_list& grads, const char* why) {
+  if (!at::GradMode::is_enabled()) return Node::gradients(ctx, grads);
+  torch::autograd::variable_list out, inputs = ctx->get_saved_variables();
+  {
+    at::AutoGradMode no_grad(false);
+    out = Node::gradients(ctx, grads);
+  }
+  inputs.insert(inputs.end(), grads.begin(), grads.end());
+  if (!std::any_of(inputs.begin(), inputs.end(), [](const Tensor& t) { return t.defined() && t.requires_grad(); })) return out;
+  const auto node = std::make_shared<torch::autograd::Error>(why, torch::autograd::collect_next_edges(inputs));
+  for (Tensor& t : out)
+    if (t.defined()) torch::autograd::set_history(t = t.detach(), node);
+  return out;
+}
+
 // Inputs: x, delta (may be missing), gamma, beta (may be missing).  Outputs: y, or h and y.
 struct NormNode : torch::autograd::Function<NormNode> {
   static torch::autograd::variable_list forward(torch::autograd::AutogradContext* ctx, const Tensor& x, const optional<Tensor>& delta,
@@ -119,21 +139,8 @@ struct NormNode : torch::autograd::Function<NormNode> {
     if (delta) return {h, y};
     return {y};
   }
-  // The kernels leave no graph: differentiating these gradients again is an error (first_derivative_only in ops/direct.py).
   static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx, torch::autograd::variable_list grads) {
-    if (!at::GradMode::is_enabled()) return gradients(ctx, grads);
-    torch::autograd::variable_list out, inputs = ctx->get_saved_variables();
-    {
-      at::AutoGradMode no_grad(false);
-      out = gradients(ctx, grads);
-    }
-    inputs.insert(inputs.end(), grads.begin(), grads.end());
-    if (!std::any_of(inputs.begin(), inputs.end(), [](const Tensor& t) { return t.defined() && t.requires_grad(); })) return out;
-    const auto node = std::make_shared<torch::autograd::Error>("Norm: second derivatives are not implemented",
-                                                               torch::autograd::collect_next_edges(inputs));
-    for (Tensor& t : out)
-      if (t.defined()) torch::autograd::set_history(t = t.detach(), node);
-    return out;
+    return first_derivative<NormNode>(ctx, grads, "Norm: second derivatives are not implemented");
   }
   static torch::autograd::variable_list gradients(torch::autograd::AutogradContext* ctx, const torch::autograd::variable_list& grads) {
     const auto saved = ctx->get_saved_variables();
@@ -481,6 +488,214 @@ PyObject* py_beam_select(PyObject*, PyObject* const* a, Py_ssize_t n) {
   END_HANDLE_TH_ERRORS
 }
 
+// -------------------------------------------------------------------------------------------------- log-probabilities of tokens
+// logits [(batches,) (rows,) V] whose last dimension is dense, with the strides of the other two; tokens likewise without the last.
+struct TokenRows {
+  int64_t batches = 1, per_batch = 1, batch_stride = 0, row_stride = 0, token_batch_stride = 0, token_stride = 0, V = 0;
+  TokenRows(const Tensor& z, const Tensor& tokens) {
+    const int64_t d = z.dim();
+    V = z.size(d - 1);
+    if (d > 1) { per_batch = z.size(d - 2); row_stride = z.stride(d - 2); if (tokens.defined()) token_stride = tokens.stride(d - 2); }
+    if (d > 2) { batches = z.size(0); batch_stride = z.stride(0); if (tokens.defined()) token_batch_stride = tokens.stride(0); }
+  }
+};
+const long long* words(const Tensor& t) { return t.defined() ? reinterpret_cast<const long long*>(t.data_ptr<int64_t>()) : nullptr; }
+long long* words_out(const Tensor& t) { return t.defined() ? reinterpret_cast<long long*>(t.data_ptr<int64_t>()) : nullptr; }
+float* floats(const Tensor& t) { return t.defined() ? t.data_ptr<float>() : nullptr; }
+
+struct TokenResults { Tensor log_probs, entropy, top_log_probs, top_tokens, stats; };
+TokenResults run_token_log_probs(const Tensor& logits, const Tensor& tokens, bool entropy, int64_t top, double scale, int64_t ignored) {
+  const TokenRows r(logits, tokens);
+  const auto f32 = logits.options().dtype(at::kFloat);
+  c10::SmallVector<int64_t, 5> shape(logits.sizes().begin(), logits.sizes().end() - 1);
+  TokenResults out;
+  if (tokens.defined()) out.log_probs = at::empty(shape, f32);
+  if (entropy) out.entropy = at::empty(shape, f32);
+  if (top) {
+    shape.push_back(top);
+    out.top_log_probs = at::empty(shape, f32);
+    out.top_tokens = at::empty(shape, f32.dtype(at::kLong));
+  }
+  out.stats = at::empty({r.batches * r.per_batch, 4}, f32);
+  check(token_log_probs(logits.data_ptr(), r.batch_stride, r.row_stride, words(tokens), r.token_batch_stride, r.token_stride, floats(out.log_probs),
+                        floats(out.entropy), floats(out.top_log_probs), words_out(out.top_tokens), floats(out.stats), static_cast<int>(r.batches),
+                        static_cast<int>(r.per_batch), static_cast<int>(r.V), 0, r.V, static_cast<int>(top), static_cast<float>(scale), ignored, 1,
+                        dtype_code(logits), stream()), "axb_token_log_probs");
+  return out;
+}
+
+// Inputs: logits, tokens (may be missing).  Outputs: those asked for of log_probs, entropy, top_log_probs and top_tokens.
+struct TokenLogProbsNode : torch::autograd::Function<TokenLogProbsNode> {
+  static torch::autograd::variable_list forward(torch::autograd::AutogradContext* ctx, const Tensor& logits, const optional<Tensor>& tokens,
+                                                bool entropy, int64_t top, double scale, int64_t ignored) {
+    const TokenResults r = run_token_log_probs(logits, tokens ? *tokens : Tensor(), entropy, top, scale, ignored);
+    ctx->save_for_backward({logits, tokens ? *tokens : Tensor(), r.stats, r.top_tokens});
+    ctx->saved_data["entropy"] = entropy;
+    ctx->saved_data["top"] = top;
+    ctx->saved_data["scale"] = scale;
+    ctx->saved_data["ignored"] = ignored;
+    ctx->set_materialize_grads(false);
+    torch::autograd::variable_list out;
+    for (const Tensor& t : {r.log_probs, r.entropy, r.top_log_probs, r.top_tokens})
+      if (t.defined()) out.push_back(t);
+    if (top) ctx->mark_non_differentiable({out.back()});
+    return out;
+  }
+  static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx, torch::autograd::variable_list grads) {
+    return first_derivative<TokenLogProbsNode>(ctx, grads, "TokenLogProbs: second derivatives are not implemented");
+  }
+  static torch::autograd::variable_list gradients(torch::autograd::AutogradContext* ctx, const torch::autograd::variable_list& grads) {
+    const auto saved = ctx->get_saved_variables();
+    // what hooks (offloading, compression) give back may lie in another layout
+    const Tensor logits = saved[0].dim() > 3 || (saved[0].stride(-1) != 1 && saved[0].size(-1) != 1) ? saved[0].contiguous() : saved[0];
+    const Tensor &tokens = saved[1], stats = dense(saved[2]), at = saved[3].defined() ? saved[3].contiguous() : saved[3];
+    const int64_t top = ctx->saved_data["top"].toInt();
+    size_t i = 0;
+    Tensor d[3];
+    const bool asked[3] = {tokens.defined(), ctx->saved_data["entropy"].toBool(), top > 0};
+    for (int k = 0; k < 3; ++k)
+      if (asked[k]) {
+        if (grads[i].defined()) d[k] = grads[i].contiguous();
+        ++i;
+      }
+    Tensor out;
+    if (d[0].defined() || d[1].defined() || d[2].defined()) {
+      const TokenRows r(logits, tokens);
+      out = at::empty(logits.sizes(), logits.options());
+      check(token_log_probs_bwd(logits.data_ptr(), r.batch_stride, r.row_stride, words(tokens), r.token_batch_stride, r.token_stride,
+                                stats.data_ptr<float>(), floats(d[0]), floats(d[1]), floats(d[2]), words(at), out.data_ptr(),
+                                static_cast<int>(r.batches), static_cast<int>(r.per_batch), static_cast<int>(r.V), 0, r.V, static_cast<int>(top),
+                                static_cast<float>(ctx->saved_data["scale"].toDouble()), ctx->saved_data["ignored"].toInt(), dtype_code(logits),
+                                stream()), "axb_token_log_probs_bwd");
+    }
+    return {out, Tensor(), Tensor(), Tensor(), Tensor(), Tensor()};
+  }
+};
+
+// token_log_probs(logits, tokens | None, entropy, top, 1 / temperature, ignore_index) -> (log_probs | None, entropy | None,
+// top_log_probs | None, top_tokens | None) or None
+PyObject* py_token_log_probs(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  if (n != 6 || !plain(a[0]) || (a[1] != Py_None && !plain(a[1])) || observed()) Py_RETURN_NONE;
+  const Tensor& logits = THPVariable_Unpack(a[0]);
+  const Tensor tokens = a[1] == Py_None ? Tensor() : THPVariable_Unpack(a[1]);
+  const bool entropy = PyObject_IsTrue(a[2]) == 1;
+  const long top = PyLong_AsLong(a[3]);
+  const double scale = PyFloat_AsDouble(a[4]);
+  const long long ignored = PyLong_AsLongLong(a[5]);
+  if (PyErr_Occurred()) return nullptr;
+  const int64_t d = logits.dim();
+  if (d == 0 || d > 3 || dtype_code(logits) < 0 || logits.numel() == 0 || logits.get_device() != c10::cuda::current_device() ||
+      (logits.stride(d - 1) != 1 && logits.size(d - 1) != 1) || logits.size(d - 1) > (1 << 30) || logits.numel() / logits.size(d - 1) > INT32_MAX ||
+      top < 0 || top > std::min<int64_t>(32, logits.size(d - 1)) || (!tokens.defined() && !entropy && !top) ||
+      !(scale > 0 && std::isfinite(scale) && std::isfinite(static_cast<float>(scale)) && static_cast<float>(scale) > 0))
+    Py_RETURN_NONE;
+  if (tokens.defined() && (tokens.scalar_type() != at::kLong || tokens.device() != logits.device() || tokens.sizes() != logits.sizes().slice(0, d - 1)))
+    Py_RETURN_NONE;
+  Tensor out[4];
+  {
+    NoGil no_gil;
+    if (wants_grad(logits)) {
+      const auto list = TokenLogProbsNode::apply(logits, tokens.defined() ? optional<Tensor>(tokens) : std::nullopt, entropy, static_cast<int64_t>(top), scale,
+                                                 static_cast<int64_t>(ignored));
+      const bool asked[4] = {tokens.defined(), entropy, top > 0, top > 0};
+      size_t i = 0;
+      for (int k = 0; k < 4; ++k)
+        if (asked[k]) out[k] = list[i++];
+    } else {
+      const TokenResults r = run_token_log_probs(logits, tokens, entropy, top, scale, ignored);
+      out[0] = r.log_probs; out[1] = r.entropy; out[2] = r.top_log_probs; out[3] = r.top_tokens;
+    }
+  }
+  return tuple_of({out[0], out[1], out[2], out[3]});
+  END_HANDLE_TH_ERRORS
+}
+
+// ---------------------------------------------------------------------------------------------------------------- table lookup
+int index_bytes(const Tensor& tokens) { return tokens.scalar_type() == at::kLong ? 8 : tokens.scalar_type() == at::kInt ? 4 : 0; }
+
+Tensor run_embedding(const Tensor& tokens, const Tensor& weight, double scale) {
+  const Tensor t = tokens.contiguous(), w = weight.stride(1) != 1 && weight.size(1) != 1 ? weight.contiguous() : weight;
+  c10::SmallVector<int64_t, 5> shape(t.sizes().begin(), t.sizes().end());
+  shape.push_back(w.size(1));
+  const Tensor out = at::empty(shape, w.options());
+  if (out.numel())
+    check(embedding(t.data_ptr(), index_bytes(t), t.numel(), w.data_ptr(), w.stride(0), static_cast<int>(w.size(0)), static_cast<int>(w.size(1)),
+                    static_cast<float>(scale), out.data_ptr(), dtype_code(w), stream()), "axb_embedding");
+  return out;
+}
+Tensor run_embedding_grad(const Tensor& tokens, const Tensor& dy, int64_t V, double scale, int64_t padding) {
+  const int64_t H = dy.size(-1);
+  const Tensor t = tokens.contiguous();
+  Tensor rows = dy.reshape({-1, H});
+  if (rows.stride(1) != 1 && H != 1) rows = rows.contiguous();
+  const int64_t n = t.numel();
+  const Tensor out = at::empty({V, H}, rows.options());
+  const Tensor work = at::empty({embedding_grad_words(n, static_cast<int>(V), static_cast<int>(H))}, rows.options().dtype(at::kInt));
+  check(embedding_grad(t.data_ptr(), index_bytes(t), n, rows.data_ptr(), rows.stride(0), static_cast<int>(V), static_cast<int>(H),
+                       static_cast<float>(scale), padding, out.data_ptr(), work.data_ptr(), dtype_code(rows), stream()), "axb_embedding_grad",
+        n == 0 ? 0 : n < 64 ? 2 : 3);
+  return out;
+}
+
+// The gradient of the table as a function of that of the rows; and its own: rows of the table that it is asked with.
+struct EmbeddingGradNode : torch::autograd::Function<EmbeddingGradNode> {
+  static Tensor forward(torch::autograd::AutogradContext* ctx, const Tensor& tokens, const Tensor& dy, int64_t V, double scale, int64_t padding);
+  static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx, torch::autograd::variable_list grads);
+};
+struct EmbeddingNode : torch::autograd::Function<EmbeddingNode> {
+  static Tensor forward(torch::autograd::AutogradContext* ctx, const Tensor& tokens, const Tensor& weight, double scale, int64_t padding) {
+    ctx->save_for_backward({tokens});
+    ctx->saved_data["V"] = weight.size(0);
+    ctx->saved_data["scale"] = scale;
+    ctx->saved_data["padding"] = padding;
+    return run_embedding(tokens, weight, scale);
+  }
+  static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx, torch::autograd::variable_list grads) {
+    const Tensor tokens = ctx->get_saved_variables()[0];
+    const int64_t V = ctx->saved_data["V"].toInt(), padding = ctx->saved_data["padding"].toInt();
+    const double scale = ctx->saved_data["scale"].toDouble();
+    return {Tensor(), wants_grad(grads[0]) ? EmbeddingGradNode::apply(tokens, grads[0], V, scale, padding)
+                                           : run_embedding_grad(tokens, grads[0], V, scale, padding), Tensor(), Tensor()};
+  }
+};
+Tensor EmbeddingGradNode::forward(torch::autograd::AutogradContext* ctx, const Tensor& tokens, const Tensor& dy, int64_t V, double scale, int64_t padding) {
+  ctx->save_for_backward({tokens});
+  ctx->saved_data["scale"] = scale;
+  ctx->saved_data["padding"] = padding;
+  return run_embedding_grad(tokens, dy, V, scale, padding);
+}
+torch::autograd::variable_list EmbeddingGradNode::backward(torch::autograd::AutogradContext* ctx, torch::autograd::variable_list grads) {
+  const Tensor tokens = ctx->get_saved_variables()[0], &table = grads[0];
+  const double scale = ctx->saved_data["scale"].toDouble();
+  const Tensor none = tokens.lt(0).logical_or(tokens.ge(table.size(0))).logical_or(tokens.eq(ctx->saved_data["padding"].toInt()));
+  const Tensor there = tokens.masked_fill(none, 0);
+  const Tensor rows = wants_grad(table) ? EmbeddingNode::apply(there, table, scale, static_cast<int64_t>(-1)) : run_embedding(there, table, scale);
+  return {Tensor(), rows.masked_fill(none.unsqueeze(-1), 0), Tensor(), Tensor(), Tensor()};
+}
+
+// embedding(tokens, weight [V, H], scale, padding | -1) -> weight[tokens] * scale or None
+PyObject* py_embedding(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  if (n != 4 || !plain(a[0]) || !plain(a[1]) || observed()) Py_RETURN_NONE;
+  const Tensor &tokens = THPVariable_Unpack(a[0]), &weight = THPVariable_Unpack(a[1]);
+  const double scale = PyFloat_AsDouble(a[2]);
+  const long padding = PyLong_AsLong(a[3]);
+  if (PyErr_Occurred()) return nullptr;
+  if (!index_bytes(tokens) || weight.dim() != 2 || dtype_code(weight) < 0 || weight.numel() == 0 || weight.size(0) > (1 << 30) ||
+      weight.size(1) > (1 << 25) || tokens.numel() > INT32_MAX || tokens.device() != weight.device() ||
+      weight.get_device() != c10::cuda::current_device() || !std::isfinite(scale) || !std::isfinite(static_cast<float>(scale)) || padding < -1 ||
+      padding >= weight.size(0))
+    Py_RETURN_NONE;
+  Tensor out;
+  {
+    NoGil no_gil;
+    out = wants_grad(weight) ? EmbeddingNode::apply(tokens, weight, scale, static_cast<int64_t>(padding)) : run_embedding(tokens, weight, scale);
+  }
+  return THPVariable_Wrap(out);
+  END_HANDLE_TH_ERRORS
+}
+
 // bind({launcher name: address}, KernelError, Parameter, axb_interface() of the library they are from) -> False if it is another one
 PyObject* py_bind(PyObject*, PyObject* const* a, Py_ssize_t n) {
   HANDLE_TH_ERRORS
@@ -514,6 +729,8 @@ PyMethodDef methods[] = {
     {"cached_attention", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(py_cached_attention)), METH_FASTCALL, nullptr},
     {"reorder_blocks", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(py_reorder_blocks)), METH_FASTCALL, nullptr},
     {"beam_select", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(py_beam_select)), METH_FASTCALL, nullptr},
+    {"token_log_probs", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(py_token_log_probs)), METH_FASTCALL, nullptr},
+    {"embedding", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(py_embedding)), METH_FASTCALL, nullptr},
     {"launches", py_launches, METH_NOARGS, nullptr},
     {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "axonn_host", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};

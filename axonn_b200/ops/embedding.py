@@ -6,7 +6,7 @@ import torch
 import torch.nn.functional as F
 
 from . import _lib
-from .direct import no_graph, plain_tensors
+from .direct import host_paths, no_graph, plain_tensors
 from .kv_cache import _elsewhere
 
 _DT = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
@@ -20,6 +20,10 @@ def embedding(tokens, weight, scale=1.0, padding_idx=None):
     The gradient of ``weight`` has the sums of the rows of equal tokens, 32-bit in the order of the tokens (the same bits on every run),
     scaled and rounded once; ``padding_idx`` gets none.  Gradients of gradients are lookups again.  A token outside the table
     gives a row of NaN and no gradient on a GPU, and is an error on the CPU.  The call never synchronises and can be captured into a CUDA graph."""
+    if weight.is_cuda and (host := host_paths()) is not None:
+        out = host.embedding(tokens, weight, scale, -1 if padding_idx is None else padding_idx if padding_idx >= 0 else -2)
+        if out is not None:
+            return out
     if weight.ndim != 2 or weight.dtype not in _DT:
         raise ValueError(f"weight must be [V, H] in bf16, fp16 or fp32, not {weight.dtype} {list(weight.shape)}")
     if tokens.dtype not in _INDEX:
@@ -32,7 +36,8 @@ def embedding(tokens, weight, scale=1.0, padding_idx=None):
     if padding_idx is not None:
         if not -V <= padding_idx < V:
             raise ValueError(f"padding_idx {padding_idx} is outside the table of {V} rows")
-        padding_idx %= V
+        if padding_idx < 0:
+            return embedding(tokens, weight, scale, padding_idx + V)
     if not plain_tensors(tokens, weight) or weight.numel() == 0 or V > 1 << 30 or weight.shape[1] > 1 << 25 or tokens.numel() >= 1 << 31:
         return _torch(tokens, weight, scale, padding_idx)
     if _elsewhere(weight.device):
@@ -74,6 +79,7 @@ def _table_gradient(tokens, dy, V, scale, padding):
     st = L.axb_embedding_grad(tokens.data_ptr(), _INDEX[tokens.dtype], n, dy.data_ptr(), dy.stride(0), V, H, scale, padding, out.data_ptr(),
                               work.data_ptr(), _DT[dy.dtype], _lib.stream())
     _lib.check(st, "axb_embedding_grad")
+    _lib.add_launches(-1 if n == 0 else 1 if n < 64 else 2)
     return out
 
 

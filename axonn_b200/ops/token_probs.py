@@ -10,7 +10,7 @@ import torch
 import torch.distributed as dist
 
 from . import _lib
-from .direct import first_derivative_only
+from .direct import first_derivative_only, host_paths
 from .kv_cache import _elsewhere
 
 MOST_ALTERNATIVES = 32
@@ -40,6 +40,10 @@ def token_log_probs(logits, tokens=None, entropy=False, top=0, temperature=1.0, 
     left as they are.  With ``group`` the last dimension is this rank's contiguous slice of the vocabulary, of equal size on all ranks (rank
     order = slice order); ``tokens`` and every result count the whole vocabulary, and the gradients of the results are those of all
     ranks, as for ``cross_entropy``.  Neither synchronises: calls without ``group`` can be captured into a CUDA graph."""
+    if group is None and logits.is_cuda and temperature and (host := host_paths()) is not None:
+        out = host.token_log_probs(logits, tokens, entropy, top, 1 / temperature, ignore_index)
+        if out is not None:
+            return TokenLogProbs(*out)
     dev = logits.device
     if _elsewhere(dev):
         with torch.cuda.device(dev):

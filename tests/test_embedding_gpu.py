@@ -54,7 +54,7 @@ def _check(tokens, weight, dy, scale=1.0, padding=None):
         assert torch.equal(ops.embedding(tokens, w, scale, padding), out.detach())
     before = _lib.launch_count
     (grad,) = torch.autograd.grad(out, w, dy)
-    assert _lib.launch_count > before and grad.shape == w.shape and grad.dtype == w.dtype
+    assert (_lib.launch_count > before or tokens.numel() == 0) and grad.shape == w.shape and grad.dtype == w.dtype
     want, size, count = _sums(tokens, dy, V, scale, padding)
     # every addition is off by 2^-24 of the sizes at most, and so is the product with the scale
     tol = HALF_STEP[w.dtype] * want.abs() + SMALLEST[w.dtype] + (1 + HALF_STEP[w.dtype]) * size * 2.0 ** -24 * (count + 1)
