@@ -5,12 +5,27 @@
 //   dz_j = scale ( sum_i g_i [j = t_i] - p_j ( sum_i g_i + h (d_j - log s + H) ) ),  p_j = exp(d_j) / s
 // with g_i the gradients of the log-probabilities of the token and of the alternatives t_i, h that of the entropy H.
 //
-// A block per row, which reads it once for the maximum, once for the sums and once for every alternative.
+// Bound by reading the logits, once forward and once backward (which writes as many).  Forward, a row belongs to a block, or to a cluster
+// where there are few rows: its blocks put their statistics together through distributed shared memory, in one launch and without a
+// workspace.  A thread keeps its own maximum and rescales its sums when 16-byte words of the next tile raise it.
+//
+// Alternatives come in the same pass.  The K-th largest of the threads' maxima over the first tile is reached by at least K of its values,
+// and by few others; what is above it later goes to a list in shared memory, from which the K best are taken in the end (and when it gets
+// long, which raises the bound).  Values that equal the bound count in the first tile only: behind it they come after K that are no
+// smaller.  A tile with more such values than the list has room for, and rows with NaN, are gone through word by word, the list cut down to
+// K after each.
+#include <type_traits>
+
 #include "common.cuh"
 
 namespace axb {
 
-constexpr int TP_THREADS = 256, TP_MOST = 32;
+constexpr int TP_MOST = 32;                // alternatives
+constexpr int TP_WORDS = 4;                // 16-byte words of a thread, of a tile
+constexpr int TP_KEEP = 64;                // entries of a list that are put in order by counting
+constexpr float TP_LOG2E = 1.4426950408889634f;
+constexpr double TP_LN2 = 0.6931471805599453;
+constexpr float TP_FAR = -8192.f;          // exponents below are this: their powers are zero, and their products with them too
 
 struct TokenProbsArgs {
   const void* logits;
@@ -23,6 +38,66 @@ struct TokenProbsArgs {
   long long ignored;
 };
 
+// 32-bit key with the order of the numbers, a NaN above all of them; -0 counts as 0.  Every key is above 0 and below 2^32 - 1.
+__device__ __forceinline__ uint32_t tp_key(float x) {
+  if (x != x) return 0xff800001u;            // +inf has 0xff800000
+  const uint32_t b = __float_as_uint(x + 0.f);
+  return b & 0x80000000u ? ~b : b | 0x80000000u;
+}
+__device__ __forceinline__ float tp_key_value(uint32_t k) { return __uint_as_float(k & 0x80000000u ? k & 0x7fffffffu : ~k); }
+
+__device__ __forceinline__ float tp_exp2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+// Two 32-bit numbers in a register pair.
+struct Two {
+  unsigned long long p;
+  __device__ __forceinline__ Two() {}
+  __device__ __forceinline__ Two(float a, float b) { asm("mov.b64 %0, {%1, %2};" : "=l"(p) : "f"(a), "f"(b)); }
+  __device__ __forceinline__ void get(float& a, float& b) const { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(p)); }
+};
+__device__ __forceinline__ Two operator+(Two a, Two b) { Two d; asm("add.rn.ftz.f32x2 %0, %1, %2;" : "=l"(d.p) : "l"(a.p), "l"(b.p)); return d; }
+__device__ __forceinline__ Two operator*(Two a, Two b) { Two d; asm("mul.rn.ftz.f32x2 %0, %1, %2;" : "=l"(d.p) : "l"(a.p), "l"(b.p)); return d; }
+__device__ __forceinline__ Two fma(Two a, Two b, Two c) {
+  Two d;
+  asm("fma.rn.ftz.f32x2 %0, %1, %2, %3;" : "=l"(d.p) : "l"(a.p), "l"(b.p), "l"(c.p));
+  return d;
+}
+
+// 16 bytes of logits
+template <typename T> struct Word {
+  static constexpr int COUNT = 16 / sizeof(T);
+  uint32_t u[4];
+  __device__ __forceinline__ void pair(int i, float& a, float& b) const {       // values 2 i and 2 i + 1
+    if constexpr (__is_same(T, float)) { a = __uint_as_float(u[2 * i]); b = __uint_as_float(u[2 * i + 1]); }
+    else if constexpr (__is_same(T, __nv_bfloat16)) { a = __uint_as_float(u[i] << 16); b = __uint_as_float(u[i] & 0xffff0000u); }
+    else {
+      const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&u[i]));
+      a = f.x; b = f.y;
+    }
+  }
+  __device__ __forceinline__ void set_pair(int i, float a, float b) {
+    if constexpr (__is_same(T, float)) { u[2 * i] = __float_as_uint(a); u[2 * i + 1] = __float_as_uint(b); }
+    else if constexpr (__is_same(T, __nv_bfloat16)) { const __nv_bfloat162 h = __floats2bfloat162_rn(a, b); u[i] = *reinterpret_cast<const uint32_t*>(&h); }
+    else { const __half2 h = __floats2half2_rn(a, b); u[i] = *reinterpret_cast<const uint32_t*>(&h); }
+  }
+  __device__ __forceinline__ float largest() const {                            // NaN left out
+    if constexpr (__is_same(T, float))
+      return fmaxf(fmaxf(__uint_as_float(u[0]), __uint_as_float(u[1])), fmaxf(__uint_as_float(u[2]), __uint_as_float(u[3])));
+    else {
+      using H = std::conditional_t<__is_same(T, __half), __half2, __nv_bfloat162>;
+      const H* h = reinterpret_cast<const H*>(u);
+      const H m = __hmax2(__hmax2(h[0], h[1]), __hmax2(h[2], h[3]));
+      Word w;
+      w.u[0] = *reinterpret_cast<const uint32_t*>(&m);
+      float a, b;
+      w.pair(0, a, b);
+      return fmaxf(a, b);
+    }
+  }
+};
 template <typename T> __device__ __forceinline__ float tp_value(const T* z, int j) {
   if constexpr (__is_same(T, float)) return z[j];
   else if constexpr (__is_same(T, __half)) return __half2float(z[j]);
@@ -33,132 +108,460 @@ template <typename T> __device__ __forceinline__ T tp_store(float x) {
   else if constexpr (__is_same(T, __half)) return __float2half_rn(x);
   else return __float2bfloat16_rn(x);
 }
-// 32-bit key with the order of the numbers, a NaN above all of them; -0 counts as 0.
-__device__ __forceinline__ uint32_t tp_key(float x) {
-  if (x != x) return 0xff800001u;           // +inf has 0xff800000
-  const uint32_t b = __float_as_uint(x + 0.f);
-  return b & 0x80000000u ? ~b : b | 0x80000000u;
-}
-__device__ __forceinline__ float tp_key_value(uint32_t k) { return __uint_as_float(k & 0x80000000u ? k & 0x7fffffffu : ~k); }
 
-__device__ __forceinline__ unsigned long long tp_block_max(unsigned long long v, unsigned long long* red) {
+// A row of V values as 16-byte words on the 16-byte boundaries of `like` (the row itself, or the row that its gradient is written to):
+// word i holds values [i COUNT - lead, (i + 1) COUNT - lead), of which the first and the last may have some only.  What is not there is -inf.
+template <typename T> struct RowWords {
+  static constexpr int COUNT = Word<T>::COUNT;
+  const T* z;
+  int V, lead, words, shift;                 // shift: bytes from the boundary in front of a word to the word, in the row itself
+  __device__ __forceinline__ RowWords(const T* z_, int V_, const T* like) : z(z_), V(V_) {
+    lead = static_cast<int>(reinterpret_cast<unsigned long long>(like) % 16 / sizeof(T));
+    words = (V + lead + COUNT - 1) / COUNT;
+    shift = static_cast<int>((reinterpret_cast<unsigned long long>(z_) - reinterpret_cast<unsigned long long>(like)) & 15u);
+  }
+  __device__ __forceinline__ bool whole(int i) const { return i * COUNT >= lead && (i + 1) * COUNT - lead <= V; }
+  __device__ __forceinline__ Word<T> operator[](int i) const {
+    const int j = i * COUNT - lead;
+    Word<T> w;
+    if (shift == 0 && whole(i)) {
+      const uint4 u = __ldcs(reinterpret_cast<const uint4*>(z + j));
+      w.u[0] = u.x; w.u[1] = u.y; w.u[2] = u.z; w.u[3] = u.w;
+    } else if (shift != 0 && j >= COUNT && j + 2 * COUNT <= V) {
+      // the words on both sides of the boundary inside, moved together
+      const uint4* p = reinterpret_cast<const uint4*>(reinterpret_cast<const char*>(z + j) - shift);
+      const uint4 a = __ldg(p), b = __ldg(p + 1);
+      uint32_t t[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+      if (shift & 8) {
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) v = max(v, __shfl_xor_sync(0xffffffffu, v, o));
+        for (int k = 0; k < 6; ++k) t[k] = t[k + 2];
+      }
+      if (shift & 4) {
+#pragma unroll
+        for (int k = 0; k < 5; ++k) t[k] = t[k + 1];
+      }
+#pragma unroll
+      for (int k = 0; k < 4; ++k) w.u[k] = __funnelshift_r(t[k], t[k + 1], 8 * (shift & 3));
+    } else {
+#pragma unroll
+      for (int k = 0; k < COUNT; k += 2) {
+        const float a = j + k >= 0 && j + k < V ? tp_value(z, j + k) : -INFINITY, b = j + k + 1 >= 0 && j + k + 1 < V ? tp_value(z, j + k + 1) : -INFINITY;
+        w.set_pair(k / 2, a, b);
+      }
+    }
+    return w;
+  }
+};
+template <typename T> __device__ __forceinline__ Word<T> tp_nothing() {
+  Word<T> w;
+  for (int k = 0; k < 4; ++k) w.u[k] = __is_same(T, float) ? 0xff800000u : __is_same(T, __half) ? 0xfc00fc00u : 0xff80ff80u;
+  return w;
+}
+
+// Sums with the reference m: s of exp2((z - m) c), w of that times its exponent.  m = -inf: nothing so far.
+struct Stats {
+  float m, s, w;
+  __device__ __forceinline__ void rescale(float to, float c) {          // to >= m
+    if (to == m) return;
+    const float x = fmaxf((m - to) * c, TP_FAR), f = tp_exp2(x);
+    w = f * (w + s * x);
+    s *= f;
+    m = to;
+  }
+  __device__ __forceinline__ void join(Stats o, float c) {
+    const float to = fmaxf(m, o.m);
+    rescale(to, c);
+    o.rescale(to, c);
+    s += o.s; w += o.w;
+  }
+};
+
+using Entry = unsigned long long;            // key << 32 | 2^32 - 1 - place: the largest comes first
+__device__ __forceinline__ Entry tp_entry(uint32_t key, int place) { return static_cast<Entry>(key) << 32 | (0xffffffffu - static_cast<uint32_t>(place)); }
+__device__ __forceinline__ int tp_place(Entry e) { return static_cast<int>(0xffffffffu - static_cast<uint32_t>(e)); }
+
+constexpr Entry TP_NONE = 0;                 // below all others
+
+// Shared memory of a block's list.
+template <int THREADS> struct List {
+  static constexpr int ROOM = THREADS * 8 + TP_KEEP, LONG = 2 * TP_KEEP;      // LONG: cut down before the next tile
+  Entry entry[ROOM], some[TP_KEEP], best[TP_MOST];
+  int count, n[3];
+};
+
+// The K largest of the first n entries, n >= K, in their order, to best.  All threads of the block.
+template <int THREADS> __device__ __noinline__ void take_best(List<THREADS>& l, int n, int K) {
+  const int tid = threadIdx.x;
+  if (tid < 3) l.n[tid] = 0;
   __syncthreads();
-  if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = v;
+  Entry least = 0;
+  if (n > TP_KEEP) {
+    // the bits of a bound that at least K reach, until few do; entries differ, so that the last bit leaves K
+    int reach = n;
+    for (int bit = 63, turn = 0; bit >= 0 && reach > TP_KEEP; --bit, turn = turn == 2 ? 0 : turn + 1) {
+      const Entry t = least | 1ull << bit;
+      int mine = 0;
+      for (int i = tid; i < n; i += THREADS) mine += l.entry[i] >= t;
+      mine = __reduce_add_sync(0xffffffffu, mine);
+      if ((tid & 31) == 0 && mine) atomicAdd(&l.n[turn], mine);
+      __syncthreads();
+      const int all = l.n[turn];
+      if (tid == 0) l.n[turn == 0 ? 2 : turn - 1] = 0;       // all have read that one
+      if (all >= K) { least = t; reach = all; }
+    }
+    __syncthreads();
+    if (tid == 0) l.n[0] = 0;
+    __syncthreads();
+  }
+  for (int i = tid; i < n; i += THREADS) {
+    const Entry e = l.entry[i];
+    if (e >= least) l.some[atomicAdd(&l.n[0], 1)] = e;
+  }
   __syncthreads();
-  for (int i = 0; i < TP_THREADS / 32; ++i) v = max(v, red[i]);
+  const int some = l.n[0];
+  if (tid < some) {
+    const Entry e = l.some[tid];
+    int rank = 0;
+    for (int k = 0; k < some; ++k) rank += l.some[k] > e;
+    if (rank < K) l.best[rank] = e;
+  }
+  __syncthreads();
+}
+// ... which the list then consists of.  Returns the key of the last.
+template <int THREADS> __device__ __forceinline__ uint32_t keep_best(List<THREADS>& l, int n, int K) {
+  take_best(l, n, K);
+  if (threadIdx.x < K) l.entry[threadIdx.x] = l.best[threadIdx.x];
+  if (threadIdx.x == 0) l.count = K;
+  __syncthreads();
+  return static_cast<uint32_t>(l.best[K - 1] >> 32);
+}
+
+// The values of words [from, to) whose keys are above `over`, word by word of every thread.
+template <typename T, int THREADS> __device__ __noinline__ uint32_t gather_slowly(List<THREADS>& l, const RowWords<T>& row, int from, int to, uint32_t over, int K) {
+  const int had = l.count;
+  __syncthreads();                           // all have read it
+  if (had > TP_KEEP) over = max(over, keep_best(l, had, K));
+  for (int base = from; base < to; base += THREADS) {
+    const int i = base + threadIdx.x, j0 = i * Word<T>::COUNT - row.lead;
+    if (i < to) {
+      for (int k = 0; k < Word<T>::COUNT; ++k) {
+        const int j = j0 + k;
+        if (j < 0 || j >= row.V) continue;
+        const uint32_t key = tp_key(tp_value(row.z, j));
+        if (key > over) l.entry[atomicAdd(&l.count, 1)] = tp_entry(key, j);
+      }
+    }
+    __syncthreads();
+    const int n = l.count;
+    __syncthreads();
+    if (n > TP_KEEP) over = max(over, keep_best(l, n, K));
+  }
+  return over;
+}
+
+__device__ __forceinline__ uint32_t tp_ctas() {
+  uint32_t r;
+  asm volatile("mov.u32 %0, %%cluster_nctarank;" : "=r"(r));
+  return r;
+}
+__device__ __forceinline__ uint32_t tp_of_cta(const void* p, uint32_t cta) {
+  uint32_t a;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(smem_u32(p)), "r"(cta));
+  return a;
+}
+__device__ __forceinline__ float tp_read_float(uint32_t a) {
+  float v;
+  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(a) : "memory");
   return v;
 }
-__device__ __forceinline__ float tp_block_sum(float v, float* red) {
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-  __syncthreads();
-  if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = v;
-  __syncthreads();
-  v = 0.f;
-  for (int i = 0; i < TP_THREADS / 32; ++i) v += red[i];
+__device__ __forceinline__ Entry tp_read_entry(uint32_t a) {
+  Entry v;
+  asm volatile("ld.shared::cluster.u64 %0, [%1];" : "=l"(v) : "r"(a) : "memory");
   return v;
 }
+template <int LANES> __device__ __forceinline__ Stats tp_join_lanes(Stats t, float c) {
+#pragma unroll
+  for (int o = LANES / 2; o > 0; o >>= 1)
+    t.join({__shfl_xor_sync(0xffffffffu, t.m, o), __shfl_xor_sync(0xffffffffu, t.s, o), __shfl_xor_sync(0xffffffffu, t.w, o)}, c);
+  return t;
+}
 
-template <typename T>
-__global__ void __launch_bounds__(TP_THREADS)
+template <typename T, bool ENTROPY, bool TOP, int THREADS>
+__global__ void __launch_bounds__(THREADS)
 token_probs_kernel(const TokenProbsArgs a, float* log_probs, float* entropy, float* top_log_probs, long long* top_tokens, float4* stats) {
-  __shared__ unsigned long long red[TP_THREADS / 32];
-  __shared__ float redf[TP_THREADS / 32];
-  const int row = blockIdx.x, b = row / a.per_batch, r = row - b * a.per_batch;
+  constexpr int COUNT = Word<T>::COUNT, TILE = THREADS * TP_WORDS, WARPS = THREADS / 32;
+  __shared__ Stats s_stats[WARPS], s_all;
+  __shared__ std::conditional_t<TOP, List<THREADS>, int> s_list;
+  pdl_launch_next();
+  pdl_wait();
+  const int tid = threadIdx.x, lane = tid & 31, ctas = static_cast<int>(tp_ctas()), cta = static_cast<int>(cluster_cta_rank()), K = a.top;
+  const int line = blockIdx.x / ctas, b = line / a.per_batch, r = line - b * a.per_batch;
   const T* z = static_cast<const T*>(a.logits) + b * a.batch_stride + r * a.row_stride;
   const long long token = a.tokens ? a.tokens[b * a.token_batch_stride + r * a.token_stride] : 0;
   if (a.tokens && token == a.ignored) {
-    if (threadIdx.x == 0) {
-      if (log_probs) log_probs[row] = 0.f;
-      if (entropy) entropy[row] = 0.f;
-      stats[row] = make_float4(0.f, 1.f, 0.f, 0.f);
+    if (cta != 0) return;
+    if (tid == 0) {
+      if (log_probs) log_probs[line] = 0.f;
+      if (entropy) entropy[line] = 0.f;
+      stats[line] = make_float4(0.f, 1.f, 0.f, 0.f);
     }
-    if (threadIdx.x < a.top) {
-      top_log_probs[static_cast<long long>(row) * a.top + threadIdx.x] = 0.f;
-      top_tokens[static_cast<long long>(row) * a.top + threadIdx.x] = -1;
+    if (TOP && tid < K) {
+      top_log_probs[static_cast<long long>(line) * K + tid] = 0.f;
+      top_tokens[static_cast<long long>(line) * K + tid] = -1;
     }
     return;
   }
-  // key of the largest number, NaN left out
-  unsigned long long most = 0ull;
-  for (int j = threadIdx.x; j < a.V; j += TP_THREADS) {
-    const float x = tp_value(z, j);
-    if (x == x) most = max(most, static_cast<unsigned long long>(tp_key(x)));
+  const long long t = token - a.start;
+  float zt = 0.f;
+  if (tid == 0 && a.tokens) zt = token < 0 || token >= a.total ? __int_as_float(0x7fffffff) : t >= 0 && t < a.V ? tp_value(z, static_cast<int>(t)) : 0.f;
+  if constexpr (TOP) {
+    if (tid == 0) s_list.count = 0;
+    __syncthreads();
   }
-  most = tp_block_max(most, red);
-  const float m = most ? tp_key_value(static_cast<uint32_t>(most)) : -INFINITY, ref = m == -INFINITY ? 0.f : m;
-  float s = 0.f, w = 0.f;
-  for (int j = threadIdx.x; j < a.V; j += TP_THREADS) {
-    const float d = (tp_value(z, j) - ref) * a.scale, e = __expf(d);
-    s += e;
-    if (e > 0.f) w += e * d;
+  const RowWords<T> row(z, a.V, z);
+  const int share = (row.words + ctas - 1) / ctas, from = min(cta * share, row.words), to = min(from + share, row.words);
+  const float c = a.scale * TP_LOG2E;
+  Word<T> next[TP_WORDS];
+  const auto fetch = [&](int i) {
+#pragma unroll
+    for (int k = 0; k < TP_WORDS; ++k) {
+      if (i + k * THREADS < to) next[k] = row[i + k * THREADS];
+      else next[k] = tp_nothing<T>();
+    }
+  };
+  Stats st = {-INFINITY, 0.f, 0.f};
+  uint32_t over = 0u;                        // a bound that K values reach which come before the next tile
+  fetch(from + tid);
+  for (int base = from; base < to; base += TILE) {
+    Word<T> now[TP_WORDS];
+    float most[TP_WORDS];
+#pragma unroll
+    for (int k = 0; k < TP_WORDS; ++k) now[k] = next[k];
+    if (base + TILE < to) fetch(base + TILE + tid);
+#pragma unroll
+    for (int k = 0; k < TP_WORDS; ++k) most[k] = now[k].largest();
+    const float top = fmaxf(fmaxf(most[0], most[1]), fmaxf(most[2], most[3]));
+    st.rescale(fmaxf(st.m, top), c);
+    const float ref = st.m == -INFINITY ? 0.f : st.m;
+    const Two minus(-ref, -ref), by(c, c);
+    Two s2(0.f, 0.f), w2(0.f, 0.f);
+#pragma unroll
+    for (int k = 0; k < TP_WORDS; ++k) {
+#pragma unroll
+      for (int i = 0; i < COUNT / 2; ++i) {
+        float u, v;
+        now[k].pair(i, u, v);
+        ((Two(u, v) + minus) * by).get(u, v);
+        const Two e(tp_exp2(u), tp_exp2(v));
+        s2 = s2 + e;
+        if constexpr (ENTROPY) w2 = fma(e, Two(fmaxf(u, TP_FAR), fmaxf(v, TP_FAR)), w2);
+      }
+    }
+    float u, v;
+    s2.get(u, v);
+    st.s += u + v;
+    if constexpr (ENTROPY) {
+      w2.get(u, v);
+      st.w += u + v;
+    }
+    if constexpr (TOP) {
+      const bool first = base == from;
+      if (first) {
+        // 16 bits of the K-th largest of the threads' maxima (of a tile that is not full, of fewer: there is no other then)
+        const uint32_t key = tp_key(top) >> 16;
+        uint32_t least = 0u;
+        for (int bit = 15; bit >= 0; --bit) {
+          const uint32_t with = least | 1u << bit;
+          const int reach = __syncthreads_count(key >= with);
+          if (reach >= K) least = with;
+          if (reach == K) break;
+        }
+        over = least << 16;
+      }
+      const int before = s_list.count;
+      const float bound = over <= 0x007fffffu ? -INFINITY : tp_key_value(over);
+      __syncthreads();                       // all have read the count
+      if (first ? top >= bound : top > bound) {
+#pragma unroll
+        for (int k = 0; k < TP_WORDS; ++k) {
+          if (!(first ? most[k] >= bound : most[k] > bound)) continue;
+          const int j0 = (base + tid + k * THREADS) * COUNT - row.lead;
+#pragma unroll
+          for (int i = 0; i < COUNT; i += 2) {
+            float x[2];
+            now[k].pair(i / 2, x[0], x[1]);
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              const int j = j0 + i + h;
+              if ((first ? x[h] >= bound : x[h] > bound) && j >= 0 && j < a.V) {
+                const int n = atomicAdd(&s_list.count, 1);
+                if (n < List<THREADS>::ROOM) s_list.entry[n] = tp_entry(tp_key(x[h]), j);
+              }
+            }
+          }
+        }
+      }
+      __syncthreads();
+      const int n = s_list.count;
+      if (n > List<THREADS>::ROOM) {
+        __syncthreads();
+        if (tid == 0) s_list.count = before;
+        __syncthreads();
+        over = gather_slowly<T, THREADS>(s_list, row, base, min(base + TILE, to), first ? 0u : over, K);
+      } else if (n > K + K / 2 + 8 && (n > List<THREADS>::LONG || base + TILE < to)) {
+        over = max(over, keep_best(s_list, n, K));
+      }
+    }
   }
-  s = tp_block_sum(s, redf);
-  w = tp_block_sum(w, redf);
-  const double log_s = log(static_cast<double>(s));
-  const float H = static_cast<float>(log_s - static_cast<double>(w) / s);
-  if (threadIdx.x == 0) {
-    const long long t = token - a.start;
-    float zt = a.tokens && t >= 0 && t < a.V ? tp_value(z, static_cast<int>(t)) : 0.f;
-    if (a.tokens && (token < 0 || token >= a.total)) zt = __int_as_float(0x7fffffff);
+  st = tp_join_lanes<32>(st, c);
+  if (lane == 0) s_stats[tid >> 5] = st;
+  __syncthreads();
+  if (tid < 32) {
+    st = lane < WARPS ? s_stats[lane] : Stats{-INFINITY, 0.f, 0.f};
+    st = tp_join_lanes<WARPS>(st, c);
+    if (lane == 0) s_all = st;
+  }
+  __syncthreads();
+  if constexpr (TOP) {
+    if (s_all.s != s_all.s) {                // NaN among them: the bounds were not those of the keys
+      if (tid == 0) s_list.count = 0;
+      __syncthreads();
+      gather_slowly<T, THREADS>(s_list, row, from, to, 0u, K);
+    }
+    const int n = s_list.count;
+    if (tid < TP_MOST) s_list.best[tid] = TP_NONE;
+    __syncthreads();
+    if (n > 0) take_best(s_list, n, min(n, K));
+  }
+  if (ctas > 1) {
+    __syncwarp();
+    cluster_sync_all();
+    if (cta == 0) {
+      if (tid < 32) {
+        st = {-INFINITY, 0.f, 0.f};
+        if (lane < ctas) {
+          const uint32_t p = tp_of_cta(&s_all, lane);
+          st = {tp_read_float(p), tp_read_float(p + 4), tp_read_float(p + 8)};
+        }
+        st = tp_join_lanes<8>(st, c);        // 8 CTAs at most
+      }
+      if constexpr (TOP) {
+        for (int i = tid; i < ctas * K; i += THREADS) s_list.entry[i] = tp_read_entry(tp_of_cta(&s_list.best[i % K], i / K));
+      }
+    }
+    __syncwarp();
+    cluster_sync_all();
+    if (cta != 0) return;
+    if constexpr (TOP) take_best(s_list, ctas * K, K);
+    if (tid == 0) s_all = st;
+    __syncthreads();
+  }
+  st = s_all;
+  const double log_s = log(static_cast<double>(st.s));
+  const float w = static_cast<float>(st.w * TP_LN2);
+  if (tid == 0) {
+    const float H = ENTROPY ? static_cast<float>(log_s - st.w * TP_LN2 / st.s) : 0.f;
     if (a.whole) {
-      if (log_probs) log_probs[row] = static_cast<float>((static_cast<double>(zt) - m) * a.scale - log_s);
-      if (entropy) entropy[row] = H;
+      if (log_probs) log_probs[line] = static_cast<float>((static_cast<double>(zt) - st.m) * a.scale - log_s);
+      if (entropy) entropy[line] = H;
     }
-    stats[row] = make_float4(m, s, a.whole ? H : w, zt);
+    stats[line] = make_float4(st.m, st.s, a.whole ? H : w, zt);
   }
-  unsigned long long before = ~0ull;
-  for (int i = 0; i < a.top; ++i) {
-    unsigned long long best = 0ull;
-    for (int j = threadIdx.x; j < a.V; j += TP_THREADS) {
-      const unsigned long long k = static_cast<unsigned long long>(tp_key(tp_value(z, j))) << 32 | (0xffffffffu - j);
-      if (k < before) best = max(best, k);
-    }
-    before = tp_block_max(best, red);
-    if (threadIdx.x == 0) {
-      const int j = static_cast<int>(0xffffffffu - static_cast<uint32_t>(before));
-      const float x = tp_value(z, j);
-      top_log_probs[static_cast<long long>(row) * a.top + i] = a.whole ? static_cast<float>((static_cast<double>(x) - m) * a.scale - log_s) : x;
-      top_tokens[static_cast<long long>(row) * a.top + i] = a.start + j;
+  if constexpr (TOP) {
+    if (tid < K) {
+      const Entry e = s_list.best[tid];
+      const float x = tp_key_value(static_cast<uint32_t>(e >> 32));
+      const long long i = static_cast<long long>(line) * K + tid;
+      top_log_probs[i] = a.whole ? static_cast<float>((static_cast<double>(x) - st.m) * a.scale - log_s) : x;
+      top_tokens[i] = a.start + tp_place(e);
     }
   }
 }
 
-// out [rows, V] dense; stats (m, s, H) of the whole vocabulary; null gradients are zeros
-template <typename T>
-__global__ void __launch_bounds__(TP_THREADS)
+// out [rows, V] dense; stats (m, s, H) of the whole vocabulary; null gradients are zeros.  A block has `span` words of a row.
+constexpr int TP_BWD_THREADS = 256;
+template <typename T, bool ENTROPY>
+__global__ void __launch_bounds__(TP_BWD_THREADS)
 token_probs_bwd_kernel(const TokenProbsArgs a, const float4* stats, const float* d_log_probs, const float* d_entropy, const float* d_top,
-                       const long long* top_tokens, T* out) {
+                       const long long* top_tokens, T* out, int spans, int span) {
+  constexpr int COUNT = Word<T>::COUNT, TILE = TP_BWD_THREADS * TP_WORDS;
   __shared__ float s_g[TP_MOST + 1];
   __shared__ long long s_t[TP_MOST + 1];
-  const int row = blockIdx.x, b = row / a.per_batch, r = row - b * a.per_batch;
+  pdl_launch_next();
+  pdl_wait();
+  const int tid = threadIdx.x, line = blockIdx.x / spans, part = blockIdx.x - line * spans, b = line / a.per_batch, r = line - b * a.per_batch;
   const T* z = static_cast<const T*>(a.logits) + b * a.batch_stride + r * a.row_stride;
-  T* dz = out + static_cast<long long>(row) * a.V;
+  T* dz = out + static_cast<long long>(line) * a.V;
+  const RowWords<T> row(z, a.V, dz);
+  const int from = part * span, to = min(from + span, row.words);
+  const auto put = [&](int i, const Word<T>& w) {
+    const int j = i * COUNT - row.lead;
+    if (row.whole(i)) __stcs(reinterpret_cast<uint4*>(dz + j), make_uint4(w.u[0], w.u[1], w.u[2], w.u[3]));
+    else {
+#pragma unroll
+      for (int k = 0; k < COUNT; k += 2) {
+        float x, y;
+        w.pair(k / 2, x, y);
+        if (j + k >= 0 && j + k < a.V) dz[j + k] = tp_store<T>(x);
+        if (j + k + 1 >= 0 && j + k + 1 < a.V) dz[j + k + 1] = tp_store<T>(y);
+      }
+    }
+  };
   const long long token = a.tokens ? a.tokens[b * a.token_batch_stride + r * a.token_stride] : 0;
   if (a.tokens && token == a.ignored) {
-    for (int j = threadIdx.x; j < a.V; j += TP_THREADS) dz[j] = tp_store<T>(0.f);
+    Word<T> zero;
+    zero.u[0] = zero.u[1] = zero.u[2] = zero.u[3] = 0u;
+    for (int i = from + tid; i < to; i += TP_BWD_THREADS) put(i, zero);
     return;
   }
   const int n = 1 + (d_top ? a.top : 0);
-  if (threadIdx.x < n) {
-    const long long i = static_cast<long long>(row) * a.top + threadIdx.x - 1;
-    float g = threadIdx.x ? d_top[i] : d_log_probs ? d_log_probs[row] : 0.f;
-    if (threadIdx.x == 0 && d_log_probs && (token < 0 || token >= a.total)) g = __int_as_float(0x7fffffff);
-    s_g[threadIdx.x] = g;
-    s_t[threadIdx.x] = threadIdx.x ? top_tokens[i] - a.start : a.tokens ? token - a.start : -1;
+  if (tid < n) {
+    const long long i = static_cast<long long>(line) * a.top + tid - 1;
+    float g = tid ? d_top[i] : d_log_probs ? d_log_probs[line] : 0.f;
+    if (tid == 0 && d_log_probs && (token < 0 || token >= a.total)) g = __int_as_float(0x7fffffff);
+    s_g[tid] = g;
+    s_t[tid] = tid ? top_tokens[i] - a.start : a.tokens ? token - a.start : -1;
   }
   __syncthreads();
-  const float4 st = stats[row];
-  const float log_s = static_cast<float>(log(static_cast<double>(st.y))), h = d_entropy ? d_entropy[row] : 0.f;
+  const float4 st = stats[line];
+  const float log_s = static_cast<float>(log(static_cast<double>(st.y))), h = ENTROPY ? d_entropy[line] : 0.f, c = a.scale * TP_LOG2E;
   float all = 0.f;
   for (int i = 0; i < n; ++i) all += s_g[i];
-  for (int j = threadIdx.x; j < a.V; j += TP_THREADS) {
-    const float d = (tp_value(z, j) - st.x) * a.scale, p = __expf(d) / st.y;
-    float g = -p * (all + (p > 0.f ? h * (d - log_s + st.z) : 0.f));
-    for (int i = 0; i < n; ++i) if (s_t[i] == j) g += s_g[i];
-    dz[j] = tp_store<T>(g * a.scale);
+  // exp2(x) (A + B x), x = (z - m) c
+  const float by_s = -a.scale / st.y, A = by_s * (all + h * (st.z - log_s)), B = by_s * h * static_cast<float>(TP_LN2);
+  const Two minus(-st.x, -st.x), by(c, c), A2(A, A), B2(B, B);
+  for (int base = from; base < to; base += TILE) {
+    Word<T> now[TP_WORDS];
+#pragma unroll
+    for (int k = 0; k < TP_WORDS; ++k)
+      if (base + tid + k * TP_BWD_THREADS < to) now[k] = row[base + tid + k * TP_BWD_THREADS];
+#pragma unroll
+    for (int k = 0; k < TP_WORDS; ++k) {
+      if (base + tid + k * TP_BWD_THREADS >= to) break;
+#pragma unroll
+      for (int i = 0; i < COUNT / 2; ++i) {
+        float u, v;
+        now[k].pair(i, u, v);
+        ((Two(u, v) + minus) * by).get(u, v);
+        Two e(tp_exp2(u), tp_exp2(v));
+        if constexpr (ENTROPY) e = e * fma(B2, Two(fmaxf(u, TP_FAR), fmaxf(v, TP_FAR)), A2);
+        else e = e * A2;
+        e.get(u, v);
+        now[k].set_pair(i, u, v);
+      }
+      put(base + tid + k * TP_BWD_THREADS, now[k]);
+    }
+  }
+  // the tokens that have a gradient of their own, of this block's words
+  __syncthreads();
+  if (tid < n && s_t[tid] >= 0 && s_t[tid] < a.V) {
+    const int j = static_cast<int>(s_t[tid]), i = (j + row.lead) / COUNT;
+    if (i >= from && i < to) {
+      const float x = (tp_value(z, j) - st.x) * c;
+      float g = 0.f;
+      for (int k = 0; k < n; ++k) if (s_t[k] == j) g += s_g[k];
+      dz[j] = tp_store<T>(tp_exp2(x) * (A + (ENTROPY ? B * fmaxf(x, TP_FAR) : 0.f)) + g * a.scale);
+    }
   }
 }
 
@@ -174,6 +577,48 @@ static int fill(TokenProbsArgs& a, const char* what, const void* logits, long lo
   return 0;
 }
 
+template <typename T, bool ENTROPY, bool TOP, int THREADS>
+static int tell(const TokenProbsArgs& a, long long rows, float* log_probs, float* entropy, float* top_log_probs, long long* top_tokens, float4* stats,
+                cudaStream_t s) {
+  // blocks of a row: as many as there is room for with four on every SM, each with a word at least for all of its threads
+  const long long words = (a.V + Word<T>::COUNT - 1) / Word<T>::COUNT, room = 4ll * sm_count_current();
+  unsigned ctas = 1;
+  while (ctas < 8 && rows * ctas * 2 <= room && words / (2 * ctas) >= THREADS) ctas *= 2;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(static_cast<unsigned>(rows) * ctas); cfg.blockDim = dim3(THREADS); cfg.stream = s;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = ctas; attr[0].val.clusterDim.y = 1; attr[0].val.clusterDim.z = 1;
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[1].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr; cfg.numAttrs = max_ctas() == 0 ? 2 : 1;
+  AXB_CUDA(cudaLaunchKernelEx(&cfg, token_probs_kernel<T, ENTROPY, TOP, THREADS>, a, log_probs, entropy, top_log_probs, top_tokens, stats));
+  return 0;
+}
+
+template <typename T>
+static int tell_of(const TokenProbsArgs& a, long long rows, float* log_probs, float* entropy, float* top_log_probs, long long* top_tokens,
+                   float4* stats, cudaStream_t s) {
+  const bool H = entropy || !a.whole, narrow = static_cast<long long>(a.V) * sizeof(T) <= 16384;
+  const auto go = narrow ? (H ? (a.top ? tell<T, true, true, 64> : tell<T, true, false, 64>) : (a.top ? tell<T, false, true, 64> : tell<T, false, false, 64>))
+                         : (H ? (a.top ? tell<T, true, true, 256> : tell<T, true, false, 256>) : (a.top ? tell<T, false, true, 256> : tell<T, false, false, 256>));
+  return go(a, rows, log_probs, entropy, top_log_probs, top_tokens, stats, s);
+}
+
+template <typename T>
+static int untell(const TokenProbsArgs& a, long long rows, const float4* stats, const float* d_log_probs, const float* d_entropy, const float* d_top,
+                  const long long* top_tokens, void* out, cudaStream_t s) {
+  const long long words = a.V / Word<T>::COUNT + 2, tile = TP_BWD_THREADS * TP_WORDS, tiles = (words + tile - 1) / tile;
+  long long spans = 16ll * sm_count_current() / rows;
+  spans = spans < 1 ? 1 : spans > tiles ? tiles : spans;
+  const long long span = (tiles + spans - 1) / spans * tile;
+  spans = (words + span - 1) / span;
+  AXB_CUDA(pdl_launch(d_entropy ? token_probs_bwd_kernel<T, true> : token_probs_bwd_kernel<T, false>, dim3(static_cast<unsigned>(rows * spans)),
+                      dim3(TP_BWD_THREADS), 0, s, a, stats, d_log_probs, d_entropy, d_top, top_tokens, static_cast<T*>(out), static_cast<int>(spans),
+                      static_cast<int>(span)));
+  return 0;
+}
+
 }  // namespace axb
 
 using namespace axb;
@@ -185,12 +630,9 @@ extern "C" int axb_token_log_probs(const void* logits, long long batch_stride, l
   TokenProbsArgs a;
   if (fill(a, "token log-probabilities", logits, batch_stride, row_stride, tokens, token_batch_stride, token_stride, batches, per_batch, V,
            start, total, top, scale, ignored, whole, dtype)) return -1;
-  const int rows = batches * per_batch;
-  auto kernel = dtype == 0 ? token_probs_kernel<__nv_bfloat16> : dtype == 1 ? token_probs_kernel<__half> : token_probs_kernel<float>;
-  kernel<<<rows, TP_THREADS, 0, static_cast<cudaStream_t>(stream)>>>(a, log_probs, entropy, top_log_probs, top_tokens,
-                                                                   reinterpret_cast<float4*>(stats));
-  AXB_CUDA(cudaGetLastError());
-  return 0;
+  const auto go = dtype == 0 ? tell_of<__nv_bfloat16> : dtype == 1 ? tell_of<__half> : tell_of<float>;
+  return go(a, static_cast<long long>(batches) * per_batch, log_probs, entropy, top_log_probs, top_tokens, reinterpret_cast<float4*>(stats),
+            static_cast<cudaStream_t>(stream));
 }
 
 extern "C" int axb_token_log_probs_bwd(const void* logits, long long batch_stride, long long row_stride, const long long* tokens,
@@ -201,12 +643,7 @@ extern "C" int axb_token_log_probs_bwd(const void* logits, long long batch_strid
   TokenProbsArgs a;
   if (fill(a, "gradient of token log-probabilities", logits, batch_stride, row_stride, tokens, token_batch_stride, token_stride, batches,
            per_batch, V, start, total, top, scale, ignored, 1, dtype)) return -1;
-  const int rows = batches * per_batch;
-  const cudaStream_t s = static_cast<cudaStream_t>(stream);
-  const float4* st = reinterpret_cast<const float4*>(stats);
-  if (dtype == 0) token_probs_bwd_kernel<<<rows, TP_THREADS, 0, s>>>(a, st, d_log_probs, d_entropy, d_top, top_tokens, static_cast<__nv_bfloat16*>(out));
-  else if (dtype == 1) token_probs_bwd_kernel<<<rows, TP_THREADS, 0, s>>>(a, st, d_log_probs, d_entropy, d_top, top_tokens, static_cast<__half*>(out));
-  else token_probs_bwd_kernel<<<rows, TP_THREADS, 0, s>>>(a, st, d_log_probs, d_entropy, d_top, top_tokens, static_cast<float*>(out));
-  AXB_CUDA(cudaGetLastError());
-  return 0;
+  const auto go = dtype == 0 ? untell<__nv_bfloat16> : dtype == 1 ? untell<__half> : untell<float>;
+  return go(a, static_cast<long long>(batches) * per_batch, reinterpret_cast<const float4*>(stats), d_log_probs, d_entropy, d_top, top_tokens, out,
+            static_cast<cudaStream_t>(stream));
 }
