@@ -9,11 +9,11 @@
 // where there are few rows: its blocks put their statistics together through distributed shared memory, in one launch and without a
 // workspace.  A thread keeps its own maximum and rescales its sums when 16-byte words of the next tile raise it.
 //
-// Alternatives come in the same pass.  The K-th largest of the threads' maxima over the first tile is reached by at least K of its values,
-// and by few others; what is above it later goes to a list in shared memory, from which the K best are taken in the end (and when it gets
-// long, which raises the bound).  Values that equal the bound count in the first tile only: behind it they come after K that are no
-// smaller.  A tile with more such values than the list has room for, and rows with NaN, are gone through word by word, the list cut down to
-// K after each.
+// Alternatives come in the same pass.  The K-th largest of the threads' maxima so far (of 32 of them, the largest of every warp's) is
+// reached by K of the values, and by few others: what is above it goes to a list in shared memory.  The bound is taken anew whenever the
+// values behind it have doubled.  Values that equal it count in the first tile only: later ones come after K that are no
+// smaller.  In the end what is below the last bound is dropped and the rest put in order by counting.  A list that is too short for that
+// (rows of mostly equal values, growing ones) or has missed a NaN is made again word by word, cut down to K after each.
 #include <type_traits>
 
 #include "common.cuh"
@@ -22,9 +22,10 @@ namespace axb {
 
 constexpr int TP_MOST = 32;                // alternatives
 constexpr int TP_WORDS = 4;                // 16-byte words of a thread, of a tile
-constexpr int TP_KEEP = 64;                // entries of a list that are put in order by counting
+constexpr int TP_KEEP = 64;                // entries that a list is cut down to, at most
 constexpr float TP_LOG2E = 1.4426950408889634f;
 constexpr double TP_LN2 = 0.6931471805599453;
+constexpr long long TP_NARROW = 8192, TP_MIDDLE = 65536;      // bytes of a row for blocks of 32 and 128 threads
 constexpr float TP_FAR = -8192.f;          // exponents below are this: their powers are zero, and their products with them too
 
 struct TokenProbsArgs {
@@ -44,6 +45,7 @@ __device__ __forceinline__ uint32_t tp_key(float x) {
   const uint32_t b = __float_as_uint(x + 0.f);
   return b & 0x80000000u ? ~b : b | 0x80000000u;
 }
+constexpr uint32_t TP_LOWEST = 0x007fffffu;  // of -inf
 __device__ __forceinline__ float tp_key_value(uint32_t k) { return __uint_as_float(k & 0x80000000u ? k & 0x7fffffffu : ~k); }
 
 __device__ __forceinline__ float tp_exp2(float x) {
@@ -77,6 +79,13 @@ template <typename T> struct Word {
       const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&u[i]));
       a = f.x; b = f.y;
     }
+  }
+  __device__ __forceinline__ float one(int i) const {                           // value i
+    const int k = __is_same(T, float) ? i : i / 2;
+    const uint32_t lower = k & 1 ? u[1] : u[0], upper = k & 1 ? u[3] : u[2], x = k & 2 ? upper : lower;
+    if constexpr (__is_same(T, float)) return __uint_as_float(x);
+    else if constexpr (__is_same(T, __nv_bfloat16)) return __uint_as_float(i & 1 ? x & 0xffff0000u : x << 16);
+    else return __half2float(__ushort_as_half(static_cast<unsigned short>(i & 1 ? x >> 16 : x & 0xffffu)));
   }
   __device__ __forceinline__ void set_pair(int i, float a, float b) {
     if constexpr (__is_same(T, float)) { u[2 * i] = __float_as_uint(a); u[2 * i + 1] = __float_as_uint(b); }
@@ -168,12 +177,6 @@ struct Stats {
     s *= f;
     m = to;
   }
-  __device__ __forceinline__ void join(Stats o, float c) {
-    const float to = fmaxf(m, o.m);
-    rescale(to, c);
-    o.rescale(to, c);
-    s += o.s; w += o.w;
-  }
 };
 
 using Entry = unsigned long long;            // key << 32 | 2^32 - 1 - place: the largest comes first
@@ -184,65 +187,111 @@ constexpr Entry TP_NONE = 0;                 // below all others
 
 // Shared memory of a block's list.
 template <int THREADS> struct List {
-  static constexpr int ROOM = THREADS * 8 + TP_KEEP, LONG = 2 * TP_KEEP;      // LONG: cut down before the next tile
-  Entry entry[ROOM], some[TP_KEEP], best[TP_MOST];
+  static constexpr int ROOM = THREADS * 8 + TP_KEEP, SOME = THREADS < TP_KEEP ? TP_KEEP : THREADS;
+  static constexpr int SHARE = THREADS < 64 ? 32 : THREADS / 2;       // of a cluster's list, of a block; eight have room
+  Entry entry[ROOM], some[SOME], best[TP_MOST];
+  uint32_t bound[2][32];
   int count, n[3];
+  static_assert(8 * SHARE <= ROOM && SHARE >= TP_MOST, "a cluster's list");
 };
+
+// Threads of a row wait for one another: a warp alone (blocks of several rows), or the block.
+template <int THREADS> __device__ __forceinline__ void tp_sync() {
+  if constexpr (THREADS == 32) __syncwarp();
+  else __syncthreads();
+}
+
+// The upper 16 bits of a key that at least K of the row's threads reach with theirs: the K-th largest of 32 of these, the largest of every
+// warp's.
+template <int THREADS> __device__ __forceinline__ uint32_t bound_of(List<THREADS>& l, uint32_t key, int K, int turn) {
+  constexpr int EACH = 32 / (THREADS / 32);
+  const int lane = threadIdx.x & 31;
+  if constexpr (THREADS > 32) {
+    uint32_t mine = 0u;
+#pragma unroll
+    for (int i = 0; i < EACH; ++i) {
+      const uint32_t most = __reduce_max_sync(0xffffffffu, key);
+      if (lane == __ffs(__ballot_sync(0xffffffffu, key == most)) - 1) key = 0u;
+      if (lane == i) mine = most;
+    }
+    if (lane < EACH) l.bound[turn][threadIdx.x / 32 * EACH + lane] = mine;
+    __syncthreads();
+    key = l.bound[turn][lane];
+  }
+  uint32_t least = 0u;
+#pragma unroll 1
+  for (uint32_t bit = 0x80000000u; bit >= 0x10000u; bit >>= 1)
+    if (__popc(__ballot_sync(0xffffffffu, key >= (least | bit))) >= K) least |= bit;
+  return least;
+}
+
+// The K largest of some[0, n), n <= SOME, in their order, to best: what an entry's place is, its threads count.
+template <int THREADS> __device__ __forceinline__ void put_in_order(List<THREADS>& l, int n, int K) {
+  const int tid = threadIdx.x % THREADS;
+  int each = 1;                              // threads of an entry
+  while (each < 32 && 2 * each * n <= THREADS) each *= 2;
+  const int part = tid & (each - 1);
+  for (int base = 0; base < n; base += THREADS / each) {
+    const int i = base + tid / each;
+    const Entry e = i < n ? l.some[i] : TP_NONE;
+    int rank = 0;
+    for (int k = part; k < n; k += each) rank += l.some[k] > e;
+    for (int o = each / 2; o > 0; o >>= 1) rank += __shfl_xor_sync(0xffffffffu, rank, o);
+    if (part == 0 && i < n && rank < K) l.best[rank] = e;
+  }
+  tp_sync<THREADS>();
+}
 
 // The K largest of the first n entries, n >= K, in their order, to best.  All threads of the block.
 template <int THREADS> __device__ __noinline__ void take_best(List<THREADS>& l, int n, int K) {
-  const int tid = threadIdx.x;
+  const int tid = threadIdx.x % THREADS;
   if (tid < 3) l.n[tid] = 0;
-  __syncthreads();
+  tp_sync<THREADS>();
   Entry least = 0;
-  if (n > TP_KEEP) {
+  if (n > List<THREADS>::SOME) {
     // the bits of a bound that at least K reach, until few do; entries differ, so that the last bit leaves K
     int reach = n;
-    for (int bit = 63, turn = 0; bit >= 0 && reach > TP_KEEP; --bit, turn = turn == 2 ? 0 : turn + 1) {
+    for (int bit = 63, turn = 0; bit >= 0 && reach > List<THREADS>::SOME; --bit, turn = turn == 2 ? 0 : turn + 1) {
       const Entry t = least | 1ull << bit;
       int mine = 0;
       for (int i = tid; i < n; i += THREADS) mine += l.entry[i] >= t;
       mine = __reduce_add_sync(0xffffffffu, mine);
       if ((tid & 31) == 0 && mine) atomicAdd(&l.n[turn], mine);
-      __syncthreads();
+      tp_sync<THREADS>();
       const int all = l.n[turn];
       if (tid == 0) l.n[turn == 0 ? 2 : turn - 1] = 0;       // all have read that one
       if (all >= K) { least = t; reach = all; }
     }
-    __syncthreads();
+    tp_sync<THREADS>();
     if (tid == 0) l.n[0] = 0;
-    __syncthreads();
+    tp_sync<THREADS>();
   }
   for (int i = tid; i < n; i += THREADS) {
     const Entry e = l.entry[i];
     if (e >= least) l.some[atomicAdd(&l.n[0], 1)] = e;
   }
-  __syncthreads();
-  const int some = l.n[0];
-  if (tid < some) {
-    const Entry e = l.some[tid];
-    int rank = 0;
-    for (int k = 0; k < some; ++k) rank += l.some[k] > e;
-    if (rank < K) l.best[rank] = e;
-  }
-  __syncthreads();
+  tp_sync<THREADS>();
+  put_in_order(l, l.n[0], K);
 }
 // ... which the list then consists of.  Returns the key of the last.
 template <int THREADS> __device__ __forceinline__ uint32_t keep_best(List<THREADS>& l, int n, int K) {
+  const int tid = threadIdx.x % THREADS;
   take_best(l, n, K);
-  if (threadIdx.x < K) l.entry[threadIdx.x] = l.best[threadIdx.x];
-  if (threadIdx.x == 0) l.count = K;
-  __syncthreads();
+  if (tid < K) l.entry[tid] = l.best[tid];
+  if (tid == 0) l.count = K;
+  tp_sync<THREADS>();
   return static_cast<uint32_t>(l.best[K - 1] >> 32);
 }
 
-// The values of words [from, to) whose keys are above `over`, word by word of every thread.
-template <typename T, int THREADS> __device__ __noinline__ uint32_t gather_slowly(List<THREADS>& l, const RowWords<T>& row, int from, int to, uint32_t over, int K) {
-  const int had = l.count;
-  __syncthreads();                           // all have read it
-  if (had > TP_KEEP) over = max(over, keep_best(l, had, K));
+// The list of words [from, to), a word of every thread at a time: what comes later counts where its key is above the K-th so far.
+template <typename T, int THREADS> __device__ __noinline__ void gather_slowly(List<THREADS>& l, const RowWords<T>& row, int from, int to, int K) {
+  const int tid = threadIdx.x % THREADS;
+  uint32_t over = 0u;
+  tp_sync<THREADS>();                        // all have read the count
+  if (tid == 0) l.count = 0;
+  tp_sync<THREADS>();
   for (int base = from; base < to; base += THREADS) {
-    const int i = base + threadIdx.x, j0 = i * Word<T>::COUNT - row.lead;
+    const int i = base + tid, j0 = i * Word<T>::COUNT - row.lead;
     if (i < to) {
       for (int k = 0; k < Word<T>::COUNT; ++k) {
         const int j = j0 + k;
@@ -251,12 +300,11 @@ template <typename T, int THREADS> __device__ __noinline__ uint32_t gather_slowl
         if (key > over) l.entry[atomicAdd(&l.count, 1)] = tp_entry(key, j);
       }
     }
-    __syncthreads();
+    tp_sync<THREADS>();
     const int n = l.count;
-    __syncthreads();
-    if (n > TP_KEEP) over = max(over, keep_best(l, n, K));
+    tp_sync<THREADS>();
+    if (n > TP_KEEP) over = keep_best(l, n, K);
   }
-  return over;
 }
 
 __device__ __forceinline__ uint32_t tp_ctas() {
@@ -274,28 +322,48 @@ __device__ __forceinline__ float tp_read_float(uint32_t a) {
   asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(a) : "memory");
   return v;
 }
+__device__ __forceinline__ uint32_t tp_read_word(uint32_t a) {
+  uint32_t v;
+  asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(a) : "memory");
+  return v;
+}
 __device__ __forceinline__ Entry tp_read_entry(uint32_t a) {
   Entry v;
   asm volatile("ld.shared::cluster.u64 %0, [%1];" : "=l"(v) : "r"(a) : "memory");
   return v;
 }
 template <int LANES> __device__ __forceinline__ Stats tp_join_lanes(Stats t, float c) {
+  float m = t.m;
 #pragma unroll
-  for (int o = LANES / 2; o > 0; o >>= 1)
-    t.join({__shfl_xor_sync(0xffffffffu, t.m, o), __shfl_xor_sync(0xffffffffu, t.s, o), __shfl_xor_sync(0xffffffffu, t.w, o)}, c);
+  for (int o = LANES / 2; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+  t.rescale(m, c);
+#pragma unroll
+  for (int o = LANES / 2; o > 0; o >>= 1) {
+    t.s += __shfl_xor_sync(0xffffffffu, t.s, o);
+    t.w += __shfl_xor_sync(0xffffffffu, t.w, o);
+  }
   return t;
 }
 
+// Threads of a block: four rows of a warp each, or one row.
+template <int THREADS> constexpr int TP_BLOCK = THREADS == 32 ? 128 : THREADS;
+
 template <typename T, bool ENTROPY, bool TOP, int THREADS>
-__global__ void __launch_bounds__(THREADS)
-token_probs_kernel(const TokenProbsArgs a, float* log_probs, float* entropy, float* top_log_probs, long long* top_tokens, float4* stats) {
+__global__ void __launch_bounds__(TP_BLOCK<THREADS>)
+token_probs_kernel(const TokenProbsArgs a, int rows, float* log_probs, float* entropy, float* top_log_probs, long long* top_tokens, float4* stats) {
   constexpr int COUNT = Word<T>::COUNT, TILE = THREADS * TP_WORDS, WARPS = THREADS / 32;
-  __shared__ Stats s_stats[WARPS], s_all;
-  __shared__ std::conditional_t<TOP, List<THREADS>, int> s_list;
+  constexpr int ROWS = TP_BLOCK<THREADS> / THREADS;
+  __shared__ Stats s_stats[WARPS], s_alls[ROWS];
+  __shared__ std::conditional_t<TOP, List<THREADS>, int> s_lists[ROWS];
   pdl_launch_next();
   pdl_wait();
-  const int tid = threadIdx.x, lane = tid & 31, ctas = static_cast<int>(tp_ctas()), cta = static_cast<int>(cluster_cta_rank()), K = a.top;
-  const int line = blockIdx.x / ctas, b = line / a.per_batch, r = line - b * a.per_batch;
+  const int tid = threadIdx.x % THREADS, lane = tid & 31, K = a.top;
+  const int ctas = ROWS > 1 ? 1 : static_cast<int>(tp_ctas()), cta = ROWS > 1 ? 0 : static_cast<int>(cluster_cta_rank());
+  if (ROWS > 1 && blockIdx.x * ROWS + threadIdx.x / THREADS >= static_cast<unsigned>(rows)) return;
+  const int line = ROWS > 1 ? static_cast<int>(blockIdx.x * ROWS + threadIdx.x / THREADS) : blockIdx.x / ctas;
+  const int b = line / a.per_batch, r = line - b * a.per_batch;
+  auto& s_list = s_lists[ROWS > 1 ? threadIdx.x / THREADS : 0];
+  Stats& s_all = s_alls[ROWS > 1 ? threadIdx.x / THREADS : 0];
   const T* z = static_cast<const T*>(a.logits) + b * a.batch_stride + r * a.row_stride;
   const long long token = a.tokens ? a.tokens[b * a.token_batch_stride + r * a.token_stride] : 0;
   if (a.tokens && token == a.ignored) {
@@ -316,28 +384,50 @@ token_probs_kernel(const TokenProbsArgs a, float* log_probs, float* entropy, flo
   if (tid == 0 && a.tokens) zt = token < 0 || token >= a.total ? __int_as_float(0x7fffffff) : t >= 0 && t < a.V ? tp_value(z, static_cast<int>(t)) : 0.f;
   if constexpr (TOP) {
     if (tid == 0) s_list.count = 0;
-    __syncthreads();
+    tp_sync<THREADS>();
   }
   const RowWords<T> row(z, a.V, z);
   const int share = (row.words + ctas - 1) / ctas, from = min(cta * share, row.words), to = min(from + share, row.words);
+  // whole words are [lo, hi); the values in front of and behind them, of the row's first and last word, are taken one by one
+  const int lo = from + (from == 0 && row.lead > 0), hi = to - (to == row.words && to > lo && !row.whole(to - 1));
+  const int head = from == 0 && to > 0 && row.lead > 0 ? min(COUNT - row.lead, a.V) : 0;
+  const int behind = to == row.words && to > 0 ? max(hi * COUNT - row.lead, head) : a.V;
+  const uint4* words = reinterpret_cast<const uint4*>(z - row.lead);
   const float c = a.scale * TP_LOG2E;
+  const Word<T> nothing = tp_nothing<T>();
   Word<T> next[TP_WORDS];
-  const auto fetch = [&](int i) {
+  const auto load = [&](Word<T>& w, int i) {
+    const uint4 u = __ldcs(words + i);
+    w.u[0] = u.x; w.u[1] = u.y; w.u[2] = u.z; w.u[3] = u.w;
+  };
+  const auto fetch = [&](int base) {
+    if (base + TILE <= hi) {
 #pragma unroll
-    for (int k = 0; k < TP_WORDS; ++k) {
-      if (i + k * THREADS < to) next[k] = row[i + k * THREADS];
-      else next[k] = tp_nothing<T>();
+      for (int k = 0; k < TP_WORDS; ++k) load(next[k], base + tid + k * THREADS);
+    } else {
+#pragma unroll
+      for (int k = 0; k < TP_WORDS; ++k) {
+        next[k] = nothing;
+        if (base + tid + k * THREADS < hi) load(next[k], base + tid + k * THREADS);
+      }
     }
   };
-  Stats st = {-INFINITY, 0.f, 0.f};
+  const auto single = [&](float x) {         // statistics of one value: exp(x - x) is 1, or NaN
+    const float y = x == -INFINITY ? 0.f : x;
+    return Stats{fmaxf(x, -INFINITY), tp_exp2(x - y), 0.f};
+  };
+  fetch(lo);
+  const float x_head = tid < head ? tp_value(z, tid) : -INFINITY;
+  Stats st = single(x_head);
   uint32_t over = 0u;                        // a bound that K values reach which come before the next tile
-  fetch(from + tid);
-  for (int base = from; base < to; base += TILE) {
+  int tiles = 0, turn = 0;
+  int base = lo;
+  do {
     Word<T> now[TP_WORDS];
     float most[TP_WORDS];
 #pragma unroll
     for (int k = 0; k < TP_WORDS; ++k) now[k] = next[k];
-    if (base + TILE < to) fetch(base + TILE + tid);
+    if (base + TILE < hi) fetch(base + TILE);
 #pragma unroll
     for (int k = 0; k < TP_WORDS; ++k) most[k] = now[k].largest();
     const float top = fmaxf(fmaxf(most[0], most[1]), fmaxf(most[2], most[3]));
@@ -365,76 +455,95 @@ token_probs_kernel(const TokenProbsArgs a, float* log_probs, float* entropy, flo
       st.w += u + v;
     }
     if constexpr (TOP) {
-      const bool first = base == from;
+      const bool first = base == lo;
       if (first) {
-        // 16 bits of the K-th largest of the threads' maxima (of a tile that is not full, of fewer: there is no other then)
-        const uint32_t key = tp_key(top) >> 16;
-        uint32_t least = 0u;
-        for (int bit = 15; bit >= 0; --bit) {
-          const uint32_t with = least | 1u << bit;
-          const int reach = __syncthreads_count(key >= with);
-          if (reach >= K) least = with;
-          if (reach == K) break;
-        }
-        over = least << 16;
+        over = bound_of(s_list, tp_key(st.m), K, 0);
+        if (tid < head && tp_key(x_head) >= over) s_list.entry[atomicAdd(&s_list.count, 1)] = tp_entry(tp_key(x_head), tid);
       }
-      const int before = s_list.count;
-      const float bound = over <= 0x007fffffu ? -INFINITY : tp_key_value(over);
-      __syncthreads();                       // all have read the count
-      if (first ? top >= bound : top > bound) {
+      const float bound = over <= TP_LOWEST ? -INFINITY : tp_key_value(over);
+      if (__any_sync(0xffffffffu, first ? top >= bound : top > bound)) {
+        // a warp looks at the words with such values one after another, a lane at each of the values
+        const int j0 = (base + tid) * COUNT - row.lead;
 #pragma unroll
         for (int k = 0; k < TP_WORDS; ++k) {
-          if (!(first ? most[k] >= bound : most[k] > bound)) continue;
-          const int j0 = (base + tid + k * THREADS) * COUNT - row.lead;
+          for (unsigned some = __ballot_sync(0xffffffffu, (first ? most[k] >= bound : most[k] > bound) && base + tid + k * THREADS < hi); some;
+               some &= some - 1u) {
+            const int of = __ffs(some) - 1;
+            Word<T> w;
 #pragma unroll
-          for (int i = 0; i < COUNT; i += 2) {
-            float x[2];
-            now[k].pair(i / 2, x[0], x[1]);
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-              const int j = j0 + i + h;
-              if ((first ? x[h] >= bound : x[h] > bound) && j >= 0 && j < a.V) {
-                const int n = atomicAdd(&s_list.count, 1);
-                if (n < List<THREADS>::ROOM) s_list.entry[n] = tp_entry(tp_key(x[h]), j);
-              }
-            }
+            for (int i = 0; i < 4; ++i) w.u[i] = __shfl_sync(0xffffffffu, now[k].u[i], of);
+            const float x = w.one(lane & (COUNT - 1));
+            const unsigned hits = __ballot_sync(0xffffffffu, lane < COUNT && (first ? x >= bound : x > bound));
+            const int j = __shfl_sync(0xffffffffu, j0, of) + k * THREADS * COUNT + lane;
+            int at = 0;
+            if (lane == 0) at = atomicAdd(&s_list.count, __popc(hits));
+            at = __shfl_sync(0xffffffffu, at, 0) + __popc(hits & ((1u << lane) - 1u));
+            if ((hits >> lane & 1u) && at < List<THREADS>::ROOM) s_list.entry[at] = tp_entry(tp_key(x), j);
           }
         }
       }
-      __syncthreads();
-      const int n = s_list.count;
-      if (n > List<THREADS>::ROOM) {
-        __syncthreads();
-        if (tid == 0) s_list.count = before;
-        __syncthreads();
-        over = gather_slowly<T, THREADS>(s_list, row, base, min(base + TILE, to), first ? 0u : over, K);
-      } else if (n > K + K / 2 + 8 && (n > List<THREADS>::LONG || base + TILE < to)) {
-        over = max(over, keep_best(s_list, n, K));
+      if (++tiles >= 2 && (tiles & (tiles - 1)) == 0 && base + TILE < hi) over = bound_of(s_list, tp_key(st.m), K, turn ^= 1);
+    }
+    base += TILE;
+  } while (base < hi);
+  if (to == row.words && behind + tid < a.V && tid < COUNT) {
+    const float x = tp_value(z, behind + tid);
+    Stats o = single(x);
+    const float m = fmaxf(st.m, o.m);
+    st.rescale(m, c);
+    o.rescale(m, c);
+    st.s += o.s; st.w += o.w;
+    if constexpr (TOP) {
+      if (tp_key(x) >= over) {
+        const int at = atomicAdd(&s_list.count, 1);
+        if (at < List<THREADS>::ROOM) s_list.entry[at] = tp_entry(tp_key(x), behind + tid);
       }
     }
   }
+  if constexpr (TOP) over = bound_of(s_list, tp_key(st.m), K, turn ^= 1);
   st = tp_join_lanes<32>(st, c);
-  if (lane == 0) s_stats[tid >> 5] = st;
-  __syncthreads();
-  if (tid < 32) {
-    st = lane < WARPS ? s_stats[lane] : Stats{-INFINITY, 0.f, 0.f};
-    st = tp_join_lanes<WARPS>(st, c);
-    if (lane == 0) s_all = st;
-  }
-  __syncthreads();
-  if constexpr (TOP) {
-    if (s_all.s != s_all.s) {                // NaN among them: the bounds were not those of the keys
-      if (tid == 0) s_list.count = 0;
-      __syncthreads();
-      gather_slowly<T, THREADS>(s_list, row, from, to, 0u, K);
-    }
-    const int n = s_list.count;
-    if (tid < TP_MOST) s_list.best[tid] = TP_NONE;
+  if constexpr (WARPS > 1) {
+    if (lane == 0) s_stats[tid >> 5] = st;
     __syncthreads();
-    if (n > 0) take_best(s_list, n, min(n, K));
+    if (tid < 32) {
+      st = lane < WARPS ? s_stats[lane] : Stats{-INFINITY, 0.f, 0.f};
+      st = tp_join_lanes<WARPS>(st, c);
+    }
+  }
+  if (tid == 0) s_all = st;
+  tp_sync<THREADS>();
+  if constexpr (TOP) {
+    // entries that reach the bound, K at least where the block has as many
+    int n = s_list.count;
+    if (n > List<THREADS>::ROOM || s_all.s != s_all.s) {      // some are missing, or a NaN is
+      gather_slowly<T, THREADS>(s_list, row, from, to, K);
+      n = s_list.count;
+      over = 0u;
+    }
+    const int few = ctas > 1 ? List<THREADS>::SHARE : List<THREADS>::SOME;
+    if (tid == 0) s_list.n[0] = 0;
+    tp_sync<THREADS>();
+    for (int i = tid; i < n; i += THREADS) {
+      const Entry e = s_list.entry[i];
+      if (static_cast<uint32_t>(e >> 32) >= over) {
+        const int at = atomicAdd(&s_list.n[0], 1);
+        if (at < few) s_list.some[at] = e;
+      }
+    }
+    tp_sync<THREADS>();
+    int some = s_list.n[0];
+    tp_sync<THREADS>();
+    if (some > few) {
+      take_best(s_list, n, K);
+      if (tid < K) s_list.some[tid] = s_list.best[tid];
+      tp_sync<THREADS>();
+      some = K;
+    }
+    if (ctas == 1) put_in_order(s_list, some, K);
+    else if (tid == 0) { s_list.n[0] = some; s_list.n[1] = static_cast<int>(over); }
   }
   if (ctas > 1) {
-    __syncwarp();
+    tp_sync<THREADS>();
     cluster_sync_all();
     if (cta == 0) {
       if (tid < 32) {
@@ -446,16 +555,30 @@ token_probs_kernel(const TokenProbsArgs a, float* log_probs, float* entropy, flo
         st = tp_join_lanes<8>(st, c);        // 8 CTAs at most
       }
       if constexpr (TOP) {
-        for (int i = tid; i < ctas * K; i += THREADS) s_list.entry[i] = tp_read_entry(tp_of_cta(&s_list.best[i % K], i / K));
+        // what reaches the largest of the bounds
+        for (int k = 0; k < ctas; ++k) over = max(over, tp_read_word(tp_of_cta(&s_list.n[1], k)));
+        if (tid == 0) s_list.count = 0;
+        tp_sync<THREADS>();
+        for (int i = tid; i < ctas * List<THREADS>::SHARE; i += THREADS) {
+          const int k = i / List<THREADS>::SHARE, e = i % List<THREADS>::SHARE;
+          if (e < static_cast<int>(tp_read_word(tp_of_cta(&s_list.n[0], k)))) {
+            const Entry x = tp_read_entry(tp_of_cta(&s_list.some[e], k));
+            if (static_cast<uint32_t>(x >> 32) >= over) s_list.entry[atomicAdd(&s_list.count, 1)] = x;
+          }
+        }
       }
     }
-    __syncwarp();
+    tp_sync<THREADS>();
     cluster_sync_all();
     if (cta != 0) return;
-    if constexpr (TOP) take_best(s_list, ctas * K, K);
+    if constexpr (TOP) {
+      const int n = s_list.count;
+      take_best(s_list, n, K);
+    }
     if (tid == 0) s_all = st;
-    __syncthreads();
+    tp_sync<THREADS>();
   }
+  if (tid >= 32) return;
   st = s_all;
   const double log_s = log(static_cast<double>(st.s));
   const float w = static_cast<float>(st.w * TP_LN2);
@@ -583,25 +706,31 @@ static int tell(const TokenProbsArgs& a, long long rows, float* log_probs, float
   // blocks of a row: as many as there is room for with four on every SM, each with a word at least for all of its threads
   const long long words = (a.V + Word<T>::COUNT - 1) / Word<T>::COUNT, room = 4ll * sm_count_current();
   unsigned ctas = 1;
-  while (ctas < 8 && rows * ctas * 2 <= room && words / (2 * ctas) >= THREADS) ctas *= 2;
+  while (THREADS > 32 && ctas < 8 && rows * ctas * 2 * THREADS <= room * 256 && words / (2 * ctas) >= THREADS) ctas *= 2;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(static_cast<unsigned>(rows) * ctas); cfg.blockDim = dim3(THREADS); cfg.stream = s;
+  constexpr int ROWS = TP_BLOCK<THREADS> / THREADS;
+  cfg.gridDim = dim3(static_cast<unsigned>((rows + ROWS - 1) / ROWS * ctas)); cfg.blockDim = dim3(TP_BLOCK<THREADS>); cfg.stream = s;
   cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeClusterDimension;
   attr[0].val.clusterDim.x = ctas; attr[0].val.clusterDim.y = 1; attr[0].val.clusterDim.z = 1;
   attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[1].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr; cfg.numAttrs = max_ctas() == 0 ? 2 : 1;
-  AXB_CUDA(cudaLaunchKernelEx(&cfg, token_probs_kernel<T, ENTROPY, TOP, THREADS>, a, log_probs, entropy, top_log_probs, top_tokens, stats));
+  AXB_CUDA(cudaLaunchKernelEx(&cfg, token_probs_kernel<T, ENTROPY, TOP, THREADS>, a, static_cast<int>(rows), log_probs, entropy, top_log_probs, top_tokens, stats));
   return 0;
 }
 
 template <typename T>
 static int tell_of(const TokenProbsArgs& a, long long rows, float* log_probs, float* entropy, float* top_log_probs, long long* top_tokens,
                    float4* stats, cudaStream_t s) {
-  const bool H = entropy || !a.whole, narrow = static_cast<long long>(a.V) * sizeof(T) <= 16384;
-  const auto go = narrow ? (H ? (a.top ? tell<T, true, true, 64> : tell<T, true, false, 64>) : (a.top ? tell<T, false, true, 64> : tell<T, false, false, 64>))
-                         : (H ? (a.top ? tell<T, true, true, 256> : tell<T, true, false, 256>) : (a.top ? tell<T, false, true, 256> : tell<T, false, false, 256>));
+  const bool H = entropy || !a.whole;
+  const long long bytes = static_cast<long long>(a.V) * sizeof(T);
+  const auto with = [&](auto threads) {
+    constexpr int N = decltype(threads)::value;
+    return H ? (a.top ? tell<T, true, true, N> : tell<T, true, false, N>) : (a.top ? tell<T, false, true, N> : tell<T, false, false, N>);
+  };
+  const auto go = bytes <= TP_NARROW ? with(std::integral_constant<int, 32>()) : bytes <= TP_MIDDLE ? with(std::integral_constant<int, 128>())
+                                                                                                  : with(std::integral_constant<int, 256>());
   return go(a, rows, log_probs, entropy, top_log_probs, top_tokens, stats, s);
 }
 
