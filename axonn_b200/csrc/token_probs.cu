@@ -25,7 +25,8 @@ constexpr int TP_WORDS = 4;                // 16-byte words of a thread, of a ti
 constexpr int TP_KEEP = 64;                // entries that a list is cut down to, at most
 constexpr float TP_LOG2E = 1.4426950408889634f;
 constexpr double TP_LN2 = 0.6931471805599453;
-constexpr long long TP_NARROW = 8192, TP_MIDDLE = 65536;      // bytes of a row for blocks of 32 and 128 threads
+constexpr long long TP_NARROW = 8192, TP_MIDDLE = 32768;      // bytes of a row for blocks of 32 and 128 threads
+constexpr long long TP_ROOM = 2;
 constexpr float TP_FAR = -8192.f;          // exponents below are this: their powers are zero, and their products with them too
 
 struct TokenProbsArgs {
@@ -185,14 +186,19 @@ __device__ __forceinline__ int tp_place(Entry e) { return static_cast<int>(0xfff
 
 constexpr Entry TP_NONE = 0;                 // below all others
 
-// Shared memory of a block's list.
+// Shared memory of a row's list.
 template <int THREADS> struct List {
-  static constexpr int ROOM = THREADS * 8 + TP_KEEP, SOME = THREADS < TP_KEEP ? TP_KEEP : THREADS;
-  static constexpr int SHARE = THREADS < 64 ? 32 : THREADS / 2;       // of a cluster's list, of a block; eight have room
+  static constexpr int ROOM = THREADS * 8 + TP_KEEP, SOME = THREADS == 32 ? TP_KEEP : 8 * TP_MOST;
+  static constexpr int WARPS = THREADS / 32, SHARE = ROOM / WARPS;    // every warp fills a part of its own
   Entry entry[ROOM], some[SOME], best[TP_MOST];
-  uint32_t bound[2][32];
-  int count, n[3];
-  static_assert(8 * SHARE <= ROOM && SHARE >= TP_MOST, "a cluster's list");
+  alignas(16) uint32_t bound[2][32];
+  int filled[WARPS];
+  int count, few, n[3];
+};
+// ... and of what the blocks of a cluster give to the first of them
+struct Gathered {
+  Entry best[8][TP_MOST];
+  Stats stats[8];
 };
 
 // Threads of a row wait for one another: a warp alone (blocks of several rows), or the block.
@@ -201,12 +207,13 @@ template <int THREADS> __device__ __forceinline__ void tp_sync() {
   else __syncthreads();
 }
 
-// The upper 16 bits of a key that at least K of the row's threads reach with theirs: the K-th largest of 32 of these, the largest of every
-// warp's.
+// A key that at least K of the row's threads reach with theirs: the K-th largest of 32 of these, the largest of every warp's.
 template <int THREADS> __device__ __forceinline__ uint32_t bound_of(List<THREADS>& l, uint32_t key, int K, int turn) {
   constexpr int EACH = 32 / (THREADS / 32);
   const int lane = threadIdx.x & 31;
-  if constexpr (THREADS > 32) {
+  if constexpr (THREADS == 32) {
+    l.bound[turn][lane] = key;
+  } else {
     uint32_t mine = 0u;
 #pragma unroll
     for (int i = 0; i < EACH; ++i) {
@@ -215,14 +222,16 @@ template <int THREADS> __device__ __forceinline__ uint32_t bound_of(List<THREADS
       if (lane == i) mine = most;
     }
     if (lane < EACH) l.bound[turn][threadIdx.x / 32 * EACH + lane] = mine;
-    __syncthreads();
-    key = l.bound[turn][lane];
   }
-  uint32_t least = 0u;
-#pragma unroll 1
-  for (uint32_t bit = 0x80000000u; bit >= 0x10000u; bit >>= 1)
-    if (__popc(__ballot_sync(0xffffffffu, key >= (least | bit))) >= K) least |= bit;
-  return least;
+  tp_sync<THREADS>();
+  key = l.bound[turn][lane];
+  int larger = 0;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const uint4 k = *reinterpret_cast<const uint4*>(&l.bound[turn][4 * i]);
+    larger += (k.x > key) + (k.y > key) + (k.z > key) + (k.w > key);
+  }
+  return __reduce_min_sync(0xffffffffu, larger < K ? key : 0xffffffffu);
 }
 
 // The K largest of some[0, n), n <= SOME, in their order, to best: what an entry's place is, its threads count.
@@ -312,25 +321,19 @@ __device__ __forceinline__ uint32_t tp_ctas() {
   asm volatile("mov.u32 %0, %%cluster_nctarank;" : "=r"(r));
   return r;
 }
-__device__ __forceinline__ uint32_t tp_of_cta(const void* p, uint32_t cta) {
+__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory"); }
+__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.aligned;" ::: "memory"); }
+// Into the shared memory of the cluster's first block, where the variable is at the same address.
+__device__ __forceinline__ uint32_t tp_of_first(const void* p) {
   uint32_t a;
-  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(smem_u32(p)), "r"(cta));
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(smem_u32(p)), "r"(0));
   return a;
 }
-__device__ __forceinline__ float tp_read_float(uint32_t a) {
-  float v;
-  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(a) : "memory");
-  return v;
+__device__ __forceinline__ void tp_give(float* to, float v) {
+  asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(tp_of_first(to)), "f"(v) : "memory");
 }
-__device__ __forceinline__ uint32_t tp_read_word(uint32_t a) {
-  uint32_t v;
-  asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(a) : "memory");
-  return v;
-}
-__device__ __forceinline__ Entry tp_read_entry(uint32_t a) {
-  Entry v;
-  asm volatile("ld.shared::cluster.u64 %0, [%1];" : "=l"(v) : "r"(a) : "memory");
-  return v;
+__device__ __forceinline__ void tp_give(Entry* to, Entry v) {
+  asm volatile("st.shared::cluster.u64 [%0], %1;" ::"r"(tp_of_first(to)), "l"(v) : "memory");
 }
 template <int LANES> __device__ __forceinline__ Stats tp_join_lanes(Stats t, float c) {
   float m = t.m;
@@ -353,7 +356,8 @@ __global__ void __launch_bounds__(TP_BLOCK<THREADS>)
 token_probs_kernel(const TokenProbsArgs a, int rows, float* log_probs, float* entropy, float* top_log_probs, long long* top_tokens, float4* stats) {
   constexpr int COUNT = Word<T>::COUNT, TILE = THREADS * TP_WORDS, WARPS = THREADS / 32;
   constexpr int ROWS = TP_BLOCK<THREADS> / THREADS;
-  __shared__ Stats s_stats[WARPS], s_alls[ROWS];
+  __shared__ Stats s_stats[WARPS];
+  __shared__ std::conditional_t<(ROWS > 1), int, Gathered> s_gathered;
   __shared__ std::conditional_t<TOP, List<THREADS>, int> s_lists[ROWS];
   pdl_launch_next();
   pdl_wait();
@@ -363,29 +367,8 @@ token_probs_kernel(const TokenProbsArgs a, int rows, float* log_probs, float* en
   const int line = ROWS > 1 ? static_cast<int>(blockIdx.x * ROWS + threadIdx.x / THREADS) : blockIdx.x / ctas;
   const int b = line / a.per_batch, r = line - b * a.per_batch;
   auto& s_list = s_lists[ROWS > 1 ? threadIdx.x / THREADS : 0];
-  Stats& s_all = s_alls[ROWS > 1 ? threadIdx.x / THREADS : 0];
   const T* z = static_cast<const T*>(a.logits) + b * a.batch_stride + r * a.row_stride;
   const long long token = a.tokens ? a.tokens[b * a.token_batch_stride + r * a.token_stride] : 0;
-  if (a.tokens && token == a.ignored) {
-    if (cta != 0) return;
-    if (tid == 0) {
-      if (log_probs) log_probs[line] = 0.f;
-      if (entropy) entropy[line] = 0.f;
-      stats[line] = make_float4(0.f, 1.f, 0.f, 0.f);
-    }
-    if (TOP && tid < K) {
-      top_log_probs[static_cast<long long>(line) * K + tid] = 0.f;
-      top_tokens[static_cast<long long>(line) * K + tid] = -1;
-    }
-    return;
-  }
-  const long long t = token - a.start;
-  float zt = 0.f;
-  if (tid == 0 && a.tokens) zt = token < 0 || token >= a.total ? __int_as_float(0x7fffffff) : t >= 0 && t < a.V ? tp_value(z, static_cast<int>(t)) : 0.f;
-  if constexpr (TOP) {
-    if (tid == 0) s_list.count = 0;
-    tp_sync<THREADS>();
-  }
   const RowWords<T> row(z, a.V, z);
   const int share = (row.words + ctas - 1) / ctas, from = min(cta * share, row.words), to = min(from + share, row.words);
   // whole words are [lo, hi); the values in front of and behind them, of the row's first and last word, are taken one by one
@@ -416,7 +399,45 @@ token_probs_kernel(const TokenProbsArgs a, int rows, float* log_probs, float* en
     const float y = x == -INFINITY ? 0.f : x;
     return Stats{fmaxf(x, -INFINITY), tp_exp2(x - y), 0.f};
   };
-  fetch(lo);
+  // a warp's part of the list
+  int filled = 0;
+  const auto push = [&](bool hit, float x, int j) {
+    if constexpr (TOP) {
+      const unsigned hits = __ballot_sync(0xffffffffu, hit);
+      const int at = filled + __popc(hits & ((1u << lane) - 1u));
+      if (hit && at < List<THREADS>::SHARE) s_list.entry[(tid >> 5) * List<THREADS>::SHARE + at] = tp_entry(tp_key(x), j);
+      filled += __popc(hits);
+    }
+  };
+  // where few blocks run, the token is not waited for: an ignored row then costs the reading of a tile
+  const bool early = ROWS > 1 || ctas > 1;
+  if (early) fetch(lo);
+  if (a.tokens && token == a.ignored) {     // for all blocks of a cluster
+    if (cta != 0) return;
+    if (tid == 0) {
+      if (log_probs) log_probs[line] = 0.f;
+      if (entropy) entropy[line] = 0.f;
+      stats[line] = make_float4(0.f, 1.f, 0.f, 0.f);
+    }
+    if (TOP && tid < K) {
+      top_log_probs[static_cast<long long>(line) * K + tid] = 0.f;
+      top_tokens[static_cast<long long>(line) * K + tid] = -1;
+    }
+    return;
+  }
+  const long long t = token - a.start;
+  float zt = 0.f;
+  if (tid == 0 && a.tokens) zt = token < 0 || token >= a.total ? __int_as_float(0x7fffffff) : t >= 0 && t < a.V ? tp_value(z, static_cast<int>(t)) : 0.f;
+  if constexpr (TOP) {
+    if (tid == 0) s_list.count = s_list.few = 0;
+    if (tid < TP_MOST) s_list.best[tid] = TP_NONE;
+    tp_sync<THREADS>();
+  }
+  if (ROWS == 1 && ctas > 1) {
+    __syncwarp();
+    cluster_arrive();
+  }
+  if (!early) fetch(lo);
   const float x_head = tid < head ? tp_value(z, tid) : -INFINITY;
   Stats st = single(x_head);
   uint32_t over = 0u;                        // a bound that K values reach which come before the next tile
@@ -458,7 +479,7 @@ token_probs_kernel(const TokenProbsArgs a, int rows, float* log_probs, float* en
       const bool first = base == lo;
       if (first) {
         over = bound_of(s_list, tp_key(st.m), K, 0);
-        if (tid < head && tp_key(x_head) >= over) s_list.entry[atomicAdd(&s_list.count, 1)] = tp_entry(tp_key(x_head), tid);
+        if (head) push(tid < head && tp_key(x_head) >= over, x_head, tid);
       }
       const float bound = over <= TP_LOWEST ? -INFINITY : tp_key_value(over);
       if (__any_sync(0xffffffffu, first ? top >= bound : top > bound)) {
@@ -473,12 +494,8 @@ token_probs_kernel(const TokenProbsArgs a, int rows, float* log_probs, float* en
 #pragma unroll
             for (int i = 0; i < 4; ++i) w.u[i] = __shfl_sync(0xffffffffu, now[k].u[i], of);
             const float x = w.one(lane & (COUNT - 1));
-            const unsigned hits = __ballot_sync(0xffffffffu, lane < COUNT && (first ? x >= bound : x > bound));
             const int j = __shfl_sync(0xffffffffu, j0, of) + k * THREADS * COUNT + lane;
-            int at = 0;
-            if (lane == 0) at = atomicAdd(&s_list.count, __popc(hits));
-            at = __shfl_sync(0xffffffffu, at, 0) + __popc(hits & ((1u << lane) - 1u));
-            if ((hits >> lane & 1u) && at < List<THREADS>::ROOM) s_list.entry[at] = tp_entry(tp_key(x), j);
+            push(lane < COUNT && (first ? x >= bound : x > bound), x, j);
           }
         }
       }
@@ -486,100 +503,90 @@ token_probs_kernel(const TokenProbsArgs a, int rows, float* log_probs, float* en
     }
     base += TILE;
   } while (base < hi);
-  if (to == row.words && behind + tid < a.V && tid < COUNT) {
-    const float x = tp_value(z, behind + tid);
+  if (to == row.words && behind < a.V && tid < 32) {
+    const bool there = lane < COUNT && behind + lane < a.V;
+    const float x = there ? tp_value(z, behind + lane) : -INFINITY;
     Stats o = single(x);
     const float m = fmaxf(st.m, o.m);
     st.rescale(m, c);
     o.rescale(m, c);
     st.s += o.s; st.w += o.w;
-    if constexpr (TOP) {
-      if (tp_key(x) >= over) {
-        const int at = atomicAdd(&s_list.count, 1);
-        if (at < List<THREADS>::ROOM) s_list.entry[at] = tp_entry(tp_key(x), behind + tid);
-      }
-    }
+    push(there && tp_key(x) >= over, x, behind + lane);
   }
-  if constexpr (TOP) over = bound_of(s_list, tp_key(st.m), K, turn ^= 1);
+  const float most_of_thread = st.m;
   st = tp_join_lanes<32>(st, c);
+  if (lane == 0) {
+    if (WARPS > 1) s_stats[tid >> 5] = st;
+    if constexpr (TOP) s_list.filled[tid >> 5] = filled;
+  }
+  if constexpr (TOP) over = bound_of(s_list, tp_key(most_of_thread), K, turn ^ 1);      // waits for all
+  else tp_sync<THREADS>();
   if constexpr (WARPS > 1) {
-    if (lane == 0) s_stats[tid >> 5] = st;
-    __syncthreads();
-    if (tid < 32) {
-      st = lane < WARPS ? s_stats[lane] : Stats{-INFINITY, 0.f, 0.f};
-      st = tp_join_lanes<WARPS>(st, c);
-    }
+    st = s_stats[lane & (WARPS - 1)];
+    st = tp_join_lanes<WARPS>(st, c);
   }
-  if (tid == 0) s_all = st;
-  tp_sync<THREADS>();
   if constexpr (TOP) {
-    // entries that reach the bound, K at least where the block has as many
-    int n = s_list.count;
-    if (n > List<THREADS>::ROOM || s_all.s != s_all.s) {      // some are missing, or a NaN is
-      gather_slowly<T, THREADS>(s_list, row, from, to, K);
-      n = s_list.count;
-      over = 0u;
-    }
-    const int few = ctas > 1 ? List<THREADS>::SHARE : List<THREADS>::SOME;
-    if (tid == 0) s_list.n[0] = 0;
-    tp_sync<THREADS>();
-    for (int i = tid; i < n; i += THREADS) {
-      const Entry e = s_list.entry[i];
-      if (static_cast<uint32_t>(e >> 32) >= over) {
-        const int at = atomicAdd(&s_list.n[0], 1);
-        if (at < few) s_list.some[at] = e;
+    // entries that reach the bound: K at least, where the block has as many
+    bool again = st.s != st.s;               // a NaN is missing, or what there was no room for
+#pragma unroll
+    for (int i = 0; i < WARPS; ++i) again |= s_list.filled[i] > List<THREADS>::SHARE;
+    if (!again) {
+      for (int i = 0; i < filled; i += 32) {
+        const Entry e = i + lane < filled ? s_list.entry[(tid >> 5) * List<THREADS>::SHARE + i + lane] : TP_NONE;
+        const bool good = e != TP_NONE && static_cast<uint32_t>(e >> 32) >= over;
+        const unsigned those = __ballot_sync(0xffffffffu, good);
+        int at = 0;
+        if (lane == 0 && those) at = atomicAdd(&s_list.few, __popc(those));
+        at = __shfl_sync(0xffffffffu, at, 0) + __popc(those & ((1u << lane) - 1u));
+        if (good && at < List<THREADS>::SOME) s_list.some[at] = e;
       }
-    }
-    tp_sync<THREADS>();
-    int some = s_list.n[0];
-    tp_sync<THREADS>();
-    if (some > few) {
-      take_best(s_list, n, K);
-      if (tid < K) s_list.some[tid] = s_list.best[tid];
       tp_sync<THREADS>();
-      some = K;
+      again = s_list.few > List<THREADS>::SOME;
     }
-    if (ctas == 1) put_in_order(s_list, some, K);
-    else if (tid == 0) { s_list.n[0] = some; s_list.n[1] = static_cast<int>(over); }
+    if (again) {
+      gather_slowly<T, THREADS>(s_list, row, from, to, K);
+      if (tid == 0) s_list.few = s_list.count;
+      for (int i = tid; i < s_list.count; i += THREADS) s_list.some[i] = s_list.entry[i];
+      tp_sync<THREADS>();
+    }
+    put_in_order(s_list, s_list.few, K);
   }
-  if (ctas > 1) {
-    tp_sync<THREADS>();
-    cluster_sync_all();
-    if (cta == 0) {
+  if constexpr (ROWS == 1) {
+    if (ctas > 1) {
+      __syncwarp();
+      cluster_wait();                        // the first block runs
       if (tid < 32) {
-        st = {-INFINITY, 0.f, 0.f};
-        if (lane < ctas) {
-          const uint32_t p = tp_of_cta(&s_all, lane);
-          st = {tp_read_float(p), tp_read_float(p + 4), tp_read_float(p + 8)};
+        if constexpr (TOP) {
+          if (lane < K) tp_give(&s_gathered.best[cta][lane], s_list.best[lane]);
         }
-        st = tp_join_lanes<8>(st, c);        // 8 CTAs at most
+        if (lane == 0) {
+          tp_give(&s_gathered.stats[cta].m, st.m);
+          tp_give(&s_gathered.stats[cta].s, st.s);
+          tp_give(&s_gathered.stats[cta].w, st.w);
+        }
       }
       if constexpr (TOP) {
-        // what reaches the largest of the bounds
-        for (int k = 0; k < ctas; ++k) over = max(over, tp_read_word(tp_of_cta(&s_list.n[1], k)));
-        if (tid == 0) s_list.count = 0;
-        tp_sync<THREADS>();
-        for (int i = tid; i < ctas * List<THREADS>::SHARE; i += THREADS) {
-          const int k = i / List<THREADS>::SHARE, e = i % List<THREADS>::SHARE;
-          if (e < static_cast<int>(tp_read_word(tp_of_cta(&s_list.n[0], k)))) {
-            const Entry x = tp_read_entry(tp_of_cta(&s_list.some[e], k));
-            if (static_cast<uint32_t>(x >> 32) >= over) s_list.entry[atomicAdd(&s_list.count, 1)] = x;
-          }
+        if (tid == 0) s_list.few = 0;
+      }
+      __syncthreads();
+      cluster_sync_all();
+      if (cta != 0) return;
+      st = (lane & 7) < ctas ? s_gathered.stats[lane & 7] : Stats{-INFINITY, 0.f, 0.f};
+      st = tp_join_lanes<8>(st, c);          // 8 blocks at most
+      if constexpr (TOP) {
+        // what reaches the largest of the blocks' K-th
+        over = __reduce_max_sync(0xffffffffu, lane < ctas ? static_cast<uint32_t>(s_gathered.best[lane][K - 1] >> 32) : 0u);
+        for (int i = tid; i < ctas * TP_MOST; i += THREADS) {
+          if (i % TP_MOST >= K) continue;
+          const Entry e = s_gathered.best[i / TP_MOST][i % TP_MOST];
+          if (e != TP_NONE && static_cast<uint32_t>(e >> 32) >= over) s_list.some[atomicAdd(&s_list.few, 1)] = e;
         }
+        __syncthreads();
+        put_in_order(s_list, s_list.few, K);
       }
     }
-    tp_sync<THREADS>();
-    cluster_sync_all();
-    if (cta != 0) return;
-    if constexpr (TOP) {
-      const int n = s_list.count;
-      take_best(s_list, n, K);
-    }
-    if (tid == 0) s_all = st;
-    tp_sync<THREADS>();
   }
   if (tid >= 32) return;
-  st = s_all;
   const double log_s = log(static_cast<double>(st.s));
   const float w = static_cast<float>(st.w * TP_LN2);
   if (tid == 0) {
@@ -704,7 +711,7 @@ template <typename T, bool ENTROPY, bool TOP, int THREADS>
 static int tell(const TokenProbsArgs& a, long long rows, float* log_probs, float* entropy, float* top_log_probs, long long* top_tokens, float4* stats,
                 cudaStream_t s) {
   // blocks of a row: as many as there is room for with four on every SM, each with a word at least for all of its threads
-  const long long words = (a.V + Word<T>::COUNT - 1) / Word<T>::COUNT, room = 4ll * sm_count_current();
+  const long long words = (a.V + Word<T>::COUNT - 1) / Word<T>::COUNT, room = (TOP ? TP_ROOM : 4ll) * sm_count_current();
   unsigned ctas = 1;
   while (THREADS > 32 && ctas < 8 && rows * ctas * 2 * THREADS <= room * 256 && words / (2 * ctas) >= THREADS) ctas *= 2;
   cudaLaunchConfig_t cfg = {};
@@ -729,8 +736,9 @@ static int tell_of(const TokenProbsArgs& a, long long rows, float* log_probs, fl
     constexpr int N = decltype(threads)::value;
     return H ? (a.top ? tell<T, true, true, N> : tell<T, true, false, N>) : (a.top ? tell<T, false, true, N> : tell<T, false, false, N>);
   };
-  const auto go = bytes <= TP_NARROW ? with(std::integral_constant<int, 32>()) : bytes <= TP_MIDDLE ? with(std::integral_constant<int, 128>())
-                                                                                                  : with(std::integral_constant<int, 256>());
+  const bool many = rows >= 4ll * sm_count_current();
+  const auto go = bytes <= TP_NARROW && a.top <= (2 * bytes <= TP_NARROW ? 24 : 4) ? with(std::integral_constant<int, 32>())
+                : many || bytes <= TP_MIDDLE ? with(std::integral_constant<int, 128>()) : with(std::integral_constant<int, 256>());
   return go(a, rows, log_probs, entropy, top_log_probs, top_tokens, stats, s);
 }
 
