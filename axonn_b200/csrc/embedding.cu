@@ -6,23 +6,26 @@
 //
 // Both are bound by the rows' bytes.  The gradient sorts (token, place) pairs and sums along the sorted list, so that every row of the
 // gradient is written once, by one block, and no addition depends on when a block runs:
-//   1. One cluster sorts by a stable radix sort; its CTAs exchange the digits' counts through distributed shared memory.  It also notes
-//      which tokens there are.
+//   1. One cluster sorts by a stable radix sort; its CTAs exchange counts, and up to 32,768 pairs, through distributed shared memory.  It
+//      also notes which tokens there are.
 //   2. Blocks sum chunks of 32 pairs, columns split over blocks; other blocks of the same launch zero the rows of the tokens that
 //      there are not.  A chunk is summed with what the last token of it has in the next one, unless that token fills the whole next
 //      chunk: then its sum so far goes to the workspace.  A segment of any length so takes many blocks, and one of up to 32 pairs
 //      no extra traffic.
-//   3. The partial sums of long segments are joined in their order.
+//   3. The partial sums of long segments are joined in their order; where they are is found out while the sums are still made.
 #include "common.cuh"
 
 namespace axb {
 
 constexpr int SORT_THREADS = 1024, SORT_WARPS = SORT_THREADS / 32, SORT_DIGIT = 9, SORT_BINS = 1 << SORT_DIGIT;
-constexpr int SORT_SMEM = SORT_WARPS * SORT_BINS * 4;
+constexpr int SORT_CTAS = 8, SORT_KEEP = 4;       // pairs of a thread that stay in registers
+constexpr int SORT_SHARE = SORT_THREADS * SORT_KEEP, SORT_SMALL = SORT_CTAS * SORT_SHARE;
+constexpr int SORT_ALONE = 2 * SORT_THREADS;      // tokens that one CTA sorts
+constexpr int SORT_SMEM = SORT_WARPS * SORT_BINS * 4, SORT_SMEM_SMALL = SORT_SMEM + 2 * SORT_SHARE * 8;
 constexpr int CHUNK = 32;                     // pairs of a block of sums: a warp's lanes look one chunk ahead
 constexpr int SUM_THREADS = 128, SUM_AHEAD = 8;
 constexpr int ZERO_BYTES = 1 << 17;           // of the table, of a block that zeroes
-constexpr int JOIN_THREADS = 256, JOIN_COLS = 128, JOIN_BLOCKS = 32;
+constexpr int JOIN_THREADS = 256, JOIN_COLS = 128, JOIN_BLOCKS = 128;
 constexpr int ROW_THREADS = 256, ROW_AHEAD = 4;
 
 template <typename T> __device__ __forceinline__ float to_float(T x) {
@@ -40,33 +43,58 @@ template <typename T> __device__ __forceinline__ T from_float(float x) {
 template <typename T, int N> struct alignas(sizeof(T) * N) Piece { T v[N]; };
 
 // ------------------------------------------------------------------------------------------------------------------------ lookup
-// `group` threads (a power of two) a row, ROWS rows for each of them at a time
+// `group` threads (a power of two) a row, ROWS rows for each of them at a time, 16 bytes of each in pieces of N values.  Tokens are read a
+// step ahead.
 template <typename T, typename I, int N, int ROWS>
 __global__ void __launch_bounds__(ROW_THREADS)
 embedding_kernel(const I* __restrict__ tokens, long long n, const T* __restrict__ table, long long pitch, int V, int H, float scale,
                  T* __restrict__ out, int group) {
   using P = Piece<T, N>;
+  constexpr int PIECES = 16 / sizeof(P);
   pdl_launch_next();
   pdl_wait();
   const int groups = ROW_THREADS / group, at = threadIdx.x & (group - 1);
-  const long long first = (static_cast<long long>(blockIdx.x) * groups + threadIdx.x / group) * ROWS;
-  long long t[ROWS];
+  long long first = (static_cast<long long>(blockIdx.x) * groups + threadIdx.x / group) * ROWS;
+  const long long step = static_cast<long long>(gridDim.x) * groups * ROWS;
+  const bool as_is = scale == 1.f;
+  I next[ROWS];
+  const auto fetch = [&](long long i) {
 #pragma unroll
-  for (int r = 0; r < ROWS; ++r) {
-    t[r] = first + r < n ? static_cast<long long>(tokens[first + r]) : -1;
-    if (t[r] >= V) t[r] = -1;
-  }
-  for (int c = at * N; c < H; c += group * N) {
-    P p[ROWS];
-#pragma unroll
-    for (int r = 0; r < ROWS; ++r)
-      if (t[r] >= 0) p[r] = *reinterpret_cast<const P*>(table + t[r] * pitch + c);
+    for (int r = 0; r < ROWS; ++r) next[r] = i + r < n ? tokens[i + r] : I(-1);
+  };
+  fetch(first);
+  for (; first < n; first += step) {
+    const T* from[ROWS];
+    bool there[ROWS];
 #pragma unroll
     for (int r = 0; r < ROWS; ++r) {
-      if (first + r >= n) break;
+      there[r] = next[r] >= 0 && next[r] < V;
+      from[r] = table + (there[r] ? static_cast<long long>(next[r]) * pitch : 0ll);
+    }
+    fetch(first + step);
+    T* to = out + first * H;
+    const int rows = static_cast<int>(min(static_cast<long long>(ROWS), n - first));
+    for (int c0 = at * N; c0 < H; c0 += group * N * PIECES) {
+      P p[ROWS][PIECES];
 #pragma unroll
-      for (int i = 0; i < N; ++i) p[r].v[i] = from_float<T>(t[r] >= 0 ? to_float(p[r].v[i]) * scale : __int_as_float(0x7fffffff));
-      *reinterpret_cast<P*>(out + (first + r) * H + c) = p[r];
+      for (int r = 0; r < ROWS; ++r)
+#pragma unroll
+        for (int k = 0; k < PIECES; ++k)
+          if (c0 + k * group * N < H) p[r][k] = *reinterpret_cast<const P*>(from[r] + c0 + k * group * N);
+#pragma unroll
+      for (int r = 0; r < ROWS; ++r) {
+        if (r >= rows) break;
+        if (!as_is || !there[r]) {
+          const float by = there[r] ? scale : __int_as_float(0x7fffffff);
+#pragma unroll
+          for (int k = 0; k < PIECES; ++k)
+#pragma unroll
+            for (int i = 0; i < N; ++i) p[r][k].v[i] = from_float<T>(to_float(p[r][k].v[i]) * by);
+        }
+#pragma unroll
+        for (int k = 0; k < PIECES; ++k)
+          if (c0 + k * group * N < H) *reinterpret_cast<P*>(to + static_cast<long long>(r) * H + c0 + k * group * N) = p[r][k];
+      }
     }
   }
 }
@@ -86,46 +114,97 @@ __device__ __forceinline__ uint32_t read_of_cta(const uint32_t* p, uint32_t cta)
   return v;
 }
 
-// One cluster.  `a` and `b` take turns; the result is in `b` after an odd number of passes, in `a` after an even one.  Tokens without a
-// gradient have the key V.  A warp has a contiguous run of pairs and counts of its own, so that equal digits keep their order.
-template <typename I>
+// Lanes of the warp with the same digit of `bits` bits, of those that are there.
+__device__ __forceinline__ uint32_t same_digit(uint32_t d, int bits, bool there) {
+  uint32_t same = __ballot_sync(0xffffffffu, there);
+  for (int b = 0; b < bits; ++b) {
+    const uint32_t set = __ballot_sync(0xffffffffu, d >> b & 1u);
+    same &= d >> b & 1u ? set : ~set;
+  }
+  return same;
+}
+
+__device__ __forceinline__ void give_to_cta(uint2* p, uint32_t cta, uint2 v) {
+  uint32_t addr;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(addr) : "r"(smem_u32(p)), "r"(cta));
+  asm volatile("st.shared::cluster.v2.u32 [%0], {%1, %2};" ::"r"(addr), "r"(v.x), "r"(v.y) : "memory");
+}
+
+// One cluster.  Tokens without a gradient have the key V.  A warp has a contiguous run of pairs and counts of its own, so that equal
+// digits keep their order.  SMALL: a warp's pairs stay in registers, and the CTAs hand them to one another through shared memory, of which
+// each has two parts of the whole list.  Otherwise they go through `a` and `b` in turns.  The result is in `a` if SMALL or after an even
+// number of passes, and in `b` after an odd one.
+template <typename I, bool SMALL>
 __global__ void __launch_bounds__(SORT_THREADS)
-sort_tokens_kernel(const I* __restrict__ tokens, int n, int V, long long padding, Digits digits, uint2* a, uint2* b, uint32_t* met) {
-  extern __shared__ uint32_t s_count[];         // [SORT_WARPS][SORT_BINS]
+sort_tokens_kernel(const I* __restrict__ tokens, int n, int V, long long padding, Digits digits, uint2* a, uint2* b, uint8_t* met) {
+  extern __shared__ uint4 s_memory[];
+  uint32_t* const s_count = reinterpret_cast<uint32_t*>(s_memory);         // [SORT_WARPS][SORT_BINS]
+  uint2* const s_pairs = reinterpret_cast<uint2*>(s_count + SORT_WARPS * SORT_BINS);
   __shared__ uint32_t s_total[SORT_BINS], s_base[SORT_BINS], s_warp[SORT_BINS / 32];
   pdl_launch_next();
   pdl_wait();
   const int tid = threadIdx.x, lane = tid & 31, w = tid >> 5;
-  const uint32_t cta = cluster_cta_rank(), ctas = cluster_ctas();
-  for (uint32_t i = cta * SORT_THREADS + tid; i < (V + 31u) / 32u; i += ctas * SORT_THREADS) met[i] = 0u;
+  const uint32_t cta = cluster_cta_rank(), ctas = cluster_ctas(), lower = (1u << lane) - 1u;
   const long long warps = static_cast<long long>(ctas) * SORT_WARPS, run = ((n + warps - 1) / warps + 31) / 32 * 32;
   const long long from = (static_cast<long long>(cta) * SORT_WARPS + w) * run, to = min(from + run, static_cast<long long>(n));
+  const uint32_t share = static_cast<uint32_t>(run) * SORT_WARPS;          // pairs of a CTA (SMALL)
   uint32_t* mine = s_count + w * SORT_BINS;
-  const uint2* in = nullptr;
-  uint2* out = b;
-  int shift = 0;
-  auto pair_at = [&](long long i) {
-    if (in) return __ldcg(in + i);
+  const auto key_of = [&](long long i) {
     const long long t = tokens[i];
     return make_uint2(t >= 0 && t < V && t != padding ? static_cast<uint32_t>(t) : static_cast<uint32_t>(V), static_cast<uint32_t>(i));
   };
+  uint2 kept[SORT_KEEP];
+#pragma unroll
+  for (int k = 0; k < SORT_KEEP; ++k) kept[k] = from + 32 * k + lane < to ? key_of(from + 32 * k + lane) : make_uint2(0u, 0u);
+  for (long long i = cta * SORT_THREADS + tid; i < (V + 15ll) / 16; i += ctas * SORT_THREADS) reinterpret_cast<uint4*>(met)[i] = make_uint4(0u, 0u, 0u, 0u);
+  const uint2* in = nullptr;
+  uint2* out = b;
+  int shift = 0;
   for (int pass = 0; pass < digits.passes; ++pass) {
     const int bits = digits.bits[pass], bins = 1 << bits;
     const uint32_t mask = bins - 1u;
+    const bool last = pass + 1 == digits.passes;
+    uint32_t kept_same[SORT_KEEP];
+    const auto pair_at = [&](long long i) {
+      if (i >= to) return make_uint2(0u, 0u);
+      return in ? __ldcg(in + i) : key_of(i);
+    };
+    const auto count = [&](uint2 p, bool there) {
+      const uint32_t d = p.x >> shift & mask, same = same_digit(d, bits, there);
+      if (there && (same & lower) == 0u) mine[d] += __popc(same);
+      __syncwarp();
+      return same;
+    };
+    const auto place = [&](uint2 p, uint32_t same, bool there) {
+      const uint32_t d = p.x >> shift & mask;
+      uint32_t at = 0u;
+      if (there) at = s_base[d] + mine[d] + __popc(same & lower);
+      __syncwarp();
+      if (there) {
+        if ((same & lower) == 0u) mine[d] += __popc(same);
+        if (last && p.x < static_cast<uint32_t>(V)) met[p.x] = 1;          // of equal tokens, all write the same
+        if (!SMALL) out[at] = p;
+        else if (last) a[at] = p;
+        else give_to_cta(s_pairs + (pass & 1) * SORT_SHARE + at % share, at / share, p);
+      }
+      __syncwarp();
+    };
     for (int i = lane; i < bins; i += 32) mine[i] = 0u;
     __syncwarp();
-    for (long long i = from; i < to; i += 32) {
-      const bool there = i + lane < to;
-      const uint32_t d = there ? pair_at(i + lane).x >> shift & mask : 0xffffffffu;
-      const uint32_t same = __match_any_sync(0xffffffffu, d);
-      if (there && (same & ((1u << lane) - 1u)) == 0u) mine[d] += __popc(same);
-      __syncwarp();
+    if (!SMALL && pass > 0) {
+#pragma unroll
+      for (int k = 0; k < SORT_KEEP; ++k) kept[k] = pair_at(from + 32 * k + lane);
     }
+#pragma unroll
+    for (int k = 0; k < SORT_KEEP; ++k)
+      if (from + 32 * k < to) kept_same[k] = count(kept[k], from + 32 * k + lane < to);
+    if (!SMALL)
+      for (long long i = from + 32 * SORT_KEEP; i < to; i += 32) count(pair_at(i + lane), i + lane < to);
     __syncthreads();
     // counts of the warps before, then those of the CTAs before and of the smaller digits
     if (tid < bins) {
       uint32_t sum = 0u;
-#pragma unroll 8
+#pragma unroll
       for (int k = 0; k < SORT_WARPS; ++k) {
         const uint32_t c = s_count[k * SORT_BINS + tid];
         s_count[k * SORT_BINS + tid] = sum;
@@ -137,12 +216,14 @@ sort_tokens_kernel(const I* __restrict__ tokens, int n, int V, long long padding
     cluster_sync_all();                          // also: `met` is zero
     uint32_t before = 0u, all = 0u, upto = 0u;
     if (tid < SORT_BINS) {
-      if (tid < bins)
-        for (uint32_t k = 0; k < ctas; ++k) {
-          const uint32_t c = read_of_cta(s_total + tid, k);
+      if (tid < bins) {
+#pragma unroll
+        for (uint32_t k = 0; k < SORT_CTAS; ++k) {
+          const uint32_t c = k < ctas ? read_of_cta(s_total + tid, k) : 0u;
           if (k < cta) before += c;
           all += c;
         }
+      }
       upto = all;
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
@@ -153,56 +234,60 @@ sort_tokens_kernel(const I* __restrict__ tokens, int n, int V, long long padding
     }
     __syncthreads();
     if (tid < bins) {
-      for (int k = 0; k < w; ++k) upto += s_warp[k];
+#pragma unroll
+      for (int k = 0; k < SORT_BINS / 32; ++k) if (k < w) upto += s_warp[k];
       s_base[tid] = upto - all + before;
     }
     __syncthreads();
-    for (long long i = from; i < to; i += 32) {
-      const bool there = i + lane < to;
-      const uint2 p = there ? pair_at(i + lane) : make_uint2(0u, 0u);
-      const uint32_t d = there ? p.x >> shift & mask : 0xffffffffu;
-      const uint32_t same = __match_any_sync(0xffffffffu, d), lower = same & ((1u << lane) - 1u);
-      uint32_t at = 0u;
-      if (there) at = s_base[d] + mine[d] + __popc(lower);
-      __syncwarp();
-      if (there) {
-        if (lower == 0u) mine[d] += __popc(same);
-        if (pass == 0 && p.x < static_cast<uint32_t>(V)) atomicOr(met + (p.x >> 5), 1u << (p.x & 31u));
-        out[at] = p;
+#pragma unroll
+    for (int k = 0; k < SORT_KEEP; ++k)
+      if (from + 32 * k < to) place(kept[k], kept_same[k], from + 32 * k + lane < to);
+    if (!SMALL)
+      for (long long i = from + 32 * SORT_KEEP; i < to; i += 32) {
+        const uint2 p = pair_at(i + lane);
+        const bool there = i + lane < to;
+        place(p, same_digit(p.x >> shift & mask, bits, there), there);
       }
-      __syncwarp();
-    }
+    __syncwarp();
     cluster_sync_all();                          // the pairs are there, and the totals have been read
+    if (SMALL && !last) {
+#pragma unroll
+      for (int k = 0; k < SORT_KEEP; ++k)
+        if (from + 32 * k + lane < to) kept[k] = s_pairs[(pass & 1) * SORT_SHARE + w * run + 32 * k + lane];
+    }
     in = out;
     out = out == b ? a : b;
     shift += bits;
   }
 }
 
-// Where a chunk's work lies in the sorted list: pairs [from, to); `partial`: the last segment goes on in the next chunk's work, or began in
-// an earlier one.
+// Sums of a chunk, 16 bytes of columns per thread in pieces of N values; behind the blocks of the sums those that zero rows.
 template <typename T, int N>
 __global__ void __launch_bounds__(SUM_THREADS)
 sum_rows_kernel(const uint2* __restrict__ pairs, int n, const T* __restrict__ dy, long long pitch, int V, int H, int Hp, float scale,
-                const uint32_t* __restrict__ met, T* __restrict__ dtable, float* __restrict__ partial, int slices, long long sum_blocks,
+                const uint8_t* __restrict__ met, T* __restrict__ dtable, float* __restrict__ partial, int slices, long long sum_blocks,
                 int zero_rows) {
   using P = Piece<T, N>;
+  constexpr int PIECES = 16 / sizeof(P), STEP = SUM_THREADS * N;
   __shared__ uint2 s_pair[2 * CHUNK + 1];
-  pdl_launch_next();
   pdl_wait();
+  pdl_launch_next();                             // what the next kernel reads before it waits has been there before this one
   const int tid = threadIdx.x, lane = tid & 31;
   if (blockIdx.x >= sum_blocks) {
-    const int words = H / N, v0 = static_cast<int>(blockIdx.x - sum_blocks) * zero_rows, rows = min(zero_rows, V - v0);
-    const int row_step = SUM_THREADS / words, col_step = SUM_THREADS - row_step * words;
-    int row = tid / words, col = tid - row * words;
-    P zero;
-#pragma unroll
-    for (int i = 0; i < N; ++i) zero.v[i] = from_float<T>(0.f);
-    while (row < rows) {
-      const int v = v0 + row;
-      if (!(__ldg(met + (v >> 5)) >> (v & 31) & 1u)) *reinterpret_cast<P*>(dtable + static_cast<long long>(v) * H + col * N) = zero;
-      row += row_step; col += col_step;
-      if (col >= words) { col -= words; ++row; }
+    // a warp a row: the values in front of the first 16-byte boundary, whole words, the values behind the last
+    const int v0 = static_cast<int>(blockIdx.x - sum_blocks) * zero_rows, v1 = min(v0 + zero_rows, V);
+    constexpr int COUNT = 16 / sizeof(T);
+    for (int v = v0 + tid / 32; v < v1; v += SUM_THREADS / 32) {
+      if (__ldg(met + v)) continue;
+      T* row = dtable + static_cast<long long>(v) * H;
+      const int head = N == COUNT ? 0 : min(static_cast<int>((16u - (reinterpret_cast<unsigned long long>(row) & 15u)) % 16u / sizeof(T)), H);
+      const int words = (H - head) / COUNT;
+      uint4* to = reinterpret_cast<uint4*>(row + head);
+      for (int i = lane; i < words; i += 32) to[i] = make_uint4(0u, 0u, 0u, 0u);
+      if (N < COUNT) {
+        if (lane < head) row[lane] = from_float<T>(0.f);
+        if (head + words * COUNT + lane < H) row[head + words * COUNT + lane] = from_float<T>(0.f);
+      }
     }
     return;
   }
@@ -228,36 +313,49 @@ sum_rows_kernel(const uint2* __restrict__ pairs, int n, const T* __restrict__ dy
     if (all_one) open = true;
     else from = __ffs(~__ballot_sync(0xffffffffu, lane < here && key(lane) == first)) - 1;
   }
-  if (from >= here) return;
-  const int col = (slice * SUM_THREADS + tid) * N;
+  if (from >= here || key(from) >= static_cast<uint32_t>(V)) return;
+  // tokens without a gradient are the last ones
+  if (last >= static_cast<uint32_t>(V)) {
+    to = min(to, from + __popc(__ballot_sync(0xffffffffu, from + lane < here && key(from + lane) < static_cast<uint32_t>(V))));
+    open = false;
+  }
+  const int col = slice * STEP * PIECES + tid * N;
   if (col >= H) return;
-  float sum[N] = {};
+  float sum[PIECES][N] = {};
   uint32_t now = key(from);
   const auto store = [&] {
-    if (now >= static_cast<uint32_t>(V)) return;
-    P p;
 #pragma unroll
-    for (int i = 0; i < N; ++i) { p.v[i] = from_float<T>(sum[i] * scale); sum[i] = 0.f; }
-    *reinterpret_cast<P*>(dtable + static_cast<long long>(now) * H + col) = p;
+    for (int c = 0; c < PIECES; ++c) {
+      P p;
+#pragma unroll
+      for (int i = 0; i < N; ++i) { p.v[i] = from_float<T>(sum[c][i] * scale); sum[c][i] = 0.f; }
+      if (col + c * STEP < H) *reinterpret_cast<P*>(dtable + static_cast<long long>(now) * H + col + c * STEP) = p;
+    }
   };
   for (int i = from; i < to; i += SUM_AHEAD) {
-    P p[SUM_AHEAD];
-#pragma unroll
-    for (int k = 0; k < SUM_AHEAD; ++k)
-      if (i + k < to && key(i + k) < static_cast<uint32_t>(V)) p[k] = *reinterpret_cast<const P*>(dy + s_pair[1 + i + k].y * pitch + col);
+    P p[SUM_AHEAD][PIECES];
 #pragma unroll
     for (int k = 0; k < SUM_AHEAD; ++k) {
-      if (i + k >= to || key(i + k) >= static_cast<uint32_t>(V)) break;
+      const T* row = dy + s_pair[1 + min(i + k, to - 1)].y * pitch + col;
+#pragma unroll
+      for (int c = 0; c < PIECES; ++c) if (col + c * STEP < H) p[k][c] = *reinterpret_cast<const P*>(row + c * STEP);
+    }
+#pragma unroll
+    for (int k = 0; k < SUM_AHEAD; ++k) {
+      if (i + k >= to) break;
       if (key(i + k) != now) { store(); now = key(i + k); }
 #pragma unroll
-      for (int c = 0; c < N; ++c) sum[c] += to_float(p[k].v[c]);
+      for (int c = 0; c < PIECES; ++c)
+#pragma unroll
+        for (int j = 0; j < N; ++j) sum[c][j] += to_float(p[k][c].v[j]);
     }
   }
   if (!open || now != last) { store(); return; }
-  if (now >= static_cast<uint32_t>(V)) return;
   float* to_part = partial + static_cast<long long>(chunk) * Hp + col;
 #pragma unroll
-  for (int c = 0; c < N; ++c) to_part[c] = sum[c];
+  for (int c = 0; c < PIECES; ++c)
+#pragma unroll
+    for (int j = 0; j < N; ++j) if (col + c * STEP < H) to_part[c * STEP + j] = sum[c][j];
 }
 
 // Segments that fill the chunk behind the one that they begin in: their pieces are that chunk and all that they fill.
@@ -269,12 +367,12 @@ join_rows_kernel(const uint2* __restrict__ pairs, int n, int V, int H, int Hp, f
   __shared__ int s_warp[JOIN_THREADS / 32];
   __shared__ float4 s_sum[JOIN_THREADS / 32][32];
   pdl_launch_next();
-  pdl_wait();
+  // the sorted pairs were there before the kernel of the sums began, which this one may start beside
   const int tid = threadIdx.x, lane = tid & 31, w = tid >> 5;
   const int full = n / CHUNK;                    // chunks that a segment can fill
   const auto last_of = [&](long long chunk) { return pairs[chunk * CHUNK + CHUNK - 1].x; };
   const int col = blockIdx.y * JOIN_COLS + lane * 4;
-  int seen = 0;
+  unsigned seen = 0;
   for (int c0 = 0; c0 + 1 < full; c0 += JOIN_THREADS) {
     const int c = c0 + tid;
     bool begins = false;
@@ -290,7 +388,7 @@ join_rows_kernel(const uint2* __restrict__ pairs, int n, int V, int H, int Hp, f
     if (begins) s_first[before + __popc(flags & ((1u << lane) - 1u))] = c;
     __syncthreads();
     for (int i = 0; i < count; ++i) {
-      if ((seen + i) % JOIN_BLOCKS != static_cast<int>(blockIdx.x)) continue;
+      if ((seen + i) % gridDim.x != blockIdx.x) continue;
       const int begin = s_first[i];
       const uint32_t k = last_of(begin);
       int pieces = 1;
@@ -298,6 +396,7 @@ join_rows_kernel(const uint2* __restrict__ pairs, int n, int V, int H, int Hp, f
         const int at = begin + pieces + tid;
         more = __syncthreads_count(at < full && last_of(at) == k);
       }
+      pdl_wait();
       float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
       if (col < Hp) {
 #pragma unroll 4
@@ -323,6 +422,7 @@ join_rows_kernel(const uint2* __restrict__ pairs, int n, int V, int H, int Hp, f
     seen += count;
     __syncthreads();
   }
+  pdl_wait();                                    // this kernel's end stands for the sums' too
 }
 
 // ------------------------------------------------------------------------------------------------------------------------ launches
@@ -337,14 +437,16 @@ static unsigned long long address(const void* p) { return reinterpret_cast<unsig
 
 template <typename T, typename I, int N>
 static int look_up(const void* tokens, long long n, const void* table, long long pitch, int V, int H, float scale, void* out, cudaStream_t s) {
-  const int words = H / N;
+  constexpr int COUNT = 16 / sizeof(T);
+  const int words = (H + COUNT - 1) / COUNT;
   int group = 32;
   while (group < ROW_THREADS && group < words) group *= 2;
   const int groups = ROW_THREADS / group;
   // several rows at a time where there are blocks enough for all SMs without
-  const bool ahead = n / groups >= 8ll * ROW_AHEAD * sm_count_current();
-  const long long per = static_cast<long long>(groups) * (ahead ? ROW_AHEAD : 1);
-  AXB_CUDA(pdl_launch(ahead ? embedding_kernel<T, I, N, ROW_AHEAD> : embedding_kernel<T, I, N, 1>, dim3(static_cast<unsigned>((n + per - 1) / per)),
+  const long long room = 2048ll / ROW_THREADS * sm_count_current();
+  const bool ahead = n / groups >= room * ROW_AHEAD;
+  const long long per = static_cast<long long>(groups) * (ahead ? ROW_AHEAD : 1), blocks = (n + per - 1) / per;
+  AXB_CUDA(pdl_launch(ahead ? embedding_kernel<T, I, N, ROW_AHEAD> : embedding_kernel<T, I, N, 1>, dim3(static_cast<unsigned>(blocks < room ? blocks : room)),
                       dim3(ROW_THREADS), 0, s, static_cast<const I*>(tokens), n, static_cast<const T*>(table), pitch, V, H, scale,
                       static_cast<T*>(out), group));
   return 0;
@@ -355,14 +457,14 @@ struct GradWork {
   GradWork(long long n, int V, int H) {
     chunks = (n + CHUNK - 1) / CHUNK;
     Hp = (H + 3) / 4 * 4;
-    met = ((V + 31ll) / 32 + 3) / 4 * 4;
+    met = (V + 15ll) / 16 * 4;                   // a byte for every token
     pairs = (2 * n + 3) / 4 * 4;
     words = met + 2 * pairs + (chunks > 1 ? chunks * Hp : 0);
   }
 };
 
 template <typename I>
-static int sort_tokens(const void* tokens, int n, int V, long long padding, uint2* a, uint2* b, uint32_t* met, Digits& digits, cudaStream_t s) {
+static int sort_tokens(const void* tokens, int n, int V, long long padding, uint2* a, uint2* b, uint8_t* met, Digits& digits, cudaStream_t s) {
   int bits = 0;
   while (V >> bits) ++bits;                      // V itself is the key of tokens without a gradient
   digits.passes = (bits + SORT_DIGIT - 1) / SORT_DIGIT;
@@ -370,11 +472,13 @@ static int sort_tokens(const void* tokens, int n, int V, long long padding, uint
     digits.bits[i] = (left + digits.passes - i - 1) / (digits.passes - i);
     left -= digits.bits[i];
   }
-  auto kernel = sort_tokens_kernel<I>;
-  AXB_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, SORT_SMEM));
+  const bool small = n <= SORT_SMALL;
+  const auto kernel = small ? sort_tokens_kernel<I, true> : sort_tokens_kernel<I, false>;
+  const int smem = small ? SORT_SMEM_SMALL : SORT_SMEM;
+  AXB_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
   cudaLaunchConfig_t cfg = {};
-  const unsigned ctas = n <= 2 * SORT_THREADS ? 1 : 8;
-  cfg.gridDim = dim3(ctas); cfg.blockDim = dim3(SORT_THREADS); cfg.dynamicSmemBytes = SORT_SMEM; cfg.stream = s;
+  const unsigned ctas = n <= SORT_ALONE ? 1 : SORT_CTAS;
+  cfg.gridDim = dim3(ctas); cfg.blockDim = dim3(SORT_THREADS); cfg.dynamicSmemBytes = smem; cfg.stream = s;
   cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeClusterDimension;
   attr[0].val.clusterDim.x = ctas; attr[0].val.clusterDim.y = 1; attr[0].val.clusterDim.z = 1;
@@ -387,8 +491,8 @@ static int sort_tokens(const void* tokens, int n, int V, long long padding, uint
 
 template <typename T, int N>
 static int sum_rows(const uint2* pairs, int n, const void* dy, long long pitch, int V, int H, const GradWork& work, float scale,
-                    const uint32_t* met, void* dtable, float* partial, cudaStream_t s) {
-  const int slices = (H / N + SUM_THREADS - 1) / SUM_THREADS;
+                    const uint8_t* met, void* dtable, float* partial, cudaStream_t s) {
+  const int slices = (H + SUM_THREADS * 16 / static_cast<int>(sizeof(T)) - 1) / (SUM_THREADS * 16 / static_cast<int>(sizeof(T)));
   const int row_bytes = H * static_cast<int>(sizeof(T));
   const int zero_rows = row_bytes >= ZERO_BYTES ? 1 : ZERO_BYTES / row_bytes;
   const long long sum_blocks = work.chunks * slices, blocks = sum_blocks + (V + static_cast<long long>(zero_rows) - 1) / zero_rows;
@@ -409,16 +513,17 @@ static int gradient(const void* tokens, int token_bytes, int n, const void* dy, 
   uint2 *a = reinterpret_cast<uint2*>(words + work.met), *b = reinterpret_cast<uint2*>(words + work.met + work.pairs);
   float* partial = reinterpret_cast<float*>(words + work.met + 2 * work.pairs);
   Digits digits;
-  if (token_bytes == 8 ? sort_tokens<long long>(tokens, n, V, padding, a, b, words, digits, s)
-                       : sort_tokens<int>(tokens, n, V, padding, a, b, words, digits, s)) return -1;
-  const uint2* pairs = digits.passes % 2 ? b : a;
+  uint8_t* met = reinterpret_cast<uint8_t*>(words);
+  if (token_bytes == 8 ? sort_tokens<long long>(tokens, n, V, padding, a, b, met, digits, s)
+                       : sort_tokens<int>(tokens, n, V, padding, a, b, met, digits, s)) return -1;
+  const uint2* pairs = n > SORT_SMALL && digits.passes % 2 ? b : a;
   const int size = sizeof(T), bytes = piece_bytes(size, {address(dy), address(dtable), static_cast<unsigned long long>(H) * size,
                                                          static_cast<unsigned long long>(pitch) * size});
   const auto sums = bytes == 16 ? sum_rows<T, 16 / sizeof(T)> : bytes == 8 ? sum_rows<T, 8 / sizeof(T)> : bytes == 4 ? sum_rows<T, 4 / sizeof(T)>
                                                                                                                      : sum_rows<T, 1>;
-  if (sums(pairs, n, dy, pitch, V, H, work, scale, words, dtable, partial, s)) return -1;
+  if (sums(pairs, n, dy, pitch, V, H, work, scale, met, dtable, partial, s)) return -1;
   if (n < 2 * CHUNK) return 0;
-  AXB_CUDA(pdl_launch(join_rows_kernel<T>, dim3(JOIN_BLOCKS, static_cast<unsigned>((work.Hp + JOIN_COLS - 1) / JOIN_COLS)), dim3(JOIN_THREADS), 0, s,
+  AXB_CUDA(pdl_launch(join_rows_kernel<T>, dim3(n / CHUNK / 2 < JOIN_BLOCKS ? n / CHUNK / 2 : JOIN_BLOCKS, static_cast<unsigned>((work.Hp + JOIN_COLS - 1) / JOIN_COLS)), dim3(JOIN_THREADS), 0, s,
                       pairs, n, V, H, static_cast<int>(work.Hp), scale, static_cast<const float*>(partial), static_cast<T*>(dtable)));
   return 0;
 }
