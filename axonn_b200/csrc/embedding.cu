@@ -12,7 +12,7 @@
 //      there are not.  A chunk is summed with what the last token of it has in the next one, unless that token fills the whole next
 //      chunk: then its sum so far goes to the workspace.  A segment of any length so takes many blocks, and one of up to 32 pairs
 //      no extra traffic.
-//   3. The partial sums of long segments are joined in their order; where they are is found out while the sums are still made.
+//   3. The partial sums of long segments, which the blocks of the sums have noted, are joined in their order.
 #include "common.cuh"
 
 namespace axb {
@@ -25,7 +25,7 @@ constexpr int SORT_SMEM = SORT_WARPS * SORT_BINS * 4, SORT_SMEM_SMALL = SORT_SME
 constexpr int CHUNK = 32;                     // pairs of a block of sums: a warp's lanes look one chunk ahead
 constexpr int SUM_THREADS = 128, SUM_AHEAD = 8;
 constexpr int ZERO_BYTES = 1 << 17;           // of the table, of a block that zeroes
-constexpr int JOIN_THREADS = 256, JOIN_COLS = 128, JOIN_BLOCKS = 128;
+constexpr int JOIN_THREADS = 256, JOIN_COLS = 128, JOIN_BLOCKS = 64;
 constexpr int ROW_THREADS = 256, ROW_AHEAD = 4;
 
 template <typename T> __device__ __forceinline__ float to_float(T x) {
@@ -114,10 +114,11 @@ __device__ __forceinline__ uint32_t read_of_cta(const uint32_t* p, uint32_t cta)
   return v;
 }
 
-// Lanes of the warp with the same digit of `bits` bits, of those that are there.
-__device__ __forceinline__ uint32_t same_digit(uint32_t d, int bits, bool there) {
+// Lanes of the warp with the same digit, of those that are there.  (__match_any_sync takes as many steps as there are digits.)
+__device__ __forceinline__ uint32_t same_digit(uint32_t d, bool there) {
   uint32_t same = __ballot_sync(0xffffffffu, there);
-  for (int b = 0; b < bits; ++b) {
+#pragma unroll
+  for (int b = 0; b < SORT_DIGIT; ++b) {
     const uint32_t set = __ballot_sync(0xffffffffu, d >> b & 1u);
     same &= d >> b & 1u ? set : ~set;
   }
@@ -136,7 +137,7 @@ __device__ __forceinline__ void give_to_cta(uint2* p, uint32_t cta, uint2 v) {
 // number of passes, and in `b` after an odd one.
 template <typename I, bool SMALL>
 __global__ void __launch_bounds__(SORT_THREADS)
-sort_tokens_kernel(const I* __restrict__ tokens, int n, int V, long long padding, Digits digits, uint2* a, uint2* b, uint8_t* met) {
+sort_tokens_kernel(const I* __restrict__ tokens, int n, int V, long long padding, Digits digits, uint2* a, uint2* b, uint8_t* met, int* longs) {
   extern __shared__ uint4 s_memory[];
   uint32_t* const s_count = reinterpret_cast<uint32_t*>(s_memory);         // [SORT_WARPS][SORT_BINS]
   uint2* const s_pairs = reinterpret_cast<uint2*>(s_count + SORT_WARPS * SORT_BINS);
@@ -157,6 +158,7 @@ sort_tokens_kernel(const I* __restrict__ tokens, int n, int V, long long padding
 #pragma unroll
   for (int k = 0; k < SORT_KEEP; ++k) kept[k] = from + 32 * k + lane < to ? key_of(from + 32 * k + lane) : make_uint2(0u, 0u);
   for (long long i = cta * SORT_THREADS + tid; i < (V + 15ll) / 16; i += ctas * SORT_THREADS) reinterpret_cast<uint4*>(met)[i] = make_uint4(0u, 0u, 0u, 0u);
+  if (cta == 0 && tid == 0) *longs = 0;
   const uint2* in = nullptr;
   uint2* out = b;
   int shift = 0;
@@ -170,7 +172,7 @@ sort_tokens_kernel(const I* __restrict__ tokens, int n, int V, long long padding
       return in ? __ldcg(in + i) : key_of(i);
     };
     const auto count = [&](uint2 p, bool there) {
-      const uint32_t d = p.x >> shift & mask, same = same_digit(d, bits, there);
+      const uint32_t d = p.x >> shift & mask, same = same_digit(d, there);
       if (there && (same & lower) == 0u) mine[d] += __popc(same);
       __syncwarp();
       return same;
@@ -246,7 +248,7 @@ sort_tokens_kernel(const I* __restrict__ tokens, int n, int V, long long padding
       for (long long i = from + 32 * SORT_KEEP; i < to; i += 32) {
         const uint2 p = pair_at(i + lane);
         const bool there = i + lane < to;
-        place(p, same_digit(p.x >> shift & mask, bits, there), there);
+        place(p, same_digit(p.x >> shift & mask, there), there);
       }
     __syncwarp();
     cluster_sync_all();                          // the pairs are there, and the totals have been read
@@ -261,17 +263,20 @@ sort_tokens_kernel(const I* __restrict__ tokens, int n, int V, long long padding
   }
 }
 
+// A segment that fills the chunk behind the one that it begins in; of the first one of the list, `token` is their number.
+struct Long { int token, chunk, pieces, unused; };
+
 // Sums of a chunk, 16 bytes of columns per thread in pieces of N values; behind the blocks of the sums those that zero rows.
 template <typename T, int N>
 __global__ void __launch_bounds__(SUM_THREADS)
 sum_rows_kernel(const uint2* __restrict__ pairs, int n, const T* __restrict__ dy, long long pitch, int V, int H, int Hp, float scale,
-                const uint8_t* __restrict__ met, T* __restrict__ dtable, float* __restrict__ partial, int slices, long long sum_blocks,
-                int zero_rows) {
+                const uint8_t* __restrict__ met, T* __restrict__ dtable, float* __restrict__ partial, Long* __restrict__ longs, int slices,
+                long long sum_blocks, int zero_rows) {
   using P = Piece<T, N>;
   constexpr int PIECES = 16 / sizeof(P), STEP = SUM_THREADS * N;
   __shared__ uint2 s_pair[2 * CHUNK + 1];
+  pdl_launch_next();
   pdl_wait();
-  pdl_launch_next();                             // what the next kernel reads before it waits has been there before this one
   const int tid = threadIdx.x, lane = tid & 31;
   if (blockIdx.x >= sum_blocks) {
     // a warp a row: the values in front of the first 16-byte boundary, whole words, the values behind the last
@@ -319,6 +324,15 @@ sum_rows_kernel(const uint2* __restrict__ pairs, int n, const T* __restrict__ dy
     to = min(to, from + __popc(__ballot_sync(0xffffffffu, from + lane < here && key(from + lane) < static_cast<uint32_t>(V))));
     open = false;
   }
+  if (open && slice == 0 && !(goes_on && all_one)) {
+    // a long segment begins here: how many chunks it takes (those that it fills, and this one)
+    int pieces = 1;
+    for (int more = SUM_THREADS; more == SUM_THREADS; pieces += more) {
+      const long long end = base + static_cast<long long>(pieces + tid + 1) * CHUNK;
+      more = __syncthreads_count(end <= n && pairs[end - 1].x == last);
+    }
+    if (tid == 0) longs[1 + atomicAdd(&longs->token, 1)] = {static_cast<int>(last), chunk, pieces, 0};
+  }
   const int col = slice * STEP * PIECES + tid * N;
   if (col >= H) return;
   float sum[PIECES][N] = {};
@@ -358,71 +372,39 @@ sum_rows_kernel(const uint2* __restrict__ pairs, int n, const T* __restrict__ dy
     for (int j = 0; j < N; ++j) if (col + c * STEP < H) to_part[c * STEP + j] = sum[c][j];
 }
 
-// Segments that fill the chunk behind the one that they begin in: their pieces are that chunk and all that they fill.
+// The pieces of long segments, in whatever order these were noted: a segment's own pieces are added up in their order.
 template <typename T>
 __global__ void __launch_bounds__(JOIN_THREADS)
-join_rows_kernel(const uint2* __restrict__ pairs, int n, int V, int H, int Hp, float scale, const float* __restrict__ partial,
-                 T* __restrict__ dtable) {
-  __shared__ int s_first[JOIN_THREADS];
-  __shared__ int s_warp[JOIN_THREADS / 32];
+join_rows_kernel(const Long* __restrict__ longs, int H, int Hp, float scale, const float* __restrict__ partial, T* __restrict__ dtable) {
   __shared__ float4 s_sum[JOIN_THREADS / 32][32];
   pdl_launch_next();
-  // the sorted pairs were there before the kernel of the sums began, which this one may start beside
-  const int tid = threadIdx.x, lane = tid & 31, w = tid >> 5;
-  const int full = n / CHUNK;                    // chunks that a segment can fill
-  const auto last_of = [&](long long chunk) { return pairs[chunk * CHUNK + CHUNK - 1].x; };
-  const int col = blockIdx.y * JOIN_COLS + lane * 4;
-  unsigned seen = 0;
-  for (int c0 = 0; c0 + 1 < full; c0 += JOIN_THREADS) {
-    const int c = c0 + tid;
-    bool begins = false;
-    if (c + 1 < full) {
-      const uint32_t k = last_of(c);
-      begins = k < static_cast<uint32_t>(V) && last_of(c + 1) == k && (c == 0 || last_of(c - 1) != k);
+  pdl_wait();
+  const int lane = threadIdx.x & 31, w = threadIdx.x >> 5, col = blockIdx.y * JOIN_COLS + lane * 4, count = longs->token;
+  for (int i = blockIdx.x; i < count; i += gridDim.x) {
+    const Long segment = longs[1 + i];
+    float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (col < Hp) {
+      const float* from = partial + static_cast<long long>(segment.chunk) * Hp + col;
+#pragma unroll 8
+      for (int r = w; r < segment.pieces; r += JOIN_THREADS / 32) {
+        const float4 p = *reinterpret_cast<const float4*>(from + static_cast<long long>(r) * Hp);
+        sum.x += p.x; sum.y += p.y; sum.z += p.z; sum.w += p.w;
+      }
     }
-    const unsigned flags = __ballot_sync(0xffffffffu, begins);
-    if (lane == 0) s_warp[w] = __popc(flags);
+    s_sum[w][lane] = sum;
     __syncthreads();
-    int before = 0, count = 0;
-    for (int i = 0; i < JOIN_THREADS / 32; ++i) { if (i < w) before += s_warp[i]; count += s_warp[i]; }
-    if (begins) s_first[before + __popc(flags & ((1u << lane) - 1u))] = c;
-    __syncthreads();
-    for (int i = 0; i < count; ++i) {
-      if ((seen + i) % gridDim.x != blockIdx.x) continue;
-      const int begin = s_first[i];
-      const uint32_t k = last_of(begin);
-      int pieces = 1;
-      for (int more = JOIN_THREADS; more == JOIN_THREADS; pieces += more) {
-        const int at = begin + pieces + tid;
-        more = __syncthreads_count(at < full && last_of(at) == k);
-      }
-      pdl_wait();
-      float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
-      if (col < Hp) {
-#pragma unroll 4
-        for (int r = w; r < pieces; r += JOIN_THREADS / 32) {
-          const float4 p = *reinterpret_cast<const float4*>(partial + static_cast<long long>(begin + r) * Hp + col);
-          sum.x += p.x; sum.y += p.y; sum.z += p.z; sum.w += p.w;
-        }
-      }
-      s_sum[w][lane] = sum;
-      __syncthreads();
-      if (w == 0) {
+    if (w == 0) {
 #pragma unroll
-        for (int g = 1; g < JOIN_THREADS / 32; ++g) {
-          const float4 p = s_sum[g][lane];
-          sum.x += p.x; sum.y += p.y; sum.z += p.z; sum.w += p.w;
-        }
-        const float v[4] = {sum.x, sum.y, sum.z, sum.w};
-#pragma unroll
-        for (int g = 0; g < 4; ++g) if (col + g < H) dtable[static_cast<long long>(k) * H + col + g] = from_float<T>(v[g] * scale);
+      for (int g = 1; g < JOIN_THREADS / 32; ++g) {
+        const float4 p = s_sum[g][lane];
+        sum.x += p.x; sum.y += p.y; sum.z += p.z; sum.w += p.w;
       }
-      __syncthreads();
+      const float v[4] = {sum.x, sum.y, sum.z, sum.w};
+#pragma unroll
+      for (int g = 0; g < 4; ++g) if (col + g < H) dtable[static_cast<long long>(segment.token) * H + col + g] = from_float<T>(v[g] * scale);
     }
-    seen += count;
     __syncthreads();
   }
-  pdl_wait();                                    // this kernel's end stands for the sums' too
 }
 
 // ------------------------------------------------------------------------------------------------------------------------ launches
@@ -453,18 +435,19 @@ static int look_up(const void* tokens, long long n, const void* table, long long
 }
 
 struct GradWork {
-  long long chunks, Hp, met, pairs, words;       // words before `met`: none; pairs of 2 words begin behind it
+  long long chunks, Hp, met, pairs, longs, words;       // met, two lists of pairs, longs and partial sums lie behind one another
   GradWork(long long n, int V, int H) {
     chunks = (n + CHUNK - 1) / CHUNK;
     Hp = (H + 3) / 4 * 4;
     met = (V + 15ll) / 16 * 4;                   // a byte for every token
     pairs = (2 * n + 3) / 4 * 4;
-    words = met + 2 * pairs + (chunks > 1 ? chunks * Hp : 0);
+    longs = 4 * (1 + n / (2 * CHUNK));           // each fills a chunk, and begins in another
+    words = met + 2 * pairs + longs + (chunks > 1 ? chunks * Hp : 0);
   }
 };
 
 template <typename I>
-static int sort_tokens(const void* tokens, int n, int V, long long padding, uint2* a, uint2* b, uint8_t* met, Digits& digits, cudaStream_t s) {
+static int sort_tokens(const void* tokens, int n, int V, long long padding, uint2* a, uint2* b, uint8_t* met, Digits& digits, int* longs, cudaStream_t s) {
   int bits = 0;
   while (V >> bits) ++bits;                      // V itself is the key of tokens without a gradient
   digits.passes = (bits + SORT_DIGIT - 1) / SORT_DIGIT;
@@ -485,20 +468,20 @@ static int sort_tokens(const void* tokens, int n, int V, long long padding, uint
   attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[1].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr; cfg.numAttrs = max_ctas() == 0 ? 2 : 1;
-  AXB_CUDA(cudaLaunchKernelEx(&cfg, kernel, static_cast<const I*>(tokens), n, V, padding, digits, a, b, met));
+  AXB_CUDA(cudaLaunchKernelEx(&cfg, kernel, static_cast<const I*>(tokens), n, V, padding, digits, a, b, met, longs));
   return 0;
 }
 
 template <typename T, int N>
 static int sum_rows(const uint2* pairs, int n, const void* dy, long long pitch, int V, int H, const GradWork& work, float scale,
-                    const uint8_t* met, void* dtable, float* partial, cudaStream_t s) {
+                    const uint8_t* met, void* dtable, float* partial, Long* longs, cudaStream_t s) {
   const int slices = (H + SUM_THREADS * 16 / static_cast<int>(sizeof(T)) - 1) / (SUM_THREADS * 16 / static_cast<int>(sizeof(T)));
   const int row_bytes = H * static_cast<int>(sizeof(T));
   const int zero_rows = row_bytes >= ZERO_BYTES ? 1 : ZERO_BYTES / row_bytes;
   const long long sum_blocks = work.chunks * slices, blocks = sum_blocks + (V + static_cast<long long>(zero_rows) - 1) / zero_rows;
   if (blocks > 0x7fffffffll) { set_error("gradient of an embedding: %d tokens with rows of %d values are too many blocks", n, H); return -1; }
   AXB_CUDA(pdl_launch(sum_rows_kernel<T, N>, dim3(static_cast<unsigned>(blocks)), dim3(SUM_THREADS), 0, s, pairs, n, static_cast<const T*>(dy),
-                      pitch, V, H, static_cast<int>(work.Hp), scale, met, static_cast<T*>(dtable), partial, slices, sum_blocks, zero_rows));
+                      pitch, V, H, static_cast<int>(work.Hp), scale, met, static_cast<T*>(dtable), partial, longs, slices, sum_blocks, zero_rows));
   return 0;
 }
 
@@ -511,20 +494,21 @@ static int gradient(const void* tokens, int token_bytes, int n, const void* dy, 
   }
   const GradWork work(n, V, H);
   uint2 *a = reinterpret_cast<uint2*>(words + work.met), *b = reinterpret_cast<uint2*>(words + work.met + work.pairs);
-  float* partial = reinterpret_cast<float*>(words + work.met + 2 * work.pairs);
+  Long* longs = reinterpret_cast<Long*>(words + work.met + 2 * work.pairs);
+  float* partial = reinterpret_cast<float*>(words + work.met + 2 * work.pairs + work.longs);
   Digits digits;
   uint8_t* met = reinterpret_cast<uint8_t*>(words);
-  if (token_bytes == 8 ? sort_tokens<long long>(tokens, n, V, padding, a, b, met, digits, s)
-                       : sort_tokens<int>(tokens, n, V, padding, a, b, met, digits, s)) return -1;
+  if (token_bytes == 8 ? sort_tokens<long long>(tokens, n, V, padding, a, b, met, digits, &longs->token, s)
+                       : sort_tokens<int>(tokens, n, V, padding, a, b, met, digits, &longs->token, s)) return -1;
   const uint2* pairs = n > SORT_SMALL && digits.passes % 2 ? b : a;
   const int size = sizeof(T), bytes = piece_bytes(size, {address(dy), address(dtable), static_cast<unsigned long long>(H) * size,
                                                          static_cast<unsigned long long>(pitch) * size});
   const auto sums = bytes == 16 ? sum_rows<T, 16 / sizeof(T)> : bytes == 8 ? sum_rows<T, 8 / sizeof(T)> : bytes == 4 ? sum_rows<T, 4 / sizeof(T)>
                                                                                                                      : sum_rows<T, 1>;
-  if (sums(pairs, n, dy, pitch, V, H, work, scale, met, dtable, partial, s)) return -1;
+  if (sums(pairs, n, dy, pitch, V, H, work, scale, met, dtable, partial, longs, s)) return -1;
   if (n < 2 * CHUNK) return 0;
   AXB_CUDA(pdl_launch(join_rows_kernel<T>, dim3(n / CHUNK / 2 < JOIN_BLOCKS ? n / CHUNK / 2 : JOIN_BLOCKS, static_cast<unsigned>((work.Hp + JOIN_COLS - 1) / JOIN_COLS)), dim3(JOIN_THREADS), 0, s,
-                      pairs, n, V, H, static_cast<int>(work.Hp), scale, static_cast<const float*>(partial), static_cast<T*>(dtable)));
+                      static_cast<const Long*>(longs), H, static_cast<int>(work.Hp), scale, static_cast<const float*>(partial), static_cast<T*>(dtable)));
   return 0;
 }
 
