@@ -17,8 +17,8 @@
 
 namespace axb {
 
-constexpr int SORT_THREADS = 1024, SORT_WARPS = SORT_THREADS / 32, SORT_DIGIT = 9, SORT_BINS = 1 << SORT_DIGIT;
-constexpr int SORT_CTAS = 8, SORT_KEEP = 4;       // pairs of a thread that stay in registers
+constexpr int SORT_THREADS = 512, SORT_WARPS = SORT_THREADS / 32, SORT_DIGIT = 9, SORT_BINS = 1 << SORT_DIGIT;
+constexpr int SORT_CTAS = 16, SORT_KEEP = 4;      // KEEP: pairs of a thread that stay in registers
 constexpr int SORT_SHARE = SORT_THREADS * SORT_KEEP, SORT_SMALL = SORT_CTAS * SORT_SHARE;
 constexpr int SORT_ALONE = 2 * SORT_THREADS;      // tokens that one CTA sorts
 constexpr int SORT_SMEM = SORT_WARPS * SORT_BINS * 4, SORT_SMEM_SMALL = SORT_SMEM + 2 * SORT_SHARE * 8;
@@ -26,7 +26,7 @@ constexpr int CHUNK = 32;                     // pairs of a block of sums: a war
 constexpr int SUM_THREADS = 128, SUM_AHEAD = 8;
 constexpr int ZERO_BYTES = 1 << 17;           // of the table, of a block that zeroes
 constexpr int JOIN_THREADS = 256, JOIN_COLS = 128, JOIN_BLOCKS = 64;
-constexpr int ROW_THREADS = 256, ROW_AHEAD = 4;
+constexpr int ROW_THREADS = 256, ROW_AHEAD = 2, ROW_BLOCKS = 8;
 
 template <typename T> __device__ __forceinline__ float to_float(T x) {
   if constexpr (__is_same(T, float)) return x;
@@ -44,15 +44,16 @@ template <typename T, int N> struct alignas(sizeof(T) * N) Piece { T v[N]; };
 
 // ------------------------------------------------------------------------------------------------------------------------ lookup
 // `group` threads (a power of two) a row, ROWS rows for each of them at a time, 16 bytes of each in pieces of N values.  Tokens are read a
-// step ahead.
+// step ahead.  `beside` the sorting of the same tokens, which lets this kernel begin when all work before both has ended, it does not wait
+// for that.
 template <typename T, typename I, int N, int ROWS>
-__global__ void __launch_bounds__(ROW_THREADS)
+__global__ void __launch_bounds__(ROW_THREADS, ROW_BLOCKS)
 embedding_kernel(const I* __restrict__ tokens, long long n, const T* __restrict__ table, long long pitch, int V, int H, float scale,
-                 T* __restrict__ out, int group) {
+                 T* __restrict__ out, int group, bool beside) {
   using P = Piece<T, N>;
   constexpr int PIECES = 16 / sizeof(P);
   pdl_launch_next();
-  pdl_wait();
+  if (!beside) pdl_wait();
   const int groups = ROW_THREADS / group, at = threadIdx.x & (group - 1);
   long long first = (static_cast<long long>(blockIdx.x) * groups + threadIdx.x / group) * ROWS;
   const long long step = static_cast<long long>(gridDim.x) * groups * ROWS;
@@ -97,6 +98,7 @@ embedding_kernel(const I* __restrict__ tokens, long long n, const T* __restrict_
       }
     }
   }
+  if (beside) pdl_wait();                        // this kernel's end stands for the sorting kernel's too
 }
 
 // ------------------------------------------------------------------------------------------------------------------------ gradient
@@ -125,6 +127,8 @@ __device__ __forceinline__ uint32_t same_digit(uint32_t d, bool there) {
   return same;
 }
 
+__device__ __forceinline__ void cluster_arrive_relaxed() { asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory"); }
+__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.aligned;" ::: "memory"); }
 __device__ __forceinline__ void give_to_cta(uint2* p, uint32_t cta, uint2 v) {
   uint32_t addr;
   asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(addr) : "r"(smem_u32(p)), "r"(cta));
@@ -137,28 +141,27 @@ __device__ __forceinline__ void give_to_cta(uint2* p, uint32_t cta, uint2 v) {
 // number of passes, and in `b` after an odd one.
 template <typename I, bool SMALL>
 __global__ void __launch_bounds__(SORT_THREADS)
-sort_tokens_kernel(const I* __restrict__ tokens, int n, int V, long long padding, Digits digits, uint2* a, uint2* b, uint8_t* met, int* longs) {
+sort_tokens_kernel(const I* __restrict__ tokens, int n, int V, long long padding, Digits digits, uint2* a, uint2* b, uint8_t* met) {
   extern __shared__ uint4 s_memory[];
   uint32_t* const s_count = reinterpret_cast<uint32_t*>(s_memory);         // [SORT_WARPS][SORT_BINS]
   uint2* const s_pairs = reinterpret_cast<uint2*>(s_count + SORT_WARPS * SORT_BINS);
   __shared__ uint32_t s_total[SORT_BINS], s_base[SORT_BINS], s_warp[SORT_BINS / 32];
-  pdl_launch_next();
   pdl_wait();
+  pdl_launch_next();                             // the lookup beside this reads what was there before
   const int tid = threadIdx.x, lane = tid & 31, w = tid >> 5;
   const uint32_t cta = cluster_cta_rank(), ctas = cluster_ctas(), lower = (1u << lane) - 1u;
-  const long long warps = static_cast<long long>(ctas) * SORT_WARPS, run = ((n + warps - 1) / warps + 31) / 32 * 32;
-  const long long from = (static_cast<long long>(cta) * SORT_WARPS + w) * run, to = min(from + run, static_cast<long long>(n));
-  const uint32_t share = static_cast<uint32_t>(run) * SORT_WARPS;          // pairs of a CTA (SMALL)
+  // n is below 2^31, and what is added to it below 2^14: unsigned numbers do
+  const uint32_t end = n, warps = ctas * SORT_WARPS, run = ((end + warps - 1u) / warps + 31u) / 32u * 32u;
+  const uint32_t from = (cta * SORT_WARPS + w) * run, to = min(from + run, end), share = run * SORT_WARPS;      // share: of a CTA
   uint32_t* mine = s_count + w * SORT_BINS;
-  const auto key_of = [&](long long i) {
+  const auto key_of = [&](uint32_t i) {
     const long long t = tokens[i];
-    return make_uint2(t >= 0 && t < V && t != padding ? static_cast<uint32_t>(t) : static_cast<uint32_t>(V), static_cast<uint32_t>(i));
+    return make_uint2(t >= 0 && t < V && t != padding ? static_cast<uint32_t>(t) : static_cast<uint32_t>(V), i);
   };
   uint2 kept[SORT_KEEP];
 #pragma unroll
   for (int k = 0; k < SORT_KEEP; ++k) kept[k] = from + 32 * k + lane < to ? key_of(from + 32 * k + lane) : make_uint2(0u, 0u);
-  for (long long i = cta * SORT_THREADS + tid; i < (V + 15ll) / 16; i += ctas * SORT_THREADS) reinterpret_cast<uint4*>(met)[i] = make_uint4(0u, 0u, 0u, 0u);
-  if (cta == 0 && tid == 0) *longs = 0;
+  for (uint32_t i = cta * SORT_THREADS + tid; i < (V + 15u) / 16u; i += ctas * SORT_THREADS) reinterpret_cast<uint4*>(met)[i] = make_uint4(0u, 0u, 0u, 0u);
   const uint2* in = nullptr;
   uint2* out = b;
   int shift = 0;
@@ -167,7 +170,7 @@ sort_tokens_kernel(const I* __restrict__ tokens, int n, int V, long long padding
     const uint32_t mask = bins - 1u;
     const bool last = pass + 1 == digits.passes;
     uint32_t kept_same[SORT_KEEP];
-    const auto pair_at = [&](long long i) {
+    const auto pair_at = [&](uint32_t i) {
       if (i >= to) return make_uint2(0u, 0u);
       return in ? __ldcg(in + i) : key_of(i);
     };
@@ -187,7 +190,12 @@ sort_tokens_kernel(const I* __restrict__ tokens, int n, int V, long long padding
         if (last && p.x < static_cast<uint32_t>(V)) met[p.x] = 1;          // of equal tokens, all write the same
         if (!SMALL) out[at] = p;
         else if (last) a[at] = p;
-        else give_to_cta(s_pairs + (pass & 1) * SORT_SHARE + at % share, at / share, p);
+        else {
+          uint32_t to_cta = 0u;
+#pragma unroll
+          for (uint32_t k = 1; k < SORT_CTAS; ++k) to_cta += at >= k * share;
+          give_to_cta(s_pairs + (pass & 1) * SORT_SHARE + at - to_cta * share, to_cta, p);
+        }
       }
       __syncwarp();
     };
@@ -201,16 +209,17 @@ sort_tokens_kernel(const I* __restrict__ tokens, int n, int V, long long padding
     for (int k = 0; k < SORT_KEEP; ++k)
       if (from + 32 * k < to) kept_same[k] = count(kept[k], from + 32 * k + lane < to);
     if (!SMALL)
-      for (long long i = from + 32 * SORT_KEEP; i < to; i += 32) count(pair_at(i + lane), i + lane < to);
+      for (uint32_t i = from + 32 * SORT_KEEP; i < to; i += 32) count(pair_at(i + lane), i + lane < to);
     __syncthreads();
     // counts of the warps before, then those of the CTAs before and of the smaller digits
     if (tid < bins) {
-      uint32_t sum = 0u;
+      uint32_t of[SORT_WARPS], sum = 0u;
+#pragma unroll
+      for (int k = 0; k < SORT_WARPS; ++k) of[k] = s_count[k * SORT_BINS + tid];
 #pragma unroll
       for (int k = 0; k < SORT_WARPS; ++k) {
-        const uint32_t c = s_count[k * SORT_BINS + tid];
         s_count[k * SORT_BINS + tid] = sum;
-        sum += c;
+        sum += of[k];
       }
       s_total[tid] = sum;
     }
@@ -241,18 +250,23 @@ sort_tokens_kernel(const I* __restrict__ tokens, int n, int V, long long padding
       s_base[tid] = upto - all + before;
     }
     __syncthreads();
+    if (last) cluster_arrive_relaxed();          // this CTA has read the others' totals; nobody reads what it stores from here on
 #pragma unroll
     for (int k = 0; k < SORT_KEEP; ++k)
       if (from + 32 * k < to) place(kept[k], kept_same[k], from + 32 * k + lane < to);
     if (!SMALL)
-      for (long long i = from + 32 * SORT_KEEP; i < to; i += 32) {
+      for (uint32_t i = from + 32 * SORT_KEEP; i < to; i += 32) {
         const uint2 p = pair_at(i + lane);
         const bool there = i + lane < to;
         place(p, same_digit(p.x >> shift & mask, there), there);
       }
     __syncwarp();
+    if (last) {
+      cluster_wait();                            // no CTA ends before its totals have been read
+      return;
+    }
     cluster_sync_all();                          // the pairs are there, and the totals have been read
-    if (SMALL && !last) {
+    if (SMALL) {
 #pragma unroll
       for (int k = 0; k < SORT_KEEP; ++k)
         if (from + 32 * k + lane < to) kept[k] = s_pairs[(pass & 1) * SORT_SHARE + w * run + 32 * k + lane];
@@ -263,14 +277,11 @@ sort_tokens_kernel(const I* __restrict__ tokens, int n, int V, long long padding
   }
 }
 
-// A segment that fills the chunk behind the one that it begins in; of the first one of the list, `token` is their number.
-struct Long { int token, chunk, pieces, unused; };
-
 // Sums of a chunk, 16 bytes of columns per thread in pieces of N values; behind the blocks of the sums those that zero rows.
 template <typename T, int N>
 __global__ void __launch_bounds__(SUM_THREADS)
 sum_rows_kernel(const uint2* __restrict__ pairs, int n, const T* __restrict__ dy, long long pitch, int V, int H, int Hp, float scale,
-                const uint8_t* __restrict__ met, T* __restrict__ dtable, float* __restrict__ partial, Long* __restrict__ longs, int slices,
+                const uint8_t* __restrict__ met, T* __restrict__ dtable, float* __restrict__ partial, int* __restrict__ pieces, int slices,
                 long long sum_blocks, int zero_rows) {
   using P = Piece<T, N>;
   constexpr int PIECES = 16 / sizeof(P), STEP = SUM_THREADS * N;
@@ -318,21 +329,24 @@ sum_rows_kernel(const uint2* __restrict__ pairs, int n, const T* __restrict__ dy
     if (all_one) open = true;
     else from = __ffs(~__ballot_sync(0xffffffffu, lane < here && key(lane) == first)) - 1;
   }
-  if (from >= here || key(from) >= static_cast<uint32_t>(V)) return;
   // tokens without a gradient are the last ones
   if (last >= static_cast<uint32_t>(V)) {
     to = min(to, from + __popc(__ballot_sync(0xffffffffu, from + lane < here && key(from + lane) < static_cast<uint32_t>(V))));
     open = false;
   }
-  if (open && slice == 0 && !(goes_on && all_one)) {
-    // a long segment begins here: how many chunks it takes (those that it fills, and this one)
-    int pieces = 1;
-    for (int more = SUM_THREADS; more == SUM_THREADS; pieces += more) {
-      const long long end = base + static_cast<long long>(pieces + tid + 1) * CHUNK;
-      more = __syncthreads_count(end <= n && pairs[end - 1].x == last);
+  if (slice == 0) {
+    // of a long segment that begins here: how many chunks it takes, this one and those that it fills
+    int count = 0;
+    if (open && !(goes_on && all_one)) {
+      count = 1;
+      for (int more = SUM_THREADS; more == SUM_THREADS; count += more) {
+        const long long end = base + static_cast<long long>(count + tid + 1) * CHUNK;
+        more = __syncthreads_count(end <= n && pairs[end - 1].x == last);
+      }
     }
-    if (tid == 0) longs[1 + atomicAdd(&longs->token, 1)] = {static_cast<int>(last), chunk, pieces, 0};
+    if (tid == 0) pieces[chunk] = count;
   }
+  if (from >= to) return;
   const int col = slice * STEP * PIECES + tid * N;
   if (col >= H) return;
   float sum[PIECES][N] = {};
@@ -372,37 +386,56 @@ sum_rows_kernel(const uint2* __restrict__ pairs, int n, const T* __restrict__ dy
     for (int j = 0; j < N; ++j) if (col + c * STEP < H) to_part[c * STEP + j] = sum[c][j];
 }
 
-// The pieces of long segments, in whatever order these were noted: a segment's own pieces are added up in their order.
+// The pieces of long segments, in their order.
 template <typename T>
 __global__ void __launch_bounds__(JOIN_THREADS)
-join_rows_kernel(const Long* __restrict__ longs, int H, int Hp, float scale, const float* __restrict__ partial, T* __restrict__ dtable) {
+join_rows_kernel(const uint2* __restrict__ pairs, const int* __restrict__ pieces, int chunks, int H, int Hp, float scale,
+                 const float* __restrict__ partial, T* __restrict__ dtable) {
+  __shared__ int2 s_begin[JOIN_THREADS];         // chunk, pieces
+  __shared__ int s_warp[JOIN_THREADS / 32];
   __shared__ float4 s_sum[JOIN_THREADS / 32][32];
   pdl_launch_next();
   pdl_wait();
-  const int lane = threadIdx.x & 31, w = threadIdx.x >> 5, col = blockIdx.y * JOIN_COLS + lane * 4, count = longs->token;
-  for (int i = blockIdx.x; i < count; i += gridDim.x) {
-    const Long segment = longs[1 + i];
-    float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
-    if (col < Hp) {
-      const float* from = partial + static_cast<long long>(segment.chunk) * Hp + col;
-#pragma unroll 8
-      for (int r = w; r < segment.pieces; r += JOIN_THREADS / 32) {
-        const float4 p = *reinterpret_cast<const float4*>(from + static_cast<long long>(r) * Hp);
-        sum.x += p.x; sum.y += p.y; sum.z += p.z; sum.w += p.w;
-      }
-    }
-    s_sum[w][lane] = sum;
+  const int tid = threadIdx.x, lane = tid & 31, w = tid >> 5, col = blockIdx.y * JOIN_COLS + lane * 4;
+  unsigned seen = 0;
+  for (int c0 = 0; c0 < chunks; c0 += JOIN_THREADS) {
+    const int own = c0 + tid < chunks ? pieces[c0 + tid] : 0;
+    const unsigned flags = __ballot_sync(0xffffffffu, own > 0);
+    if (lane == 0) s_warp[w] = __popc(flags);
     __syncthreads();
-    if (w == 0) {
+    int before = 0, count = 0;
 #pragma unroll
-      for (int g = 1; g < JOIN_THREADS / 32; ++g) {
-        const float4 p = s_sum[g][lane];
-        sum.x += p.x; sum.y += p.y; sum.z += p.z; sum.w += p.w;
+    for (int i = 0; i < JOIN_THREADS / 32; ++i) { if (i < w) before += s_warp[i]; count += s_warp[i]; }
+    if (own > 0) s_begin[before + __popc(flags & ((1u << lane) - 1u))] = make_int2(c0 + tid, own);
+    __syncthreads();
+    // every gridDim.x-th of all
+    for (int i = static_cast<int>((blockIdx.x + gridDim.x - seen % gridDim.x) % gridDim.x); i < count; i += gridDim.x) {
+      const int2 begin = s_begin[i];
+      const uint32_t token = pairs[static_cast<long long>(begin.x) * CHUNK + CHUNK - 1].x;
+      float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
+      if (col < Hp) {
+        const float* from = partial + static_cast<long long>(begin.x) * Hp + col;
+#pragma unroll 8
+        for (int r = w; r < begin.y; r += JOIN_THREADS / 32) {
+          const float4 p = *reinterpret_cast<const float4*>(from + static_cast<long long>(r) * Hp);
+          sum.x += p.x; sum.y += p.y; sum.z += p.z; sum.w += p.w;
+        }
       }
-      const float v[4] = {sum.x, sum.y, sum.z, sum.w};
+      s_sum[w][lane] = sum;
+      __syncthreads();
+      if (w == 0) {
 #pragma unroll
-      for (int g = 0; g < 4; ++g) if (col + g < H) dtable[static_cast<long long>(segment.token) * H + col + g] = from_float<T>(v[g] * scale);
+        for (int g = 1; g < JOIN_THREADS / 32; ++g) {
+          const float4 p = s_sum[g][lane];
+          sum.x += p.x; sum.y += p.y; sum.z += p.z; sum.w += p.w;
+        }
+        const float v[4] = {sum.x, sum.y, sum.z, sum.w};
+#pragma unroll
+        for (int g = 0; g < 4; ++g) if (col + g < H) dtable[static_cast<long long>(token) * H + col + g] = from_float<T>(v[g] * scale);
+      }
+      __syncthreads();
     }
+    seen += count;
     __syncthreads();
   }
 }
@@ -418,47 +451,60 @@ static int piece_bytes(int value, std::initializer_list<unsigned long long> of) 
 static unsigned long long address(const void* p) { return reinterpret_cast<unsigned long long>(p); }
 
 template <typename T, typename I, int N>
-static int look_up(const void* tokens, long long n, const void* table, long long pitch, int V, int H, float scale, void* out, cudaStream_t s) {
+static int look_up(const void* tokens, long long n, const void* table, long long pitch, int V, int H, float scale, void* out, bool beside,
+                   cudaStream_t s) {
   constexpr int COUNT = 16 / sizeof(T);
   const int words = (H + COUNT - 1) / COUNT;
   int group = 32;
   while (group < ROW_THREADS && group < words) group *= 2;
   const int groups = ROW_THREADS / group;
   // several rows at a time where there are blocks enough for all SMs without
-  const long long room = 2048ll / ROW_THREADS * sm_count_current();
+  const long long room = static_cast<long long>(ROW_BLOCKS) * sm_count_current();
   const bool ahead = n / groups >= room * ROW_AHEAD;
   const long long per = static_cast<long long>(groups) * (ahead ? ROW_AHEAD : 1), blocks = (n + per - 1) / per;
   AXB_CUDA(pdl_launch(ahead ? embedding_kernel<T, I, N, ROW_AHEAD> : embedding_kernel<T, I, N, 1>, dim3(static_cast<unsigned>(blocks < room ? blocks : room)),
                       dim3(ROW_THREADS), 0, s, static_cast<const I*>(tokens), n, static_cast<const T*>(table), pitch, V, H, scale,
-                      static_cast<T*>(out), group));
+                      static_cast<T*>(out), group, beside));
   return 0;
 }
 
-struct GradWork {
-  long long chunks, Hp, met, pairs, longs, words;       // met, two lists of pairs, longs and partial sums lie behind one another
-  GradWork(long long n, int V, int H) {
-    chunks = (n + CHUNK - 1) / CHUNK;
-    Hp = (H + 3) / 4 * 4;
-    met = (V + 15ll) / 16 * 4;                   // a byte for every token
+// What the gradient needs of the tokens: a byte for every token of the table, and the sorted pairs (a second list for many: they take turns).
+struct Sorted {
+  long long met, pairs, words;
+  Sorted(long long n, int V) {
+    met = (V + 15ll) / 16 * 4;
     pairs = (2 * n + 3) / 4 * 4;
-    longs = 4 * (1 + n / (2 * CHUNK));           // each fills a chunk, and begins in another
-    words = met + 2 * pairs + longs + (chunks > 1 ? chunks * Hp : 0);
+    words = met + (n > SORT_SMALL ? 2 : 1) * pairs;
   }
 };
+// Bits of the passes; V itself is the key of tokens without a gradient.
+static Digits digits_of(int V) {
+  Digits d = {};
+  int bits = 0;
+  while (V >> bits) ++bits;
+  d.passes = (bits + SORT_DIGIT - 1) / SORT_DIGIT;
+  for (int i = 0, left = bits; i < d.passes; ++i) {
+    d.bits[i] = (left + d.passes - i - 1) / (d.passes - i);
+    left -= d.bits[i];
+  }
+  return d;
+}
+static const uint2* sorted_pairs(const void* sorted, long long n, int V) {
+  const Sorted at(n, V);
+  const uint32_t* words = static_cast<const uint32_t*>(sorted);
+  return reinterpret_cast<const uint2*>(words + at.met + (n > SORT_SMALL && digits_of(V).passes % 2 ? at.pairs : 0));
+}
 
 template <typename I>
-static int sort_tokens(const void* tokens, int n, int V, long long padding, uint2* a, uint2* b, uint8_t* met, Digits& digits, int* longs, cudaStream_t s) {
-  int bits = 0;
-  while (V >> bits) ++bits;                      // V itself is the key of tokens without a gradient
-  digits.passes = (bits + SORT_DIGIT - 1) / SORT_DIGIT;
-  for (int i = 0, left = bits; i < digits.passes; ++i) {
-    digits.bits[i] = (left + digits.passes - i - 1) / (digits.passes - i);
-    left -= digits.bits[i];
-  }
+static int sort_tokens(const void* tokens, int n, int V, long long padding, void* sorted, cudaStream_t s) {
+  const Sorted at(n, V);
+  uint32_t* words = static_cast<uint32_t*>(sorted);
+  uint2 *a = reinterpret_cast<uint2*>(words + at.met), *b = reinterpret_cast<uint2*>(words + at.met + (n > SORT_SMALL ? at.pairs : 0));
   const bool small = n <= SORT_SMALL;
   const auto kernel = small ? sort_tokens_kernel<I, true> : sort_tokens_kernel<I, false>;
   const int smem = small ? SORT_SMEM_SMALL : SORT_SMEM;
   AXB_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+  AXB_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
   cudaLaunchConfig_t cfg = {};
   const unsigned ctas = n <= SORT_ALONE ? 1 : SORT_CTAS;
   cfg.gridDim = dim3(ctas); cfg.blockDim = dim3(SORT_THREADS); cfg.dynamicSmemBytes = smem; cfg.stream = s;
@@ -468,60 +514,65 @@ static int sort_tokens(const void* tokens, int n, int V, long long padding, uint
   attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[1].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr; cfg.numAttrs = max_ctas() == 0 ? 2 : 1;
-  AXB_CUDA(cudaLaunchKernelEx(&cfg, kernel, static_cast<const I*>(tokens), n, V, padding, digits, a, b, met, longs));
+  AXB_CUDA(cudaLaunchKernelEx(&cfg, kernel, static_cast<const I*>(tokens), n, V, padding, digits_of(V), a, b, reinterpret_cast<uint8_t*>(words)));
   return 0;
 }
 
+// Partial sums of the chunks, and how many chunks the segments take that begin in them.
+struct GradWork {
+  long long chunks, Hp, pieces, words;
+  GradWork(long long n, int H) {
+    chunks = (n + CHUNK - 1) / CHUNK;
+    Hp = (H + 3) / 4 * 4;
+    pieces = (chunks + 3) / 4 * 4;
+    words = pieces + (chunks > 1 ? chunks * Hp : 0);
+  }
+};
+
 template <typename T, int N>
-static int sum_rows(const uint2* pairs, int n, const void* dy, long long pitch, int V, int H, const GradWork& work, float scale,
-                    const uint8_t* met, void* dtable, float* partial, Long* longs, cudaStream_t s) {
-  const int slices = (H + SUM_THREADS * 16 / static_cast<int>(sizeof(T)) - 1) / (SUM_THREADS * 16 / static_cast<int>(sizeof(T)));
+static int sum_rows(const void* sorted, int n, const void* dy, long long pitch, int V, int H, float scale, void* dtable, int* words, cudaStream_t s) {
+  const GradWork work(n, H);
+  const int columns = SUM_THREADS * 16 / static_cast<int>(sizeof(T)), slices = (H + columns - 1) / columns;
   const int row_bytes = H * static_cast<int>(sizeof(T));
   const int zero_rows = row_bytes >= ZERO_BYTES ? 1 : ZERO_BYTES / row_bytes;
   const long long sum_blocks = work.chunks * slices, blocks = sum_blocks + (V + static_cast<long long>(zero_rows) - 1) / zero_rows;
   if (blocks > 0x7fffffffll) { set_error("gradient of an embedding: %d tokens with rows of %d values are too many blocks", n, H); return -1; }
+  const uint2* pairs = sorted_pairs(sorted, n, V);
+  float* partial = reinterpret_cast<float*>(words + work.pieces);
   AXB_CUDA(pdl_launch(sum_rows_kernel<T, N>, dim3(static_cast<unsigned>(blocks)), dim3(SUM_THREADS), 0, s, pairs, n, static_cast<const T*>(dy),
-                      pitch, V, H, static_cast<int>(work.Hp), scale, met, static_cast<T*>(dtable), partial, longs, slices, sum_blocks, zero_rows));
+                      pitch, V, H, static_cast<int>(work.Hp), scale, static_cast<const uint8_t*>(sorted), static_cast<T*>(dtable), partial, words,
+                      slices, sum_blocks, zero_rows));
+  if (n < 2 * CHUNK) return 0;
+  const int full = n / CHUNK;                    // a long segment fills one chunk and begins in another
+  AXB_CUDA(pdl_launch(join_rows_kernel<T>, dim3(full / 2 < JOIN_BLOCKS ? full / 2 : JOIN_BLOCKS, static_cast<unsigned>((work.Hp + JOIN_COLS - 1) / JOIN_COLS)),
+                      dim3(JOIN_THREADS), 0, s, pairs, static_cast<const int*>(words), full, H, static_cast<int>(work.Hp), scale,
+                      static_cast<const float*>(partial), static_cast<T*>(dtable)));
   return 0;
 }
 
 template <typename T>
-static int gradient(const void* tokens, int token_bytes, int n, const void* dy, long long pitch, int V, int H, float scale, long long padding,
-                    void* dtable, uint32_t* words, cudaStream_t s) {
+static int gradient(const void* sorted, int n, const void* dy, long long pitch, int V, int H, float scale, void* dtable, int* work, cudaStream_t s) {
   if (n == 0) {
     AXB_CUDA(cudaMemsetAsync(dtable, 0, static_cast<size_t>(V) * H * sizeof(T), s));
     return 0;
   }
-  const GradWork work(n, V, H);
-  uint2 *a = reinterpret_cast<uint2*>(words + work.met), *b = reinterpret_cast<uint2*>(words + work.met + work.pairs);
-  Long* longs = reinterpret_cast<Long*>(words + work.met + 2 * work.pairs);
-  float* partial = reinterpret_cast<float*>(words + work.met + 2 * work.pairs + work.longs);
-  Digits digits;
-  uint8_t* met = reinterpret_cast<uint8_t*>(words);
-  if (token_bytes == 8 ? sort_tokens<long long>(tokens, n, V, padding, a, b, met, digits, &longs->token, s)
-                       : sort_tokens<int>(tokens, n, V, padding, a, b, met, digits, &longs->token, s)) return -1;
-  const uint2* pairs = n > SORT_SMALL && digits.passes % 2 ? b : a;
   const int size = sizeof(T), bytes = piece_bytes(size, {address(dy), address(dtable), static_cast<unsigned long long>(H) * size,
                                                          static_cast<unsigned long long>(pitch) * size});
   const auto sums = bytes == 16 ? sum_rows<T, 16 / sizeof(T)> : bytes == 8 ? sum_rows<T, 8 / sizeof(T)> : bytes == 4 ? sum_rows<T, 4 / sizeof(T)>
                                                                                                                      : sum_rows<T, 1>;
-  if (sums(pairs, n, dy, pitch, V, H, work, scale, met, dtable, partial, longs, s)) return -1;
-  if (n < 2 * CHUNK) return 0;
-  AXB_CUDA(pdl_launch(join_rows_kernel<T>, dim3(n / CHUNK / 2 < JOIN_BLOCKS ? n / CHUNK / 2 : JOIN_BLOCKS, static_cast<unsigned>((work.Hp + JOIN_COLS - 1) / JOIN_COLS)), dim3(JOIN_THREADS), 0, s,
-                      static_cast<const Long*>(longs), H, static_cast<int>(work.Hp), scale, static_cast<const float*>(partial), static_cast<T*>(dtable)));
-  return 0;
+  return sums(sorted, n, dy, pitch, V, H, scale, dtable, work, s);
 }
 
 template <typename T>
 static int look_up_by(const void* tokens, int token_bytes, long long n, const void* table, long long pitch, int V, int H, float scale, void* out,
-                      cudaStream_t s) {
+                      bool beside, cudaStream_t s) {
   const int size = sizeof(T), bytes = piece_bytes(size, {address(table), address(out), static_cast<unsigned long long>(H) * size,
                                                          static_cast<unsigned long long>(pitch) * size});
   const auto go = [&](auto index) {
     using I = decltype(index);
     const auto kernel = bytes == 16 ? look_up<T, I, 16 / sizeof(T)> : bytes == 8 ? look_up<T, I, 8 / sizeof(T)>
                       : bytes == 4 ? look_up<T, I, 4 / sizeof(T)> : look_up<T, I, 1>;
-    return kernel(tokens, n, table, pitch, V, H, scale, out, s);
+    return kernel(tokens, n, table, pitch, V, H, scale, out, beside, s);
   };
   return token_bytes == 8 ? go(0ll) : go(0);
 }
@@ -535,22 +586,31 @@ static int refused(const char* what, long long n, int V, int H, int dtype, int t
   set_error("%s: %lld tokens of %d bytes, table %d x %d of type %d", what, n, token_bytes, V, H, dtype);
   return -1;
 }
-
-extern "C" int axb_embedding(const void* tokens, int token_bytes, long long n, const void* table, long long pitch, int V, int H, float scale,
-                             void* out, int dtype, void* stream) {
-  if (refused("embedding", n, V, H, dtype, token_bytes)) return -1;
-  if (n == 0) return 0;
-  const auto go = dtype == 0 ? look_up_by<__nv_bfloat16> : dtype == 1 ? look_up_by<__half> : look_up_by<float>;
-  return go(tokens, token_bytes, n, table, pitch, V, H, scale, out, static_cast<cudaStream_t>(stream));
+static int misaligned(const char* what, const void* p) {
+  if (address(p) % 16 == 0) return 0;
+  set_error("%s: the workspace must be 16-byte aligned", what);
+  return -1;
 }
 
-extern "C" long long axb_embedding_grad_words(long long n, int V, int H) { return GradWork(n, V, H).words; }
+extern "C" long long axb_embedding_sorted_words(long long n, int V) { return Sorted(n, V).words; }
 
-extern "C" int axb_embedding_grad(const void* tokens, int token_bytes, long long n, const void* dy, long long pitch, int V, int H, float scale,
-                                  long long padding, void* dtable, void* work, int dtype, void* stream) {
-  if (refused("gradient of an embedding", n, V, H, dtype, token_bytes)) return -1;
-  if (address(work) % 16) { set_error("gradient of an embedding: the workspace must be 16-byte aligned"); return -1; }
+extern "C" int axb_embedding(const void* tokens, int token_bytes, long long n, const void* table, long long pitch, int V, int H, float scale,
+                             void* out, long long padding, void* sorted, int dtype, void* stream) {
+  if (refused("embedding", n, V, H, dtype, token_bytes) || misaligned("embedding", sorted)) return -1;
+  if (n == 0) return 0;
+  const cudaStream_t s = static_cast<cudaStream_t>(stream);
+  if (sorted && (token_bytes == 8 ? sort_tokens<long long>(tokens, static_cast<int>(n), V, padding, sorted, s)
+                                  : sort_tokens<int>(tokens, static_cast<int>(n), V, padding, sorted, s))) return -1;
+  const auto go = dtype == 0 ? look_up_by<__nv_bfloat16> : dtype == 1 ? look_up_by<__half> : look_up_by<float>;
+  return go(tokens, token_bytes, n, table, pitch, V, H, scale, out, sorted != nullptr && max_ctas() == 0, s);
+}
+
+extern "C" long long axb_embedding_grad_words(long long n, int H) { return GradWork(n, H).words; }
+
+extern "C" int axb_embedding_grad(const void* sorted, long long n, const void* dy, long long pitch, int V, int H, float scale, void* dtable,
+                                  void* work, int dtype, void* stream) {
+  if (refused("gradient of an embedding", n, V, H, dtype, 8) || misaligned("gradient of an embedding", work) ||
+      misaligned("gradient of an embedding", sorted)) return -1;
   const auto go = dtype == 0 ? gradient<__nv_bfloat16> : dtype == 1 ? gradient<__half> : gradient<float>;
-  return go(tokens, token_bytes, static_cast<int>(n), dy, pitch, V, H, scale, padding, dtable, static_cast<uint32_t*>(work),
-            static_cast<cudaStream_t>(stream));
+  return go(sorted, static_cast<int>(n), dy, pitch, V, H, scale, dtable, static_cast<int*>(work), static_cast<cudaStream_t>(stream));
 }

@@ -41,7 +41,7 @@ using std::optional;
   X(axb_cached_attention_words, attention_words) X(axb_cached_attention, cached_attention) \
   X(axb_beam_select_words, beam_words) X(axb_beam_select, beam_select) \
   X(axb_token_log_probs, token_log_probs) X(axb_token_log_probs_bwd, token_log_probs_bwd) \
-  X(axb_embedding, embedding) X(axb_embedding_grad_words, embedding_grad_words) X(axb_embedding_grad, embedding_grad)
+  X(axb_embedding_sorted_words, embedding_sorted_words) X(axb_embedding, embedding) X(axb_embedding_grad_words, embedding_grad_words) X(axb_embedding_grad, embedding_grad)
 #define AXB_DECLARE(symbol, name) decltype(&::symbol) name = nullptr;
 AXB_LAUNCHERS(AXB_DECLARE)
 PyObject *kernel_error = nullptr, *parameter_type = nullptr;
@@ -614,56 +614,61 @@ PyObject* py_token_log_probs(PyObject*, PyObject* const* a, Py_ssize_t n) {
 // ---------------------------------------------------------------------------------------------------------------- table lookup
 int index_bytes(const Tensor& tokens) { return tokens.scalar_type() == at::kLong ? 8 : tokens.scalar_type() == at::kInt ? 4 : 0; }
 
-Tensor run_embedding(const Tensor& tokens, const Tensor& weight, double scale) {
+// With `sorted` also what the gradient needs of the tokens.
+Tensor run_embedding(const Tensor& tokens, const Tensor& weight, double scale, int64_t padding = -1, Tensor* sorted = nullptr) {
   const Tensor t = tokens.contiguous(), w = weight.stride(1) != 1 && weight.size(1) != 1 ? weight.contiguous() : weight;
+  const int V = static_cast<int>(w.size(0)), H = static_cast<int>(w.size(1));
   c10::SmallVector<int64_t, 5> shape(t.sizes().begin(), t.sizes().end());
-  shape.push_back(w.size(1));
+  shape.push_back(H);
   const Tensor out = at::empty(shape, w.options());
+  if (sorted) *sorted = at::empty({embedding_sorted_words(t.numel(), V)}, w.options().dtype(at::kInt));
   if (out.numel())
-    check(embedding(t.data_ptr(), index_bytes(t), t.numel(), w.data_ptr(), w.stride(0), static_cast<int>(w.size(0)), static_cast<int>(w.size(1)),
-                    static_cast<float>(scale), out.data_ptr(), dtype_code(w), stream()), "axb_embedding");
+    check(embedding(t.data_ptr(), index_bytes(t), t.numel(), w.data_ptr(), w.stride(0), V, H, static_cast<float>(scale), out.data_ptr(), padding,
+                    sorted ? sorted->data_ptr() : nullptr, dtype_code(w), stream()), "axb_embedding", sorted ? 2 : 1);
   return out;
 }
-Tensor run_embedding_grad(const Tensor& tokens, const Tensor& dy, int64_t V, double scale, int64_t padding) {
+Tensor run_embedding_grad(const Tensor& sorted, const Tensor& dy, int64_t V, double scale) {
   const int64_t H = dy.size(-1);
-  const Tensor t = tokens.contiguous();
   Tensor rows = dy.reshape({-1, H});
   if (rows.stride(1) != 1 && H != 1) rows = rows.contiguous();
-  const int64_t n = t.numel();
-  const Tensor out = at::empty({V, H}, rows.options());
-  const Tensor work = at::empty({embedding_grad_words(n, static_cast<int>(V), static_cast<int>(H))}, rows.options().dtype(at::kInt));
-  check(embedding_grad(t.data_ptr(), index_bytes(t), n, rows.data_ptr(), rows.stride(0), static_cast<int>(V), static_cast<int>(H),
-                       static_cast<float>(scale), padding, out.data_ptr(), work.data_ptr(), dtype_code(rows), stream()), "axb_embedding_grad",
-        n == 0 ? 0 : n < 64 ? 2 : 3);
+  const int64_t n = rows.size(0);
+  const Tensor out = at::empty({V, H}, rows.options()), by = sorted.contiguous();
+  const Tensor work = at::empty({embedding_grad_words(n, static_cast<int>(H))}, rows.options().dtype(at::kInt));
+  check(embedding_grad(by.data_ptr(), n, rows.data_ptr(), rows.stride(0), static_cast<int>(V), static_cast<int>(H), static_cast<float>(scale),
+                       out.data_ptr(), work.data_ptr(), dtype_code(rows), stream()), "axb_embedding_grad", n == 0 ? 0 : n < 64 ? 1 : 2);
   return out;
 }
 
 // The gradient of the table as a function of that of the rows; and its own: rows of the table that it is asked with.
 struct EmbeddingGradNode : torch::autograd::Function<EmbeddingGradNode> {
-  static Tensor forward(torch::autograd::AutogradContext* ctx, const Tensor& tokens, const Tensor& dy, int64_t V, double scale, int64_t padding);
+  static Tensor forward(torch::autograd::AutogradContext* ctx, const Tensor& tokens, const Tensor& sorted, const Tensor& dy, int64_t V, double scale,
+                        int64_t padding);
   static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx, torch::autograd::variable_list grads);
 };
 struct EmbeddingNode : torch::autograd::Function<EmbeddingNode> {
   static Tensor forward(torch::autograd::AutogradContext* ctx, const Tensor& tokens, const Tensor& weight, double scale, int64_t padding) {
-    ctx->save_for_backward({tokens});
+    Tensor sorted;
+    const Tensor out = run_embedding(tokens, weight, scale, padding, &sorted);
+    ctx->save_for_backward({tokens, sorted});
     ctx->saved_data["V"] = weight.size(0);
     ctx->saved_data["scale"] = scale;
     ctx->saved_data["padding"] = padding;
-    return run_embedding(tokens, weight, scale);
+    return out;
   }
   static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx, torch::autograd::variable_list grads) {
-    const Tensor tokens = ctx->get_saved_variables()[0];
+    const auto saved = ctx->get_saved_variables();
     const int64_t V = ctx->saved_data["V"].toInt(), padding = ctx->saved_data["padding"].toInt();
     const double scale = ctx->saved_data["scale"].toDouble();
-    return {Tensor(), wants_grad(grads[0]) ? EmbeddingGradNode::apply(tokens, grads[0], V, scale, padding)
-                                           : run_embedding_grad(tokens, grads[0], V, scale, padding), Tensor(), Tensor()};
+    return {Tensor(), wants_grad(grads[0]) ? EmbeddingGradNode::apply(saved[0], saved[1], grads[0], V, scale, padding)
+                                           : run_embedding_grad(saved[1], grads[0], V, scale), Tensor(), Tensor()};
   }
 };
-Tensor EmbeddingGradNode::forward(torch::autograd::AutogradContext* ctx, const Tensor& tokens, const Tensor& dy, int64_t V, double scale, int64_t padding) {
+Tensor EmbeddingGradNode::forward(torch::autograd::AutogradContext* ctx, const Tensor& tokens, const Tensor& sorted, const Tensor& dy, int64_t V,
+                                  double scale, int64_t padding) {
   ctx->save_for_backward({tokens});
   ctx->saved_data["scale"] = scale;
   ctx->saved_data["padding"] = padding;
-  return run_embedding_grad(tokens, dy, V, scale, padding);
+  return run_embedding_grad(sorted, dy, V, scale);
 }
 torch::autograd::variable_list EmbeddingGradNode::backward(torch::autograd::AutogradContext* ctx, torch::autograd::variable_list grads) {
   const Tensor tokens = ctx->get_saved_variables()[0], &table = grads[0];
@@ -671,7 +676,7 @@ torch::autograd::variable_list EmbeddingGradNode::backward(torch::autograd::Auto
   const Tensor none = tokens.lt(0).logical_or(tokens.ge(table.size(0))).logical_or(tokens.eq(ctx->saved_data["padding"].toInt()));
   const Tensor there = tokens.masked_fill(none, 0);
   const Tensor rows = wants_grad(table) ? EmbeddingNode::apply(there, table, scale, static_cast<int64_t>(-1)) : run_embedding(there, table, scale);
-  return {Tensor(), rows.masked_fill(none.unsqueeze(-1), 0), Tensor(), Tensor(), Tensor()};
+  return {Tensor(), Tensor(), rows.masked_fill(none.unsqueeze(-1), 0), Tensor(), Tensor(), Tensor()};
 }
 
 // embedding(tokens, weight [V, H], scale, padding | -1) -> weight[tokens] * scale or None

@@ -33,7 +33,7 @@ _HOST = _UNSET = object()
 _HOST_LAUNCHERS = ("axb_norm_fwd", "axb_norm_bwd", "axb_add_norm_fwd", "axb_add_norm_bwd", "axb_norm_grid", "axb_gemm",
                    "axb_flash_attn_fwd", "axb_last_error", "axb_plan_blocks", "axb_store_blocks", "axb_reorder_blocks",
                    "axb_cached_attention_words", "axb_cached_attention", "axb_beam_select_words", "axb_beam_select", "axb_token_log_probs",
-                   "axb_token_log_probs_bwd", "axb_embedding", "axb_embedding_grad_words", "axb_embedding_grad")
+                   "axb_token_log_probs_bwd", "axb_embedding_sorted_words", "axb_embedding", "axb_embedding_grad_words", "axb_embedding_grad")
 
 
 def __getattr__(name):
@@ -92,9 +92,10 @@ _SIGNATURES = {
     "axb_beam_select": "ppp" "i" "ppppp" "iiii" "p",
     "axb_token_log_probs": "p" "ll" "p" "ll" "ppppp" "iii" "ll" "i" "f" "l" "ii" "p",
     "axb_token_log_probs_bwd": "p" "ll" "p" "ll" "pppppp" "iii" "ll" "i" "f" "l" "i" "p",
-    "axb_embedding": "p" "i" "l" "p" "l" "ii" "f" "p" "i" "p",
-    "axb_embedding_grad_words": "l" "ii",
-    "axb_embedding_grad": "p" "i" "l" "p" "l" "ii" "f" "l" "pp" "i" "p",
+    "axb_embedding_sorted_words": "l" "i",
+    "axb_embedding": "p" "i" "l" "p" "l" "ii" "f" "p" "l" "p" "i" "p",
+    "axb_embedding_grad_words": "l" "i",
+    "axb_embedding_grad": "p" "l" "p" "l" "ii" "f" "pp" "i" "p",
 }
 # Switches of kernels that are gone.  The one kernel that is left covers what they selected; a program that still sets
 # one is told so instead of being ignored.
@@ -126,7 +127,8 @@ def lib():
             for name, sig in _SIGNATURES.items():
                 if hasattr(L, name):
                     getattr(L, name).argtypes = [_CTYPES[c] for c in sig]
-            for name in ("axb_flash_attn_bwd_scratch", "axb_cached_attention_words", "axb_beam_select_words", "axb_embedding_grad_words"):
+            for name in ("axb_flash_attn_bwd_scratch", "axb_cached_attention_words", "axb_beam_select_words", "axb_embedding_sorted_words",
+                         "axb_embedding_grad_words"):
                 if hasattr(L, name):
                     getattr(L, name).restype = ctypes.c_longlong
             ms = os.environ.get("AXONN_COMM_TIMEOUT_MS")

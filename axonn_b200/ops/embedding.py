@@ -44,7 +44,7 @@ def embedding(tokens, weight, scale=1.0, padding_idx=None):
         with torch.cuda.device(weight.device):
             return embedding(tokens, weight, scale, padding_idx)
     if no_graph(weight):
-        return _rows(tokens, weight, scale)
+        return _rows(tokens, weight, scale)[0]
     return _EmbeddingFn.apply(tokens, weight, scale, -1 if padding_idx is None else padding_idx)
 
 
@@ -53,57 +53,58 @@ def _torch(tokens, weight, scale, padding_idx):
     return out if scale == 1.0 else (out.float() * scale).to(weight.dtype)
 
 
-def _rows(tokens, weight, scale):
+def _rows(tokens, weight, scale, padding=-1, sort=False):
+    """``weight[tokens] * scale``; with ``sort`` also what the gradient needs of the tokens."""
     weight = weight.detach()
     if weight.shape[1] > 1 and weight.stride(1) != 1:
         weight = weight.contiguous()
-    tokens = tokens.contiguous()
-    out = torch.empty(*tokens.shape, weight.shape[1], dtype=weight.dtype, device=weight.device)
+    tokens, (V, H), L = tokens.contiguous(), weight.shape, _lib.lib()
+    out = torch.empty(*tokens.shape, H, dtype=weight.dtype, device=weight.device)
+    sorted_ = torch.empty(L.axb_embedding_sorted_words(tokens.numel(), V), dtype=torch.int32, device=weight.device) if sort else None
     if out.numel():
-        st = _lib.lib().axb_embedding(tokens.data_ptr(), _INDEX[tokens.dtype], tokens.numel(), weight.data_ptr(), weight.stride(0), *weight.shape, scale,
-                                      out.data_ptr(), _DT[weight.dtype], _lib.stream())
+        st = L.axb_embedding(tokens.data_ptr(), _INDEX[tokens.dtype], tokens.numel(), weight.data_ptr(), weight.stride(0), V, H, scale, out.data_ptr(),
+                             padding, _lib.addr(sorted_), _DT[weight.dtype], _lib.stream())
         _lib.check(st, "axb_embedding")
-    return out
+        _lib.add_launches(int(sort))
+    return out, sorted_
 
 
-def _table_gradient(tokens, dy, V, scale, padding):
+def _table_gradient(sorted_, dy, V, scale):
     """``dy [..., H]`` summed by token; the rows may have any stride."""
     H = dy.shape[-1]
     dy = dy.reshape(-1, H)
     if H > 1 and dy.stride(1) != 1:
         dy = dy.contiguous()
-    tokens = tokens.reshape(-1).contiguous()
-    n, L = tokens.numel(), _lib.lib()
+    n, L = dy.shape[0], _lib.lib()
     out = torch.empty(V, H, dtype=dy.dtype, device=dy.device)
-    work = torch.empty(L.axb_embedding_grad_words(n, V, H), dtype=torch.int32, device=dy.device)
-    st = L.axb_embedding_grad(tokens.data_ptr(), _INDEX[tokens.dtype], n, dy.data_ptr(), dy.stride(0), V, H, scale, padding, out.data_ptr(),
-                              work.data_ptr(), _DT[dy.dtype], _lib.stream())
+    work = torch.empty(L.axb_embedding_grad_words(n, H), dtype=torch.int32, device=dy.device)
+    st = L.axb_embedding_grad(sorted_.data_ptr(), n, dy.data_ptr(), dy.stride(0), V, H, scale, out.data_ptr(), work.data_ptr(), _DT[dy.dtype], _lib.stream())
     _lib.check(st, "axb_embedding_grad")
-    _lib.add_launches(-1 if n == 0 else 1 if n < 64 else 2)
+    _lib.add_launches(-1 if n == 0 else 0 if n < 64 else 1)
     return out
 
 
 class _EmbeddingFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, tokens, weight, scale, padding):
-        ctx.save_for_backward(tokens)
+        out, sorted_ = _rows(tokens, weight, scale, padding, True)
+        ctx.save_for_backward(tokens, sorted_)
         ctx.scale, ctx.padding, ctx.V = scale, padding, weight.shape[0]
-        return _rows(tokens, weight, scale)
+        return out
 
     @staticmethod
     def backward(ctx, dy):
-        (tokens,) = ctx.saved_tensors
-        return None, _EmbeddingGradFn.apply(tokens, dy, ctx.V, ctx.scale, ctx.padding), None, None
+        return None, _EmbeddingGradFn.apply(*ctx.saved_tensors, dy, ctx.V, ctx.scale, ctx.padding), None, None
 
 
 class _EmbeddingGradFn(torch.autograd.Function):
     """The gradient of the table as a function of that of the rows, and its own: rows of the table that it is asked with."""
 
     @staticmethod
-    def forward(ctx, tokens, dy, V, scale, padding):
+    def forward(ctx, tokens, sorted_, dy, V, scale, padding):
         ctx.save_for_backward(tokens)
         ctx.scale, ctx.padding = scale, padding
-        return _table_gradient(tokens, dy, V, scale, padding)
+        return _table_gradient(sorted_.contiguous(), dy, V, scale)
 
     @staticmethod
     def backward(ctx, d_table):
@@ -111,4 +112,4 @@ class _EmbeddingGradFn(torch.autograd.Function):
         V = d_table.shape[0]
         none = (tokens < 0) | (tokens >= V) | (tokens == ctx.padding)
         rows = embedding(tokens.masked_fill(none, 0), d_table, ctx.scale)
-        return None, rows.masked_fill(none[..., None], 0), None, None, None
+        return None, None, rows.masked_fill(none[..., None], 0), None, None, None
