@@ -13,6 +13,9 @@
 //      chunk: then its sum so far goes to the workspace.  A segment of any length so takes many blocks, and one of up to 32 pairs
 //      no extra traffic.
 //   3. The partial sums of long segments, which the blocks of the sums have noted, are joined in their order.
+#include <atomic>
+#include <initializer_list>
+
 #include "common.cuh"
 
 namespace axb {
@@ -503,8 +506,14 @@ static int sort_tokens(const void* tokens, int n, int V, long long padding, void
   const bool small = n <= SORT_SMALL;
   const auto kernel = small ? sort_tokens_kernel<I, true> : sort_tokens_kernel<I, false>;
   const int smem = small ? SORT_SMEM_SMALL : SORT_SMEM;
-  AXB_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
-  AXB_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
+  static std::atomic<bool> configured[64][2];    // set once per device: 3 us of host time otherwise
+  int device;
+  AXB_CUDA(cudaGetDevice(&device));
+  if (!configured[device & 63][small].load(std::memory_order_acquire)) {
+    AXB_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+    AXB_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
+    configured[device & 63][small].store(true, std::memory_order_release);
+  }
   cudaLaunchConfig_t cfg = {};
   const unsigned ctas = n <= SORT_ALONE ? 1 : SORT_CTAS;
   cfg.gridDim = dim3(ctas); cfg.blockDim = dim3(SORT_THREADS); cfg.dynamicSmemBytes = smem; cfg.stream = s;
