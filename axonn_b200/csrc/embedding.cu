@@ -21,8 +21,8 @@
 namespace axb {
 
 constexpr int SORT_THREADS = 512, SORT_WARPS = SORT_THREADS / 32, SORT_DIGIT = 9, SORT_BINS = 1 << SORT_DIGIT;
-constexpr int SORT_CTAS = 16, SORT_KEEP = 4;      // KEEP: pairs of a thread that stay in registers
-constexpr int SORT_SHARE = SORT_THREADS * SORT_KEEP, SORT_SMALL = SORT_CTAS * SORT_SHARE;
+constexpr int SORT_CTAS = 16, SORT_PORTABLE = 8, SORT_KEEP = 4;      // KEEP: pairs of a thread that stay in registers
+constexpr int SORT_SHARE = SORT_THREADS * SORT_KEEP;
 constexpr int SORT_ALONE = 2 * SORT_THREADS;      // tokens that one CTA sorts
 constexpr int SORT_SMEM = SORT_WARPS * SORT_BINS * 4, SORT_SMEM_SMALL = SORT_SMEM + 2 * SORT_SHARE * 8;
 constexpr int CHUNK = 32;                     // pairs of a block of sums: a warp's lanes look one chunk ahead
@@ -477,9 +477,45 @@ struct Sorted {
   Sorted(long long n, int V) {
     met = (V + 15ll) / 16 * 4;
     pairs = (2 * n + 3) / 4 * 4;
-    words = met + (n > SORT_SMALL ? 2 : 1) * pairs;
+    words = met + (n > SORT_PORTABLE * SORT_SHARE ? 2 : 1) * pairs;
   }
 };
+static cudaLaunchConfig_t sort_config(unsigned ctas, int smem, cudaStream_t s, cudaLaunchAttribute* attr) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(ctas); cfg.blockDim = dim3(SORT_THREADS); cfg.dynamicSmemBytes = smem; cfg.stream = s;
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = ctas; attr[0].val.clusterDim.y = 1; attr[0].val.clusterDim.z = 1;
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[1].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr; cfg.numAttrs = max_ctas() == 0 ? 2 : 1;
+  return cfg;
+}
+// CTAs of the cluster on the current device: 16 where it can run as many together (a part of a GPU may not), otherwise 8.  The kernels'
+// attributes are set along with it, once per device: 3 us of host time otherwise.  0: an error.
+static int sort_ctas() {
+  static std::atomic<int> known[64];
+  int device;
+  if (check_cuda(cudaGetDevice(&device), "cudaGetDevice")) return 0;
+  int ctas = known[device & 63].load(std::memory_order_acquire);
+  if (ctas) return ctas;
+  const auto set = [](auto kernel, int smem) {
+    return check_cuda(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem), "shared memory of the sorting kernel") ||
+           check_cuda(cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1), "cluster of the sorting kernel");
+  };
+  if (set(sort_tokens_kernel<long long, true>, SORT_SMEM_SMALL) || set(sort_tokens_kernel<int, true>, SORT_SMEM_SMALL) ||
+      set(sort_tokens_kernel<long long, false>, SORT_SMEM) || set(sort_tokens_kernel<int, false>, SORT_SMEM)) return 0;
+  cudaLaunchAttribute attr[2];
+  cudaLaunchConfig_t cfg = sort_config(SORT_CTAS, SORT_SMEM_SMALL, nullptr, attr);
+  cfg.numAttrs = 1;
+  int clusters = 0;
+  if (cudaOccupancyMaxActiveClusters(&clusters, sort_tokens_kernel<long long, true>, &cfg) != cudaSuccess) {
+    cudaGetLastError();
+    clusters = 0;
+  }
+  ctas = clusters > 0 ? SORT_CTAS : SORT_PORTABLE;
+  known[device & 63].store(ctas, std::memory_order_release);
+  return ctas;
+}
 // Bits of the passes; V itself is the key of tokens without a gradient.
 static Digits digits_of(int V) {
   Digits d = {};
@@ -492,37 +528,23 @@ static Digits digits_of(int V) {
   }
   return d;
 }
-static const uint2* sorted_pairs(const void* sorted, long long n, int V) {
+static const uint2* sorted_pairs(const void* sorted, long long n, int V, int ctas) {
   const Sorted at(n, V);
   const uint32_t* words = static_cast<const uint32_t*>(sorted);
-  return reinterpret_cast<const uint2*>(words + at.met + (n > SORT_SMALL && digits_of(V).passes % 2 ? at.pairs : 0));
+  return reinterpret_cast<const uint2*>(words + at.met + (n > ctas * SORT_SHARE && digits_of(V).passes % 2 ? at.pairs : 0));
 }
 
 template <typename I>
 static int sort_tokens(const void* tokens, int n, int V, long long padding, void* sorted, cudaStream_t s) {
+  const int most = sort_ctas();
+  if (!most) return -1;
   const Sorted at(n, V);
   uint32_t* words = static_cast<uint32_t*>(sorted);
-  uint2 *a = reinterpret_cast<uint2*>(words + at.met), *b = reinterpret_cast<uint2*>(words + at.met + (n > SORT_SMALL ? at.pairs : 0));
-  const bool small = n <= SORT_SMALL;
+  const bool small = n <= most * SORT_SHARE;
+  uint2 *a = reinterpret_cast<uint2*>(words + at.met), *b = small ? nullptr : reinterpret_cast<uint2*>(words + at.met + at.pairs);
   const auto kernel = small ? sort_tokens_kernel<I, true> : sort_tokens_kernel<I, false>;
-  const int smem = small ? SORT_SMEM_SMALL : SORT_SMEM;
-  static std::atomic<bool> configured[64][2];    // set once per device: 3 us of host time otherwise
-  int device;
-  AXB_CUDA(cudaGetDevice(&device));
-  if (!configured[device & 63][small].load(std::memory_order_acquire)) {
-    AXB_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
-    AXB_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
-    configured[device & 63][small].store(true, std::memory_order_release);
-  }
-  cudaLaunchConfig_t cfg = {};
-  const unsigned ctas = n <= SORT_ALONE ? 1 : SORT_CTAS;
-  cfg.gridDim = dim3(ctas); cfg.blockDim = dim3(SORT_THREADS); cfg.dynamicSmemBytes = smem; cfg.stream = s;
   cudaLaunchAttribute attr[2];
-  attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = ctas; attr[0].val.clusterDim.y = 1; attr[0].val.clusterDim.z = 1;
-  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[1].val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = attr; cfg.numAttrs = max_ctas() == 0 ? 2 : 1;
+  const cudaLaunchConfig_t cfg = sort_config(n <= SORT_ALONE ? 1 : most, small ? SORT_SMEM_SMALL : SORT_SMEM, s, attr);
   AXB_CUDA(cudaLaunchKernelEx(&cfg, kernel, static_cast<const I*>(tokens), n, V, padding, digits_of(V), a, b, reinterpret_cast<uint8_t*>(words)));
   return 0;
 }
@@ -546,7 +568,9 @@ static int sum_rows(const void* sorted, int n, const void* dy, long long pitch, 
   const int zero_rows = row_bytes >= ZERO_BYTES ? 1 : ZERO_BYTES / row_bytes;
   const long long sum_blocks = work.chunks * slices, blocks = sum_blocks + (V + static_cast<long long>(zero_rows) - 1) / zero_rows;
   if (blocks > 0x7fffffffll) { set_error("gradient of an embedding: %d tokens with rows of %d values are too many blocks", n, H); return -1; }
-  const uint2* pairs = sorted_pairs(sorted, n, V);
+  const int ctas = sort_ctas();
+  if (!ctas) return -1;
+  const uint2* pairs = sorted_pairs(sorted, n, V, ctas);
   float* partial = reinterpret_cast<float*>(words + work.pieces);
   AXB_CUDA(pdl_launch(sum_rows_kernel<T, N>, dim3(static_cast<unsigned>(blocks)), dim3(SUM_THREADS), 0, s, pairs, n, static_cast<const T*>(dy),
                       pitch, V, H, static_cast<int>(work.Hp), scale, static_cast<const uint8_t*>(sorted), static_cast<T*>(dtable), partial, words,

@@ -632,7 +632,7 @@ Tensor run_embedding_grad(const Tensor& sorted, const Tensor& dy, int64_t V, dou
   Tensor rows = dy.reshape({-1, H});
   if (rows.stride(1) != 1 && H != 1) rows = rows.contiguous();
   const int64_t n = rows.size(0);
-  const Tensor out = at::empty({V, H}, rows.options()), by = sorted.contiguous();
+  const Tensor out = at::empty({V, H}, rows.options()), by = dense(sorted);
   const Tensor work = at::empty({embedding_grad_words(n, static_cast<int>(H))}, rows.options().dtype(at::kInt));
   check(embedding_grad(by.data_ptr(), n, rows.data_ptr(), rows.stride(0), static_cast<int>(V), static_cast<int>(H), static_cast<float>(scale),
                        out.data_ptr(), work.data_ptr(), dtype_code(rows), stream()), "axb_embedding_grad", n == 0 ? 0 : n < 64 ? 1 : 2);

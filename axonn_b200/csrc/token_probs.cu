@@ -25,7 +25,13 @@ constexpr int TP_WORDS = 4;                // 16-byte words of a thread, of a ti
 constexpr int TP_KEEP = 64;                // entries that a list is cut down to, at most
 constexpr float TP_LOG2E = 1.4426950408889634f;
 constexpr double TP_LN2 = 0.6931471805599453;
-constexpr long long TP_NARROW = 8192, TP_MIDDLE = 32768;      // bytes of a row for blocks of 32 and 128 threads
+// Bytes of a row that a warp takes (four rows of 4096 values: 14.7 us with 5 alternatives for 16.4 with blocks of 128 threads; with 20,
+// 30 for 19) and that a block of 128 threads takes where there are few rows (one of 32,000 bf16 values, 5 alternatives: 6.9 us with
+// clusters of 256, 7.3 with those of 128).  Many rows always take 128: their last tile is emptier with 256 (8 x 2047 rows of 50,304 values
+// 221 us for 251).
+constexpr long long TP_NARROW = 8192, TP_MIDDLE = 32768;
+// Blocks per SM up to which rows are split over clusters, where alternatives are asked for: 64 rows of 128,256 values with 20 of them and a
+// part of the vocabulary masked 16.5 us, with 4 blocks 20.
 constexpr long long TP_ROOM = 2;
 constexpr float TP_FAR = -8192.f;          // exponents below are this: their powers are zero, and their products with them too
 
@@ -499,7 +505,10 @@ token_probs_kernel(const TokenProbsArgs a, int rows, float* log_probs, float* en
           }
         }
       }
-      if (++tiles >= 2 && (tiles & (tiles - 1)) == 0 && base + TILE < hi) over = bound_of(s_list, tp_key(st.m), K, turn ^= 1);
+      // anew after 2, 4, 8 ... tiles, where it saves more than it takes: 110 instructions of every warp, against some 35 of one for every
+      // word with values above the old bound, of which a tile has K / tiles (4096 rows of 32,000 values, one alternative: 61 us for 66)
+      if (++tiles >= 2 && (tiles & (tiles - 1)) == 0 && K * ((hi - base) / TILE) > WARPS * tiles)
+        over = bound_of(s_list, tp_key(st.m), K, turn ^= 1);
     }
     base += TILE;
   } while (base < hi);
@@ -519,20 +528,30 @@ token_probs_kernel(const TokenProbsArgs a, int rows, float* log_probs, float* en
     if (WARPS > 1) s_stats[tid >> 5] = st;
     if constexpr (TOP) s_list.filled[tid >> 5] = filled;
   }
-  if constexpr (TOP) over = bound_of(s_list, tp_key(most_of_thread), K, turn ^ 1);      // waits for all
-  else tp_sync<THREADS>();
+  tp_sync<THREADS>();
   if constexpr (WARPS > 1) {
     st = s_stats[lane & (WARPS - 1)];
     st = tp_join_lanes<WARPS>(st, c);
   }
   if constexpr (TOP) {
-    // entries that reach the bound: K at least, where the block has as many
     bool again = st.s != st.s;               // a NaN is missing, or what there was no room for
+    int few = 0, before = 0;
 #pragma unroll
-    for (int i = 0; i < WARPS; ++i) again |= s_list.filled[i] > List<THREADS>::SHARE;
-    if (!again) {
+    for (int i = 0; i < WARPS; ++i) {
+      const int n = s_list.filled[i];
+      again |= n > List<THREADS>::SHARE;
+      if (i < (tid >> 5)) before += n;
+      few += n;
+    }
+    const Entry* mine = s_list.entry + (tid >> 5) * List<THREADS>::SHARE;
+    if (!again && few <= TP_KEEP) {
+      for (int i = lane; i < filled; i += 32) s_list.some[before + i] = mine[i];
+      tp_sync<THREADS>();
+    } else if (!again) {
+      // those that reach a last bound: K at least, where the block has as many
+      over = bound_of(s_list, tp_key(most_of_thread), K, turn ^ 1);
       for (int i = 0; i < filled; i += 32) {
-        const Entry e = i + lane < filled ? s_list.entry[(tid >> 5) * List<THREADS>::SHARE + i + lane] : TP_NONE;
+        const Entry e = i + lane < filled ? mine[i + lane] : TP_NONE;
         const bool good = e != TP_NONE && static_cast<uint32_t>(e >> 32) >= over;
         const unsigned those = __ballot_sync(0xffffffffu, good);
         int at = 0;
@@ -541,15 +560,16 @@ token_probs_kernel(const TokenProbsArgs a, int rows, float* log_probs, float* en
         if (good && at < List<THREADS>::SOME) s_list.some[at] = e;
       }
       tp_sync<THREADS>();
-      again = s_list.few > List<THREADS>::SOME;
+      few = s_list.few;
+      again = few > List<THREADS>::SOME;
     }
     if (again) {
       gather_slowly<T, THREADS>(s_list, row, from, to, K);
-      if (tid == 0) s_list.few = s_list.count;
-      for (int i = tid; i < s_list.count; i += THREADS) s_list.some[i] = s_list.entry[i];
+      few = s_list.count;
+      for (int i = tid; i < few; i += THREADS) s_list.some[i] = s_list.entry[i];
       tp_sync<THREADS>();
     }
-    put_in_order(s_list, s_list.few, K);
+    put_in_order(s_list, few, K);
   }
   if constexpr (ROWS == 1) {
     if (ctas > 1) {

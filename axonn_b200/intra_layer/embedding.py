@@ -12,6 +12,10 @@ adds the token gradients into the owners' gradient shards with remote atomics
 (``csrc/p2p.cu``; ``AXONN_EMBEDDING_P2P=0`` keeps the gather).  For a 128256 x
 4096 table that replaces 1 GB of all-gather per forward and a 1 GB
 reduce-scatter per backward by the rows actually used.
+
+Otherwise rows are looked up by ``ops.embedding``: on GPUs the package's kernels,
+with the gradient by sorted tokens, unless the layer asks for what those do not do
+(``max_norm``, ``scale_grad_by_freq``, ``sparse``).
 """
 
 import torch
@@ -19,6 +23,7 @@ import torch.distributed as dist
 import torch.nn.functional as F
 
 from .. import axonn as ax
+from .. import ops
 from ..ops.direct import no_graph, own_forward, plain_layer
 from ..utils import divide
 from .communication import ForwardGather_BackwardReduceScatter, Gather, _gather
@@ -71,11 +76,12 @@ class Embedding(torch.nn.Module):
     """Drop-in ``nn.Embedding`` whose table is split along the embedding dimension over one tensor-parallel group
     (the outer group, or the inner one with ``transpose=True``) and flat-sharded over the depth group.  On GPUs
     with a depth group the needed rows are fetched from the owning ranks over peer memory instead of gathering
-    the table (reference ``axonn/intra_layer/embedding.py:57-222``)."""
+    the table (reference ``axonn/intra_layer/embedding.py:57-222``).  ``scale`` multiplies the rows, as models do that
+    scale them by the root of their width."""
 
     def __init__(self, num_embeddings, embedding_dim, padding_idx=None, max_norm=None, norm_type=2.0,
                  scale_grad_by_freq=False, sparse=False, _weight=None, _freeze=False, *args,
-                 transpose=False, init_method=None, expert_mode=False, dtype=None, **kwargs):
+                 transpose=False, init_method=None, expert_mode=False, dtype=None, scale=1.0, **kwargs):
         assert _weight is None, "_weight argument is not supported."
         super().__init__()
         assert ax.is_initialized
@@ -86,7 +92,7 @@ class Embedding(torch.nn.Module):
             if padding_idx < 0:
                 padding_idx += num_embeddings
         self.padding_idx, self.max_norm, self.norm_type = padding_idx, max_norm, norm_type
-        self.scale_grad_by_freq, self.sparse = scale_grad_by_freq, sparse
+        self.scale_grad_by_freq, self.sparse, self.scale = scale_grad_by_freq, sparse, scale
         ch = ax.comm_handle
         self.inner_group = ch.inner_intra_layer_parallel_group
         self.outer_group = ch.outer_intra_layer_parallel_group
@@ -147,17 +153,24 @@ class Embedding(torch.nn.Module):
         """``self(torch.arange(first, first + count, device=device))``.  Without gradients, collectives or hooks the rows are a
         slice of the table: two launches less for the positions of a short prompt (logits of a two-layer GPT 364 -> 351 us)."""
         w = self.weight
-        if (plain_layer(self) and self.depth_group_size == 1 and self.expert_mode and self.max_norm is None
+        if (plain_layer(self) and self.scale == 1.0 and self.depth_group_size == 1 and self.expert_mode and self.max_norm is None
                 and 0 <= first and first + count <= self.num_embeddings and no_graph(w) and w.device == torch.device(device)
                 and w.is_contiguous()):
             return w.detach().view(self.num_embeddings, self.local_out_features)[first:first + count]
-        return self(torch.arange(first, first + count, device=device))
+        ids = torch.arange(first, first + count, device=device)
+        # rows that the table has not got are refused as torch.nn.functional.embedding does it; the kernel would give NaN
+        return self(ids) if 0 <= first and first + count <= self.num_embeddings else self._look_up(ids, False)
 
     def forward(self, x):
+        return self._look_up(x, True)
+
+    def _look_up(self, x, kernels):
         if self._p2p_rows(x):
             x = _EmbeddingRowsP2P.apply(x, self.weight, self.depth_group,
                                         self.num_embeddings // self.depth_group_size, self.local_out_features,
                                         self.padding_idx)
+            if self.scale != 1.0:
+                x = x * self.scale
             if not self.expert_mode:
                 x = Gather.apply(x, self.hidden_group)
             return x
@@ -165,8 +178,14 @@ class Embedding(torch.nn.Module):
         if self.depth_group_size > 1 or not no_graph(weight):
             weight = ForwardGather_BackwardReduceScatter.apply(weight, self.depth_group)
         weight = weight.reshape(self.local_in_features, self.local_out_features)
-        x = F.embedding(x, weight, self.padding_idx, self.max_norm, self.norm_type,
-                        self.scale_grad_by_freq, self.sparse)
+        if (kernels and self.max_norm is None and not self.scale_grad_by_freq and not self.sparse
+                and weight.dtype in ops.EMBEDDING_TYPES):
+            x = ops.embedding(x, weight, self.scale, self.padding_idx)
+        else:
+            x = F.embedding(x, weight, self.padding_idx, self.max_norm, self.norm_type,
+                            self.scale_grad_by_freq, self.sparse)
+            if self.scale != 1.0:
+                x = x * self.scale
         if not self.expert_mode:
             x = Gather.apply(x, self.hidden_group)
         return x

@@ -1,4 +1,4 @@
-"""Greedy decoding and beam search with the tensor-parallel language models (inference through the same layers and kernels).
+"""Greedy decoding, beam search and scoring with the tensor-parallel language models (inference through the same layers and kernels).
 
 The reference runs inference by handing its patched Hugging Face models to ``generate``; the models of this
 package return logits whose vocabulary dimension is split over the ranks of ``model.head.group``, so choosing the
@@ -11,6 +11,8 @@ import torch.distributed as dist
 from .. import ops
 from ..intra_layer.communication import _gather
 from .cache import BlockCache
+
+_LEFT_OUT = -100
 
 
 @torch.no_grad()
@@ -31,8 +33,45 @@ def parallel_argmax(logits, group=None):
     return indices.gather(-1, best).squeeze(-1)
 
 
+def score_tokens(model, tokens, lengths=None, entropy=False, top=0, temperature=1.0):
+    """What ``model`` makes of given sequences: the ``ops.TokenLogProbs`` of ``tokens[:, 1:]`` (``tokens [B, S]``, int64), each after the
+    tokens in front of it, all of shape ``[B, S - 1]``.  Row ``r`` is ``tokens[r, :lengths[r]]`` (``None``: all of it); behind that the
+    results are zeros (alternatives -1).  With gradients enabled the results are functions of the model's parameters: a policy-gradient or
+    distillation loss is a sum of them.  Every rank of a tensor-parallel group passes the same ``tokens``."""
+    if tokens.ndim != 2 or tokens.dtype != torch.int64 or tokens.shape[1] < 2:
+        raise ValueError(f"sequences of two tokens and more are scored, int64 [B, S], not {tokens.dtype} {list(tokens.shape)}")
+    targets = tokens[:, 1:]
+    if lengths is not None:
+        lengths = torch.as_tensor(lengths, device=tokens.device)
+        if lengths.shape != tokens.shape[:1]:
+            raise ValueError(f"lengths must be {tokens.shape[0]} numbers, not {list(lengths.shape)}")
+        places = torch.arange(1, tokens.shape[1], device=tokens.device)
+        targets = targets.masked_fill(places >= lengths[:, None], _LEFT_OUT)
+    logits = model(tokens)                                                   # [B, S, vocab / |group|]
+    return ops.token_log_probs(logits[:, :-1], targets, entropy, top, temperature, getattr(model.head, "group", None), _LEFT_OUT)
+
+
+class _Told:
+    """Log-probabilities of the new tokens of a batch, step by step, with ``top`` alternatives."""
+
+    def __init__(self, top, group):
+        self.top, self.group, self.steps = top, group, []
+
+    def step(self, logits, tokens, done):
+        if done is not None:
+            tokens = tokens.masked_fill(done, _LEFT_OUT)
+        self.steps.append(ops.token_log_probs(logits, tokens, top=self.top, group=self.group, ignore_index=_LEFT_OUT))
+
+    def result(self, rows, device):
+        if self.steps:
+            return ops.TokenLogProbs(*(None if t[0] is None else torch.stack(t, 1) for t in zip(*self.steps)))
+        none = torch.empty(rows, 0, device=device)
+        best = none.new_empty(rows, 0, self.top) if self.top else None
+        return ops.TokenLogProbs(none, None, best, None if best is None else best.long())
+
+
 @torch.no_grad()
-def greedy_generate(model, tokens, max_new_tokens: int, eos_id=None, cache_dtype=None, prompt_lengths=None, block_tokens=64):
+def greedy_generate(model, tokens, max_new_tokens: int, eos_id=None, cache_dtype=None, prompt_lengths=None, block_tokens=64, alternatives=None):
     """Extend ``tokens`` ``[B, S0]`` by up to ``max_new_tokens`` greedily chosen tokens; returns ``[B, S0 + new]``.
 
     Every rank of a tensor-parallel group passes the same ``tokens`` (ranks that differ in data or depth
@@ -44,17 +83,24 @@ def greedy_generate(model, tokens, max_new_tokens: int, eos_id=None, cache_dtype
     ``block_tokens`` and every token is evaluated once; scores differ by the rounding of what is stored.  Prompts may then differ in
     length: row ``r`` is ``tokens[r, :prompt_lengths[r]]``, and its new tokens follow there; what is left of a row is ``eos_id`` (or 0).
     A ``Mixtral``'s expert capacity is that of a step's tokens, one per row, padding of the prompts among them: what is dropped differs
-    from an evaluation of whole prefixes unless ``capacity_factor`` leaves room for all."""
+    from an evaluation of whole prefixes unless ``capacity_factor`` leaves room for all.
+
+    With ``alternatives`` (0 to 32) the result is ``(tokens, ops.TokenLogProbs)``: the log-probabilities ``[B, new]`` of the new tokens,
+    and as many of the likeliest tokens at each of their places; zeros (-1) for rows that have ended."""
     if cache_dtype is None and prompt_lengths is not None:
         raise ValueError("prompts of different lengths need a cache (cache_dtype)")
+    if alternatives is not None and not 0 <= alternatives <= ops.MOST_ALTERNATIVES:
+        raise ValueError(f"0 to {ops.MOST_ALTERNATIVES} alternatives, not {alternatives}")
+    told = None if alternatives is None else _Told(alternatives, getattr(model.head, "group", None))
     was_training = model.training
     model.eval()
     limit = getattr(getattr(model, "cfg", None), "seq_len", None)
     if cache_dtype is not None:
         try:
-            return _greedy_cached(model, tokens, max_new_tokens, eos_id, limit, cache_dtype, prompt_lengths, block_tokens)
+            out = _greedy_cached(model, tokens, max_new_tokens, eos_id, limit, cache_dtype, prompt_lengths, block_tokens, told)
         finally:
             model.train(was_training)
+        return out if told is None else (out, told.result(tokens.shape[0], tokens.device))
     done = torch.zeros(tokens.shape[0], dtype=torch.bool, device=tokens.device)
     try:
         for _ in range(max_new_tokens):
@@ -62,6 +108,8 @@ def greedy_generate(model, tokens, max_new_tokens: int, eos_id=None, cache_dtype
                 break
             logits = model(tokens)                                           # [B, S, vocab / |group|]
             nxt = parallel_argmax(logits[:, -1], getattr(model.head, "group", None)).to(tokens.dtype)
+            if told is not None:
+                told.step(logits[:, -1], nxt.long(), done if eos_id is not None else None)
             if eos_id is not None:
                 nxt = torch.where(done, torch.full_like(nxt, eos_id), nxt)
                 done = done | (nxt == eos_id)
@@ -70,7 +118,7 @@ def greedy_generate(model, tokens, max_new_tokens: int, eos_id=None, cache_dtype
                 break
     finally:
         model.train(was_training)
-    return tokens
+    return tokens if told is None else (tokens, told.result(tokens.shape[0], tokens.device))
 
 
 def _prompt(tokens, max_new_tokens, limit, prompt_lengths):
@@ -90,7 +138,7 @@ def _prompt(tokens, max_new_tokens, limit, prompt_lengths):
     return lengths, max(room, 0)
 
 
-def _greedy_cached(model, tokens, max_new_tokens, eos_id, limit, dtype, prompt_lengths, block_tokens):
+def _greedy_cached(model, tokens, max_new_tokens, eos_id, limit, dtype, prompt_lengths, block_tokens, told):
     lengths, room = _prompt(tokens, max_new_tokens, limit, prompt_lengths)
     B, S = tokens.shape
     pad = 0 if eos_id is None else eos_id
@@ -105,6 +153,8 @@ def _greedy_cached(model, tokens, max_new_tokens, eos_id, limit, dtype, prompt_l
     for i in range(room):
         logits = model(step, cache=cache)                                    # [B, 1, vocab / |group|]
         nxt = parallel_argmax(logits[:, -1], getattr(model.head, "group", None)).to(tokens.dtype)
+        if told is not None:
+            told.step(logits[:, -1], nxt.long(), done if eos_id is not None else None)
         if eos_id is not None:
             nxt = torch.where(done, torch.full_like(nxt, eos_id), nxt)
             done = done | (nxt == eos_id)

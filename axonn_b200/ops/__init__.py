@@ -8,7 +8,7 @@ PyTorch composition used on CPU (and as the numerical oracle in the tests).
 from .activation import gelu_backward_colsum, gelu, gelu_backward, swiglu  # noqa: F401
 from .attention import flash_attention, flash_attention_packed  # noqa: F401
 from .beam import MOST_BEAMS, BeamStep, beam_select  # noqa: F401
-from .embedding import embedding  # noqa: F401
+from .embedding import EMBEDDING_TYPES, embedding  # noqa: F401
 from .gemm import (  # noqa: F401
     gemm_on_pairs,
     EPI_BIAS,

@@ -7,10 +7,12 @@ import torch.nn.functional as F
 
 from . import _lib
 from .direct import host_paths, no_graph, plain_tensors
+from .gemm import as_written
 from .kv_cache import _elsewhere
 
 _DT = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
 _INDEX = {torch.int32: 4, torch.int64: 8}
+EMBEDDING_TYPES = tuple(_DT)
 
 
 def embedding(tokens, weight, scale=1.0, padding_idx=None):
@@ -104,7 +106,7 @@ class _EmbeddingGradFn(torch.autograd.Function):
     def forward(ctx, tokens, sorted_, dy, V, scale, padding):
         ctx.save_for_backward(tokens)
         ctx.scale, ctx.padding = scale, padding
-        return _table_gradient(sorted_.contiguous(), dy, V, scale)
+        return _table_gradient(as_written(sorted_), dy, V, scale)
 
     @staticmethod
     def backward(ctx, d_table):

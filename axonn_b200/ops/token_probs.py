@@ -11,6 +11,7 @@ import torch.distributed as dist
 
 from . import _lib
 from .direct import first_derivative_only, host_paths
+from .gemm import as_written
 from .kv_cache import _elsewhere
 
 MOST_ALTERNATIVES = 32
@@ -174,6 +175,8 @@ class _TokenLogProbsFn(torch.autograd.Function):
     @first_derivative_only
     def backward(ctx, d_log_probs, d_entropy, d_top, _):
         logits, tokens, stats, at = ctx.saved_tensors
+        # what hooks (offloading, compression) give back may lie in another layout
+        stats, at = as_written(stats), None if at is None else at.contiguous()
         if d_log_probs is None and d_entropy is None and d_top is None:
             return (None,) * 7
         V, rows = logits.shape[-1], logits.numel() // logits.shape[-1]
