@@ -356,15 +356,15 @@ int axb_token_log_probs_bwd(const void* logits, long long batch_stride, long lon
                             int V, long long start, long long total, int top, float scale, long long ignored, int dtype, void* stream);
 
 /* ---- table lookup (embedding.cu): out [n, H] = scale * rows of table [V, H] (pitch in values) by tokens [n] of 4 or 8 bytes.  sorted (or
- * NULL): axb_embedding_sorted_words() 32-bit words, 16-byte aligned, that receive what the gradient needs of the tokens, of which
- * `padding` (-1: no such) has none.  grad: dtable [V, H] from rows dy [n, H] (pitch in values) and `sorted` of the same n and V; work:
- * axb_embedding_grad_words() 32-bit words, 16-byte aligned, of this call alone */
+ * NULL): axb_embedding_sorted_words() 32-bit words (0 for few tokens, which are not sorted), 16-byte aligned, that receive what the
+ * gradient needs of the tokens, of which `padding` (-1: no such) has none.  grad: dtable [V, H] from rows dy [n, H] (pitch in values), with
+ * the `sorted` of the same tokens, V and padding; work: axb_embedding_grad_words() 32-bit words, 16-byte aligned, of this call alone */
 long long axb_embedding_sorted_words(long long n, int V);
 int axb_embedding(const void* tokens, int token_bytes, long long n, const void* table, long long pitch, int V, int H, float scale, void* out,
                   long long padding, void* sorted, int dtype, void* stream);
 long long axb_embedding_grad_words(long long n, int H);
-int axb_embedding_grad(const void* sorted, long long n, const void* dy, long long pitch, int V, int H, float scale, void* dtable, void* work,
-                       int dtype, void* stream);
+int axb_embedding_grad(const void* tokens, int token_bytes, const void* sorted, long long n, const void* dy, long long pitch, int V, int H,
+                       float scale, long long padding, void* dtable, void* work, int dtype, void* stream);
 
 /* ---- top-k gradient pruning (prune.cu): keep the k largest |g|, zero the rest, in place.
  * dtype: the codes above (0 bf16, 1 fp16, 2 fp32).  `work`: device scratch of axb_prune_workspace_words() 32-bit words, 8-byte aligned. */

@@ -13,6 +13,7 @@
 //      chunk: then its sum so far goes to the workspace.  A segment of any length so takes many blocks, and one of up to 32 pairs
 //      no extra traffic.
 //   3. The partial sums of long segments, which the blocks of the sums have noted, are joined in their order.
+// Up to 256 tokens are looked through by every block instead: one launch, for steps that are bound by the host's launches.
 #include <atomic>
 #include <initializer_list>
 
@@ -28,6 +29,7 @@ constexpr int SORT_SMEM = SORT_WARPS * SORT_BINS * 4, SORT_SMEM_SMALL = SORT_SME
 constexpr int CHUNK = 32;                     // pairs of a block of sums: a warp's lanes look one chunk ahead
 constexpr int SUM_THREADS = 128, SUM_AHEAD = 8;
 constexpr int ZERO_BYTES = 1 << 17;           // of the table, of a block that zeroes
+constexpr int FEW = 256, FEW_ZERO = 4096;     // tokens that are not sorted; rows of a block that zeroes, then
 constexpr int JOIN_THREADS = 256, JOIN_COLS = 128, JOIN_BLOCKS = 64;
 constexpr int ROW_THREADS = 256, ROW_AHEAD = 2, ROW_BLOCKS = 8;
 
@@ -280,6 +282,99 @@ sort_tokens_kernel(const I* __restrict__ tokens, int n, int V, long long padding
   }
 }
 
+// Rows [v0, v1) but those that are `met`, a warp a row: the values in front of the first 16-byte boundary, whole words, the values
+// behind the last.
+template <typename T, int N, typename Met> __device__ __forceinline__ void zero_rows_of(T* dtable, int v0, int v1, int H, Met met) {
+  constexpr int COUNT = 16 / sizeof(T);
+  const int lane = threadIdx.x & 31;
+  for (int v = v0 + threadIdx.x / 32; v < v1; v += SUM_THREADS / 32) {
+    if (met(v)) continue;
+    T* row = dtable + static_cast<long long>(v) * H;
+    const int head = N == COUNT ? 0 : min(static_cast<int>((16u - (reinterpret_cast<unsigned long long>(row) & 15u)) % 16u / sizeof(T)), H);
+    const int words = (H - head) / COUNT;
+    uint4* to = reinterpret_cast<uint4*>(row + head);
+    for (int i = lane; i < words; i += 32) to[i] = make_uint4(0u, 0u, 0u, 0u);
+    if (N < COUNT) {
+      if (lane < head) row[lane] = from_float<T>(0.f);
+      if (head + words * COUNT + lane < H) row[head + words * COUNT + lane] = from_float<T>(0.f);
+    }
+  }
+}
+
+// Few tokens: a block and 16 bytes of columns per thread for each of them, which sums the rows of its token if it is the first with it;
+// the other blocks zero the rows of the tokens that there are not.
+template <typename T, typename I, int N>
+__global__ void __launch_bounds__(SUM_THREADS)
+sum_few_rows_kernel(const I* __restrict__ tokens, int n, const T* __restrict__ dy, long long pitch, int V, int H, float scale, long long padding,
+                    T* __restrict__ dtable, int slices, int zero_rows) {
+  using P = Piece<T, N>;
+  constexpr int PIECES = 16 / sizeof(P), STEP = SUM_THREADS * N;
+  __shared__ int s_token[FEW];                   // -1: without a gradient
+  __shared__ uint32_t s_met[FEW_ZERO / 32];
+  __shared__ int s_at[FEW], s_count[SUM_THREADS / 32];
+  pdl_launch_next();
+  pdl_wait();
+  const int tid = threadIdx.x, lane = tid & 31, w = tid >> 5;
+  for (int i = tid; i < n; i += SUM_THREADS) {
+    const long long t = tokens[i];
+    s_token[i] = t >= 0 && t < V && t != padding ? static_cast<int>(t) : -1;
+  }
+  const int sums = n * slices;
+  if (static_cast<int>(blockIdx.x) >= sums) {
+    const int v0 = (static_cast<int>(blockIdx.x) - sums) * zero_rows, v1 = min(v0 + zero_rows, V);
+    for (int i = tid; i < (zero_rows + 31) / 32; i += SUM_THREADS) s_met[i] = 0u;
+    __syncthreads();
+    for (int i = tid; i < n; i += SUM_THREADS)
+      if (s_token[i] >= v0 && s_token[i] < v1) atomicOr(&s_met[(s_token[i] - v0) / 32], 1u << (s_token[i] - v0) % 32);
+    __syncthreads();
+    zero_rows_of<T, N>(dtable, v0, v1, H, [&](int v) { return (s_met[(v - v0) / 32] >> (v - v0) % 32 & 1u) != 0u; });
+    return;
+  }
+  __syncthreads();
+  const int own = static_cast<int>(blockIdx.x) / slices, slice = static_cast<int>(blockIdx.x) - own * slices, token = s_token[own];
+  if (token < 0) return;
+  // the places of the token, in their order; none in front of this one
+  int count = 0;
+  for (int i0 = 0; i0 < n; i0 += SUM_THREADS) {
+    const bool mine = i0 + tid < n && s_token[i0 + tid] == token;
+    if (__syncthreads_or(mine && i0 + tid < own)) return;
+    const unsigned met = __ballot_sync(0xffffffffu, mine);
+    if (lane == 0) s_count[w] = __popc(met);
+    __syncthreads();
+    int before = count;
+    for (int k = 0; k < SUM_THREADS / 32; ++k) { if (k < w) before += s_count[k]; count += s_count[k]; }
+    if (mine) s_at[before + __popc(met & ((1u << lane) - 1u))] = i0 + tid;
+    __syncthreads();
+  }
+  const int col = slice * STEP * PIECES + tid * N;
+  if (col >= H) return;
+  float sum[PIECES][N] = {};
+  for (int i = 0; i < count; i += SUM_AHEAD) {
+    P p[SUM_AHEAD][PIECES];
+#pragma unroll
+    for (int k = 0; k < SUM_AHEAD; ++k) {
+      const T* row = dy + s_at[min(i + k, count - 1)] * pitch + col;
+#pragma unroll
+      for (int c = 0; c < PIECES; ++c) if (col + c * STEP < H) p[k][c] = *reinterpret_cast<const P*>(row + c * STEP);
+    }
+#pragma unroll
+    for (int k = 0; k < SUM_AHEAD; ++k) {
+      if (i + k >= count) break;
+#pragma unroll
+      for (int c = 0; c < PIECES; ++c)
+#pragma unroll
+        for (int j = 0; j < N; ++j) sum[c][j] += to_float(p[k][c].v[j]);
+    }
+  }
+#pragma unroll
+  for (int c = 0; c < PIECES; ++c) {
+    P p;
+#pragma unroll
+    for (int j = 0; j < N; ++j) p.v[j] = from_float<T>(sum[c][j] * scale);
+    if (col + c * STEP < H) *reinterpret_cast<P*>(dtable + static_cast<long long>(token) * H + col + c * STEP) = p;
+  }
+}
+
 // Sums of a chunk, 16 bytes of columns per thread in pieces of N values; behind the blocks of the sums those that zero rows.
 template <typename T, int N>
 __global__ void __launch_bounds__(SUM_THREADS)
@@ -293,21 +388,8 @@ sum_rows_kernel(const uint2* __restrict__ pairs, int n, const T* __restrict__ dy
   pdl_wait();
   const int tid = threadIdx.x, lane = tid & 31;
   if (blockIdx.x >= sum_blocks) {
-    // a warp a row: the values in front of the first 16-byte boundary, whole words, the values behind the last
     const int v0 = static_cast<int>(blockIdx.x - sum_blocks) * zero_rows, v1 = min(v0 + zero_rows, V);
-    constexpr int COUNT = 16 / sizeof(T);
-    for (int v = v0 + tid / 32; v < v1; v += SUM_THREADS / 32) {
-      if (__ldg(met + v)) continue;
-      T* row = dtable + static_cast<long long>(v) * H;
-      const int head = N == COUNT ? 0 : min(static_cast<int>((16u - (reinterpret_cast<unsigned long long>(row) & 15u)) % 16u / sizeof(T)), H);
-      const int words = (H - head) / COUNT;
-      uint4* to = reinterpret_cast<uint4*>(row + head);
-      for (int i = lane; i < words; i += 32) to[i] = make_uint4(0u, 0u, 0u, 0u);
-      if (N < COUNT) {
-        if (lane < head) row[lane] = from_float<T>(0.f);
-        if (head + words * COUNT + lane < H) row[head + words * COUNT + lane] = from_float<T>(0.f);
-      }
-    }
+    zero_rows_of<T, N>(dtable, v0, v1, H, [&](int v) { return __ldg(met + v) != 0; });
     return;
   }
   const int chunk = static_cast<int>(blockIdx.x / slices), slice = static_cast<int>(blockIdx.x - static_cast<long long>(chunk) * slices);
@@ -471,13 +553,13 @@ static int look_up(const void* tokens, long long n, const void* table, long long
   return 0;
 }
 
-// What the gradient needs of the tokens: a byte for every token of the table, and the sorted pairs (a second list for many: they take turns).
+// What the gradient needs of more than a few tokens: a byte for every token of the table, and the sorted pairs (a second list for many: they take turns).
 struct Sorted {
   long long met, pairs, words;
   Sorted(long long n, int V) {
     met = (V + 15ll) / 16 * 4;
     pairs = (2 * n + 3) / 4 * 4;
-    words = met + (n > SORT_PORTABLE * SORT_SHARE ? 2 : 1) * pairs;
+    words = n <= FEW ? 0 : met + (n > SORT_PORTABLE * SORT_SHARE ? 2 : 1) * pairs;
   }
 };
 static cudaLaunchConfig_t sort_config(unsigned ctas, int smem, cudaStream_t s, cudaLaunchAttribute* attr) {
@@ -556,16 +638,32 @@ struct GradWork {
     chunks = (n + CHUNK - 1) / CHUNK;
     Hp = (H + 3) / 4 * 4;
     pieces = (chunks + 3) / 4 * 4;
-    words = pieces + (chunks > 1 ? chunks * Hp : 0);
+    words = n <= FEW ? 0 : pieces + chunks * Hp;
   }
 };
+
+static int rows_to_zero(int row_bytes) { return row_bytes >= ZERO_BYTES ? 1 : ZERO_BYTES / row_bytes; }
+
+template <typename T, int N>
+static int sum_few_rows(const void* tokens, int token_bytes, int n, const void* dy, long long pitch, int V, int H, float scale, long long padding,
+                        void* dtable, cudaStream_t s) {
+  const int columns = SUM_THREADS * 16 / static_cast<int>(sizeof(T)), slices = (H + columns - 1) / columns;
+  const int most = rows_to_zero(H * static_cast<int>(sizeof(T))), zero_rows = most < FEW_ZERO ? most : FEW_ZERO;
+  const dim3 grid(static_cast<unsigned>(n * slices + (V + zero_rows - 1) / zero_rows));
+  if (token_bytes == 8)
+    AXB_CUDA(pdl_launch(sum_few_rows_kernel<T, long long, N>, grid, dim3(SUM_THREADS), 0, s, static_cast<const long long*>(tokens), n,
+                        static_cast<const T*>(dy), pitch, V, H, scale, padding, static_cast<T*>(dtable), slices, zero_rows));
+  else
+    AXB_CUDA(pdl_launch(sum_few_rows_kernel<T, int, N>, grid, dim3(SUM_THREADS), 0, s, static_cast<const int*>(tokens), n, static_cast<const T*>(dy),
+                        pitch, V, H, scale, padding, static_cast<T*>(dtable), slices, zero_rows));
+  return 0;
+}
 
 template <typename T, int N>
 static int sum_rows(const void* sorted, int n, const void* dy, long long pitch, int V, int H, float scale, void* dtable, int* words, cudaStream_t s) {
   const GradWork work(n, H);
   const int columns = SUM_THREADS * 16 / static_cast<int>(sizeof(T)), slices = (H + columns - 1) / columns;
-  const int row_bytes = H * static_cast<int>(sizeof(T));
-  const int zero_rows = row_bytes >= ZERO_BYTES ? 1 : ZERO_BYTES / row_bytes;
+  const int zero_rows = rows_to_zero(H * static_cast<int>(sizeof(T)));
   const long long sum_blocks = work.chunks * slices, blocks = sum_blocks + (V + static_cast<long long>(zero_rows) - 1) / zero_rows;
   if (blocks > 0x7fffffffll) { set_error("gradient of an embedding: %d tokens with rows of %d values are too many blocks", n, H); return -1; }
   const int ctas = sort_ctas();
@@ -575,7 +673,6 @@ static int sum_rows(const void* sorted, int n, const void* dy, long long pitch, 
   AXB_CUDA(pdl_launch(sum_rows_kernel<T, N>, dim3(static_cast<unsigned>(blocks)), dim3(SUM_THREADS), 0, s, pairs, n, static_cast<const T*>(dy),
                       pitch, V, H, static_cast<int>(work.Hp), scale, static_cast<const uint8_t*>(sorted), static_cast<T*>(dtable), partial, words,
                       slices, sum_blocks, zero_rows));
-  if (n < 2 * CHUNK) return 0;
   const int full = n / CHUNK;                    // a long segment fills one chunk and begins in another
   AXB_CUDA(pdl_launch(join_rows_kernel<T>, dim3(full / 2 < JOIN_BLOCKS ? full / 2 : JOIN_BLOCKS, static_cast<unsigned>((work.Hp + JOIN_COLS - 1) / JOIN_COLS)),
                       dim3(JOIN_THREADS), 0, s, pairs, static_cast<const int*>(words), full, H, static_cast<int>(work.Hp), scale,
@@ -584,13 +681,19 @@ static int sum_rows(const void* sorted, int n, const void* dy, long long pitch, 
 }
 
 template <typename T>
-static int gradient(const void* sorted, int n, const void* dy, long long pitch, int V, int H, float scale, void* dtable, int* work, cudaStream_t s) {
+static int gradient(const void* tokens, int token_bytes, const void* sorted, int n, const void* dy, long long pitch, int V, int H, float scale,
+                    long long padding, void* dtable, int* work, cudaStream_t s) {
   if (n == 0) {
     AXB_CUDA(cudaMemsetAsync(dtable, 0, static_cast<size_t>(V) * H * sizeof(T), s));
     return 0;
   }
   const int size = sizeof(T), bytes = piece_bytes(size, {address(dy), address(dtable), static_cast<unsigned long long>(H) * size,
                                                          static_cast<unsigned long long>(pitch) * size});
+  if (n <= FEW) {
+    const auto sums = bytes == 16 ? sum_few_rows<T, 16 / sizeof(T)> : bytes == 8 ? sum_few_rows<T, 8 / sizeof(T)>
+                    : bytes == 4 ? sum_few_rows<T, 4 / sizeof(T)> : sum_few_rows<T, 1>;
+    return sums(tokens, token_bytes, n, dy, pitch, V, H, scale, padding, dtable, s);
+  }
   const auto sums = bytes == 16 ? sum_rows<T, 16 / sizeof(T)> : bytes == 8 ? sum_rows<T, 8 / sizeof(T)> : bytes == 4 ? sum_rows<T, 4 / sizeof(T)>
                                                                                                                      : sum_rows<T, 1>;
   return sums(sorted, n, dy, pitch, V, H, scale, dtable, work, s);
@@ -632,18 +735,20 @@ extern "C" int axb_embedding(const void* tokens, int token_bytes, long long n, c
   if (refused("embedding", n, V, H, dtype, token_bytes) || misaligned("embedding", sorted)) return -1;
   if (n == 0) return 0;
   const cudaStream_t s = static_cast<cudaStream_t>(stream);
-  if (sorted && (token_bytes == 8 ? sort_tokens<long long>(tokens, static_cast<int>(n), V, padding, sorted, s)
-                                  : sort_tokens<int>(tokens, static_cast<int>(n), V, padding, sorted, s))) return -1;
+  const bool sort = sorted && n > FEW;
+  if (sort && (token_bytes == 8 ? sort_tokens<long long>(tokens, static_cast<int>(n), V, padding, sorted, s)
+                                : sort_tokens<int>(tokens, static_cast<int>(n), V, padding, sorted, s))) return -1;
   const auto go = dtype == 0 ? look_up_by<__nv_bfloat16> : dtype == 1 ? look_up_by<__half> : look_up_by<float>;
-  return go(tokens, token_bytes, n, table, pitch, V, H, scale, out, sorted != nullptr && max_ctas() == 0, s);
+  return go(tokens, token_bytes, n, table, pitch, V, H, scale, out, sort && max_ctas() == 0, s);
 }
 
 extern "C" long long axb_embedding_grad_words(long long n, int H) { return GradWork(n, H).words; }
 
-extern "C" int axb_embedding_grad(const void* sorted, long long n, const void* dy, long long pitch, int V, int H, float scale, void* dtable,
-                                  void* work, int dtype, void* stream) {
-  if (refused("gradient of an embedding", n, V, H, dtype, 8) || misaligned("gradient of an embedding", work) ||
+extern "C" int axb_embedding_grad(const void* tokens, int token_bytes, const void* sorted, long long n, const void* dy, long long pitch, int V, int H,
+                                  float scale, long long padding, void* dtable, void* work, int dtype, void* stream) {
+  if (refused("gradient of an embedding", n, V, H, dtype, token_bytes) || misaligned("gradient of an embedding", work) ||
       misaligned("gradient of an embedding", sorted)) return -1;
   const auto go = dtype == 0 ? gradient<__nv_bfloat16> : dtype == 1 ? gradient<__half> : gradient<float>;
-  return go(sorted, static_cast<int>(n), dy, pitch, V, H, scale, dtable, static_cast<int*>(work), static_cast<cudaStream_t>(stream));
+  return go(tokens, token_bytes, sorted, static_cast<int>(n), dy, pitch, V, H, scale, padding, dtable, static_cast<int*>(work),
+            static_cast<cudaStream_t>(stream));
 }

@@ -10,6 +10,7 @@
 #include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/autograd/functions/utils.h>
 #include <torch/csrc/autograd/python_variable.h>
+#include <torch/csrc/autograd/saved_variable.h>
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/jit/frontend/tracer.h>
 #include <ATen/autocast_mode.h>
@@ -524,52 +525,64 @@ TokenResults run_token_log_probs(const Tensor& logits, const Tensor& tokens, boo
   return out;
 }
 
-// Inputs: logits, tokens (may be missing).  Outputs: those asked for of log_probs, entropy, top_log_probs and top_tokens.
-struct TokenLogProbsNode : torch::autograd::Function<TokenLogProbsNode> {
-  static torch::autograd::variable_list forward(torch::autograd::AutogradContext* ctx, const Tensor& logits, const optional<Tensor>& tokens,
-                                                bool entropy, int64_t top, double scale, int64_t ignored) {
-    const TokenResults r = run_token_log_probs(logits, tokens ? *tokens : Tensor(), entropy, top, scale, ignored);
-    ctx->save_for_backward({logits, tokens ? *tokens : Tensor(), r.stats, r.top_tokens});
-    ctx->saved_data["entropy"] = entropy;
-    ctx->saved_data["top"] = top;
-    ctx->saved_data["scale"] = scale;
-    ctx->saved_data["ignored"] = ignored;
-    ctx->set_materialize_grads(false);
-    torch::autograd::variable_list out;
-    for (const Tensor& t : {r.log_probs, r.entropy, r.top_log_probs, r.top_tokens})
-      if (t.defined()) out.push_back(t);
-    if (top) ctx->mark_non_differentiable({out.back()});
-    return out;
+// A node without the conveniences of torch::autograd::Function, which cost a short step 5 us (a table of named values, wrapped outputs).
+template <typename Node> std::shared_ptr<Node> node_of(const Tensor& input) {
+  std::shared_ptr<Node> node(new Node(), torch::autograd::deleteNode);
+  node->set_next_edges(torch::autograd::collect_next_edges(input));
+  return node;
+}
+
+// Outputs: those asked for of log_probs, entropy and top_log_probs.
+struct TokenLogProbsNode : torch::autograd::Node {
+  torch::autograd::SavedVariable logits, tokens, stats, top_tokens;
+  bool has_tokens = false, entropy = false;
+  int64_t top = 0, ignored = 0;
+  double scale = 1;
+
+  torch::autograd::variable_list apply(torch::autograd::variable_list&& grads) override {
+    std::lock_guard<std::mutex> lock(mutex_);
+    const Tensor z = logits.unpack(), t = has_tokens ? tokens.unpack() : Tensor(), s = stats.unpack(), best = top ? top_tokens.unpack() : Tensor();
+    if (!at::GradMode::is_enabled()) return {gradient(z, t, s, best, grads)};
+    Tensor out;
+    {
+      at::AutoGradMode no_grad(false);
+      out = gradient(z, t, s, best, grads);
+    }
+    // the kernels leave no graph (first_derivative_only in ops/direct.py)
+    torch::autograd::variable_list inputs(grads.begin(), grads.end());
+    inputs.push_back(z);
+    if (out.defined() && std::any_of(inputs.begin(), inputs.end(), [](const Tensor& x) { return x.defined() && x.requires_grad(); }))
+      torch::autograd::set_history(out = out.detach(), std::make_shared<torch::autograd::Error>("TokenLogProbs: second derivatives are not implemented",
+                                                                                              torch::autograd::collect_next_edges(inputs)));
+    return {out};
   }
-  static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx, torch::autograd::variable_list grads) {
-    return first_derivative<TokenLogProbsNode>(ctx, grads, "TokenLogProbs: second derivatives are not implemented");
-  }
-  static torch::autograd::variable_list gradients(torch::autograd::AutogradContext* ctx, const torch::autograd::variable_list& grads) {
-    const auto saved = ctx->get_saved_variables();
+  Tensor gradient(const Tensor& given, const Tensor& t, const Tensor& s, const Tensor& best, const torch::autograd::variable_list& grads) {
     // what hooks (offloading, compression) give back may lie in another layout
-    const Tensor logits = saved[0].dim() > 3 || (saved[0].stride(-1) != 1 && saved[0].size(-1) != 1) ? saved[0].contiguous() : saved[0];
-    const Tensor &tokens = saved[1], stats = dense(saved[2]), at = saved[3].defined() ? saved[3].contiguous() : saved[3];
-    const int64_t top = ctx->saved_data["top"].toInt();
+    const Tensor z = given.dim() > 3 || (given.stride(-1) != 1 && given.size(-1) != 1) ? given.contiguous() : given;
+    const Tensor by = dense(s), at_ = best.defined() ? best.contiguous() : best;
     size_t i = 0;
-    Tensor d[3];
-    const bool asked[3] = {tokens.defined(), ctx->saved_data["entropy"].toBool(), top > 0};
+    Tensor d[3], out;
+    const bool asked[3] = {has_tokens, entropy, top > 0};
     for (int k = 0; k < 3; ++k)
       if (asked[k]) {
         if (grads[i].defined()) d[k] = grads[i].contiguous();
         ++i;
       }
-    Tensor out;
     if (d[0].defined() || d[1].defined() || d[2].defined()) {
-      const TokenRows r(logits, tokens);
-      out = at::empty(logits.sizes(), logits.options());
-      check(token_log_probs_bwd(logits.data_ptr(), r.batch_stride, r.row_stride, words(tokens), r.token_batch_stride, r.token_stride,
-                                stats.data_ptr<float>(), floats(d[0]), floats(d[1]), floats(d[2]), words(at), out.data_ptr(),
-                                static_cast<int>(r.batches), static_cast<int>(r.per_batch), static_cast<int>(r.V), 0, r.V, static_cast<int>(top),
-                                static_cast<float>(ctx->saved_data["scale"].toDouble()), ctx->saved_data["ignored"].toInt(), dtype_code(logits),
-                                stream()), "axb_token_log_probs_bwd");
+      const TokenRows r(z, t);
+      out = at::empty(z.sizes(), z.options());
+      check(token_log_probs_bwd(z.data_ptr(), r.batch_stride, r.row_stride, words(t), r.token_batch_stride, r.token_stride, by.data_ptr<float>(),
+                                floats(d[0]), floats(d[1]), floats(d[2]), words(at_), out.data_ptr(), static_cast<int>(r.batches),
+                                static_cast<int>(r.per_batch), static_cast<int>(r.V), 0, r.V, static_cast<int>(top), static_cast<float>(scale), ignored,
+                                dtype_code(z), ::stream()), "axb_token_log_probs_bwd");
     }
-    return {out, Tensor(), Tensor(), Tensor(), Tensor(), Tensor()};
+    return out;
   }
+  void release_variables() override {
+    std::lock_guard<std::mutex> lock(mutex_);
+    logits.reset_data(); tokens.reset_data(); stats.reset_data(); top_tokens.reset_data();
+  }
+  std::string name() const override { return "TokenLogProbsBackward"; }
 };
 
 // token_log_probs(logits, tokens | None, entropy, top, 1 / temperature, ignore_index) -> (log_probs | None, entropy | None,
@@ -595,16 +608,21 @@ PyObject* py_token_log_probs(PyObject*, PyObject* const* a, Py_ssize_t n) {
   Tensor out[4];
   {
     NoGil no_gil;
+    const TokenResults r = run_token_log_probs(logits, tokens, entropy, top, scale, ignored);
+    out[0] = r.log_probs; out[1] = r.entropy; out[2] = r.top_log_probs; out[3] = r.top_tokens;
     if (wants_grad(logits)) {
-      const auto list = TokenLogProbsNode::apply(logits, tokens.defined() ? optional<Tensor>(tokens) : std::nullopt, entropy, static_cast<int64_t>(top), scale,
-                                                 static_cast<int64_t>(ignored));
-      const bool asked[4] = {tokens.defined(), entropy, top > 0, top > 0};
-      size_t i = 0;
-      for (int k = 0; k < 4; ++k)
-        if (asked[k]) out[k] = list[i++];
-    } else {
-      const TokenResults r = run_token_log_probs(logits, tokens, entropy, top, scale, ignored);
-      out[0] = r.log_probs; out[1] = r.entropy; out[2] = r.top_log_probs; out[3] = r.top_tokens;
+      const auto node = node_of<TokenLogProbsNode>(logits);
+      node->logits = torch::autograd::SavedVariable(logits, false);
+      if (tokens.defined()) node->tokens = torch::autograd::SavedVariable(tokens, false);
+      node->stats = torch::autograd::SavedVariable(r.stats, false);
+      if (top) node->top_tokens = torch::autograd::SavedVariable(r.top_tokens, false);
+      node->has_tokens = tokens.defined();
+      node->entropy = entropy;
+      node->top = top;
+      node->ignored = ignored;
+      node->scale = scale;
+      for (int k = 0; k < 3; ++k)
+        if (out[k].defined()) torch::autograd::set_history(out[k], node);
     }
   }
   return tuple_of({out[0], out[1], out[2], out[3]});
@@ -614,68 +632,85 @@ PyObject* py_token_log_probs(PyObject*, PyObject* const* a, Py_ssize_t n) {
 // ---------------------------------------------------------------------------------------------------------------- table lookup
 int index_bytes(const Tensor& tokens) { return tokens.scalar_type() == at::kLong ? 8 : tokens.scalar_type() == at::kInt ? 4 : 0; }
 
-// With `sorted` also what the gradient needs of the tokens.
+// With `sorted` also what the gradient needs of the tokens (nothing for few).
 Tensor run_embedding(const Tensor& tokens, const Tensor& weight, double scale, int64_t padding = -1, Tensor* sorted = nullptr) {
   const Tensor t = tokens.contiguous(), w = weight.stride(1) != 1 && weight.size(1) != 1 ? weight.contiguous() : weight;
   const int V = static_cast<int>(w.size(0)), H = static_cast<int>(w.size(1));
   c10::SmallVector<int64_t, 5> shape(t.sizes().begin(), t.sizes().end());
   shape.push_back(H);
   const Tensor out = at::empty(shape, w.options());
-  if (sorted) *sorted = at::empty({embedding_sorted_words(t.numel(), V)}, w.options().dtype(at::kInt));
+  const int64_t count = sorted ? embedding_sorted_words(t.numel(), V) : 0;
+  if (count) *sorted = at::empty({count}, w.options().dtype(at::kInt));
   if (out.numel())
     check(embedding(t.data_ptr(), index_bytes(t), t.numel(), w.data_ptr(), w.stride(0), V, H, static_cast<float>(scale), out.data_ptr(), padding,
-                    sorted ? sorted->data_ptr() : nullptr, dtype_code(w), stream()), "axb_embedding", sorted ? 2 : 1);
+                    count ? sorted->data_ptr() : nullptr, dtype_code(w), stream()), "axb_embedding", count ? 2 : 1);
   return out;
 }
-Tensor run_embedding_grad(const Tensor& sorted, const Tensor& dy, int64_t V, double scale) {
+Tensor run_embedding_grad(const Tensor& tokens, const Tensor& sorted, const Tensor& dy, int64_t V, double scale, int64_t padding) {
   const int64_t H = dy.size(-1);
-  Tensor rows = dy.reshape({-1, H});
+  Tensor rows = dy.dim() == 2 ? dy : dy.reshape({-1, H});
   if (rows.stride(1) != 1 && H != 1) rows = rows.contiguous();
   const int64_t n = rows.size(0);
-  const Tensor out = at::empty({V, H}, rows.options()), by = dense(sorted);
-  const Tensor work = at::empty({embedding_grad_words(n, static_cast<int>(H))}, rows.options().dtype(at::kInt));
-  check(embedding_grad(by.data_ptr(), n, rows.data_ptr(), rows.stride(0), static_cast<int>(V), static_cast<int>(H), static_cast<float>(scale),
-                       out.data_ptr(), work.data_ptr(), dtype_code(rows), stream()), "axb_embedding_grad", n == 0 ? 0 : n < 64 ? 1 : 2);
+  const Tensor out = at::empty({V, H}, rows.options()), t = tokens.contiguous(), by = sorted.defined() ? dense(sorted) : sorted;
+  const int64_t count = embedding_grad_words(n, static_cast<int>(H));
+  Tensor work;
+  if (count) work = at::empty({count}, rows.options().dtype(at::kInt));
+  check(embedding_grad(t.data_ptr(), index_bytes(t), by.defined() ? by.data_ptr() : nullptr, n, rows.data_ptr(), rows.stride(0), static_cast<int>(V),
+                       static_cast<int>(H), static_cast<float>(scale), padding, out.data_ptr(), count ? work.data_ptr() : nullptr, dtype_code(rows),
+                       stream()), "axb_embedding_grad", n == 0 ? 0 : count ? 2 : 1);
   return out;
 }
 
 // The gradient of the table as a function of that of the rows; and its own: rows of the table that it is asked with.
 struct EmbeddingGradNode : torch::autograd::Function<EmbeddingGradNode> {
-  static Tensor forward(torch::autograd::AutogradContext* ctx, const Tensor& tokens, const Tensor& sorted, const Tensor& dy, int64_t V, double scale,
-                        int64_t padding);
-  static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx, torch::autograd::variable_list grads);
-};
-struct EmbeddingNode : torch::autograd::Function<EmbeddingNode> {
-  static Tensor forward(torch::autograd::AutogradContext* ctx, const Tensor& tokens, const Tensor& weight, double scale, int64_t padding) {
-    Tensor sorted;
-    const Tensor out = run_embedding(tokens, weight, scale, padding, &sorted);
-    ctx->save_for_backward({tokens, sorted});
-    ctx->saved_data["V"] = weight.size(0);
+  static Tensor forward(torch::autograd::AutogradContext* ctx, const Tensor& tokens, const optional<Tensor>& sorted, const Tensor& dy, int64_t V,
+                        double scale, int64_t padding) {
+    ctx->save_for_backward({tokens});
     ctx->saved_data["scale"] = scale;
     ctx->saved_data["padding"] = padding;
-    return out;
+    return run_embedding_grad(tokens, sorted ? *sorted : Tensor(), dy, V, scale, padding);
   }
-  static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx, torch::autograd::variable_list grads) {
-    const auto saved = ctx->get_saved_variables();
-    const int64_t V = ctx->saved_data["V"].toInt(), padding = ctx->saved_data["padding"].toInt();
-    const double scale = ctx->saved_data["scale"].toDouble();
-    return {Tensor(), wants_grad(grads[0]) ? EmbeddingGradNode::apply(saved[0], saved[1], grads[0], V, scale, padding)
-                                           : run_embedding_grad(saved[1], grads[0], V, scale), Tensor(), Tensor()};
-  }
+  static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx, torch::autograd::variable_list grads);
 };
-Tensor EmbeddingGradNode::forward(torch::autograd::AutogradContext* ctx, const Tensor& tokens, const Tensor& sorted, const Tensor& dy, int64_t V,
-                                  double scale, int64_t padding) {
-  ctx->save_for_backward({tokens});
-  ctx->saved_data["scale"] = scale;
-  ctx->saved_data["padding"] = padding;
-  return run_embedding_grad(sorted, dy, V, scale);
+struct EmbeddingNode : torch::autograd::Node {
+  torch::autograd::SavedVariable tokens, sorted;
+  bool has_sorted = false;
+  int64_t V = 0, padding = -1;
+  double scale = 1;
+
+  torch::autograd::variable_list apply(torch::autograd::variable_list&& grads) override {
+    std::lock_guard<std::mutex> lock(mutex_);
+    if (!grads[0].defined()) return {Tensor()};
+    const Tensor t = tokens.unpack(), s = has_sorted ? sorted.unpack() : Tensor();
+    if (wants_grad(grads[0]))
+      return {EmbeddingGradNode::apply(t, s.defined() ? optional<Tensor>(s) : std::nullopt, grads[0], V, scale, padding)};
+    return {run_embedding_grad(t, s, grads[0], V, scale, padding)};
+  }
+  void release_variables() override {
+    std::lock_guard<std::mutex> lock(mutex_);
+    tokens.reset_data(); sorted.reset_data();
+  }
+  std::string name() const override { return "EmbeddingRowsBackward"; }
+};
+Tensor embedding_with_graph(const Tensor& tokens, const Tensor& weight, double scale, int64_t padding) {
+  Tensor sorted;
+  const Tensor out = run_embedding(tokens, weight, scale, padding, &sorted);
+  const auto node = node_of<EmbeddingNode>(weight);
+  node->tokens = torch::autograd::SavedVariable(tokens, false);
+  if (sorted.defined()) node->sorted = torch::autograd::SavedVariable(sorted, false);
+  node->has_sorted = sorted.defined();
+  node->V = weight.size(0);
+  node->padding = padding;
+  node->scale = scale;
+  torch::autograd::set_history(out, node);
+  return out;
 }
 torch::autograd::variable_list EmbeddingGradNode::backward(torch::autograd::AutogradContext* ctx, torch::autograd::variable_list grads) {
   const Tensor tokens = ctx->get_saved_variables()[0], &table = grads[0];
   const double scale = ctx->saved_data["scale"].toDouble();
   const Tensor none = tokens.lt(0).logical_or(tokens.ge(table.size(0))).logical_or(tokens.eq(ctx->saved_data["padding"].toInt()));
   const Tensor there = tokens.masked_fill(none, 0);
-  const Tensor rows = wants_grad(table) ? EmbeddingNode::apply(there, table, scale, static_cast<int64_t>(-1)) : run_embedding(there, table, scale);
+  const Tensor rows = wants_grad(table) ? embedding_with_graph(there, table, scale, -1) : run_embedding(there, table, scale);
   return {Tensor(), Tensor(), rows.masked_fill(none.unsqueeze(-1), 0), Tensor(), Tensor(), Tensor()};
 }
 
@@ -695,7 +730,7 @@ PyObject* py_embedding(PyObject*, PyObject* const* a, Py_ssize_t n) {
   Tensor out;
   {
     NoGil no_gil;
-    out = wants_grad(weight) ? EmbeddingNode::apply(tokens, weight, scale, static_cast<int64_t>(padding)) : run_embedding(tokens, weight, scale);
+    out = wants_grad(weight) ? embedding_with_graph(tokens, weight, scale, padding) : run_embedding(tokens, weight, scale);
   }
   return THPVariable_Wrap(out);
   END_HANDLE_TH_ERRORS

@@ -95,7 +95,7 @@ _SIGNATURES = {
     "axb_embedding_sorted_words": "l" "i",
     "axb_embedding": "p" "i" "l" "p" "l" "ii" "f" "p" "l" "p" "i" "p",
     "axb_embedding_grad_words": "l" "i",
-    "axb_embedding_grad": "p" "l" "p" "l" "ii" "f" "pp" "i" "p",
+    "axb_embedding_grad": "p" "i" "p" "l" "p" "l" "ii" "f" "l" "pp" "i" "p",
 }
 # Switches of kernels that are gone.  The one kernel that is left covers what they selected; a program that still sets
 # one is told so instead of being ignored.

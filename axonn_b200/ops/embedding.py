@@ -67,22 +67,23 @@ def _rows(tokens, weight, scale, padding=-1, sort=False):
         st = L.axb_embedding(tokens.data_ptr(), _INDEX[tokens.dtype], tokens.numel(), weight.data_ptr(), weight.stride(0), V, H, scale, out.data_ptr(),
                              padding, _lib.addr(sorted_), _DT[weight.dtype], _lib.stream())
         _lib.check(st, "axb_embedding")
-        _lib.add_launches(int(sort))
+        _lib.add_launches(int(sort and sorted_.numel() > 0))
     return out, sorted_
 
 
-def _table_gradient(sorted_, dy, V, scale):
+def _table_gradient(tokens, sorted_, dy, V, scale, padding):
     """``dy [..., H]`` summed by token; the rows may have any stride."""
     H = dy.shape[-1]
     dy = dy.reshape(-1, H)
     if H > 1 and dy.stride(1) != 1:
         dy = dy.contiguous()
-    n, L = dy.shape[0], _lib.lib()
+    n, L, tokens = dy.shape[0], _lib.lib(), tokens.contiguous()
     out = torch.empty(V, H, dtype=dy.dtype, device=dy.device)
     work = torch.empty(L.axb_embedding_grad_words(n, H), dtype=torch.int32, device=dy.device)
-    st = L.axb_embedding_grad(sorted_.data_ptr(), n, dy.data_ptr(), dy.stride(0), V, H, scale, out.data_ptr(), work.data_ptr(), _DT[dy.dtype], _lib.stream())
+    st = L.axb_embedding_grad(tokens.data_ptr(), _INDEX[tokens.dtype], sorted_.data_ptr(), n, dy.data_ptr(), dy.stride(0), V, H, scale, padding,
+                              out.data_ptr(), work.data_ptr(), _DT[dy.dtype], _lib.stream())
     _lib.check(st, "axb_embedding_grad")
-    _lib.add_launches(-1 if n == 0 else 0 if n < 64 else 1)
+    _lib.add_launches(-1 if n == 0 else int(sorted_.numel() > 0))
     return out
 
 
@@ -106,7 +107,7 @@ class _EmbeddingGradFn(torch.autograd.Function):
     def forward(ctx, tokens, sorted_, dy, V, scale, padding):
         ctx.save_for_backward(tokens)
         ctx.scale, ctx.padding = scale, padding
-        return _table_gradient(as_written(sorted_), dy, V, scale)
+        return _table_gradient(tokens, as_written(sorted_), dy, V, scale, padding)
 
     @staticmethod
     def backward(ctx, d_table):

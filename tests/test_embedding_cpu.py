@@ -39,9 +39,9 @@ def test_launchers_refuse():
     L, p = _lib.lib(), 4096
     for call in (lambda: L.axb_embedding(p, 4, 1, p, 8, 0, 8, 1.0, p, -1, None, 0, None), lambda: L.axb_embedding(p, 2, 1, p, 8, 4, 8, 1.0, p, -1, None, 0, None),
                  lambda: L.axb_embedding(p, 8, 1 << 31, p, 8, 4, 8, 1.0, p, -1, p, 0, None), lambda: L.axb_embedding(p, 8, 1, p, 8, 4, 8, 1.0, p, -1, p, 3, None),
-                 lambda: L.axb_embedding(p, 8, 1, p, 8, 4, 8, 1.0, p, -1, p + 4, 0, None), lambda: L.axb_embedding_grad(p, -1, p, 8, 4, 8, 1.0, p, p, 0, None),
-                 lambda: L.axb_embedding_grad(p, 1, p, 8, (1 << 30) + 1, 8, 1.0, p, p, 0, None),
-                 lambda: L.axb_embedding_grad(p, 1, p, 8, 4, 8, 1.0, p, p + 8, 0, None), lambda: L.axb_embedding_grad(p + 8, 1, p, 8, 4, 8, 1.0, p, p, 0, None),
+                 lambda: L.axb_embedding(p, 8, 1, p, 8, 4, 8, 1.0, p, -1, p + 4, 0, None), lambda: L.axb_embedding_grad(p, 8, p, -1, p, 8, 4, 8, 1.0, -1, p, p, 0, None),
+                 lambda: L.axb_embedding_grad(p, 8, p, 1, p, 8, (1 << 30) + 1, 8, 1.0, -1, p, p, 0, None),
+                 lambda: L.axb_embedding_grad(p, 8, p, 1, p, 8, 4, 8, 1.0, -1, p, p + 8, 0, None), lambda: L.axb_embedding_grad(p, 4, p + 8, 1, p, 8, 4, 8, 1.0, -1, p, p, 0, None),
                  lambda: L.axb_token_log_probs(p, 8, 8, p, 1, 1, p, p, p, p, p, 1, 0, 8, 0, 8, 0, 1.0, -100, 1, 0, None),
                  lambda: L.axb_token_log_probs(p, 8, 8, p, 1, 1, p, p, p, p, p, 1, 1, 8, 0, 8, 9, 1.0, -100, 1, 0, None),
                  lambda: L.axb_token_log_probs(p, 8, 8, p, 1, 1, p, p, p, p, p, 1, 1, 80, 0, 80, 33, 1.0, -100, 1, 0, None),

@@ -69,9 +69,12 @@ def _check(tokens, weight, dy, scale=1.0, padding=None):
     (1, 1, 1, "any"), (1, 5, 7, "any"), (0, 9, 16, "any"), (2, 3, 2, "same"), (31, 40, 33, "any"), (33, 2, 64, "any"), (64, 64, 8, "order"),
     (65, 64, 8, "same"), (200, 1000, 1001, "text"), (777, 50, 24, "runs"), (2048, 2048, 128, "order"), (3000, 70000, 50, "text"),
     (5000, 3, 40, "any"), (8193, 32000, 96, "text"), (20000, 300, 72, "same"), (20011, 140000, 16, "any"), (100003, 1000, 12, "text"),
-    (300, 20, 9000, "any"), (70, 2 ** 20 + 3, 4, "any"), (40000, 513, 520, "text")])
+    (300, 20, 9000, "any"), (70, 2 ** 20 + 3, 4, "any"), (40000, 513, 520, "text"), (256, 40, 24, "text"), (257, 40, 24, "text"),
+    (256, 2 ** 18, 5, "same"), (1024, 600, 8, "runs"), (1025, 600, 8, "runs"), (32768, 2000, 8, "text"), (32769, 2000, 8, "text"), (5000, 511, 20, "runs"),
+    (4096, 512, 16, "same")])
 def test_table(n, V, H, kind, dtype):
-    """One token to many, tables of one row to a million, rows of one value to nine thousand, segments of every length."""
+    """One token to many (256, 1024 and 32,768 are the most that are not sorted, sorted by one block, and kept on the chip), tables of one
+    row to a million, rows of one value to nine thousand, segments of every length."""
     g = torch.Generator(device=DEV).manual_seed(n + V)
     tokens = _tokens(n, V, kind, g)
     weight = torch.randn(V, H, generator=g, device=DEV).to(dtype)
