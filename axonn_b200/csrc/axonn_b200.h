@@ -343,9 +343,10 @@ int axb_beam_select(const void* logits, const float* scores, const void* done, i
 /* ---- log-probabilities of given tokens (token_probs.cu): rows of V logits at batch * batch_stride + row * row_stride (strides in values),
  * a slice of a vocabulary of `total` that begins at `start`; tokens [batches, per_batch] int64 (strides in words) or NULL, rows of the token
  * `ignored` are left out; scale: 1 / temperature.  stats [rows, 4] fp32, 16-byte aligned, is written in any case.  whole: the slice is all of
- * the vocabulary, and log_probs and entropy [rows] (or NULL) and the top log-probabilities [rows, top] are finished and stats (m, s, H, z_t);
+ * the vocabulary, and log_probs and entropy [rows] (or NULL) and the top log-probabilities [rows, top] are finished and stats (m, s, H,
+ * log s), H with an entropy only;
  * otherwise stats are (m, s, w, z_t) of the slice and the top logits are as they are.
- * bwd: stats (m, s, H) of the whole vocabulary, gradients of log_probs, entropy and the top ones (or NULL), out [rows, V] dense. */
+ * bwd: stats (m, s, H, log s) of the whole vocabulary, gradients of log_probs, entropy and the top ones (or NULL), out [rows, V] dense. */
 int axb_token_log_probs(const void* logits, long long batch_stride, long long row_stride, const long long* tokens,
                         long long token_batch_stride, long long token_stride, float* log_probs, float* entropy, float* top_log_probs,
                         long long* top_tokens, float* stats, int batches, int per_batch, int V, long long start, long long total, int top,

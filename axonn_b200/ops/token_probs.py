@@ -195,7 +195,7 @@ class _TokenLogProbsFn(torch.autograd.Function):
 
 
 def _finish(stats, best, at, tokens, entropy, top, scale, ignore_index, front):
-    """Results from the statistics of the whole vocabulary, and what the backward takes: (m, s, entropy) of every row."""
+    """Results from the statistics of the whole vocabulary, and what the backward takes: (m, s, entropy, log s) of every row."""
     m, s, w, zt = stats.unbind(-1)
     H = s.log() - w / s
     ignored = None if tokens is None else tokens.reshape(-1) == ignore_index
@@ -203,7 +203,7 @@ def _finish(stats, best, at, tokens, entropy, top, scale, ignore_index, front):
     log_probs = None if tokens is None else keep((zt - m) * scale - s.log(), 0).float().view(front)
     top_log_probs = keep((best - m[:, None]) * scale - s.log()[:, None], 0).float().view(*front, top) if top else None
     top_tokens = keep(at, -1).view(*front, top) if top else None
-    return log_probs, keep(H, 0).float().view(front) if entropy else None, top_log_probs, top_tokens, torch.stack([m, s, H, zt], -1).float()
+    return log_probs, keep(H, 0).float().view(front) if entropy else None, top_log_probs, top_tokens, torch.stack([m, s, H, s.log()], -1).float()
 
 
 def _backward_torch(ctx, logits, tokens, stats, at, d_log_probs, d_entropy, d_top):
