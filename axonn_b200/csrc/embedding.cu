@@ -56,8 +56,8 @@ template <typename T, int N> struct alignas(sizeof(T) * N) Piece { T v[N]; };
 
 // ------------------------------------------------------------------------------------------------------------------------ lookup
 // `group` threads (a power of two) a row, ROWS rows for each of them at a time, 16 bytes of each in pieces of N values.  Tokens are read a
-// step ahead.  `beside` the sorting of the same tokens, which lets this kernel begin when all work before both has ended, it does not wait
-// for that.
+// step ahead.  `beside` the sorting of the same tokens, which lets this kernel begin when all work before both has ended, it waits for
+// that at its end only.
 template <typename T, typename I, int N, int ROWS>
 __global__ void __launch_bounds__(ROW_THREADS, ROW_BLOCKS)
 embedding_kernel(const I* __restrict__ tokens, long long n, const T* __restrict__ table, long long pitch, int V, int H, float scale,
@@ -755,6 +755,7 @@ extern "C" int axb_embedding_grad(const void* tokens, int token_bytes, const voi
                                   float scale, long long padding, void* dtable, void* work, int dtype, void* stream) {
   if (refused("gradient of an embedding", n, V, H, dtype, token_bytes) || misaligned("gradient of an embedding", work) ||
       misaligned("gradient of an embedding", sorted)) return -1;
+  if (n > FEW && (!sorted || !work)) { set_error("gradient of an embedding: %lld tokens have been sorted, and take a workspace", n); return -1; }
   const auto go = dtype == 0 ? gradient<__nv_bfloat16> : dtype == 1 ? gradient<__half> : gradient<float>;
   return go(tokens, token_bytes, sorted, static_cast<int>(n), dy, pitch, V, H, scale, padding, dtable, static_cast<int*>(work),
             static_cast<cudaStream_t>(stream));

@@ -18,7 +18,7 @@
 // One B200, device time: 4096 rows of 128,256 bf16 values with entropy 161.8 us (their bytes at the copy's rate: 160.7), the gradient 336
 // (321); 8 x 2047 rows of 50,304, 15 % of them ignored, 219 (214).  6.4 instructions a value, 8.0 with entropy.  64 rows of 128,256
 // with 20 alternatives 16.5 us, without 8.3: a chain of loads, bounds, lists and the exchange, 29,000 cycles, in which no other block fills in.
-// Tried: every value of a list's words by its own thread (5,000 instructions a warp for 3,000), bounds by 16 counts over the block
+// Tried: every value of a word by the thread that has it (9.4 M instructions for 8.0 there), bounds by 16 counts over the block
 // (20.6 us for 12.4 with one alternative), one list with atomics for the block (no faster), three blocks' registers for four (no faster).
 #include <type_traits>
 
@@ -736,7 +736,11 @@ token_probs_bwd_kernel(const TokenProbsArgs a, const float4* stats, const float*
 
 static int fill(TokenProbsArgs& a, const char* what, const void* logits, long long batch_stride, long long row_stride, const long long* tokens,
                 long long token_batch_stride, long long token_stride, int batches, int per_batch, int V, long long start, long long total, int top,
-                float scale, long long ignored, int whole, int dtype) {
+                float scale, long long ignored, int whole, int dtype, const float* stats, bool best) {
+  if (reinterpret_cast<unsigned long long>(stats) % 16 || !stats || (top > 0 && !best)) {
+    set_error("%s: statistics must be there, on 16 bytes, and the alternatives' tensors where some are asked for", what);
+    return -1;
+  }
   if (batches < 1 || per_batch < 1 || static_cast<long long>(batches) * per_batch > 0x7fffffffll || V < 1 || V > (1 << 30) || top < 0 ||
       top > TP_MOST || top > V || !(scale > 0.f) || dtype < 0 || dtype > 2) {
     set_error("%s: %d x %d rows of %d values, %d alternatives, scale %g, type %d", what, batches, per_batch, V, top, scale, dtype);
@@ -805,7 +809,7 @@ extern "C" int axb_token_log_probs(const void* logits, long long batch_stride, l
                                    long long total, int top, float scale, long long ignored, int whole, int dtype, void* stream) {
   TokenProbsArgs a;
   if (fill(a, "token log-probabilities", logits, batch_stride, row_stride, tokens, token_batch_stride, token_stride, batches, per_batch, V,
-           start, total, top, scale, ignored, whole, dtype)) return -1;
+           start, total, top, scale, ignored, whole, dtype, stats, top_log_probs && top_tokens)) return -1;
   const auto go = dtype == 0 ? tell_of<__nv_bfloat16> : dtype == 1 ? tell_of<__half> : tell_of<float>;
   return go(a, static_cast<long long>(batches) * per_batch, log_probs, entropy, top_log_probs, top_tokens, reinterpret_cast<float4*>(stats),
             static_cast<cudaStream_t>(stream));
@@ -818,7 +822,7 @@ extern "C" int axb_token_log_probs_bwd(const void* logits, long long batch_strid
                                        void* stream) {
   TokenProbsArgs a;
   if (fill(a, "gradient of token log-probabilities", logits, batch_stride, row_stride, tokens, token_batch_stride, token_stride, batches,
-           per_batch, V, start, total, top, scale, ignored, 1, dtype)) return -1;
+           per_batch, V, start, total, top, scale, ignored, 1, dtype, stats, !d_top || top_tokens)) return -1;
   const auto go = dtype == 0 ? untell<__nv_bfloat16> : dtype == 1 ? untell<__half> : untell<float>;
   return go(a, static_cast<long long>(batches) * per_batch, reinterpret_cast<const float4*>(stats), d_log_probs, d_entropy, d_top, top_tokens, out,
             static_cast<cudaStream_t>(stream));

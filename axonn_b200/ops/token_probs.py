@@ -35,7 +35,8 @@ def token_log_probs(logits, tokens=None, entropy=False, top=0, temperature=1.0, 
 
     Positions whose token is ``ignore_index`` are not looked at: they give zeros, alternatives of -1, and no gradient.  Any other number
     outside the vocabulary gives NaN.  Logits of ``-inf`` are tokens that cannot come; a position that leaves none, or that has a NaN or
-    ``+inf`` among its logits, is NaN throughout (a NaN counts as the largest logit among the alternatives).
+    ``+inf`` among its logits, is NaN throughout (a NaN counts as the largest logit among the alternatives).  On a GPU logits below
+    2^-126 count as zero.
 
     Everything but ``top_tokens`` can be differentiated once by the logits, which may have any strides (such as ``logits[:, :-1]``) and are
     left as they are.  With ``group`` the last dimension is this rank's contiguous slice of the vocabulary, of equal size on all ranks (rank

@@ -46,5 +46,11 @@ def test_launchers_refuse():
                  lambda: L.axb_token_log_probs(p, 8, 8, p, 1, 1, p, p, p, p, p, 1, 1, 8, 0, 8, 9, 1.0, -100, 1, 0, None),
                  lambda: L.axb_token_log_probs(p, 8, 8, p, 1, 1, p, p, p, p, p, 1, 1, 80, 0, 80, 33, 1.0, -100, 1, 0, None),
                  lambda: L.axb_token_log_probs(p, 8, 8, p, 1, 1, p, p, p, p, p, 1, 1, 8, 0, 8, 0, 0.0, -100, 1, 0, None),
+                 lambda: L.axb_embedding_grad(p, 8, None, 300, p, 8, 4, 8, 1.0, -1, p, p, 0, None),
+                 lambda: L.axb_embedding_grad(p, 8, p, 300, p, 8, 4, 8, 1.0, -1, p, None, 0, None),
+                 lambda: L.axb_embedding_grad(p, 2, p, 30, p, 8, 4, 8, 1.0, -1, p, p, 0, None),
+                 lambda: L.axb_token_log_probs(p, 8, 8, p, 1, 1, p, p, p, p, p + 8, 1, 1, 8, 0, 8, 0, 1.0, -100, 1, 0, None),
+                 lambda: L.axb_token_log_probs(p, 8, 8, p, 1, 1, p, p, None, p, p, 1, 1, 8, 0, 8, 2, 1.0, -100, 1, 0, None),
+                 lambda: L.axb_token_log_probs_bwd(p, 8, 8, p, 1, 1, p, p, p, p, None, p, 1, 1, 8, 0, 8, 2, 1.0, -100, 0, None),
                  lambda: L.axb_token_log_probs_bwd(p, 8, 8, p, 1, 1, p, p, p, p, p, p, 1, 1, 8, 0, 8, 0, 1.0, -100, 3, None)):
         assert call() == -1 and _lib.lib().axb_last_error()
