@@ -241,6 +241,7 @@ template <int THREADS> __device__ __forceinline__ uint32_t bound_of(List<THREADS
     uint32_t mine = 0u;
 #pragma unroll
     for (int i = 0; i < EACH; ++i) {
+      if (i >= K) break;                     // no warp has more of the K largest
       const uint32_t most = __reduce_max_sync(0xffffffffu, key);
       if (lane == __ffs(__ballot_sync(0xffffffffu, key == most)) - 1) key = 0u;
       if (lane == i) mine = most;
