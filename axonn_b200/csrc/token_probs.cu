@@ -18,8 +18,9 @@
 // One B200, device time: 4096 rows of 128,256 bf16 values with entropy 161.8 us (their bytes at the copy's rate: 160.7), the gradient 336
 // (321); 8 x 2047 rows of 50,304, 15 % of them ignored, 219 (214).  6.4 instructions a value, 8.0 with entropy.  64 rows of 128,256
 // with 20 alternatives 16.5 us, without 8.3: a chain of loads, bounds, lists and the exchange, 29,000 cycles, in which no other block fills in.
-// Tried: every value of a word by the thread that has it (9.4 M instructions for 8.0 there), bounds by 16 counts over the block
-// (20.6 us for 12.4 with one alternative), one list with atomics for the block (no faster), three blocks' registers for four (no faster).
+// Tried: words with values above the bound one after another by the whole warp (4096 rows of 32,000, 20 alternatives: 106 us for 96), every
+// value of a tile by the thread that has it (more instructions still), bounds by 16 counts over the block (64 rows, one alternative: 20.6
+// us for 12.4), one list with atomics for the block (no faster), registers for four blocks an SM instead of three (no faster).
 #include <type_traits>
 
 #include "common.cuh"
@@ -99,6 +100,26 @@ template <typename T> struct Word {
     if constexpr (__is_same(T, float)) return __uint_as_float(x);
     else if constexpr (__is_same(T, __nv_bfloat16)) return __uint_as_float(i & 1 ? x & 0xffff0000u : x << 16);
     else return __half2float(__ushort_as_half(static_cast<unsigned short>(i & 1 ? x >> 16 : x & 0xffffu)));
+  }
+  // bit i: value i is above x, one of the type's numbers, or is x where that counts
+  __device__ __forceinline__ unsigned reaching(float x, bool equal) const {
+    if constexpr (__is_same(T, float)) {
+      unsigned hits = 0u;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) hits |= (equal ? __uint_as_float(u[i]) >= x : __uint_as_float(u[i]) > x) ? 1u << i : 0u;
+      return hits;
+    } else {
+      using H = std::conditional_t<__is_same(T, __half), __half2, __nv_bfloat162>;
+      Word like;
+      like.set_pair(0, x, x);
+      const H* h = reinterpret_cast<const H*>(u);
+      const H bound = *reinterpret_cast<const H*>(like.u);
+      unsigned m[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) m[i] = equal ? __hge2_mask(h[i], bound) : __hgt2_mask(h[i], bound);
+      const unsigned all = (m[0] & 0x00020001u) | (m[1] & 0x00080004u) | (m[2] & 0x00200010u) | (m[3] & 0x00800040u);
+      return (all | all >> 16) & 0xffu;
+    }
   }
   __device__ __forceinline__ void set_pair(int i, float a, float b) {
     if constexpr (__is_same(T, float)) { u[2 * i] = __float_as_uint(a); u[2 * i + 1] = __float_as_uint(b); }
@@ -508,25 +529,30 @@ token_probs_kernel(const TokenProbsArgs a, int rows, float* log_probs, float* en
       }
       const float bound = over <= TP_LOWEST ? -INFINITY : tp_key_value(over);
       if (__any_sync(0xffffffffu, first ? top >= bound : top > bound)) {
-        // a warp looks at the words with such values one after another, a lane at each of the values
+        // every lane takes the next of its words that have such values, and the next of these: one of each for nearly all
         const int j0 = (base + tid) * COUNT - row.lead;
+        unsigned some = 0u;
 #pragma unroll
-        for (int k = 0; k < TP_WORDS; ++k) {
-          for (unsigned some = __ballot_sync(0xffffffffu, (first ? most[k] >= bound : most[k] > bound) && base + tid + k * THREADS < hi); some;
-               some &= some - 1u) {
-            const int of = __ffs(some) - 1;
-            Word<T> w;
+        for (int k = 0; k < TP_WORDS; ++k) some |= (first ? most[k] >= bound : most[k] > bound) && base + tid + k * THREADS < hi ? 1u << k : 0u;
+        while (__any_sync(0xffffffffu, some != 0u)) {
+          const int k = some ? __ffs(some) - 1 : 0;
+          Word<T> w = now[0];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) w.u[i] = __shfl_sync(0xffffffffu, now[k].u[i], of);
-            const float x = w.one(lane & (COUNT - 1));
-            const int j = __shfl_sync(0xffffffffu, j0, of) + k * THREADS * COUNT + lane;
-            push(lane < COUNT && (first ? x >= bound : x > bound), x, j);
+          for (int i = 1; i < TP_WORDS; ++i)
+#pragma unroll
+            for (int h = 0; h < 4; ++h) w.u[h] = k == i ? now[i].u[h] : w.u[h];
+          unsigned hits = some ? w.reaching(bound, first) : 0u;
+          some &= some - 1u;
+          while (__any_sync(0xffffffffu, hits != 0u)) {
+            const int i = hits ? __ffs(hits) - 1 : 0;
+            push(hits != 0u, w.one(i), j0 + k * THREADS * COUNT + i);
+            hits &= hits - 1u;
           }
         }
       }
-      // anew after 2, 4, 8 ... tiles, where it saves more than it takes: 110 instructions of every warp, against some 35 of one for every
-      // word with values above the old bound, of which a tile has K / tiles (4096 rows of 32,000 values, one alternative: 61 us for 66)
-      if (++tiles >= 2 && (tiles & (tiles - 1)) == 0 && K * ((hi - base) / TILE) > WARPS * tiles)
+      // anew after 2, 4, 8 ... tiles, where it saves more than it takes: 110 instructions of every warp, against some 100 of one for a tile
+      // with values above the old bound, of which it has K / tiles (4096 rows of 32,000 values, 5 alternatives: 69.8 us, with half the factor 71.8)
+      if (++tiles >= 2 && (tiles & (tiles - 1)) == 0 && K * ((hi - base) / TILE) > 2 * WARPS * tiles)
         over = bound_of(s_list, tp_key(st.m), K, turn ^= 1);
     }
     base += TILE;
