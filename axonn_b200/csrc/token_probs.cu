@@ -28,7 +28,9 @@
 namespace axb {
 
 constexpr int TP_MOST = 32;                // alternatives
-constexpr int TP_WORDS = 4;                // 16-byte words of a thread, of a tile
+// 16-byte words of a thread, of a tile: 4, the next ones loaded before these are used, or 8 without, where a block has that many: 4096 rows of
+// 32,000 bf16 values 45.9 us for 48.6, 64 of 128,256 with 20 alternatives 14.4 for 16.5; a row of 32,000 over 8 blocks 7.0 for 6.5.
+constexpr int TP_FEW_WORDS = 4, TP_MANY_WORDS = 8;
 constexpr int TP_KEEP = 64;                // entries that a list is cut down to, at most
 constexpr float TP_LOG2E = 1.4426950408889634f;
 constexpr double TP_LN2 = 0.6931471805599453;
@@ -397,10 +399,10 @@ template <int LANES> __device__ __forceinline__ Stats tp_join_lanes(Stats t, flo
 // Threads of a block: four rows of a warp each, or one row.
 template <int THREADS> constexpr int TP_BLOCK = THREADS == 32 ? 128 : THREADS;
 
-template <typename T, bool ENTROPY, bool TOP, int THREADS>
+template <typename T, bool ENTROPY, bool TOP, int THREADS, int WORDS>
 __global__ void __launch_bounds__(TP_BLOCK<THREADS>)
 token_probs_kernel(const TokenProbsArgs a, int rows, float* log_probs, float* entropy, float* top_log_probs, long long* top_tokens, float4* stats) {
-  constexpr int COUNT = Word<T>::COUNT, TILE = THREADS * TP_WORDS, WARPS = THREADS / 32;
+  constexpr int COUNT = Word<T>::COUNT, TILE = THREADS * WORDS, WARPS = THREADS / 32;
   constexpr int ROWS = TP_BLOCK<THREADS> / THREADS;
   __shared__ Stats s_stats[WARPS];
   __shared__ std::conditional_t<(ROWS > 1), int, Gathered> s_gathered;
@@ -424,7 +426,7 @@ token_probs_kernel(const TokenProbsArgs a, int rows, float* log_probs, float* en
   const uint4* words = reinterpret_cast<const uint4*>(z - row.lead);
   const float c = a.scale * TP_LOG2E;
   const Word<T> nothing = tp_nothing<T>();
-  Word<T> next[TP_WORDS];
+  Word<T> next[WORDS];
   const auto load = [&](Word<T>& w, int i) {
     const uint4 u = __ldcs(words + i);
     w.u[0] = u.x; w.u[1] = u.y; w.u[2] = u.z; w.u[3] = u.w;
@@ -432,10 +434,10 @@ token_probs_kernel(const TokenProbsArgs a, int rows, float* log_probs, float* en
   const auto fetch = [&](int base) {
     if (base + TILE <= hi) {
 #pragma unroll
-      for (int k = 0; k < TP_WORDS; ++k) load(next[k], base + tid + k * THREADS);
+      for (int k = 0; k < WORDS; ++k) load(next[k], base + tid + k * THREADS);
     } else {
 #pragma unroll
-      for (int k = 0; k < TP_WORDS; ++k) {
+      for (int k = 0; k < WORDS; ++k) {
         next[k] = nothing;
         if (base + tid + k * THREADS < hi) load(next[k], base + tid + k * THREADS);
       }
@@ -490,20 +492,22 @@ token_probs_kernel(const TokenProbsArgs a, int rows, float* log_probs, float* en
   int tiles = 0, turn = 0;
   int base = lo;
   do {
-    Word<T> now[TP_WORDS];
-    float most[TP_WORDS];
+    Word<T> now[WORDS];
+    float most[WORDS];
 #pragma unroll
-    for (int k = 0; k < TP_WORDS; ++k) now[k] = next[k];
-    if (base + TILE < hi) fetch(base + TILE);
+    for (int k = 0; k < WORDS; ++k) now[k] = next[k];
+    if (WORDS == TP_FEW_WORDS && base + TILE < hi) fetch(base + TILE);
 #pragma unroll
-    for (int k = 0; k < TP_WORDS; ++k) most[k] = now[k].largest();
-    const float top = fmaxf(fmaxf(most[0], most[1]), fmaxf(most[2], most[3]));
+    for (int k = 0; k < WORDS; ++k) most[k] = now[k].largest();
+    float top = most[0];
+#pragma unroll
+    for (int k = 1; k < WORDS; ++k) top = fmaxf(top, most[k]);
     st.rescale(fmaxf(st.m, top), c);
     const float ref = st.m == -INFINITY ? 0.f : st.m;
     const Two minus(-ref, -ref), by(c, c);
     Two s2(0.f, 0.f), w2(0.f, 0.f);
 #pragma unroll
-    for (int k = 0; k < TP_WORDS; ++k) {
+    for (int k = 0; k < WORDS; ++k) {
 #pragma unroll
       for (int i = 0; i < COUNT / 2; ++i) {
         float u, v;
@@ -533,12 +537,12 @@ token_probs_kernel(const TokenProbsArgs a, int rows, float* log_probs, float* en
         const int j0 = (base + tid) * COUNT - row.lead;
         unsigned some = 0u;
 #pragma unroll
-        for (int k = 0; k < TP_WORDS; ++k) some |= (first ? most[k] >= bound : most[k] > bound) && base + tid + k * THREADS < hi ? 1u << k : 0u;
+        for (int k = 0; k < WORDS; ++k) some |= (first ? most[k] >= bound : most[k] > bound) && base + tid + k * THREADS < hi ? 1u << k : 0u;
         while (__any_sync(0xffffffffu, some != 0u)) {
           const int k = some ? __ffs(some) - 1 : 0;
           Word<T> w = now[0];
 #pragma unroll
-          for (int i = 1; i < TP_WORDS; ++i)
+          for (int i = 1; i < WORDS; ++i)
 #pragma unroll
             for (int h = 0; h < 4; ++h) w.u[h] = k == i ? now[i].u[h] : w.u[h];
           unsigned hits = some ? w.reaching(bound, first) : 0u;
@@ -556,6 +560,7 @@ token_probs_kernel(const TokenProbsArgs a, int rows, float* log_probs, float* en
         over = bound_of(s_list, tp_key(st.m), K, turn ^= 1);
     }
     base += TILE;
+    if (WORDS != TP_FEW_WORDS && base < hi) fetch(base);
   } while (base < hi);
   if (to == row.words && behind < a.V && tid < 32) {
     const bool there = lane < COUNT && behind + lane < a.V;
@@ -675,12 +680,12 @@ token_probs_kernel(const TokenProbsArgs a, int rows, float* log_probs, float* en
 // The adjoint, one pass: (sub, mul, exp2, fma, mul) a value.  Words are loaded and stored past the L1, which takes 336 us for 351 with
 // ordinary stores (4096 x 128,256 bf16); rows that lie differently to 16 bytes than their gradients' are put together from two words.
 // out [rows, V] dense; stats (m, s, H, log s) of the whole vocabulary; null gradients are zeros.  A block has `span` words of a row.
-constexpr int TP_BWD_THREADS = 256;
+constexpr int TP_BWD_THREADS = 256, TP_BWD_WORDS = 4;
 template <typename T, bool ENTROPY>
 __global__ void __launch_bounds__(TP_BWD_THREADS)
 token_probs_bwd_kernel(const TokenProbsArgs a, const float4* stats, const float* d_log_probs, const float* d_entropy, const float* d_top,
                        const long long* top_tokens, T* out, int spans, int span) {
-  constexpr int COUNT = Word<T>::COUNT, TILE = TP_BWD_THREADS * TP_WORDS;
+  constexpr int COUNT = Word<T>::COUNT, TILE = TP_BWD_THREADS * TP_BWD_WORDS;
   __shared__ float s_g[TP_MOST + 1];
   __shared__ long long s_t[TP_MOST + 1];
   pdl_launch_next();
@@ -727,12 +732,12 @@ token_probs_bwd_kernel(const TokenProbsArgs a, const float4* stats, const float*
   const float by_s = -a.scale / st.y, A = by_s * (all + h * (st.z - log_s)), B = by_s * h * static_cast<float>(TP_LN2);
   const Two minus(-st.x, -st.x), by(c, c), A2(A, A), B2(B, B);
   for (int base = from; base < to; base += TILE) {
-    Word<T> now[TP_WORDS];
+    Word<T> now[TP_BWD_WORDS];
 #pragma unroll
-    for (int k = 0; k < TP_WORDS; ++k)
+    for (int k = 0; k < TP_BWD_WORDS; ++k)
       if (base + tid + k * TP_BWD_THREADS < to) now[k] = row[base + tid + k * TP_BWD_THREADS];
 #pragma unroll
-    for (int k = 0; k < TP_WORDS; ++k) {
+    for (int k = 0; k < TP_BWD_WORDS; ++k) {
       if (base + tid + k * TP_BWD_THREADS >= to) break;
 #pragma unroll
       for (int i = 0; i < COUNT / 2; ++i) {
@@ -793,7 +798,10 @@ static int tell(const TokenProbsArgs& a, long long rows, float* log_probs, float
   attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[1].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr; cfg.numAttrs = max_ctas() == 0 ? 2 : 1;
-  AXB_CUDA(cudaLaunchKernelEx(&cfg, token_probs_kernel<T, ENTROPY, TOP, THREADS>, a, static_cast<int>(rows), log_probs, entropy, top_log_probs, top_tokens, stats));
+  auto kernel = token_probs_kernel<T, ENTROPY, TOP, THREADS, TP_FEW_WORDS>;
+  if constexpr (THREADS > 32)
+    if (words / ctas >= TP_MANY_WORDS * THREADS) kernel = token_probs_kernel<T, ENTROPY, TOP, THREADS, TP_MANY_WORDS>;
+  AXB_CUDA(cudaLaunchKernelEx(&cfg, kernel, a, static_cast<int>(rows), log_probs, entropy, top_log_probs, top_tokens, stats));
   return 0;
 }
 
@@ -815,7 +823,7 @@ static int tell_of(const TokenProbsArgs& a, long long rows, float* log_probs, fl
 template <typename T>
 static int untell(const TokenProbsArgs& a, long long rows, const float4* stats, const float* d_log_probs, const float* d_entropy, const float* d_top,
                   const long long* top_tokens, void* out, cudaStream_t s) {
-  const long long words = a.V / Word<T>::COUNT + 2, tile = TP_BWD_THREADS * TP_WORDS, tiles = (words + tile - 1) / tile;
+  const long long words = a.V / Word<T>::COUNT + 2, tile = TP_BWD_THREADS * TP_BWD_WORDS, tiles = (words + tile - 1) / tile;
   long long spans = 16ll * sm_count_current() / rows;
   spans = spans < 1 ? 1 : spans > tiles ? tiles : spans;
   const long long span = (tiles + spans - 1) / spans * tile;
