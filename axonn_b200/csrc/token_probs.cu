@@ -17,7 +17,7 @@
 //
 // One B200, device time: 4096 rows of 128,256 bf16 values with entropy 161.8 us (their bytes at the copy's rate: 160.7), the gradient 336
 // (321); 8 x 2047 rows of 50,304, 15 % of them ignored, 219 (214).  6.4 instructions a value, 8.0 with entropy.  64 rows of 128,256
-// with 20 alternatives 16.5 us, without 8.3: a chain of loads, bounds, lists and the exchange, 29,000 cycles, in which no other block fills in.
+// with 20 alternatives 14.4 us, without 8.3: a chain of loads, bounds, lists and the exchange, 25,000 cycles, in which no other block fills in.
 // Tried: words with values above the bound one after another by the whole warp (4096 rows of 32,000, 20 alternatives: 106 us for 96), every
 // value of a tile by the thread that has it (more instructions still), bounds by 16 counts over the block (64 rows, one alternative: 20.6
 // us for 12.4), one list with atomics for the block (no faster), registers for four blocks an SM instead of three (no faster).
@@ -34,13 +34,14 @@ constexpr int TP_FEW_WORDS = 4, TP_MANY_WORDS = 8;
 constexpr int TP_KEEP = 64;                // entries that a list is cut down to, at most
 constexpr float TP_LOG2E = 1.4426950408889634f;
 constexpr double TP_LN2 = 0.6931471805599453;
-// Bytes of a row that a warp takes (four rows of 4096 values: 14.7 us with 5 alternatives for 16.4 with blocks of 128 threads; with 20,
-// 30 for 19) and that a block of 128 threads takes where there are few rows (one of 32,000 bf16 values, 5 alternatives: 6.9 us with
-// clusters of 256, 7.3 with those of 128).  Many rows always take 128: their last tile is emptier with 256 (8 x 2047 rows of 50,304 values
-// 221 us for 251).
+// Bytes of a row that a warp takes, up to 8 alternatives (4000 rows of 4000 bf16 values: 20.3 us with 8 for 25.9 with blocks of 128 threads,
+// 57 with 24 for 28) and 20 of half as many (16384 rows of 2000: 57 us with 20 for 103; 300 of 1500 with 24: 22 for 7, as 32 maxima bound
+// the 24th of so few values badly); and that a block of 128 threads takes where there are few rows (one of 32,000 bf16 values, 5
+// alternatives: 6.9 us with clusters of 256, 7.3 with those of 128).  Many rows always take 128: their last tile is emptier with 256 (8 x
+// 2047 rows of 50,304 values 221 us for 251).
 constexpr long long TP_NARROW = 8192, TP_MIDDLE = 32768;
 // Blocks per SM up to which rows are split over clusters, where alternatives are asked for: 64 rows of 128,256 values with 20 of them and a
-// part of the vocabulary masked 16.5 us, with 4 blocks 20.
+// part of the vocabulary masked 16.5 us, with 4 blocks 18.5.
 constexpr long long TP_ROOM = 2;
 constexpr float TP_FAR = -8192.f;          // exponents below are this: their powers are zero, and their products with them too
 
@@ -815,7 +816,7 @@ static int tell_of(const TokenProbsArgs& a, long long rows, float* log_probs, fl
     return H ? (a.top ? tell<T, true, true, N> : tell<T, true, false, N>) : (a.top ? tell<T, false, true, N> : tell<T, false, false, N>);
   };
   const bool many = rows >= 4ll * sm_count_current();
-  const auto go = bytes <= TP_NARROW && a.top <= (2 * bytes <= TP_NARROW ? 24 : 4) ? with(std::integral_constant<int, 32>())
+  const auto go = bytes <= TP_NARROW && a.top <= (2 * bytes <= TP_NARROW ? 20 : 8) ? with(std::integral_constant<int, 32>())
                 : many || bytes <= TP_MIDDLE ? with(std::integral_constant<int, 128>()) : with(std::integral_constant<int, 256>());
   return go(a, rows, log_probs, entropy, top_log_probs, top_tokens, stats, s);
 }
