@@ -12,8 +12,9 @@
 // Alternatives come in the same pass.  The K-th largest of the threads' maxima so far (of 32 of them, the largest of every warp's) is
 // reached by K of the values, and by few others: what is above it goes to a list in shared memory.  The bound is taken anew whenever the
 // values behind it have doubled.  Values that equal it count in the first tile only: later ones come after K that are no
-// smaller.  In the end what is below the last bound is dropped and the rest put in order by counting.  A list that is too short for that
-// (rows of mostly equal values, growing ones) or has missed a NaN is made again word by word, cut down to K after each.
+// smaller.  In the end what is below the last bound is dropped and the rest put in order by counting.  Where the list was too short (rows that
+// grow, or of mostly equal values) the row is read again for what is above the last bound, and for the first values that equal it if these
+// are fewer than K; so it is for -inf, which no list has.  Rows with NaN are gone through word by word, the list cut down to K after each.
 //
 // One B200, device time: 4096 rows of 128,256 bf16 values with entropy 161.8 us (their bytes at the copy's rate: 160.7), the gradient 336
 // (321); 8 x 2047 rows of 50,304, 15 % of them ignored, 219 (214).  6.4 instructions a value, 8.0 with entropy.  64 rows of 128,256
@@ -62,7 +63,7 @@ __device__ __forceinline__ uint32_t tp_key(float x) {
   const uint32_t b = __float_as_uint(x + 0.f);
   return b & 0x80000000u ? ~b : b | 0x80000000u;
 }
-constexpr uint32_t TP_LOWEST = 0x007fffffu;  // of -inf
+constexpr uint32_t TP_LOWEST = 0x007fffffu, TP_ZERO = 0x80000000u;  // of -inf, of 0
 __device__ __forceinline__ float tp_key_value(uint32_t k) { return __uint_as_float(k & 0x80000000u ? k & 0x7fffffffu : ~k); }
 
 __device__ __forceinline__ float tp_exp2(float x) {
@@ -341,7 +342,7 @@ template <int THREADS> __device__ __forceinline__ uint32_t keep_best(List<THREAD
   return static_cast<uint32_t>(l.best[K - 1] >> 32);
 }
 
-// The list of words [from, to), a word of every thread at a time: what comes later counts where its key is above the K-th so far.
+// The list of words [from, to) by their keys, a word of every thread at a time: what comes later counts where its key is above the K-th so far.
 template <typename T, int THREADS> __device__ __noinline__ void gather_slowly(List<THREADS>& l, const RowWords<T>& row, int from, int to, int K) {
   const int tid = threadIdx.x % THREADS;
   uint32_t over = 0u;
@@ -362,6 +363,51 @@ template <typename T, int THREADS> __device__ __noinline__ void gather_slowly(Li
     const int n = l.count;
     tp_sync<THREADS>();
     if (n > TP_KEEP) over = keep_best(l, n, K);
+  }
+}
+
+// The list of words [from, to) with the keys above `over`, which K of them reach (TP_LOWEST: or not); with the first ones that equal it, where
+// the others are fewer than K.  `listed` >= 0: the others are there already, in `some`.
+template <typename T, int THREADS> __device__ __noinline__ void gather_again(List<THREADS>& l, const RowWords<T>& row, int from, int to, uint32_t over, int listed, int K) {
+  constexpr int COUNT = Word<T>::COUNT;
+  const int tid = threadIdx.x % THREADS;
+  const float bound = tp_key_value(over);
+  tp_sync<THREADS>();
+  if (tid < listed) l.entry[tid] = l.some[tid];
+  if (tid == 0) l.count = max(listed, 0);
+  tp_sync<THREADS>();
+  if (listed < 0) {
+    for (int i = from + tid; i < to; i += THREADS) {
+      const Word<T> w = row[i];
+      for (unsigned hits = w.reaching(bound, false); hits; hits &= hits - 1u) {
+        const int k = __ffs(hits) - 1;
+        const uint32_t key = tp_key(w.one(k));
+        if (key <= over) continue;           // a value that counts as zero
+        const int at = atomicAdd(&l.count, 1);
+        if (at < List<THREADS>::ROOM) l.entry[at] = tp_entry(key, i * COUNT - row.lead + k);
+      }
+    }
+    tp_sync<THREADS>();
+  }
+  int n = l.count;
+  tp_sync<THREADS>();                        // all have read the count
+  if (n > List<THREADS>::ROOM) {
+    gather_slowly<T, THREADS>(l, row, from, to, K);
+    return;
+  }
+  for (int base = from; base < to && n < K; base += THREADS) {
+    const int i = base + tid;
+    if (i < to) {
+      const Word<T> w = row[i];
+#pragma unroll
+      for (int k = 0; k < COUNT; ++k) {
+        const int j = i * COUNT - row.lead + k;
+        if (tp_key(w.one(k)) == over && j >= 0 && j < row.V) l.entry[atomicAdd(&l.count, 1)] = tp_entry(over, j);
+      }
+    }
+    tp_sync<THREADS>();
+    n = l.count;
+    tp_sync<THREADS>();
   }
 }
 
@@ -530,15 +576,17 @@ token_probs_kernel(const TokenProbsArgs a, int rows, float* log_probs, float* en
       const bool first = base == lo;
       if (first) {
         over = bound_of(s_list, tp_key(st.m), K, 0);
-        if (head) push(tid < head && tp_key(x_head) >= over, x_head, tid);
+        if (head) push(tid < head && tp_key(x_head) >= over && x_head > -INFINITY, x_head, tid);
       }
-      const float bound = over <= TP_LOWEST ? -INFINITY : tp_key_value(over);
-      if (__any_sync(0xffffffffu, first ? top >= bound : top > bound)) {
+      const bool equal = first && over > TP_LOWEST;
+      // what counts as zero may be a little less
+      const float bound = over <= TP_LOWEST ? -INFINITY : equal && over == TP_ZERO ? -1.17549435e-38f : tp_key_value(over);
+      if (filled <= List<THREADS>::SHARE && __any_sync(0xffffffffu, equal ? top >= bound : top > bound)) {
         // every lane takes the next of its words that have such values, and the next of these: one of each for nearly all
         const int j0 = (base + tid) * COUNT - row.lead;
         unsigned some = 0u;
 #pragma unroll
-        for (int k = 0; k < WORDS; ++k) some |= (first ? most[k] >= bound : most[k] > bound) && base + tid + k * THREADS < hi ? 1u << k : 0u;
+        for (int k = 0; k < WORDS; ++k) some |= (equal ? most[k] >= bound : most[k] > bound) && base + tid + k * THREADS < hi ? 1u << k : 0u;
         while (__any_sync(0xffffffffu, some != 0u)) {
           const int k = some ? __ffs(some) - 1 : 0;
           Word<T> w = now[0];
@@ -546,7 +594,7 @@ token_probs_kernel(const TokenProbsArgs a, int rows, float* log_probs, float* en
           for (int i = 1; i < WORDS; ++i)
 #pragma unroll
             for (int h = 0; h < 4; ++h) w.u[h] = k == i ? now[i].u[h] : w.u[h];
-          unsigned hits = some ? w.reaching(bound, first) : 0u;
+          unsigned hits = some ? w.reaching(bound, equal) : 0u;
           some &= some - 1u;
           while (__any_sync(0xffffffffu, hits != 0u)) {
             const int i = hits ? __ffs(hits) - 1 : 0;
@@ -571,7 +619,7 @@ token_probs_kernel(const TokenProbsArgs a, int rows, float* log_probs, float* en
     st.rescale(m, c);
     o.rescale(m, c);
     st.s += o.s; st.w += o.w;
-    push(there && tp_key(x) >= over, x, behind + lane);
+    push(there && tp_key(x) >= over && x > -INFINITY, x, behind + lane);
   }
   const float most_of_thread = st.m;
   st = tp_join_lanes<32>(st, c);
@@ -585,8 +633,8 @@ token_probs_kernel(const TokenProbsArgs a, int rows, float* log_probs, float* en
     st = tp_join_lanes<WARPS>(st, c);
   }
   if constexpr (TOP) {
-    bool again = st.s != st.s;               // a NaN is missing, or what there was no room for
-    int few = 0, before = 0;
+    int few = 0, before = 0, listed = -1;
+    bool again = false;                      // there was no room for all
 #pragma unroll
     for (int i = 0; i < WARPS; ++i) {
       const int n = s_list.filled[i];
@@ -598,10 +646,15 @@ token_probs_kernel(const TokenProbsArgs a, int rows, float* log_probs, float* en
     if (!again && few <= TP_KEEP) {
       for (int i = lane; i < filled; i += 32) s_list.some[before + i] = mine[i];
       tp_sync<THREADS>();
-    } else if (!again) {
-      // those that reach a last bound: K at least, where the block has as many
+      if (few < K) {                         // values of -inf among the best, or no others in this block
+        again = true;
+        listed = few;
+        over = TP_LOWEST;
+      }
+    } else {
+      // those that reach a last bound: K at least
       over = bound_of(s_list, tp_key(most_of_thread), K, turn ^ 1);
-      for (int i = 0; i < filled; i += 32) {
+      for (int i = 0; i < filled && !again; i += 32) {
         const Entry e = i + lane < filled ? mine[i + lane] : TP_NONE;
         const bool good = e != TP_NONE && static_cast<uint32_t>(e >> 32) >= over;
         const unsigned those = __ballot_sync(0xffffffffu, good);
@@ -612,15 +665,17 @@ token_probs_kernel(const TokenProbsArgs a, int rows, float* log_probs, float* en
       }
       tp_sync<THREADS>();
       few = s_list.few;
-      again = few > List<THREADS>::SOME;
+      again |= few > List<THREADS>::SOME;
     }
-    if (again) {
-      gather_slowly<T, THREADS>(s_list, row, from, to, K);
-      few = s_list.count;
-      for (int i = tid; i < few; i += THREADS) s_list.some[i] = s_list.entry[i];
-      tp_sync<THREADS>();
+    const bool nan = st.s != st.s;
+    if (nan || again) {
+      if (nan) gather_slowly<T, THREADS>(s_list, row, from, to, K);
+      else gather_again<T, THREADS>(s_list, row, from, to, max(over, TP_LOWEST), listed, K);
+      const int n = s_list.count;
+      if (n > 0) take_best(s_list, n, min(n, K));
+    } else {
+      put_in_order(s_list, few, K);
     }
-    put_in_order(s_list, few, K);
   }
   if constexpr (ROWS == 1) {
     if (ctas > 1) {

@@ -137,6 +137,41 @@ def test_order_of_the_vocabulary(rows, dtype):
         _check(logits[:7], tokens[:7], 20)
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("rows,V", [(1, 129), (1, 33000), (4, 128256), (900, 2600), (300, 9001)])
+def test_few_values_above_the_others(rows, V, dtype):
+    """Masks that leave fewer tokens than alternatives, or these in a few places; rows of one value but for some, and what grows behind that."""
+    j = torch.arange(V, device=DEV)
+    g = torch.Generator(device=DEV).manual_seed(V)
+    x = torch.randn(V, generator=g, device=DEV)
+    kinds = [torch.where(torch.rand(V, generator=g, device=DEV) < 0.9999, -INF, x), torch.where(j % 1024 < 16, x, -INF), torch.where(j % 256 == 9, x, -INF),
+             torch.where(j >= V - 7, x, -INF), torch.where(j % 511 == 0, 1.0, 0.0), torch.where(j % 97 == 96, -1.0, 0.0), torch.where(j < V // 2, 2.0, j / V * 4),
+             torch.where(j < V - 40, -x.abs(), 5.0), torch.where(j % 8 == 7, 3.0, j / V), torch.where(j < 3, 3.0, -INF), j / V * 8 + x / 16]
+    some = torch.stack(kinds).repeat(-(-rows // len(kinds)), 1)[:max(rows, len(kinds))].to(dtype)
+    tokens = some.float().argmax(-1)
+    for top in (1, 5, 20, 32):
+        if rows == 1:
+            for i in range(len(kinds)):
+                _check(some[i:i + 1], tokens[i:i + 1], top, gradient=False)
+        else:
+            _check(some, tokens, top, gradient=False)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("V", [65, 4097, 70000])
+def test_magnitudes_that_count_as_zero(V, dtype):
+    """Below 2^-126 they are all equal, so that the first of them come first."""
+    small = torch.tensor(2.0 ** -130, device=DEV)
+    j = torch.arange(V, device=DEV)
+    kinds = [(-small).expand(V), torch.where(j < V // 2, 0.0, small), torch.where(j % 2 == 0, -small, small), torch.where(j % 50 == 3, -small, -1.0),
+             torch.where(j % 3 == 0, -small, -INF), torch.where(j == V - 1, small, -small), torch.where(j % 2 == 0, -small, torch.tensor(-2.0 ** -126, device=DEV))]
+    logits = torch.stack(kinds).to(dtype)
+    want = torch.where(logits.float().abs() < 2.0 ** -126, 0.0, logits.float()).to(dtype)
+    tokens = torch.zeros(len(kinds), dtype=torch.int64, device=DEV)
+    for top in (1, 20):
+        check_told(ops.token_log_probs(logits, tokens, entropy=True, top=top), told(want, tokens, top), V, top)
+
+
 def test_tokens_outside_the_vocabulary():
     logits, _ = _case((5, 77), torch.bfloat16)
     tokens = torch.tensor([77, -1, -100, 76, 1 << 40], device=DEV)
