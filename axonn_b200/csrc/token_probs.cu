@@ -368,6 +368,8 @@ template <typename T, int THREADS> __device__ __noinline__ void gather_slowly(Li
 
 // The list of words [from, to) with the keys above `over`, which K of them reach (TP_LOWEST: or not); with the first ones that equal it, where
 // the others are fewer than K.  `listed` >= 0: the others are there already, in `some`.
+// A second reading, mostly from the L2: 1000 rows of 128,256 bf16 values that grow, 5 alternatives, 274 us (random ones 56); word by word with
+// the list cut down each time 2606.
 template <typename T, int THREADS> __device__ __noinline__ void gather_again(List<THREADS>& l, const RowWords<T>& row, int from, int to, uint32_t over, int listed, int K) {
   constexpr int COUNT = Word<T>::COUNT;
   const int tid = threadIdx.x % THREADS;
