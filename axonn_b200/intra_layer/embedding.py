@@ -151,20 +151,19 @@ class Embedding(torch.nn.Module):
 
     def rows(self, first, count, device):
         """``self(torch.arange(first, first + count, device=device))``.  Without gradients, collectives or hooks the rows are a
-        slice of the table: two launches less for the positions of a short prompt (logits of a two-layer GPT 364 -> 351 us)."""
+        slice of the table: two launches less for the positions of a short prompt (logits of a two-layer GPT 364 -> 351 us).
+        Rows that the table has not got are an ``IndexError``."""
+        if count > 0 and not 0 <= first <= self.num_embeddings - count:
+            # torch's own refusal, of indices on the host: a GPU's lookup of them ends the program, or gives NaN
+            return F.embedding(torch.arange(first, first + count), torch.empty(1, 1).expand(self.num_embeddings, 1))
         w = self.weight
         if (plain_layer(self) and self.scale == 1.0 and self.depth_group_size == 1 and self.expert_mode and self.max_norm is None
-                and 0 <= first and first + count <= self.num_embeddings and no_graph(w) and w.device == torch.device(device)
+                and count >= 0 and no_graph(w) and w.device == torch.device(device)
                 and w.is_contiguous()):
             return w.detach().view(self.num_embeddings, self.local_out_features)[first:first + count]
-        ids = torch.arange(first, first + count, device=device)
-        # rows that the table has not got are refused as torch.nn.functional.embedding does it; the kernel would give NaN
-        return self(ids) if 0 <= first and first + count <= self.num_embeddings else self._look_up(ids, False)
+        return self(torch.arange(first, first + count, device=device))
 
     def forward(self, x):
-        return self._look_up(x, True)
-
-    def _look_up(self, x, kernels):
         if self._p2p_rows(x):
             x = _EmbeddingRowsP2P.apply(x, self.weight, self.depth_group,
                                         self.num_embeddings // self.depth_group_size, self.local_out_features,
@@ -178,7 +177,7 @@ class Embedding(torch.nn.Module):
         if self.depth_group_size > 1 or not no_graph(weight):
             weight = ForwardGather_BackwardReduceScatter.apply(weight, self.depth_group)
         weight = weight.reshape(self.local_in_features, self.local_out_features)
-        if (kernels and self.max_norm is None and not self.scale_grad_by_freq and not self.sparse
+        if (self.max_norm is None and not self.scale_grad_by_freq and not self.sparse
                 and weight.dtype in ops.EMBEDDING_TYPES):
             x = ops.embedding(x, weight, self.scale, self.padding_idx)
         else:
