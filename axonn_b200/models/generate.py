@@ -40,6 +40,8 @@ def score_tokens(model, tokens, lengths=None, entropy=False, top=0, temperature=
     distillation loss is a sum of them.  Every rank of a tensor-parallel group passes the same ``tokens``."""
     if tokens.ndim != 2 or tokens.dtype != torch.int64 or tokens.shape[1] < 2:
         raise ValueError(f"sequences of two tokens and more are scored, int64 [B, S], not {tokens.dtype} {list(tokens.shape)}")
+    if hasattr(model, "pos_emb") and tokens.shape[1] > model.cfg.seq_len:
+        raise ValueError(f"sequences of {tokens.shape[1]} tokens for a model that has learned {model.cfg.seq_len} positions")
     targets = tokens[:, 1:]
     if lengths is not None:
         lengths = torch.as_tensor(lengths, device=tokens.device)

@@ -35,3 +35,35 @@ def _rows_outside(rank, world):
 
 def test_rows_that_the_table_has_not_got():
     run_distributed(_rows_outside, 1)
+
+
+def _model(family, vocab=96, seq_len=40):
+    from axonn_b200.models import GPT, GPTConfig, Llama, LlamaConfig
+
+    torch.manual_seed(4)
+    shape = dict(n_layers=2, hidden=64, n_heads=4, ffn=128, vocab=vocab, seq_len=seq_len)
+    return GPT(GPTConfig(**shape), dtype=torch.float32) if family == "gpt" else Llama(LlamaConfig(n_kv_heads=2, **shape), dtype=torch.float32)
+
+
+def _scores_of_long_sequences(rank, world):
+    """A model that has learned its positions refuses more of them before it looks any up; rotary ones go on."""
+    from axonn_b200.models import score_tokens
+
+    _grid(world)
+    g = torch.Generator().manual_seed(0)
+    for family in ("gpt", "llama"):
+        model = _model(family, seq_len=12)
+        for length in (11, 12, 13, 20):
+            tokens = torch.randint(0, 96, (2, length), generator=g)
+            if family == "gpt" and length > 12:
+                model.pos_emb.register_forward_pre_hook(lambda *_: pytest.fail("positions are looked up"))
+                with pytest.raises(ValueError, match="12"):
+                    score_tokens(model, tokens)
+                with pytest.raises(ValueError, match="12"):
+                    score_tokens(model, tokens, lengths=[12, 3])
+            else:
+                assert score_tokens(model, tokens).log_probs.shape == (2, length - 1)
+
+
+def test_scores_of_long_sequences():
+    run_distributed(_scores_of_long_sequences, 1)
