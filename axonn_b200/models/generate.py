@@ -33,11 +33,18 @@ def parallel_argmax(logits, group=None):
     return indices.gather(-1, best).squeeze(-1)
 
 
+def _of_the_table(model, tokens, there):
+    """``tokens`` with a token of the model's vocabulary wherever they are not ``there`` and none (-1, a label's -100): of such a number a GPU's
+    lookup makes NaN, which attention hands on to the tokens in front of it (a weight of zero times NaN)."""
+    vocab = getattr(getattr(model, "cfg", None), "vocab", None)
+    return tokens if vocab is None else torch.where(there | (tokens >= 0) & (tokens < vocab), tokens, 0)
+
+
 def score_tokens(model, tokens, lengths=None, entropy=False, top=0, temperature=1.0):
     """What ``model`` makes of given sequences: the ``ops.TokenLogProbs`` of ``tokens[:, 1:]`` (``tokens [B, S]``, int64), each after the
-    tokens in front of it, all of shape ``[B, S - 1]``.  Row ``r`` is ``tokens[r, :lengths[r]]`` (``None``: all of it); behind that the
-    results are zeros (alternatives -1).  With gradients enabled the results are functions of the model's parameters: a policy-gradient or
-    distillation loss is a sum of them.  Every rank of a tensor-parallel group passes the same ``tokens``."""
+    tokens in front of it, all of shape ``[B, S - 1]``.  Row ``r`` is ``tokens[r, :lengths[r]]`` (``None``: all of it); behind that any
+    numbers may stand, and the results are zeros (alternatives -1).  With gradients enabled the results are functions of the model's
+    parameters: a policy-gradient or distillation loss is a sum of them.  Every rank of a tensor-parallel group passes the same ``tokens``."""
     if tokens.ndim != 2 or tokens.dtype != torch.int64 or tokens.shape[1] < 2:
         raise ValueError(f"sequences of two tokens and more are scored, int64 [B, S], not {tokens.dtype} {list(tokens.shape)}")
     if hasattr(model, "pos_emb") and tokens.shape[1] > model.cfg.seq_len:
@@ -47,8 +54,9 @@ def score_tokens(model, tokens, lengths=None, entropy=False, top=0, temperature=
         lengths = torch.as_tensor(lengths, device=tokens.device)
         if lengths.shape != tokens.shape[:1]:
             raise ValueError(f"lengths must be {tokens.shape[0]} numbers, not {list(lengths.shape)}")
-        places = torch.arange(1, tokens.shape[1], device=tokens.device)
-        targets = targets.masked_fill(places >= lengths[:, None], _LEFT_OUT)
+        there = torch.arange(tokens.shape[1], device=tokens.device) < lengths[:, None]
+        targets = targets.masked_fill(~there[:, 1:], _LEFT_OUT)
+        tokens = _of_the_table(model, tokens, there)
     logits = model(tokens)                                                   # [B, S, vocab / |group|]
     return ops.token_log_probs(logits[:, :-1], targets, entropy, top, temperature, getattr(model.head, "group", None), _LEFT_OUT)
 
@@ -83,7 +91,8 @@ def greedy_generate(model, tokens, max_new_tokens: int, eos_id=None, cache_dtype
 
     With ``cache_dtype`` (``torch.float8_e4m3fn`` or ``torch.int8``) keys and values are kept in a ``BlockCache`` with blocks of
     ``block_tokens`` and every token is evaluated once; scores differ by the rounding of what is stored.  Prompts may then differ in
-    length: row ``r`` is ``tokens[r, :prompt_lengths[r]]``, and its new tokens follow there; what is left of a row is ``eos_id`` (or 0).
+    length: row ``r`` is ``tokens[r, :prompt_lengths[r]]`` (behind that any numbers may stand), and its new tokens follow there; what is left of a
+    row is ``eos_id`` (or 0).
     A ``Mixtral``'s expert capacity is that of a step's tokens, one per row, padding of the prompts among them: what is dropped differs
     from an evaluation of whole prefixes unless ``capacity_factor`` leaves room for all.
 
@@ -145,13 +154,14 @@ def _greedy_cached(model, tokens, max_new_tokens, eos_id, limit, dtype, prompt_l
     B, S = tokens.shape
     pad = 0 if eos_id is None else eos_id
     out = torch.full((B, S + room), pad, dtype=tokens.dtype, device=tokens.device)
-    out[:, :S] = torch.where(torch.arange(S, device=tokens.device) < lengths[:, None], tokens, pad)
+    there = torch.arange(S, device=tokens.device) < lengths[:, None]
+    out[:, :S] = torch.where(there, tokens, pad)
     if room == 0:
         return out
     cache = BlockCache(model, B, S + room, block_tokens, dtype)
     done = torch.zeros(B, dtype=torch.bool, device=tokens.device)
     cache.plan(S, lengths)
-    step, at = tokens, lengths.long()[:, None]
+    step, at = tokens if prompt_lengths is None else _of_the_table(model, tokens, there), lengths.long()[:, None]
     for i in range(room):
         logits = model(step, cache=cache)                                    # [B, 1, vocab / |group|]
         nxt = parallel_argmax(logits[:, -1], getattr(model.head, "group", None)).to(tokens.dtype)
@@ -190,7 +200,8 @@ def beam_generate(model, tokens, max_new_tokens: int, beams: int, eos_id=None, l
             raise ValueError(f"1 to {ops.MOST_BEAMS} beams, not {beams}")
         pad = 0 if eos_id is None else eos_id
         out = torch.full((B, beams, S + room), pad, dtype=tokens.dtype, device=device)
-        out[:, :, :S] = torch.where(torch.arange(S, device=device) < lengths[:, None], tokens, pad)[:, None]
+        there = torch.arange(S, device=device) < lengths[:, None]
+        out[:, :, :S] = torch.where(there, tokens, pad)[:, None]
         scores = torch.full((B, beams), float("-inf"), device=device)
         scores[:, 0] = 0.0
         if room == 0:
@@ -199,7 +210,8 @@ def beam_generate(model, tokens, max_new_tokens: int, beams: int, eos_id=None, l
         done = None if eos_id is None else torch.zeros(B, beams, dtype=torch.bool, device=device)
         count = torch.zeros(B, beams, dtype=torch.int64, device=device)      # new tokens of every beam
         cache.plan(S, lengths)
-        step, at, length = tokens, lengths.long()[:, None, None].expand(B, beams, 1), S
+        step = tokens if prompt_lengths is None else _of_the_table(model, tokens, there)
+        at, length = lengths.long()[:, None, None].expand(B, beams, 1), S
         for i in range(room):
             logits = model(step, cache=cache)[:, -1]
             if group is not None:

@@ -67,3 +67,34 @@ def _scores_of_long_sequences(rank, world):
 
 def test_scores_of_long_sequences():
     run_distributed(_scores_of_long_sequences, 1)
+
+
+def _padding_outside_the_table(rank, world, family):
+    """What stands behind the rows' ends is no token: any number may, and the results do not see it."""
+    from axonn_b200.models import beam_generate, greedy_generate, score_tokens
+
+    _grid(world)
+    model, g = _model(family), torch.Generator().manual_seed(0)
+    tokens, lengths = torch.randint(0, 96, (3, 14), generator=g), torch.tensor([14, 5, 1])
+    behind = torch.arange(14) >= lengths[:, None]
+    calls = [lambda t: score_tokens(model, t, lengths, entropy=True, top=3), lambda t: score_tokens(model, t, lengths.tolist()),
+             lambda t: (greedy_generate(model, t, 4, cache_dtype=torch.int8, prompt_lengths=lengths),),
+             lambda t: beam_generate(model, t, 4, 3, cache_dtype=torch.int8, prompt_lengths=lengths)]
+    for call in calls:
+        want = call(tokens.masked_fill(behind, 0))
+        for pad in (-1, -100, 96, 1 << 40, 7):
+            given = tokens.masked_fill(behind, pad)
+            kept = given.clone()
+            got = call(given)
+            assert torch.equal(given, kept)
+            for a, b in zip(got, want):
+                assert (a is None) == (b is None) and (a is None or torch.equal(a, b)), pad
+    for bad in (lambda: score_tokens(model, tokens.masked_fill(tokens == tokens[0, 3], 96), lengths),
+                lambda: score_tokens(model, tokens.masked_fill(behind, -1))):
+        with pytest.raises(IndexError):                   # within the rows there are tokens only
+            bad()
+
+
+@pytest.mark.parametrize("family", ["gpt", "llama"])
+def test_padding_outside_the_table(family):
+    run_distributed(_padding_outside_the_table, 1, family)

@@ -1,0 +1,57 @@
+"""Calls of the vocabulary's operators, and of the functions on them, at the ends of what they take: on a GPU."""
+
+import pytest
+import torch
+import torch.distributed as dist
+
+from axonn_b200 import ops
+from axonn_b200.ops import _lib
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda"
+TYPES = [torch.bfloat16, torch.float16, torch.float32]
+
+
+@pytest.fixture(scope="module", autouse=True)
+def _grid():
+    from axonn_b200 import axonn as ax
+
+    if not dist.is_initialized():
+        dist.init_process_group("nccl", store=dist.HashStore(), rank=0, world_size=1)
+    if not ax.is_initialized:
+        ax.init(G_inter=1, G_data=1, G_intra_r=1, G_intra_c=1, G_intra_d=1)
+
+
+def _model(family):
+    from axonn_b200.models import GPT, GPTConfig, Llama, LlamaConfig
+
+    torch.manual_seed(0)
+    shape = dict(n_layers=2, hidden=256, n_heads=4, ffn=512, vocab=1000, seq_len=256)
+    model = GPT(GPTConfig(**shape), dtype=torch.bfloat16) if family == "gpt" else Llama(LlamaConfig(n_kv_heads=2, **shape), dtype=torch.bfloat16)
+    return model.to(DEV)
+
+
+@pytest.mark.parametrize("family", ["gpt", "llama"])
+def test_padding_outside_the_table(family):
+    """What stands behind the rows' ends is no token: any number may, and neither the results nor the gradients see it."""
+    from axonn_b200.models import beam_generate, greedy_generate, score_tokens
+
+    model, g = _model(family), torch.Generator(device=DEV).manual_seed(1)
+    tokens, lengths = torch.randint(0, 1000, (4, 77), generator=g, device=DEV), torch.tensor([77, 40, 2, 1], device=DEV)
+    behind = torch.arange(77, device=DEV) >= lengths[:, None]
+
+    def scored(t):
+        model.zero_grad(set_to_none=True)
+        r = score_tokens(model, t, lengths, entropy=True, top=3)
+        (r.log_probs.sum() + r.entropy.sum()).backward()
+        return [x.detach() for x in r] + [p.grad for p in model.parameters()]
+
+    def generated(t):
+        return [greedy_generate(model, t, 5, cache_dtype=torch.int8, prompt_lengths=lengths),
+                *beam_generate(model, t, 5, 3, cache_dtype=torch.int8, prompt_lengths=lengths)]
+
+    for call in (scored, generated):
+        want = call(tokens.masked_fill(behind, 0))
+        assert all(bool(x.isfinite().all()) for x in want)
+        for pad in (-1, -100, 1000, 1 << 40):
+            assert all(torch.equal(a, b) for a, b in zip(call(tokens.masked_fill(behind, pad)), want)), pad
