@@ -342,7 +342,7 @@ int axb_beam_select(const void* logits, const float* scores, const void* done, i
 
 /* ---- log-probabilities of given tokens (token_probs.cu): rows of V logits at batch * batch_stride + row * row_stride (strides in values),
  * a slice of a vocabulary of `total` that begins at `start`; tokens [batches, per_batch] int64 (strides in words) or NULL, rows of the token
- * `ignored` are left out; scale: 1 / temperature.  stats [rows, 4] fp32, 16-byte aligned, is written in any case.  whole: the slice is all of
+ * `ignored` are left out; scale: 1 / temperature, 2^-100 to 2^100.  stats [rows, 4] fp32, 16-byte aligned, is written in any case.  whole: the slice is all of
  * the vocabulary, and log_probs and entropy [rows] (or NULL) and the top log-probabilities [rows, top] are finished and stats (m, s, H,
  * log s), H with an entropy only;
  * otherwise stats are (m, s, w, z_t) of the slice and the top logits are as they are.

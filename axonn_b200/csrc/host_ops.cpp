@@ -601,7 +601,7 @@ PyObject* py_token_log_probs(PyObject*, PyObject* const* a, Py_ssize_t n) {
   if (d == 0 || d > 3 || dtype_code(logits) < 0 || logits.numel() == 0 || logits.get_device() != c10::cuda::current_device() ||
       (logits.stride(d - 1) != 1 && logits.size(d - 1) != 1) || logits.size(d - 1) > (1 << 30) || logits.numel() / logits.size(d - 1) > INT32_MAX ||
       top < 0 || top > std::min<int64_t>(32, logits.size(d - 1)) || (!tokens.defined() && !entropy && !top) ||
-      !(scale > 0 && std::isfinite(scale) && std::isfinite(static_cast<float>(scale)) && static_cast<float>(scale) > 0))
+      !(scale >= 0x1p-100 && scale <= 0x1p100))
     Py_RETURN_NONE;
   if (tokens.defined() && (tokens.scalar_type() != at::kLong || tokens.device() != logits.device() || tokens.sizes() != logits.sizes().slice(0, d - 1)))
     Py_RETURN_NONE;

@@ -44,6 +44,8 @@ constexpr long long TP_NARROW = 8192, TP_MIDDLE = 32768;
 // Blocks per SM up to which rows are split over clusters, where alternatives are asked for: 64 rows of 128,256 values with 20 of them and a
 // part of the vocabulary masked 16.5 us, with 4 blocks 18.5.
 constexpr long long TP_ROOM = 2;
+// Factors 1 / temperature: a flushed one times -inf would be NaN, and so would the maximum's zero times one that overflows.
+constexpr float TP_COLDEST = 0x1p-100f;
 constexpr float TP_FAR = -8192.f;          // exponents below are this: their powers are zero, and their products with them too
 
 struct TokenProbsArgs {
@@ -832,7 +834,7 @@ static int fill(TokenProbsArgs& a, const char* what, const void* logits, long lo
     return -1;
   }
   if (batches < 1 || per_batch < 1 || static_cast<long long>(batches) * per_batch > 0x7fffffffll || V < 1 || V > (1 << 30) || top < 0 ||
-      top > TP_MOST || top > V || !(scale > 0.f) || dtype < 0 || dtype > 2) {
+      top > TP_MOST || top > V || !(scale >= TP_COLDEST && scale <= 1.f / TP_COLDEST) || dtype < 0 || dtype > 2) {
     set_error("%s: %d x %d rows of %d values, %d alternatives, scale %g, type %d", what, batches, per_batch, V, top, scale, dtype);
     return -1;
   }

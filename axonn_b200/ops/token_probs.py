@@ -16,6 +16,10 @@ from .kv_cache import _elsewhere
 
 MOST_ALTERNATIVES = 32
 _DT = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
+# Of temperatures; the hottest is its reciprocal.  32 bits hold the factor 1 / T, with log2 e and with gradients, as a normal number (one that is
+# flushed to zero would make NaN of a masked token, one that overflows of the likeliest), and differences of logits that they do not
+# hold (2^128) are no less than 2^28 beside a temperature: their exponential is zero.
+_COLDEST = 2.0 ** -100
 
 
 class TokenLogProbs(NamedTuple):
@@ -36,7 +40,7 @@ def token_log_probs(logits, tokens=None, entropy=False, top=0, temperature=1.0, 
     Positions whose token is ``ignore_index`` are not looked at: they give zeros, alternatives of -1, and no gradient.  Any other number
     outside the vocabulary gives NaN.  Logits of ``-inf`` are tokens that cannot come; a position that leaves none, or that has a NaN or
     ``+inf`` among its logits, is NaN throughout (a NaN counts as the largest logit among the alternatives).  On a GPU logits below
-    2^-126 count as zero.
+    2^-126 count as zero.  Temperatures go from 2^-100 to 2^100.
 
     Everything but ``top_tokens`` can be differentiated once by the logits, which may have any strides (such as ``logits[:, :-1]``) and are
     left as they are.  With ``group`` the last dimension is this rank's contiguous slice of the vocabulary, of equal size on all ranks (rank
@@ -57,8 +61,8 @@ def token_log_probs(logits, tokens=None, entropy=False, top=0, temperature=1.0, 
         raise ValueError(f"a vocabulary of at most {1 << 30}, not {V}")
     if not 0 <= top <= min(MOST_ALTERNATIVES, V):
         raise ValueError(f"0 to {min(MOST_ALTERNATIVES, V)} alternatives of {V} tokens, not {top}")
-    if not (temperature > 0 and math.isfinite(temperature) and 0 < _f32(1 / temperature) < math.inf):
-        raise ValueError(f"the temperature is a positive number, not {temperature}")
+    if not _COLDEST <= temperature <= 1 / _COLDEST:
+        raise ValueError(f"the temperature is a positive number from {_COLDEST:.1e} to {1 / _COLDEST:.1e}, not {temperature}")
     if tokens is None:
         if not entropy and not top:
             raise ValueError("without tokens there is something to say of the entropy or the alternatives only")
@@ -69,10 +73,6 @@ def token_log_probs(logits, tokens=None, entropy=False, top=0, temperature=1.0, 
             raise ValueError(f"tensors on {dev} and {tokens.device}")
     out = _TokenLogProbsFn.apply(logits, tokens, bool(entropy), int(top), 1 / temperature, group, ignore_index)
     return TokenLogProbs(*out)
-
-
-def _f32(x):
-    return torch.tensor(x, dtype=torch.float32).item()
 
 
 def _as_rows(t, dims):

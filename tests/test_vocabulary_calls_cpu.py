@@ -1,9 +1,15 @@
 """Calls of the vocabulary's operators, and of the layers and functions on them, at the ends of what they take: on the CPU."""
 
+import shutil
+
 import pytest
 import torch
 
+from axonn_b200 import ops
+from axonn_b200.ops import _lib
+
 from _dist import run_distributed
+from _vocabulary_ends import COLD, HOT, check_ends_of_temperature, ends_of_temperature
 
 
 def _grid(world, depth=1):
@@ -98,3 +104,27 @@ def _padding_outside_the_table(rank, world, family):
 @pytest.mark.parametrize("family", ["gpt", "llama"])
 def test_padding_outside_the_table(family):
     run_distributed(_padding_outside_the_table, 1, family)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("temperature", [COLD, HOT])
+def test_ends_of_the_temperature(dtype, temperature):
+    check_ends_of_temperature(*ends_of_temperature(dtype, "cpu"), temperature)
+
+
+def test_temperatures_that_are_refused():
+    """32 bits hold neither the factor 1 / temperature nor that with log2 e at some positive numbers: NaN for a maximum, for what is masked."""
+    logits, tokens = ends_of_temperature(torch.float32, "cpu")
+    for temperature in (1e-39, 3e-39, 1e-38, COLD / 2, 2 * HOT, 9e37, 1e38, 3e38, 0.0, -1.0, float("inf"), float("nan")):
+        with pytest.raises(ValueError, match="temperature"):
+            ops.token_log_probs(logits, tokens, temperature=temperature)
+
+
+@pytest.mark.skipif(not (_lib.available() or shutil.which("nvcc")), reason="native library not built")
+def test_factors_that_the_launchers_refuse():
+    """Addresses that are never used: the calls are refused on the host."""
+    L, p = _lib.lib(), 4096
+    for scale in (2.0 ** 101, 2.0 ** -101, 3e38, 1e-39, float("inf"), float("nan"), 0.0, -1.0):
+        for call in (lambda: L.axb_token_log_probs(p, 8, 8, p, 1, 1, p, p, p, p, p, 1, 1, 8, 0, 8, 0, scale, -100, 1, 0, None),
+                     lambda: L.axb_token_log_probs_bwd(p, 8, 8, p, 1, 1, p, p, p, p, p, p, 1, 1, 8, 0, 8, 0, scale, -100, 0, None)):
+            assert call() == -1 and b"scale" in L.axb_last_error()

@@ -7,6 +7,8 @@ import torch.distributed as dist
 from axonn_b200 import ops
 from axonn_b200.ops import _lib
 
+from _vocabulary_ends import COLD, HOT, check_ends_of_temperature, ends_of_temperature
+
 pytestmark = pytest.mark.gpu
 DEV = "cuda"
 TYPES = [torch.bfloat16, torch.float16, torch.float32]
@@ -55,3 +57,18 @@ def test_padding_outside_the_table(family):
         assert all(bool(x.isfinite().all()) for x in want)
         for pad in (-1, -100, 1000, 1 << 40):
             assert all(torch.equal(a, b) for a, b in zip(call(tokens.masked_fill(behind, pad)), want)), pad
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("temperature", [COLD, HOT])
+def test_ends_of_the_temperature(dtype, temperature, monkeypatch):
+    check_ends_of_temperature(*ends_of_temperature(dtype, DEV), temperature)
+    monkeypatch.setattr(_lib, "_HOST", None)
+    check_ends_of_temperature(*ends_of_temperature(dtype, DEV), temperature)
+
+
+def test_temperatures_that_are_refused():
+    logits, tokens = ends_of_temperature(torch.float32, DEV)
+    for temperature in (1e-39, 3e-39, COLD / 2, 2 * HOT, 9e37, 3e38, 0.0, -1.0, float("inf"), float("nan")):
+        with pytest.raises(ValueError, match="temperature"):
+            ops.token_log_probs(logits, tokens, temperature=temperature)
