@@ -478,7 +478,8 @@ sum_rows_kernel(const uint2* __restrict__ pairs, int n, const T* __restrict__ dy
     for (int j = 0; j < N; ++j) if (col + c * STEP < H) to_part[c * STEP + j] = sum[c][j];
 }
 
-// The pieces of long segments, in their order.
+// The pieces of long segments: every eighth one by the same warp, then the warps' sums.  blockIdx.x: columns (there may be more than the 65,535
+// that the grid's other dimensions have), blockIdx.y: segments.
 template <typename T>
 __global__ void __launch_bounds__(JOIN_THREADS)
 join_rows_kernel(const uint2* __restrict__ pairs, const int* __restrict__ pieces, int chunks, int H, int Hp, float scale,
@@ -488,7 +489,7 @@ join_rows_kernel(const uint2* __restrict__ pairs, const int* __restrict__ pieces
   __shared__ float4 s_sum[JOIN_THREADS / 32][32];
   pdl_launch_next();
   pdl_wait();
-  const int tid = threadIdx.x, lane = tid & 31, w = tid >> 5, col = blockIdx.y * JOIN_COLS + lane * 4;
+  const int tid = threadIdx.x, lane = tid & 31, w = tid >> 5, col = blockIdx.x * JOIN_COLS + lane * 4;
   unsigned seen = 0;
   for (int c0 = 0; c0 < chunks; c0 += JOIN_THREADS) {
     const int own = c0 + tid < chunks ? pieces[c0 + tid] : 0;
@@ -500,8 +501,8 @@ join_rows_kernel(const uint2* __restrict__ pairs, const int* __restrict__ pieces
     for (int i = 0; i < JOIN_THREADS / 32; ++i) { if (i < w) before += s_warp[i]; count += s_warp[i]; }
     if (own > 0) s_begin[before + __popc(flags & ((1u << lane) - 1u))] = make_int2(c0 + tid, own);
     __syncthreads();
-    // every gridDim.x-th of all
-    for (int i = static_cast<int>((blockIdx.x + gridDim.x - seen % gridDim.x) % gridDim.x); i < count; i += gridDim.x) {
+    // every gridDim.y-th of all
+    for (int i = static_cast<int>((blockIdx.y + gridDim.y - seen % gridDim.y) % gridDim.y); i < count; i += gridDim.y) {
       const int2 begin = s_begin[i];
       const uint32_t token = pairs[static_cast<long long>(begin.x) * CHUNK + CHUNK - 1].x;
       float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
@@ -681,7 +682,7 @@ static int sum_rows(const void* sorted, int n, const void* dy, long long pitch, 
                       pitch, V, H, static_cast<int>(work.Hp), scale, static_cast<const uint8_t*>(sorted), static_cast<T*>(dtable), partial, words,
                       slices, sum_blocks, zero_rows));
   const int full = n / CHUNK;                    // a long segment fills one chunk and begins in another
-  AXB_CUDA(pdl_launch(join_rows_kernel<T>, dim3(full / 2 < JOIN_BLOCKS ? full / 2 : JOIN_BLOCKS, static_cast<unsigned>((work.Hp + JOIN_COLS - 1) / JOIN_COLS)),
+  AXB_CUDA(pdl_launch(join_rows_kernel<T>, dim3(static_cast<unsigned>((work.Hp + JOIN_COLS - 1) / JOIN_COLS), full / 2 < JOIN_BLOCKS ? full / 2 : JOIN_BLOCKS),
                       dim3(JOIN_THREADS), 0, s, pairs, static_cast<const int*>(words), full, H, static_cast<int>(work.Hp), scale,
                       static_cast<const float*>(partial), static_cast<T*>(dtable)));
   return 0;

@@ -72,3 +72,17 @@ def test_temperatures_that_are_refused():
     for temperature in (1e-39, 3e-39, COLD / 2, 2 * HOT, 9e37, 3e38, 0.0, -1.0, float("inf"), float("nan")):
         with pytest.raises(ValueError, match="temperature"):
             ops.token_log_probs(logits, tokens, temperature=temperature)
+
+
+def test_gradient_of_wide_tables():
+    """More blocks of columns than a grid has rows of blocks.  Small whole numbers, whose sums are exact."""
+    V, H, n = 3, 65535 * 128 + 8, 300
+    g = torch.Generator(device=DEV).manual_seed(0)
+    weight = torch.randn(V, H, generator=g, device=DEV).bfloat16().requires_grad_()
+    tokens = torch.cat([torch.ones(200, dtype=torch.int64, device=DEV), torch.randint(0, V, (n - 200,), generator=g, device=DEV)])
+    dy = torch.randint(-3, 4, (H,), generator=g, device=DEV).bfloat16().expand(n, H)
+    out = ops.embedding(tokens, weight)
+    assert torch.equal(out[::37], weight.detach()[tokens[::37]])
+    (grad,) = torch.autograd.grad(out, weight, dy)
+    for v, count in enumerate(torch.bincount(tokens, minlength=V).tolist()):
+        assert torch.equal(grad[v], (dy[0].float() * count).bfloat16())
