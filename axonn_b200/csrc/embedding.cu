@@ -2,7 +2,7 @@
 //
 //   out_i = scale table[t_i];   dtable_v = scale sum_{i: t_i = v} dy_i   (nothing of the padding token)
 // A token outside the table gives a row of NaN and has no gradient.  Sums are 32-bit, in an order that the tokens alone decide, and
-// rounded once.
+// rounded once; numbers below 2^-126 are kept.
 //
 // Both are bound by the rows' bytes.  The gradient sorts (token, place) pairs and sums along the sorted list, so that every row of the
 // gradient is written once, by one block, and no addition depends on when a block runs:
@@ -49,6 +49,17 @@ template <typename T> __device__ __forceinline__ T from_float(float x) {
   if constexpr (__is_same(T, float)) return x;
   else if constexpr (__is_same(T, __half)) return __float2half_rn(x);
   else return __float2bfloat16_rn(x);
+}
+// Sums and products that keep numbers below 2^-126, which the build's fast mathematics flushes to zero.
+__device__ __forceinline__ float plus(float a, float b) {
+  float c;
+  asm("add.rn.f32 %0, %1, %2;" : "=f"(c) : "f"(a), "f"(b));
+  return c;
+}
+__device__ __forceinline__ float times(float a, float b) {
+  float c;
+  asm("mul.rn.f32 %0, %1, %2;" : "=f"(c) : "f"(a), "f"(b));
+  return c;
 }
 
 // N values that are moved at once
@@ -102,7 +113,7 @@ embedding_kernel(const I* __restrict__ tokens, long long n, const T* __restrict_
 #pragma unroll
           for (int k = 0; k < PIECES; ++k)
 #pragma unroll
-            for (int i = 0; i < N; ++i) p[r][k].v[i] = from_float<T>(to_float(p[r][k].v[i]) * by);
+            for (int i = 0; i < N; ++i) p[r][k].v[i] = from_float<T>(times(to_float(p[r][k].v[i]), by));
         }
 #pragma unroll
         for (int k = 0; k < PIECES; ++k)
@@ -370,14 +381,14 @@ sum_few_rows_kernel(const I* __restrict__ tokens, int n, const T* __restrict__ d
 #pragma unroll
       for (int c = 0; c < PIECES; ++c)
 #pragma unroll
-        for (int j = 0; j < N; ++j) sum[c][j] += to_float(p[k][c].v[j]);
+        for (int j = 0; j < N; ++j) sum[c][j] = plus(sum[c][j], to_float(p[k][c].v[j]));
     }
   }
 #pragma unroll
   for (int c = 0; c < PIECES; ++c) {
     P p;
 #pragma unroll
-    for (int j = 0; j < N; ++j) p.v[j] = from_float<T>(sum[c][j] * scale);
+    for (int j = 0; j < N; ++j) p.v[j] = from_float<T>(times(sum[c][j], scale));
     if (col + c * STEP < H) *reinterpret_cast<P*>(dtable + static_cast<long long>(token) * H + col + c * STEP) = p;
   }
 }
@@ -448,7 +459,7 @@ sum_rows_kernel(const uint2* __restrict__ pairs, int n, const T* __restrict__ dy
     for (int c = 0; c < PIECES; ++c) {
       P p;
 #pragma unroll
-      for (int i = 0; i < N; ++i) { p.v[i] = from_float<T>(sum[c][i] * scale); sum[c][i] = 0.f; }
+      for (int i = 0; i < N; ++i) { p.v[i] = from_float<T>(times(sum[c][i], scale)); sum[c][i] = 0.f; }
       if (col + c * STEP < H) *reinterpret_cast<P*>(dtable + static_cast<long long>(now) * H + col + c * STEP) = p;
     }
   };
@@ -467,7 +478,7 @@ sum_rows_kernel(const uint2* __restrict__ pairs, int n, const T* __restrict__ dy
 #pragma unroll
       for (int c = 0; c < PIECES; ++c)
 #pragma unroll
-        for (int j = 0; j < N; ++j) sum[c][j] += to_float(p[k][c].v[j]);
+        for (int j = 0; j < N; ++j) sum[c][j] = plus(sum[c][j], to_float(p[k][c].v[j]));
     }
   }
   if (!open || now != last) { store(); return; }
@@ -511,7 +522,7 @@ join_rows_kernel(const uint2* __restrict__ pairs, const int* __restrict__ pieces
 #pragma unroll 8
         for (int r = w; r < begin.y; r += JOIN_THREADS / 32) {
           const float4 p = *reinterpret_cast<const float4*>(from + static_cast<long long>(r) * Hp);
-          sum.x += p.x; sum.y += p.y; sum.z += p.z; sum.w += p.w;
+          sum.x = plus(sum.x, p.x); sum.y = plus(sum.y, p.y); sum.z = plus(sum.z, p.z); sum.w = plus(sum.w, p.w);
         }
       }
       s_sum[w][lane] = sum;
@@ -520,11 +531,11 @@ join_rows_kernel(const uint2* __restrict__ pairs, const int* __restrict__ pieces
 #pragma unroll
         for (int g = 1; g < JOIN_THREADS / 32; ++g) {
           const float4 p = s_sum[g][lane];
-          sum.x += p.x; sum.y += p.y; sum.z += p.z; sum.w += p.w;
+          sum.x = plus(sum.x, p.x); sum.y = plus(sum.y, p.y); sum.z = plus(sum.z, p.z); sum.w = plus(sum.w, p.w);
         }
         const float v[4] = {sum.x, sum.y, sum.z, sum.w};
 #pragma unroll
-        for (int g = 0; g < 4; ++g) if (col + g < H) dtable[static_cast<long long>(token) * H + col + g] = from_float<T>(v[g] * scale);
+        for (int g = 0; g < 4; ++g) if (col + g < H) dtable[static_cast<long long>(token) * H + col + g] = from_float<T>(times(v[g], scale));
       }
       __syncthreads();
     }

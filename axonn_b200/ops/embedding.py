@@ -17,7 +17,7 @@ EMBEDDING_TYPES = tuple(_DT)
 
 def embedding(tokens, weight, scale=1.0, padding_idx=None):
     """``weight[tokens] * scale``: ``tokens [...]`` (int32 or int64), ``weight [V, H]`` (bf16, fp16 or fp32), returns ``[..., H]`` in the type
-    of ``weight``, each value rounded once.
+    of ``weight``, each value rounded once (magnitudes below 2^-126 are kept).
 
     The gradient of ``weight`` has the sums of the rows of equal tokens, 32-bit in the order of the tokens (the same bits on every run),
     scaled and rounded once; ``padding_idx`` gets none.  Gradients of gradients are lookups again.  A token outside the table

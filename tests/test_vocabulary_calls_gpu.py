@@ -86,3 +86,25 @@ def test_gradient_of_wide_tables():
     (grad,) = torch.autograd.grad(out, weight, dy)
     for v, count in enumerate(torch.bincount(tokens, minlength=V).tolist()):
         assert torch.equal(grad[v], (dy[0].float() * count).bfloat16())
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("n,H,kind", [(200, 40, "any"), (3000, 40, "any"), (3000, 33, "same"), (5000, 6, "any")])
+def test_numbers_below_the_smallest_normal_one(n, H, kind, dtype):
+    """They are kept, as torch.nn.functional.embedding does it: their sums in 32 bits are exact (16-bit types: multiples of 2^-133 or 2^-24), a
+    factor that is a power of two rounds nothing but the result.  The wanted ones come from 64 bits on the CPU, rounded once."""
+    V, smallest, by = 50, torch.finfo(dtype).smallest_normal, 0.125
+    g = torch.Generator().manual_seed(n + H)
+    weight = (torch.randn(V, H, generator=g).double() * smallest * 2).to(dtype)
+    tokens = torch.full((n,), 7) if kind == "same" else torch.randint(0, V, (n,), generator=g)
+    dy = (torch.randn(n, H, generator=g).double() * smallest / 64).to(dtype)
+    assert bool((weight.abs() < smallest).any()) and bool((dy.abs() < smallest).any()) and dy.count_nonzero() > n * H / 4
+    for scale in (1.0, by):
+        w = weight.to(DEV).requires_grad_()
+        out = ops.embedding(tokens.to(DEV), w, scale)
+        assert torch.equal(out.cpu(), (weight.double() * scale).to(dtype)[tokens])
+        (grad,) = torch.autograd.grad(out, w, dy.to(DEV))
+        want, size = (torch.zeros(V, H, dtype=torch.float64).index_add_(0, tokens, d) * scale for d in (dy.double(), dy.double().abs()))
+        # fp32 has 24 bits above 2^-149: sums up to 2^-125 are exact, larger ones of n terms off by n times 2^-24 of their terms' sizes
+        tol = torch.where(size / scale > 2.0 ** -125, n * 2.0 ** -24 * size, 0.0) if dtype == torch.float32 else torch.zeros_like(want)
+        assert bool(((grad.cpu().double() - want.to(dtype).double()).abs() <= tol).all())
