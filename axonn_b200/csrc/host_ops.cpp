@@ -672,6 +672,14 @@ struct EmbeddingGradNode : torch::autograd::Function<EmbeddingGradNode> {
   }
   static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx, torch::autograd::variable_list grads);
 };
+// Of a gradient that stands for many (is_grads_batched, vectorised Jacobians): a wrapper without memory of its own, which torch's operators
+// know.  Sums in 32 bits; tokens without a gradient go to a row behind the table's.
+Tensor batched_embedding_grad(const Tensor& tokens, const Tensor& dy, int64_t V, double scale, int64_t padding) {
+  const Tensor none = tokens.lt(0).logical_or(tokens.ge(V)).logical_or(tokens.eq(padding));
+  const Tensor sums = at::embedding_dense_backward(dy.to(at::kFloat), tokens.to(at::kLong).masked_fill(none, V), V + 1, -1, false);
+  return sums.narrow(0, 0, V).mul(scale).to(dy.scalar_type());
+}
+bool batched(const Tensor& t) { return t.defined() && !t.has_storage(); }
 struct EmbeddingNode : torch::autograd::Node {
   torch::autograd::SavedVariable tokens, sorted;
   bool has_sorted = false;
@@ -682,6 +690,7 @@ struct EmbeddingNode : torch::autograd::Node {
     std::lock_guard<std::mutex> lock(mutex_);
     if (!grads[0].defined()) return {Tensor()};
     const Tensor t = tokens.unpack(), s = has_sorted ? sorted.unpack() : Tensor();
+    if (batched(grads[0]) || observed()) return {batched_embedding_grad(t, grads[0], V, scale, padding)};
     if (wants_grad(grads[0]))
       return {EmbeddingGradNode::apply(t, s.defined() ? optional<Tensor>(s) : std::nullopt, grads[0], V, scale, padding)};
     return {run_embedding_grad(t, s, grads[0], V, scale, padding)};

@@ -38,6 +38,11 @@ def plain_tensors(*tensors) -> bool:
             and forward_ad._current_level < 0 and not torch.compiler.is_compiling())
 
 
+def batched(t) -> bool:
+    """``t`` stands for many tensors (``torch.autograd.grad(is_grads_batched=True)``, vectorised Jacobians) and has no memory of its own."""
+    return t is not None and not torch._C._has_storage(t)
+
+
 def host_paths():
     """The native host paths (``_lib.host``) while neither a compiler nor a forward-mode level is active - they ask everything else
     themselves -, otherwise ``None``."""

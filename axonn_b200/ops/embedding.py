@@ -6,7 +6,7 @@ import torch
 import torch.nn.functional as F
 
 from . import _lib
-from .direct import host_paths, no_graph, plain_tensors
+from .direct import batched, host_paths, no_graph, plain_tensors
 from .gemm import as_written
 from .kv_cache import _elsewhere
 
@@ -87,6 +87,14 @@ def _table_gradient(tokens, sorted_, dy, V, scale, padding):
     return out
 
 
+def _batched_gradient(tokens, dy, V, scale, padding):
+    """Of a gradient that stands for many (``is_grads_batched``, vectorised Jacobians): a wrapper without memory of its own, which torch's
+    operators know.  Sums in 32 bits; tokens without a gradient go to a row behind the table's."""
+    none = (tokens < 0) | (tokens >= V) | (tokens == padding)
+    sums = torch.ops.aten.embedding_dense_backward(dy.float(), tokens.long().masked_fill(none, V), V + 1, -1, False)
+    return (sums[:V] * scale).to(dy.dtype)
+
+
 class _EmbeddingFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, tokens, weight, scale, padding):
@@ -97,6 +105,8 @@ class _EmbeddingFn(torch.autograd.Function):
 
     @staticmethod
     def backward(ctx, dy):
+        if batched(dy) or not plain_tensors(dy):
+            return None, _batched_gradient(ctx.saved_tensors[0], dy, ctx.V, ctx.scale, ctx.padding), None, None
         return None, _EmbeddingGradFn.apply(*ctx.saved_tensors, dy, ctx.V, ctx.scale, ctx.padding), None, None
 
 

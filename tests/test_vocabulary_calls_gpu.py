@@ -7,6 +7,7 @@ import torch.distributed as dist
 from axonn_b200 import ops
 from axonn_b200.ops import _lib
 
+from _vocabulary import HALF_STEP, SMALLEST
 from _vocabulary_ends import COLD, HOT, check_ends_of_temperature, ends_of_temperature
 
 pytestmark = pytest.mark.gpu
@@ -108,3 +109,50 @@ def test_numbers_below_the_smallest_normal_one(n, H, kind, dtype):
         # fp32 has 24 bits above 2^-149: sums up to 2^-125 are exact, larger ones of n terms off by n times 2^-24 of their terms' sizes
         tol = torch.where(size / scale > 2.0 ** -125, n * 2.0 ** -24 * size, 0.0) if dtype == torch.float32 else torch.zeros_like(want)
         assert bool(((grad.cpu().double() - want.to(dtype).double()).abs() <= tol).all())
+
+
+@pytest.mark.parametrize("native", [True, False])
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("n,kind", [(1, "any"), (150, "any"), (3000, "any"), (700, "same")])
+def test_batched_gradients(n, kind, dtype, native, monkeypatch):
+    """Many gradients of the rows at once, as of torch.nn.functional.embedding; tokens outside the table and padding have none."""
+    if not native:
+        monkeypatch.setattr(_lib, "_HOST", None)
+    V, H, scale, pad = 40, 12, -1.5, 3
+    g = torch.Generator(device=DEV).manual_seed(n)
+    weight = torch.randn(V, H, generator=g, device=DEV).to(dtype).requires_grad_()
+    tokens = torch.full((n,), 7, device=DEV) if kind == "same" else torch.randint(-2, V + 2, (n,), generator=g, device=DEV)
+    dy = torch.randn(5, n, H, generator=g, device=DEV).to(dtype)
+    for ids in (tokens, tokens.int()):
+        out = ops.embedding(ids, weight, scale, pad)
+        (got,) = torch.autograd.grad(out, weight, dy, is_grads_batched=True, retain_graph=True)
+        assert got.shape == (5, V, H) and got.dtype == dtype
+        there = (tokens >= 0) & (tokens < V) & (tokens != pad)
+        for i in range(5):
+            d, zero = dy[i][there].double(), torch.zeros(V, H, dtype=torch.float64, device=DEV)
+            want, size = zero.index_add(0, tokens[there], d, alpha=scale), zero.index_add(0, tokens[there], d.abs(), alpha=abs(scale))
+            count = torch.bincount(tokens[there], minlength=V)[:, None]
+            # as of the single gradient: every addition and the product with the scale 2^-24 of the sizes, then the type's rounding
+            tol = HALF_STEP[dtype] * want.abs() + SMALLEST[dtype] + (1 + HALF_STEP[dtype]) * size * 2.0 ** -24 * (count + 1)
+            assert bool(((got[i].double() - want).abs() <= tol).all())
+
+
+def test_vectorised_jacobians(monkeypatch):
+    """The same with and without a loop over the rows, and gradients of batched gradients."""
+    tokens = torch.tensor([[1, 4, 1], [2, 0, 4]], device=DEV)
+    weight = torch.randn(6, 4, device=DEV)
+    for native in (True, False):
+        with monkeypatch.context() as m:
+            if not native:
+                m.setattr(_lib, "_HOST", None)
+            f = lambda w: ops.embedding(tokens, w, 2.0, 2).square().sum(-1)  # noqa: E731
+            a, b = (torch.autograd.functional.jacobian(f, weight, vectorize=v) for v in (True, False))
+            assert torch.equal(a, b)
+            w = weight.clone().requires_grad_()
+            out = ops.embedding(tokens, w, 2.0, 2)
+            u = torch.randn(3, 2, 3, 4, device=DEV, requires_grad=True)
+            (g,) = torch.autograd.grad(out, w, u, is_grads_batched=True, create_graph=True)
+            c = torch.randn_like(g)
+            (gu,) = torch.autograd.grad(g, u, c)
+            keep = (tokens != 2)[None, :, :, None]
+            assert torch.equal(gu, 2.0 * c[:, tokens] * keep)
