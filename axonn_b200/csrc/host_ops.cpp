@@ -110,6 +110,9 @@ void run_norm(const Tensor& x, const optional<Tensor>& delta, const Tensor& gamm
   }
 }
 
+// A gradient that stands for many (is_grads_batched, vectorised Jacobians) is a wrapper without memory of its own.
+bool batched(const Tensor& t) { return t.defined() && !t.has_storage(); }
+
 // Node::gradients() of kernels that leave no graph: differentiating them again is an error (first_derivative_only in ops/direct.py).
 template <typename Node>
 torch::autograd::variable_list first_derivative(torch::autograd::AutogradContext* ctx, const torch::autograd::variable_list& grads, const char* why) {
@@ -541,6 +544,7 @@ struct TokenLogProbsNode : torch::autograd::Node {
 
   torch::autograd::variable_list apply(torch::autograd::variable_list&& grads) override {
     std::lock_guard<std::mutex> lock(mutex_);
+    TORCH_CHECK(!std::any_of(grads.begin(), grads.end(), batched), "TokenLogProbs: batched gradients are not implemented");
     const Tensor z = logits.unpack(), t = has_tokens ? tokens.unpack() : Tensor(), s = stats.unpack(), best = top ? top_tokens.unpack() : Tensor();
     if (!at::GradMode::is_enabled()) return {gradient(z, t, s, best, grads)};
     Tensor out;
@@ -672,14 +676,12 @@ struct EmbeddingGradNode : torch::autograd::Function<EmbeddingGradNode> {
   }
   static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx, torch::autograd::variable_list grads);
 };
-// Of a gradient that stands for many (is_grads_batched, vectorised Jacobians): a wrapper without memory of its own, which torch's operators
-// know.  Sums in 32 bits; tokens without a gradient go to a row behind the table's.
+// Of a gradient that stands for many, which torch's operators know.  Sums in 32 bits; tokens without a gradient go to a row behind the table's.
 Tensor batched_embedding_grad(const Tensor& tokens, const Tensor& dy, int64_t V, double scale, int64_t padding) {
   const Tensor none = tokens.lt(0).logical_or(tokens.ge(V)).logical_or(tokens.eq(padding));
   const Tensor sums = at::embedding_dense_backward(dy.to(at::kFloat), tokens.to(at::kLong).masked_fill(none, V), V + 1, -1, false);
   return sums.narrow(0, 0, V).mul(scale).to(dy.scalar_type());
 }
-bool batched(const Tensor& t) { return t.defined() && !t.has_storage(); }
 struct EmbeddingNode : torch::autograd::Node {
   torch::autograd::SavedVariable tokens, sorted;
   bool has_sorted = false;

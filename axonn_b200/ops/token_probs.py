@@ -10,7 +10,7 @@ import torch
 import torch.distributed as dist
 
 from . import _lib
-from .direct import first_derivative_only, host_paths
+from .direct import batched, first_derivative_only, host_paths
 from .gemm import as_written
 from .kv_cache import _elsewhere
 
@@ -42,10 +42,11 @@ def token_log_probs(logits, tokens=None, entropy=False, top=0, temperature=1.0, 
     ``+inf`` among its logits, is NaN throughout (a NaN counts as the largest logit among the alternatives).  On a GPU logits below
     2^-126 count as zero.  Temperatures go from 2^-100 to 2^100.
 
-    Everything but ``top_tokens`` can be differentiated once by the logits, which may have any strides (such as ``logits[:, :-1]``) and are
-    left as they are.  With ``group`` the last dimension is this rank's contiguous slice of the vocabulary, of equal size on all ranks (rank
-    order = slice order); ``tokens`` and every result count the whole vocabulary, and the gradients of the results are those of all
-    ranks, as for ``cross_entropy``.  Neither synchronises: calls without ``group`` can be captured into a CUDA graph."""
+    Everything but ``top_tokens`` can be differentiated once, with one gradient at a time, by the logits, which may have any strides (such
+    as ``logits[:, :-1]``) and are left as they are.  With ``group`` the last dimension is this rank's contiguous slice of the vocabulary, of
+    equal size on all ranks (rank order = slice order); ``tokens`` and every result count the whole vocabulary, and the gradients of the
+    results are those of all ranks, as for ``cross_entropy``.  Neither synchronises: calls without ``group`` can be captured into a CUDA
+    graph."""
     if group is None and logits.is_cuda and temperature and (host := host_paths()) is not None:
         out = host.token_log_probs(logits, tokens, entropy, top, 1 / temperature, ignore_index)
         if out is not None:
@@ -175,6 +176,8 @@ class _TokenLogProbsFn(torch.autograd.Function):
     @staticmethod
     @first_derivative_only
     def backward(ctx, d_log_probs, d_entropy, d_top, _):
+        if any(map(batched, (d_log_probs, d_entropy, d_top))):
+            raise RuntimeError("TokenLogProbs: batched gradients are not implemented")
         logits, tokens, stats, at = ctx.saved_tensors
         # what hooks (offloading, compression) give back may lie in another layout
         stats, at = as_written(stats), None if at is None else at.contiguous()

@@ -128,3 +128,17 @@ def test_factors_that_the_launchers_refuse():
         for call in (lambda: L.axb_token_log_probs(p, 8, 8, p, 1, 1, p, p, p, p, p, 1, 1, 8, 0, 8, 0, scale, -100, 1, 0, None),
                      lambda: L.axb_token_log_probs_bwd(p, 8, 8, p, 1, 1, p, p, p, p, p, p, 1, 1, 8, 0, 8, 0, scale, -100, 0, None)):
             assert call() == -1 and b"scale" in L.axb_last_error()
+
+
+def test_batched_gradients():
+    """Of a lookup as of torch.nn.functional.embedding; of log-probabilities they are refused."""
+    tokens, w = torch.tensor([1, 4, 1, 0]), torch.randn(6, 3, requires_grad=True)
+    dy = torch.randn(5, 4, 3)
+    (got,) = torch.autograd.grad(ops.embedding(tokens, w, 2.0, 4), w, dy, is_grads_batched=True)
+    want = torch.zeros(5, 6, 3).index_add(1, tokens[[0, 2, 3]], 2 * dy[:, [0, 2, 3]])
+    assert torch.equal(got, want)
+    z = torch.randn(4, 9, requires_grad=True)
+    for entropy in (False, True):
+        r = ops.token_log_probs(z, tokens, entropy=entropy)
+        with pytest.raises(RuntimeError, match="batched gradients"):
+            torch.autograd.grad(r.entropy if entropy else r.log_probs, z, torch.randn(3, 4), is_grads_batched=True)

@@ -156,3 +156,14 @@ def test_vectorised_jacobians(monkeypatch):
             (gu,) = torch.autograd.grad(g, u, c)
             keep = (tokens != 2)[None, :, :, None]
             assert torch.equal(gu, 2.0 * c[:, tokens] * keep)
+
+
+def test_batched_gradients_of_log_probabilities_are_refused(monkeypatch):
+    z, t = torch.randn(6, 50, device=DEV, requires_grad=True), torch.randint(0, 50, (6,), device=DEV)
+    for native in (True, False):
+        with monkeypatch.context() as m:
+            if not native:
+                m.setattr(_lib, "_HOST", None)
+            r = ops.token_log_probs(z, t, entropy=True)
+            with pytest.raises(RuntimeError, match="batched gradients"):
+                torch.autograd.grad(r.log_probs, z, torch.randn(3, 6, device=DEV), is_grads_batched=True)
