@@ -142,3 +142,43 @@ def test_batched_gradients():
         r = ops.token_log_probs(z, tokens, entropy=entropy)
         with pytest.raises(RuntimeError, match="batched gradients"):
             torch.autograd.grad(r.entropy if entropy else r.log_probs, z, torch.randn(3, 4), is_grads_batched=True)
+
+
+def _scaled_layers(rank, world, depth):
+    """The scale on every way that rows are looked up: the table gathered over depth ranks or not, torch's own lookup where a layer asks for
+    what the package's does not do, rows fetched from the owning ranks (a stub here)."""
+    from axonn_b200.intra_layer import Embedding, embedding
+    from axonn_b200.intra_layer.communication import _gather
+
+    _grid(world, depth)
+    g = torch.Generator().manual_seed(5)
+    table, tokens = torch.randn(12, 8, generator=g), torch.randint(0, 12, (3, 7), generator=g)
+    dy = torch.randn(3, 7, 8, generator=g)
+    for kw in (dict(), dict(padding_idx=3), dict(scale_grad_by_freq=True), dict(dtype=torch.float64)):
+        layer = Embedding(12, 8, expert_mode=True, scale=2.5, **kw)
+        layer.load_state_dict({"weight": table.to(layer.weight.dtype)})
+        want = torch.nn.Embedding(12, 8, _weight=table.to(layer.weight.dtype).clone(), **{k: v for k, v in kw.items() if k != "dtype"})
+        out, ref = layer(tokens), want(tokens) * 2.5
+        assert torch.equal(out, ref)
+        out.backward(dy.to(out.dtype))
+        ref.backward(dy.to(ref.dtype))
+        grad = layer.weight.grad if depth == 1 else _gather(layer.weight.grad, 0, layer.depth_group)
+        # every depth rank has the same tokens here, and their gradients are summed
+        assert torch.allclose(grad.view(12, 8), depth * want.weight.grad, rtol=1e-6, atol=1e-6)
+        assert torch.equal(layer.rows(2, 5, "cpu"), want.weight.detach()[2:7] * 2.5)
+    with torch.no_grad():
+        long = Embedding(12, 8, expert_mode=True, scale=2.5, max_norm=1.0)
+        long.load_state_dict({"weight": table})
+        assert torch.equal(long(tokens), torch.nn.functional.embedding(tokens, table.clone(), max_norm=1.0) * 2.5)
+    layer = Embedding(12, 8, expert_mode=True, scale=2.5)
+    layer._p2p_rows, kept = (lambda x: True), embedding._EmbeddingRowsP2P
+    embedding._EmbeddingRowsP2P = type("Fetched", (), {"apply": staticmethod(lambda x, *_: table[x])})
+    try:
+        assert torch.equal(layer(tokens), table[tokens] * 2.5)
+    finally:
+        embedding._EmbeddingRowsP2P = kept
+
+
+@pytest.mark.parametrize("depth", [1, 2])
+def test_scaled_layers(depth):
+    run_distributed(_scaled_layers, depth, depth)

@@ -7,7 +7,7 @@ import torch.distributed as dist
 from axonn_b200 import ops
 from axonn_b200.ops import _lib
 
-from _vocabulary import HALF_STEP, SMALLEST
+from _vocabulary import HALF_STEP, SMALLEST, check_told, told
 from _vocabulary_ends import COLD, HOT, check_ends_of_temperature, ends_of_temperature
 
 pytestmark = pytest.mark.gpu
@@ -167,3 +167,31 @@ def test_batched_gradients_of_log_probabilities_are_refused(monkeypatch):
             r = ops.token_log_probs(z, t, entropy=True)
             with pytest.raises(RuntimeError, match="batched gradients"):
                 torch.autograd.grad(r.log_probs, z, torch.randn(3, 6, device=DEV), is_grads_batched=True)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("n,V,H", [(1, 1, 1), (1, 5, 7), (33, 2, 64), (200, 1000, 1001), (257, 40, 24), (3000, 700, 50), (20011, 1400, 16), (300, 20, 9000), (16384, 3000, 264)])
+def test_lookups_are_copies(n, V, H, dtype):
+    """Without a scale every bit is the table's, whatever the sizes and wherever the rows begin; with gradients and without."""
+    g = torch.Generator(device=DEV).manual_seed(n + H)
+    tokens = torch.randint(0, V, (n,), generator=g, device=DEV)
+    flat = torch.randn(V * (H + 3) + 1, generator=g, device=DEV).to(dtype)
+    dense, off, gaps = flat[:V * H].view(V, H), flat[1:1 + V * H].view(V, H), flat[1:].view(V, H + 3)[:, 2:2 + H]
+    for table in (dense, off, gaps, dense.t().contiguous().t()):
+        want = table[tokens]
+        for ids in (tokens, tokens.int()):
+            assert torch.equal(ops.embedding(ids, table), want)
+            assert torch.equal(ops.embedding(ids, table.detach().requires_grad_()), want)
+
+
+@pytest.mark.parametrize("rows", [1, 64, 300])
+@pytest.mark.parametrize("V,dtype", [(1500, torch.bfloat16), (2048, torch.bfloat16), (2049, torch.float16), (4096, torch.float16), (4097, torch.bfloat16),
+                                     (1024, torch.float32), (1025, torch.float32), (2048, torch.float32), (2049, torch.float32)])
+def test_alternatives_of_few_narrow_rows(rows, V, dtype):
+    """Rows that a warp takes and rows that a block takes, by their bytes and by how many alternatives are asked for."""
+    g = torch.Generator(device=DEV).manual_seed(V + rows)
+    logits = (3 * torch.randn(rows, V, generator=g, device=DEV)).to(dtype)
+    logits[::3, V // 2:] = -float("inf")
+    tokens = torch.randint(0, V // 2, (rows,), generator=g, device=DEV)
+    for top in (1, 8, 9, 20, 21, 32):
+        check_told(ops.token_log_probs(logits, tokens, entropy=True, top=top), told(logits, tokens, top), V, top)
