@@ -12,12 +12,12 @@
 //      there are not.  A chunk is summed with what the last token of it has in the next one, unless that token fills the whole next
 //      chunk: then its sum so far goes to the workspace.  A segment of any length so takes many blocks, and one of up to 32 pairs
 //      no extra traffic.
-//   3. The partial sums of long segments, which the blocks of the sums have noted, are joined in their order.
+//   3. The partial sums of long segments, which the blocks of the sums have noted, are joined: every eighth by one warp, then the warps'.
 // Up to 256 tokens are looked through by every block instead: one launch, for steps that are bound by the host's launches.
 //
-// One B200, device time: 16,384 tokens, 50,304 x 2,048 bf16, lookup and gradient 85 us, of which the lookup 22 to 25 (a copy of its 67 MB
-// 22), the sums 40 (273 MB: 6.8 TB/s), the join 5 to 8; 128,256 x 4,096 229 us (1.38 GB: 210 at the copy's rate).  The sort takes 9 to 13
-// us beside the lookup.  Rows of 1001 fp32 values (4-byte pieces), 6,001 tokens of which 40 % are padding, 32,000 rows: 55 us (28).
+// One B200, device time: 16,384 tokens, 50,304 x 2,048 bf16, lookup and gradient 83 us, of which the lookup 20 to 22 (a copy of its 67 MB
+// 22), the sums 40 (273 MB: 6.8 TB/s), the join 5 to 8; 128,256 x 4,096 225 us (1.38 GB: 210 at the copy's rate).  The sort takes 9 to 13
+// us beside the lookup.  Rows of 1001 fp32 values (4-byte pieces), 6,001 tokens of which 40 % are padding, 32,000 rows: 52 us (28).
 #include <atomic>
 #include <initializer_list>
 

@@ -18,7 +18,7 @@
 //
 // One B200, device time: 4096 rows of 128,256 bf16 values with entropy 161.8 us (their bytes at the copy's rate: 160.7), the gradient 336
 // (321); 8 x 2047 rows of 50,304, 15 % of them ignored, 219 (214).  6.4 instructions a value, 8.0 with entropy.  64 rows of 128,256
-// with 20 alternatives 14.4 us, without 8.3: a chain of loads, bounds, lists and the exchange, 25,000 cycles, in which no other block fills in.
+// with 20 alternatives 16.1 to 16.9 us, without 7: a chain of loads, bounds, lists and the exchange, in which no other block fills in.
 // Tried: words with values above the bound one after another by the whole warp (4096 rows of 32,000, 20 alternatives: 106 us for 96), every
 // value of a tile by the thread that has it (more instructions still), bounds by 16 counts over the block (64 rows, one alternative: 20.6
 // us for 12.4), one list with atomics for the block (no faster), registers for four blocks an SM instead of three (no faster).
@@ -30,19 +30,22 @@ namespace axb {
 
 constexpr int TP_MOST = 32;                // alternatives
 // 16-byte words of a thread, of a tile: 4, the next ones loaded before these are used, or 8 without, where a block has that many: 4096 rows of
-// 32,000 bf16 values 45.9 us for 48.6, 64 of 128,256 with 20 alternatives 14.4 for 16.5; a row of 32,000 over 8 blocks 7.0 for 6.5.
+// 32,000 bf16 values 45.9 us for 48.6, 64 of 128,256 with 20 alternatives (a part of the vocabulary masked) 14.4 for 16.5; a row of 32,000 over 8
+// blocks 7.0 for 6.5.
 constexpr int TP_FEW_WORDS = 4, TP_MANY_WORDS = 8;
 constexpr int TP_KEEP = 64;                // entries that a list is cut down to, at most
 constexpr float TP_LOG2E = 1.4426950408889634f;
 constexpr double TP_LN2 = 0.6931471805599453;
-// Bytes of a row that a warp takes, up to 8 alternatives (4000 rows of 4000 bf16 values: 20.3 us with 8 for 25.9 with blocks of 128 threads,
-// 57 with 24 for 28) and 20 of half as many (16384 rows of 2000: 57 us with 20 for 103; 300 of 1500 with 24: 22 for 7, as 32 maxima bound
-// the 24th of so few values badly); and that a block of 128 threads takes where there are few rows (one of 32,000 bf16 values, 5
-// alternatives: 6.9 us with clusters of 256, 7.3 with those of 128).  Many rows always take 128: their last tile is emptier with 256 (8 x
-// 2047 rows of 50,304 values 221 us for 251).
+// Bytes of a row that a warp takes, up to 8 alternatives (4000 rows of 4000 bf16 values: 18.2 us with 8 for 26.7 with blocks of 128 threads,
+// 57 with 24 for 28) and 20 of half as many (16384 rows of 2000: 54 us with 20 for 101; 300 of 1500 with 24: 22 for 7, as 32 maxima bound
+// the 24th of so few values badly).  Of 4000 rows and more it saves throughout, of 1200 up to 2000 values with 8 (9.7 us for 11.3; 4000 values
+// 14.7 for 11.6), of fewer up to 1000 values (300 with 8: 4.9 for 6.5); otherwise few rows wait for one warp's longer chain, by up to 3 us: 64 of
+// 4000 with 8 9.0 for 6.5, 300 of 1500 with 20 8.0 for 7.1, one of 2000 with 20 6.9 for 4.6.  TP_MIDDLE: bytes that a block of 128 threads
+// takes where there are few rows (one of 32,000 bf16 values, 5 alternatives: 6.9 us with clusters of 256, 7.3 with those of 128).  Many
+// rows always take 128: their last tile is emptier with 256 (8 x 2047 rows of 50,304 values 221 us for 251).
 constexpr long long TP_NARROW = 8192, TP_MIDDLE = 32768;
-// Blocks per SM up to which rows are split over clusters, where alternatives are asked for: 64 rows of 128,256 values with 20 of them and a
-// part of the vocabulary masked 16.5 us, with 4 blocks 18.5.
+// Blocks per SM up to which rows are split over clusters, where alternatives are asked for: 64 rows of 128,256 values with 20 of them 16.1 us,
+// with 4 blocks 17.1; 148 of them 24.4 for 27.7, 64 of 32,000 10.7 for 13.8 (100 of 50,304 with 5 13.8 for 13.1).
 constexpr long long TP_ROOM = 2;
 // Factors 1 / temperature: a flushed one times -inf would be NaN, and so would the maximum's zero times one that overflows.
 constexpr float TP_COLDEST = 0x1p-100f;
@@ -845,7 +848,7 @@ static int fill(TokenProbsArgs& a, const char* what, const void* logits, long lo
 template <typename T, bool ENTROPY, bool TOP, int THREADS>
 static int tell(const TokenProbsArgs& a, long long rows, float* log_probs, float* entropy, float* top_log_probs, long long* top_tokens, float4* stats,
                 cudaStream_t s) {
-  // blocks of a row: as many as there is room for with four on every SM, each with a word at least for all of its threads
+  // blocks of a row: as many as there is room for with four on every SM (TP_ROOM, where alternatives are asked for), each with a word at least for all of its threads
   const long long words = (a.V + Word<T>::COUNT - 1) / Word<T>::COUNT, room = (TOP ? TP_ROOM : 4ll) * sm_count_current();
   unsigned ctas = 1;
   while (THREADS > 32 && ctas < 8 && rows * ctas * 2 * THREADS <= room * 256 && words / (2 * ctas) >= THREADS) ctas *= 2;

@@ -19,8 +19,8 @@ def embedding(tokens, weight, scale=1.0, padding_idx=None):
     """``weight[tokens] * scale``: ``tokens [...]`` (int32 or int64), ``weight [V, H]`` (bf16, fp16 or fp32), returns ``[..., H]`` in the type
     of ``weight``, each value rounded once (magnitudes below 2^-126 are kept).
 
-    The gradient of ``weight`` has the sums of the rows of equal tokens, 32-bit in the order of the tokens (the same bits on every run),
-    scaled and rounded once; ``padding_idx`` gets none.  Gradients of gradients are lookups again.  A token outside the table
+    The gradient of ``weight`` has the sums of the rows of equal tokens, 32-bit in an order that the tokens alone decide (the same bits on
+    every run), scaled and rounded once; ``padding_idx`` gets none.  Gradients of gradients are lookups again.  A token outside the table
     gives a row of NaN and no gradient on a GPU, and is an error on the CPU.  The call never synchronises and can be captured into a CUDA graph."""
     if weight.is_cuda and (host := host_paths()) is not None:
         out = host.embedding(tokens, weight, scale, -1 if padding_idx is None else padding_idx if padding_idx >= 0 else -2)

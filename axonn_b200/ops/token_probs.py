@@ -1,7 +1,7 @@
 """Log-probabilities of given tokens, with the entropy and the best alternatives (``csrc/token_probs.cu``).
 
 The logits are read once forward and once backward, in the type they have: neither their softmax nor a 32-bit copy of the
-``[tokens, vocabulary]`` matrix is stored.  Statistics are 32-bit, in the order of the vocabulary, the same bits on every run."""
+``[tokens, vocabulary]`` matrix is stored.  Statistics are 32-bit, added in an order that no timing changes: the same bits on every run."""
 
 import math
 from typing import NamedTuple, Optional
