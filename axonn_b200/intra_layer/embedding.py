@@ -155,7 +155,7 @@ class Embedding(torch.nn.Module):
         Rows that the table has not got are an ``IndexError``."""
         if count > 0 and not 0 <= first <= self.num_embeddings - count:
             # torch's own refusal, of indices on the host: a GPU's lookup of them ends the program, or gives NaN
-            return F.embedding(torch.arange(first, first + count), torch.empty(1, 1).expand(self.num_embeddings, 1))
+            return F.embedding(torch.arange(first, first + count, device="cpu"), torch.empty(1, 1, device="cpu").expand(self.num_embeddings, 1))
         w = self.weight
         if (plain_layer(self) and self.scale == 1.0 and self.depth_group_size == 1 and self.expert_mode and self.max_norm is None
                 and count >= 0 and no_graph(w) and w.device == torch.device(device)
